@@ -36,6 +36,40 @@ extern "C" {
 #define LSA_ERR_SHORT (-4)
 #define LSA_ERR_SIZE (-5)
 
+/* ---------------------------------------------------------------- shared prefix, eviction */
+
+/* Attention of a batch whose sequences share a prefix (no reference counterpart). q [B, Tq, Hq,
+ * D]; k_prefix / v_prefix [P, Hkv, D], stored once for all sequences; k / v [B, T, Hkv, D] the
+ * sequences' own caches, lengths [B] the own keys that each holds, the call's Tq new tokens
+ * among them (clamped to [0, T]). Row (b, i) sees every prefix key and the own keys
+ * j < lengths[b] - Tq + i + 1; a row that sees none reads as zeros, lse -inf. What the own
+ * caches hold at or past lengths[b] is never used. strides[13], in elements: q (b, t, h),
+ * k_prefix (t, h), v_prefix (t, h), k (b, t, h), v (b, t, h); the head dimension is contiguous,
+ * every base and stride a multiple of 16 bytes. D 64 or 128, Hq / Hkv at most 64; scale > 0.
+ * out [B, Tq, Hq, D] contiguous, lse [B, Tq, Hq] (natural logarithm) or NULL.
+ * scores / scores_out [B, Hkv, T] fp32, or both NULL: scores_out = scores + the attention
+ * weight that own key j received from every (row, query head of the group) of the call; the
+ * entries at or past lengths[b] are copied. scores_out may be scores.
+ * lsa_shared_prefix_scratch: the scratch bytes of a call (LSA_ERR_ARG for refused sizes). */
+int64_t lsa_shared_prefix_scratch(int dtype, int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_t P,
+                                  int64_t T);
+int lsa_shared_prefix_attention(const void* q, const void* k_prefix, const void* v_prefix, const void* k,
+                                const void* v, int dtype, const int64_t* strides, const int32_t* lengths, int64_t B,
+                                int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_t P, int64_t T, float scale,
+                                void* out, float* lse, const float* scores, float* scores_out, void* scratch,
+                                int64_t scratch_bytes, cudaStream_t stream);
+
+/* Eviction from a cache by score (no reference counterpart). k / v rows of row_bytes bytes (a
+ * multiple of 16) at strides[6], in bytes: k (b, t, h), v (b, t, h); scores [B, Hkv, T] fp32,
+ * lengths [B]. A (sequence, KV head) with more than budget keys keeps its first sink, its last
+ * window and the highest-scored of the others (ordered_bits order, ties to the lower index) up
+ * to budget, in their order. k_out / v_out [B, capacity, Hkv, row], scores_out / ids
+ * [B, Hkv, capacity], lengths_out [B]; past the kept keys rows and scores are 0, ids -1. */
+int lsa_evict(const void* k, const void* v, int64_t row_bytes, const int64_t* strides, const float* scores,
+              const int32_t* lengths, int64_t B, int64_t T, int64_t Hkv, int64_t budget, int64_t window, int64_t sink,
+              int64_t capacity, void* k_out, void* v_out, float* scores_out, int32_t* lengths_out, int32_t* ids,
+              cudaStream_t stream);
+
 /* ---------------------------------------------------------------- peer-memory exchange */
 
 /* The sharded decode steps' all-gathers over peer memory (no reference counterpart: the

@@ -1,0 +1,307 @@
+// prefix.cu - attention over a shared prefix and each sequence's own cache: the entry points,
+// the general kernel and the join of the parts (sm_100a). prefix.cuh has the formulas.
+#include <math.h>
+
+#include "prefix.cuh"
+
+namespace lsa {
+namespace {
+
+constexpr int kSimtRows = 16;  // rows of a work item
+constexpr int kSimtKeys = 32;  // keys of a tile: one per lane
+constexpr int kSimtWarps = 8;
+
+template <typename T, int D>
+__device__ __forceinline__ void stage_rows(float* dst, int ld, const T* src, int64_t stride, int rows, int live) {
+    for (int i = threadIdx.x; i < rows * (D / 8); i += blockDim.x) {
+        const int r = i / (D / 8), c = i % (D / 8);
+        float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (r < live) load8<T>(src + r * stride + c * 8, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dst[r * ld + c * 8 + e] = x[e];
+    }
+}
+
+// One work item: up to 16 rows of a KV head x a range of keys, on the FMA pipes in fp32. A
+// warp holds two rows; a lane scores one key of a 32-key tile for both, the warp's running
+// maximum and sum follow the tile, and a lane then owns D / 32 output columns. Rows past a
+// sequence's length are staged as zeros, so what an unwritten slot holds is never used.
+template <typename T, int D>
+__global__ void __launch_bounds__(kSimtWarps * 32) prefix_simt_kernel(const PrefixArgs a, int prefix_items, int ptiles,
+                                                                      int otiles) {
+    constexpr int LDK = D + 4, E = D / 32;
+    __shared__ float sq[kSimtRows * D], sk[kSimtKeys * LDK], sv[kSimtKeys * D];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int item = blockIdx.x;
+    const bool own = item >= prefix_items;
+    int b = 0, h, tile, split, part, nrows, k0, k1, len = 0;
+    if (!own) {
+        split = item % a.Sp, item /= a.Sp;
+        tile = item % ptiles, h = item / ptiles;
+        part = split;
+        nrows = a.B * a.Tq * a.G;
+        split_range(a.P, split, a.Sp, kSimtKeys, &k0, &k1);
+    } else {
+        item -= prefix_items;
+        split = item % a.So, item /= a.So;
+        tile = item % otiles, item /= otiles;
+        h = item % a.Hkv, b = item / a.Hkv;
+        part = a.Sp + split;
+        nrows = a.Tq * a.G;
+        len = own_length(a, b);
+        split_range(len, split, a.So, kSimtKeys, &k0, &k1);
+    }
+    const int r0 = tile * kSimtRows;
+    // q rows (segment order: token, head of the group)
+    for (int i = threadIdx.x; i < kSimtRows * (D / 8); i += blockDim.x) {
+        const int r = r0 + i / (D / 8), c = i % (D / 8);
+        float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (r < nrows) {
+            const int64_t tok = (int64_t)b * a.Tq + r / a.G;
+            load8<T>(static_cast<const T*>(a.q) + tok / a.Tq * a.q_b + tok % a.Tq * a.q_t +
+                         (h * (int64_t)a.G + r % a.G) * a.q_h + c * 8,
+                     x);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sq[(i / (D / 8)) * D + c * 8 + e] = x[e];
+    }
+    const T* kb = static_cast<const T*>(own ? a.k : a.kp) + (own ? b * a.k_b + h * a.k_h : h * a.kp_h);
+    const T* vb = static_cast<const T*>(own ? a.v : a.vp) + (own ? b * a.v_b + h * a.v_h : h * a.vp_h);
+    const int64_t kt = own ? a.k_t : a.kp_t, vt = own ? a.v_t : a.vp_t;
+    // the two rows of this warp: the first key that each does not see
+    int limit[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int r = r0 + warp + kSimtWarps * u;
+        limit[u] = r >= nrows ? 0 : (own ? len - a.Tq + r / a.G + 1 : k1);
+    }
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0, 0}, acc[2][E] = {};
+    for (int t0 = k0; t0 < k1; t0 += kSimtKeys) {
+        __syncthreads();
+        const int live = k1 - t0 < kSimtKeys ? k1 - t0 : kSimtKeys;
+        stage_rows<T, D>(sk, LDK, kb + (int64_t)t0 * kt, kt, kSimtKeys, live);
+        stage_rows<T, D>(sv, D, vb + (int64_t)t0 * vt, vt, kSimtKeys, live);
+        __syncthreads();
+        float s[2] = {0, 0};
+        const float4* k4 = reinterpret_cast<const float4*>(sk + lane * LDK);
+#pragma unroll 8
+        for (int c = 0; c < D / 4; ++c) {
+            const float4 kk = k4[c];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const float4 qq = reinterpret_cast<const float4*>(sq + (warp + kSimtWarps * u) * D)[c];
+                s[u] = fmaf(qq.x, kk.x, fmaf(qq.y, kk.y, fmaf(qq.z, kk.z, fmaf(qq.w, kk.w, s[u]))));
+            }
+        }
+        float p[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const bool see = lane < live && t0 + lane < limit[u];
+            const float x = see ? s[u] * a.scale_log2 : -INFINITY;
+            float mx = x;
+#pragma unroll
+            for (int off = 16; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, off));
+            const float mn = fmaxf(m[u], mx);
+            const float base = mn == -INFINITY ? 0.0f : mn;
+            const float alpha = exp2f(m[u] - base);
+            p[u] = exp2f(x - base);
+            float sum = p[u];
+#pragma unroll
+            for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, off);
+            l[u] = l[u] * alpha + sum;
+            m[u] = mn;
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[u][e] *= alpha;
+        }
+        for (int j = 0; j < live; ++j) {
+            const float p0 = __shfl_sync(0xFFFFFFFFu, p[0], j), p1 = __shfl_sync(0xFFFFFFFFu, p[1], j);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float vv = sv[j * D + lane * E + e];
+                acc[0][e] = fmaf(p0, vv, acc[0][e]);
+                acc[1][e] = fmaf(p1, vv, acc[1][e]);
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int r = r0 + warp + kSimtWarps * u;
+        if (r >= nrows) continue;
+        const int64_t rid = row_index(a, (int64_t)b * a.Tq + r / a.G, h, r % a.G);
+        const int64_t at = (int64_t)part * a.rows + rid;
+        if (lane == 0) a.part_lse[at] = l[u] > 0.0f ? m[u] + log2f(l[u]) : -INFINITY;
+        const float inv = l[u] > 0.0f ? 1.0f / l[u] : 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) a.part_o[at * D + lane * E + e] = acc[u][e] * inv;
+    }
+}
+
+// The parts of a row joined, one warp per row: every lane holds D / 32 columns. Parts without
+// a key (lse -inf) have weight zero and their sums are not read.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixArgs a, int parts) {
+    constexpr int E = D / 32;
+    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (row >= a.rows) return;
+    float top = -INFINITY;
+    for (int c = lane; c < parts; c += 32) top = fmaxf(top, a.part_lse[(int64_t)c * a.rows + row]);
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
+    float acc[E] = {}, total = 0.0f;
+    if (top != -INFINITY) {
+        for (int c = 0; c < parts; ++c) {
+            const float x = a.part_lse[(int64_t)c * a.rows + row];
+            if (x == -INFINITY) continue;
+            const float w = exp2f(x - top);
+            total += w;
+            const float* src = a.part_o + ((int64_t)c * a.rows + row) * D + lane * E;
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] = fmaf(w, src[e], acc[e]);
+        }
+    }
+    const float inv = total > 0.0f ? 1.0f / total : 0.0f;
+    T* dst = static_cast<T*>(a.out) + row * D + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) dst[e] = from_f32<T>(acc[e] * inv);
+    if (lane == 0) {
+        const float x = total > 0.0f ? top + log2f(total) : -INFINITY;
+        a.lse2[row] = x;
+        if (a.lse) a.lse[row] = x * 0.69314718055994531f;
+    }
+}
+
+template <typename T>
+int simt_d(const PrefixArgs& a, int D, cudaStream_t stream) {
+    const int64_t ptiles = ((int64_t)a.B * a.Tq * a.G + kSimtRows - 1) / kSimtRows;
+    const int64_t otiles = ((int64_t)a.Tq * a.G + kSimtRows - 1) / kSimtRows;
+    const int64_t pi = a.Sp * ptiles * a.Hkv, oi = (int64_t)a.So * otiles * a.Hkv * a.B;
+    if (pi + oi == 0) return LSA_OK;
+    if (pi + oi > INT32_MAX) return LSA_ERR_SIZE;
+    if (D == 128)
+        prefix_simt_kernel<T, 128><<<(unsigned)(pi + oi), kSimtWarps * 32, 0, stream>>>(a, (int)pi, (int)ptiles,
+                                                                                        (int)otiles);
+    else
+        prefix_simt_kernel<T, 64><<<(unsigned)(pi + oi), kSimtWarps * 32, 0, stream>>>(a, (int)pi, (int)ptiles,
+                                                                                       (int)otiles);
+    LSA_LAUNCH_CHECK();
+    return LSA_OK;
+}
+
+template <typename T>
+int merge_d(const PrefixArgs& a, int D, cudaStream_t stream) {
+    const unsigned grid = (unsigned)((a.rows + 7) / 8);
+    if (D == 128)
+        prefix_merge_kernel<T, 128><<<grid, 256, 0, stream>>>(a, a.Sp + a.So);
+    else
+        prefix_merge_kernel<T, 64><<<grid, 256, 0, stream>>>(a, a.Sp + a.So);
+    LSA_LAUNCH_CHECK();
+    return LSA_OK;
+}
+
+struct Plan {
+    int Sp, So;
+};
+
+// Splits enough that the work items of each segment fill the GPU about four times.
+Plan make_plan(int64_t B, int64_t Tq, int64_t Hkv, int64_t G, int64_t P, int64_t T) {
+    auto splits = [](int64_t items, int64_t keys) -> int {
+        if (keys == 0) return 0;
+        int64_t s = (592 + items - 1) / items;
+        const int64_t most = (keys + 255) / 256;
+        s = s < most ? s : most;
+        return (int)(s < kMaxParts / 2 ? s : kMaxParts / 2);
+    };
+    Plan p;
+    p.Sp = splits(Hkv * ((B * Tq * G + kSimtRows - 1) / kSimtRows), P);
+    p.So = splits(B * Hkv * ((Tq * G + kSimtRows - 1) / kSimtRows), T);
+    return p;
+}
+
+bool sizes_ok(int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_t P, int64_t T) {
+    if (B < 0 || Tq < 0 || P < 0 || T < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || Hq / Hkv > 64) return false;
+    if (D != 64 && D != 128) return false;
+    // rows and keys are counted in 32 bits (offsets in 64)
+    return P <= INT32_MAX - 256 && T <= INT32_MAX - 256 && B <= INT32_MAX && Tq <= INT32_MAX && Hq <= INT32_MAX &&
+           (B == 0 || Tq == 0 || B * Tq <= INT32_MAX / Hq);
+}
+
+int64_t round256(int64_t x) { return (x + 255) / 256 * 256; }
+
+}  // namespace
+
+int launch_prefix_simt(const PrefixArgs& a, int dtype, int D, cudaStream_t stream) {
+    if (dtype == kF32) return simt_d<float>(a, D, stream);
+    if (dtype == kF16) return simt_d<__half>(a, D, stream);
+    return simt_d<__nv_bfloat16>(a, D, stream);
+}
+
+int launch_prefix_merge(const PrefixArgs& a, int dtype, int D, cudaStream_t stream) {
+    if (dtype == kF32) return merge_d<float>(a, D, stream);
+    if (dtype == kF16) return merge_d<__half>(a, D, stream);
+    return merge_d<__nv_bfloat16>(a, D, stream);
+}
+
+}  // namespace lsa
+
+using namespace lsa;
+
+extern "C" {
+
+int64_t lsa_shared_prefix_scratch(int dtype, int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_t P,
+                                  int64_t T) {
+    if (!sizes_ok(B, Tq, Hq, Hkv, D, P, T) || dtype < kF32 || dtype > kBF16) return LSA_ERR_ARG;
+    if (B == 0 || Tq == 0) return 0;
+    const Plan p = make_plan(B, Tq, Hkv, Hq / Hkv, P, T);
+    const int64_t rows = B * Tq * Hq;
+    return round256((p.Sp + p.So) * rows * D * 4) + round256((p.Sp + p.So) * rows * 4) + round256(rows * 4);
+}
+
+int lsa_shared_prefix_attention(const void* q, const void* k_prefix, const void* v_prefix, const void* k,
+                                const void* v, int dtype, const int64_t* strides, const int32_t* lengths, int64_t B,
+                                int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_t P, int64_t T, float scale,
+                                void* out, float* lse, const float* scores, float* scores_out, void* scratch,
+                                int64_t scratch_bytes, cudaStream_t stream) {
+    if (!sizes_ok(B, Tq, Hq, Hkv, D, P, T) || dtype < kF32 || dtype > kBF16) return LSA_ERR_ARG;
+    if ((scores == nullptr) != (scores_out == nullptr) || strides == nullptr) return LSA_ERR_ARG;
+    if (!(scale > 0.0f) || !(scale < INFINITY)) return LSA_ERR_ARG;  // the kernels take the maximum before the scale
+    if (B == 0 || Tq == 0) return LSA_OK;
+    if (q == nullptr || out == nullptr || lengths == nullptr || scratch == nullptr) return LSA_ERR_ARG;
+    if ((P > 0 && (k_prefix == nullptr || v_prefix == nullptr)) || (T > 0 && (k == nullptr || v == nullptr)))
+        return LSA_ERR_ARG;
+    // 16-byte loads: every base and every stride
+    const int64_t unit = dtype == kF32 ? 4 : 8;
+    for (const void* p : {q, P ? k_prefix : nullptr, P ? v_prefix : nullptr, T ? k : nullptr, T ? v : nullptr,
+                          (const void*)out, (const void*)scratch})
+        if ((uintptr_t)p & 15) return LSA_ERR_ARG;
+    for (int i = 0; i < 13; ++i)
+        if (strides[i] < 0 || strides[i] % unit) return LSA_ERR_ARG;
+    if (scratch_bytes < lsa_shared_prefix_scratch(dtype, B, Tq, Hq, Hkv, D, P, T)) return LSA_ERR_ARG;
+    const Plan p = make_plan(B, Tq, Hkv, Hq / Hkv, P, T);
+    PrefixArgs a;
+    a.q = q, a.kp = k_prefix, a.vp = v_prefix, a.k = k, a.v = v;
+    a.q_b = strides[0], a.q_t = strides[1], a.q_h = strides[2];
+    a.kp_t = strides[3], a.kp_h = strides[4], a.vp_t = strides[5], a.vp_h = strides[6];
+    a.k_b = strides[7], a.k_t = strides[8], a.k_h = strides[9];
+    a.v_b = strides[10], a.v_t = strides[11], a.v_h = strides[12];
+    a.lengths = lengths;
+    a.out = out;
+    a.lse = lse;
+    a.B = (int)B, a.Tq = (int)Tq, a.Hq = (int)Hq, a.Hkv = (int)Hkv, a.G = (int)(Hq / Hkv);
+    a.P = (int)P, a.T = (int)T;
+    a.Sp = p.Sp, a.So = p.So;
+    a.rows = B * Tq * Hq;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    uint8_t* s = static_cast<uint8_t*>(scratch);
+    a.part_o = reinterpret_cast<float*>(s);
+    s += round256((p.Sp + p.So) * a.rows * D * 4);
+    a.part_lse = reinterpret_cast<float*>(s);
+    s += round256((p.Sp + p.So) * a.rows * 4);
+    a.lse2 = reinterpret_cast<float*>(s);
+    int rc = launch_prefix_simt(a, dtype, (int)D, stream);
+    if (rc == LSA_OK) rc = launch_prefix_merge(a, dtype, (int)D, stream);
+    if (rc == LSA_OK && scores && T > 0) rc = launch_own_weights(a, dtype, (int)D, scores, scores_out, stream);
+    return rc;
+}
+
+}  // extern "C"

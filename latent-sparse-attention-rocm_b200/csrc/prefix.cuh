@@ -1,0 +1,66 @@
+// prefix.cuh - what the kernels of the shared-prefix attention share (sm_100a).
+//
+// B sequences read the same P prefix keys, stored once, and then their own caches. Query row
+// (b, i) of Tq sees every prefix key and the own keys j < lengths[b] - Tq + i + 1 (lengths
+// count the call's Tq new tokens). For a (query row, query head) pair with logits
+// s_j = scale (q . k_j):
+//   m = max s_j,  l = sum e^(s_j - m),  o = sum e^(s_j - m) v_j / l,  lse = m + log l.
+// Sums over disjoint key ranges ("parts": the prefix's splits, the own cache's splits) join by
+//   o = sum_c 2^(lse_c - M) o_c / sum_c 2^(lse_c - M),  M = max lse_c
+// (lse in the log2 domain), so the prefix is one product of all sequences' rows with keys that
+// are read once, whatever the batch. A pair that sees no key reads as zeros, lse -inf.
+#pragma once
+
+#include <stdint.h>
+
+#include "common.cuh"
+
+namespace lsa {
+
+constexpr int kMaxParts = 64;  // prefix splits + own splits of one call
+
+// strides in elements; the last dimension is contiguous everywhere
+struct PrefixArgs {
+    const void *q, *kp, *vp, *k, *v;
+    int64_t q_b, q_t, q_h;                // q [B, Tq, Hq, D]
+    int64_t kp_t, kp_h, vp_t, vp_h;       // prefix [P, Hkv, D]
+    int64_t k_b, k_t, k_h, v_b, v_t, v_h; // own [B, T, Hkv, D]
+    const int32_t* lengths;               // [B]
+    void* out;                            // [B, Tq, Hq, D] contiguous
+    float* part_o;                        // [parts][rows][D], each part normalised by its own sum
+    float* part_lse;                      // [parts][rows], log2 domain, -inf: no key
+    float* lse2;                          // [rows], log2 domain: the joined lse
+    float* lse;                           // [rows], natural, or null
+    int B, Tq, Hq, Hkv, G;
+    int P, T;
+    int Sp, So;                           // splits of the prefix and of the own caches
+    int64_t rows;                         // B * Tq * Hq
+    float scale_log2;                     // scale * log2(e)
+};
+
+// own keys that sequence b holds
+__device__ __forceinline__ int own_length(const PrefixArgs& a, int b) {
+    const int n = a.lengths[b];
+    return n < 0 ? 0 : (n > a.T ? a.T : n);
+}
+
+// row r of KV head h in a segment's row order ((token, query head of the group) pairs):
+// the row's place in q / out and its index among all rows
+__device__ __forceinline__ int64_t row_index(const PrefixArgs& a, int64_t token, int h, int g) {
+    return token * a.Hq + (int64_t)h * a.G + g;
+}
+
+// The part of [0, n) that split s of S takes, in units of `unit` keys: sizes differ by one unit.
+__device__ __host__ __forceinline__ void split_range(int n, int s, int S, int unit, int* k0, int* k1) {
+    const int64_t units = ((int64_t)n + unit - 1) / unit;
+    const int64_t a = units * s / S * unit, b = units * (s + 1) / S * unit;
+    *k0 = (int)(a < n ? a : n);
+    *k1 = (int)(b < n ? b : n);
+}
+
+int launch_prefix_simt(const PrefixArgs& a, int dtype, int D, cudaStream_t stream);
+int launch_prefix_merge(const PrefixArgs& a, int dtype, int D, cudaStream_t stream);
+int launch_own_weights(const PrefixArgs& a, int dtype, int D, const float* scores, float* scores_out,
+                       cudaStream_t stream);
+
+}  // namespace lsa

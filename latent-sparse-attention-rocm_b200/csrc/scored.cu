@@ -1,0 +1,105 @@
+// scored.cu - attention weights of the own keys, added to a running score (sm_100a).
+//
+// With every row's lse known (prefix.cuh), key j of sequence b and KV head h gains
+//   w_j = sum over the rows r = (token, head of the group) that see j of 2^(s_rj - lse_r)
+// (log2 domain), the total attention it received. One thread owns a key, so the sum has one
+// order and one writer: no atomics, the same bits every time.
+#include "prefix.cuh"
+
+namespace lsa {
+namespace {
+
+constexpr int kWKeys = 128;  // keys of a CTA: one per thread
+constexpr int kWRows = 8;    // query rows staged at a time
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kWKeys) own_weights_kernel(const PrefixArgs a, const float* __restrict__ scores,
+                                                             float* __restrict__ scores_out) {
+    constexpr int LDK = D + 4;
+    extern __shared__ float sm[];
+    float* sk = sm;                // [kWKeys][LDK]
+    float* sq = sm + kWKeys * LDK; // [kWRows][D]
+    __shared__ float slse[kWRows];
+    const int b = blockIdx.z, h = blockIdx.y, j0 = blockIdx.x * kWKeys, tid = threadIdx.x;
+    const int len = own_length(a, b), j = j0 + tid;
+    const int64_t at = ((int64_t)b * a.Hkv + h) * a.T + j;
+    if (j0 >= len) {
+        if (j < a.T) scores_out[at] = scores[at];
+        return;
+    }
+    const T* kb = static_cast<const T*>(a.k) + b * a.k_b + h * a.k_h;
+    for (int i = tid; i < kWKeys * (D / 8); i += kWKeys) {
+        const int r = i / (D / 8), c = i % (D / 8);
+        float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (j0 + r < len) load8<T>(kb + (int64_t)(j0 + r) * a.k_t + c * 8, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sk[r * LDK + c * 8 + e] = x[e];
+    }
+    const int nrows = a.Tq * a.G;
+    const float4* k4 = reinterpret_cast<const float4*>(sk + tid * LDK);
+    float w = 0.0f;
+    for (int r0 = 0; r0 < nrows; r0 += kWRows) {
+        __syncthreads();
+        for (int i = tid; i < kWRows * (D / 8); i += kWKeys) {
+            const int r = r0 + i / (D / 8), c = i % (D / 8);
+            float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (r < nrows)
+                load8<T>(static_cast<const T*>(a.q) + b * a.q_b + r / a.G * a.q_t + (h * (int64_t)a.G + r % a.G) * a.q_h +
+                             c * 8,
+                         x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sq[(i / (D / 8)) * D + c * 8 + e] = x[e];
+        }
+        if (tid < kWRows)
+            slse[tid] = r0 + tid < nrows
+                            ? a.lse2[row_index(a, (int64_t)b * a.Tq + (r0 + tid) / a.G, h, (r0 + tid) % a.G)]
+                            : 0.0f;
+        __syncthreads();
+        float s[kWRows] = {};
+#pragma unroll 4
+        for (int c = 0; c < D / 4; ++c) {
+            const float4 kk = k4[c];
+#pragma unroll
+            for (int u = 0; u < kWRows; ++u) {
+                const float4 qq = reinterpret_cast<const float4*>(sq + u * D)[c];
+                s[u] = fmaf(qq.x, kk.x, fmaf(qq.y, kk.y, fmaf(qq.z, kk.z, fmaf(qq.w, kk.w, s[u]))));
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kWRows; ++u) {
+            const int r = r0 + u;
+            if (r < nrows && j < len - a.Tq + r / a.G + 1) w += exp2f(s[u] * a.scale_log2 - slse[u]);
+        }
+    }
+    if (j < a.T) scores_out[at] = scores[at] + w;
+}
+
+template <typename T, int D>
+int weights_launch(const PrefixArgs& a, const float* scores, float* scores_out, cudaStream_t stream) {
+    const int smem = (kWKeys * (D + 4) + kWRows * D) * 4;
+    auto kern = own_weights_kernel<T, D>;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+        return LSA_ERR_CUDA;
+    if (a.B > 65535 || a.Hkv > 65535) return LSA_ERR_SIZE;
+    dim3 grid((unsigned)((a.T + kWKeys - 1) / kWKeys), (unsigned)a.Hkv, (unsigned)a.B);
+    kern<<<grid, kWKeys, smem, stream>>>(a, scores, scores_out);
+    LSA_LAUNCH_CHECK();
+    return LSA_OK;
+}
+
+template <typename T>
+int weights_d(const PrefixArgs& a, int D, const float* scores, float* scores_out, cudaStream_t stream) {
+    return D == 128 ? weights_launch<T, 128>(a, scores, scores_out, stream)
+                    : weights_launch<T, 64>(a, scores, scores_out, stream);
+}
+
+}  // namespace
+
+int launch_own_weights(const PrefixArgs& a, int dtype, int D, const float* scores, float* scores_out,
+                       cudaStream_t stream) {
+    if (dtype == kF32) return weights_d<float>(a, D, scores, scores_out, stream);
+    if (dtype == kF16) return weights_d<__half>(a, D, scores, scores_out, stream);
+    return weights_d<__nv_bfloat16>(a, D, scores, scores_out, stream);
+}
+
+}  // namespace lsa

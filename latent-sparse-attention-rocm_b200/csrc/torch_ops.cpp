@@ -8,6 +8,10 @@
 //                     sink, top_k) -> (lists, lengths)          flat_select fused, pipeline.py:274-316
 //                     (index_queries [R, d], or raw queries [R, Hq, D]: regroup fused in)
 //   lsa::sparse_read(q, k, v, ids, lengths, scale) -> out     sparse_read_auto, read_kernel_tiled.py:147
+//   lsa::shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths, scale) -> (out, lse)
+//   lsa::scored_attention(q, k_prefix, v_prefix, k, v, lengths, scores, scale) -> (out, scores)
+//   lsa::evict(k, v, scores, lengths, budget, window, sink, capacity)
+//                     -> (k, v, scores, lengths, ids)            no reference counterpart
 //   lsa::workspace_counters() -> Tensor[]                      the cached counter buffers (checks)
 // Meta implementations give FX / torch.compile the output shapes. Workspaces: scratch (any
 // content) and int32 counters (zero at rest: the kernels that use them leave them zero) cached
@@ -17,6 +21,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 
+#include <cmath>
 #include <map>
 #include <mutex>
 #include <tuple>
@@ -181,6 +186,130 @@ at::Tensor sparse_read_cuda(const at::Tensor& q_in, const at::Tensor& k_in, cons
     return out;
 }
 
+// a tensor whose last dimension is contiguous and whose rows start on 16-byte boundaries, as
+// it is when it already is one (a cache's view is not copied)
+at::Tensor rows16(const at::Tensor& t) {
+    const int64_t unit = 16 / t.element_size();
+    bool ok = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+    for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && (t.size(i) == 1 || t.stride(i) % unit == 0);
+    if (ok) return t;
+    auto c = t.contiguous();
+    return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
+}
+
+// stride of a dimension; 0 where the dimension has one entry and any stride would do
+int64_t stride_of(const at::Tensor& t, int64_t i) { return t.size(i) == 1 ? 0 : t.stride(i); }
+
+struct PrefixOut {
+    at::Tensor out, lse, scores;
+};
+
+PrefixOut prefix_attention(const at::Tensor& q_in, const at::Tensor& kp_in, const at::Tensor& vp_in,
+                           const at::Tensor& k_in, const at::Tensor& v_in, const at::Tensor& lengths_in,
+                           const at::Tensor* scores_in, double scale, bool want_lse, const char* what) {
+    for (const at::Tensor* t : {&q_in, &kp_in, &vp_in, &k_in, &v_in, &lengths_in})
+        TORCH_CHECK_VALUE(t->is_cuda() && t->device() == q_in.device(), what,
+                          " is a CUDA kernel: every tensor on one CUDA device");
+    TORCH_CHECK_VALUE(q_in.dim() == 4 && k_in.dim() == 4 && v_in.sizes() == k_in.sizes(), what,
+                      ": q [B, Tq, Hq, D], k / v [B, T, Hkv, D]");
+    TORCH_CHECK_VALUE(kp_in.dim() == 3 && vp_in.sizes() == kp_in.sizes(), what, ": k_prefix / v_prefix [P, Hkv, D]");
+    const int64_t B = q_in.size(0), Tq = q_in.size(1), Hq = q_in.size(2), D = q_in.size(3);
+    const int64_t T = k_in.size(1), Hkv = k_in.size(2), P = kp_in.size(0);
+    TORCH_CHECK_VALUE(k_in.size(0) == B && k_in.size(3) == D && kp_in.size(1) == Hkv && kp_in.size(2) == D, what,
+                      ": batch, KV heads and head dim of q, the prefix and the own caches differ");
+    TORCH_CHECK_VALUE(Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && Hq / Hkv <= 64, what,
+                      ": query heads must group evenly onto KV heads, at most 64 to one");
+    TORCH_CHECK_VALUE(D == 64 || D == 128, what, ": head dim 64 or 128, got ", D);
+    for (const at::Tensor* t : {&kp_in, &vp_in, &k_in, &v_in})
+        TORCH_CHECK_VALUE(t->scalar_type() == q_in.scalar_type(), what, ": q, the prefix and the caches share a dtype");
+    TORCH_CHECK_VALUE(q_in.scalar_type() == at::kFloat || q_in.scalar_type() == at::kHalf ||
+                          q_in.scalar_type() == at::kBFloat16,
+                      what, ": fp32, fp16 or bf16, got ", q_in.scalar_type());
+    TORCH_CHECK_VALUE(lengths_in.numel() == B && !lengths_in.is_floating_point(), what, ": one whole length a sequence");
+    TORCH_CHECK_VALUE(std::isfinite(scale) && scale > 0, what, ": the scale must be positive, got ", scale);
+    c10::cuda::CUDAGuard guard(q_in.device());
+    auto q = rows16(q_in), kp = rows16(kp_in), vp = rows16(vp_in), k = rows16(k_in), v = rows16(v_in);
+    auto lengths = lengths_in.to(at::kInt).contiguous();
+    PrefixOut r;
+    r.out = at::empty({B, Tq, Hq, D}, q.options());
+    if (want_lse) r.lse = at::empty({B, Tq, Hq}, q.options().dtype(at::kFloat));
+    at::Tensor scores;
+    if (scores_in) {
+        TORCH_CHECK_VALUE(scores_in->device() == q_in.device() && scores_in->scalar_type() == at::kFloat &&
+                              scores_in->dim() == 3 && scores_in->size(0) == B && scores_in->size(1) == Hkv &&
+                              scores_in->size(2) == T,
+                          what, ": scores [B, Hkv, T] fp32");
+        scores = scores_in->contiguous();
+        r.scores = B * Tq == 0 ? scores.clone() : at::empty_like(scores);
+    }
+    if (B * Tq == 0) return r;
+    const int code = dtype_code(q.scalar_type());
+    const int64_t bytes = lsa_shared_prefix_scratch(code, B, Tq, Hq, Hkv, D, P, T);
+    TORCH_CHECK_VALUE(bytes >= 0, what, ": sizes out of range");
+    auto stream = at::cuda::getCurrentCUDAStream();
+    Workspace& w = workspace(q.device(), stream, bytes, 0);
+    const int64_t strides[13] = {stride_of(q, 0), stride_of(q, 1), stride_of(q, 2), stride_of(kp, 0), stride_of(kp, 1),
+                                 stride_of(vp, 0), stride_of(vp, 1), stride_of(k, 0), stride_of(k, 1),
+                                 stride_of(k, 2), stride_of(v, 0), stride_of(v, 1), stride_of(v, 2)};
+    check_rc(lsa_shared_prefix_attention(q.data_ptr(), kp.data_ptr(), vp.data_ptr(), k.data_ptr(), v.data_ptr(), code,
+                                         strides, lengths.data_ptr<int32_t>(), B, Tq, Hq, Hkv, D, P, T, (float)scale,
+                                         r.out.data_ptr(), want_lse ? r.lse.data_ptr<float>() : nullptr,
+                                         scores_in ? scores.data_ptr<float>() : nullptr,
+                                         scores_in ? r.scores.data_ptr<float>() : nullptr, w.scratch.data_ptr(),
+                                         w.scratch.numel(), stream),
+             what);
+    return r;
+}
+
+std::tuple<at::Tensor, at::Tensor> shared_prefix_cuda(const at::Tensor& q, const at::Tensor& kp, const at::Tensor& vp,
+                                                      const at::Tensor& k, const at::Tensor& v,
+                                                      const at::Tensor& lengths, double scale) {
+    auto r = prefix_attention(q, kp, vp, k, v, lengths, nullptr, scale, true, "shared_prefix_attention");
+    return {r.out, r.lse};
+}
+
+std::tuple<at::Tensor, at::Tensor> scored_cuda(const at::Tensor& q, const at::Tensor& kp, const at::Tensor& vp,
+                                               const at::Tensor& k, const at::Tensor& v, const at::Tensor& lengths,
+                                               const at::Tensor& scores, double scale) {
+    auto r = prefix_attention(q, kp, vp, k, v, lengths, &scores, scale, false, "scored_attention");
+    return {r.out, r.scores};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> evict_cuda(
+    const at::Tensor& k_in, const at::Tensor& v_in, const at::Tensor& scores_in, const at::Tensor& lengths_in,
+    int64_t budget, int64_t window, int64_t sink, int64_t capacity) {
+    for (const at::Tensor* t : {&k_in, &v_in, &scores_in, &lengths_in})
+        TORCH_CHECK_VALUE(t->is_cuda() && t->device() == k_in.device(),
+                          "evict is a CUDA kernel: every tensor on one CUDA device");
+    TORCH_CHECK_VALUE(k_in.dim() == 4 && v_in.sizes() == k_in.sizes() && v_in.scalar_type() == k_in.scalar_type(),
+                      "evict: k / v [B, T, Hkv, D] of one dtype");
+    const int64_t B = k_in.size(0), T = k_in.size(1), Hkv = k_in.size(2), D = k_in.size(3), es = k_in.element_size();
+    TORCH_CHECK_VALUE(Hkv > 0 && D > 0 && D * es % 16 == 0, "evict: rows of a multiple of 16 bytes, got ", D * es);
+    TORCH_CHECK_VALUE(scores_in.scalar_type() == at::kFloat && scores_in.dim() == 3 && scores_in.size(0) == B &&
+                          scores_in.size(1) == Hkv && scores_in.size(2) == T,
+                      "evict: scores [B, Hkv, T] fp32");
+    TORCH_CHECK_VALUE(lengths_in.numel() == B && !lengths_in.is_floating_point(), "evict: one whole length a sequence");
+    TORCH_CHECK_VALUE(budget >= 0 && window >= 0 && sink >= 0 && window + sink <= budget && capacity >= budget,
+                      "evict: window + sink (", window, " + ", sink, ") must fit the budget (", budget,
+                      "), and the budget the capacity (", capacity, ")");
+    c10::cuda::CUDAGuard guard(k_in.device());
+    auto k = rows16(k_in), v = rows16(v_in);
+    auto scores = scores_in.contiguous();
+    auto lengths = lengths_in.to(at::kInt).contiguous();
+    auto ko = at::empty({B, capacity, Hkv, D}, k.options()), vo = at::empty({B, capacity, Hkv, D}, k.options());
+    auto so = at::empty({B, Hkv, capacity}, scores.options());
+    auto lo = at::empty({B}, lengths.options()), ids = at::empty({B, Hkv, capacity}, lengths.options());
+    if (B == 0) return {ko, vo, so, lo, ids};
+    const int64_t strides[6] = {stride_of(k, 0) * es, stride_of(k, 1) * es, stride_of(k, 2) * es,
+                                stride_of(v, 0) * es, stride_of(v, 1) * es, stride_of(v, 2) * es};
+    check_rc(lsa_evict(k.data_ptr(), v.data_ptr(), D * es, strides, scores.data_ptr<float>(),
+                       lengths.data_ptr<int32_t>(), B, T, Hkv, budget, window, sink, capacity, ko.data_ptr(),
+                       vo.data_ptr(), so.data_ptr<float>(), lo.data_ptr<int32_t>(), ids.data_ptr<int32_t>(),
+                       at::cuda::getCurrentCUDAStream()),
+             "evict");
+    return {ko, vo, so, lo, ids};
+}
+
 std::vector<at::Tensor> workspace_counters() {
     std::lock_guard<std::mutex> lock(g_ws_mutex);
     std::vector<at::Tensor> out;
@@ -208,6 +337,29 @@ at::Tensor sparse_read_meta(const at::Tensor& q, const at::Tensor&, const at::Te
     return at::empty_like(q);
 }
 
+std::tuple<at::Tensor, at::Tensor> shared_prefix_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor&,
+                                                      const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                                                      double) {
+    return {at::empty(q.sizes(), q.options()),
+            at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat))};
+}
+
+std::tuple<at::Tensor, at::Tensor> scored_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor&,
+                                               const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                                               const at::Tensor& scores, double) {
+    return {at::empty(q.sizes(), q.options()), at::empty(scores.sizes(), scores.options())};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> evict_meta(
+    const at::Tensor& k, const at::Tensor&, const at::Tensor& scores, const at::Tensor& lengths, int64_t, int64_t,
+    int64_t, int64_t capacity) {
+    auto i32 = lengths.options().dtype(at::kInt);
+    const int64_t B = k.size(0), Hkv = k.size(2);
+    auto ko = at::empty({B, capacity, Hkv, k.size(3)}, k.options());
+    return {ko, at::empty_like(ko), at::empty({B, Hkv, capacity}, scores.options()), at::empty({B}, i32),
+            at::empty({B, Hkv, capacity}, i32)};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(lsa, m) {
@@ -215,6 +367,12 @@ TORCH_LIBRARY(lsa, m) {
     m.def("select_fused(Tensor index_queries, Tensor positions, Tensor centroids, Tensor members, int block, int bpb, "
           "int top_p, int window, int sink, int top_k) -> (Tensor, Tensor)");
     m.def("sparse_read(Tensor q, Tensor k, Tensor v, Tensor ids, Tensor lengths, float scale) -> Tensor");
+    m.def("shared_prefix_attention(Tensor q, Tensor k_prefix, Tensor v_prefix, Tensor k, Tensor v, Tensor lengths, "
+          "float scale) -> (Tensor, Tensor)");
+    m.def("scored_attention(Tensor q, Tensor k_prefix, Tensor v_prefix, Tensor k, Tensor v, Tensor lengths, "
+          "Tensor scores, float scale) -> (Tensor, Tensor)");
+    m.def("evict(Tensor k, Tensor v, Tensor scores, Tensor lengths, int budget, int window, int sink, int capacity) "
+          "-> (Tensor, Tensor, Tensor, Tensor, Tensor)");
     m.def("workspace_counters() -> Tensor[]", &workspace_counters);
 }
 
@@ -222,10 +380,16 @@ TORCH_LIBRARY_IMPL(lsa, CUDA, m) {
     m.impl("regroup", &regroup_cuda);
     m.impl("select_fused", &select_fused_cuda);
     m.impl("sparse_read", &sparse_read_cuda);
+    m.impl("shared_prefix_attention", &shared_prefix_cuda);
+    m.impl("scored_attention", &scored_cuda);
+    m.impl("evict", &evict_cuda);
 }
 
 TORCH_LIBRARY_IMPL(lsa, Meta, m) {
     m.impl("regroup", &regroup_meta);
     m.impl("select_fused", &select_fused_meta);
     m.impl("sparse_read", &sparse_read_meta);
+    m.impl("shared_prefix_attention", &shared_prefix_meta);
+    m.impl("scored_attention", &scored_meta);
+    m.impl("evict", &evict_meta);
 }
