@@ -45,11 +45,12 @@ extern "C" {
  * j < lengths[b] - Tq + i + 1; a row that sees none reads as zeros, lse -inf. What the own
  * caches hold at or past lengths[b] is never used. strides[13], in elements: q (b, t, h),
  * k_prefix (t, h), v_prefix (t, h), k (b, t, h), v (b, t, h); the head dimension is contiguous,
- * every base and stride a multiple of 16 bytes. D 64 or 128, Hq / Hkv at most 64; scale > 0.
+ * every base and stride a multiple of 16 bytes, every stride of a dimension longer than one positive. D 64 or 128, Hq / Hkv at most 64; scale > 0.
  * out [B, Tq, Hq, D] contiguous, lse [B, Tq, Hq] (natural logarithm) or NULL.
  * scores / scores_out [B, Hkv, T] fp32, or both NULL: scores_out = scores + the attention
  * weight that own key j received from every (row, query head of the group) of the call; the
  * entries at or past lengths[b] are copied. scores_out may be scores.
+ * status: a device int32 that receives LSA_ERR_TIMEOUT if a bounded wait expires.
  * lsa_shared_prefix_scratch: the scratch bytes of a call (LSA_ERR_ARG for refused sizes). */
 int64_t lsa_shared_prefix_scratch(int dtype, int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_t P,
                                   int64_t T);
@@ -57,7 +58,7 @@ int lsa_shared_prefix_attention(const void* q, const void* k_prefix, const void*
                                 const void* v, int dtype, const int64_t* strides, const int32_t* lengths, int64_t B,
                                 int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_t P, int64_t T, float scale,
                                 void* out, float* lse, const float* scores, float* scores_out, void* scratch,
-                                int64_t scratch_bytes, cudaStream_t stream);
+                                int64_t scratch_bytes, int32_t* status, cudaStream_t stream);
 
 /* Eviction from a cache by score (no reference counterpart). k / v rows of row_bytes bytes (a
  * multiple of 16) at strides[6], in bytes: k (b, t, h), v (b, t, h); scores [B, Hkv, T] fp32,

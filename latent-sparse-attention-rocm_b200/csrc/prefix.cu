@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(kSimtWarps * 32) prefix_simt_kernel(const Pref
         split = item % a.So, item /= a.So;
         tile = item % otiles, item /= otiles;
         h = item % a.Hkv, b = item / a.Hkv;
-        part = a.Sp + split;
+        part = a.parts_p + split;
         nrows = a.Tq * a.G;
         len = own_length(a, b);
         split_range(len, split, a.So, kSimtKeys, &k0, &k1);
@@ -192,29 +192,71 @@ template <typename T>
 int merge_d(const PrefixArgs& a, int D, cudaStream_t stream) {
     const unsigned grid = (unsigned)((a.rows + 7) / 8);
     if (D == 128)
-        prefix_merge_kernel<T, 128><<<grid, 256, 0, stream>>>(a, a.Sp + a.So);
+        prefix_merge_kernel<T, 128><<<grid, 256, 0, stream>>>(a, a.parts_p + a.parts_o);
     else
-        prefix_merge_kernel<T, 64><<<grid, 256, 0, stream>>>(a, a.Sp + a.So);
+        prefix_merge_kernel<T, 64><<<grid, 256, 0, stream>>>(a, a.parts_p + a.parts_o);
     LSA_LAUNCH_CHECK();
     return LSA_OK;
 }
 
 struct Plan {
-    int Sp, So;
+    int Sp, So, parts_p, parts_o;
+    bool tiles;  // tensor cores
+    TilePlan tile;
 };
 
-// Splits enough that the work items of each segment fill the GPU about four times.
-Plan make_plan(int64_t B, int64_t Tq, int64_t Hkv, int64_t G, int64_t P, int64_t T) {
-    auto splits = [](int64_t items, int64_t keys) -> int {
-        if (keys == 0) return 0;
-        int64_t s = (592 + items - 1) / items;
-        const int64_t most = (keys + 255) / 256;
-        s = s < most ? s : most;
-        return (int)(s < kMaxParts / 2 ? s : kMaxParts / 2);
-    };
-    Plan p;
-    p.Sp = splits(Hkv * ((B * Tq * G + kSimtRows - 1) / kSimtRows), P);
-    p.So = splits(B * Hkv * ((Tq * G + kSimtRows - 1) / kSimtRows), T);
+constexpr int kSMs = 148;
+
+// Splits of `chunks` for `items` equal work items on 148 SMs, one item an SM at a time: the
+// fewest that minimise waves x (chunks of an item + its fixed cost in chunks).
+int balance(int64_t items, int64_t chunks, int64_t fixed) {
+    if (chunks == 0) return 0;
+    int best = 1;
+    int64_t least = INT64_MAX;
+    for (int s = 1; s <= kMaxSplits && s <= chunks; ++s) {
+        const int64_t cost = (items * s + kSMs - 1) / kSMs * ((chunks + s - 1) / s + fixed);
+        if (cost < least) least = cost, best = s;
+    }
+    return best;
+}
+
+Plan make_plan(int dtype, int64_t B, int64_t Tq, int64_t Hkv, int64_t G, int64_t P, int64_t T) {
+    Plan p = {};
+    p.tiles = dtype != kF32;
+    if (!p.tiles) {
+        // splits enough that the work items of each segment fill the GPU about four times
+        auto splits = [](int64_t items, int64_t keys) -> int {
+            if (keys == 0) return 0;
+            int64_t s = (4 * kSMs + items - 1) / items;
+            const int64_t most = (keys + 255) / 256;
+            s = s < most ? s : most;
+            return (int)(s < kMaxSplits ? s : kMaxSplits);
+        };
+        p.parts_p = p.Sp = splits(Hkv * ((B * Tq * G + kSimtRows - 1) / kSimtRows), P);
+        p.parts_o = p.So = splits(B * Hkv * ((Tq * G + kSimtRows - 1) / kSimtRows), T);
+        return p;
+    }
+    TilePlan& t = p.tile;
+    const int64_t rows = Tq * G;
+    const int64_t pc = (P + 127) / 128, oc = (T + 127) / 128;
+    t.seq_streams = rows <= 128;
+    t.seq_tiles = (int)(rows <= 128 ? 1 : (rows + 255) / 256);
+    const int64_t seq = B * Hkv * t.seq_tiles;
+    t.joint = P > 0 && rows * 4 >= (int64_t)t.seq_tiles * 256 * 3;
+    if (t.joint) {
+        p.So = balance(seq, pc + oc, 3);
+        p.parts_o = p.So;
+        t.direct = p.So == 1;
+    } else {
+        t.batch_streams = B * rows <= 128;
+        t.batch_tiles = (int)(B * rows <= 128 ? 1 : (B * rows + 255) / 256);
+        p.Sp = balance(Hkv * t.batch_tiles, t.batch_streams ? (pc + 1) / 2 : pc, 3);
+        p.parts_p = p.Sp * (t.batch_streams ? 2 : 1);
+        t.batch_items = (int)(Hkv * t.batch_tiles * p.Sp);
+        p.So = balance(seq, t.seq_streams ? (oc + 1) / 2 : oc, 3);
+        p.parts_o = p.So * (t.seq_streams ? 2 : 1);
+    }
+    t.seq_items = (int)(seq * p.So);
     return p;
 }
 
@@ -252,21 +294,22 @@ int64_t lsa_shared_prefix_scratch(int dtype, int64_t B, int64_t Tq, int64_t Hq, 
                                   int64_t T) {
     if (!sizes_ok(B, Tq, Hq, Hkv, D, P, T) || dtype < kF32 || dtype > kBF16) return LSA_ERR_ARG;
     if (B == 0 || Tq == 0) return 0;
-    const Plan p = make_plan(B, Tq, Hkv, Hq / Hkv, P, T);
+    const Plan p = make_plan(dtype, B, Tq, Hkv, Hq / Hkv, P, T);
     const int64_t rows = B * Tq * Hq;
-    return round256((p.Sp + p.So) * rows * D * 4) + round256((p.Sp + p.So) * rows * 4) + round256(rows * 4);
+    const int64_t parts = p.parts_p + p.parts_o;
+    return round256(parts * rows * D * 4) + round256(parts * rows * 4) + round256(rows * 4);
 }
 
 int lsa_shared_prefix_attention(const void* q, const void* k_prefix, const void* v_prefix, const void* k,
                                 const void* v, int dtype, const int64_t* strides, const int32_t* lengths, int64_t B,
                                 int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_t P, int64_t T, float scale,
                                 void* out, float* lse, const float* scores, float* scores_out, void* scratch,
-                                int64_t scratch_bytes, cudaStream_t stream) {
+                                int64_t scratch_bytes, int32_t* status, cudaStream_t stream) {
     if (!sizes_ok(B, Tq, Hq, Hkv, D, P, T) || dtype < kF32 || dtype > kBF16) return LSA_ERR_ARG;
     if ((scores == nullptr) != (scores_out == nullptr) || strides == nullptr) return LSA_ERR_ARG;
     if (!(scale > 0.0f) || !(scale < INFINITY)) return LSA_ERR_ARG;  // the kernels take the maximum before the scale
     if (B == 0 || Tq == 0) return LSA_OK;
-    if (q == nullptr || out == nullptr || lengths == nullptr || scratch == nullptr) return LSA_ERR_ARG;
+    if (q == nullptr || out == nullptr || lengths == nullptr || scratch == nullptr || status == nullptr) return LSA_ERR_ARG;
     if ((P > 0 && (k_prefix == nullptr || v_prefix == nullptr)) || (T > 0 && (k == nullptr || v == nullptr)))
         return LSA_ERR_ARG;
     // 16-byte loads: every base and every stride
@@ -274,32 +317,39 @@ int lsa_shared_prefix_attention(const void* q, const void* k_prefix, const void*
     for (const void* p : {q, P ? k_prefix : nullptr, P ? v_prefix : nullptr, T ? k : nullptr, T ? v : nullptr,
                           (const void*)out, (const void*)scratch})
         if ((uintptr_t)p & 15) return LSA_ERR_ARG;
-    for (int i = 0; i < 13; ++i)
-        if (strides[i] < 0 || strides[i] % unit) return LSA_ERR_ARG;
+    // a dimension of one entry takes any stride: D stands for it
+    const int64_t extent[13] = {B, Tq, Hq, P, Hkv, P, Hkv, B, T, Hkv, B, T, Hkv};
+    int64_t st[13];
+    for (int i = 0; i < 13; ++i) {
+        st[i] = extent[i] > 1 ? strides[i] : D;
+        if (st[i] <= 0 || st[i] % unit || st[i] >= (int64_t)1 << 38) return LSA_ERR_ARG;
+    }
     if (scratch_bytes < lsa_shared_prefix_scratch(dtype, B, Tq, Hq, Hkv, D, P, T)) return LSA_ERR_ARG;
-    const Plan p = make_plan(B, Tq, Hkv, Hq / Hkv, P, T);
+    const Plan p = make_plan(dtype, B, Tq, Hkv, Hq / Hkv, P, T);
     PrefixArgs a;
     a.q = q, a.kp = k_prefix, a.vp = v_prefix, a.k = k, a.v = v;
-    a.q_b = strides[0], a.q_t = strides[1], a.q_h = strides[2];
-    a.kp_t = strides[3], a.kp_h = strides[4], a.vp_t = strides[5], a.vp_h = strides[6];
-    a.k_b = strides[7], a.k_t = strides[8], a.k_h = strides[9];
-    a.v_b = strides[10], a.v_t = strides[11], a.v_h = strides[12];
+    a.q_b = st[0], a.q_t = st[1], a.q_h = st[2];
+    a.kp_t = st[3], a.kp_h = st[4], a.vp_t = st[5], a.vp_h = st[6];
+    a.k_b = st[7], a.k_t = st[8], a.k_h = st[9];
+    a.v_b = st[10], a.v_t = st[11], a.v_h = st[12];
     a.lengths = lengths;
     a.out = out;
     a.lse = lse;
     a.B = (int)B, a.Tq = (int)Tq, a.Hq = (int)Hq, a.Hkv = (int)Hkv, a.G = (int)(Hq / Hkv);
     a.P = (int)P, a.T = (int)T;
-    a.Sp = p.Sp, a.So = p.So;
+    a.Sp = p.Sp, a.So = p.So, a.parts_p = p.parts_p, a.parts_o = p.parts_o;
+    a.status = status;
     a.rows = B * Tq * Hq;
     a.scale_log2 = scale * 1.4426950408889634f;
     uint8_t* s = static_cast<uint8_t*>(scratch);
     a.part_o = reinterpret_cast<float*>(s);
-    s += round256((p.Sp + p.So) * a.rows * D * 4);
+    s += round256((p.parts_p + p.parts_o) * a.rows * D * 4);
     a.part_lse = reinterpret_cast<float*>(s);
-    s += round256((p.Sp + p.So) * a.rows * 4);
+    s += round256((p.parts_p + p.parts_o) * a.rows * 4);
     a.lse2 = reinterpret_cast<float*>(s);
-    int rc = launch_prefix_simt(a, dtype, (int)D, stream);
-    if (rc == LSA_OK) rc = launch_prefix_merge(a, dtype, (int)D, stream);
+    int rc = p.tiles ? launch_prefix_tiles(a, p.tile, dtype, (int)D, stream)
+                     : launch_prefix_simt(a, dtype, (int)D, stream);
+    if (rc == LSA_OK && !(p.tiles && p.tile.direct)) rc = launch_prefix_merge(a, dtype, (int)D, stream);
     if (rc == LSA_OK && scores && T > 0) rc = launch_own_weights(a, dtype, (int)D, scores, scores_out, stream);
     return rc;
 }

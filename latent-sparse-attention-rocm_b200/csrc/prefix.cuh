@@ -17,7 +17,7 @@
 
 namespace lsa {
 
-constexpr int kMaxParts = 64;  // prefix splits + own splits of one call
+constexpr int kMaxSplits = 32;  // of the prefix, and of the own caches
 
 // strides in elements; the last dimension is contiguous everywhere
 struct PrefixArgs {
@@ -34,8 +34,19 @@ struct PrefixArgs {
     int B, Tq, Hq, Hkv, G;
     int P, T;
     int Sp, So;                           // splits of the prefix and of the own caches
+    int parts_p, parts_o;                 // parts of a row from the prefix and from its own cache
     int64_t rows;                         // B * Tq * Hq
     float scale_log2;                     // scale * log2(e)
+    int32_t* status;                      // LSA_ERR_TIMEOUT after an expired wait
+};
+
+// The work of the tensor-core kernel (prefix_tile.cu).
+struct TilePlan {
+    int batch_items, batch_tiles;  // row tiles over all sequences: prefix keys
+    int seq_items, seq_tiles;      // row tiles of a sequence: its own keys
+    bool batch_streams, seq_streams;  // tiles of at most 128 rows: two streams of chunks
+    bool joint;                    // seq tiles read the prefix too
+    bool direct;                   // a row has one part: the kernel writes the output
 };
 
 // own keys that sequence b holds
@@ -59,6 +70,7 @@ __device__ __host__ __forceinline__ void split_range(int n, int s, int S, int un
 }
 
 int launch_prefix_simt(const PrefixArgs& a, int dtype, int D, cudaStream_t stream);
+int launch_prefix_tiles(const PrefixArgs& a, const TilePlan& tp, int dtype, int D, cudaStream_t stream);
 int launch_prefix_merge(const PrefixArgs& a, int dtype, int D, cudaStream_t stream);
 int launch_own_weights(const PrefixArgs& a, int dtype, int D, const float* scores, float* scores_out,
                        cudaStream_t stream);

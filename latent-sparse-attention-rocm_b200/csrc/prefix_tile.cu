@@ -1,0 +1,583 @@
+// prefix_tile.cu - the shared-prefix attention on the 5th-generation tensor cores (sm_100a).
+//
+// A work item is a tile of query rows of one KV head x a range of 128-key chunks. Row tiles:
+//   batch tiles  rows of all sequences ((b, token, query head of the group)), prefix keys only:
+//                the whole batch meets each prefix key once;
+//   seq tiles    rows of one sequence, its own keys - after the prefix's, when the sequence's
+//                rows fill a tile by themselves (joint: no parts to join then).
+// One CTA per item, two halves of 128 rows (M = 128 each):
+//   S_h = Q_h K^T   tcgen05.mma kind::f16, Q and K in 128B-swizzled shared memory, S in TMEM
+//   softmax         one thread per row: S row from TMEM, running maximum and sum in fp32 (exp2
+//                   domain; O is rescaled only when the maximum has grown by more than 2^8), P
+//                   back over S as 16-bit pairs
+//   O_h += P_h V    tcgen05.mma with A = P from TMEM, V an MN-major shared-memory operand
+// With more than 128 rows the halves are different rows of the same chunks; with at most 128 both
+// halves hold the same rows and take alternate chunks (two streams), which keeps two softmax
+// chains in flight where the keys' bandwidth, not arithmetic, is the bound.
+// P is rounded to the inputs' 16-bit type for its product (the sum l adds the unrounded fp32
+// values); everything else is fp32.
+//
+// Warps: 0 loads K and V tiles by TMA (cp.async.bulk.tensor, one ring of 128-key tiles in the
+// order the MMAs use them), 1 issues every MMA (unrolled, one thread: 64 cycles per 128 x 128 x 16
+// MMA, the pipe's rate), 4-7 / 8-11 are the softmax of half 0 / 1. TMEM: S_0/P_0 [0, 128),
+// S_1/P_1 [128, 256), O_0 [256, 256 + D), O_1 [384, 384 + D).
+// Rows of V at or past a sequence's length are zeroed in shared memory before their product, so
+// whatever an unwritten slot holds (0 x NaN) stays out.
+//
+// Every wait is bounded (1 s); an expired wait raises a CTA-wide flag, every role leaves, copies
+// and MMAs in flight are waited for (bounded), the TMEM is released and LSA_ERR_TIMEOUT lands in
+// the status word.
+#include <cuda.h>
+
+#include "prefix.cuh"
+#include "umma.cuh"
+
+namespace lsa {
+namespace {
+
+constexpr int kThreads = 384;
+constexpr int kChunk = 128;
+constexpr uint64_t kWaitNs = 1000000000ull;
+
+struct TileMaps {
+    CUtensorMap kp, vp, k, v;
+};
+
+template <int D> struct TileShape {
+    static constexpr int kTileBytes = kChunk * D * 2;  // one K, V or half-Q tile
+    static constexpr int kStages = D == 128 ? 5 : 10;
+    static constexpr int kOffStage = 2 * kTileBytes;
+    static constexpr int kOffBar = kOffStage + kStages * kTileBytes;
+    static constexpr int kNumBars = 2 * kStages + 1 + 2 + 4 + 2 + 1;
+    static constexpr int kOffMisc = kOffBar + kNumBars * 8;
+    static constexpr int kSmem = kOffMisc + 16 + 1024;  // slack: the base is aligned to 1024 B
+    static_assert(kSmem <= 232448, "shared memory of a CTA");
+};
+
+__device__ __forceinline__ bool role_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+    bool done = mbar_try_wait(bar, parity);
+    if (__all_sync(0xFFFFFFFFu, done)) return true;
+    const uint64_t t0 = global_ns();
+    for (;;) {
+        if (!done) done = mbar_try_wait(bar, parity);
+        if (__all_sync(0xFFFFFFFFu, done)) return true;
+        int stop = 0;
+        if ((threadIdx.x & 31) == 0) stop = (*abort_flag != 0) || (global_ns() - t0 > kWaitNs);
+        if (__shfl_sync(0xFFFFFFFFu, stop, 0)) {
+            if ((threadIdx.x & 31) == 0) *abort_flag = 1;
+            return false;
+        }
+    }
+}
+
+__device__ __forceinline__ void tma_tile(uint32_t dst, const CUtensorMap* map, int x, int t, int h, int b,
+                                         uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, "
+        "%5}], [%6];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(t), "r"(h), "r"(b), "r"(smem_u32(bar))
+        : "memory");
+}
+
+__device__ __forceinline__ uint32_t pack16(float a, float b, __nv_bfloat16*) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack16(float a, float b, __half*) {
+    __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+}
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// What a CTA works on.
+struct Item {
+    bool own, streams;  // seq tile; both halves hold the same rows
+    int b, h, r0, nrows, part, len;
+    int np;      // prefix chunks of the item's chunk list
+    int c0, c1;  // its chunks of the list [0, np + own chunks)
+};
+
+__device__ __forceinline__ Item item_of(const PrefixArgs& a, const TilePlan& t) {
+    Item w;
+    int i = blockIdx.x;
+    w.own = i >= t.batch_items;
+    int chunks, S, split, tile;
+    if (!w.own) {
+        S = a.Sp;
+        split = i % S, i /= S;
+        tile = i % t.batch_tiles;
+        w.h = i / t.batch_tiles;
+        w.b = 0;
+        w.len = 0;
+        w.streams = t.batch_streams;
+        w.nrows = a.B * a.Tq * a.G;
+        w.r0 = tile * (w.streams ? 128 : 256);
+        w.np = chunks = (a.P + kChunk - 1) / kChunk;
+        w.part = 0;
+    } else {
+        i -= t.batch_items;
+        S = a.So;
+        split = i % S, i /= S;
+        w.h = i % a.Hkv, i /= a.Hkv;
+        w.b = i % a.B;
+        tile = t.seq_tiles - 1 - i / a.B;  // the longest causal ranges first
+        w.len = own_length(a, w.b);
+        w.streams = t.seq_streams;
+        w.nrows = a.Tq * a.G;
+        w.r0 = tile * (w.streams ? 128 : 256);
+        const int last = (w.r0 + (w.streams ? 128 : 256) < w.nrows ? w.r0 + (w.streams ? 128 : 256) : w.nrows) - 1;
+        int seen = w.len - a.Tq + last / a.G + 1;  // own keys that the tile's last row sees
+        seen = seen < 0 ? 0 : seen;
+        w.np = t.joint ? (a.P + kChunk - 1) / kChunk : 0;
+        chunks = w.np + (seen + kChunk - 1) / kChunk;
+        w.part = t.joint ? 0 : a.parts_p;
+    }
+    w.part += split * (w.streams ? 2 : 1);
+    split_range(chunks, split, S, 1, &w.c0, &w.c1);
+    return w;
+}
+
+template <typename T, int D>
+__device__ __forceinline__ void softmax_half(const PrefixArgs& a, const TilePlan& tp, const Item& w, uint64_t* bars,
+                                             volatile int* abort_flag, uint32_t tmem) {
+    using Sh = TileShape<D>;
+    uint64_t *bar_s = bars + 2 * Sh::kStages + 1, *bar_p = bar_s + 2, *bar_o = bar_p + 4;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int hf = (warp - 4) >> 2, qd = warp & 3;
+    const int r = w.r0 + (w.streams ? 0 : hf * 128) + qd * 32 + lane;
+    const bool live = r < w.nrows;
+    const int tok = r / a.G;
+    // own keys the row sees; a prefix key is seen by all
+    const int own_limit = !live ? 0 : (w.own ? w.len - a.Tq + tok + 1 : 0);
+    const int pre_limit = live ? a.P : 0;
+    const uint32_t lanes = (uint32_t)(qd * 32) << 16;
+    const uint32_t tS = tmem + lanes + hf * 128;
+    const uint32_t tO = tmem + lanes + 256 + hf * 128;
+    const int step = w.streams ? 2 : 1, first = w.c0 + (w.streams ? hf : 0);
+    const int n = w.c1 > first ? (w.c1 - first + step - 1) / step : 0;
+    float m = -INFINITY, l = 0.0f;
+    const float sl = a.scale_log2, thresh = 8.0f / sl;
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
+        const int c = first + j * step;
+        const int seen = c < w.np ? pre_limit - c * kChunk : own_limit - (c - w.np) * kChunk;
+        ok = role_wait(&bar_s[hf], j & 1, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t s[128];
+        tmem_ld64_wait<0>(tS, s);
+        tmem_ld64_wait<64>(tS + 64, s);
+        if (__any_sync(0xFFFFFFFFu, seen < kChunk)) {
+#pragma unroll
+            for (int i = 0; i < 128; ++i)
+                if (i >= seen) s[i] = 0xFF800000u;  // -inf
+        }
+        float mx4[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx4[i] = fmaxf(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
+#pragma unroll
+        for (int i = 8; i < 128; i += 8)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                mx4[e] = max3(mx4[e], __uint_as_float(s[i + 2 * e]), __uint_as_float(s[i + 2 * e + 1]));
+        const float mn = fmaxf(m, max3(mx4[0], mx4[1], fmaxf(mx4[2], mx4[3])));
+        float alpha = 1.0f;
+        const bool grow = mn > m + thresh;
+        if (grow) {
+            alpha = ex2_approx((m - mn) * sl);
+            m = mn;
+        }
+        const float neg = m == -INFINITY ? 0.0f : -m * sl;
+        const uint64_t sl2 = pair(sl, sl), neg2 = pair(neg, neg);
+        uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            uint32_t pk[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                const int e = 64 * half + 2 * i;
+                float x0, x1;
+                unpair(fma2(pair(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), sl2, neg2), x0, x1);
+                const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+                sum[i & 3] = add2(sum[i & 3], pair(p0, p1));
+                pk[i] = pack16(p0, p1, (T*)nullptr);
+            }
+            // O_h holds the earlier chunks' sum here (their products were issued before S_h(j) by
+            // the same thread); its rescale lands before any P of this chunk is published
+            if (half == 0 && j > 0 && __any_sync(0xFFFFFFFFu, grow)) {
+#pragma unroll 1
+                for (int cc = 0; cc < D / 32; ++cc) {
+                    uint32_t o[32];
+                    tmem_ld32_wait(tO + cc * 32, o);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                    tmem_st32(tO + cc * 32, o);
+                }
+            }
+            tmem_st32(tS + 32 * half, pk);
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(&bar_p[2 * hf + half]);
+        }
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) unpair(sum[i], x[2 * i], x[2 * i + 1]);
+        l = l * alpha + (((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7])));
+    }
+    if (ok && n > 0) ok = role_wait(&bar_o[hf], 0, abort_flag);
+    if (!ok) return;
+    const int64_t rid = row_index(a, (int64_t)w.b * a.Tq + tok, w.h, r - tok * a.G);
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const float lse = l > 0.0f ? m * sl + log2f(l) : -INFINITY;
+    if (tp.direct) {
+        if (live) {
+            a.lse2[rid] = lse;
+            if (a.lse) a.lse[rid] = lse * 0.69314718055994531f;
+        }
+        T* dst = static_cast<T*>(a.out) + rid * D;
+        if (n > 0) {
+            tc_fence_after();
+#pragma unroll
+            for (int cc = 0; cc < D / 32; ++cc) {
+                uint32_t o[32];
+                tmem_ld32_wait(tO + cc * 32, o);
+                if (live) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t u[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            u[e] = pack16(__uint_as_float(o[8 * i + 2 * e]) * inv,
+                                          __uint_as_float(o[8 * i + 2 * e + 1]) * inv, (T*)nullptr);
+                        *reinterpret_cast<uint4*>(dst + cc * 32 + i * 8) = make_uint4(u[0], u[1], u[2], u[3]);
+                    }
+                }
+            }
+        } else if (live) {
+            for (int i = 0; i < D / 8; ++i) reinterpret_cast<uint4*>(dst)[i] = make_uint4(0, 0, 0, 0);
+        }
+        return;
+    }
+    const int64_t at = (int64_t)(w.part + (w.streams ? hf : 0)) * a.rows + rid;
+    if (live) a.part_lse[at] = lse;
+    if (n > 0) {  // a part without a key is not read
+        tc_fence_after();
+        float* dst = a.part_o + at * D;
+#pragma unroll
+        for (int cc = 0; cc < D / 32; ++cc) {
+            uint32_t o[32];
+            tmem_ld32_wait(tO + cc * 32, o);
+            if (live) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    *reinterpret_cast<float4*>(dst + cc * 32 + i * 4) =
+                        make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv,
+                                    __uint_as_float(o[4 * i + 2]) * inv, __uint_as_float(o[4 * i + 3]) * inv);
+            }
+        }
+    }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    prefix_tile_kernel(const __grid_constant__ TileMaps maps, const PrefixArgs a, const TilePlan tp) {
+    using Sh = TileShape<D>;
+    constexpr int NS = Sh::kStages, KS = D / 16;
+    extern __shared__ uint8_t raw[];
+    uint8_t* sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+    const uint32_t sbase = smem_u32(sm);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Sh::kOffBar);
+    uint64_t *full = bars, *empty = bars + NS, *bar_q = bars + 2 * NS, *bar_s = bar_q + 1, *bar_p = bar_s + 2,
+             *bar_o = bar_p + 4, *bar_drain = bar_o + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + Sh::kOffMisc);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + Sh::kOffMisc + 4);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const Item w = item_of(a, tp);
+    const int n = w.c1 - w.c0;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < NS; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        mbar_init(bar_q, 256);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bar_s[i], 1);
+            mbar_init(&bar_p[2 * i], 128);
+            mbar_init(&bar_p[2 * i + 1], 128);
+            mbar_init(&bar_o[i], 1);
+        }
+        mbar_init(bar_drain, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) tmem_alloc(tmem_slot, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp >= 4) {
+        // 384 threads launch at 168 registers: 128 x 56 + 256 x 224 = 384 x 168
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;" ::: "memory");
+        // Q rows into the swizzled tiles (rows past the item's are zeros)
+        const int rows = w.streams ? 128 : 256;
+        for (int i = threadIdx.x - 128; i < rows * (D / 8); i += 256) {
+            const int row = i / (D / 8), c = i % (D / 8), r = w.r0 + row, rl = row & 127;
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (r < w.nrows) {
+                const int tok = r / a.G;
+                const int64_t bt = (int64_t)w.b * a.Tq + tok;
+                x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + bt / a.Tq * a.q_b + bt % a.Tq * a.q_t +
+                                                    (w.h * (int64_t)a.G + r - tok * a.G) * a.q_h + c * 8);
+            }
+            const uint32_t off = (row >> 7) * Sh::kTileBytes + (c >> 3) * 16384 + rl * 128 + (((c & 7) ^ (rl & 7)) << 4);
+            *reinterpret_cast<uint4*>(sm + off) = x;
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(bar_q);
+        softmax_half<T, D>(a, tp, w, bars, abort_flag, tmem);
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;" ::: "memory");
+        if (warp == 0) {
+            // ------------------------------------------------ loads, in the order the MMAs use them
+            int pos = 0;
+            auto load = [&](bool val, int c) -> bool {
+                const int s = pos % NS;
+                if (pos >= NS && !role_wait(&empty[s], (pos / NS - 1) & 1, abort_flag)) return false;
+                if (lane == 0) {
+                    const uint32_t dst = sbase + Sh::kOffStage + s * Sh::kTileBytes;
+                    const bool pre = c < w.np;
+                    const CUtensorMap* map = pre ? (val ? &maps.vp : &maps.kp) : (val ? &maps.v : &maps.k);
+                    const int t = (pre ? c : c - w.np) * kChunk, b = pre ? 0 : w.b;
+                    mbar_arrive_expect_tx(&full[s], Sh::kTileBytes);
+#pragma unroll
+                    for (int x = 0; x < D; x += 64) tma_tile(dst + x * 256, map, x, t, w.h, b, &full[s]);
+                }
+                __syncwarp();
+                ++pos;
+                return true;
+            };
+            bool ok = true;
+            const int ahead = w.streams ? 2 : 1;  // K chunks scored before the first product with V
+            for (int c = w.c0; ok && c < w.c1 && c < w.c0 + ahead; ++c) ok = load(false, c);
+            for (int c = w.c0; ok && c < w.c1; ++c) {
+                ok = load(true, c);
+                if (ok && c + ahead < w.c1) ok = load(false, c + ahead);
+            }
+            if (!ok) {  // every copy issued lands before the CTA leaves
+                for (int p = pos > NS ? pos - NS : 0; p < pos; ++p) mbar_wait_bounded(&full[p % NS], (p / NS) & 1);
+            }
+        } else if (warp == 1) {
+            // ------------------------------------------------ every MMA of the CTA
+            constexpr uint32_t idS = umma_idesc_f16<T>(128, 128, false);
+            constexpr uint32_t idO = umma_idesc_f16<T>(128, D, true);
+            int pos = 0;
+            auto stage = [&](int p) { return sbase + Sh::kOffStage + (p % NS) * Sh::kTileBytes; };
+            auto ready = [&](int p) { return role_wait(&full[p % NS], (p / NS) & 1, abort_flag); };
+            auto scores = [&](int hf, int p, bool last_use) {
+                if (lane == 0) {
+                    const uint32_t qa = sbase + (w.streams ? 0 : hf * Sh::kTileBytes), ka = stage(p);
+#pragma unroll
+                    for (int kk = 0; kk < KS; ++kk) {
+                        const uint32_t off = (kk >> 2) * 16384 + (kk & 3) * 32;
+                        umma_f16_ss(tmem + hf * 128, sw128_desc(qa + off, 16, 1024), sw128_desc(ka + off, 16, 1024),
+                                    idS, kk > 0);
+                    }
+                    umma_commit(&bar_s[hf]);
+                    if (last_use) umma_commit(&empty[p % NS]);
+                }
+                __syncwarp();
+            };
+            auto product = [&](int hf, int p, bool fresh, int half) {
+                if (lane == 0) {
+                    const uint32_t va = stage(p);
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) {
+                        const int k8 = half * 4 + kk;
+                        umma_f16_ts(tmem + 256 + hf * 128, tmem + hf * 128 + k8 * 8,
+                                    sw128_desc(va + k8 * 2048, 16384, 1024), idO, !fresh || k8 > 0);
+                    }
+                }
+                __syncwarp();
+            };
+            auto free_stage = [&](int p) {
+                if (lane == 0) umma_commit(&empty[p % NS]);
+                __syncwarp();
+            };
+            // rows of V past the sequence's keys: zeros, whatever the slots hold
+            auto clean = [&](int p, int c) {
+                if (c < w.np) return;
+                const int valid = w.len - (c - w.np) * kChunk;
+                if (valid >= kChunk) return;
+                uint8_t* va = sm + Sh::kOffStage + (p % NS) * Sh::kTileBytes;
+                for (int i = (valid < 0 ? 0 : valid) * 8 + lane; i < kChunk * 8; i += 32)
+#pragma unroll
+                    for (int x = 0; x < D / 64; ++x)
+                        *reinterpret_cast<uint4*>(va + x * 16384 + i * 16) = make_uint4(0, 0, 0, 0);
+                fence_proxy_async_smem();
+                __syncwarp();
+            };
+            bool ok = n == 0 || role_wait(bar_q, 0, abort_flag);
+            if (!w.streams) {
+                if (ok && n > 0) {
+                    ok = ready(0);
+                    tc_fence_after();
+                    if (ok) scores(0, 0, false), scores(1, 0, true);
+                    pos = 1;
+                }
+                for (int j = 0; ok && j < n; ++j) {
+                    const int pv = pos, pk = pos + 1;
+                    const bool more = j + 1 < n;
+                    for (int hf = 0; ok && hf < 2; ++hf) {
+                        if (hf == 0) {
+                            ok = ready(pv);
+                            if (ok) clean(pv, w.c0 + j);
+                        }
+                        for (int half = 0; ok && half < 2; ++half) {
+                            ok = role_wait(&bar_p[2 * hf + half], j & 1, abort_flag);
+                            tc_fence_after();
+                            if (ok) product(hf, pv, j == 0, half);
+                        }
+                        if (ok && hf == 1) free_stage(pv);
+                        if (ok && more) {
+                            if (hf == 0) {
+                                ok = ready(pk);
+                                tc_fence_after();
+                            }
+                            if (ok) scores(hf, pk, hf == 1);
+                        }
+                    }
+                    pos += more ? 2 : 1;
+                }
+            } else {
+                for (int c = 0; ok && c < n && c < 2; ++c) {
+                    ok = ready(pos);
+                    tc_fence_after();
+                    if (ok) scores(c, pos, true);
+                    ++pos;
+                }
+                for (int c = 0; ok && c < n; ++c) {
+                    const int hf = c & 1;
+                    ok = ready(pos);
+                    if (ok) clean(pos, w.c0 + c);
+                    for (int half = 0; ok && half < 2; ++half) {
+                        ok = role_wait(&bar_p[2 * hf + half], (c >> 1) & 1, abort_flag);
+                        tc_fence_after();
+                        if (ok) product(hf, pos, c < 2, half);
+                    }
+                    if (ok) free_stage(pos);
+                    ++pos;
+                    if (ok && c + 2 < n) {
+                        ok = ready(pos);
+                        tc_fence_after();
+                        if (ok) scores(hf, pos, true);
+                        ++pos;
+                    }
+                }
+            }
+            if (lane == 0) {
+                if (ok) umma_commit(&bar_o[0]), umma_commit(&bar_o[1]);
+                umma_commit(bar_drain);  // every MMA completes before the TMEM is released
+            }
+            __syncwarp();
+            mbar_wait_bounded(bar_drain, 0);
+            __syncwarp();
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+    if (threadIdx.x == 0 && *abort_flag) atomicExch(a.status, LSA_ERR_TIMEOUT);
+}
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encode_fn() {
+    static EncodeFn fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) !=
+                cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<EncodeFn>(p);
+    }();
+    return fn;
+}
+
+// [B, T, H, D] rows as 64-element x 128-key boxes, 128-byte swizzle; zeros past the extents.
+bool encode_rows(CUtensorMap* map, bool bf16, const void* base, int64_t D, int64_t T, int64_t H, int64_t B,
+                 int64_t st, int64_t sh, int64_t sb) {
+    const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)T, (cuuint64_t)H, (cuuint64_t)B};
+    const cuuint64_t strides[3] = {(cuuint64_t)st * 2, (cuuint64_t)sh * 2, (cuuint64_t)sb * 2};
+    const cuuint32_t box[4] = {64, kChunk, 1, 1}, es[4] = {1, 1, 1, 1};
+    return encode_fn()(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                       const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int D>
+int launch(const TileMaps& maps, const PrefixArgs& a, const TilePlan& tp, unsigned grid, cudaStream_t stream) {
+    auto kern = prefix_tile_kernel<T, D>;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, TileShape<D>::kSmem) != cudaSuccess)
+        return LSA_ERR_CUDA;
+    kern<<<grid, kThreads, TileShape<D>::kSmem, stream>>>(maps, a, tp);
+    LSA_LAUNCH_CHECK();
+    return LSA_OK;
+}
+
+}  // namespace
+
+int launch_prefix_tiles(const PrefixArgs& a, const TilePlan& tp, int dtype, int D, cudaStream_t stream) {
+    const int64_t items = (int64_t)tp.batch_items + tp.seq_items;
+    if (items == 0) return LSA_OK;
+    if (items > INT32_MAX) return LSA_ERR_SIZE;
+    if (encode_fn() == nullptr) return LSA_ERR_CUDA;
+    TileMaps maps;
+    const bool bf = dtype == kBF16;
+    bool ok = true;
+    if (a.P > 0 && (tp.batch_items || tp.joint))
+        ok = encode_rows(&maps.kp, bf, a.kp, D, a.P, a.Hkv, 1, a.kp_t, a.kp_h, (int64_t)D) &&
+             encode_rows(&maps.vp, bf, a.vp, D, a.P, a.Hkv, 1, a.vp_t, a.vp_h, (int64_t)D);
+    if (ok && a.T > 0 && tp.seq_items)
+        ok = encode_rows(&maps.k, bf, a.k, D, a.T, a.Hkv, a.B, a.k_t, a.k_h, a.k_b) &&
+             encode_rows(&maps.v, bf, a.v, D, a.T, a.Hkv, a.B, a.v_t, a.v_h, a.v_b);
+    if (!ok) return LSA_ERR_ARG;
+    const unsigned grid = (unsigned)items;
+    if (dtype == kBF16)
+        return D == 128 ? launch<__nv_bfloat16, 128>(maps, a, tp, grid, stream)
+                        : launch<__nv_bfloat16, 64>(maps, a, tp, grid, stream);
+    return D == 128 ? launch<__half, 128>(maps, a, tp, grid, stream)
+                    : launch<__half, 64>(maps, a, tp, grid, stream);
+}
+
+}  // namespace lsa

@@ -186,12 +186,12 @@ at::Tensor sparse_read_cuda(const at::Tensor& q_in, const at::Tensor& k_in, cons
     return out;
 }
 
-// a tensor whose last dimension is contiguous and whose rows start on 16-byte boundaries, as
-// it is when it already is one (a cache's view is not copied)
+// a tensor whose last dimension is contiguous and whose rows start on 16-byte boundaries, a
+// stride apart: as it is when it already is one (a cache's view is not copied), else a copy
 at::Tensor rows16(const at::Tensor& t) {
     const int64_t unit = 16 / t.element_size();
     bool ok = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
-    for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && (t.size(i) == 1 || t.stride(i) % unit == 0);
+    for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && (t.size(i) <= 1 || (t.stride(i) > 0 && t.stride(i) % unit == 0));
     if (ok) return t;
     auto c = t.contiguous();
     return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
@@ -247,7 +247,7 @@ PrefixOut prefix_attention(const at::Tensor& q_in, const at::Tensor& kp_in, cons
     const int64_t bytes = lsa_shared_prefix_scratch(code, B, Tq, Hq, Hkv, D, P, T);
     TORCH_CHECK_VALUE(bytes >= 0, what, ": sizes out of range");
     auto stream = at::cuda::getCurrentCUDAStream();
-    Workspace& w = workspace(q.device(), stream, bytes, 0);
+    Workspace& w = workspace(q.device(), stream, bytes, 64);
     const int64_t strides[13] = {stride_of(q, 0), stride_of(q, 1), stride_of(q, 2), stride_of(kp, 0), stride_of(kp, 1),
                                  stride_of(vp, 0), stride_of(vp, 1), stride_of(k, 0), stride_of(k, 1),
                                  stride_of(k, 2), stride_of(v, 0), stride_of(v, 1), stride_of(v, 2)};
@@ -256,7 +256,7 @@ PrefixOut prefix_attention(const at::Tensor& q_in, const at::Tensor& kp_in, cons
                                          r.out.data_ptr(), want_lse ? r.lse.data_ptr<float>() : nullptr,
                                          scores_in ? scores.data_ptr<float>() : nullptr,
                                          scores_in ? r.scores.data_ptr<float>() : nullptr, w.scratch.data_ptr(),
-                                         w.scratch.numel(), stream),
+                                         w.scratch.numel(), w.counters.data_ptr<int32_t>(), stream),
              what);
     return r;
 }

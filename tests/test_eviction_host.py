@@ -59,7 +59,7 @@ def test_c_entries_refuse_before_any_cuda_call():
     buf = ctypes.c_void_p(4096)  # never dereferenced
     ok = dict(q=buf, kp=buf, vp=buf, k=buf, v=buf, dtype=2, strides=[1024, 1024, 128] + [256, 128] * 2 + [2048, 256, 128] * 2,
               lengths=buf, B=2, Tq=1, Hq=8, Hkv=2, D=128, P=16, T=8, scale=0.1, out=buf, lse=None, scores=None,
-              scores_out=None, scratch=buf, bytes=1 << 30)
+              scores_out=None, scratch=buf, bytes=1 << 30, status=buf)
 
     def call(**kw):
         a = dict(ok, **kw)
@@ -67,11 +67,11 @@ def test_c_entries_refuse_before_any_cuda_call():
         return L.lsa_shared_prefix_attention(a["q"], a["kp"], a["vp"], a["k"], a["v"], a["dtype"], st, a["lengths"],
                                              a["B"], a["Tq"], a["Hq"], a["Hkv"], a["D"], a["P"], a["T"], a["scale"],
                                              a["out"], a["lse"], a["scores"], a["scores_out"], a["scratch"],
-                                             a["bytes"], None)
+                                             a["bytes"], a["status"], None)
 
     for kw in (dict(D=96), dict(Hq=7), dict(Hq=130, Hkv=2), dict(Hkv=0), dict(dtype=3), dict(B=-1), dict(P=-1),
                dict(T=1 << 31), dict(q=None), dict(kp=None), dict(v=None), dict(out=None), dict(lengths=None),
-               dict(scratch=None), dict(bytes=16), dict(strides=None), dict(scores=buf), dict(scores_out=buf),
+               dict(scratch=None), dict(bytes=16), dict(status=None), dict(strides=None), dict(scores=buf), dict(scores_out=buf),
                dict(q=ctypes.c_void_p(4100)), dict(vp=ctypes.c_void_p(4098)), dict(scale=0.0), dict(scale=-1.0),
                dict(scale=float("nan")), dict(strides=[1024, 1024, 132] + [256, 128] * 2 + [2048, 256, 128] * 2),
                dict(strides=[-8] + [1024, 128] + [256, 128] * 2 + [2048, 256, 128] * 2)):
