@@ -201,29 +201,31 @@ int merge_d(const PrefixArgs& a, int D, cudaStream_t stream) {
 
 struct Plan {
     int Sp, So, parts_p, parts_o;
-    bool tiles;  // tensor cores
+    bool simt, logits;  // fp32 inputs; the own keys' logits are kept for their weights
     TilePlan tile;
+    RowsPlan rows;
 };
 
 constexpr int kSMs = 148;
+constexpr int kFewRows = 16;  // rows of a KV head that the few-row kernel takes
 
-// Splits of `chunks` for `items` equal work items on 148 SMs, one item an SM at a time: the
+// Splits of `chunks` for `items` equal work items on `slots` places that hold one item each: the
 // fewest that minimise waves x (chunks of an item + its fixed cost in chunks).
-int balance(int64_t items, int64_t chunks, int64_t fixed) {
+int balance(int64_t items, int64_t chunks, int64_t fixed, int64_t slots) {
     if (chunks == 0) return 0;
     int best = 1;
     int64_t least = INT64_MAX;
     for (int s = 1; s <= kMaxSplits && s <= chunks; ++s) {
-        const int64_t cost = (items * s + kSMs - 1) / kSMs * ((chunks + s - 1) / s + fixed);
+        const int64_t cost = (items * s + slots - 1) / slots * ((chunks + s - 1) / s + fixed);
         if (cost < least) least = cost, best = s;
     }
     return best;
 }
 
-Plan make_plan(int dtype, int64_t B, int64_t Tq, int64_t Hkv, int64_t G, int64_t P, int64_t T) {
+Plan make_plan(int dtype, int64_t B, int64_t Tq, int64_t Hkv, int64_t G, int64_t P, int64_t T, bool scored) {
     Plan p = {};
-    p.tiles = dtype != kF32;
-    if (!p.tiles) {
+    p.simt = dtype == kF32;
+    if (p.simt) {
         // splits enough that the work items of each segment fill the GPU about four times
         auto splits = [](int64_t items, int64_t keys) -> int {
             if (keys == 0) return 0;
@@ -244,19 +246,31 @@ Plan make_plan(int dtype, int64_t B, int64_t Tq, int64_t Hkv, int64_t G, int64_t
     const int64_t seq = B * Hkv * t.seq_tiles;
     t.joint = P > 0 && rows * 4 >= (int64_t)t.seq_tiles * 256 * 3;
     if (t.joint) {
-        p.So = balance(seq, pc + oc, 3);
+        p.So = balance(seq, pc + oc, 3, kSMs);
         p.parts_o = p.So;
+        t.seq_items = (int)(seq * p.So);
         t.direct = p.So == 1;
+        return p;
+    }
+    if (B * rows <= kFewRows) {
+        p.parts_p = p.Sp = balance(Hkv, (P + 63) / 64, 2, 2 * kSMs);
+        p.rows.prefix_items = (int)(Hkv * p.Sp);
     } else {
         t.batch_streams = B * rows <= 128;
         t.batch_tiles = (int)(B * rows <= 128 ? 1 : (B * rows + 255) / 256);
-        p.Sp = balance(Hkv * t.batch_tiles, t.batch_streams ? (pc + 1) / 2 : pc, 3);
+        p.Sp = balance(Hkv * t.batch_tiles, t.batch_streams ? (pc + 1) / 2 : pc, 3, kSMs);
         p.parts_p = p.Sp * (t.batch_streams ? 2 : 1);
         t.batch_items = (int)(Hkv * t.batch_tiles * p.Sp);
-        p.So = balance(seq, t.seq_streams ? (oc + 1) / 2 : oc, 3);
-        p.parts_o = p.So * (t.seq_streams ? 2 : 1);
     }
-    t.seq_items = (int)(seq * p.So);
+    if (rows <= kFewRows) {
+        p.parts_o = p.So = balance(B * Hkv, (T + 63) / 64, 2, 2 * kSMs);
+        p.rows.own_items = (int)(B * Hkv * p.So);
+        p.logits = scored;
+    } else {
+        p.So = balance(seq, t.seq_streams ? (oc + 1) / 2 : oc, 3, kSMs);
+        p.parts_o = p.So * (t.seq_streams ? 2 : 1);
+        t.seq_items = (int)(seq * p.So);
+    }
     return p;
 }
 
@@ -291,13 +305,14 @@ using namespace lsa;
 extern "C" {
 
 int64_t lsa_shared_prefix_scratch(int dtype, int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_t P,
-                                  int64_t T) {
+                                  int64_t T, int scored) {
     if (!sizes_ok(B, Tq, Hq, Hkv, D, P, T) || dtype < kF32 || dtype > kBF16) return LSA_ERR_ARG;
     if (B == 0 || Tq == 0) return 0;
-    const Plan p = make_plan(dtype, B, Tq, Hkv, Hq / Hkv, P, T);
+    const Plan p = make_plan(dtype, B, Tq, Hkv, Hq / Hkv, P, T, scored);
     const int64_t rows = B * Tq * Hq;
     const int64_t parts = p.parts_p + p.parts_o;
-    return round256(parts * rows * D * 4) + round256(parts * rows * 4) + round256(rows * 4);
+    return round256(parts * rows * D * 4) + round256(parts * rows * 4) + round256(rows * 4) +
+           (p.logits ? round256(rows * T * 4) : 0);
 }
 
 int lsa_shared_prefix_attention(const void* q, const void* k_prefix, const void* v_prefix, const void* k,
@@ -324,8 +339,8 @@ int lsa_shared_prefix_attention(const void* q, const void* k_prefix, const void*
         st[i] = extent[i] > 1 ? strides[i] : D;
         if (st[i] <= 0 || st[i] % unit || st[i] >= (int64_t)1 << 38) return LSA_ERR_ARG;
     }
-    if (scratch_bytes < lsa_shared_prefix_scratch(dtype, B, Tq, Hq, Hkv, D, P, T)) return LSA_ERR_ARG;
-    const Plan p = make_plan(dtype, B, Tq, Hkv, Hq / Hkv, P, T);
+    if (scratch_bytes < lsa_shared_prefix_scratch(dtype, B, Tq, Hq, Hkv, D, P, T, scores != nullptr)) return LSA_ERR_ARG;
+    const Plan p = make_plan(dtype, B, Tq, Hkv, Hq / Hkv, P, T, scores != nullptr);
     PrefixArgs a;
     a.q = q, a.kp = k_prefix, a.vp = v_prefix, a.k = k, a.v = v;
     a.q_b = st[0], a.q_t = st[1], a.q_h = st[2];
@@ -347,10 +362,15 @@ int lsa_shared_prefix_attention(const void* q, const void* k_prefix, const void*
     a.part_lse = reinterpret_cast<float*>(s);
     s += round256((p.parts_p + p.parts_o) * a.rows * 4);
     a.lse2 = reinterpret_cast<float*>(s);
-    int rc = p.tiles ? launch_prefix_tiles(a, p.tile, dtype, (int)D, stream)
-                     : launch_prefix_simt(a, dtype, (int)D, stream);
-    if (rc == LSA_OK && !(p.tiles && p.tile.direct)) rc = launch_prefix_merge(a, dtype, (int)D, stream);
-    if (rc == LSA_OK && scores && T > 0) rc = launch_own_weights(a, dtype, (int)D, scores, scores_out, stream);
+    RowsPlan rows = p.rows;
+    if (p.logits) rows.logits = reinterpret_cast<float*>(s + round256(a.rows * 4));
+    int rc = p.simt ? launch_prefix_simt(a, dtype, (int)D, stream) : LSA_OK;
+    if (rc == LSA_OK && !p.simt) rc = launch_prefix_tiles(a, p.tile, dtype, (int)D, stream);
+    if (rc == LSA_OK && !p.simt) rc = launch_prefix_rows(a, rows, dtype, (int)D, stream);
+    if (rc == LSA_OK && !p.tile.direct) rc = launch_prefix_merge(a, dtype, (int)D, stream);
+    if (rc == LSA_OK && scores && T > 0)
+        rc = p.logits ? launch_logit_weights(a, rows.logits, scores, scores_out, stream)
+                      : launch_own_weights(a, dtype, (int)D, scores, scores_out, stream);
     return rc;
 }
 

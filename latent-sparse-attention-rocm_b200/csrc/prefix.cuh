@@ -69,10 +69,19 @@ __device__ __host__ __forceinline__ void split_range(int n, int s, int S, int un
     *k1 = (int)(b < n ? b : n);
 }
 
+// The work of the few-row kernel (prefix_rows.cu): segments of at most 16 rows a KV head.
+struct RowsPlan {
+    int prefix_items, own_items;
+    float* logits;  // [B, Hkv, Tq * G, T] log2-domain logits of the own keys, or null
+};
+
 int launch_prefix_simt(const PrefixArgs& a, int dtype, int D, cudaStream_t stream);
 int launch_prefix_tiles(const PrefixArgs& a, const TilePlan& tp, int dtype, int D, cudaStream_t stream);
+int launch_prefix_rows(const PrefixArgs& a, const RowsPlan& rp, int dtype, int D, cudaStream_t stream);
 int launch_prefix_merge(const PrefixArgs& a, int dtype, int D, cudaStream_t stream);
 int launch_own_weights(const PrefixArgs& a, int dtype, int D, const float* scores, float* scores_out,
                        cudaStream_t stream);
+int launch_logit_weights(const PrefixArgs& a, const float* logits, const float* scores, float* scores_out,
+                         cudaStream_t stream);
 
 }  // namespace lsa

@@ -244,7 +244,7 @@ PrefixOut prefix_attention(const at::Tensor& q_in, const at::Tensor& kp_in, cons
     }
     if (B * Tq == 0) return r;
     const int code = dtype_code(q.scalar_type());
-    const int64_t bytes = lsa_shared_prefix_scratch(code, B, Tq, Hq, Hkv, D, P, T);
+    const int64_t bytes = lsa_shared_prefix_scratch(code, B, Tq, Hq, Hkv, D, P, T, scores_in != nullptr);
     TORCH_CHECK_VALUE(bytes >= 0, what, ": sizes out of range");
     auto stream = at::cuda::getCurrentCUDAStream();
     Workspace& w = workspace(q.device(), stream, bytes, 64);

@@ -77,8 +77,8 @@ def test_c_entries_refuse_before_any_cuda_call():
                dict(strides=[-8] + [1024, 128] + [256, 128] * 2 + [2048, 256, 128] * 2)):
         assert call(**kw) == _lib.ERR_ARG, kw
     assert call(B=0) == _lib.OK and call(Tq=0) == _lib.OK
-    assert L.lsa_shared_prefix_scratch(2, 2, 1, 8, 2, 100, 16, 8) == _lib.ERR_ARG
-    assert L.lsa_shared_prefix_scratch(2, 2, 1, 8, 2, 128, 16, 8) > 0
+    assert L.lsa_shared_prefix_scratch(2, 2, 1, 8, 2, 100, 16, 8, 0) == _lib.ERR_ARG
+    assert L.lsa_shared_prefix_scratch(2, 2, 1, 8, 2, 128, 16, 8, 1) > 0
 
 
 def test_evict_entry_refuses_before_any_cuda_call():
