@@ -1,5 +1,5 @@
 // prefix.cu - attention over a shared prefix and each sequence's own cache: the entry points,
-// the general kernel and the join of the parts (sm_100a). prefix.cuh has the formulas.
+// the fp32 kernel and the join of the parts (sm_100a). prefix.cuh has the formulas.
 #include <math.h>
 
 #include "prefix.cuh"
@@ -11,22 +11,22 @@ constexpr int kSimtRows = 16;  // rows of a work item
 constexpr int kSimtKeys = 32;  // keys of a tile: one per lane
 constexpr int kSimtWarps = 8;
 
-template <typename T, int D>
-__device__ __forceinline__ void stage_rows(float* dst, int ld, const T* src, int64_t stride, int rows, int live) {
+template <int D>
+__device__ __forceinline__ void stage_rows(float* dst, int ld, const float* src, int64_t stride, int rows, int live) {
     for (int i = threadIdx.x; i < rows * (D / 8); i += blockDim.x) {
         const int r = i / (D / 8), c = i % (D / 8);
         float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (r < live) load8<T>(src + r * stride + c * 8, x);
+        if (r < live) load8<float>(src + r * stride + c * 8, x);
 #pragma unroll
         for (int e = 0; e < 8; ++e) dst[r * ld + c * 8 + e] = x[e];
     }
 }
 
-// One work item: up to 16 rows of a KV head x a range of keys, on the FMA pipes in fp32. A
+// fp32 inputs. One work item: up to 16 rows of a KV head x a range of keys, on the FMA pipes. A
 // warp holds two rows; a lane scores one key of a 32-key tile for both, the warp's running
 // maximum and sum follow the tile, and a lane then owns D / 32 output columns. Rows past a
 // sequence's length are staged as zeros, so what an unwritten slot holds is never used.
-template <typename T, int D>
+template <int D>
 __global__ void __launch_bounds__(kSimtWarps * 32) prefix_simt_kernel(const PrefixArgs a, int prefix_items, int ptiles,
                                                                       int otiles) {
     constexpr int LDK = D + 4, E = D / 32;
@@ -58,15 +58,15 @@ __global__ void __launch_bounds__(kSimtWarps * 32) prefix_simt_kernel(const Pref
         float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
         if (r < nrows) {
             const int64_t tok = (int64_t)b * a.Tq + r / a.G;
-            load8<T>(static_cast<const T*>(a.q) + tok / a.Tq * a.q_b + tok % a.Tq * a.q_t +
+            load8<float>(static_cast<const float*>(a.q) + tok / a.Tq * a.q_b + tok % a.Tq * a.q_t +
                          (h * (int64_t)a.G + r % a.G) * a.q_h + c * 8,
                      x);
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) sq[(i / (D / 8)) * D + c * 8 + e] = x[e];
     }
-    const T* kb = static_cast<const T*>(own ? a.k : a.kp) + (own ? b * a.k_b + h * a.k_h : h * a.kp_h);
-    const T* vb = static_cast<const T*>(own ? a.v : a.vp) + (own ? b * a.v_b + h * a.v_h : h * a.vp_h);
+    const float* kb = static_cast<const float*>(own ? a.k : a.kp) + (own ? b * a.k_b + h * a.k_h : h * a.kp_h);
+    const float* vb = static_cast<const float*>(own ? a.v : a.vp) + (own ? b * a.v_b + h * a.v_h : h * a.vp_h);
     const int64_t kt = own ? a.k_t : a.kp_t, vt = own ? a.v_t : a.vp_t;
     // the two rows of this warp: the first key that each does not see
     int limit[2];
@@ -79,8 +79,8 @@ __global__ void __launch_bounds__(kSimtWarps * 32) prefix_simt_kernel(const Pref
     for (int t0 = k0; t0 < k1; t0 += kSimtKeys) {
         __syncthreads();
         const int live = k1 - t0 < kSimtKeys ? k1 - t0 : kSimtKeys;
-        stage_rows<T, D>(sk, LDK, kb + (int64_t)t0 * kt, kt, kSimtKeys, live);
-        stage_rows<T, D>(sv, D, vb + (int64_t)t0 * vt, vt, kSimtKeys, live);
+        stage_rows<D>(sk, LDK, kb + (int64_t)t0 * kt, kt, kSimtKeys, live);
+        stage_rows<D>(sv, D, vb + (int64_t)t0 * vt, vt, kSimtKeys, live);
         __syncthreads();
         float s[2] = {0, 0};
         const float4* k4 = reinterpret_cast<const float4*>(sk + lane * LDK);
@@ -171,22 +171,25 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixArgs a, i
     }
 }
 
-template <typename T>
-int simt_d(const PrefixArgs& a, int D, cudaStream_t stream) {
+}  // namespace
+
+int launch_prefix_simt(const PrefixArgs& a, int D, cudaStream_t stream) {
     const int64_t ptiles = ((int64_t)a.B * a.Tq * a.G + kSimtRows - 1) / kSimtRows;
     const int64_t otiles = ((int64_t)a.Tq * a.G + kSimtRows - 1) / kSimtRows;
     const int64_t pi = a.Sp * ptiles * a.Hkv, oi = (int64_t)a.So * otiles * a.Hkv * a.B;
     if (pi + oi == 0) return LSA_OK;
     if (pi + oi > INT32_MAX) return LSA_ERR_SIZE;
     if (D == 128)
-        prefix_simt_kernel<T, 128><<<(unsigned)(pi + oi), kSimtWarps * 32, 0, stream>>>(a, (int)pi, (int)ptiles,
+        prefix_simt_kernel<128><<<(unsigned)(pi + oi), kSimtWarps * 32, 0, stream>>>(a, (int)pi, (int)ptiles,
                                                                                         (int)otiles);
     else
-        prefix_simt_kernel<T, 64><<<(unsigned)(pi + oi), kSimtWarps * 32, 0, stream>>>(a, (int)pi, (int)ptiles,
+        prefix_simt_kernel<64><<<(unsigned)(pi + oi), kSimtWarps * 32, 0, stream>>>(a, (int)pi, (int)ptiles,
                                                                                        (int)otiles);
     LSA_LAUNCH_CHECK();
     return LSA_OK;
 }
+
+namespace {
 
 template <typename T>
 int merge_d(const PrefixArgs& a, int D, cudaStream_t stream) {
@@ -286,12 +289,6 @@ int64_t round256(int64_t x) { return (x + 255) / 256 * 256; }
 
 }  // namespace
 
-int launch_prefix_simt(const PrefixArgs& a, int dtype, int D, cudaStream_t stream) {
-    if (dtype == kF32) return simt_d<float>(a, D, stream);
-    if (dtype == kF16) return simt_d<__half>(a, D, stream);
-    return simt_d<__nv_bfloat16>(a, D, stream);
-}
-
 int launch_prefix_merge(const PrefixArgs& a, int dtype, int D, cudaStream_t stream) {
     if (dtype == kF32) return merge_d<float>(a, D, stream);
     if (dtype == kF16) return merge_d<__half>(a, D, stream);
@@ -364,13 +361,14 @@ int lsa_shared_prefix_attention(const void* q, const void* k_prefix, const void*
     a.lse2 = reinterpret_cast<float*>(s);
     RowsPlan rows = p.rows;
     if (p.logits) rows.logits = reinterpret_cast<float*>(s + round256(a.rows * 4));
-    int rc = p.simt ? launch_prefix_simt(a, dtype, (int)D, stream) : LSA_OK;
+    int rc = p.simt ? launch_prefix_simt(a, (int)D, stream) : LSA_OK;
     if (rc == LSA_OK && !p.simt) rc = launch_prefix_tiles(a, p.tile, dtype, (int)D, stream);
     if (rc == LSA_OK && !p.simt) rc = launch_prefix_rows(a, rows, dtype, (int)D, stream);
     if (rc == LSA_OK && !p.tile.direct) rc = launch_prefix_merge(a, dtype, (int)D, stream);
     if (rc == LSA_OK && scores && T > 0)
         rc = p.logits ? launch_logit_weights(a, rows.logits, scores, scores_out, stream)
-                      : launch_own_weights(a, dtype, (int)D, scores, scores_out, stream);
+             : p.simt ? launch_own_weights(a, (int)D, scores, scores_out, stream)
+                      : launch_tile_weights(a, dtype, (int)D, scores, scores_out, stream);
     return rc;
 }
 

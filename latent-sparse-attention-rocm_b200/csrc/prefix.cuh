@@ -75,12 +75,13 @@ struct RowsPlan {
     float* logits;  // [B, Hkv, Tq * G, T] log2-domain logits of the own keys, or null
 };
 
-int launch_prefix_simt(const PrefixArgs& a, int dtype, int D, cudaStream_t stream);
+int launch_prefix_simt(const PrefixArgs& a, int D, cudaStream_t stream);  // fp32 inputs
 int launch_prefix_tiles(const PrefixArgs& a, const TilePlan& tp, int dtype, int D, cudaStream_t stream);
 int launch_prefix_rows(const PrefixArgs& a, const RowsPlan& rp, int dtype, int D, cudaStream_t stream);
 int launch_prefix_merge(const PrefixArgs& a, int dtype, int D, cudaStream_t stream);
-int launch_own_weights(const PrefixArgs& a, int dtype, int D, const float* scores, float* scores_out,
-                       cudaStream_t stream);
+int launch_own_weights(const PrefixArgs& a, int D, const float* scores, float* scores_out, cudaStream_t stream);
+int launch_tile_weights(const PrefixArgs& a, int dtype, int D, const float* scores, float* scores_out,
+                        cudaStream_t stream);
 int launch_logit_weights(const PrefixArgs& a, const float* logits, const float* scores, float* scores_out,
                          cudaStream_t stream);
 

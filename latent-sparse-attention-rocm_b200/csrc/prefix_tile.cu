@@ -27,18 +27,12 @@
 // Every wait is bounded (1 s); an expired wait raises a CTA-wide flag, every role leaves, copies
 // and MMAs in flight are waited for (bounded), the TMEM is released and LSA_ERR_TIMEOUT lands in
 // the status word.
-#include <cuda.h>
-
-#include "prefix.cuh"
-#include "umma.cuh"
+#include "prefix_umma.cuh"
 
 namespace lsa {
 namespace {
 
 constexpr int kThreads = 384;
-constexpr int kChunk = 128;
-constexpr uint64_t kWaitNs = 1000000000ull;
-
 struct TileMaps {
     CUtensorMap kp, vp, k, v;
 };
@@ -53,63 +47,6 @@ template <int D> struct TileShape {
     static constexpr int kSmem = kOffMisc + 16 + 1024;  // slack: the base is aligned to 1024 B
     static_assert(kSmem <= 232448, "shared memory of a CTA");
 };
-
-__device__ __forceinline__ bool role_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-    bool done = mbar_try_wait(bar, parity);
-    if (__all_sync(0xFFFFFFFFu, done)) return true;
-    const uint64_t t0 = global_ns();
-    for (;;) {
-        if (!done) done = mbar_try_wait(bar, parity);
-        if (__all_sync(0xFFFFFFFFu, done)) return true;
-        int stop = 0;
-        if ((threadIdx.x & 31) == 0) stop = (*abort_flag != 0) || (global_ns() - t0 > kWaitNs);
-        if (__shfl_sync(0xFFFFFFFFu, stop, 0)) {
-            if ((threadIdx.x & 31) == 0) *abort_flag = 1;
-            return false;
-        }
-    }
-}
-
-__device__ __forceinline__ void tma_tile(uint32_t dst, const CUtensorMap* map, int x, int t, int h, int b,
-                                         uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, "
-        "%5}], [%6];" ::"r"(dst),
-        "l"(map), "r"(x), "r"(t), "r"(h), "r"(b), "r"(smem_u32(bar))
-        : "memory");
-}
-
-__device__ __forceinline__ uint32_t pack16(float a, float b, __nv_bfloat16*) {
-    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<uint32_t*>(&h);
-}
-__device__ __forceinline__ uint32_t pack16(float a, float b, __half*) {
-    __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<uint32_t*>(&h);
-}
-__device__ __forceinline__ uint64_t pair(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
 
 // What a CTA works on.
 struct Item {
@@ -516,35 +453,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (threadIdx.x == 0 && *abort_flag) atomicExch(a.status, LSA_ERR_TIMEOUT);
 }
 
-using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeFn encode_fn() {
-    static EncodeFn fn = [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult found;
-        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) !=
-                cudaSuccess ||
-            found != cudaDriverEntryPointSuccess)
-            p = nullptr;
-        return reinterpret_cast<EncodeFn>(p);
-    }();
-    return fn;
-}
-
-// [B, T, H, D] rows as 64-element x 128-key boxes, 128-byte swizzle; zeros past the extents.
-bool encode_rows(CUtensorMap* map, bool bf16, const void* base, int64_t D, int64_t T, int64_t H, int64_t B,
-                 int64_t st, int64_t sh, int64_t sb) {
-    const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)T, (cuuint64_t)H, (cuuint64_t)B};
-    const cuuint64_t strides[3] = {(cuuint64_t)st * 2, (cuuint64_t)sh * 2, (cuuint64_t)sb * 2};
-    const cuuint32_t box[4] = {64, kChunk, 1, 1}, es[4] = {1, 1, 1, 1};
-    return encode_fn()(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-                       const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <typename T, int D>
 int launch(const TileMaps& maps, const PrefixArgs& a, const TilePlan& tp, unsigned grid, cudaStream_t stream) {
     auto kern = prefix_tile_kernel<T, D>;
@@ -566,11 +474,11 @@ int launch_prefix_tiles(const PrefixArgs& a, const TilePlan& tp, int dtype, int 
     const bool bf = dtype == kBF16;
     bool ok = true;
     if (a.P > 0 && (tp.batch_items || tp.joint))
-        ok = encode_rows(&maps.kp, bf, a.kp, D, a.P, a.Hkv, 1, a.kp_t, a.kp_h, (int64_t)D) &&
-             encode_rows(&maps.vp, bf, a.vp, D, a.P, a.Hkv, 1, a.vp_t, a.vp_h, (int64_t)D);
+        ok = encode_keys(&maps.kp, bf, a.kp, D, a.P, a.Hkv, 1, a.kp_t, a.kp_h, (int64_t)D) &&
+             encode_keys(&maps.vp, bf, a.vp, D, a.P, a.Hkv, 1, a.vp_t, a.vp_h, (int64_t)D);
     if (ok && a.T > 0 && tp.seq_items)
-        ok = encode_rows(&maps.k, bf, a.k, D, a.T, a.Hkv, a.B, a.k_t, a.k_h, a.k_b) &&
-             encode_rows(&maps.v, bf, a.v, D, a.T, a.Hkv, a.B, a.v_t, a.v_h, a.v_b);
+        ok = encode_keys(&maps.k, bf, a.k, D, a.T, a.Hkv, a.B, a.k_t, a.k_h, a.k_b) &&
+             encode_keys(&maps.v, bf, a.v, D, a.T, a.Hkv, a.B, a.v_t, a.v_h, a.v_b);
     if (!ok) return LSA_ERR_ARG;
     const unsigned grid = (unsigned)items;
     if (dtype == kBF16)

@@ -12,7 +12,8 @@ namespace {
 constexpr int kWKeys = 128;  // keys of a CTA: one per thread
 constexpr int kWRows = 8;    // query rows staged at a time
 
-template <typename T, int D>
+// fp32 inputs: the scores computed again on the FMA pipes, eight rows at a time.
+template <int D>
 __global__ void __launch_bounds__(kWKeys) own_weights_kernel(const PrefixArgs a, const float* __restrict__ scores,
                                                              float* __restrict__ scores_out) {
     constexpr int LDK = D + 4;
@@ -27,11 +28,11 @@ __global__ void __launch_bounds__(kWKeys) own_weights_kernel(const PrefixArgs a,
         if (j < a.T) scores_out[at] = scores[at];
         return;
     }
-    const T* kb = static_cast<const T*>(a.k) + b * a.k_b + h * a.k_h;
+    const float* kb = static_cast<const float*>(a.k) + b * a.k_b + h * a.k_h;
     for (int i = tid; i < kWKeys * (D / 8); i += kWKeys) {
         const int r = i / (D / 8), c = i % (D / 8);
         float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (j0 + r < len) load8<T>(kb + (int64_t)(j0 + r) * a.k_t + c * 8, x);
+        if (j0 + r < len) load8<float>(kb + (int64_t)(j0 + r) * a.k_t + c * 8, x);
 #pragma unroll
         for (int e = 0; e < 8; ++e) sk[r * LDK + c * 8 + e] = x[e];
     }
@@ -44,7 +45,7 @@ __global__ void __launch_bounds__(kWKeys) own_weights_kernel(const PrefixArgs a,
             const int r = r0 + i / (D / 8), c = i % (D / 8);
             float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
             if (r < nrows)
-                load8<T>(static_cast<const T*>(a.q) + b * a.q_b + r / a.G * a.q_t + (h * (int64_t)a.G + r % a.G) * a.q_h +
+                load8<float>(static_cast<const float*>(a.q) + b * a.q_b + r / a.G * a.q_t + (h * (int64_t)a.G + r % a.G) * a.q_h +
                              c * 8,
                          x);
 #pragma unroll
@@ -97,10 +98,10 @@ __global__ void __launch_bounds__(256) logit_weights_kernel(const PrefixArgs a, 
     scores_out[bh * a.T + j] = scores[bh * a.T + j] + w;
 }
 
-template <typename T, int D>
+template <int D>
 int weights_launch(const PrefixArgs& a, const float* scores, float* scores_out, cudaStream_t stream) {
     const int smem = (kWKeys * (D + 4) + kWRows * D) * 4;
-    auto kern = own_weights_kernel<T, D>;
+    auto kern = own_weights_kernel<D>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
         return LSA_ERR_CUDA;
     if (a.B > 65535 || a.Hkv > 65535) return LSA_ERR_SIZE;
@@ -108,12 +109,6 @@ int weights_launch(const PrefixArgs& a, const float* scores, float* scores_out, 
     kern<<<grid, kWKeys, smem, stream>>>(a, scores, scores_out);
     LSA_LAUNCH_CHECK();
     return LSA_OK;
-}
-
-template <typename T>
-int weights_d(const PrefixArgs& a, int D, const float* scores, float* scores_out, cudaStream_t stream) {
-    return D == 128 ? weights_launch<T, 128>(a, scores, scores_out, stream)
-                    : weights_launch<T, 64>(a, scores, scores_out, stream);
 }
 
 }  // namespace
@@ -127,11 +122,9 @@ int launch_logit_weights(const PrefixArgs& a, const float* logits, const float* 
     return LSA_OK;
 }
 
-int launch_own_weights(const PrefixArgs& a, int dtype, int D, const float* scores, float* scores_out,
-                       cudaStream_t stream) {
-    if (dtype == kF32) return weights_d<float>(a, D, scores, scores_out, stream);
-    if (dtype == kF16) return weights_d<__half>(a, D, scores, scores_out, stream);
-    return weights_d<__nv_bfloat16>(a, D, scores, scores_out, stream);
+int launch_own_weights(const PrefixArgs& a, int D, const float* scores, float* scores_out, cudaStream_t stream) {
+    return D == 128 ? weights_launch<128>(a, scores, scores_out, stream)
+                    : weights_launch<64>(a, scores, scores_out, stream);
 }
 
 }  // namespace lsa
