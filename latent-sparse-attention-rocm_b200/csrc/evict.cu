@@ -11,14 +11,17 @@
 namespace lsa {
 namespace {
 
-constexpr int kSelThreads = 1024;
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kBins = 2048;     // 11 bits a pass: 3 passes over 32-bit keys
+constexpr int kCached = 16384;  // keys held in a CTA's shared memory (more are read again)
 
 struct EvictArgs {
     const void *k, *v;
     int64_t k_b, k_t, k_h, v_b, v_t, v_h;  // strides in bytes
     const float* scores;                   // [B, Hkv, T]
     const int32_t* lengths;                // [B]
-    int B, T, Hkv, row_bytes;
+    int B, T, Hkv, row_bytes, row_lanes;
     int budget, window, sink, capacity;
     void *k_out, *v_out;                   // [B, capacity, Hkv, D] contiguous
     float* scores_out;                     // [B, Hkv, capacity]
@@ -28,94 +31,227 @@ struct EvictArgs {
 
 __device__ __forceinline__ uint32_t score_key(float f) { return (uint32_t)ordered_bits(f) ^ 0x80000000u; }
 
-// One CTA per (sequence, KV head): the key of the last score that stays by a radix search
-// (8 bits a pass, highest first), then an ordered compaction.
-__global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictArgs a) {
-    __shared__ int hist[256], scan_sm[40], s_digit, s_need;
-    const int h = blockIdx.x % a.Hkv, b = blockIdx.x / a.Hkv, tid = threadIdx.x;
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// the address, in the cluster's shared memory, of `p` in CTA `rank`
+__device__ __forceinline__ uint32_t at_rank(const void* p, uint32_t rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ int4 ld_cluster4(uint32_t addr) {
+    int4 v;
+    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+
+__device__ __forceinline__ void add_cluster(uint32_t addr, int v) {
+    if (v) asm volatile("red.relaxed.cluster.shared::cluster.add.s32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
+// Every row (sequence, KV head) is served by `ranks` CTAs.
+//  1. The last score that stays: a radix search over the competing keys, 11 bits a pass from the
+//     top; it ends early when all keys of a bin stay.
+//  2. Output slots from kept counts, by warp ballots, in index order: ids and scores.
+//  3. The kept rows of K and V are copied, every CTA an equal share of the output slots whoever
+//     selected them (heavy keys crowd together: the sinks, the window).
+// kSliced false: every CTA of a row selects over all its keys by itself, without a word to the
+// others - the selection is latency, not work, while its keys fit one CTA's shared memory. true: the
+// CTAs are a cluster, hold a slice of the keys each, and join their histograms (DSMEM adds into the
+// bins' owner, one cluster barrier a pass) and their kept counts.
+// Selection is a chain of short steps, the copy is bandwidth: with several CTAs an SM one row's
+// copy covers another's chain.
+template <bool kSliced>
+__global__ void __launch_bounds__(kThreads) evict_kernel(const EvictArgs a, int ranks_arg) {
+    __shared__ __align__(16) int hist[kBins];
+    __shared__ __align__(16) int joined[kSliced ? 3 * kBins / 2 : 4];  // this rank's bins, one set a pass
+    __shared__ int scan[kWarps], wkeep[kWarps], wtie[kWarps];
+    __shared__ __align__(16) int4 found;   // digit, keys still needed, keys of the digit
+    __shared__ __align__(16) int4 counts;  // keys of the slice that stay for sure, and on the level
+    extern __shared__ uint32_t keys[];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int ranks = ranks_arg, rank = blockIdx.x % ranks;  // the cluster rank, when sliced
+    const int row = blockIdx.x / ranks, h = row % a.Hkv, b = row / a.Hkv;
     int n = a.lengths[b];
     n = n < 0 ? 0 : (n > a.T ? a.T : n);
     const int kept = n < a.budget ? n : a.budget;
     const float* sc = a.scores + ((int64_t)b * a.Hkv + h) * a.T;
     int32_t* ids = a.ids + ((int64_t)b * a.Hkv + h) * a.capacity;
     float* so = a.scores_out + ((int64_t)b * a.Hkv + h) * a.capacity;
-    if (h == 0 && tid == 0) a.lengths_out[b] = kept;
-    const int lo = a.sink, hi = n - a.window;  // the keys that compete, when n > budget
-    uint32_t cut = 0;
-    int level = 0;  // keys equal to the cut that stay
+    if (h == 0 && rank == 0 && tid == 0) a.lengths_out[b] = kept;
+    // the output's slots, an equal share a CTA
+    const int m0 = (int)((int64_t)a.capacity * rank / ranks), m1 = (int)((int64_t)a.capacity * (rank + 1) / ranks);
+
     if (n > a.budget) {
+        const int s0 = kSliced ? (int)((int64_t)n * rank / ranks) : 0;
+        const int s1 = kSliced ? (int)((int64_t)n * (rank + 1) / ranks) : n;
+        const int lo = a.sink, hi = n - a.window;  // the keys that compete
+        const int cached = s1 - s0 < kCached ? s1 - s0 : kCached;
+        auto key_at = [&](int j) { return j - s0 < kCached ? keys[j - s0] : score_key(sc[j]); };
         int need = a.budget - a.sink - a.window;
+        // a key stays when its top bits are above `cut`; on the level, the first `level` by index
+        uint32_t cut = 0;
+        int shift = 0, level = 0;
+#pragma unroll 4
+        for (int j = tid; j < cached; j += kThreads) keys[j] = score_key(sc[s0 + j]);
+        if (kSliced) {
+            for (int i = tid; i < 3 * kBins / 2; i += kThreads) joined[i] = 0;
+            cluster_sync();
+        }
         if (need == 0) {
-            cut = 0xFFFFFFFFu;  // nothing is above it, and none of the level stays
+            cut = 0xFFFFFFFFu;
+            __syncthreads();
         } else {
-            for (int shift = 24; shift >= 0; shift -= 8) {
-                for (int i = tid; i < 256; i += kSelThreads) hist[i] = 0;
+            shift = 32;
+#pragma unroll
+            for (int pass = 0; pass < 3; ++pass) {
+                const int width = pass == 2 ? 10 : 11, up = shift;
+                shift -= width;
+                *reinterpret_cast<int4*>(hist + 4 * tid) = make_int4(0, 0, 0, 0);
                 __syncthreads();
-                for (int j = lo + tid; j < hi; j += kSelThreads) {
-                    const uint32_t u = score_key(sc[j]);
-                    if (shift == 24 || (u >> (shift + 8)) == (cut >> (shift + 8))) atomicAdd(&hist[(u >> shift) & 255], 1);
+                for (int j = (s0 > lo ? s0 : lo) + tid; j < s1 && j < hi; j += kThreads) {
+                    const uint32_t u = key_at(j);
+                    if (pass == 0 || (u >> up) == cut) atomicAdd(&hist[(u >> shift) & ((1u << width) - 1)], 1);
                 }
                 __syncthreads();
-                if (tid == 0) {
-                    int d = 255, above = 0;
-                    while (above + hist[d] < need) above += hist[d--];
-                    s_digit = d;
-                    s_need = need - above;
+                // bins in descending order, four a thread
+                const int at = kBins - 4 - 4 * tid;
+                int4 c = *reinterpret_cast<const int4*>(hist + at);
+                if (kSliced) {
+                    // bins [owner * per, ..) join at rank `owner`; per = 2048 / ranks, ranks >= 2
+                    const int per = kBins / ranks, owner = at / per, slot = pass * (kBins / 2) + at % per;
+                    const uint32_t to = at_rank(joined + slot, owner);
+                    add_cluster(to, c.x), add_cluster(to + 4, c.y), add_cluster(to + 8, c.z), add_cluster(to + 12, c.w);
+                    cluster_sync();
+                    c = ld_cluster4(to);
+                }
+                const int sum = c.x + c.y + c.z + c.w;
+                int above = sum;
+#pragma unroll
+                for (int off = 1; off < 32; off <<= 1) {
+                    const int y = __shfl_up_sync(0xFFFFFFFFu, above, off);
+                    if (lane >= off) above += y;
+                }
+                if (lane == 31) scan[warp] = above;
+                __syncthreads();
+                above -= sum;  // keys in higher bins than this thread's
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) above += w < warp ? scan[w] : 0;
+                if (above < need && above + sum >= need) {
+                    int d = 3, in = c.w;
+                    if (above + in < need) above += in, d = 2, in = c.z;
+                    if (above + in < need) above += in, d = 1, in = c.y;
+                    if (above + in < need) above += in, d = 0, in = c.x;
+                    found = make_int4(at + d, need - above, in, 0);
                 }
                 __syncthreads();
-                cut |= (uint32_t)s_digit << shift;
-                need = s_need;
-            }
-            level = need;
-        }
-    }
-    int out = 0, taken = 0;  // kept keys and level keys before this chunk
-    for (int j0 = 0; j0 < n; j0 += kSelThreads) {
-        const int j = j0 + tid;
-        bool stay = false, tie = false;
-        if (j < n) {
-            if (n <= a.budget || j < lo || j >= hi) {
-                stay = true;
-            } else {
-                const uint32_t u = score_key(sc[j]);
-                stay = u > cut;
-                tie = u == cut;
+                cut = pass == 0 ? (uint32_t)found.x : (cut << width) | (uint32_t)found.x;
+                level = need = found.y;
+                if (found.y == found.z) break;  // the whole bin stays
             }
         }
-        int total;
-        const int ties_before = taken + block_exclusive_scan(tie, scan_sm, &total);
-        taken += total;
-        if (tie && ties_before < level) stay = true;
-        const int at = out + block_exclusive_scan(stay, scan_sm, &total);
-        out += total;
-        if (stay) {
-            ids[at] = j;
-            so[at] = sc[j];
+        // keys that stay for sure and keys on the level, by warp segments of whole ballots
+        const int seg = ((s1 - s0 + 31) / 32 + kWarps - 1) / kWarps * 32;
+        const int w0 = s0 + warp * seg < s1 ? s0 + warp * seg : s1, w1 = w0 + seg < s1 ? w0 + seg : s1;
+        auto classify = [&](int j, bool* keep, bool* tie) {
+            *keep = *tie = false;
+            if (j < w1) {
+                const uint32_t u = key_at(j) >> shift;
+                const bool forced = j < lo || j >= hi;
+                *keep = forced || u > cut;
+                *tie = !forced && u == cut;
+            }
+        };
+        int nk = 0, nt = 0;
+#pragma unroll 4
+        for (int j0 = w0; j0 < w1; j0 += 32) {
+            bool keep, tie;
+            classify(j0 + lane, &keep, &tie);
+            nk += keep, nt += tie;
+        }
+        nk = __reduce_add_sync(0xFFFFFFFFu, nk), nt = __reduce_add_sync(0xFFFFFFFFu, nt);
+        if (lane == 0) wkeep[warp] = nk, wtie[warp] = nt;
+        __syncthreads();
+        int keep_before = 0, tie_before = 0;
+        if (kSliced) {
+            if (warp == 0) {
+                const int x = __reduce_add_sync(0xFFFFFFFFu, lane < kWarps ? wkeep[lane] : 0);
+                const int y = __reduce_add_sync(0xFFFFFFFFu, lane < kWarps ? wtie[lane] : 0);
+                if (lane == 0) counts = make_int4(x, y, 0, 0);
+            }
+            cluster_sync();
+            int4 x = make_int4(0, 0, 0, 0);
+            if (lane < rank) x = ld_cluster4(at_rank(&counts, lane));
+            keep_before = __reduce_add_sync(0xFFFFFFFFu, x.x), tie_before = __reduce_add_sync(0xFFFFFFFFu, x.y);
+        }
+        keep_before += __reduce_add_sync(0xFFFFFFFFu, lane < warp && lane < kWarps ? wkeep[lane] : 0);
+        tie_before += __reduce_add_sync(0xFFFFFFFFu, lane < warp && lane < kWarps ? wtie[lane] : 0);
+        for (int j0 = w0; j0 < w1; j0 += 32) {
+            const int j = j0 + lane;
+            bool keep, tie;
+            classify(j, &keep, &tie);
+            const uint32_t below = (1u << lane) - 1, km = __ballot_sync(0xFFFFFFFFu, keep),
+                           tm = __ballot_sync(0xFFFFFFFFu, tie);
+            const int ties = tie_before + __popc(tm & below);
+            const int slot = keep_before + __popc(km & below) + (ties < level ? ties : level);
+            // a CTA that selects alone writes its own share
+            if ((keep || (tie && ties < level)) && (kSliced || (slot >= m0 && slot < m1))) {
+                ids[slot] = j;
+                so[slot] = sc[j];
+            }
+            keep_before += __popc(km);
+            tie_before += __popc(tm);
+        }
+    } else {
+        for (int m = m0 + tid; m < m1 && m < kept; m += kThreads) {
+            ids[m] = m;
+            so[m] = sc[m];
         }
     }
-    for (int m = kept + tid; m < a.capacity; m += kSelThreads) {
+    for (int m = (m0 > kept ? m0 : kept) + tid; m < m1; m += kThreads) {
         ids[m] = -1;
         so[m] = 0.0f;
     }
-}
-
-// Rows of K and V by the kept ids, 16 bytes a thread; zeros past the kept count.
-__global__ void __launch_bounds__(256) evict_gather_kernel(const EvictArgs a) {
-    const int chunks = a.row_bytes / 16;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int c = (int)(i % chunks);
-    const int64_t m = i / chunks;
-    if (m >= a.capacity) return;
-    const int h = blockIdx.y, b = blockIdx.z;
-    const int id = a.ids[((int64_t)b * a.Hkv + h) * a.capacity + m];
-    uint4 x = make_uint4(0, 0, 0, 0), y = x;
-    if (id >= 0) {
-        x = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.k) + b * a.k_b + id * a.k_t + h * a.k_h + c * 16);
-        y = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.v) + b * a.v_b + id * a.v_t + h * a.v_h + c * 16);
+    if (kSliced)
+        cluster_sync();  // the ids of every CTA; and no CTA leaves while its counts are read
+    else
+        __syncthreads();
+    // a row of 16-byte chunks to the next power of two of lanes (at most a warp), four rows a
+    // thread in flight
+    const int chunks = a.row_bytes >> 4, lanes = a.row_lanes;
+    const int sub = tid / lanes, step = kThreads / lanes;
+    const uint8_t* kb = static_cast<const uint8_t*>(a.k) + b * a.k_b + h * a.k_h;
+    const uint8_t* vb = static_cast<const uint8_t*>(a.v) + b * a.v_b + h * a.v_h;
+    const int64_t out_t = (int64_t)a.Hkv * a.row_bytes;
+    uint8_t* ko = static_cast<uint8_t*>(a.k_out) + ((int64_t)b * a.capacity * a.Hkv + h) * a.row_bytes;
+    uint8_t* vo = static_cast<uint8_t*>(a.v_out) + ((int64_t)b * a.capacity * a.Hkv + h) * a.row_bytes;
+    for (int c = tid % lanes; c < chunks; c += lanes) {
+        for (int m = m0 + sub; m < m1; m += 4 * step) {
+            uint4 x[4], y[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int mu = m + u * step;
+                const int id = mu < m1 ? ids[mu] : -1;
+                x[u] = y[u] = make_uint4(0, 0, 0, 0);
+                if (id >= 0) {
+                    x[u] = __ldg(reinterpret_cast<const uint4*>(kb + id * a.k_t) + c);
+                    y[u] = __ldg(reinterpret_cast<const uint4*>(vb + id * a.v_t) + c);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int mu = m + u * step;
+                if (mu < m1) {
+                    reinterpret_cast<uint4*>(ko + mu * out_t)[c] = x[u];
+                    reinterpret_cast<uint4*>(vo + mu * out_t)[c] = y[u];
+                }
+            }
+        }
     }
-    const int64_t to = (((int64_t)b * a.capacity + m) * a.Hkv + h) * a.row_bytes + c * 16;
-    *reinterpret_cast<uint4*>(static_cast<uint8_t*>(a.k_out) + to) = x;
-    *reinterpret_cast<uint4*>(static_cast<uint8_t*>(a.v_out) + to) = y;
 }
 
 }  // namespace
@@ -142,7 +278,7 @@ int lsa_evict(const void* k, const void* v, int64_t row_bytes, const int64_t* st
         return LSA_ERR_ARG;
     for (const void* p : {k, v, (const void*)k_out, (const void*)v_out})
         if ((uintptr_t)p & 15) return LSA_ERR_ARG;
-    if (B > 65535 || Hkv > 65535 || B * Hkv > INT32_MAX) return LSA_ERR_SIZE;
+    if (B > INT32_MAX / 16 / Hkv) return LSA_ERR_SIZE;  // one cluster of at most 16 CTAs a row
     EvictArgs a;
     a.k = k, a.v = v;
     a.k_b = strides[0], a.k_t = strides[1], a.k_h = strides[2];
@@ -152,14 +288,33 @@ int lsa_evict(const void* k, const void* v, int64_t row_bytes, const int64_t* st
     a.budget = (int)(budget < INT32_MAX ? budget : INT32_MAX), a.window = (int)window, a.sink = (int)sink;
     a.capacity = (int)capacity;
     a.k_out = k_out, a.v_out = v_out, a.scores_out = scores_out, a.lengths_out = lengths_out, a.ids = ids;
-    evict_select_kernel<<<(unsigned)(B * Hkv), kSelThreads, 0, stream>>>(a);
-    LSA_LAUNCH_CHECK();
-    if (capacity > 0) {
-        const int64_t work = capacity * (row_bytes / 16);
-        dim3 grid((unsigned)((work + 255) / 256), (unsigned)Hkv, (unsigned)B);
-        evict_gather_kernel<<<grid, 256, 0, stream>>>(a);
-        LSA_LAUNCH_CHECK();
-    }
+    a.row_lanes = row_bytes / 16 >= 32 ? 32 : next_pow2((int)(row_bytes / 16));
+    // A row's CTAs: enough that all rows' copies fill the GPU, none with fewer than 64 slots to copy.
+    // Keys that fit one CTA are selected by each of them, more in slices by a cluster.
+    const int64_t units = B * Hkv;
+    const bool sliced = T > kCached;
+    int64_t ranks = 1;
+    while (ranks < 16 && (units * ranks < 4 * 148 && capacity / (2 * ranks) >= 64)) ranks *= 2;
+    if (sliced)
+        while (ranks < 16 && (ranks < 2 || T / ranks > kCached / 2)) ranks *= 2;
+    const int64_t slice = sliced ? (T + ranks - 1) / ranks : T;
+    const int smem = (int)((slice < kCached ? slice : kCached) * 4);
+    auto kern = sliced ? evict_kernel<true> : evict_kernel<false>;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kCached * 4) != cudaSuccess ||
+        cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+        return LSA_ERR_CUDA;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = sliced ? (unsigned)ranks : 1;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(units * ranks));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, kern, a, (int)ranks) != cudaSuccess) return LSA_ERR_CUDA;
     return LSA_OK;
 }
 

@@ -136,28 +136,62 @@ __global__ void __launch_bounds__(kSimtWarps * 32) prefix_simt_kernel(const Pref
     }
 }
 
-// The parts of a row joined, one warp per row: every lane holds D / 32 columns. Parts without
-// a key (lse -inf) have weight zero and their sums are not read.
+// The parts of a row joined, one warp per row: every lane holds D / 32 columns. The lse of up to
+// 128 parts are loaded at once, then the parts' columns eight loads at a time; a part without a
+// key (lse -inf) has weight zero and its columns, never written, are not read (the heaviest part's
+// are, in their place: finite, times zero).
 template <typename T, int D>
 __global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixArgs a, int parts) {
-    constexpr int E = D / 32;
+    constexpr int E = D / 32, kPer = 4 * kMaxSplits / 32;
     const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (row >= a.rows) return;
-    float top = -INFINITY;
-    for (int c = lane; c < parts; c += 32) top = fmaxf(top, a.part_lse[(int64_t)c * a.rows + row]);
+    float x[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+        x[i] = lane + 32 * i < parts ? a.part_lse[(int64_t)(lane + 32 * i) * a.rows + row] : -INFINITY;
+    float top = x[0];
+#pragma unroll
+    for (int i = 1; i < kPer; ++i) top = fmaxf(top, x[i]);
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
     float acc[E] = {}, total = 0.0f;
     if (top != -INFINITY) {
-        for (int c = 0; c < parts; ++c) {
-            const float x = a.part_lse[(int64_t)c * a.rows + row];
-            if (x == -INFINITY) continue;
-            const float w = exp2f(x - top);
-            total += w;
-            const float* src = a.part_o + ((int64_t)c * a.rows + row) * D + lane * E;
+        int best = 0;
 #pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] = fmaf(w, src[e], acc[e]);
+        for (int i = kPer - 1; i >= 0; --i) {
+            const uint32_t at = __ballot_sync(0xFFFFFFFFu, x[i] == top);
+            if (at) best = 32 * i + __ffs(at) - 1;
+        }
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            if (32 * i >= parts) break;
+            const float w = exp2f(x[i] - top);
+            const int n = parts - 32 * i < 32 ? parts - 32 * i : 32;
+            for (int c0 = 0; c0 < n; c0 += 8) {
+                float v[8][E], f[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    f[u] = __shfl_sync(0xFFFFFFFFu, w, c0 + u);  // past the parts: exp2(-inf) = 0
+                    const int c = f[u] > 0.0f ? 32 * i + c0 + u : best;
+                    const float* src = a.part_o + ((int64_t)c * a.rows + row) * D + lane * E;
+                    if constexpr (E == 4) {
+                        const float4 y = __ldcs(reinterpret_cast<const float4*>(src));
+                        v[u][0] = y.x, v[u][1] = y.y, v[u][2] = y.z, v[u][3] = y.w;
+                    } else {
+                        const float2 y = __ldcs(reinterpret_cast<const float2*>(src));
+                        v[u][0] = y.x, v[u][1] = y.y;
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    total += f[u];
+#pragma unroll
+                    for (int e = 0; e < E; ++e) acc[e] = fmaf(f[u], v[u][e], acc[e]);
+                }
+            }
         }
     }
     const float inv = total > 0.0f ? 1.0f / total : 0.0f;
@@ -165,9 +199,9 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixArgs a, i
 #pragma unroll
     for (int e = 0; e < E; ++e) dst[e] = from_f32<T>(acc[e] * inv);
     if (lane == 0) {
-        const float x = total > 0.0f ? top + log2f(total) : -INFINITY;
-        a.lse2[row] = x;
-        if (a.lse) a.lse[row] = x * 0.69314718055994531f;
+        const float y = total > 0.0f ? top + log2f(total) : -INFINITY;
+        a.lse2[row] = y;
+        if (a.lse) a.lse[row] = y * 0.69314718055994531f;
     }
 }
 
@@ -194,12 +228,8 @@ namespace {
 template <typename T>
 int merge_d(const PrefixArgs& a, int D, cudaStream_t stream) {
     const unsigned grid = (unsigned)((a.rows + 7) / 8);
-    if (D == 128)
-        prefix_merge_kernel<T, 128><<<grid, 256, 0, stream>>>(a, a.parts_p + a.parts_o);
-    else
-        prefix_merge_kernel<T, 64><<<grid, 256, 0, stream>>>(a, a.parts_p + a.parts_o);
-    LSA_LAUNCH_CHECK();
-    return LSA_OK;
+    auto kern = D == 128 ? prefix_merge_kernel<T, 128> : prefix_merge_kernel<T, 64>;
+    return launch_after(kern, dim3(grid), 256, 0, stream, a, a.parts_p + a.parts_o);
 }
 
 struct Plan {

@@ -49,6 +49,23 @@ struct TilePlan {
     bool direct;                   // a row has one part: the kernel writes the output
 };
 
+// Launch that may start while the kernel before it drains (programmatic dependent launch): the
+// kernel waits (griddepcontrol.wait) before it touches what an earlier kernel writes.
+template <typename K, typename... A>
+int launch_after(K kern, dim3 grid, unsigned threads, size_t smem, cudaStream_t stream, const A&... args) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess ? LSA_OK : LSA_ERR_CUDA;
+}
+
 // own keys that sequence b holds
 __device__ __forceinline__ int own_length(const PrefixArgs& a, int b) {
     const int n = a.lengths[b];
