@@ -18,8 +18,8 @@
 // values); everything else is fp32.
 //
 // Warps: 0 loads K and V tiles by TMA (cp.async.bulk.tensor, one ring of 128-key tiles in the
-// order the MMAs use them), 1 issues every MMA (unrolled, one thread: 64 cycles per 128 x 128 x 16
-// MMA, the pipe's rate), 4-7 / 8-11 are the softmax of half 0 / 1. TMEM: S_0/P_0 [0, 128),
+// order the MMAs use them), one thread of warp 1 issues every MMA (unrolled: 64 cycles per 128 x 128 x
+// 16 MMA, the pipe's rate), 2 zeroes a sequence's V tail, 4-7 / 8-11 are the softmax of half 0 / 1. TMEM: S_0/P_0 [0, 128),
 // S_1/P_1 [128, 256), O_0 [256, 256 + D), O_1 [384, 384 + D).
 // Rows of V at or past a sequence's length are zeroed in shared memory before their product, so
 // whatever an unwritten slot holds (0 x NaN) stays out.
@@ -42,7 +42,7 @@ template <int D> struct TileShape {
     static constexpr int kStages = D == 128 ? 5 : 10;
     static constexpr int kOffStage = 2 * kTileBytes;
     static constexpr int kOffBar = kOffStage + kStages * kTileBytes;
-    static constexpr int kNumBars = 2 * kStages + 1 + 2 + 4 + 2 + 1;
+    static constexpr int kNumBars = 2 * kStages + 1 + 2 + 4 + 2 + 1 + 2;
     static constexpr int kOffMisc = kOffBar + kNumBars * 8;
     static constexpr int kSmem = kOffMisc + 16 + 1024;  // slack: the base is aligned to 1024 B
     static_assert(kSmem <= 232448, "shared memory of a CTA");
@@ -247,12 +247,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t sbase = smem_u32(sm);
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Sh::kOffBar);
     uint64_t *full = bars, *empty = bars + NS, *bar_q = bars + 2 * NS, *bar_s = bar_q + 1, *bar_p = bar_s + 2,
-             *bar_o = bar_p + 4, *bar_drain = bar_o + 2;
+             *bar_o = bar_p + 4, *bar_drain = bar_o + 2, *bar_tail = bar_drain + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + Sh::kOffMisc);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + Sh::kOffMisc + 4);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const Item w = item_of(a, tp);
     const int n = w.c1 - w.c0;
+    // the item's last chunk reaches past the sequence's keys
+    const bool tail = n > 0 && w.c1 > w.np && (w.c1 - w.np) * kChunk > w.len;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < NS; ++s) {
@@ -267,6 +269,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&bar_o[i], 1);
         }
         mbar_init(bar_drain, 1);
+        mbar_init(bar_tail, 1);
+        mbar_init(bar_tail + 1, 32);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -328,120 +332,120 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int p = pos > NS ? pos - NS : 0; p < pos; ++p) mbar_wait_bounded(&full[p % NS], (p / NS) & 1);
             }
         } else if (warp == 1) {
-            // ------------------------------------------------ every MMA of the CTA
+            // ------------------------------------------------ every MMA of the CTA, from one thread
             constexpr uint32_t idS = umma_idesc_f16<T>(128, 128, false);
             constexpr uint32_t idO = umma_idesc_f16<T>(128, D, true);
-            int pos = 0;
-            auto stage = [&](int p) { return sbase + Sh::kOffStage + (p % NS) * Sh::kTileBytes; };
-            auto ready = [&](int p) { return role_wait(&full[p % NS], (p / NS) & 1, abort_flag); };
-            auto scores = [&](int hf, int p, bool last_use) {
-                if (lane == 0) {
-                    const uint32_t qa = sbase + (w.streams ? 0 : hf * Sh::kTileBytes), ka = stage(p);
+            if (elect_one()) {
+                const uint64_t qd0 = sw128_desc(sbase, 16, 1024);
+                const uint64_t kd0 = sw128_desc(sbase + Sh::kOffStage, 16, 1024);
+                const uint64_t vd0 = sw128_desc(sbase + Sh::kOffStage, 16384, 1024);
+                const uint32_t q1 = w.streams ? 0 : Sh::kTileBytes;
+                int stage = 0, phase = 0;  // of the next tile of the ring
+                auto advance = [&]() {
+                    if (++stage == NS) stage = 0, phase ^= 1;
+                };
+                auto scores = [&](int hf, int st) {
+                    const uint64_t qd = desc_at(qd0, hf ? q1 : 0), kd = desc_at(kd0, st * Sh::kTileBytes);
 #pragma unroll
                     for (int kk = 0; kk < KS; ++kk) {
                         const uint32_t off = (kk >> 2) * 16384 + (kk & 3) * 32;
-                        umma_f16_ss(tmem + hf * 128, sw128_desc(qa + off, 16, 1024), sw128_desc(ka + off, 16, 1024),
-                                    idS, kk > 0);
+                        umma_f16_ss(tmem + hf * 128, desc_at(qd, off), desc_at(kd, off), idS, kk > 0);
                     }
                     umma_commit(&bar_s[hf]);
-                    if (last_use) umma_commit(&empty[p % NS]);
-                }
-                __syncwarp();
-            };
-            auto product = [&](int hf, int p, bool fresh, int half) {
-                if (lane == 0) {
-                    const uint32_t va = stage(p);
+                };
+                // P_h's first and last 64 keys as they come; O_h starts afresh on a half's first chunk
+                auto product = [&](int hf, int st, bool fresh, uint32_t parity) -> bool {
+                    const uint64_t vd = desc_at(vd0, st * Sh::kTileBytes);
+                    const uint32_t o = tmem + 256 + hf * 128, p = tmem + hf * 128;
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk) {
-                        const int k8 = half * 4 + kk;
-                        umma_f16_ts(tmem + 256 + hf * 128, tmem + hf * 128 + k8 * 8,
-                                    sw128_desc(va + k8 * 2048, 16384, 1024), idO, !fresh || k8 > 0);
+                    for (int half = 0; half < 2; ++half) {
+                        if (!thread_wait(&bar_p[2 * hf + half], parity, abort_flag)) return false;
+                        tc_fence_after();
+#pragma unroll
+                        for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
+                            umma_f16_ts(o, p + kk * 8, desc_at(vd, kk * 2048), idO, kk > 0 || !fresh);
+                    }
+                    return true;
+                };
+                // the V tile at the front of the ring; its rows past the sequence's keys zeroed
+                auto value = [&](bool last) -> bool {
+                    if (!thread_wait(&full[stage], phase, abort_flag)) return false;
+                    if (last && tail) {
+                        mbar_arrive(bar_tail);
+                        if (!thread_wait(bar_tail + 1, 0, abort_flag)) return false;
+                    }
+                    return true;
+                };
+                auto key = [&]() -> bool {
+                    const bool ok = thread_wait(&full[stage], phase, abort_flag);
+                    tc_fence_after();
+                    return ok;
+                };
+                bool ok = n == 0 || thread_wait(bar_q, 0, abort_flag);
+                if (ok && n > 0 && !w.streams) {
+                    ok = key();
+                    if (ok) {
+                        scores(0, stage), scores(1, stage);
+                        umma_commit(&empty[stage]);
+                        advance();
+                    }
+                    for (int j = 0; ok && j < n; ++j) {
+                        const bool more = j + 1 < n;
+                        const int sv = stage;
+                        if (!(ok = value(!more))) break;
+                        advance();
+                        if (!(ok = product(0, sv, j == 0, j & 1))) break;
+                        if (more) {
+                            if (!(ok = key())) break;
+                            scores(0, stage);
+                        }
+                        if (!(ok = product(1, sv, j == 0, j & 1))) break;
+                        umma_commit(&empty[sv]);
+                        if (more) {
+                            scores(1, stage);
+                            umma_commit(&empty[stage]);
+                            advance();
+                        }
+                    }
+                } else if (ok && n > 0) {
+                    for (int c = 0; ok && c < n && c < 2; ++c) {
+                        ok = key();
+                        if (ok) {
+                            scores(c, stage);
+                            umma_commit(&empty[stage]);
+                            advance();
+                        }
+                    }
+                    for (int c = 0; ok && c < n; ++c) {
+                        const int hf = c & 1;
+                        if (!(ok = value(c + 1 == n))) break;
+                        if (!(ok = product(hf, stage, c < 2, (c >> 1) & 1))) break;
+                        umma_commit(&empty[stage]);
+                        advance();
+                        if (c + 2 < n) {
+                            if (!(ok = key())) break;
+                            scores(hf, stage);
+                            umma_commit(&empty[stage]);
+                            advance();
+                        }
                     }
                 }
-                __syncwarp();
-            };
-            auto free_stage = [&](int p) {
-                if (lane == 0) umma_commit(&empty[p % NS]);
-                __syncwarp();
-            };
-            // rows of V past the sequence's keys: zeros, whatever the slots hold
-            auto clean = [&](int p, int c) {
-                if (c < w.np) return;
-                const int valid = w.len - (c - w.np) * kChunk;
-                if (valid >= kChunk) return;
-                uint8_t* va = sm + Sh::kOffStage + (p % NS) * Sh::kTileBytes;
-                for (int i = (valid < 0 ? 0 : valid) * 8 + lane; i < kChunk * 8; i += 32)
+                if (ok) umma_commit(&bar_o[0]), umma_commit(&bar_o[1]);
+                umma_commit(bar_drain);  // every MMA completes before the TMEM is released
+                mbar_wait_bounded(bar_drain, 0);
+            }
+            __syncwarp();
+        } else if (warp == 2 && tail) {
+            // ------------------------------------------------ the tail of a sequence's last V tile
+            if (role_wait(bar_tail, 0, abort_flag)) {
+                uint8_t* va = sm + Sh::kOffStage + ((2 * n - 1) % NS) * Sh::kTileBytes;  // the last load
+                for (int i = (w.len - (w.c1 - 1 - w.np) * kChunk) * 8 + lane; i < kChunk * 8; i += 32)
 #pragma unroll
                     for (int x = 0; x < D / 64; ++x)
                         *reinterpret_cast<uint4*>(va + x * 16384 + i * 16) = make_uint4(0, 0, 0, 0);
                 fence_proxy_async_smem();
-                __syncwarp();
-            };
-            bool ok = n == 0 || role_wait(bar_q, 0, abort_flag);
-            if (!w.streams) {
-                if (ok && n > 0) {
-                    ok = ready(0);
-                    tc_fence_after();
-                    if (ok) scores(0, 0, false), scores(1, 0, true);
-                    pos = 1;
-                }
-                for (int j = 0; ok && j < n; ++j) {
-                    const int pv = pos, pk = pos + 1;
-                    const bool more = j + 1 < n;
-                    for (int hf = 0; ok && hf < 2; ++hf) {
-                        if (hf == 0) {
-                            ok = ready(pv);
-                            if (ok) clean(pv, w.c0 + j);
-                        }
-                        for (int half = 0; ok && half < 2; ++half) {
-                            ok = role_wait(&bar_p[2 * hf + half], j & 1, abort_flag);
-                            tc_fence_after();
-                            if (ok) product(hf, pv, j == 0, half);
-                        }
-                        if (ok && hf == 1) free_stage(pv);
-                        if (ok && more) {
-                            if (hf == 0) {
-                                ok = ready(pk);
-                                tc_fence_after();
-                            }
-                            if (ok) scores(hf, pk, hf == 1);
-                        }
-                    }
-                    pos += more ? 2 : 1;
-                }
-            } else {
-                for (int c = 0; ok && c < n && c < 2; ++c) {
-                    ok = ready(pos);
-                    tc_fence_after();
-                    if (ok) scores(c, pos, true);
-                    ++pos;
-                }
-                for (int c = 0; ok && c < n; ++c) {
-                    const int hf = c & 1;
-                    ok = ready(pos);
-                    if (ok) clean(pos, w.c0 + c);
-                    for (int half = 0; ok && half < 2; ++half) {
-                        ok = role_wait(&bar_p[2 * hf + half], (c >> 1) & 1, abort_flag);
-                        tc_fence_after();
-                        if (ok) product(hf, pos, c < 2, half);
-                    }
-                    if (ok) free_stage(pos);
-                    ++pos;
-                    if (ok && c + 2 < n) {
-                        ok = ready(pos);
-                        tc_fence_after();
-                        if (ok) scores(hf, pos, true);
-                        ++pos;
-                    }
-                }
+                mbar_arrive(bar_tail + 1);
             }
-            if (lane == 0) {
-                if (ok) umma_commit(&bar_o[0]), umma_commit(&bar_o[1]);
-                umma_commit(bar_drain);  // every MMA completes before the TMEM is released
-            }
-            __syncwarp();
-            mbar_wait_bounded(bar_drain, 0);
-            __syncwarp();
         }
     }
     tc_fence_before();

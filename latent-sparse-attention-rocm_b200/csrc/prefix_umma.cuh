@@ -29,6 +29,36 @@ __device__ __forceinline__ bool role_wait(uint64_t* bar, uint32_t parity, volati
     }
 }
 
+// The same for a role that is one thread.
+__device__ __forceinline__ bool thread_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = global_ns();
+    for (;;) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*abort_flag != 0 || global_ns() - t0 > kRoleWaitNs) {
+            *abort_flag = 1;
+            return false;
+        }
+    }
+}
+
+// One lane of a converged warp. An MMA-issuing thread chosen this way issues a 128 x 128 x 16 MMA
+// every 64 cycles, the pipe's rate, with barrier waits between them; chosen by lane == 0 it took
+// 83-95 (measured on B200: the compiler knows the elected branch to be one thread).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred P;\n\t"
+        "elect.sync _|P, 0xFFFFFFFF;\n\t"
+        "selp.u32 %0, 1, 0, P;\n\t}"
+        : "=r"(p));
+    return p != 0;
+}
+
+// A 128-byte-swizzled operand's descriptor is base + (byte offset >> 4) in its low word: the
+// start address stays within its 14 bits everywhere in shared memory.
+__device__ __forceinline__ uint64_t desc_at(uint64_t base, uint32_t byte_offset) { return base + (byte_offset >> 4); }
+
 __device__ __forceinline__ void tma_tile(uint32_t dst, const CUtensorMap* map, int x, int c1, int c2, int c3,
                                          uint64_t* bar) {
     asm volatile(

@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(kThreads, 1)
              *sfull = qempty + kQStages, *sfree = sfull + 4, *drain = sfree + 4;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + Sh::kOffMisc);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + Sh::kOffMisc + 4);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
     int i = blockIdx.x;
     const int split = i % wp.splits;
@@ -132,39 +132,37 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == 1) {
         // ---------------------------------------------------- MMAs
         constexpr uint32_t idS = umma_idesc_f16<T>(128, 128, false);
-        int kpos = 0, qpos = 0, it = 0;
-        bool ok = true;
-        for (int p = p0; ok && p < p1; ++p, kpos += 2) {
-            for (int t = 0; ok && t < nr; ++t, ++it) {
-                const int q = resident ? t : qpos;
-                ok = role_wait(&qfull[q % kQStages], resident ? 0 : (q / kQStages) & 1, abort_flag);
-                for (int g = 0; ok && g < 2; ++g) {
-                    const int ks = (kpos + g) % kKStages, buf = 2 * g + (it & 1);
-                    if (t == 0) ok = role_wait(&kfull[ks], ((kpos + g) / kKStages) & 1, abort_flag);
-                    if (ok && it >= 2) ok = role_wait(&sfree[buf], (it / 2 - 1) & 1, abort_flag);
-                    if (!ok) break;
-                    tc_fence_after();
-                    if (lane == 0) {
-                        const uint32_t ka = sbase + ks * Sh::kTileBytes;
-                        const uint32_t qa = sbase + Sh::kOffQ + (q % kQStages) * Sh::kTileBytes;
+        if (elect_one()) {
+            const uint64_t kd0 = sw128_desc(sbase, 16, 1024), qd0 = sw128_desc(sbase + Sh::kOffQ, 16, 1024);
+            int kpos = 0, qpos = 0, it = 0;
+            bool ok = true;
+            for (int p = p0; ok && p < p1; ++p, kpos += 2) {
+                for (int t = 0; ok && t < nr; ++t, ++it) {
+                    const int q = resident ? t : qpos;
+                    ok = thread_wait(&qfull[q % kQStages], resident ? 0 : (q / kQStages) & 1, abort_flag);
+                    for (int g = 0; ok && g < 2; ++g) {
+                        const int ks = (kpos + g) % kKStages, buf = 2 * g + (it & 1);
+                        if (t == 0) ok = thread_wait(&kfull[ks], ((kpos + g) / kKStages) & 1, abort_flag);
+                        if (ok && it >= 2) ok = thread_wait(&sfree[buf], (it / 2 - 1) & 1, abort_flag);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint64_t kd = desc_at(kd0, ks * Sh::kTileBytes);
+                        const uint64_t qd = desc_at(qd0, (q % kQStages) * Sh::kTileBytes);
 #pragma unroll
                         for (int kk = 0; kk < D / 16; ++kk) {
                             const uint32_t off = (kk >> 2) * 16384 + (kk & 3) * 32;
-                            umma_f16_ss(tmem + buf * 128, sw128_desc(ka + off, 16, 1024),
-                                        sw128_desc(qa + off, 16, 1024), idS, kk > 0);
+                            umma_f16_ss(tmem + buf * 128, desc_at(kd, off), desc_at(qd, off), idS, kk > 0);
                         }
                         umma_commit(&sfull[buf]);
                         if (t == nr - 1) umma_commit(&kempty[ks]);
                         if (g == 1 && !resident) umma_commit(&qempty[q % kQStages]);
                     }
-                    __syncwarp();
+                    ++qpos;
                 }
-                ++qpos;
             }
+            umma_commit(drain);  // every MMA completes before the TMEM is released
+            mbar_wait_bounded(drain, 0);
         }
-        if (lane == 0) umma_commit(drain);  // every MMA completes before the TMEM is released
-        __syncwarp();
-        mbar_wait_bounded(drain, 0);
         __syncwarp();
     } else if (warp >= 4) {
         // ---------------------------------------------------- weights: group g, tile 2p + g
