@@ -141,10 +141,16 @@ __global__ void __launch_bounds__(kSimtWarps * 32) prefix_simt_kernel(const Pref
 // key (lse -inf) has weight zero and its columns, never written, are not read (the heaviest part's
 // are, in their place: finite, times zero).
 template <typename T, int D>
-__global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixArgs a, int parts) {
+__global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixArgs a, const TilePlan tp, int parts) {
     constexpr int E = D / 32, kPer = 4 * kMaxSplits / 32;
-    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
+    if (tp.whole) {  // the rows of the split seq tiles, 256 a tile
+        int b, h, tile;
+        seq_tile(a, tp, tp.whole + (int)(row >> 8), &b, &h, &tile);
+        const int r = tile * 256 + (int)(row & 255), tok = r / a.G;
+        row = tok < a.Tq ? row_index(a, (int64_t)b * a.Tq + tok, h, r - tok * a.G) : a.rows;
+    }
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (row >= a.rows) return;
@@ -226,15 +232,16 @@ int launch_prefix_simt(const PrefixArgs& a, int D, cudaStream_t stream) {
 namespace {
 
 template <typename T>
-int merge_d(const PrefixArgs& a, int D, cudaStream_t stream) {
-    const unsigned grid = (unsigned)((a.rows + 7) / 8);
+int merge_d(const PrefixArgs& a, const TilePlan& tp, int D, cudaStream_t stream) {
+    const int64_t rows = tp.whole ? ((int64_t)a.B * a.Hkv * tp.seq_tiles - tp.whole) * 256 : a.rows;
     auto kern = D == 128 ? prefix_merge_kernel<T, 128> : prefix_merge_kernel<T, 64>;
-    return launch_after(kern, dim3(grid), 256, 0, stream, a, a.parts_p + a.parts_o);
+    return launch_after(kern, dim3((unsigned)((rows + 7) / 8)), 256, 0, stream, a, tp, a.parts_p + a.parts_o);
 }
 
 struct Plan {
     int Sp, So, parts_p, parts_o;
     bool simt, logits;  // fp32 inputs; the own keys' logits are kept for their weights
+    bool merge;         // some row has parts to join
     TilePlan tile;
     RowsPlan rows;
 };
@@ -257,6 +264,7 @@ int balance(int64_t items, int64_t chunks, int64_t fixed, int64_t slots) {
 
 Plan make_plan(int dtype, int64_t B, int64_t Tq, int64_t Hkv, int64_t G, int64_t P, int64_t T, bool scored) {
     Plan p = {};
+    p.merge = true;
     p.simt = dtype == kF32;
     if (p.simt) {
         // splits enough that the work items of each segment fill the GPU about four times
@@ -279,10 +287,15 @@ Plan make_plan(int dtype, int64_t B, int64_t Tq, int64_t Hkv, int64_t G, int64_t
     const int64_t seq = B * Hkv * t.seq_tiles;
     t.joint = P > 0 && rows * 4 >= (int64_t)t.seq_tiles * 256 * 3;
     if (t.joint) {
-        p.So = balance(seq, pc + oc, 3, kSMs);
-        p.parts_o = p.So;
-        t.seq_items = (int)(seq * p.So);
-        t.direct = p.So == 1;
+        // whole rounds of one tile an SM are not split (no parts to write, read and join); the tiles
+        // of the last, short round are, so that it too fills the GPU
+        t.whole = (int)(seq / kSMs * kSMs);
+        const int64_t rest = seq - t.whole;
+        p.So = rest ? balance(rest, pc + oc, 3, kSMs) : 1;
+        if (p.So == 1) t.whole = (int)seq;
+        p.merge = p.So > 1;
+        p.parts_o = p.merge ? p.So : 0;
+        t.seq_items = (int)(t.whole + (seq - t.whole) * p.So);
         return p;
     }
     if (B * rows <= kFewRows) {
@@ -319,10 +332,10 @@ int64_t round256(int64_t x) { return (x + 255) / 256 * 256; }
 
 }  // namespace
 
-int launch_prefix_merge(const PrefixArgs& a, int dtype, int D, cudaStream_t stream) {
-    if (dtype == kF32) return merge_d<float>(a, D, stream);
-    if (dtype == kF16) return merge_d<__half>(a, D, stream);
-    return merge_d<__nv_bfloat16>(a, D, stream);
+int launch_prefix_merge(const PrefixArgs& a, const TilePlan& tp, int dtype, int D, cudaStream_t stream) {
+    if (dtype == kF32) return merge_d<float>(a, tp, D, stream);
+    if (dtype == kF16) return merge_d<__half>(a, tp, D, stream);
+    return merge_d<__nv_bfloat16>(a, tp, D, stream);
 }
 
 }  // namespace lsa
@@ -394,7 +407,7 @@ int lsa_shared_prefix_attention(const void* q, const void* k_prefix, const void*
     int rc = p.simt ? launch_prefix_simt(a, (int)D, stream) : LSA_OK;
     if (rc == LSA_OK && !p.simt) rc = launch_prefix_tiles(a, p.tile, dtype, (int)D, stream);
     if (rc == LSA_OK && !p.simt) rc = launch_prefix_rows(a, rows, dtype, (int)D, stream);
-    if (rc == LSA_OK && !p.tile.direct) rc = launch_prefix_merge(a, dtype, (int)D, stream);
+    if (rc == LSA_OK && p.merge) rc = launch_prefix_merge(a, p.tile, dtype, (int)D, stream);
     if (rc == LSA_OK && scores && T > 0)
         rc = p.logits ? launch_logit_weights(a, rows.logits, scores, scores_out, stream)
              : p.simt ? launch_own_weights(a, (int)D, scores, scores_out, stream)

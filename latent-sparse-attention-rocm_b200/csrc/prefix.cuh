@@ -43,11 +43,18 @@ struct PrefixArgs {
 // The work of the tensor-core kernel (prefix_tile.cu).
 struct TilePlan {
     int batch_items, batch_tiles;  // row tiles over all sequences: prefix keys
-    int seq_items, seq_tiles;      // row tiles of a sequence: its own keys
+    int seq_items, seq_tiles;      // row tiles of a sequence: its own keys (items; tiles of a sequence)
     bool batch_streams, seq_streams;  // tiles of at most 128 rows: two streams of chunks
     bool joint;                    // seq tiles read the prefix too
-    bool direct;                   // a row has one part: the kernel writes the output
+    int whole;                     // the first seq tiles, not split: they write the output themselves
 };
+
+// Seq tile i: (sequence, KV head, row tile), the longest causal ranges first.
+__device__ __forceinline__ void seq_tile(const PrefixArgs& a, const TilePlan& t, int i, int* b, int* h, int* tile) {
+    *h = i % a.Hkv, i /= a.Hkv;
+    *b = i % a.B;
+    *tile = t.seq_tiles - 1 - i / a.B;
+}
 
 // Launch that may start while the kernel before it drains (programmatic dependent launch): the
 // kernel waits (griddepcontrol.wait) before it touches what an earlier kernel writes.
@@ -95,7 +102,7 @@ struct RowsPlan {
 int launch_prefix_simt(const PrefixArgs& a, int D, cudaStream_t stream);  // fp32 inputs
 int launch_prefix_tiles(const PrefixArgs& a, const TilePlan& tp, int dtype, int D, cudaStream_t stream);
 int launch_prefix_rows(const PrefixArgs& a, const RowsPlan& rp, int dtype, int D, cudaStream_t stream);
-int launch_prefix_merge(const PrefixArgs& a, int dtype, int D, cudaStream_t stream);
+int launch_prefix_merge(const PrefixArgs& a, const TilePlan& tp, int dtype, int D, cudaStream_t stream);
 int launch_own_weights(const PrefixArgs& a, int D, const float* scores, float* scores_out, cudaStream_t stream);
 int launch_tile_weights(const PrefixArgs& a, int dtype, int D, const float* scores, float* scores_out,
                         cudaStream_t stream);

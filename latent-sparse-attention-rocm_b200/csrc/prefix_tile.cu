@@ -51,6 +51,7 @@ template <int D> struct TileShape {
 // What a CTA works on.
 struct Item {
     bool own, streams;  // seq tile; both halves hold the same rows
+    bool direct;        // all of its rows' keys: it writes the output itself
     int b, h, r0, nrows, part, len;
     int np;      // prefix chunks of the item's chunk list
     int c0, c1;  // its chunks of the list [0, np + own chunks)
@@ -73,13 +74,13 @@ __device__ __forceinline__ Item item_of(const PrefixArgs& a, const TilePlan& t) 
         w.r0 = tile * (w.streams ? 128 : 256);
         w.np = chunks = (a.P + kChunk - 1) / kChunk;
         w.part = 0;
+        w.direct = false;
     } else {
         i -= t.batch_items;
-        S = a.So;
-        split = i % S, i /= S;
-        w.h = i % a.Hkv, i /= a.Hkv;
-        w.b = i % a.B;
-        tile = t.seq_tiles - 1 - i / a.B;  // the longest causal ranges first
+        w.direct = i < t.whole;
+        S = w.direct ? 1 : a.So;
+        split = w.direct ? 0 : (i - t.whole) % S;
+        seq_tile(a, t, w.direct ? i : t.whole + (i - t.whole) / S, &w.b, &w.h, &tile);
         w.len = own_length(a, w.b);
         w.streams = t.seq_streams;
         w.nrows = a.Tq * a.G;
@@ -97,7 +98,7 @@ __device__ __forceinline__ Item item_of(const PrefixArgs& a, const TilePlan& t) 
 }
 
 template <typename T, int D>
-__device__ __forceinline__ void softmax_half(const PrefixArgs& a, const TilePlan& tp, const Item& w, uint64_t* bars,
+__device__ __forceinline__ void softmax_half(const PrefixArgs& a, const Item& w, uint64_t* bars, uint8_t* stage,
                                              volatile int* abort_flag, uint32_t tmem) {
     using Sh = TileShape<D>;
     uint64_t *bar_s = bars + 2 * Sh::kStages + 1, *bar_p = bar_s + 2, *bar_o = bar_p + 4;
@@ -117,6 +118,12 @@ __device__ __forceinline__ void softmax_half(const PrefixArgs& a, const TilePlan
     float m = -INFINITY, l = 0.0f;
     const float sl = a.scale_log2, thresh = 8.0f / sl;
     bool ok = true;
+    auto publish = [&](uint64_t* bar) {  // this warp's P so far: one arrival a warp
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
+    };
     for (int j = 0; j < n; ++j) {
         const int c = first + j * step;
         const int seen = c < w.np ? pre_limit - c * kChunk : own_limit - (c - w.np) * kChunk;
@@ -124,46 +131,61 @@ __device__ __forceinline__ void softmax_half(const PrefixArgs& a, const TilePlan
         if (!ok) break;
         tc_fence_after();
         uint32_t s[128];
-        tmem_ld64_wait<0>(tS, s);
-        tmem_ld64_wait<64>(tS + 64, s);
+        tmem_ld128_wait(tS, s);
         if (__any_sync(0xFFFFFFFFu, seen < kChunk)) {
 #pragma unroll
             for (int i = 0; i < 128; ++i)
                 if (i >= seen) s[i] = 0xFF800000u;  // -inf
         }
-        float mx4[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mx4[i] = fmaxf(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
-#pragma unroll
-        for (int i = 8; i < 128; i += 8)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                mx4[e] = max3(mx4[e], __uint_as_float(s[i + 2 * e]), __uint_as_float(s[i + 2 * e + 1]));
-        const float mn = fmaxf(m, max3(mx4[0], mx4[1], fmaxf(mx4[2], mx4[3])));
+        // The exponentials start from the maximum of the chunks before, while this chunk's is
+        // found beside them (a longest path of 64 dependent steps otherwise): fp32 and 16-bit P
+        // carry a factor of up to 2^8 as well as 1. Only when the maximum has grown by more does
+        // the warp take the new one, do the first 96 keys again and rescale O - always on a row's
+        // first chunk.
         float alpha = 1.0f;
-        const bool grow = mn > m + thresh;
-        if (grow) {
-            alpha = ex2_approx((m - mn) * sl);
-            m = mn;
-        }
-        const float neg = m == -INFINITY ? 0.0f : -m * sl;
-        const uint64_t sl2 = pair(sl, sl), neg2 = pair(neg, neg);
-        uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
+        bool grow = false;
+        uint64_t sum[4];
+        const uint64_t sl2 = pair(sl, sl);
+        auto exps = [&](uint32_t& pk, int e, uint64_t neg2) {
+            float x0, x1;
+            unpair(fma2(pair(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), sl2, neg2), x0, x1);
+            const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+            sum[(e >> 1) & 3] = add2(sum[(e >> 1) & 3], pair(p0, p1));
+            pk = pack16(p0, p1, (T*)nullptr);
+        };
+        uint64_t neg2;
+#pragma unroll 1
+        for (bool again = false;; again = true) {
+            const float neg = m == -INFINITY ? 0.0f : -m * sl;
+            neg2 = pair(neg, neg);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            uint32_t pk[32];
+            for (int i = 0; i < 4; ++i) sum[i] = 0ull;
+            uint32_t pk[32], pk2[16];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const int e = 64 * half + 2 * i;
-                float x0, x1;
-                unpair(fma2(pair(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), sl2, neg2), x0, x1);
-                const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
-                sum[i & 3] = add2(sum[i & 3], pair(p0, p1));
-                pk[i] = pack16(p0, p1, (T*)nullptr);
+            for (int i = 0; i < 32; ++i) exps(pk[i], 2 * i, neg2);
+            tmem_st32(tS, pk);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) exps(pk2[i], 64 + 2 * i, neg2);
+            tmem_st16(tS + 32, pk2);
+            if (again) break;
+            float mx4[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx4[i] = fmaxf(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
+#pragma unroll
+            for (int i = 8; i < 128; i += 8)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    mx4[e] = max3(mx4[e], __uint_as_float(s[i + 2 * e]), __uint_as_float(s[i + 2 * e + 1]));
+            const float mx = max3(mx4[0], mx4[1], fmaxf(mx4[2], mx4[3]));
+            grow = mx > m + thresh;
+            if (!__any_sync(0xFFFFFFFFu, grow)) break;
+            if (grow) {
+                alpha = ex2_approx((m - mx) * sl);
+                m = mx;
             }
             // O_h holds the earlier chunks' sum here (their products were issued before S_h(j) by
             // the same thread); its rescale lands before any P of this chunk is published
-            if (half == 0 && j > 0 && __any_sync(0xFFFFFFFFu, grow)) {
+            if (j > 0) {
 #pragma unroll 1
                 for (int cc = 0; cc < D / 32; ++cc) {
                     uint32_t o[32];
@@ -173,11 +195,15 @@ __device__ __forceinline__ void softmax_half(const PrefixArgs& a, const TilePlan
                     tmem_st32(tO + cc * 32, o);
                 }
             }
-            tmem_st32(tS + 32 * half, pk);
-            tmem_wait_st();
-            tc_fence_before();
-            mbar_arrive(&bar_p[2 * hf + half]);
         }
+        publish(&bar_p[2 * hf]);
+        {
+            uint32_t pk2[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) exps(pk2[i], 96 + 2 * i, neg2);
+            tmem_st16(tS + 48, pk2);
+        }
+        publish(&bar_p[2 * hf + 1]);
         float x[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) unpair(sum[i], x[2 * i], x[2 * i + 1]);
@@ -188,53 +214,57 @@ __device__ __forceinline__ void softmax_half(const PrefixArgs& a, const TilePlan
     const int64_t rid = row_index(a, (int64_t)w.b * a.Tq + tok, w.h, r - tok * a.G);
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
     const float lse = l > 0.0f ? m * sl + log2f(l) : -INFINITY;
-    if (tp.direct) {
-        if (live) {
+    const int64_t at = (int64_t)(w.part + (w.streams ? hf : 0)) * a.rows + rid;
+    if (live) {
+        if (w.direct) {
             a.lse2[rid] = lse;
             if (a.lse) a.lse[rid] = lse * 0.69314718055994531f;
+        } else {
+            a.part_lse[at] = lse;
         }
-        T* dst = static_cast<T*>(a.out) + rid * D;
-        if (n > 0) {
-            tc_fence_after();
-#pragma unroll
-            for (int cc = 0; cc < D / 32; ++cc) {
-                uint32_t o[32];
-                tmem_ld32_wait(tO + cc * 32, o);
-                if (live) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t u[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            u[e] = pack16(__uint_as_float(o[8 * i + 2 * e]) * inv,
-                                          __uint_as_float(o[8 * i + 2 * e + 1]) * inv, (T*)nullptr);
-                        *reinterpret_cast<uint4*>(dst + cc * 32 + i * 8) = make_uint4(u[0], u[1], u[2], u[3]);
-                    }
-                }
-            }
-        } else if (live) {
-            for (int i = 0; i < D / 8; ++i) reinterpret_cast<uint4*>(dst)[i] = make_uint4(0, 0, 0, 0);
-        }
+    }
+    if (n == 0) {  // a part without a key is not read
+        if (w.direct && live)
+            for (int i = 0; i < D / 8; ++i)
+                reinterpret_cast<uint4*>(static_cast<T*>(a.out) + rid * D)[i] = make_uint4(0, 0, 0, 0);
         return;
     }
-    const int64_t at = (int64_t)(w.part + (w.streams ? hf : 0)) * a.rows + rid;
-    if (live) a.part_lse[at] = lse;
-    if (n > 0) {  // a part without a key is not read
-        tc_fence_after();
-        float* dst = a.part_o + at * D;
+    // The row through shared memory (the ring: every MMA is done) and out by one bulk copy: a thread
+    // holds a whole row, so its own stores would touch 32 rows an instruction. Rows 16 bytes apart
+    // from a multiple of 128: eight lanes' 16-byte stores fall into different banks.
+    tc_fence_after();
+    constexpr int kPitch = D * 4 + 16;
+    uint8_t* line = stage + ((warp - 4) * 32 + lane) * kPitch;
 #pragma unroll
-        for (int cc = 0; cc < D / 32; ++cc) {
-            uint32_t o[32];
-            tmem_ld32_wait(tO + cc * 32, o);
-            if (live) {
+    for (int cc = 0; cc < D / 32; ++cc) {
+        uint32_t o[32];
+        tmem_ld32_wait(tO + cc * 32, o);
+        if (w.direct) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    *reinterpret_cast<float4*>(dst + cc * 32 + i * 4) =
-                        make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv,
-                                    __uint_as_float(o[4 * i + 2]) * inv, __uint_as_float(o[4 * i + 3]) * inv);
+            for (int i = 0; i < 4; ++i) {
+                uint32_t u[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    u[e] = pack16(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv,
+                                  (T*)nullptr);
+                *reinterpret_cast<uint4*>(line + cc * 64 + i * 16) = make_uint4(u[0], u[1], u[2], u[3]);
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                *reinterpret_cast<float4*>(line + cc * 128 + i * 16) =
+                    make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv,
+                                __uint_as_float(o[4 * i + 2]) * inv, __uint_as_float(o[4 * i + 3]) * inv);
         }
     }
+    fence_proxy_async_smem();
+    if (live) {
+        if (w.direct)
+            bulk_s2g(static_cast<T*>(a.out) + rid * D, smem_u32(line), D * 2);
+        else
+            bulk_s2g(a.part_o + at * D, smem_u32(line), D * 4);
+    }
+    bulk_commit_wait();
 }
 
 template <typename T, int D>
@@ -264,8 +294,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(bar_q, 256);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bar_s[i], 1);
-            mbar_init(&bar_p[2 * i], 128);
-            mbar_init(&bar_p[2 * i + 1], 128);
+            mbar_init(&bar_p[2 * i], 4);
+            mbar_init(&bar_p[2 * i + 1], 4);
             mbar_init(&bar_o[i], 1);
         }
         mbar_init(bar_drain, 1);
@@ -284,22 +314,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         // 384 threads launch at 168 registers: 128 x 56 + 256 x 224 = 384 x 168
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;" ::: "memory");
         // Q rows into the swizzled tiles (rows past the item's are zeros)
-        const int rows = w.streams ? 128 : 256;
-        for (int i = threadIdx.x - 128; i < rows * (D / 8); i += 256) {
-            const int row = i / (D / 8), c = i % (D / 8), r = w.r0 + row, rl = row & 127;
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (r < w.nrows) {
-                const int tok = r / a.G;
-                const int64_t bt = (int64_t)w.b * a.Tq + tok;
-                x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + bt / a.Tq * a.q_b + bt % a.Tq * a.q_t +
-                                                    (w.h * (int64_t)a.G + r - tok * a.G) * a.q_h + c * 8);
-            }
-            const uint32_t off = (row >> 7) * Sh::kTileBytes + (c >> 3) * 16384 + rl * 128 + (((c & 7) ^ (rl & 7)) << 4);
-            *reinterpret_cast<uint4*>(sm + off) = x;
+        constexpr int C = D / 8, kRowsStep = 256 / C;
+        const int c = (threadIdx.x - 128) % C, row0 = (threadIdx.x - 128) / C;
+        const T* qb = static_cast<const T*>(a.q) + w.b * a.q_b + (int64_t)w.h * a.G * a.q_h + c * 8;
+#pragma unroll
+        for (int row = row0; row < 256; row += kRowsStep) {
+            const int r = w.r0 + row, rl = row & 127;
+            const bool in = r < w.nrows && (row < 128 || !w.streams);
+            const unsigned tok = in ? (unsigned)r / (unsigned)a.G : 0u;
+            const unsigned sb = w.own ? 0u : tok / (unsigned)a.Tq;  // batch tiles: tokens of all sequences
+            const T* src = qb + sb * a.q_b + (tok - sb * a.Tq) * a.q_t + (in ? r - (int)tok * a.G : 0) * a.q_h;
+            cp_async16(sbase + (row >> 7) * Sh::kTileBytes + (c >> 3) * 16384 + rl * 128 + (((c & 7) ^ (rl & 7)) << 4),
+                       src, in ? 16u : 0u);
         }
+        cp_async_wait_all();
         fence_proxy_async_smem();
         mbar_arrive(bar_q);
-        softmax_half<T, D>(a, tp, w, bars, abort_flag, tmem);
+        softmax_half<T, D>(a, w, bars, sm + Sh::kOffStage, abort_flag, tmem);
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;" ::: "memory");
         if (warp == 0) {
@@ -353,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     umma_commit(&bar_s[hf]);
                 };
-                // P_h's first and last 64 keys as they come; O_h starts afresh on a half's first chunk
+                // P_h's first 96 and last 32 keys as they come; O_h starts afresh on a half's first chunk
                 auto product = [&](int hf, int st, bool fresh, uint32_t parity) -> bool {
                     const uint64_t vd = desc_at(vd0, st * Sh::kTileBytes);
                     const uint32_t o = tmem + 256 + hf * 128, p = tmem + hf * 128;
@@ -362,7 +393,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (!thread_wait(&bar_p[2 * hf + half], parity, abort_flag)) return false;
                         tc_fence_after();
 #pragma unroll
-                        for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
+                        for (int kk = 6 * half; kk < 6 + 2 * half; ++kk)
                             umma_f16_ts(o, p + kk * 8, desc_at(vd, kk * 2048), idO, kk > 0 || !fresh);
                     }
                     return true;

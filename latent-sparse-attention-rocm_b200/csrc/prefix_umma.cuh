@@ -68,6 +68,16 @@ __device__ __forceinline__ void tma_tile(uint32_t dst, const CUtensorMap* map, i
         : "memory");
 }
 
+// Untiled bulk copy shared -> global (16-byte aligned, whole multiples of 16 bytes), one group a
+// thread: committed and waited for by the thread that issued it.
+__device__ __forceinline__ void bulk_s2g(void* dst, uint32_t src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes)
+                 : "memory");
+}
+__device__ __forceinline__ void bulk_commit_wait() {
+    asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group 0;" ::: "memory");
+}
+
 __device__ __forceinline__ uint32_t pack16(float a, float b, __nv_bfloat16*) {
     __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<uint32_t*>(&h);
@@ -115,6 +125,17 @@ inline EncodeFn encode_fn() {
         return reinterpret_cast<EncodeFn>(p);
     }();
     return fn;
+}
+
+// tcgen05.st 32x32b.x16 (complete after tmem_wait_st).
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16};"
+        :
+        : "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
 }
 
 // A 4-dimensional map of 16-bit elements (D innermost, then the three extents and strides given,
