@@ -10,6 +10,7 @@ namespace {
 constexpr int kSimtRows = 16;  // rows of a work item
 constexpr int kSimtKeys = 32;  // keys of a tile: one per lane
 constexpr int kSimtWarps = 8;
+constexpr int kFewRows = 16;   // rows of a KV head that the few-row kernel takes
 
 template <int D>
 __device__ __forceinline__ void stage_rows(float* dst, int ld, const float* src, int64_t stride, int rows, int live) {
@@ -136,14 +137,82 @@ __global__ void __launch_bounds__(kSimtWarps * 32) prefix_simt_kernel(const Pref
     }
 }
 
+// The lse of a row from its parts, by one warp (log2 domain; every lane has it).
+__device__ __forceinline__ float joined_lse(const PrefixArgs& a, int64_t row, int parts) {
+    const int lane = threadIdx.x & 31;
+    float x[4 * kMaxSplits / 32], top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4 * kMaxSplits / 32; ++i) {
+        x[i] = lane + 32 * i < parts ? a.part_lse[(int64_t)(lane + 32 * i) * a.rows + row] : -INFINITY;
+        top = fmaxf(top, x[i]);
+    }
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
+    if (top == -INFINITY) return top;
+#pragma unroll
+    for (int i = 0; i < 4 * kMaxSplits / 32; ++i) sum += exp2f(x[i] - top);
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, off);
+    return top + log2f(sum);
+}
+
+constexpr int kWeightKeys = 1024;  // keys of a weights block: four a thread
+
+// Own keys' weights from the logits that the few-row kernel kept (at most 16 rows a KV head: 4
+// bytes a row and key against the 256 bytes of K that scoring the key again would read):
+//   w_j = sum over the rows r that see j of 2^(s_rj - lse_r).
+// One thread owns a key, so the sum has one order and one writer. The block joins its rows' lse
+// itself, beside the blocks that join the output: one launch for both.
+__device__ __forceinline__ void own_weights(const PrefixArgs& a, int parts, const float* __restrict__ logits,
+                                            const float* __restrict__ scores, float* __restrict__ scores_out) {
+    __shared__ float slse[kFewRows];
+    const int per = (int)(((int64_t)a.T + kWeightKeys - 1) / kWeightKeys);
+    const int64_t bh = blockIdx.x / per;
+    const int b = (int)(bh / a.Hkv), h = (int)(bh % a.Hkv), nrows = a.Tq * a.G, warp = threadIdx.x >> 5;
+    const int len = own_length(a, b), j0 = (blockIdx.x % per) * kWeightKeys;
+    if (j0 < len) {
+        for (int r = warp; r < nrows; r += 8) {
+            const float x = joined_lse(a, row_index(a, (int64_t)b * a.Tq + r / a.G, h, r % a.G), parts);
+            if ((threadIdx.x & 31) == 0) slse[r] = x;
+        }
+        __syncthreads();
+    }
+    float w[4] = {0, 0, 0, 0};
+    int j[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) j[u] = j0 + u * 256 + threadIdx.x;
+    if (j0 < len)
+        for (int r = 0; r < nrows; ++r) {
+            const float* src = logits + (bh * nrows + r) * a.T;
+            float s[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) s[u] = j[u] < len ? __ldcs(src + j[u]) : -INFINITY;
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (s[u] != -INFINITY) w[u] += exp2f(s[u] - slse[r]);  // -inf: the row does not see the key
+        }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+        if (j[u] < a.T) scores_out[bh * a.T + j[u]] = scores[bh * a.T + j[u]] + w[u];
+}
+
 // The parts of a row joined, one warp per row: every lane holds D / 32 columns. The lse of up to
 // 128 parts are loaded at once, then the parts' columns eight loads at a time; a part without a
 // key (lse -inf) has weight zero and its columns, never written, are not read (the heaviest part's
 // are, in their place: finite, times zero).
 template <typename T, int D>
-__global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixArgs a, const TilePlan tp, int parts) {
+__global__ void __launch_bounds__(256) prefix_finish_kernel(const PrefixArgs a, const TilePlan tp, int parts,
+                                                            unsigned weight_blocks, const float* __restrict__ logits,
+                                                            const float* __restrict__ scores,
+                                                            float* __restrict__ scores_out) {
     constexpr int E = D / 32, kPer = 4 * kMaxSplits / 32;
-    int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    grid_trigger();
+    grid_wait();
+    if (blockIdx.x < weight_blocks) {
+        own_weights(a, parts, logits, scores, scores_out);
+        return;
+    }
+    int64_t row = (int64_t)(blockIdx.x - weight_blocks) * 8 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     if (tp.whole) {  // the rows of the split seq tiles, 256 a tile
         int b, h, tile;
@@ -151,8 +220,6 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixArgs a, c
         const int r = tile * 256 + (int)(row & 255), tok = r / a.G;
         row = tok < a.Tq ? row_index(a, (int64_t)b * a.Tq + tok, h, r - tok * a.G) : a.rows;
     }
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (row >= a.rows) return;
     float x[kPer];
 #pragma unroll
@@ -232,10 +299,15 @@ int launch_prefix_simt(const PrefixArgs& a, int D, cudaStream_t stream) {
 namespace {
 
 template <typename T>
-int merge_d(const PrefixArgs& a, const TilePlan& tp, int D, cudaStream_t stream) {
+int finish_d(const PrefixArgs& a, const TilePlan& tp, int D, const float* logits, const float* scores,
+             float* scores_out, cudaStream_t stream) {
     const int64_t rows = tp.whole ? ((int64_t)a.B * a.Hkv * tp.seq_tiles - tp.whole) * 256 : a.rows;
-    auto kern = D == 128 ? prefix_merge_kernel<T, 128> : prefix_merge_kernel<T, 64>;
-    return launch_after(kern, dim3((unsigned)((rows + 7) / 8)), 256, 0, stream, a, tp, a.parts_p + a.parts_o);
+    const int64_t blocks = (rows + 7) / 8;
+    const int64_t weights = logits ? (int64_t)a.B * a.Hkv * (((int64_t)a.T + kWeightKeys - 1) / kWeightKeys) : 0;
+    if (blocks + weights > INT32_MAX) return LSA_ERR_SIZE;
+    auto kern = D == 128 ? prefix_finish_kernel<T, 128> : prefix_finish_kernel<T, 64>;
+    return launch_after(kern, dim3((unsigned)(blocks + weights)), 256, 0, stream, a, tp, a.parts_p + a.parts_o,
+                        (unsigned)weights, logits, scores, scores_out);
 }
 
 struct Plan {
@@ -247,7 +319,6 @@ struct Plan {
 };
 
 constexpr int kSMs = 148;
-constexpr int kFewRows = 16;  // rows of a KV head that the few-row kernel takes
 
 // Splits of `chunks` for `items` equal work items on `slots` places that hold one item each: the
 // fewest that minimise waves x (chunks of an item + its fixed cost in chunks).
@@ -312,6 +383,7 @@ Plan make_plan(int dtype, int64_t B, int64_t Tq, int64_t Hkv, int64_t G, int64_t
         p.parts_o = p.So = balance(B * Hkv, (T + 63) / 64, 2, 2 * kSMs);
         p.rows.own_items = (int)(B * Hkv * p.So);
         p.logits = scored;
+        p.rows.follows = t.batch_items > 0;
     } else {
         p.So = balance(seq, t.seq_streams ? (oc + 1) / 2 : oc, 3, kSMs);
         p.parts_o = p.So * (t.seq_streams ? 2 : 1);
@@ -332,10 +404,11 @@ int64_t round256(int64_t x) { return (x + 255) / 256 * 256; }
 
 }  // namespace
 
-int launch_prefix_merge(const PrefixArgs& a, const TilePlan& tp, int dtype, int D, cudaStream_t stream) {
-    if (dtype == kF32) return merge_d<float>(a, tp, D, stream);
-    if (dtype == kF16) return merge_d<__half>(a, tp, D, stream);
-    return merge_d<__nv_bfloat16>(a, tp, D, stream);
+int launch_prefix_finish(const PrefixArgs& a, const TilePlan& tp, int dtype, int D, const float* logits,
+                         const float* scores, float* scores_out, cudaStream_t stream) {
+    if (dtype == kF32) return finish_d<float>(a, tp, D, logits, scores, scores_out, stream);
+    if (dtype == kF16) return finish_d<__half>(a, tp, D, logits, scores, scores_out, stream);
+    return finish_d<__nv_bfloat16>(a, tp, D, logits, scores, scores_out, stream);
 }
 
 }  // namespace lsa
@@ -402,16 +475,20 @@ int lsa_shared_prefix_attention(const void* q, const void* k_prefix, const void*
     a.part_lse = reinterpret_cast<float*>(s);
     s += round256((p.parts_p + p.parts_o) * a.rows * 4);
     a.lse2 = reinterpret_cast<float*>(s);
-    RowsPlan rows = p.rows;
-    if (p.logits) rows.logits = reinterpret_cast<float*>(s + round256(a.rows * 4));
-    int rc = p.simt ? launch_prefix_simt(a, (int)D, stream) : LSA_OK;
-    if (rc == LSA_OK && !p.simt) rc = launch_prefix_tiles(a, p.tile, dtype, (int)D, stream);
-    if (rc == LSA_OK && !p.simt) rc = launch_prefix_rows(a, rows, dtype, (int)D, stream);
-    if (rc == LSA_OK && p.merge) rc = launch_prefix_merge(a, p.tile, dtype, (int)D, stream);
-    if (rc == LSA_OK && scores && T > 0)
-        rc = p.logits ? launch_logit_weights(a, rows.logits, scores, scores_out, stream)
-             : p.simt ? launch_own_weights(a, (int)D, scores, scores_out, stream)
-                      : launch_tile_weights(a, dtype, (int)D, scores, scores_out, stream);
+    RowsPlan few = p.rows;
+    if (p.logits) few.logits = reinterpret_cast<float*>(s + round256(a.rows * 4));
+    int rc = LSA_OK;
+    if (p.simt) {
+        rc = launch_prefix_simt(a, (int)D, stream);
+    } else {
+        rc = launch_prefix_tiles(a, p.tile, dtype, (int)D, stream);
+        if (rc == LSA_OK) rc = launch_prefix_rows(a, few, dtype, (int)D, stream);
+    }
+    if (rc == LSA_OK && p.merge)
+        rc = launch_prefix_finish(a, p.tile, dtype, (int)D, T > 0 ? few.logits : nullptr, scores, scores_out, stream);
+    if (rc == LSA_OK && scores && T > 0 && !p.logits)
+        rc = p.simt ? launch_own_weights(a, (int)D, scores, scores_out, stream)
+                    : launch_tile_weights(a, dtype, (int)D, scores, scores_out, stream);
     return rc;
 }
 

@@ -13,6 +13,8 @@
 
 #include <stdint.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace lsa {
@@ -73,6 +75,21 @@ int launch_after(K kern, dim3 grid, unsigned threads, size_t smem, cudaStream_t 
     return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess ? LSA_OK : LSA_ERR_CUDA;
 }
 
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// A kernel's shared-memory limit raised once per device (the call costs about a microsecond).
+template <auto kKernel> bool allow_smem(int bytes) {
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return false;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (done.load() & bit) return true;
+    if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+    done.fetch_or(bit);
+    return true;
+}
+
 // own keys that sequence b holds
 __device__ __forceinline__ int own_length(const PrefixArgs& a, int b) {
     const int n = a.lengths[b];
@@ -96,17 +113,18 @@ __device__ __host__ __forceinline__ void split_range(int n, int s, int S, int un
 // The work of the few-row kernel (prefix_rows.cu): segments of at most 16 rows a KV head.
 struct RowsPlan {
     int prefix_items, own_items;
+    bool follows;   // launched behind this call's tensor-core kernel, whose output it does not read
     float* logits;  // [B, Hkv, Tq * G, T] log2-domain logits of the own keys, or null
 };
 
 int launch_prefix_simt(const PrefixArgs& a, int D, cudaStream_t stream);  // fp32 inputs
 int launch_prefix_tiles(const PrefixArgs& a, const TilePlan& tp, int dtype, int D, cudaStream_t stream);
 int launch_prefix_rows(const PrefixArgs& a, const RowsPlan& rp, int dtype, int D, cudaStream_t stream);
-int launch_prefix_merge(const PrefixArgs& a, const TilePlan& tp, int dtype, int D, cudaStream_t stream);
+// The parts joined; with logits (few-row kernel) also the own keys' weights, in the same launch.
+int launch_prefix_finish(const PrefixArgs& a, const TilePlan& tp, int dtype, int D, const float* logits,
+                         const float* scores, float* scores_out, cudaStream_t stream);
 int launch_own_weights(const PrefixArgs& a, int D, const float* scores, float* scores_out, cudaStream_t stream);
 int launch_tile_weights(const PrefixArgs& a, int dtype, int D, const float* scores, float* scores_out,
                         cudaStream_t stream);
-int launch_logit_weights(const PrefixArgs& a, const float* logits, const float* scores, float* scores_out,
-                         cudaStream_t stream);
 
 }  // namespace lsa

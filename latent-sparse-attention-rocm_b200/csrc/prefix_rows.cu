@@ -68,6 +68,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) prefix_rows_kernel(const Prefi
     constexpr int C = D / 8;  // 16-byte chunks of a row
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // Behind the call's tensor-core kernel (which waited for everything before the call) this one
+    // starts as that one's CTAs leave; what follows needs both, so the wait comes last.
+    if (!rp.follows) grid_wait();
+    grid_trigger();
     int item = blockIdx.x;
     const bool own = item >= rp.prefix_items;
     int b = 0, h, part, nrows, k0, k1, len = 0;
@@ -258,16 +262,13 @@ __global__ void __launch_bounds__(kWarps * 32, 2) prefix_rows_kernel(const Prefi
         if (c == 0) a.part_lse[at] = total > 0.0f ? top + log2f(total) : -INFINITY;
         *reinterpret_cast<float4*>(a.part_o + at * D + c) = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
     }
+    if (rp.follows) grid_wait();
 }
 
 template <typename T, int D>
 int launch(const PrefixArgs& a, const RowsPlan& rp, unsigned grid, cudaStream_t stream) {
-    auto kern = prefix_rows_kernel<T, D>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsShape<D>::kSmem) != cudaSuccess)
-        return LSA_ERR_CUDA;
-    kern<<<grid, kWarps * 32, RowsShape<D>::kSmem, stream>>>(a, rp);
-    LSA_LAUNCH_CHECK();
-    return LSA_OK;
+    if (!allow_smem<prefix_rows_kernel<T, D>>(RowsShape<D>::kSmem)) return LSA_ERR_CUDA;
+    return launch_after(prefix_rows_kernel<T, D>, dim3(grid), kWarps * 32, RowsShape<D>::kSmem, stream, a, rp);
 }
 
 }  // namespace

@@ -281,11 +281,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + Sh::kOffMisc);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + Sh::kOffMisc + 4);
     const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const Item w = item_of(a, tp);
-    const int n = w.c1 - w.c0;
-    // the item's last chunk reaches past the sequence's keys
-    const bool tail = n > 0 && w.c1 > w.np && (w.c1 - w.np) * kChunk > w.len;
-
     if (threadIdx.x == 0) {
         for (int s = 0; s < NS; ++s) {
             mbar_init(&full[s], 1);
@@ -305,6 +300,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) tmem_alloc(tmem_slot, 512);
+    grid_wait();  // the inputs, the lengths among them, and the parts' last readers
+    grid_trigger();
+    const Item w = item_of(a, tp);
+    const int n = w.c1 - w.c0;
+    // the item's last chunk reaches past the sequence's keys
+    const bool tail = n > 0 && w.c1 > w.np && (w.c1 - w.np) * kChunk > w.len;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -490,12 +491,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 template <typename T, int D>
 int launch(const TileMaps& maps, const PrefixArgs& a, const TilePlan& tp, unsigned grid, cudaStream_t stream) {
-    auto kern = prefix_tile_kernel<T, D>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, TileShape<D>::kSmem) != cudaSuccess)
-        return LSA_ERR_CUDA;
-    kern<<<grid, kThreads, TileShape<D>::kSmem, stream>>>(maps, a, tp);
-    LSA_LAUNCH_CHECK();
-    return LSA_OK;
+    if (!allow_smem<prefix_tile_kernel<T, D>>(TileShape<D>::kSmem)) return LSA_ERR_CUDA;
+    return launch_after(prefix_tile_kernel<T, D>, dim3(grid), kThreads, TileShape<D>::kSmem, stream, maps, a, tp);
 }
 
 }  // namespace

@@ -1,4 +1,4 @@
-// scored.cu - attention weights of the own keys, added to a running score (sm_100a).
+// scored.cu - attention weights of the own keys of fp32 caches, added to a running score (sm_100a).
 //
 // With every row's lse known (prefix.cuh), key j of sequence b and KV head h gains
 //   w_j = sum over the rows r = (token, head of the group) that see j of 2^(s_rj - lse_r)
@@ -75,52 +75,18 @@ __global__ void __launch_bounds__(kWKeys) own_weights_kernel(const PrefixArgs a,
     if (j < a.T) scores_out[at] = scores[at] + w;
 }
 
-// From the logits that the few-row kernel kept (at most 16 rows a KV head: 4 bytes a row and key
-// against the 256 bytes of K that scoring the key again would read).
-__global__ void __launch_bounds__(256) logit_weights_kernel(const PrefixArgs a, const float* __restrict__ logits,
-                                                            const float* __restrict__ scores,
-                                                            float* __restrict__ scores_out) {
-    __shared__ float slse[16];
-    const int b = blockIdx.z, h = blockIdx.y, nrows = a.Tq * a.G;
-    const int64_t bh = (int64_t)b * a.Hkv + h;
-    if (threadIdx.x < nrows)
-        slse[threadIdx.x] =
-            a.lse2[row_index(a, (int64_t)b * a.Tq + threadIdx.x / a.G, h, threadIdx.x % a.G)];
-    __syncthreads();
-    const int j = blockIdx.x * 256 + threadIdx.x;
-    if (j >= a.T) return;
-    float w = 0.0f;
-    if (j < own_length(a, b))
-        for (int r = 0; r < nrows; ++r) {
-            const float s = logits[(bh * nrows + r) * a.T + j];
-            if (s != -INFINITY) w += exp2f(s - slse[r]);  // -inf: the row does not see the key
-        }
-    scores_out[bh * a.T + j] = scores[bh * a.T + j] + w;
-}
-
 template <int D>
 int weights_launch(const PrefixArgs& a, const float* scores, float* scores_out, cudaStream_t stream) {
     const int smem = (kWKeys * (D + 4) + kWRows * D) * 4;
-    auto kern = own_weights_kernel<D>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-        return LSA_ERR_CUDA;
+    if (!allow_smem<own_weights_kernel<D>>(smem)) return LSA_ERR_CUDA;
     if (a.B > 65535 || a.Hkv > 65535) return LSA_ERR_SIZE;
     dim3 grid((unsigned)((a.T + kWKeys - 1) / kWKeys), (unsigned)a.Hkv, (unsigned)a.B);
-    kern<<<grid, kWKeys, smem, stream>>>(a, scores, scores_out);
+    own_weights_kernel<D><<<grid, kWKeys, smem, stream>>>(a, scores, scores_out);
     LSA_LAUNCH_CHECK();
     return LSA_OK;
 }
 
 }  // namespace
-
-int launch_logit_weights(const PrefixArgs& a, const float* logits, const float* scores, float* scores_out,
-                         cudaStream_t stream) {
-    if (a.B > 65535 || a.Hkv > 65535) return LSA_ERR_SIZE;
-    dim3 grid((unsigned)(((int64_t)a.T + 255) / 256), (unsigned)a.Hkv, (unsigned)a.B);
-    logit_weights_kernel<<<grid, 256, 0, stream>>>(a, logits, scores, scores_out);
-    LSA_LAUNCH_CHECK();
-    return LSA_OK;
-}
 
 int launch_own_weights(const PrefixArgs& a, int D, const float* scores, float* scores_out, cudaStream_t stream) {
     return D == 128 ? weights_launch<128>(a, scores, scores_out, stream)

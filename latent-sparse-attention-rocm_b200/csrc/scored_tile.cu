@@ -55,6 +55,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + Sh::kOffMisc + 4);
     const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
+    grid_wait();
+    grid_trigger();
     int i = blockIdx.x;
     const int split = i % wp.splits;
     i /= wp.splits;
@@ -254,12 +256,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <typename T, int D>
 int launch(const WeightMaps& maps, const PrefixArgs& a, const WeightPlan& wp, unsigned grid, const float* scores,
            float* scores_out, cudaStream_t stream) {
-    auto kern = weights_tile_kernel<T, D>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, WeightShape<D>::kSmem) != cudaSuccess)
-        return LSA_ERR_CUDA;
-    kern<<<grid, kThreads, WeightShape<D>::kSmem, stream>>>(maps, a, wp, scores, scores_out);
-    LSA_LAUNCH_CHECK();
-    return LSA_OK;
+    if (!allow_smem<weights_tile_kernel<T, D>>(WeightShape<D>::kSmem)) return LSA_ERR_CUDA;
+    return launch_after(weights_tile_kernel<T, D>, dim3(grid), kThreads, WeightShape<D>::kSmem, stream, maps, a, wp,
+                        scores, scores_out);
 }
 
 }  // namespace

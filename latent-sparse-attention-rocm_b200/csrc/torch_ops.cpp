@@ -8,7 +8,7 @@
 //                     sink, top_k) -> (lists, lengths)          flat_select fused, pipeline.py:274-316
 //                     (index_queries [R, d], or raw queries [R, Hq, D]: regroup fused in)
 //   lsa::sparse_read(q, k, v, ids, lengths, scale) -> out     sparse_read_auto, read_kernel_tiled.py:147
-//   lsa::shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths, scale) -> (out, lse)
+//   lsa::shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths, scale, return_lse) -> (out, lse)
 //   lsa::scored_attention(q, k_prefix, v_prefix, k, v, lengths, scores, scale) -> (out, scores)
 //   lsa::evict(k, v, scores, lengths, budget, window, sink, capacity)
 //                     -> (k, v, scores, lengths, ids)            no reference counterpart
@@ -263,9 +263,9 @@ PrefixOut prefix_attention(const at::Tensor& q_in, const at::Tensor& kp_in, cons
 
 std::tuple<at::Tensor, at::Tensor> shared_prefix_cuda(const at::Tensor& q, const at::Tensor& kp, const at::Tensor& vp,
                                                       const at::Tensor& k, const at::Tensor& v,
-                                                      const at::Tensor& lengths, double scale) {
-    auto r = prefix_attention(q, kp, vp, k, v, lengths, nullptr, scale, true, "shared_prefix_attention");
-    return {r.out, r.lse};
+                                                      const at::Tensor& lengths, double scale, bool return_lse) {
+    auto r = prefix_attention(q, kp, vp, k, v, lengths, nullptr, scale, return_lse, "shared_prefix_attention");
+    return {r.out, return_lse ? r.lse : at::empty({0}, q.options().dtype(at::kFloat))};
 }
 
 std::tuple<at::Tensor, at::Tensor> scored_cuda(const at::Tensor& q, const at::Tensor& kp, const at::Tensor& vp,
@@ -339,9 +339,10 @@ at::Tensor sparse_read_meta(const at::Tensor& q, const at::Tensor&, const at::Te
 
 std::tuple<at::Tensor, at::Tensor> shared_prefix_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor&,
                                                       const at::Tensor&, const at::Tensor&, const at::Tensor&,
-                                                      double) {
+                                                      double, bool return_lse) {
+    auto f32 = q.options().dtype(at::kFloat);
     return {at::empty(q.sizes(), q.options()),
-            at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat))};
+            return_lse ? at::empty({q.size(0), q.size(1), q.size(2)}, f32) : at::empty({0}, f32)};
 }
 
 std::tuple<at::Tensor, at::Tensor> scored_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor&,
@@ -368,7 +369,7 @@ TORCH_LIBRARY(lsa, m) {
           "int top_p, int window, int sink, int top_k) -> (Tensor, Tensor)");
     m.def("sparse_read(Tensor q, Tensor k, Tensor v, Tensor ids, Tensor lengths, float scale) -> Tensor");
     m.def("shared_prefix_attention(Tensor q, Tensor k_prefix, Tensor v_prefix, Tensor k, Tensor v, Tensor lengths, "
-          "float scale) -> (Tensor, Tensor)");
+          "float scale, bool return_lse=False) -> (Tensor, Tensor)");
     m.def("scored_attention(Tensor q, Tensor k_prefix, Tensor v_prefix, Tensor k, Tensor v, Tensor lengths, "
           "Tensor scores, float scale) -> (Tensor, Tensor)");
     m.def("evict(Tensor k, Tensor v, Tensor scores, Tensor lengths, int budget, int window, int sink, int capacity) "

@@ -28,6 +28,6 @@ def shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths, scale=None, re
     log-sum-exp of every row's scaled logits, fp32 [B, Tq, Hq]."""
     require_cuda(q, k_prefix, v_prefix, k, v, lengths, what="shared_prefix_attention")
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
-    out, lse = _lib.torch_ops().shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths, scale)
+    out, lse = _lib.torch_ops().shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths, scale, return_lse)
     _lib.after_call(q.device, "shared_prefix_attention")
     return (out, lse) if return_lse else out

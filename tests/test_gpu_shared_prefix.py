@@ -107,6 +107,8 @@ CASES = [
     (1, 1, 32, 8, 128, 0, 20000),
     (2, 3, 5, 1, 64, 0, 128),
     (7, 4, 4, 1, 128, 256, 4),       # caches that hold the call's tokens alone
+    (40, 64, 16, 4, 128, 300, 130),  # more row tiles than SMs: whole ones, and a split rest
+    (25, 150, 12, 3, 64, 200, 160),  # 600 rows a sequence, 75 of them in the last tile of three
 ]
 
 
