@@ -10,7 +10,8 @@ namespace {
 constexpr int kSimtRows = 16;  // rows of a work item
 constexpr int kSimtKeys = 32;  // keys of a tile: one per lane
 constexpr int kSimtWarps = 8;
-constexpr int kFewRows = 16;   // rows of a KV head that the few-row kernel takes
+constexpr int kFewRows = 16;   // rows of a KV head in an item of the few-row kernel
+constexpr int kMostFew = 64;   // rows of a sequence and KV head that it takes at most
 
 template <int D>
 __device__ __forceinline__ void stage_rows(float* dst, int ld, const float* src, int64_t stride, int rows, int live) {
@@ -158,14 +159,14 @@ __device__ __forceinline__ float joined_lse(const PrefixArgs& a, int64_t row, in
 
 constexpr int kWeightKeys = 1024;  // keys of a weights block: four a thread
 
-// Own keys' weights from the logits that the few-row kernel kept (at most 16 rows a KV head: 4
-// bytes a row and key against the 256 bytes of K that scoring the key again would read):
+// Own keys' weights from the logits that the few-row kernel kept (4 bytes a row and key, 16 for a
+// decode step of 4 heads, against the 256 bytes of K that scoring the key again would read):
 //   w_j = sum over the rows r that see j of 2^(s_rj - lse_r).
 // One thread owns a key, so the sum has one order and one writer. The block joins its rows' lse
 // itself, beside the blocks that join the output: one launch for both.
 __device__ __forceinline__ void own_weights(const PrefixArgs& a, int parts, const float* __restrict__ logits,
                                             const float* __restrict__ scores, float* __restrict__ scores_out) {
-    __shared__ float slse[kFewRows];
+    __shared__ float slse[kMostFew];
     const int per = (int)(((int64_t)a.T + kWeightKeys - 1) / kWeightKeys);
     const int64_t bh = blockIdx.x / per;
     const int b = (int)(bh / a.Hkv), h = (int)(bh % a.Hkv), nrows = a.Tq * a.G, warp = threadIdx.x >> 5;
@@ -217,8 +218,10 @@ __global__ void __launch_bounds__(256) prefix_finish_kernel(const PrefixArgs a, 
     if (tp.whole) {  // the rows of the split seq tiles, 256 a tile
         int b, h, tile;
         seq_tile(a, tp, tp.whole + (int)(row >> 8), &b, &h, &tile);
-        const int r = tile * 256 + (int)(row & 255), tok = r / a.G;
-        row = tok < a.Tq ? row_index(a, (int64_t)b * a.Tq + tok, h, r - tok * a.G) : a.rows;
+        int tok, g;
+        const bool in = tile_row(a, tp, (int)(row >> 7) & 1, (int)(row & 127), &tok, &g);
+        tok += tile * 2 * tp.tokens;
+        row = in && tok < a.Tq ? row_index(a, (int64_t)b * a.Tq + tok, h, g) : a.rows;
     }
     if (row >= a.rows) return;
     float x[kPer];
@@ -320,20 +323,7 @@ struct Plan {
 
 constexpr int kSMs = 148;
 
-// Splits of `chunks` for `items` equal work items on `slots` places that hold one item each: the
-// fewest that minimise waves x (chunks of an item + its fixed cost in chunks).
-int balance(int64_t items, int64_t chunks, int64_t fixed, int64_t slots) {
-    if (chunks == 0) return 0;
-    int best = 1;
-    int64_t least = INT64_MAX;
-    for (int s = 1; s <= kMaxSplits && s <= chunks; ++s) {
-        const int64_t cost = (items * s + slots - 1) / slots * ((chunks + s - 1) / s + fixed);
-        if (cost < least) least = cost, best = s;
-    }
-    return best;
-}
-
-Plan make_plan(int dtype, int64_t B, int64_t Tq, int64_t Hkv, int64_t G, int64_t P, int64_t T, bool scored) {
+Plan make_plan(int dtype, int64_t B, int64_t Tq, int64_t Hkv, int64_t G, int64_t D, int64_t P, int64_t T, bool scored) {
     Plan p = {};
     p.merge = true;
     p.simt = dtype == kF32;
@@ -353,8 +343,9 @@ Plan make_plan(int dtype, int64_t B, int64_t Tq, int64_t Hkv, int64_t G, int64_t
     TilePlan& t = p.tile;
     const int64_t rows = Tq * G;
     const int64_t pc = (P + 127) / 128, oc = (T + 127) / 128;
-    t.seq_streams = rows <= 128;
-    t.seq_tiles = (int)(rows <= 128 ? 1 : (rows + 255) / 256);
+    t.tokens = (int)(128 / G);
+    t.seq_streams = Tq <= t.tokens;
+    t.seq_tiles = (int)((Tq + 2 * t.tokens - 1) / (2 * t.tokens));
     const int64_t seq = B * Hkv * t.seq_tiles;
     t.joint = P > 0 && rows * 4 >= (int64_t)t.seq_tiles * 256 * 3;
     if (t.joint) {
@@ -362,7 +353,7 @@ Plan make_plan(int dtype, int64_t B, int64_t Tq, int64_t Hkv, int64_t G, int64_t
         // of the last, short round are, so that it too fills the GPU
         t.whole = (int)(seq / kSMs * kSMs);
         const int64_t rest = seq - t.whole;
-        p.So = rest ? balance(rest, pc + oc, 3, kSMs) : 1;
+        p.So = rest ? balance(rest, pc + oc, 2, kSMs) : 1;
         if (p.So == 1) t.whole = (int)seq;
         p.merge = p.So > 1;
         p.parts_o = p.merge ? p.So : 0;
@@ -373,19 +364,23 @@ Plan make_plan(int dtype, int64_t B, int64_t Tq, int64_t Hkv, int64_t G, int64_t
         p.parts_p = p.Sp = balance(Hkv, (P + 63) / 64, 2, 2 * kSMs);
         p.rows.prefix_items = (int)(Hkv * p.Sp);
     } else {
-        t.batch_streams = B * rows <= 128;
-        t.batch_tiles = (int)(B * rows <= 128 ? 1 : (B * rows + 255) / 256);
-        p.Sp = balance(Hkv * t.batch_tiles, t.batch_streams ? (pc + 1) / 2 : pc, 3, kSMs);
+        t.batch_streams = B * Tq <= t.tokens;
+        t.batch_tiles = (int)((B * Tq + 2 * t.tokens - 1) / (2 * t.tokens));
+        p.Sp = balance(Hkv * t.batch_tiles, t.batch_streams ? (pc + 1) / 2 : pc, 2, kSMs);
         p.parts_p = p.Sp * (t.batch_streams ? 2 : 1);
         t.batch_items = (int)(Hkv * t.batch_tiles * p.Sp);
     }
-    if (rows <= kFewRows) {
-        p.parts_o = p.So = balance(B * Hkv, (T + 63) / 64, 2, 2 * kSMs);
-        p.rows.own_items = (int)(B * Hkv * p.So);
-        p.logits = scored;
+    // few rows: the few-row kernel reads the keys once for each 16 of them, from L2 after the first
+    // time, and has no fixed cost to speak of; a tensor-core item spends about 6 us, 32 MB of keys
+    const int64_t tiles = (rows + kFewRows - 1) / kFewRows;
+    if (tiles == 1 || (rows <= kMostFew && (tiles - 1) * B * T * Hkv * D * 4 <= 32 << 20)) {
+        p.rows.own_tiles = (int)tiles;
+        p.parts_o = p.So = balance(B * Hkv * tiles, (T + 63) / 64, 2, 2 * kSMs);
+        p.rows.own_items = (int)(B * Hkv * tiles * p.So);
         p.rows.follows = t.batch_items > 0;
+        p.logits = scored;
     } else {
-        p.So = balance(seq, t.seq_streams ? (oc + 1) / 2 : oc, 3, kSMs);
+        p.So = balance(seq, t.seq_streams ? (oc + 1) / 2 : oc, 2, kSMs);
         p.parts_o = p.So * (t.seq_streams ? 2 : 1);
         t.seq_items = (int)(seq * p.So);
     }
@@ -421,7 +416,7 @@ int64_t lsa_shared_prefix_scratch(int dtype, int64_t B, int64_t Tq, int64_t Hq, 
                                   int64_t T, int scored) {
     if (!sizes_ok(B, Tq, Hq, Hkv, D, P, T) || dtype < kF32 || dtype > kBF16) return LSA_ERR_ARG;
     if (B == 0 || Tq == 0) return 0;
-    const Plan p = make_plan(dtype, B, Tq, Hkv, Hq / Hkv, P, T, scored);
+    const Plan p = make_plan(dtype, B, Tq, Hkv, Hq / Hkv, D, P, T, scored);
     const int64_t rows = B * Tq * Hq;
     const int64_t parts = p.parts_p + p.parts_o;
     return round256(parts * rows * D * 4) + round256(parts * rows * 4) + round256(rows * 4) +
@@ -452,8 +447,10 @@ int lsa_shared_prefix_attention(const void* q, const void* k_prefix, const void*
         st[i] = extent[i] > 1 ? strides[i] : D;
         if (st[i] <= 0 || st[i] % unit || st[i] >= (int64_t)1 << 38) return LSA_ERR_ARG;
     }
+    // the tensor-core kernel's tiles run over all sequences' tokens: one stride between them
+    if (dtype != kF32 && B > 1 && Tq > 1 && st[0] != Tq * st[1]) return LSA_ERR_ARG;
     if (scratch_bytes < lsa_shared_prefix_scratch(dtype, B, Tq, Hq, Hkv, D, P, T, scores != nullptr)) return LSA_ERR_ARG;
-    const Plan p = make_plan(dtype, B, Tq, Hkv, Hq / Hkv, P, T, scores != nullptr);
+    const Plan p = make_plan(dtype, B, Tq, Hkv, Hq / Hkv, D, P, T, scores != nullptr);
     PrefixArgs a;
     a.q = q, a.kp = k_prefix, a.vp = v_prefix, a.k = k, a.v = v;
     a.q_b = st[0], a.q_t = st[1], a.q_h = st[2];

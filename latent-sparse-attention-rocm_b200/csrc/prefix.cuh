@@ -42,14 +42,25 @@ struct PrefixArgs {
     int32_t* status;                      // LSA_ERR_TIMEOUT after an expired wait
 };
 
-// The work of the tensor-core kernel (prefix_tile.cu).
+// The work of the tensor-core kernel (prefix_tile.cu). A row tile is two halves of `tokens` tokens,
+// the G query heads of each (at most 128 rows a half).
 struct TilePlan {
+    int tokens;                    // 128 / G
+
     int batch_items, batch_tiles;  // row tiles over all sequences: prefix keys
     int seq_items, seq_tiles;      // row tiles of a sequence: its own keys (items; tiles of a sequence)
-    bool batch_streams, seq_streams;  // tiles of at most 128 rows: two streams of chunks
+    bool batch_streams, seq_streams;  // tiles of one half's rows: two streams of chunks
     bool joint;                    // seq tiles read the prefix too
     int whole;                     // the first seq tiles, not split: they write the output themselves
 };
+
+// Row rl of half `hf` of a row tile: (token of the tile, head of the group); false: no row there.
+__device__ __forceinline__ bool tile_row(const PrefixArgs& a, const TilePlan& t, int hf, int rl, int* tok, int* g) {
+    const int tl = rl / a.G;
+    *tok = hf * t.tokens + tl;
+    *g = rl - tl * a.G;
+    return tl < t.tokens;
+}
 
 // Seq tile i: (sequence, KV head, row tile), the longest causal ranges first.
 __device__ __forceinline__ void seq_tile(const PrefixArgs& a, const TilePlan& t, int i, int* b, int* h, int* tile) {
@@ -90,6 +101,19 @@ template <auto kKernel> bool allow_smem(int bytes) {
     return true;
 }
 
+// Splits of `chunks` for `items` equal work items on `slots` places that hold one item each: the
+// fewest that minimise rounds x (chunks of an item + its fixed cost in chunks).
+inline int balance(int64_t items, int64_t chunks, double fixed, int64_t slots) {
+    if (chunks == 0) return 0;
+    int best = 1;
+    double least = 1e300;
+    for (int s = 1; s <= kMaxSplits && s <= chunks; ++s) {
+        const double cost = (double)((items * s + slots - 1) / slots) * ((double)chunks / s + fixed);
+        if (cost < 0.99 * least) least = cost, best = s;
+    }
+    return best;
+}
+
 // own keys that sequence b holds
 __device__ __forceinline__ int own_length(const PrefixArgs& a, int b) {
     const int n = a.lengths[b];
@@ -110,9 +134,10 @@ __device__ __host__ __forceinline__ void split_range(int n, int s, int S, int un
     *k1 = (int)(b < n ? b : n);
 }
 
-// The work of the few-row kernel (prefix_rows.cu): segments of at most 16 rows a KV head.
+// The work of the few-row kernel (prefix_rows.cu), 16 rows of a KV head an item.
 struct RowsPlan {
     int prefix_items, own_items;
+    int own_tiles;  // row tiles of a sequence (the prefix's rows are one tile)
     bool follows;   // launched behind this call's tensor-core kernel, whose output it does not read
     float* logits;  // [B, Hkv, Tq * G, T] log2-domain logits of the own keys, or null
 };

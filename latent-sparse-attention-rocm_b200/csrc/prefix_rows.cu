@@ -1,7 +1,8 @@
 // prefix_rows.cu - the shared-prefix attention of few rows: decode steps (sm_100a).
 //
 // A work item is at most 16 query rows of one KV head (a sequence's decode rows against its own
-// cache, or a small batch's against the prefix) x a range of keys. The keys' bytes bound it: 512
+// cache, or a small batch's against the prefix) x a range of keys; a sequence with up to 64 rows and
+// a short cache is several items that read the same keys, from L2 after the first. The keys' bytes bound it: 512
 // bytes of K and V per key and head (D = 128, 16 bits) against 16 rows of arithmetic. So nothing
 // waits for a neighbour in the main loop: each of a CTA's four warps copies its own tiles of 16
 // keys (cp.async, 16 bytes, three stages of 8 KB in flight per warp, two CTAs an SM) and runs its
@@ -74,7 +75,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) prefix_rows_kernel(const Prefi
     grid_trigger();
     int item = blockIdx.x;
     const bool own = item >= rp.prefix_items;
-    int b = 0, h, part, nrows, k0, k1, len = 0;
+    int b = 0, h, part, nrows, r0 = 0, k0, k1, len = 0;
     if (!own) {
         const int split = item % a.Sp;
         h = item / a.Sp;
@@ -85,6 +86,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) prefix_rows_kernel(const Prefi
         item -= rp.prefix_items;
         const int split = item % a.So;
         item /= a.So;
+        r0 = item % rp.own_tiles * kRows;
+        item /= rp.own_tiles;
         h = item % a.Hkv, b = item / a.Hkv;
         part = a.parts_p + split;
         nrows = a.Tq * a.G;
@@ -119,13 +122,13 @@ __global__ void __launch_bounds__(kWarps * 32, 2) prefix_rows_kernel(const Prefi
 #pragma unroll
     for (int i = 0; i < kRing - 1; ++i) copy(i);
 
-    // Q fragments: rows lane / 4 and lane / 4 + 8
+    // Q fragments: rows r0 + lane / 4 and r0 + lane / 4 + 8
     uint32_t qf[D / 16][4];
     int limit[2];
     const int quad = lane >> 2, qc = (lane & 3) * 2;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-        const int r = quad + 8 * u;
+        const int r = r0 + quad + 8 * u;
         const int tok = r / a.G;
         limit[u] = r >= nrows ? 0 : (own ? len - a.Tq + tok + 1 : k1);
         const int64_t bt = (int64_t)b * a.Tq + tok;
@@ -144,7 +147,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) prefix_rows_kernel(const Prefi
         for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
     float* logits = own && rp.logits
-                        ? rp.logits + (((int64_t)b * a.Hkv + h) * nrows + quad) * a.T
+                        ? rp.logits + (((int64_t)b * a.Hkv + h) * nrows + r0 + quad) * a.T
                         : nullptr;
 
     for (int i = 0; i < tiles; ++i) {
@@ -172,7 +175,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) prefix_rows_kernel(const Prefi
         if (logits) {
 #pragma unroll
             for (int u = 0; u < 2; ++u)
-                if (quad + 8 * u < nrows)
+                if (r0 + quad + 8 * u < nrows)
 #pragma unroll
                     for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -240,7 +243,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) prefix_rows_kernel(const Prefi
         if ((lane & 3) == 0) sml[warp * kRows + quad + 8 * u] = make_float2(m[u], l[u]);
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < nrows * (D / 4); i += kWarps * 32) {
+    const int live = nrows - r0 < kRows ? nrows - r0 : kRows;
+    for (int i = threadIdx.x; i < live * (D / 4); i += kWarps * 32) {
         const int r = i / (D / 4), c = i % (D / 4) * 4;
         float top = -INFINITY;
 #pragma unroll
@@ -256,8 +260,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) prefix_rows_kernel(const Prefi
             x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w);
         }
         const float inv = total > 0.0f ? 1.0f / total : 0.0f;
-        const int tok = r / a.G;
-        const int64_t rid = row_index(a, (int64_t)b * a.Tq + tok, h, r - tok * a.G);
+        const int tok = (r0 + r) / a.G;
+        const int64_t rid = row_index(a, (int64_t)b * a.Tq + tok, h, r0 + r - tok * a.G);
         const int64_t at = (int64_t)part * a.rows + rid;
         if (c == 0) a.part_lse[at] = total > 0.0f ? top + log2f(total) : -INFINITY;
         *reinterpret_cast<float4*>(a.part_o + at * D + c) = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);

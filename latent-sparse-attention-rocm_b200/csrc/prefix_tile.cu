@@ -34,7 +34,7 @@ namespace {
 
 constexpr int kThreads = 384;
 struct TileMaps {
-    CUtensorMap kp, vp, k, v;
+    CUtensorMap kp, vp, k, v, q;
 };
 
 template <int D> struct TileShape {
@@ -52,7 +52,8 @@ template <int D> struct TileShape {
 struct Item {
     bool own, streams;  // seq tile; both halves hold the same rows
     bool direct;        // all of its rows' keys: it writes the output itself
-    int b, h, r0, nrows, part, len;
+    int b, h, part, len;
+    int t0, tokens;  // first token of the tile, tokens of the segment (all sequences' or one's)
     int np;      // prefix chunks of the item's chunk list
     int c0, c1;  // its chunks of the list [0, np + own chunks)
 };
@@ -70,8 +71,8 @@ __device__ __forceinline__ Item item_of(const PrefixArgs& a, const TilePlan& t) 
         w.b = 0;
         w.len = 0;
         w.streams = t.batch_streams;
-        w.nrows = a.B * a.Tq * a.G;
-        w.r0 = tile * (w.streams ? 128 : 256);
+        w.tokens = a.B * a.Tq;
+        w.t0 = tile * 2 * t.tokens;
         w.np = chunks = (a.P + kChunk - 1) / kChunk;
         w.part = 0;
         w.direct = false;
@@ -83,10 +84,10 @@ __device__ __forceinline__ Item item_of(const PrefixArgs& a, const TilePlan& t) 
         seq_tile(a, t, w.direct ? i : t.whole + (i - t.whole) / S, &w.b, &w.h, &tile);
         w.len = own_length(a, w.b);
         w.streams = t.seq_streams;
-        w.nrows = a.Tq * a.G;
-        w.r0 = tile * (w.streams ? 128 : 256);
-        const int last = (w.r0 + (w.streams ? 128 : 256) < w.nrows ? w.r0 + (w.streams ? 128 : 256) : w.nrows) - 1;
-        int seen = w.len - a.Tq + last / a.G + 1;  // own keys that the tile's last row sees
+        w.tokens = a.Tq;
+        w.t0 = tile * 2 * t.tokens;
+        const int end = w.t0 + 2 * t.tokens < a.Tq ? w.t0 + 2 * t.tokens : a.Tq;
+        int seen = w.len - a.Tq + end;  // own keys that the tile's last row sees
         seen = seen < 0 ? 0 : seen;
         w.np = t.joint ? (a.P + kChunk - 1) / kChunk : 0;
         chunks = w.np + (seen + kChunk - 1) / kChunk;
@@ -98,15 +99,16 @@ __device__ __forceinline__ Item item_of(const PrefixArgs& a, const TilePlan& t) 
 }
 
 template <typename T, int D>
-__device__ __forceinline__ void softmax_half(const PrefixArgs& a, const Item& w, uint64_t* bars, uint8_t* stage,
-                                             volatile int* abort_flag, uint32_t tmem) {
+__device__ __forceinline__ void softmax_half(const PrefixArgs& a, const TilePlan& tp, const Item& w, uint64_t* bars,
+                                             uint8_t* stage, volatile int* abort_flag, uint32_t tmem) {
     using Sh = TileShape<D>;
     uint64_t *bar_s = bars + 2 * Sh::kStages + 1, *bar_p = bar_s + 2, *bar_o = bar_p + 4;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int hf = (warp - 4) >> 2, qd = warp & 3;
-    const int r = w.r0 + (w.streams ? 0 : hf * 128) + qd * 32 + lane;
-    const bool live = r < w.nrows;
-    const int tok = r / a.G;
+    int tok, g;
+    bool live = tile_row(a, tp, w.streams ? 0 : hf, qd * 32 + lane, &tok, &g);
+    tok += w.t0;
+    live = live && tok < w.tokens;
     // own keys the row sees; a prefix key is seen by all
     const int own_limit = !live ? 0 : (w.own ? w.len - a.Tq + tok + 1 : 0);
     const int pre_limit = live ? a.P : 0;
@@ -211,7 +213,7 @@ __device__ __forceinline__ void softmax_half(const PrefixArgs& a, const Item& w,
     }
     if (ok && n > 0) ok = role_wait(&bar_o[hf], 0, abort_flag);
     if (!ok) return;
-    const int64_t rid = row_index(a, (int64_t)w.b * a.Tq + tok, w.h, r - tok * a.G);
+    const int64_t rid = row_index(a, (int64_t)w.b * a.Tq + tok, w.h, g);
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
     const float lse = l > 0.0f ? m * sl + log2f(l) : -INFINITY;
     const int64_t at = (int64_t)(w.part + (w.streams ? hf : 0)) * a.rows + rid;
@@ -281,12 +283,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + Sh::kOffMisc);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + Sh::kOffMisc + 4);
     const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    if (warp == 1) tmem_alloc(tmem_slot, 512);
     if (threadIdx.x == 0) {
         for (int s = 0; s < NS; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
-        mbar_init(bar_q, 256);
+        mbar_init(bar_q, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bar_s[i], 1);
             mbar_init(&bar_p[2 * i], 4);
@@ -299,13 +302,50 @@ __global__ void __launch_bounds__(kThreads, 1)
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 0) tmem_alloc(tmem_slot, 512);
     grid_wait();  // the inputs, the lengths among them, and the parts' last readers
     grid_trigger();
     const Item w = item_of(a, tp);
     const int n = w.c1 - w.c0;
     // the item's last chunk reaches past the sequence's keys
     const bool tail = n > 0 && w.c1 > w.np && (w.c1 - w.np) * kChunk > w.len;
+    // Tile p of the ring, in the order the MMAs use them: one chunk's K (two, with two streams)
+    // ahead of the first V, then V and the K that follows in turn.
+    auto load = [&](int p) {
+        int c, val;
+        if (!w.streams) {
+            val = p & 1, c = p >> 1;
+        } else if (p < 2 && p < n) {
+            val = 0, c = p;
+        } else if (n == 1) {
+            val = 1, c = 0;
+        } else {
+            const int i = p - 2;
+            val = i >= 2 * (n - 2) || (i & 1) == 0;
+            c = i >= 2 * (n - 2) ? i - (n - 2) : (i >> 1) + (val ? 0 : 2);
+        }
+        c += w.c0;
+        const int s = p % NS;
+        const uint32_t dst = sbase + Sh::kOffStage + s * Sh::kTileBytes;
+        const bool pre = c < w.np;
+        const CUtensorMap* map = pre ? (val ? &maps.vp : &maps.kp) : (val ? &maps.v : &maps.k);
+        const int t = (pre ? c : c - w.np) * kChunk, b = pre ? 0 : w.b;
+        mbar_arrive_expect_tx(&full[s], Sh::kTileBytes);
+#pragma unroll
+        for (int x = 0; x < D; x += 64) tma_tile(dst + x * 256, map, x, t, w.h, b, &full[s]);
+    };
+    const int early = 2 * n < NS ? 2 * n : NS;
+    if (threadIdx.x == 0 && n > 0) {
+        // Q: whole tokens, the rows of one KV head (a box past the segment's tokens holds other
+        // sequences' rows or zeros; their lanes of S and O are no one's)
+        const int halves = w.streams ? 1 : 2;
+        mbar_arrive_expect_tx(bar_q, halves * tp.tokens * a.G * D * 2);
+        for (int hf = 0; hf < halves; ++hf)
+#pragma unroll
+            for (int x = 0; x < D; x += 64)
+                tma_tile(sbase + hf * Sh::kTileBytes + x * 256, &maps.q, x, w.h * a.G,
+                         w.b * a.Tq + w.t0 + hf * tp.tokens, 0, bar_q);
+        for (int p = 0; p < early; ++p) load(p);
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -314,55 +354,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp >= 4) {
         // 384 threads launch at 168 registers: 128 x 56 + 256 x 224 = 384 x 168
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;" ::: "memory");
-        // Q rows into the swizzled tiles (rows past the item's are zeros)
-        constexpr int C = D / 8, kRowsStep = 256 / C;
-        const int c = (threadIdx.x - 128) % C, row0 = (threadIdx.x - 128) / C;
-        const T* qb = static_cast<const T*>(a.q) + w.b * a.q_b + (int64_t)w.h * a.G * a.q_h + c * 8;
-#pragma unroll
-        for (int row = row0; row < 256; row += kRowsStep) {
-            const int r = w.r0 + row, rl = row & 127;
-            const bool in = r < w.nrows && (row < 128 || !w.streams);
-            const unsigned tok = in ? (unsigned)r / (unsigned)a.G : 0u;
-            const unsigned sb = w.own ? 0u : tok / (unsigned)a.Tq;  // batch tiles: tokens of all sequences
-            const T* src = qb + sb * a.q_b + (tok - sb * a.Tq) * a.q_t + (in ? r - (int)tok * a.G : 0) * a.q_h;
-            cp_async16(sbase + (row >> 7) * Sh::kTileBytes + (c >> 3) * 16384 + rl * 128 + (((c & 7) ^ (rl & 7)) << 4),
-                       src, in ? 16u : 0u);
-        }
-        cp_async_wait_all();
-        fence_proxy_async_smem();
-        mbar_arrive(bar_q);
-        softmax_half<T, D>(a, w, bars, sm + Sh::kOffStage, abort_flag, tmem);
+        softmax_half<T, D>(a, tp, w, bars, sm + Sh::kOffStage, abort_flag, tmem);
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;" ::: "memory");
         if (warp == 0) {
-            // ------------------------------------------------ loads, in the order the MMAs use them
-            int pos = 0;
-            auto load = [&](bool val, int c) -> bool {
-                const int s = pos % NS;
-                if (pos >= NS && !role_wait(&empty[s], (pos / NS - 1) & 1, abort_flag)) return false;
-                if (lane == 0) {
-                    const uint32_t dst = sbase + Sh::kOffStage + s * Sh::kTileBytes;
-                    const bool pre = c < w.np;
-                    const CUtensorMap* map = pre ? (val ? &maps.vp : &maps.kp) : (val ? &maps.v : &maps.k);
-                    const int t = (pre ? c : c - w.np) * kChunk, b = pre ? 0 : w.b;
-                    mbar_arrive_expect_tx(&full[s], Sh::kTileBytes);
-#pragma unroll
-                    for (int x = 0; x < D; x += 64) tma_tile(dst + x * 256, map, x, t, w.h, b, &full[s]);
+            // ------------------------------------------------ loads
+            if (lane == 0) {
+                int p = early;
+                for (; p < 2 * n; ++p) {
+                    if (!thread_wait(&empty[p % NS], (p / NS - 1) & 1, abort_flag)) break;
+                    load(p);
                 }
-                __syncwarp();
-                ++pos;
-                return true;
-            };
-            bool ok = true;
-            const int ahead = w.streams ? 2 : 1;  // K chunks scored before the first product with V
-            for (int c = w.c0; ok && c < w.c1 && c < w.c0 + ahead; ++c) ok = load(false, c);
-            for (int c = w.c0; ok && c < w.c1; ++c) {
-                ok = load(true, c);
-                if (ok && c + ahead < w.c1) ok = load(false, c + ahead);
+                if (p < 2 * n) {  // every copy issued lands before the CTA leaves
+                    for (int i = p > NS ? p - NS : 0; i < p; ++i) mbar_wait_bounded(&full[i % NS], (i / NS) & 1);
+                    mbar_wait_bounded(bar_q, 0);
+                }
             }
-            if (!ok) {  // every copy issued lands before the CTA leaves
-                for (int p = pos > NS ? pos - NS : 0; p < pos; ++p) mbar_wait_bounded(&full[p % NS], (p / NS) & 1);
-            }
+            __syncwarp();
         } else if (warp == 1) {
             // ------------------------------------------------ every MMA of the CTA, from one thread
             constexpr uint32_t idS = umma_idesc_f16<T>(128, 128, false);
@@ -482,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 0) {
+    if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
@@ -504,8 +512,10 @@ int launch_prefix_tiles(const PrefixArgs& a, const TilePlan& tp, int dtype, int 
     if (encode_fn() == nullptr) return LSA_ERR_CUDA;
     TileMaps maps;
     const bool bf = dtype == kBF16;
-    bool ok = true;
-    if (a.P > 0 && (tp.batch_items || tp.joint))
+    // q's tokens of all sequences in one dimension (the entry point checks that they are)
+    bool ok = encode_map(&maps.q, bf, a.q, D, a.Hq, (int64_t)a.B * a.Tq, 1, a.q_h, a.Tq > 1 ? a.q_t : a.q_b, D, a.G,
+                         tp.tokens);
+    if (ok && a.P > 0 && (tp.batch_items || tp.joint))
         ok = encode_keys(&maps.kp, bf, a.kp, D, a.P, a.Hkv, 1, a.kp_t, a.kp_h, (int64_t)D) &&
              encode_keys(&maps.vp, bf, a.vp, D, a.P, a.Hkv, 1, a.vp_t, a.vp_h, (int64_t)D);
     if (ok && a.T > 0 && tp.seq_items)

@@ -69,13 +69,13 @@ __device__ __forceinline__ void tma_tile(uint32_t dst, const CUtensorMap* map, i
 }
 
 // Untiled bulk copy shared -> global (16-byte aligned, whole multiples of 16 bytes), one group a
-// thread: committed and waited for by the thread that issued it.
+// thread: committed by the thread that issued it, which waits until shared memory has been read.
 __device__ __forceinline__ void bulk_s2g(void* dst, uint32_t src, uint32_t bytes) {
     asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes)
                  : "memory");
 }
 __device__ __forceinline__ void bulk_commit_wait() {
-    asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group 0;" ::: "memory");
+    asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
 }
 
 __device__ __forceinline__ uint32_t pack16(float a, float b, __nv_bfloat16*) {

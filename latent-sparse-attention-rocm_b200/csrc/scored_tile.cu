@@ -269,11 +269,9 @@ int launch_tile_weights(const PrefixArgs& a, int dtype, int D, const float* scor
     WeightPlan wp;
     wp.tokens = 128 / a.G;
     wp.row_tiles = (a.Tq + wp.tokens - 1) / wp.tokens;
-    // one CTA an SM: splits enough for two rounds, each of at least two pairs of key tiles
+    // one CTA an SM: the splits that fill whole rounds best, each of at least two pairs of key tiles
     const int64_t units = (int64_t)a.B * a.Hkv, pairs = ((int64_t)a.T + 2 * kChunk - 1) / (2 * kChunk);
-    int64_t s = (2 * 148 + units - 1) / units;
-    if (s > (pairs + 1) / 2) s = (pairs + 1) / 2;
-    wp.splits = (int)(s < 1 ? 1 : s);
+    wp.splits = balance(units, (pairs + 1) / 2, 1, 148);
     if (units * wp.splits > INT32_MAX) return LSA_ERR_SIZE;
     WeightMaps maps;
     const bool bf = dtype == kBF16;

@@ -229,6 +229,7 @@ PrefixOut prefix_attention(const at::Tensor& q_in, const at::Tensor& kp_in, cons
     TORCH_CHECK_VALUE(std::isfinite(scale) && scale > 0, what, ": the scale must be positive, got ", scale);
     c10::cuda::CUDAGuard guard(q_in.device());
     auto q = rows16(q_in), kp = rows16(kp_in), vp = rows16(vp_in), k = rows16(k_in), v = rows16(v_in);
+    if (B > 1 && Tq > 1 && q.stride(0) != Tq * q.stride(1)) q = q.contiguous();  // tokens one stride apart
     auto lengths = lengths_in.to(at::kInt).contiguous();
     PrefixOut r;
     r.out = at::empty({B, Tq, Hq, D}, q.options());
