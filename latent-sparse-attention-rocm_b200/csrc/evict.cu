@@ -31,6 +31,11 @@ struct EvictArgs {
 
 __device__ __forceinline__ uint32_t score_key(float f) { return (uint32_t)ordered_bits(f) ^ 0x80000000u; }
 
+__device__ __forceinline__ float key_score(uint32_t u) {  // the score itself again, bit for bit
+    const int32_t o = (int32_t)(u ^ 0x80000000u);
+    return __int_as_float(o >= 0 ? o : o ^ 0x7FFFFFFF);
+}
+
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -66,7 +71,7 @@ __device__ __forceinline__ void add_cluster(uint32_t addr, int v) {
 // Selection is a chain of short steps, the copy is bandwidth: with several CTAs an SM one row's
 // copy covers another's chain.
 template <bool kSliced>
-__global__ void __launch_bounds__(kThreads) evict_kernel(const EvictArgs a, int ranks_arg) {
+__global__ void __launch_bounds__(kThreads, 2) evict_kernel(const EvictArgs a, int ranks_arg) {
     __shared__ __align__(16) int hist[kBins];
     __shared__ __align__(16) int joined[kSliced ? 3 * kBins / 2 : 4];  // this rank's bins, one set a pass
     __shared__ int scan[kWarps], wkeep[kWarps], wtie[kWarps];
@@ -90,14 +95,39 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(const EvictArgs a, int 
         const int s0 = kSliced ? (int)((int64_t)n * rank / ranks) : 0;
         const int s1 = kSliced ? (int)((int64_t)n * (rank + 1) / ranks) : n;
         const int lo = a.sink, hi = n - a.window;  // the keys that compete
-        const int cached = s1 - s0 < kCached ? s1 - s0 : kCached;
-        auto key_at = [&](int j) { return j - s0 < kCached ? keys[j - s0] : score_key(sc[j]); };
+        auto key_at = [&](int j) {
+            if (!kSliced) return keys[j];
+            return j - s0 < kCached ? keys[j - s0] : score_key(sc[j]);
+        };
         int need = a.budget - a.sink - a.window;
         // a key stays when its top bits are above `cut`; on the level, the first `level` by index
         uint32_t cut = 0;
         int shift = 0, level = 0;
-#pragma unroll 4
-        for (int j = tid; j < cached; j += kThreads) keys[j] = score_key(sc[s0 + j]);
+        // warp w owns the keys [w0, w1), a lane every 32nd; loads go in groups at clamped indices, so
+        // that a group's are all in flight
+        const int seg = ((s1 - s0 + 31) / 32 + kWarps - 1) / kWarps * 32;
+        const int w0 = s0 + warp * seg < s1 ? s0 + warp * seg : s1, w1 = w0 + seg < s1 ? w0 + seg : s1;
+        for (int j0 = w0; j0 < w1 && j0 - s0 < kCached; j0 += 32 * 16) {
+            float x[16];
+#pragma unroll
+            for (int u = 0; u < 16; ++u) {
+                const int j = j0 + 32 * u + lane;
+                x[u] = __ldg(sc + (j < w1 ? j : w1 - 1));
+            }
+#pragma unroll
+            for (int u = 0; u < 16; ++u) {
+                const int j = j0 + 32 * u + lane;
+                if (j < w1 && j - s0 < kCached) keys[j - s0] = score_key(x[u]);
+            }
+        }
+        // f(j, key) for the warp's keys, 32 consecutive ones a step (j at or past w1: no key)
+        auto each = [&](auto f) {
+#pragma unroll 2
+            for (int j0 = w0; j0 < w1; j0 += 32) {
+                const int j = j0 + lane;
+                f(j, j < w1 ? key_at(j) : 0u);
+            }
+        };
         if (kSliced) {
             for (int i = tid; i < 3 * kBins / 2; i += kThreads) joined[i] = 0;
             cluster_sync();
@@ -154,25 +184,14 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(const EvictArgs a, int 
                 if (found.y == found.z) break;  // the whole bin stays
             }
         }
-        // keys that stay for sure and keys on the level, by warp segments of whole ballots
-        const int seg = ((s1 - s0 + 31) / 32 + kWarps - 1) / kWarps * 32;
-        const int w0 = s0 + warp * seg < s1 ? s0 + warp * seg : s1, w1 = w0 + seg < s1 ? w0 + seg : s1;
-        auto classify = [&](int j, bool* keep, bool* tie) {
-            *keep = *tie = false;
-            if (j < w1) {
-                const uint32_t u = key_at(j) >> shift;
-                const bool forced = j < lo || j >= hi;
-                *keep = forced || u > cut;
-                *tie = !forced && u == cut;
-            }
-        };
+        // keys that stay for sure, and keys on the level
         int nk = 0, nt = 0;
-#pragma unroll 4
-        for (int j0 = w0; j0 < w1; j0 += 32) {
-            bool keep, tie;
-            classify(j0 + lane, &keep, &tie);
-            nk += keep, nt += tie;
-        }
+        each([&](int j, uint32_t key) {
+            const uint32_t u = key >> shift;
+            const bool in = j < w1, forced = j < lo || j >= hi;
+            nk += in && (forced || u > cut);
+            nt += in && !forced && u == cut;
+        });
         nk = __reduce_add_sync(0xFFFFFFFFu, nk), nt = __reduce_add_sync(0xFFFFFFFFu, nt);
         if (lane == 0) wkeep[warp] = nk, wtie[warp] = nt;
         __syncthreads();
@@ -190,10 +209,10 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(const EvictArgs a, int 
         }
         keep_before += __reduce_add_sync(0xFFFFFFFFu, lane < warp && lane < kWarps ? wkeep[lane] : 0);
         tie_before += __reduce_add_sync(0xFFFFFFFFu, lane < warp && lane < kWarps ? wtie[lane] : 0);
-        for (int j0 = w0; j0 < w1; j0 += 32) {
-            const int j = j0 + lane;
-            bool keep, tie;
-            classify(j, &keep, &tie);
+        each([&](int j, uint32_t key) {
+            const uint32_t u = key >> shift;
+            const bool in = j < w1, forced = j < lo || j >= hi;
+            const bool keep = in && (forced || u > cut), tie = in && !forced && u == cut;
             const uint32_t below = (1u << lane) - 1, km = __ballot_sync(0xFFFFFFFFu, keep),
                            tm = __ballot_sync(0xFFFFFFFFu, tie);
             const int ties = tie_before + __popc(tm & below);
@@ -201,11 +220,11 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(const EvictArgs a, int 
             // a CTA that selects alone writes its own share
             if ((keep || (tie && ties < level)) && (kSliced || (slot >= m0 && slot < m1))) {
                 ids[slot] = j;
-                so[slot] = sc[j];
+                so[slot] = key_score(key);
             }
             keep_before += __popc(km);
             tie_before += __popc(tm);
-        }
+        });
     } else {
         for (int m = m0 + tid; m < m1 && m < kept; m += kThreads) {
             ids[m] = m;
@@ -295,8 +314,12 @@ int lsa_evict(const void* k, const void* v, int64_t row_bytes, const int64_t* st
     const bool sliced = T > kCached;
     int64_t ranks = 1;
     while (ranks < 16 && (units * ranks < 4 * 148 && capacity / (2 * ranks) >= 64)) ranks *= 2;
-    if (sliced)
-        while (ranks < 16 && (ranks < 2 || T / ranks > kCached / 2)) ranks *= 2;
+    if (sliced) {
+        // clusters of 8 (a cluster of 16 fills most of a GPC: 101 against 80 us for 32 rows of 131072
+        // keys), of 16 where the rows are few or the slices outgrow shared memory
+        ranks = 8;
+        if (units * ranks < 148 || T > 8 * kCached) ranks = 16;
+    }
     const int64_t slice = sliced ? (T + ranks - 1) / ranks : T;
     const int smem = (int)((slice < kCached ? slice : kCached) * 4);
     auto kern = sliced ? evict_kernel<true> : evict_kernel<false>;
