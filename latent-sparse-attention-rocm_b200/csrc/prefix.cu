@@ -162,39 +162,40 @@ constexpr int kWeightKeys = 1024;  // keys of a weights block: four a thread
 // Own keys' weights from the logits that the few-row kernel kept (4 bytes a row and key, 16 for a
 // decode step of 4 heads, against the 256 bytes of K that scoring the key again would read):
 //   w_j = sum over the rows r that see j of 2^(s_rj - lse_r).
-// One thread owns a key, so the sum has one order and one writer. The block joins its rows' lse
+// One thread owns four keys, so a sum has one order and one writer. The block joins its rows' lse
 // itself, beside the blocks that join the output: one launch for both.
-__device__ __forceinline__ void own_weights(const PrefixArgs& a, int parts, const float* __restrict__ logits,
+__device__ __forceinline__ void own_weights(const PrefixArgs& a, const RowsPlan& rp, int parts,
                                             const float* __restrict__ scores, float* __restrict__ scores_out) {
     __shared__ float slse[kMostFew];
     const int per = (int)(((int64_t)a.T + kWeightKeys - 1) / kWeightKeys);
     const int64_t bh = blockIdx.x / per;
     const int b = (int)(bh / a.Hkv), h = (int)(bh % a.Hkv), nrows = a.Tq * a.G, warp = threadIdx.x >> 5;
-    const int len = own_length(a, b), j0 = (blockIdx.x % per) * kWeightKeys;
+    const int len = own_length(a, b), j0 = (blockIdx.x % per) * kWeightKeys, j = j0 + 4 * (int)threadIdx.x;
+    float old[4], w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int u = 0; u < 4; ++u) old[u] = j + u < a.T ? scores[bh * a.T + j + u] : 0.0f;
     if (j0 < len) {
         for (int r = warp; r < nrows; r += 8) {
             const float x = joined_lse(a, row_index(a, (int64_t)b * a.Tq + r / a.G, h, r % a.G), parts);
             if ((threadIdx.x & 31) == 0) slse[r] = x;
         }
         __syncthreads();
-    }
-    float w[4] = {0, 0, 0, 0};
-    int j[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) j[u] = j0 + u * 256 + threadIdx.x;
-    if (j0 < len)
-        for (int r = 0; r < nrows; ++r) {
-            const float* src = logits + (bh * nrows + r) * a.T;
-            float s[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) s[u] = j[u] < len ? __ldcs(src + j[u]) : -INFINITY;
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (s[u] != -INFINITY) w[u] += exp2f(s[u] - slse[r]);  // -inf: the row does not see the key
+        if (j < len) {
+            const float* src = rp.logits + bh * nrows * rp.pitch + j;
+#pragma unroll 4
+            for (int r = 0; r < nrows; ++r) {
+                const float4 s = __ldcs(reinterpret_cast<const float4*>(src + r * rp.pitch));
+                const float l = slse[r];  // -inf: a row that sees no key, and whose logits are -inf
+                w[0] += s.x == -INFINITY ? 0.0f : exp2f(s.x - l);
+                w[1] += s.y == -INFINITY ? 0.0f : exp2f(s.y - l);
+                w[2] += s.z == -INFINITY ? 0.0f : exp2f(s.z - l);
+                w[3] += s.w == -INFINITY ? 0.0f : exp2f(s.w - l);
+            }
         }
+    }
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-        if (j[u] < a.T) scores_out[bh * a.T + j[u]] = scores[bh * a.T + j[u]] + w[u];
+        if (j + u < a.T) scores_out[bh * a.T + j + u] = j + u < len ? old[u] + w[u] : old[u];
 }
 
 // The parts of a row joined, one warp per row: every lane holds D / 32 columns. The lse of up to
@@ -203,14 +204,14 @@ __device__ __forceinline__ void own_weights(const PrefixArgs& a, int parts, cons
 // are, in their place: finite, times zero).
 template <typename T, int D>
 __global__ void __launch_bounds__(256) prefix_finish_kernel(const PrefixArgs a, const TilePlan tp, int parts,
-                                                            unsigned weight_blocks, const float* __restrict__ logits,
+                                                            const RowsPlan rp, unsigned weight_blocks,
                                                             const float* __restrict__ scores,
                                                             float* __restrict__ scores_out) {
     constexpr int E = D / 32, kPer = 4 * kMaxSplits / 32;
     grid_trigger();
     grid_wait();
     if (blockIdx.x < weight_blocks) {
-        own_weights(a, parts, logits, scores, scores_out);
+        own_weights(a, rp, parts, scores, scores_out);
         return;
     }
     int64_t row = (int64_t)(blockIdx.x - weight_blocks) * 8 + (threadIdx.x >> 5);
@@ -302,15 +303,15 @@ int launch_prefix_simt(const PrefixArgs& a, int D, cudaStream_t stream) {
 namespace {
 
 template <typename T>
-int finish_d(const PrefixArgs& a, const TilePlan& tp, int D, const float* logits, const float* scores,
+int finish_d(const PrefixArgs& a, const TilePlan& tp, int D, const RowsPlan& rp, const float* scores,
              float* scores_out, cudaStream_t stream) {
     const int64_t rows = tp.whole ? ((int64_t)a.B * a.Hkv * tp.seq_tiles - tp.whole) * 256 : a.rows;
     const int64_t blocks = (rows + 7) / 8;
-    const int64_t weights = logits ? (int64_t)a.B * a.Hkv * (((int64_t)a.T + kWeightKeys - 1) / kWeightKeys) : 0;
+    const int64_t weights = rp.logits ? (int64_t)a.B * a.Hkv * (((int64_t)a.T + kWeightKeys - 1) / kWeightKeys) : 0;
     if (blocks + weights > INT32_MAX) return LSA_ERR_SIZE;
     auto kern = D == 128 ? prefix_finish_kernel<T, 128> : prefix_finish_kernel<T, 64>;
-    return launch_after(kern, dim3((unsigned)(blocks + weights)), 256, 0, stream, a, tp, a.parts_p + a.parts_o,
-                        (unsigned)weights, logits, scores, scores_out);
+    return launch_after(kern, dim3((unsigned)(blocks + weights)), 256, 0, stream, a, tp, a.parts_p + a.parts_o, rp,
+                        (unsigned)weights, scores, scores_out);
 }
 
 struct Plan {
@@ -360,16 +361,7 @@ Plan make_plan(int dtype, int64_t B, int64_t Tq, int64_t Hkv, int64_t G, int64_t
         t.seq_items = (int)(t.whole + (seq - t.whole) * p.So);
         return p;
     }
-    if (B * rows <= kFewRows) {
-        p.parts_p = p.Sp = balance(Hkv, (P + 63) / 64, 2, 2 * kSMs);
-        p.rows.prefix_items = (int)(Hkv * p.Sp);
-    } else {
-        t.batch_streams = B * Tq <= t.tokens;
-        t.batch_tiles = (int)((B * Tq + 2 * t.tokens - 1) / (2 * t.tokens));
-        p.Sp = balance(Hkv * t.batch_tiles, t.batch_streams ? (pc + 1) / 2 : pc, 2, kSMs);
-        p.parts_p = p.Sp * (t.batch_streams ? 2 : 1);
-        t.batch_items = (int)(Hkv * t.batch_tiles * p.Sp);
-    }
+    double beside = 0;  // the few-row kernel's work on the own caches, in chunks of the tensor-core kernel a SM
     // few rows: the few-row kernel reads the keys once for each 16 of them, from L2 after the first
     // time, and has no fixed cost to speak of; a tensor-core item spends about 6 us, 32 MB of keys
     const int64_t tiles = (rows + kFewRows - 1) / kFewRows;
@@ -377,12 +369,25 @@ Plan make_plan(int dtype, int64_t B, int64_t Tq, int64_t Hkv, int64_t G, int64_t
         p.rows.own_tiles = (int)tiles;
         p.parts_o = p.So = balance(B * Hkv * tiles, (T + 63) / 64, 2, 2 * kSMs);
         p.rows.own_items = (int)(B * Hkv * tiles * p.So);
-        p.rows.follows = t.batch_items > 0;
+        // about 6 MB of keys a microsecond, caches three quarters full; a chunk takes 1.6 us
+        beside = 0.75 * (double)(B * T * Hkv * D * 4) / 6e6 / 1.6;
+        p.rows.pitch = (T + 15) / 16 * 16;
         p.logits = scored;
     } else {
         p.So = balance(seq, t.seq_streams ? (oc + 1) / 2 : oc, 2, kSMs);
         p.parts_o = p.So * (t.seq_streams ? 2 : 1);
         t.seq_items = (int)(seq * p.So);
+    }
+    if (B * rows <= kFewRows) {
+        p.parts_p = p.Sp = balance(Hkv, (P + 63) / 64, 2, 2 * kSMs);
+        p.rows.prefix_items = (int)(Hkv * p.Sp);
+    } else {
+        t.batch_streams = B * Tq <= t.tokens;
+        t.batch_tiles = (int)((B * Tq + 2 * t.tokens - 1) / (2 * t.tokens));
+        p.Sp = balance_beside(Hkv * t.batch_tiles, t.batch_streams ? (pc + 1) / 2 : pc, 4, kSMs, beside);
+        p.parts_p = p.Sp * (t.batch_streams ? 2 : 1);
+        t.batch_items = (int)(Hkv * t.batch_tiles * p.Sp);
+        p.rows.follows = t.batch_items > 0;
     }
     return p;
 }
@@ -399,11 +404,11 @@ int64_t round256(int64_t x) { return (x + 255) / 256 * 256; }
 
 }  // namespace
 
-int launch_prefix_finish(const PrefixArgs& a, const TilePlan& tp, int dtype, int D, const float* logits,
+int launch_prefix_finish(const PrefixArgs& a, const TilePlan& tp, int dtype, int D, const RowsPlan& rp,
                          const float* scores, float* scores_out, cudaStream_t stream) {
-    if (dtype == kF32) return finish_d<float>(a, tp, D, logits, scores, scores_out, stream);
-    if (dtype == kF16) return finish_d<__half>(a, tp, D, logits, scores, scores_out, stream);
-    return finish_d<__nv_bfloat16>(a, tp, D, logits, scores, scores_out, stream);
+    if (dtype == kF32) return finish_d<float>(a, tp, D, rp, scores, scores_out, stream);
+    if (dtype == kF16) return finish_d<__half>(a, tp, D, rp, scores, scores_out, stream);
+    return finish_d<__nv_bfloat16>(a, tp, D, rp, scores, scores_out, stream);
 }
 
 }  // namespace lsa
@@ -420,7 +425,7 @@ int64_t lsa_shared_prefix_scratch(int dtype, int64_t B, int64_t Tq, int64_t Hq, 
     const int64_t rows = B * Tq * Hq;
     const int64_t parts = p.parts_p + p.parts_o;
     return round256(parts * rows * D * 4) + round256(parts * rows * 4) + round256(rows * 4) +
-           (p.logits ? round256(rows * T * 4) : 0);
+           (p.logits ? round256(rows * p.rows.pitch * 4) : 0);
 }
 
 int lsa_shared_prefix_attention(const void* q, const void* k_prefix, const void* v_prefix, const void* k,
@@ -473,7 +478,7 @@ int lsa_shared_prefix_attention(const void* q, const void* k_prefix, const void*
     s += round256((p.parts_p + p.parts_o) * a.rows * 4);
     a.lse2 = reinterpret_cast<float*>(s);
     RowsPlan few = p.rows;
-    if (p.logits) few.logits = reinterpret_cast<float*>(s + round256(a.rows * 4));
+    if (p.logits && T > 0) few.logits = reinterpret_cast<float*>(s + round256(a.rows * 4));
     int rc = LSA_OK;
     if (p.simt) {
         rc = launch_prefix_simt(a, (int)D, stream);
@@ -482,7 +487,7 @@ int lsa_shared_prefix_attention(const void* q, const void* k_prefix, const void*
         if (rc == LSA_OK) rc = launch_prefix_rows(a, few, dtype, (int)D, stream);
     }
     if (rc == LSA_OK && p.merge)
-        rc = launch_prefix_finish(a, p.tile, dtype, (int)D, T > 0 ? few.logits : nullptr, scores, scores_out, stream);
+        rc = launch_prefix_finish(a, p.tile, dtype, (int)D, few, scores, scores_out, stream);
     if (rc == LSA_OK && scores && T > 0 && !p.logits)
         rc = p.simt ? launch_own_weights(a, (int)D, scores, scores_out, stream)
                     : launch_tile_weights(a, dtype, (int)D, scores, scores_out, stream);

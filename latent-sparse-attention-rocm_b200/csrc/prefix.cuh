@@ -114,6 +114,22 @@ inline int balance(int64_t items, int64_t chunks, double fixed, int64_t slots) {
     return best;
 }
 
+// The same for work that shares the GPU with `beside` chunks' worth of other work per place, which
+// starts on the places left free: the least of the longer of its own rounds and all the work together.
+inline int balance_beside(int64_t items, int64_t chunks, double fixed, int64_t slots, double beside) {
+    if (chunks == 0) return 0;
+    int best = 1;
+    double least = 1e300;
+    for (int s = 1; s <= kMaxSplits && s <= chunks; ++s) {
+        const double one = (double)chunks / s + fixed;
+        const double alone = (double)((items * s + slots - 1) / slots) * one;
+        const double all = (double)(items * s) * one / slots + beside;
+        const double cost = alone > all ? alone : all;
+        if (cost < 0.99 * least) least = cost, best = s;
+    }
+    return best;
+}
+
 // own keys that sequence b holds
 __device__ __forceinline__ int own_length(const PrefixArgs& a, int b) {
     const int n = a.lengths[b];
@@ -139,14 +155,15 @@ struct RowsPlan {
     int prefix_items, own_items;
     int own_tiles;  // row tiles of a sequence (the prefix's rows are one tile)
     bool follows;   // launched behind this call's tensor-core kernel, whose output it does not read
-    float* logits;  // [B, Hkv, Tq * G, T] log2-domain logits of the own keys, or null
+    int64_t pitch;  // T to whole tiles of 16 keys
+    float* logits;  // [B, Hkv, Tq * G, pitch] log2-domain logits of the own keys, or null
 };
 
 int launch_prefix_simt(const PrefixArgs& a, int D, cudaStream_t stream);  // fp32 inputs
 int launch_prefix_tiles(const PrefixArgs& a, const TilePlan& tp, int dtype, int D, cudaStream_t stream);
 int launch_prefix_rows(const PrefixArgs& a, const RowsPlan& rp, int dtype, int D, cudaStream_t stream);
 // The parts joined; with logits (few-row kernel) also the own keys' weights, in the same launch.
-int launch_prefix_finish(const PrefixArgs& a, const TilePlan& tp, int dtype, int D, const float* logits,
+int launch_prefix_finish(const PrefixArgs& a, const TilePlan& tp, int dtype, int D, const RowsPlan& rp,
                          const float* scores, float* scores_out, cudaStream_t stream);
 int launch_own_weights(const PrefixArgs& a, int D, const float* scores, float* scores_out, cudaStream_t stream);
 int launch_tile_weights(const PrefixArgs& a, int dtype, int D, const float* scores, float* scores_out,

@@ -70,7 +70,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) prefix_rows_kernel(const Prefi
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // Behind the call's tensor-core kernel (which waited for everything before the call) this one
-    // starts as that one's CTAs leave; what follows needs both, so the wait comes last.
+    // starts on what that one leaves free; what follows needs both, so one CTA, the last, waits for it
+    // at its end (a wait of every CTA would keep their places until then).
     if (!rp.follows) grid_wait();
     grid_trigger();
     int item = blockIdx.x;
@@ -147,7 +148,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) prefix_rows_kernel(const Prefi
         for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
     float* logits = own && rp.logits
-                        ? rp.logits + (((int64_t)b * a.Hkv + h) * nrows + r0 + quad) * a.T
+                        ? rp.logits + (((int64_t)b * a.Hkv + h) * nrows + r0 + quad) * rp.pitch
                         : nullptr;
 
     for (int i = 0; i < tiles; ++i) {
@@ -172,17 +173,14 @@ __global__ void __launch_bounds__(kWarps * 32, 2) prefix_rows_kernel(const Prefi
                 const int key = key0 + t * 8 + qc + (e & 1);
                 s[t][e] = key < k1 && key < limit[e >> 1] ? s[t][e] * a.scale_log2 : -INFINITY;
             }
-        if (logits) {
+        if (logits) {  // whole 32-byte sectors: four lanes a row; the rows' pitch covers a last, ragged tile
 #pragma unroll
             for (int u = 0; u < 2; ++u)
                 if (r0 + quad + 8 * u < nrows)
 #pragma unroll
                     for (int t = 0; t < 2; ++t)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const int key = key0 + t * 8 + qc + e;
-                            if (key < k1) logits[(int64_t)8 * u * a.T + key] = s[t][2 * u + e];
-                        }
+                        *reinterpret_cast<float2*>(logits + (int64_t)8 * u * rp.pitch + key0 + t * 8 + qc) =
+                            make_float2(s[t][2 * u], s[t][2 * u + 1]);
         }
         float mx[2];
 #pragma unroll
@@ -266,7 +264,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) prefix_rows_kernel(const Prefi
         if (c == 0) a.part_lse[at] = total > 0.0f ? top + log2f(total) : -INFINITY;
         *reinterpret_cast<float4*>(a.part_o + at * D + c) = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
     }
-    if (rp.follows) grid_wait();
+    if (rp.follows && blockIdx.x == gridDim.x - 1) grid_wait();
 }
 
 template <typename T, int D>

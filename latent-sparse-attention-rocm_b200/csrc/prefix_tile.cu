@@ -214,8 +214,9 @@ __device__ __forceinline__ void softmax_half(const PrefixArgs& a, const TilePlan
     if (ok && n > 0) ok = role_wait(&bar_o[hf], 0, abort_flag);
     if (!ok) return;
     const int64_t rid = row_index(a, (int64_t)w.b * a.Tq + tok, w.h, g);
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    const float lse = l > 0.0f ? m * sl + log2f(l) : -INFINITY;
+    const bool some = m != -INFINITY;  // the row has seen a key
+    const float inv = some ? 1.0f / l : 0.0f;
+    const float lse = some ? m * sl + log2f(l) : -INFINITY;
     const int64_t at = (int64_t)(w.part + (w.streams ? hf : 0)) * a.rows + rid;
     if (live) {
         if (w.direct) {

@@ -29,15 +29,18 @@ __device__ __forceinline__ bool role_wait(uint64_t* bar, uint32_t parity, volati
     }
 }
 
-// The same for a role that is one thread.
+// The same for a role that is one thread; the flag and the clock are looked at now and then.
 __device__ __forceinline__ bool thread_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const uint64_t t0 = global_ns();
-    for (;;) {
+    uint64_t t0 = 0;
+    for (int i = 0;; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
-        if (*abort_flag != 0 || global_ns() - t0 > kRoleWaitNs) {
-            *abort_flag = 1;
-            return false;
+        if ((i & 15) == 15) {
+            const uint64_t now = global_ns();
+            if (t0 == 0) t0 = now;
+            if (*abort_flag != 0 || now - t0 > kRoleWaitNs) {
+                *abort_flag = 1;
+                return false;
+            }
         }
     }
 }
