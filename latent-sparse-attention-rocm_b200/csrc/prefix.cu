@@ -138,20 +138,25 @@ __global__ void __launch_bounds__(kSimtWarps * 32) prefix_simt_kernel(const Pref
     }
 }
 
+constexpr int kPer = kMaxParts / 32;  // parts of a row that a lane holds
+
 // The lse of a row from its parts, by one warp (log2 domain; every lane has it).
 __device__ __forceinline__ float joined_lse(const PrefixArgs& a, int64_t row, int parts) {
     const int lane = threadIdx.x & 31;
-    float x[4 * kMaxSplits / 32], top = -INFINITY, sum = 0.0f;
+    float x[kPer], top = -INFINITY, sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4 * kMaxSplits / 32; ++i) {
-        x[i] = lane + 32 * i < parts ? a.part_lse[(int64_t)(lane + 32 * i) * a.rows + row] : -INFINITY;
-        top = fmaxf(top, x[i]);
+    for (int i = 0; i < kPer; ++i) {
+        x[i] = -INFINITY;
+        if (32 * i < parts && lane + 32 * i < parts) x[i] = a.part_lse[(int64_t)(lane + 32 * i) * a.rows + row];
     }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) top = fmaxf(top, x[i]);
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
     if (top == -INFINITY) return top;
 #pragma unroll
-    for (int i = 0; i < 4 * kMaxSplits / 32; ++i) sum += exp2f(x[i] - top);
+    for (int i = 0; i < kPer; ++i)
+        if (32 * i < parts) sum += exp2f(x[i] - top);
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, off);
     return top + log2f(sum);
@@ -175,21 +180,30 @@ __device__ __forceinline__ void own_weights(const PrefixArgs& a, const RowsPlan&
 #pragma unroll
     for (int u = 0; u < 4; ++u) old[u] = j + u < a.T ? scores[bh * a.T + j + u] : 0.0f;
     if (j0 < len) {
+        // the first rows' logits are on their way while the lse are joined
+        const float* src = rp.logits + bh * nrows * rp.pitch + (j < len ? j : j0);
+        float4 s[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) s[u] = __ldcs(reinterpret_cast<const float4*>(src + (u < nrows ? u : 0) * rp.pitch));
         for (int r = warp; r < nrows; r += 8) {
             const float x = joined_lse(a, row_index(a, (int64_t)b * a.Tq + r / a.G, h, r % a.G), parts);
             if ((threadIdx.x & 31) == 0) slse[r] = x;
         }
         __syncthreads();
-        if (j < len) {
-            const float* src = rp.logits + bh * nrows * rp.pitch + j;
-#pragma unroll 4
-            for (int r = 0; r < nrows; ++r) {
-                const float4 s = __ldcs(reinterpret_cast<const float4*>(src + r * rp.pitch));
-                const float l = slse[r];  // -inf: a row that sees no key, and whose logits are -inf
-                w[0] += s.x == -INFINITY ? 0.0f : exp2f(s.x - l);
-                w[1] += s.y == -INFINITY ? 0.0f : exp2f(s.y - l);
-                w[2] += s.z == -INFINITY ? 0.0f : exp2f(s.z - l);
-                w[3] += s.w == -INFINITY ? 0.0f : exp2f(s.w - l);
+        for (int r0 = 0; r0 < nrows; r0 += 4) {
+            if (r0) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    s[u] = __ldcs(reinterpret_cast<const float4*>(src + (r0 + u < nrows ? r0 + u : 0) * rp.pitch));
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (r0 + u >= nrows) break;
+                const float l = slse[r0 + u];  // -inf: a row that sees no key, and whose logits are -inf
+                w[0] += s[u].x == -INFINITY ? 0.0f : exp2f(s[u].x - l);
+                w[1] += s[u].y == -INFINITY ? 0.0f : exp2f(s[u].y - l);
+                w[2] += s[u].z == -INFINITY ? 0.0f : exp2f(s[u].z - l);
+                w[3] += s[u].w == -INFINITY ? 0.0f : exp2f(s[u].w - l);
             }
         }
     }
@@ -198,8 +212,8 @@ __device__ __forceinline__ void own_weights(const PrefixArgs& a, const RowsPlan&
         if (j + u < a.T) scores_out[bh * a.T + j + u] = j + u < len ? old[u] + w[u] : old[u];
 }
 
-// The parts of a row joined, one warp per row: every lane holds D / 32 columns. The lse of up to
-// 128 parts are loaded at once, then the parts' columns eight loads at a time; a part without a
+// The parts of a row joined, one warp per row: every lane holds D / 32 columns. The lse of all
+// parts are loaded at once, then the parts' columns eight loads at a time; a part without a
 // key (lse -inf) has weight zero and its columns, never written, are not read (the heaviest part's
 // are, in their place: finite, times zero).
 template <typename T, int D>
@@ -207,7 +221,7 @@ __global__ void __launch_bounds__(256) prefix_finish_kernel(const PrefixArgs a, 
                                                             const RowsPlan rp, unsigned weight_blocks,
                                                             const float* __restrict__ scores,
                                                             float* __restrict__ scores_out) {
-    constexpr int E = D / 32, kPer = 4 * kMaxSplits / 32;
+    constexpr int E = D / 32;
     grid_trigger();
     grid_wait();
     if (blockIdx.x < weight_blocks) {
@@ -227,8 +241,10 @@ __global__ void __launch_bounds__(256) prefix_finish_kernel(const PrefixArgs a, 
     if (row >= a.rows) return;
     float x[kPer];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
-        x[i] = lane + 32 * i < parts ? a.part_lse[(int64_t)(lane + 32 * i) * a.rows + row] : -INFINITY;
+    for (int i = 0; i < kPer; ++i) {
+        x[i] = -INFINITY;
+        if (32 * i < parts && lane + 32 * i < parts) x[i] = a.part_lse[(int64_t)(lane + 32 * i) * a.rows + row];
+    }
     float top = x[0];
 #pragma unroll
     for (int i = 1; i < kPer; ++i) top = fmaxf(top, x[i]);
@@ -323,6 +339,21 @@ struct Plan {
 };
 
 constexpr int kSMs = 148;
+constexpr int kItemsAPlace = 2;
+
+// Splits of the few-row kernel for `items` of `chunks` steps of 64 keys. One length: 256 CTAs draw the
+// memory's whole bandwidth, and more parts cost more to join (one sequence of 24k keys, 8 KV heads: 24.2
+// us in 32 parts, 25.6 in 37). Many sequences, of lengths that the host does not know: several
+// items a place, so that the long ones even out (one of 64k keys among four of 14k on average: 125 us with
+// one item a place, 85 with two).
+int few_splits(int64_t items, int64_t chunks, bool ragged) {
+    if (chunks == 0) return 0;
+    int64_t s = ragged ? (kItemsAPlace * 2 * kSMs + items / 2) / items : 256 / items;
+    const int64_t most = items * kMaxSplits >= 256 ? kMaxSplits : 3 * kMaxSplits;
+    if (s > most) s = most;
+    if (s > chunks / 4) s = chunks / 4;
+    return (int)(s < 1 ? 1 : s);
+}
 
 Plan make_plan(int dtype, int64_t B, int64_t Tq, int64_t Hkv, int64_t G, int64_t D, int64_t P, int64_t T, bool scored) {
     Plan p = {};
@@ -354,7 +385,7 @@ Plan make_plan(int dtype, int64_t B, int64_t Tq, int64_t Hkv, int64_t G, int64_t
         // of the last, short round are, so that it too fills the GPU
         t.whole = (int)(seq / kSMs * kSMs);
         const int64_t rest = seq - t.whole;
-        p.So = rest ? balance(rest, pc + oc, 2, kSMs) : 1;
+        p.So = rest ? balance(rest, pc + oc, 4, kSMs, kMaxSplits) : 1;
         if (p.So == 1) t.whole = (int)seq;
         p.merge = p.So > 1;
         p.parts_o = p.merge ? p.So : 0;
@@ -367,19 +398,19 @@ Plan make_plan(int dtype, int64_t B, int64_t Tq, int64_t Hkv, int64_t G, int64_t
     const int64_t tiles = (rows + kFewRows - 1) / kFewRows;
     if (tiles == 1 || (rows <= kMostFew && (tiles - 1) * B * T * Hkv * D * 4 <= 32 << 20)) {
         p.rows.own_tiles = (int)tiles;
-        p.parts_o = p.So = balance(B * Hkv * tiles, (T + 63) / 64, 2, 2 * kSMs);
+        p.parts_o = p.So = few_splits(B * Hkv * tiles, (T + 63) / 64, B > 1);
         p.rows.own_items = (int)(B * Hkv * tiles * p.So);
         // about 6 MB of keys a microsecond, caches three quarters full; a chunk takes 1.6 us
         beside = 0.75 * (double)(B * T * Hkv * D * 4) / 6e6 / 1.6;
         p.rows.pitch = (T + 15) / 16 * 16;
         p.logits = scored;
     } else {
-        p.So = balance(seq, t.seq_streams ? (oc + 1) / 2 : oc, 2, kSMs);
+        p.So = balance(seq, t.seq_streams ? (oc + 1) / 2 : oc, 4, kSMs, kMaxSplits);
         p.parts_o = p.So * (t.seq_streams ? 2 : 1);
         t.seq_items = (int)(seq * p.So);
     }
     if (B * rows <= kFewRows) {
-        p.parts_p = p.Sp = balance(Hkv, (P + 63) / 64, 2, 2 * kSMs);
+        p.parts_p = p.Sp = few_splits(Hkv, (P + 63) / 64, false);
         p.rows.prefix_items = (int)(Hkv * p.Sp);
     } else {
         t.batch_streams = B * Tq <= t.tokens;
@@ -446,7 +477,8 @@ int lsa_shared_prefix_attention(const void* q, const void* k_prefix, const void*
                           (const void*)out, (const void*)scratch})
         if ((uintptr_t)p & 15) return LSA_ERR_ARG;
     // a dimension of one entry takes any stride: D stands for it
-    const int64_t extent[13] = {B, Tq, Hq, P, Hkv, P, Hkv, B, T, Hkv, B, T, Hkv};
+    const int64_t ph = P ? Hkv : 1, ob = T ? B : 1, oh = T ? Hkv : 1;  // nor do the strides of nothing matter
+    const int64_t extent[13] = {B, Tq, Hq, P, ph, P, ph, ob, T, oh, ob, T, oh};
     int64_t st[13];
     for (int i = 0; i < 13; ++i) {
         st[i] = extent[i] > 1 ? strides[i] : D;

@@ -19,7 +19,8 @@
 
 namespace lsa {
 
-constexpr int kMaxSplits = 32;  // of the prefix, and of the own caches
+constexpr int kMaxSplits = 32;  // of the prefix, and of the own caches (few rows: three times that)
+constexpr int kMaxParts = 256;  // of a row: at most 96 + 96, or 64 + 64 (two parts a split), or 96 + 64
 
 // strides in elements; the last dimension is contiguous everywhere
 struct PrefixArgs {
@@ -103,11 +104,11 @@ template <auto kKernel> bool allow_smem(int bytes) {
 
 // Splits of `chunks` for `items` equal work items on `slots` places that hold one item each: the
 // fewest that minimise rounds x (chunks of an item + its fixed cost in chunks).
-inline int balance(int64_t items, int64_t chunks, double fixed, int64_t slots) {
+inline int balance(int64_t items, int64_t chunks, double fixed, int64_t slots, int most) {
     if (chunks == 0) return 0;
     int best = 1;
     double least = 1e300;
-    for (int s = 1; s <= kMaxSplits && s <= chunks; ++s) {
+    for (int s = 1; s <= most && s <= chunks; ++s) {
         const double cost = (double)((items * s + slots - 1) / slots) * ((double)chunks / s + fixed);
         if (cost < 0.99 * least) least = cost, best = s;
     }

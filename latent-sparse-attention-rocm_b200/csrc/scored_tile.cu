@@ -121,7 +121,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (resident && p0 < p1)
             for (int t = 0; t < nr; ++t) load_q(t);
         for (int p = p0; ok && p < p1; ++p) {
-            ok = load_k(2 * p) && load_k(2 * p + 1);
+            const int q = p0 + p1 - 1 - p;  // from the end: what the attention pass read last is still in L2
+            ok = load_k(2 * q) && load_k(2 * q + 1);
             if (!resident)
                 for (int t = 0; ok && t < nr; ++t) ok = load_q(t);
         }
@@ -192,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool ok = true;
         int it = 0;
         for (int p = p0; p < p1; ++p) {  // to the end also after an expired wait: the group's barriers pair up
-            const int j = (2 * p + g) * kChunk + tid;
+            const int j = (2 * (p0 + p1 - 1 - p) + g) * kChunk + tid;
             const float old = j < len ? scores[bh + j] : 0.0f;
             // rows before this one do not see key j
             const int64_t first = ((int64_t)j - (len - a.Tq)) * a.G;
@@ -271,7 +272,7 @@ int launch_tile_weights(const PrefixArgs& a, int dtype, int D, const float* scor
     wp.row_tiles = (a.Tq + wp.tokens - 1) / wp.tokens;
     // one CTA an SM: the splits that fill whole rounds best, each of at least two pairs of key tiles
     const int64_t units = (int64_t)a.B * a.Hkv, pairs = ((int64_t)a.T + 2 * kChunk - 1) / (2 * kChunk);
-    wp.splits = balance(units, (pairs + 1) / 2, 1, 148);
+    wp.splits = balance(units, (pairs + 1) / 2, 2, 148, 4 * kMaxSplits);
     if (units * wp.splits > INT32_MAX) return LSA_ERR_SIZE;
     WeightMaps maps;
     const bool bf = dtype == kBF16;

@@ -9,7 +9,7 @@
 //                     (index_queries [R, d], or raw queries [R, Hq, D]: regroup fused in)
 //   lsa::sparse_read(q, k, v, ids, lengths, scale) -> out     sparse_read_auto, read_kernel_tiled.py:147
 //   lsa::shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths, scale, return_lse) -> (out, lse)
-//   lsa::scored_attention(q, k_prefix, v_prefix, k, v, lengths, scores, scale) -> (out, scores)
+//   lsa::scored_attention(q, k, v, lengths, scores, scale, k_prefix, v_prefix) -> (out, scores)
 //   lsa::evict(k, v, scores, lengths, budget, window, sink, capacity)
 //                     -> (k, v, scores, lengths, ids)            no reference counterpart
 //   lsa::workspace_counters() -> Tensor[]                      the cached counter buffers (checks)
@@ -24,6 +24,7 @@
 #include <cmath>
 #include <map>
 #include <mutex>
+#include <optional>
 #include <tuple>
 #include <vector>
 
@@ -200,37 +201,47 @@ at::Tensor rows16(const at::Tensor& t) {
 // stride of a dimension; 0 where the dimension has one entry and any stride would do
 int64_t stride_of(const at::Tensor& t, int64_t i) { return t.size(i) == 1 ? 0 : t.stride(i); }
 
+at::Tensor as_lengths(const at::Tensor& t) {
+    return t.scalar_type() == at::kInt && t.is_contiguous() ? t : t.to(at::kInt).contiguous();
+}
+
 struct PrefixOut {
     at::Tensor out, lse, scores;
 };
 
-PrefixOut prefix_attention(const at::Tensor& q_in, const at::Tensor& kp_in, const at::Tensor& vp_in,
+PrefixOut prefix_attention(const at::Tensor& q_in, const at::Tensor* kp_in, const at::Tensor* vp_in,
                            const at::Tensor& k_in, const at::Tensor& v_in, const at::Tensor& lengths_in,
                            const at::Tensor* scores_in, double scale, bool want_lse, const char* what) {
-    for (const at::Tensor* t : {&q_in, &kp_in, &vp_in, &k_in, &v_in, &lengths_in})
-        TORCH_CHECK_VALUE(t->is_cuda() && t->device() == q_in.device(), what,
-                          " is a CUDA kernel: every tensor on one CUDA device");
+    TORCH_CHECK_VALUE((kp_in == nullptr) == (vp_in == nullptr), what, ": a prefix has keys and values");
+    for (const at::Tensor* t : {&q_in, kp_in, vp_in, &k_in, &v_in, &lengths_in})
+        TORCH_CHECK_VALUE(t == nullptr || (t->is_cuda() && t->device() == q_in.device()), what,
+                          " is a CUDA kernel (B200, sm_100a): every tensor on one CUDA device");
     TORCH_CHECK_VALUE(q_in.dim() == 4 && k_in.dim() == 4 && v_in.sizes() == k_in.sizes(), what,
                       ": q [B, Tq, Hq, D], k / v [B, T, Hkv, D]");
-    TORCH_CHECK_VALUE(kp_in.dim() == 3 && vp_in.sizes() == kp_in.sizes(), what, ": k_prefix / v_prefix [P, Hkv, D]");
+    TORCH_CHECK_VALUE(kp_in == nullptr || (kp_in->dim() == 3 && vp_in->sizes() == kp_in->sizes()), what,
+                      ": k_prefix / v_prefix [P, Hkv, D]");
     const int64_t B = q_in.size(0), Tq = q_in.size(1), Hq = q_in.size(2), D = q_in.size(3);
-    const int64_t T = k_in.size(1), Hkv = k_in.size(2), P = kp_in.size(0);
-    TORCH_CHECK_VALUE(k_in.size(0) == B && k_in.size(3) == D && kp_in.size(1) == Hkv && kp_in.size(2) == D, what,
+    const int64_t T = k_in.size(1), Hkv = k_in.size(2), P = kp_in ? kp_in->size(0) : 0;
+    TORCH_CHECK_VALUE(k_in.size(0) == B && k_in.size(3) == D &&
+                          (kp_in == nullptr || (kp_in->size(1) == Hkv && kp_in->size(2) == D)),
+                      what,
                       ": batch, KV heads and head dim of q, the prefix and the own caches differ");
     TORCH_CHECK_VALUE(Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && Hq / Hkv <= 64, what,
                       ": query heads must group evenly onto KV heads, at most 64 to one");
     TORCH_CHECK_VALUE(D == 64 || D == 128, what, ": head dim 64 or 128, got ", D);
-    for (const at::Tensor* t : {&kp_in, &vp_in, &k_in, &v_in})
-        TORCH_CHECK_VALUE(t->scalar_type() == q_in.scalar_type(), what, ": q, the prefix and the caches share a dtype");
+    for (const at::Tensor* t : {kp_in, vp_in, &k_in, &v_in})
+        TORCH_CHECK_VALUE(t == nullptr || t->scalar_type() == q_in.scalar_type(), what, ": q, the prefix and the caches share a dtype");
     TORCH_CHECK_VALUE(q_in.scalar_type() == at::kFloat || q_in.scalar_type() == at::kHalf ||
                           q_in.scalar_type() == at::kBFloat16,
                       what, ": fp32, fp16 or bf16, got ", q_in.scalar_type());
     TORCH_CHECK_VALUE(lengths_in.numel() == B && !lengths_in.is_floating_point(), what, ": one whole length a sequence");
     TORCH_CHECK_VALUE(std::isfinite(scale) && scale > 0, what, ": the scale must be positive, got ", scale);
     c10::cuda::CUDAGuard guard(q_in.device());
-    auto q = rows16(q_in), kp = rows16(kp_in), vp = rows16(vp_in), k = rows16(k_in), v = rows16(v_in);
+    auto q = rows16(q_in), k = rows16(k_in), v = rows16(v_in);
+    at::Tensor kp, vp;
+    if (P > 0) kp = rows16(*kp_in), vp = rows16(*vp_in);
     if (B > 1 && Tq > 1 && q.stride(0) != Tq * q.stride(1)) q = q.contiguous();  // tokens one stride apart
-    auto lengths = lengths_in.to(at::kInt).contiguous();
+    auto lengths = as_lengths(lengths_in);
     PrefixOut r;
     r.out = at::empty({B, Tq, Hq, D}, q.options());
     if (want_lse) r.lse = at::empty({B, Tq, Hq}, q.options().dtype(at::kFloat));
@@ -249,10 +260,12 @@ PrefixOut prefix_attention(const at::Tensor& q_in, const at::Tensor& kp_in, cons
     TORCH_CHECK_VALUE(bytes >= 0, what, ": sizes out of range");
     auto stream = at::cuda::getCurrentCUDAStream();
     Workspace& w = workspace(q.device(), stream, bytes, 64);
-    const int64_t strides[13] = {stride_of(q, 0), stride_of(q, 1), stride_of(q, 2), stride_of(kp, 0), stride_of(kp, 1),
-                                 stride_of(vp, 0), stride_of(vp, 1), stride_of(k, 0), stride_of(k, 1),
+    const int64_t strides[13] = {stride_of(q, 0), stride_of(q, 1), stride_of(q, 2), P ? stride_of(kp, 0) : 0,
+                                 P ? stride_of(kp, 1) : 0, P ? stride_of(vp, 0) : 0, P ? stride_of(vp, 1) : 0,
+                                 stride_of(k, 0), stride_of(k, 1),
                                  stride_of(k, 2), stride_of(v, 0), stride_of(v, 1), stride_of(v, 2)};
-    check_rc(lsa_shared_prefix_attention(q.data_ptr(), kp.data_ptr(), vp.data_ptr(), k.data_ptr(), v.data_ptr(), code,
+    check_rc(lsa_shared_prefix_attention(q.data_ptr(), P ? kp.data_ptr() : nullptr, P ? vp.data_ptr() : nullptr,
+                                         k.data_ptr(), v.data_ptr(), code,
                                          strides, lengths.data_ptr<int32_t>(), B, Tq, Hq, Hkv, D, P, T, (float)scale,
                                          r.out.data_ptr(), want_lse ? r.lse.data_ptr<float>() : nullptr,
                                          scores_in ? scores.data_ptr<float>() : nullptr,
@@ -265,14 +278,16 @@ PrefixOut prefix_attention(const at::Tensor& q_in, const at::Tensor& kp_in, cons
 std::tuple<at::Tensor, at::Tensor> shared_prefix_cuda(const at::Tensor& q, const at::Tensor& kp, const at::Tensor& vp,
                                                       const at::Tensor& k, const at::Tensor& v,
                                                       const at::Tensor& lengths, double scale, bool return_lse) {
-    auto r = prefix_attention(q, kp, vp, k, v, lengths, nullptr, scale, return_lse, "shared_prefix_attention");
+    auto r = prefix_attention(q, &kp, &vp, k, v, lengths, nullptr, scale, return_lse, "shared_prefix_attention");
     return {r.out, return_lse ? r.lse : at::empty({0}, q.options().dtype(at::kFloat))};
 }
 
-std::tuple<at::Tensor, at::Tensor> scored_cuda(const at::Tensor& q, const at::Tensor& kp, const at::Tensor& vp,
-                                               const at::Tensor& k, const at::Tensor& v, const at::Tensor& lengths,
-                                               const at::Tensor& scores, double scale) {
-    auto r = prefix_attention(q, kp, vp, k, v, lengths, &scores, scale, false, "scored_attention");
+std::tuple<at::Tensor, at::Tensor> scored_cuda(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                               const at::Tensor& lengths, const at::Tensor& scores, double scale,
+                                               const std::optional<at::Tensor>& kp,
+                                               const std::optional<at::Tensor>& vp) {
+    auto r = prefix_attention(q, kp ? &*kp : nullptr, vp ? &*vp : nullptr, k, v, lengths, &scores, scale, false,
+                              "scored_attention");
     return {r.out, r.scores};
 }
 
@@ -281,7 +296,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> evict_cud
     int64_t budget, int64_t window, int64_t sink, int64_t capacity) {
     for (const at::Tensor* t : {&k_in, &v_in, &scores_in, &lengths_in})
         TORCH_CHECK_VALUE(t->is_cuda() && t->device() == k_in.device(),
-                          "evict is a CUDA kernel: every tensor on one CUDA device");
+                          "evict is a CUDA kernel (B200, sm_100a): every tensor on one CUDA device");
     TORCH_CHECK_VALUE(k_in.dim() == 4 && v_in.sizes() == k_in.sizes() && v_in.scalar_type() == k_in.scalar_type(),
                       "evict: k / v [B, T, Hkv, D] of one dtype");
     const int64_t B = k_in.size(0), T = k_in.size(1), Hkv = k_in.size(2), D = k_in.size(3), es = k_in.element_size();
@@ -296,7 +311,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> evict_cud
     c10::cuda::CUDAGuard guard(k_in.device());
     auto k = rows16(k_in), v = rows16(v_in);
     auto scores = scores_in.contiguous();
-    auto lengths = lengths_in.to(at::kInt).contiguous();
+    auto lengths = as_lengths(lengths_in);
     auto ko = at::empty({B, capacity, Hkv, D}, k.options()), vo = at::empty({B, capacity, Hkv, D}, k.options());
     auto so = at::empty({B, Hkv, capacity}, scores.options());
     auto lo = at::empty({B}, lengths.options()), ids = at::empty({B, Hkv, capacity}, lengths.options());
@@ -347,8 +362,8 @@ std::tuple<at::Tensor, at::Tensor> shared_prefix_meta(const at::Tensor& q, const
 }
 
 std::tuple<at::Tensor, at::Tensor> scored_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor&,
-                                               const at::Tensor&, const at::Tensor&, const at::Tensor&,
-                                               const at::Tensor& scores, double) {
+                                               const at::Tensor&, const at::Tensor& scores, double,
+                                               const std::optional<at::Tensor>&, const std::optional<at::Tensor>&) {
     return {at::empty(q.sizes(), q.options()), at::empty(scores.sizes(), scores.options())};
 }
 
@@ -371,8 +386,8 @@ TORCH_LIBRARY(lsa, m) {
     m.def("sparse_read(Tensor q, Tensor k, Tensor v, Tensor ids, Tensor lengths, float scale) -> Tensor");
     m.def("shared_prefix_attention(Tensor q, Tensor k_prefix, Tensor v_prefix, Tensor k, Tensor v, Tensor lengths, "
           "float scale, bool return_lse=False) -> (Tensor, Tensor)");
-    m.def("scored_attention(Tensor q, Tensor k_prefix, Tensor v_prefix, Tensor k, Tensor v, Tensor lengths, "
-          "Tensor scores, float scale) -> (Tensor, Tensor)");
+    m.def("scored_attention(Tensor q, Tensor k, Tensor v, Tensor lengths, Tensor scores, float scale, "
+          "Tensor? k_prefix=None, Tensor? v_prefix=None) -> (Tensor, Tensor)");
     m.def("evict(Tensor k, Tensor v, Tensor scores, Tensor lengths, int budget, int window, int sink, int capacity) "
           "-> (Tensor, Tensor, Tensor, Tensor, Tensor)");
     m.def("workspace_counters() -> Tensor[]", &workspace_counters);
@@ -382,6 +397,13 @@ TORCH_LIBRARY_IMPL(lsa, CUDA, m) {
     m.impl("regroup", &regroup_cuda);
     m.impl("select_fused", &select_fused_cuda);
     m.impl("sparse_read", &sparse_read_cuda);
+    m.impl("shared_prefix_attention", &shared_prefix_cuda);
+    m.impl("scored_attention", &scored_cuda);
+    m.impl("evict", &evict_cuda);
+}
+
+// CPU tensors: the operators' own refusal (a ValueError) in place of the dispatcher's
+TORCH_LIBRARY_IMPL(lsa, CPU, m) {
     m.impl("shared_prefix_attention", &shared_prefix_cuda);
     m.impl("scored_attention", &scored_cuda);
     m.impl("evict", &evict_cuda);

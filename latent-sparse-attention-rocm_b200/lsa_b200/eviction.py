@@ -18,7 +18,6 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from ._lib import require_cuda
 
 
 class EvictedCache(NamedTuple):
@@ -38,13 +37,8 @@ def scored_attention(q, k, v, lengths, scores, scale=None, k_prefix=None, v_pref
     that see it and the query heads of KV head h, the weights those of the whole softmax
     (prefix keys included); entries at or past ``lengths[b]`` are copied. The prefix's own keys
     are not scored. Every entry has one writer: the same inputs give the same bits."""
-    if (k_prefix is None) != (v_prefix is None):
-        raise ValueError("scored_attention: a prefix has keys and values")
-    require_cuda(q, k, v, lengths, scores, k_prefix, v_prefix, what="scored_attention")
-    if k_prefix is None:
-        k_prefix = v_prefix = k.new_empty((0, k.shape[2], k.shape[3])) if k.dim() == 4 else k
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
-    out = _lib.torch_ops().scored_attention(q, k_prefix, v_prefix, k, v, lengths, scores, scale)
+    out = _lib.torch_ops().scored_attention(q, k, v, lengths, scores, scale, k_prefix, v_prefix)
     _lib.after_call(q.device, "scored_attention")
     return out
 
@@ -57,8 +51,7 @@ def evict(k, v, scores, lengths, budget: int, window_size: int = 64, sink_size: 
     ``sink_size``, the last ``window_size`` and the highest-scored others stay: scores in the
     order of the selection's packed keys (+NaN above +inf, -0 below +0), ties to the lower
     index. The new cache has ``capacity`` slots (default ``budget``), zero past the kept keys."""
-    require_cuda(k, v, scores, lengths, what="evict")
     capacity = budget if capacity is None else capacity
-    r = _lib.torch_ops().evict(k, v, scores, lengths, int(budget), int(window_size), int(sink_size), int(capacity))
+    r = _lib.torch_ops().evict(k, v, scores, lengths, budget, window_size, sink_size, capacity)
     _lib.after_call(k.device, "evict")
     return EvictedCache(*r)

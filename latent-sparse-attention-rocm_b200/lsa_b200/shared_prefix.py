@@ -11,7 +11,6 @@ one sequence against its own cache.
 from __future__ import annotations
 
 from . import _lib
-from ._lib import require_cuda
 
 
 def shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths, scale=None, return_lse: bool = False):
@@ -26,7 +25,6 @@ def shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths, scale=None, re
     boundaries); others are copied. fp32, fp16 or bf16; D 64 or 128. ``scale`` defaults to
     ``D ** -0.5``. Output like q, contiguous; with ``return_lse`` also the natural
     log-sum-exp of every row's scaled logits, fp32 [B, Tq, Hq]."""
-    require_cuda(q, k_prefix, v_prefix, k, v, lengths, what="shared_prefix_attention")
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     out, lse = _lib.torch_ops().shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths, scale, return_lse)
     _lib.after_call(q.device, "shared_prefix_attention")

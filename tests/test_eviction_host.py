@@ -23,7 +23,7 @@ def test_meta_shapes():
     assert out.shape == a[0].shape and out.dtype == a[0].dtype
     assert lse.shape == (2, 3, 8) and lse.dtype == torch.float32
     s = torch.empty(2, 2, 8, device="meta")
-    out, s2 = ops.scored_attention(*a, s, 0.1)
+    out, s2 = ops.scored_attention(a[0], a[3], a[4], a[5], s, 0.1, a[1], a[2])
     assert out.shape == a[0].shape and s2.shape == s.shape
     k, v, s2, n, ids = ops.evict(a[3], a[4], s, a[5], 4, 1, 1, 6)
     assert k.shape == v.shape == (2, 6, 2, 128) and s2.shape == ids.shape == (2, 2, 6) and n.shape == (2,)
