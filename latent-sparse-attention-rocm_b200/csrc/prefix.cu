@@ -131,8 +131,8 @@ __global__ void __launch_bounds__(kSimtWarps * 32) prefix_simt_kernel(const Pref
         if (r >= nrows) continue;
         const int64_t rid = row_index(a, (int64_t)b * a.Tq + r / a.G, h, r % a.G);
         const int64_t at = (int64_t)part * a.rows + rid;
-        if (lane == 0) a.part_lse[at] = l[u] > 0.0f ? m[u] + log2f(l[u]) : -INFINITY;
-        const float inv = l[u] > 0.0f ? 1.0f / l[u] : 0.0f;
+        if (lane == 0) a.part_lse[at] = l[u] == 0.0f ? -INFINITY : m[u] + log2f(l[u]);
+        const float inv = l[u] == 0.0f ? 0.0f : 1.0f / l[u];
 #pragma unroll
         for (int e = 0; e < E; ++e) a.part_o[at * D + lane * E + e] = acc[u][e] * inv;
     }
@@ -150,10 +150,13 @@ __device__ __forceinline__ float joined_lse(const PrefixArgs& a, int64_t row, in
         if (32 * i < parts && lane + 32 * i < parts) x[i] = a.part_lse[(int64_t)(lane + 32 * i) * a.rows + row];
     }
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) top = fmaxf(top, x[i]);
+    for (int i = 0; i < kPer; ++i) {
+        top = fmaxf(top, x[i]);
+        sum += x[i] != x[i] ? x[i] : 0.0f;  // a NaN part makes the row NaN
+    }
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
-    if (top == -INFINITY) return top;
+    if (top == -INFINITY) top = 0.0f;  // no part has a key: the sum is 0, its logarithm -inf
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
         if (32 * i < parts) sum += exp2f(x[i] - top);
@@ -246,12 +249,15 @@ __global__ void __launch_bounds__(256) prefix_finish_kernel(const PrefixArgs a, 
         if (32 * i < parts && lane + 32 * i < parts) x[i] = a.part_lse[(int64_t)(lane + 32 * i) * a.rows + row];
     }
     float top = x[0];
+    bool bad = x[0] != x[0];
 #pragma unroll
-    for (int i = 1; i < kPer; ++i) top = fmaxf(top, x[i]);
+    for (int i = 1; i < kPer; ++i) top = fmaxf(top, x[i]), bad = bad || x[i] != x[i];
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
     float acc[E] = {}, total = 0.0f;
-    if (top != -INFINITY) {
+    if (__any_sync(0xFFFFFFFFu, bad)) {  // a part is NaN: so is the row
+        total = NAN;
+    } else if (top != -INFINITY) {
         int best = 0;
 #pragma unroll
         for (int i = kPer - 1; i >= 0; --i) {
@@ -287,12 +293,12 @@ __global__ void __launch_bounds__(256) prefix_finish_kernel(const PrefixArgs a, 
             }
         }
     }
-    const float inv = total > 0.0f ? 1.0f / total : 0.0f;
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     T* dst = static_cast<T*>(a.out) + row * D + lane * E;
 #pragma unroll
     for (int e = 0; e < E; ++e) dst[e] = from_f32<T>(acc[e] * inv);
     if (lane == 0) {
-        const float y = total > 0.0f ? top + log2f(total) : -INFINITY;
+        const float y = total == 0.0f ? -INFINITY : top + log2f(total);
         a.lse2[row] = y;
         if (a.lse) a.lse[row] = y * 0.69314718055994531f;
     }
@@ -426,7 +432,8 @@ Plan make_plan(int dtype, int64_t B, int64_t Tq, int64_t Hkv, int64_t G, int64_t
 bool sizes_ok(int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_t P, int64_t T) {
     if (B < 0 || Tq < 0 || P < 0 || T < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || Hq / Hkv > 64) return false;
     if (D != 64 && D != 128) return false;
-    // rows and keys are counted in 32 bits (offsets in 64)
+    // rows, work items and keys are counted in 32 bits (offsets in 64)
+    if (B > (1 << 24) / Hkv || Hkv > 1 << 16) return false;
     return P <= INT32_MAX - 256 && T <= INT32_MAX - 256 && B <= INT32_MAX && Tq <= INT32_MAX && Hq <= INT32_MAX &&
            (B == 0 || Tq == 0 || B * Tq <= INT32_MAX / Hq);
 }

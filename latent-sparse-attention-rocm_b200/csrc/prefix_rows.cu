@@ -252,16 +252,16 @@ __global__ void __launch_bounds__(kWarps * 32, 2) prefix_rows_kernel(const Prefi
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
             const float2 ml = sml[w * kRows + r];
-            const float f = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - top);
+            const float f = ml.y == 0.0f ? 0.0f : exp2f(ml.x - top);  // NaN passes on
             const float4 y = *reinterpret_cast<const float4*>(smem + w * Sh::kWarpBytes + (r * D + c) * 4);
             total = fmaf(f, ml.y, total);
             x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w);
         }
-        const float inv = total > 0.0f ? 1.0f / total : 0.0f;
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
         const int tok = (r0 + r) / a.G;
         const int64_t rid = row_index(a, (int64_t)b * a.Tq + tok, h, r0 + r - tok * a.G);
         const int64_t at = (int64_t)part * a.rows + rid;
-        if (c == 0) a.part_lse[at] = total > 0.0f ? top + log2f(total) : -INFINITY;
+        if (c == 0) a.part_lse[at] = total == 0.0f ? -INFINITY : top + log2f(total);
         *reinterpret_cast<float4*>(a.part_o + at * D + c) = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
     }
     if (rp.follows && blockIdx.x == gridDim.x - 1) grid_wait();

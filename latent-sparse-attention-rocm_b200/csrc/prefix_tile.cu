@@ -118,7 +118,7 @@ __device__ __forceinline__ void softmax_half(const PrefixArgs& a, const TilePlan
     const int step = w.streams ? 2 : 1, first = w.c0 + (w.streams ? hf : 0);
     const int n = w.c1 > first ? (w.c1 - first + step - 1) / step : 0;
     float m = -INFINITY, l = 0.0f;
-    const float sl = a.scale_log2, thresh = 8.0f / sl;
+    const float sl = a.scale_log2, thresh = fminf(8.0f / sl, 1e30f);
     bool ok = true;
     auto publish = [&](uint64_t* bar) {  // this warp's P so far: one arrival a warp
         tmem_wait_st();
@@ -214,9 +214,9 @@ __device__ __forceinline__ void softmax_half(const PrefixArgs& a, const TilePlan
     if (ok && n > 0) ok = role_wait(&bar_o[hf], 0, abort_flag);
     if (!ok) return;
     const int64_t rid = row_index(a, (int64_t)w.b * a.Tq + tok, w.h, g);
-    const bool some = m != -INFINITY;  // the row has seen a key
-    const float inv = some ? 1.0f / l : 0.0f;
-    const float lse = some ? m * sl + log2f(l) : -INFINITY;
+    const bool none = l == 0.0f;  // the row has seen no key (a NaN logit makes l NaN, and the output)
+    const float inv = none ? 0.0f : 1.0f / l;
+    const float lse = none ? -INFINITY : m * sl + log2f(l);
     const int64_t at = (int64_t)(w.part + (w.streams ? hf : 0)) * a.rows + rid;
     if (live) {
         if (w.direct) {

@@ -21,7 +21,8 @@ __global__ void __launch_bounds__(kWKeys) own_weights_kernel(const PrefixArgs a,
     float* sk = sm;                // [kWKeys][LDK]
     float* sq = sm + kWKeys * LDK; // [kWRows][D]
     __shared__ float slse[kWRows];
-    const int b = blockIdx.z, h = blockIdx.y, j0 = blockIdx.x * kWKeys, tid = threadIdx.x;
+    const int per = (int)(((int64_t)a.T + kWKeys - 1) / kWKeys), bh = blockIdx.x / per;
+    const int b = bh / a.Hkv, h = bh % a.Hkv, j0 = (blockIdx.x % per) * kWKeys, tid = threadIdx.x;
     const int len = own_length(a, b), j = j0 + tid;
     const int64_t at = ((int64_t)b * a.Hkv + h) * a.T + j;
     if (j0 >= len) {
@@ -79,9 +80,9 @@ template <int D>
 int weights_launch(const PrefixArgs& a, const float* scores, float* scores_out, cudaStream_t stream) {
     const int smem = (kWKeys * (D + 4) + kWRows * D) * 4;
     if (!allow_smem<own_weights_kernel<D>>(smem)) return LSA_ERR_CUDA;
-    if (a.B > 65535 || a.Hkv > 65535) return LSA_ERR_SIZE;
-    dim3 grid((unsigned)((a.T + kWKeys - 1) / kWKeys), (unsigned)a.Hkv, (unsigned)a.B);
-    own_weights_kernel<D><<<grid, kWKeys, smem, stream>>>(a, scores, scores_out);
+    const int64_t grid = ((int64_t)a.T + kWKeys - 1) / kWKeys * a.Hkv * a.B;
+    if (grid > INT32_MAX) return LSA_ERR_SIZE;
+    own_weights_kernel<D><<<(unsigned)grid, kWKeys, smem, stream>>>(a, scores, scores_out);
     LSA_LAUNCH_CHECK();
     return LSA_OK;
 }

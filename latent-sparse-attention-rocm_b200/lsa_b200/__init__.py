@@ -9,6 +9,7 @@ errors. Every operator runs hand-written CUDA kernels through the C-ABI library
 
 from . import _lib, pipeline, prefill, read_kernel, read_kernel_tiled, select_fused  # noqa: F401
 from ._lib import check_status  # noqa: F401
+from .budgeted import BudgetedCache  # noqa: F401
 from .eviction import EvictedCache, evict, scored_attention  # noqa: F401
 from .index_space import make_index_space  # noqa: F401
 from .pipeline import (  # noqa: F401
@@ -35,4 +36,5 @@ __all__ = [
     "build_hierarchy_gpu", "dense_read", "flat_select", "flat_select_reference", "lsa_read",
     "make_index_space", "position_buckets", "select_from_queries", "tree_select", "visible_counts",
     "check_status", "shared_prefix_attention", "scored_attention", "evict", "EvictedCache",
+    "BudgetedCache",
 ]

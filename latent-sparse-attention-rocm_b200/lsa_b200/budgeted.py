@@ -1,0 +1,68 @@
+"""Decoding under a shared prefix with every sequence's own cache held to a budget.
+
+The loop that ``shared_prefix_attention``, ``scored_attention`` and ``evict`` are for: a batch
+starts from one long prompt, stored once; each sequence appends its tokens to its own cache,
+every step scores the cached keys by the attention they receive, and when the room is used up
+the keys that matter least leave. No reference counterpart.
+
+    cache = BudgetedCache(k, v, lengths, budget=2048, room=64, k_prefix=kp, v_prefix=vp)
+    for q, k_new, v_new in steps:              # [B, Tq, Hq, D], [B, Tq, Hkv, D] twice
+        out = cache.step(q, k_new, v_new)
+"""
+
+from __future__ import annotations
+
+import torch
+
+from .eviction import evict, scored_attention
+
+
+class BudgetedCache:
+    """The own caches of a decoding batch: at most ``budget`` keys a (sequence, KV head) after an
+    eviction, ``room`` more until the next.
+
+    k, v [B, T, Hkv, D] hold the sequences' own prompts, ``lengths`` [B] (host integers) how much of
+    them; ``scores`` fp32 [B, Hkv, T] what they have collected so far (zeros when None: then
+    an eviction keeps the oldest of the keys that nothing has read). The sinks and the window
+    are those of ``evict``."""
+
+    def __init__(self, k, v, lengths, budget: int, room: int, window_size: int = 64, sink_size: int = 4,
+                 k_prefix=None, v_prefix=None, scores=None):
+        if room < 1:
+            raise ValueError(f"a budgeted cache needs room to append to, got {room}")
+        B, T, Hkv, _ = k.shape
+        lengths = [int(n) for n in lengths]
+        if len(lengths) != B or any(n < 0 or n > T for n in lengths):
+            raise ValueError(f"one length in [0, {T}] a sequence, got {lengths}")
+        self.budget, self.capacity = int(budget), int(budget) + int(room)
+        self.window_size, self.sink_size = window_size, sink_size
+        self.k_prefix, self.v_prefix = k_prefix, v_prefix
+        if scores is None:
+            scores = torch.zeros(B, Hkv, T, dtype=torch.float32, device=k.device)
+        self.k, self.v, self.scores = k, v, scores
+        self.lengths = torch.tensor(lengths, dtype=torch.int32, device=k.device)
+        self._longest = max(lengths, default=0)  # of the batch, known without asking the device
+        self._rows = torch.arange(B, device=k.device)[:, None]
+        self._evict()
+
+    def _evict(self):
+        kept = evict(self.k, self.v, self.scores, self.lengths, self.budget, self.window_size, self.sink_size,
+                     self.capacity)
+        self.k, self.v, self.scores, self.lengths = kept.k, kept.v, kept.scores, kept.lengths
+        self._longest = min(self._longest, self.budget)
+
+    def step(self, q, k_new, v_new, scale=None):
+        """Append the step's Tq tokens, attend to the prefix and the own cache, score the keys.
+        Evicts first when the longest sequence has no room for them. Output like q."""
+        Tq = q.shape[1]
+        if Tq > self.capacity - self.budget:
+            raise ValueError(f"a step of {Tq} tokens does not fit the room of {self.capacity - self.budget}")
+        if self._longest + Tq > self.capacity:
+            self._evict()
+        at = self.lengths.long()[:, None] + torch.arange(Tq, device=q.device)
+        self.k[self._rows, at], self.v[self._rows, at] = k_new, v_new
+        self.lengths = self.lengths + Tq
+        self._longest += Tq
+        out, self.scores = scored_attention(q, self.k, self.v, self.lengths, self.scores, scale, self.k_prefix,
+                                            self.v_prefix)
+        return out

@@ -158,3 +158,51 @@ def test_other_stream_and_graph(lsa):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(got, w2))
+
+
+@pytest.mark.parametrize("dt", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("Tq,P", [(1, 500), (3, 0)])
+def test_serving_loop(lsa, dt, Tq, P):
+    """The whole loop: every step's output and scores against the formula in 64 bits on the state
+    that the step started from, through several evictions. Tolerances as in the attention's tests."""
+    B, Hq, Hkv, D, T, budget, room = 3, 8, 2, 128, 150, 96, 7
+    g = torch.Generator(device=DEV)
+    g.manual_seed(Tq)
+    r = lambda *s: torch.randn(*s, generator=g, device=DEV).to(dt)
+    kp, vp = (r(P, Hkv, D), r(P, Hkv, D)) if P else (None, None)
+    cache = lsa.BudgetedCache(r(B, T, Hkv, D), r(B, T, Hkv, D), [150, 96, 20], budget, room, window_size=16,
+                              sink_size=4, k_prefix=kp, v_prefix=vp, scores=torch.rand(B, Hkv, T, device=DEV))
+    assert cache.lengths.tolist() == [96, 96, 20] and cache.k.shape[1] == budget + room
+    u = 2.0 ** -8 if dt == BF else 0.0
+    evictions = 0
+    for _ in range(20):
+        before = [int(n) for n in cache.lengths]
+        q, k_new, v_new = r(B, Tq, Hq, D), r(B, Tq, Hkv, D), r(B, Tq, Hkv, D)
+        old = cache.scores
+        out = cache.step(q, k_new, v_new)
+        after = [int(n) for n in cache.lengths]
+        evicted = after[0] != before[0] + Tq
+        evictions += evicted
+        assert after == [min(n, budget if evicted else n) + Tq for n in before]
+        for b in range(B):
+            n = after[b]
+            assert torch.equal(cache.k[b, n - Tq:n], k_new[b]) and torch.equal(cache.v[b, n - Tq:n], v_new[b])
+            for h in range(Hkv):
+                key, val = cache.k[b, :n, h].double(), cache.v[b, :n, h].double()
+                if P:
+                    key, val = torch.cat([kp[:, h].double(), key]), torch.cat([vp[:, h].double(), val])
+                s = torch.einsum("tgd,jd->tgj", q[b, :, 4 * h:4 * h + 4].double(), key) * D ** -0.5
+                last = P + n - Tq + torch.arange(Tq, device=DEV)
+                s = s.masked_fill(torch.arange(P + n, device=DEV) > last[:, None, None], -float("inf"))
+                p = torch.softmax(s, -1)
+                want, absum = p @ val, p @ val.abs()
+                assert float(((out[b, :, 4 * h:4 * h + 4].double() - want).abs() - u * want.abs()
+                              - (u + 2e-4) * absum - 1e-6).max()) <= 0
+                if not evicted:
+                    w = p[..., P:].sum((0, 1))
+                    assert float(((cache.scores[b, h, :n].double() - old[b, h, :n].double() - w).abs()
+                                  - 2e-4 * w - 2.0 ** -22 * (old[b, h, :n] + 1)).max()) <= 0
+    assert evictions >= 2
+    with pytest.raises(ValueError, match="room"):
+        cache.step(r(B, 8, Hq, D), r(B, 8, Hkv, D), r(B, 8, Hkv, D))
+    lsa.check_status()

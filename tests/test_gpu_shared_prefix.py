@@ -147,6 +147,20 @@ def test_unwritten_slots_are_never_used(lsa, dt, Tq, Hq, T):
         assert torch.equal(got[0], clean[0]) and torch.equal(got[1], clean[1])
 
 
+@pytest.mark.parametrize("dt", [BF, HF, F32], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("Tq,B,P", [(1, 3, 40), (1, 30, 400), (40, 3, 0), (70, 2, 300)])
+def test_a_nan_query_stays_in_its_row(lsa, dt, Tq, B, P):
+    """A NaN row gives NaN outputs, and no other row's bits change."""
+    q, kp, vp, k, v, lengths, scores = make(B, Tq, 8, 2, 128, P, 100, dt, seed=6)
+    clean = lsa.shared_prefix_attention(q, kp, vp, k, v, lengths)
+    q2 = q.clone()
+    q2[B - 1, Tq - 1, 5] = math.nan
+    got, lse = lsa.shared_prefix_attention(q2, kp, vp, k, v, lengths, return_lse=True)
+    assert torch.isnan(got[B - 1, Tq - 1, 5]).all() and torch.isnan(lse[B - 1, Tq - 1, 5])
+    got[B - 1, Tq - 1, 5] = clean[B - 1, Tq - 1, 5]
+    assert torch.equal(got, clean)
+
+
 @pytest.mark.parametrize("dt", [BF, HF], ids=["bf16", "fp16"])
 @pytest.mark.parametrize("Tq,B", [(1, 3), (16, 3), (1, 70)])
 def test_strided_views(lsa, dt, Tq, B):
@@ -193,6 +207,43 @@ def test_prefix_equals_copies_in_every_cache(lsa):
     whole_v = torch.cat([vp[None].expand(20, -1, -1, -1), v], 1)
     b = lsa.shared_prefix_attention(q, kp[:0], vp[:0], whole_k, whole_v, lengths + 800)
     assert float((a.float() - b.float()).abs().max()) <= 2e-2
+
+
+@pytest.mark.parametrize("Tq", [1, 40])
+def test_tiny_scales(lsa, Tq):
+    """All weights equal in the limit: the mean of the visible values."""
+    q, kp, vp, k, v, lengths, scores = make(2, Tq, 8, 2, 128, 90, 140, BF, seed=12, lengths=[140, 77])
+    for scale in (1e-30, 1e-44):
+        out, absum, _, _ = want(q, kp, vp, k, v, lengths, scale)
+        check_out(lsa.shared_prefix_attention(q, kp, vp, k, v, lengths, scale), out, absum, BF)
+
+
+def test_refusals(lsa):
+    q, kp, vp, k, v, lengths, scores = make(2, 1, 8, 2, 128, 16, 32, BF)
+    bad = [(q.float(), kp, vp, k, v, lengths), (q, kp[:, :1], vp[:, :1], k, v, lengths), (q, kp, vp[:8], k, v, lengths),
+           (q, kp, vp, k, v[:, :8], lengths), (q[:1], kp, vp, k, v, lengths), (q, kp, vp, k, v, lengths[:1]),
+           (q, kp, vp, k, v, lengths.float()), (q[:, :, :7], kp, vp, k, v, lengths), (q[0], kp, vp, k, v, lengths),
+           (q[..., :32], kp[..., :32], vp[..., :32], k[..., :32], v[..., :32], lengths),
+           (q, kp, vp, k.cpu(), v, lengths), (q, kp, vp, k, v, lengths.cpu())]
+    for args in bad:
+        with pytest.raises(ValueError):
+            lsa.shared_prefix_attention(*args)
+    for scale in (0.0, -1.0, math.inf, math.nan):
+        with pytest.raises(ValueError, match="scale"):
+            lsa.shared_prefix_attention(q, kp, vp, k, v, lengths, scale)
+    for s in (scores[:, :1], scores.double(), scores[:, :, :8], scores[0]):
+        with pytest.raises(ValueError, match="scores"):
+            lsa.scored_attention(q, k, v, lengths, s)
+    with pytest.raises(ValueError, match="prefix"):
+        lsa.scored_attention(q, k, v, lengths, scores, v_prefix=vp)
+    for kw in (dict(budget=-1), dict(budget=10, window_size=8, sink_size=4), dict(budget=20, window_size=8, capacity=10),
+               dict(budget=20, window_size=-1), dict(budget=20, window_size=4, sink_size=-1)):
+        with pytest.raises(ValueError):
+            lsa.evict(k, v, scores, lengths, **kw)
+    with pytest.raises(ValueError, match="16 bytes"):
+        lsa.evict(k[..., :4].contiguous(), v[..., :4].contiguous(), scores, lengths, 20, 4)
+    empty = lsa.shared_prefix_attention(q[:0], kp, vp, k[:0], v[:0], lengths[:0])
+    assert empty.shape == (0, 1, 8, 128)
 
 
 def test_same_bits_every_time(lsa):
