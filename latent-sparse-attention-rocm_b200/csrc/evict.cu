@@ -23,6 +23,7 @@ struct EvictArgs {
     const int32_t* lengths;                // [B]
     int B, T, Hkv, row_bytes, row_lanes;
     int budget, window, sink, capacity;
+    bool copy;                             // the selecting kernel copies the rows too
     void *k_out, *v_out;                   // [B, capacity, Hkv, D] contiguous
     float* scores_out;                     // [B, Hkv, capacity]
     int32_t* lengths_out;                  // [B]
@@ -56,6 +57,43 @@ __device__ __forceinline__ int4 ld_cluster4(uint32_t addr) {
 
 __device__ __forceinline__ void add_cluster(uint32_t addr, int v) {
     if (v) asm volatile("red.relaxed.cluster.shared::cluster.add.s32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
+// The rows of K and V of slots [m0, m1) by their ids: a row of 16-byte chunks to the next power of
+// two of lanes (at most a warp), four rows a thread in flight; zeros for a slot without an id.
+__device__ __forceinline__ void copy_rows(const EvictArgs& a, int b, int h, int m0, int m1) {
+    const int32_t* ids = a.ids + ((int64_t)b * a.Hkv + h) * a.capacity;
+    const int tid = threadIdx.x;
+    const int chunks = a.row_bytes >> 4, lanes = a.row_lanes;
+    const int sub = tid / lanes, step = kThreads / lanes;
+    const uint8_t* kb = static_cast<const uint8_t*>(a.k) + b * a.k_b + h * a.k_h;
+    const uint8_t* vb = static_cast<const uint8_t*>(a.v) + b * a.v_b + h * a.v_h;
+    const int64_t out_t = (int64_t)a.Hkv * a.row_bytes;
+    uint8_t* ko = static_cast<uint8_t*>(a.k_out) + ((int64_t)b * a.capacity * a.Hkv + h) * a.row_bytes;
+    uint8_t* vo = static_cast<uint8_t*>(a.v_out) + ((int64_t)b * a.capacity * a.Hkv + h) * a.row_bytes;
+    for (int c = tid % lanes; c < chunks; c += lanes) {
+        for (int m = m0 + sub; m < m1; m += 4 * step) {
+            uint4 x[4], y[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int mu = m + u * step;
+                const int id = mu < m1 ? ids[mu] : -1;
+                x[u] = y[u] = make_uint4(0, 0, 0, 0);
+                if (id >= 0) {
+                    x[u] = __ldg(reinterpret_cast<const uint4*>(kb + id * a.k_t) + c);
+                    y[u] = __ldg(reinterpret_cast<const uint4*>(vb + id * a.v_t) + c);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int mu = m + u * step;
+                if (mu < m1) {
+                    reinterpret_cast<uint4*>(ko + mu * out_t)[c] = x[u];
+                    reinterpret_cast<uint4*>(vo + mu * out_t)[c] = y[u];
+                }
+            }
+        }
+    }
 }
 
 // Every row (sequence, KV head) is served by `ranks` CTAs.
@@ -239,38 +277,15 @@ __global__ void __launch_bounds__(kThreads, 2) evict_kernel(const EvictArgs a, i
         cluster_sync();  // the ids of every CTA; and no CTA leaves while its counts are read
     else
         __syncthreads();
-    // a row of 16-byte chunks to the next power of two of lanes (at most a warp), four rows a
-    // thread in flight
-    const int chunks = a.row_bytes >> 4, lanes = a.row_lanes;
-    const int sub = tid / lanes, step = kThreads / lanes;
-    const uint8_t* kb = static_cast<const uint8_t*>(a.k) + b * a.k_b + h * a.k_h;
-    const uint8_t* vb = static_cast<const uint8_t*>(a.v) + b * a.v_b + h * a.v_h;
-    const int64_t out_t = (int64_t)a.Hkv * a.row_bytes;
-    uint8_t* ko = static_cast<uint8_t*>(a.k_out) + ((int64_t)b * a.capacity * a.Hkv + h) * a.row_bytes;
-    uint8_t* vo = static_cast<uint8_t*>(a.v_out) + ((int64_t)b * a.capacity * a.Hkv + h) * a.row_bytes;
-    for (int c = tid % lanes; c < chunks; c += lanes) {
-        for (int m = m0 + sub; m < m1; m += 4 * step) {
-            uint4 x[4], y[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int mu = m + u * step;
-                const int id = mu < m1 ? ids[mu] : -1;
-                x[u] = y[u] = make_uint4(0, 0, 0, 0);
-                if (id >= 0) {
-                    x[u] = __ldg(reinterpret_cast<const uint4*>(kb + id * a.k_t) + c);
-                    y[u] = __ldg(reinterpret_cast<const uint4*>(vb + id * a.v_t) + c);
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int mu = m + u * step;
-                if (mu < m1) {
-                    reinterpret_cast<uint4*>(ko + mu * out_t)[c] = x[u];
-                    reinterpret_cast<uint4*>(vo + mu * out_t)[c] = y[u];
-                }
-            }
-        }
-    }
+    if (a.copy) copy_rows(a, b, h, m0, m1);
+}
+
+// The copy alone, for rows whose selecting CTAs are too few to draw the memory's bandwidth: every
+// CTA an equal share of a row's slots.
+__global__ void __launch_bounds__(kThreads, 2) evict_copy_kernel(const EvictArgs a, int ranks) {
+    const int rank = blockIdx.x % ranks, row = blockIdx.x / ranks;
+    copy_rows(a, row / a.Hkv, row % a.Hkv, (int)((int64_t)a.capacity * rank / ranks),
+              (int)((int64_t)a.capacity * (rank + 1) / ranks));
 }
 
 }  // namespace
@@ -308,18 +323,17 @@ int lsa_evict(const void* k, const void* v, int64_t row_bytes, const int64_t* st
     a.capacity = (int)capacity;
     a.k_out = k_out, a.v_out = v_out, a.scores_out = scores_out, a.lengths_out = lengths_out, a.ids = ids;
     a.row_lanes = row_bytes / 16 >= 32 ? 32 : next_pow2((int)(row_bytes / 16));
-    // A row's CTAs: enough that all rows' copies fill the GPU, none with fewer than 64 slots to copy.
-    // Keys that fit one CTA are selected by each of them, more in slices by a cluster.
+    // A row's CTAs. Keys that fit one CTA are selected by each of them: as many as have 64 slots to copy,
+    // up to 128 in all (more than one an SM slow each other's selection: 9.6 us for a step of 8 rows in
+    // 128 CTAs, 12.4 in 256), a second one for a large batch. More keys go in slices to a cluster of 8
+    // (of 16 for few rows, or slices past its shared memory; it fills most of a GPC: 101 against 76
+    // us for 32 rows of 131072 keys).
     const int64_t units = B * Hkv;
     const bool sliced = T > kCached;
     int64_t ranks = 1;
-    while (ranks < 16 && (units * ranks < 4 * 148 && capacity / (2 * ranks) >= 64)) ranks *= 2;
-    if (sliced) {
-        // clusters of 8 (a cluster of 16 fills most of a GPC: 101 against 80 us for 32 rows of 131072
-        // keys), of 16 where the rows are few or the slices outgrow shared memory
-        ranks = 8;
-        if (units * ranks < 148 || T > 8 * kCached) ranks = 16;
-    }
+    while (units * ranks * 2 <= 148 && capacity / (2 * ranks) >= 64) ranks *= 2;
+    if (units > 148 && units < 4 * 148) ranks = 2;
+    if (sliced) ranks = units * 8 < 148 || T > 8 * kCached ? 16 : 8;
     const int64_t slice = sliced ? (T + ranks - 1) / ranks : T;
     const int smem = (int)((slice < kCached ? slice : kCached) * 4);
     auto kern = sliced ? evict_kernel<true> : evict_kernel<false>;
@@ -337,7 +351,14 @@ int lsa_evict(const void* k, const void* v, int64_t row_bytes, const int64_t* st
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
+    // few CTAs with much to copy leave it to a launch of its own
+    a.copy = units * ranks >= 100 || units * capacity * row_bytes <= 4 << 20;
     if (cudaLaunchKernelEx(&cfg, kern, a, (int)ranks) != cudaSuccess) return LSA_ERR_CUDA;
+    if (!a.copy) {
+        const int64_t each = (4 * 148 + units - 1) / units;
+        evict_copy_kernel<<<(unsigned)(units * each), kThreads, 0, stream>>>(a, (int)each);
+        LSA_LAUNCH_CHECK();
+    }
     return LSA_OK;
 }
 

@@ -141,13 +141,13 @@ __global__ void __launch_bounds__(kSimtWarps * 32) prefix_simt_kernel(const Pref
 constexpr int kPer = kMaxParts / 32;  // parts of a row that a lane holds
 
 // The lse of a row from its parts, by one warp (log2 domain; every lane has it).
-__device__ __forceinline__ float joined_lse(const PrefixArgs& a, int64_t row, int parts) {
+template <typename F> __device__ __forceinline__ float joined_lse(int parts, F part) {
     const int lane = threadIdx.x & 31;
     float x[kPer], top = -INFINITY, sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         x[i] = -INFINITY;
-        if (32 * i < parts && lane + 32 * i < parts) x[i] = a.part_lse[(int64_t)(lane + 32 * i) * a.rows + row];
+        if (32 * i < parts && lane + 32 * i < parts) x[i] = part(lane + 32 * i);
     }
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -166,6 +166,7 @@ __device__ __forceinline__ float joined_lse(const PrefixArgs& a, int64_t row, in
 }
 
 constexpr int kWeightKeys = 1024;  // keys of a weights block: four a thread
+constexpr int kHeldLse = 4096;     // parts' lse that a weights block holds in shared memory
 
 // Own keys' weights from the logits that the few-row kernel kept (4 bytes a row and key, 16 for a
 // decode step of 4 heads, against the 256 bytes of K that scoring the key again would read):
@@ -174,7 +175,7 @@ constexpr int kWeightKeys = 1024;  // keys of a weights block: four a thread
 // itself, beside the blocks that join the output: one launch for both.
 __device__ __forceinline__ void own_weights(const PrefixArgs& a, const RowsPlan& rp, int parts,
                                             const float* __restrict__ scores, float* __restrict__ scores_out) {
-    __shared__ float slse[kMostFew];
+    __shared__ float slse[kMostFew], held[kHeldLse];
     const int per = (int)(((int64_t)a.T + kWeightKeys - 1) / kWeightKeys);
     const int64_t bh = blockIdx.x / per;
     const int b = (int)(bh / a.Hkv), h = (int)(bh % a.Hkv), nrows = a.Tq * a.G, warp = threadIdx.x >> 5;
@@ -188,8 +189,19 @@ __device__ __forceinline__ void own_weights(const PrefixArgs& a, const RowsPlan&
         float4 s[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) s[u] = __ldcs(reinterpret_cast<const float4*>(src + (u < nrows ? u : 0) * rp.pitch));
+        // all parts' lse of the rows at once, then a warp a row
+        for (int i = threadIdx.x; i < nrows * parts && i < kHeldLse; i += 256) {
+            const int c = i / nrows, r = i - c * nrows, tok = r / a.G;
+            held[i] = a.part_lse[c * a.rows + row_index(a, (int64_t)b * a.Tq + tok, h, r - tok * a.G)];
+        }
+        __syncthreads();
         for (int r = warp; r < nrows; r += 8) {
-            const float x = joined_lse(a, row_index(a, (int64_t)b * a.Tq + r / a.G, h, r % a.G), parts);
+            const int tok = r / a.G;
+            const int64_t row = row_index(a, (int64_t)b * a.Tq + tok, h, r - tok * a.G);
+            const float x = joined_lse(parts, [&](int c) {
+                const int i = c * nrows + r;
+                return i < kHeldLse ? held[i] : a.part_lse[c * a.rows + row];
+            });
             if ((threadIdx.x & 31) == 0) slse[r] = x;
         }
         __syncthreads();
@@ -399,10 +411,13 @@ Plan make_plan(int dtype, int64_t B, int64_t Tq, int64_t Hkv, int64_t G, int64_t
         return p;
     }
     double beside = 0;  // the few-row kernel's work on the own caches, in chunks of the tensor-core kernel a SM
-    // few rows: the few-row kernel reads the keys once for each 16 of them, from L2 after the first
-    // time, and has no fixed cost to speak of; a tensor-core item spends about 6 us, 32 MB of keys
-    const int64_t tiles = (rows + kFewRows - 1) / kFewRows;
-    if (tiles == 1 || (rows <= kMostFew && (tiles - 1) * B * T * Hkv * D * 4 <= 32 << 20)) {
+    // Few rows: the few-row kernel reads the keys once for each 16 of them, from L2 after the first
+    // time, where the tensor-core kernel reads them once but has a fixed cost of some 6 us (20 rows:
+    // 12.4 against 13.7 us at 17 MB of keys, 26 against 22 at 67 MB). With scores that cost comes
+    // twice, and a few rows' logits are cheap (20 rows: 20 / 33 / 66 us against 23 / 34 / 81 at 17 /
+    // 67 / 268 MB; 32 rows: 32 against 26 at 33 MB).
+    const int64_t tiles = (rows + kFewRows - 1) / kFewRows, again = (tiles - 1) * B * T * Hkv * D * 4;
+    if (tiles == 1 || (rows <= kMostFew && (again <= 16 << 20 || (scored && rows <= 24)))) {
         p.rows.own_tiles = (int)tiles;
         p.parts_o = p.So = few_splits(B * Hkv * tiles, (T + 63) / 64, B > 1);
         p.rows.own_items = (int)(B * Hkv * tiles * p.So);
