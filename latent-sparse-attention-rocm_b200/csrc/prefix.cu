@@ -7,6 +7,7 @@
 namespace lsa {
 namespace {
 
+constexpr int kSMs = 148;
 constexpr int kSimtRows = 16;  // rows of a work item
 constexpr int kSimtKeys = 32;  // keys of a tile: one per lane
 constexpr int kSimtWarps = 8;
@@ -165,86 +166,114 @@ template <typename F> __device__ __forceinline__ float joined_lse(int parts, F p
     return top + log2f(sum);
 }
 
-constexpr int kWeightKeys = 1024;  // keys of a weights block: four a thread
-constexpr int kHeldLse = 4096;     // parts' lse that a weights block holds in shared memory
+// Groups of threads that share a weights block's rows: a block of 256 threads takes 1024 / groups keys,
+// four a thread. Few rows: one group, the longest runs of keys; more: four, or a thread would
+// load them one group of four after another (64 rows: 26 us of latency).
+__host__ __device__ __forceinline__ int weight_groups(int nrows) { return nrows > 8 ? 4 : 1; }
+
+constexpr int kHeldLse = 2048;  // parts' lse that a weights block holds in shared memory
 
 // Own keys' weights from the logits that the few-row kernel kept (4 bytes a row and key, 16 for a
 // decode step of 4 heads, against the 256 bytes of K that scoring the key again would read):
 //   w_j = sum over the rows r that see j of 2^(s_rj - lse_r).
-// One thread owns four keys, so a sum has one order and one writer. The block joins its rows' lse
+// A key's sum has one order and one writer. The block joins its rows' lse
 // itself, beside the blocks that join the output: one launch for both.
 __device__ __forceinline__ void own_weights(const PrefixArgs& a, const RowsPlan& rp, int parts,
                                             const float* __restrict__ scores, float* __restrict__ scores_out) {
-    __shared__ float slse[kMostFew], held[kHeldLse];
-    const int per = (int)(((int64_t)a.T + kWeightKeys - 1) / kWeightKeys);
+    __shared__ float slse[kMostFew];
+    __shared__ __align__(16) float held[kHeldLse];
+    const int nrows = a.Tq * a.G, warp = threadIdx.x >> 5, groups = weight_groups(nrows), quads = 256 / groups;
+    const int keys = 4 * quads, per = (int)(((int64_t)a.T + keys - 1) / keys);
     const int64_t bh = blockIdx.x / per;
-    const int b = (int)(bh / a.Hkv), h = (int)(bh % a.Hkv), nrows = a.Tq * a.G, warp = threadIdx.x >> 5;
-    const int len = own_length(a, b), j0 = (blockIdx.x % per) * kWeightKeys, j = j0 + 4 * (int)threadIdx.x;
-    float old[4], w[4] = {0, 0, 0, 0};
+    const int b = (int)(bh / a.Hkv), h = (int)(bh % a.Hkv);
+    const int group = threadIdx.x / quads, quad = threadIdx.x % quads;
+    const int len = own_length(a, b), j0 = (blockIdx.x % per) * keys, j = j0 + 4 * quad;
+    float old[4] = {0, 0, 0, 0}, w[4] = {0, 0, 0, 0};
+    if (group == 0) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) old[u] = j + u < a.T ? scores[bh * a.T + j + u] : 0.0f;
+        for (int u = 0; u < 4; ++u) old[u] = j + u < a.T ? scores[bh * a.T + j + u] : 0.0f;
+    }
     if (j0 < len) {
         // the first rows' logits are on their way while the lse are joined
         const float* src = rp.logits + bh * nrows * rp.pitch + (j < len ? j : j0);
         float4 s[4];
+        auto load = [&](int r0) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) s[u] = __ldcs(reinterpret_cast<const float4*>(src + (u < nrows ? u : 0) * rp.pitch));
-        // all parts' lse of the rows at once, then a warp a row
-        for (int i = threadIdx.x; i < nrows * parts && i < kHeldLse; i += 256) {
-            const int c = i / nrows, r = i - c * nrows, tok = r / a.G;
-            held[i] = a.part_lse[c * a.rows + row_index(a, (int64_t)b * a.Tq + tok, h, r - tok * a.G)];
+            for (int u = 0; u < 4; ++u) {
+                const int r = r0 + u * groups;
+                s[u] = __ldcs(reinterpret_cast<const float4*>(src + (r < nrows ? r : 0) * rp.pitch));
+            }
+        };
+        load(group);
+        // a warp a row; more than eight rows' parts are fetched together first, not a row at a time
+        const bool many = nrows > 8;
+        if (many) {
+            for (int i = threadIdx.x; i < nrows * parts && i < kHeldLse; i += 256) {
+                const int c = i / nrows, r = i - c * nrows, tok = r / a.G;
+                held[i] = a.part_lse[c * a.rows + row_index(a, (int64_t)b * a.Tq + tok, h, r - tok * a.G)];
+            }
+            __syncthreads();
         }
-        __syncthreads();
         for (int r = warp; r < nrows; r += 8) {
             const int tok = r / a.G;
             const int64_t row = row_index(a, (int64_t)b * a.Tq + tok, h, r - tok * a.G);
             const float x = joined_lse(parts, [&](int c) {
                 const int i = c * nrows + r;
-                return i < kHeldLse ? held[i] : a.part_lse[c * a.rows + row];
+                return many && i < kHeldLse ? held[i] : a.part_lse[c * a.rows + row];
             });
             if ((threadIdx.x & 31) == 0) slse[r] = x;
         }
         __syncthreads();
-        for (int r0 = 0; r0 < nrows; r0 += 4) {
-            if (r0) {
-#pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    s[u] = __ldcs(reinterpret_cast<const float4*>(src + (r0 + u < nrows ? r0 + u : 0) * rp.pitch));
-            }
+        for (int r0 = group; r0 < nrows; r0 += 4 * groups) {
+            if (r0 != group) load(r0);
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                if (r0 + u >= nrows) break;
-                const float l = slse[r0 + u];  // -inf: a row that sees no key, and whose logits are -inf
+                if (r0 + u * groups >= nrows) break;
+                const float l = slse[r0 + u * groups];  // -inf: a row that sees no key, and whose logits are -inf
                 w[0] += s[u].x == -INFINITY ? 0.0f : exp2f(s[u].x - l);
                 w[1] += s[u].y == -INFINITY ? 0.0f : exp2f(s[u].y - l);
                 w[2] += s[u].z == -INFINITY ? 0.0f : exp2f(s[u].z - l);
                 w[3] += s[u].w == -INFINITY ? 0.0f : exp2f(s[u].w - l);
             }
         }
+        if (groups > 1) {  // the groups' sums in their order
+            float4* sums = reinterpret_cast<float4*>(held);
+            __syncthreads();
+            sums[threadIdx.x] = make_float4(w[0], w[1], w[2], w[3]);
+            __syncthreads();
+            if (group == 0)
+                for (int g = 1; g < groups; ++g) {
+                    const float4 x = sums[g * quads + quad];
+                    w[0] += x.x, w[1] += x.y, w[2] += x.z, w[3] += x.w;
+                }
+        }
     }
+    if (group != 0) return;
 #pragma unroll
     for (int u = 0; u < 4; ++u)
         if (j + u < a.T) scores_out[bh * a.T + j + u] = j + u < len ? old[u] + w[u] : old[u];
 }
 
-// The parts of a row joined, one warp per row: every lane holds D / 32 columns. The lse of all
-// parts are loaded at once, then the parts' columns eight loads at a time; a part without a
-// key (lse -inf) has weight zero and its columns, never written, are not read (the heaviest part's
-// are, in their place: finite, times zero).
+// The parts of a row joined by `spread` warps (1 to 8: more where the rows are few, so that the loads
+// of many parts fly together): every lane holds D / 32 columns of a warp's share. The lse of
+// all parts are loaded at once, then the parts' columns eight loads at a time; a part without
+// a key (lse -inf) has weight zero and its columns, never written, are not read (the heaviest part's
+// are, in their place: finite, times zero). The warps' sums add in their order.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) prefix_finish_kernel(const PrefixArgs a, const TilePlan tp, int parts,
-                                                            const RowsPlan rp, unsigned weight_blocks,
+__global__ void __launch_bounds__(256, 4) prefix_finish_kernel(const PrefixArgs a, const TilePlan tp, int parts,
+                                                            const RowsPlan rp, unsigned weight_blocks, int spread,
                                                             const float* __restrict__ scores,
                                                             float* __restrict__ scores_out) {
     constexpr int E = D / 32;
+    __shared__ float weight[8][kMaxParts], sums[8][D], totals[8];
     grid_trigger();
     grid_wait();
     if (blockIdx.x < weight_blocks) {
         own_weights(a, rp, parts, scores, scores_out);
         return;
     }
-    int64_t row = (int64_t)(blockIdx.x - weight_blocks) * 8 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % spread;
+    int64_t row = (int64_t)(blockIdx.x - weight_blocks) * (8 / spread) + warp / spread;
     if (tp.whole) {  // the rows of the split seq tiles, 256 a tile
         int b, h, tile;
         seq_tile(a, tp, tp.whole + (int)(row >> 8), &b, &h, &tile);
@@ -253,40 +282,39 @@ __global__ void __launch_bounds__(256) prefix_finish_kernel(const PrefixArgs a, 
         tok += tile * 2 * tp.tokens;
         row = in && tok < a.Tq ? row_index(a, (int64_t)b * a.Tq + tok, h, g) : a.rows;
     }
-    if (row >= a.rows) return;
-    float x[kPer];
+    float acc[E] = {}, total = 0.0f, top = -INFINITY;
+    if (row < a.rows) {
+        float x[kPer];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        x[i] = -INFINITY;
-        if (32 * i < parts && lane + 32 * i < parts) x[i] = a.part_lse[(int64_t)(lane + 32 * i) * a.rows + row];
-    }
-    float top = x[0];
-    bool bad = x[0] != x[0];
+        for (int i = 0; i < kPer; ++i) {
+            x[i] = -INFINITY;
+            if (32 * i < parts && lane + 32 * i < parts) x[i] = a.part_lse[(int64_t)(lane + 32 * i) * a.rows + row];
+        }
+        bool bad = false;
 #pragma unroll
-    for (int i = 1; i < kPer; ++i) top = fmaxf(top, x[i]), bad = bad || x[i] != x[i];
+        for (int i = 0; i < kPer; ++i) top = fmaxf(top, x[i]), bad = bad || x[i] != x[i];
 #pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
-    float acc[E] = {}, total = 0.0f;
-    if (__any_sync(0xFFFFFFFFu, bad)) {  // a part is NaN: so is the row
-        total = NAN;
-    } else if (top != -INFINITY) {
+        for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
         int best = 0;
 #pragma unroll
         for (int i = kPer - 1; i >= 0; --i) {
+            if (32 * i >= parts) continue;
             const uint32_t at = __ballot_sync(0xFFFFFFFFu, x[i] == top);
             if (at) best = 32 * i + __ffs(at) - 1;
+            weight[warp][32 * i + lane] = top == -INFINITY ? 0.0f : exp2f(x[i] - top);  // past the parts: 0
         }
+        __syncwarp();
+        if (__any_sync(0xFFFFFFFFu, bad)) {  // a part is NaN: so is the row
+            total = NAN;
+        } else {
+            for (int c0 = 8 * sub; c0 < parts; c0 += 8 * spread) {
+                float v[8][E], f[8], some = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            if (32 * i >= parts) break;
-            const float w = exp2f(x[i] - top);
-            const int n = parts - 32 * i < 32 ? parts - 32 * i : 32;
-            for (int c0 = 0; c0 < n; c0 += 8) {
-                float v[8][E], f[8];
+                for (int u = 0; u < 8; ++u) some += f[u] = weight[warp][c0 + u];
+                if (some == 0.0f) continue;
 #pragma unroll
                 for (int u = 0; u < 8; ++u) {
-                    f[u] = __shfl_sync(0xFFFFFFFFu, w, c0 + u);  // past the parts: exp2(-inf) = 0
-                    const int c = f[u] > 0.0f ? 32 * i + c0 + u : best;
+                    const int c = f[u] > 0.0f ? c0 + u : best;
                     const float* src = a.part_o + ((int64_t)c * a.rows + row) * D + lane * E;
                     if constexpr (E == 4) {
                         const float4 y = __ldcs(reinterpret_cast<const float4*>(src));
@@ -305,6 +333,19 @@ __global__ void __launch_bounds__(256) prefix_finish_kernel(const PrefixArgs a, 
             }
         }
     }
+    if (spread > 1) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) sums[warp][lane * E + e] = acc[e];
+        if (lane == 0) totals[warp] = total;
+        __syncthreads();
+        if (sub != 0) return;
+        for (int w = warp + 1; w < warp + spread; ++w) {
+            total += totals[w];
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] += sums[w][lane * E + e];
+        }
+    }
+    if (row >= a.rows) return;
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     T* dst = static_cast<T*>(a.out) + row * D + lane * E;
 #pragma unroll
@@ -340,12 +381,16 @@ template <typename T>
 int finish_d(const PrefixArgs& a, const TilePlan& tp, int D, const RowsPlan& rp, const float* scores,
              float* scores_out, cudaStream_t stream) {
     const int64_t rows = tp.whole ? ((int64_t)a.B * a.Hkv * tp.seq_tiles - tp.whole) * 256 : a.rows;
-    const int64_t blocks = (rows + 7) / 8;
-    const int64_t weights = rp.logits ? (int64_t)a.B * a.Hkv * (((int64_t)a.T + kWeightKeys - 1) / kWeightKeys) : 0;
+    const int parts = a.parts_p + a.parts_o;
+    int spread = 1;  // warps of a row: no more than the groups of eight parts, while the rows leave SMs idle
+    while (spread < 8 && 8 * spread < parts && rows * spread < 8 * kSMs) spread *= 2;
+    const int64_t blocks = (rows * spread + 7) / 8;
+    const int64_t keys = 1024 / weight_groups(a.Tq * a.G);
+    const int64_t weights = rp.logits ? (int64_t)a.B * a.Hkv * (((int64_t)a.T + keys - 1) / keys) : 0;
     if (blocks + weights > INT32_MAX) return LSA_ERR_SIZE;
     auto kern = D == 128 ? prefix_finish_kernel<T, 128> : prefix_finish_kernel<T, 64>;
-    return launch_after(kern, dim3((unsigned)(blocks + weights)), 256, 0, stream, a, tp, a.parts_p + a.parts_o, rp,
-                        (unsigned)weights, scores, scores_out);
+    return launch_after(kern, dim3((unsigned)(blocks + weights)), 256, 0, stream, a, tp, parts, rp,
+                        (unsigned)weights, spread, scores, scores_out);
 }
 
 struct Plan {
@@ -356,7 +401,6 @@ struct Plan {
     RowsPlan rows;
 };
 
-constexpr int kSMs = 148;
 constexpr int kItemsAPlace = 2;
 
 // Splits of the few-row kernel for `items` of `chunks` steps of 64 keys. One length: 256 CTAs draw the
