@@ -6,7 +6,7 @@
 // -NaN < -inf < ... < -0 < +0 < ... < +inf < +NaN), ties go to the lower index. The kept keys
 // keep their order: out slot m holds kept key ids[m], ascending; slots past the kept count are
 // zeros (ids -1).
-#include "common.cuh"
+#include "launch.cuh"
 
 namespace lsa {
 namespace {
@@ -337,8 +337,7 @@ int lsa_evict(const void* k, const void* v, int64_t row_bytes, const int64_t* st
     const int64_t slice = sliced ? (T + ranks - 1) / ranks : T;
     const int smem = (int)((slice < kCached ? slice : kCached) * 4);
     auto kern = sliced ? evict_kernel<true> : evict_kernel<false>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kCached * 4) != cudaSuccess ||
-        cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+    if (!(sliced ? allow_kernel<evict_kernel<true>>(kCached * 4, true) : allow_kernel<evict_kernel<false>>(kCached * 4)))
         return LSA_ERR_CUDA;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;

@@ -13,9 +13,7 @@
 
 #include <stdint.h>
 
-#include <atomic>
-
-#include "common.cuh"
+#include "launch.cuh"
 
 namespace lsa {
 
@@ -68,38 +66,6 @@ __device__ __forceinline__ void seq_tile(const PrefixArgs& a, const TilePlan& t,
     *h = i % a.Hkv, i /= a.Hkv;
     *b = i % a.B;
     *tile = t.seq_tiles - 1 - i / a.B;
-}
-
-// Launch that may start while the kernel before it drains (programmatic dependent launch): the
-// kernel waits (griddepcontrol.wait) before it touches what an earlier kernel writes.
-template <typename K, typename... A>
-int launch_after(K kern, dim3 grid, unsigned threads, size_t smem, cudaStream_t stream, const A&... args) {
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess ? LSA_OK : LSA_ERR_CUDA;
-}
-
-__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void grid_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
-// A kernel's shared-memory limit raised once per device (the call costs about a microsecond).
-template <auto kKernel> bool allow_smem(int bytes) {
-    static std::atomic<uint64_t> done{0};
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return false;
-    const uint64_t bit = 1ull << (dev & 63);
-    if (done.load() & bit) return true;
-    if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
-    done.fetch_or(bit);
-    return true;
 }
 
 // Splits of `chunks` for `items` equal work items on `slots` places that hold one item each: the

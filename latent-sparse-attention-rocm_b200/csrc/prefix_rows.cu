@@ -29,6 +29,13 @@ template <int D> struct RowsShape {
     static_assert(kWarpBytes >= kRows * D * 4, "the join reuses a warp's ring");
 };
 
+// 16-byte copy under an L2 policy; src_bytes 0 zero-fills without reading.
+__device__ __forceinline__ void cp_async16_hint(uint32_t dst, const void* src, uint32_t src_bytes, uint64_t policy) {
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src),
+                 "r"(src_bytes), "l"(policy)
+                 : "memory");
+}
+
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -104,6 +111,12 @@ __global__ void __launch_bounds__(kWarps * 32, 2) prefix_rows_kernel(const Prefi
     // (32 / C)-th row
     const int tiles = k1 - k0 > warp * kKeys ? (k1 - k0 - warp * kKeys + kWarps * kKeys - 1) / (kWarps * kKeys) : 0;
     const int lc = lane % C, lr = lane / C;
+    // keys that nothing reads again leave L2 before the logits do
+    uint64_t policy;
+    if (own && rp.logits && rp.own_tiles == 1)
+        asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+    else
+        asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy));
     auto copy = [&](int i) {
         if (i < tiles) {
             const int key0 = k0 + (warp + kWarps * i) * kKeys;
@@ -114,8 +127,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) prefix_rows_kernel(const Prefi
                 const bool in = key < k1;
                 const int64_t at = in ? key : k0;
                 const uint32_t to = dst + row * D * 2 + ((lc ^ (row & 7)) << 4);
-                cp_async16(to, kb + at * kt + lc * 8, in ? 16u : 0u);
-                cp_async16(to + Sh::kTile, vb + at * vt + lc * 8, in ? 16u : 0u);
+                cp_async16_hint(to, kb + at * kt + lc * 8, in ? 16u : 0u, policy);
+                cp_async16_hint(to + Sh::kTile, vb + at * vt + lc * 8, in ? 16u : 0u, policy);
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -269,7 +282,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) prefix_rows_kernel(const Prefi
 
 template <typename T, int D>
 int launch(const PrefixArgs& a, const RowsPlan& rp, unsigned grid, cudaStream_t stream) {
-    if (!allow_smem<prefix_rows_kernel<T, D>>(RowsShape<D>::kSmem)) return LSA_ERR_CUDA;
+    if (!allow_kernel<prefix_rows_kernel<T, D>>(RowsShape<D>::kSmem)) return LSA_ERR_CUDA;
     return launch_after(prefix_rows_kernel<T, D>, dim3(grid), kWarps * 32, RowsShape<D>::kSmem, stream, a, rp);
 }
 

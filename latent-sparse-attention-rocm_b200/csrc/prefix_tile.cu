@@ -500,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 template <typename T, int D>
 int launch(const TileMaps& maps, const PrefixArgs& a, const TilePlan& tp, unsigned grid, cudaStream_t stream) {
-    if (!allow_smem<prefix_tile_kernel<T, D>>(TileShape<D>::kSmem)) return LSA_ERR_CUDA;
+    if (!allow_kernel<prefix_tile_kernel<T, D>>(TileShape<D>::kSmem)) return LSA_ERR_CUDA;
     return launch_after(prefix_tile_kernel<T, D>, dim3(grid), kThreads, TileShape<D>::kSmem, stream, maps, a, tp);
 }
 

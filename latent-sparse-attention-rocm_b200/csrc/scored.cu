@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(kWKeys) own_weights_kernel(const PrefixArgs a,
 template <int D>
 int weights_launch(const PrefixArgs& a, const float* scores, float* scores_out, cudaStream_t stream) {
     const int smem = (kWKeys * (D + 4) + kWRows * D) * 4;
-    if (!allow_smem<own_weights_kernel<D>>(smem)) return LSA_ERR_CUDA;
+    if (!allow_kernel<own_weights_kernel<D>>(smem)) return LSA_ERR_CUDA;
     const int64_t grid = ((int64_t)a.T + kWKeys - 1) / kWKeys * a.Hkv * a.B;
     if (grid > INT32_MAX) return LSA_ERR_SIZE;
     own_weights_kernel<D><<<(unsigned)grid, kWKeys, smem, stream>>>(a, scores, scores_out);

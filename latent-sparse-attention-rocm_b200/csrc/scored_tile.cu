@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <typename T, int D>
 int launch(const WeightMaps& maps, const PrefixArgs& a, const WeightPlan& wp, unsigned grid, const float* scores,
            float* scores_out, cudaStream_t stream) {
-    if (!allow_smem<weights_tile_kernel<T, D>>(WeightShape<D>::kSmem)) return LSA_ERR_CUDA;
+    if (!allow_kernel<weights_tile_kernel<T, D>>(WeightShape<D>::kSmem)) return LSA_ERR_CUDA;
     return launch_after(weights_tile_kernel<T, D>, dim3(grid), kThreads, WeightShape<D>::kSmem, stream, maps, a, wp,
                         scores, scores_out);
 }
