@@ -1,5 +1,10 @@
 // prefix.cu - attention over a shared prefix and each sequence's own cache: the entry points,
 // the fp32 kernel and the join of the parts (sm_100a). prefix.cuh has the formulas.
+//
+// Which kernel reads which segment (make_plan): fp32 inputs the FMA-pipe kernel here; 16-bit inputs
+// segments of up to 16 rows a KV head (64 where the keys are few) the few-row kernel, others the
+// tensor-core kernel; sequences whose rows fill tiles by themselves read prefix and own keys in one
+// item and, but for the last round of tiles, write the output at once.
 #include <math.h>
 
 #include "prefix.cuh"

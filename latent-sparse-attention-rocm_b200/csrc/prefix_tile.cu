@@ -21,6 +21,15 @@
 // order the MMAs use them), one thread of warp 1 issues every MMA (unrolled: 64 cycles per 128 x 128 x
 // 16 MMA, the pipe's rate), 2 zeroes a sequence's V tail, 4-7 / 8-11 are the softmax of half 0 / 1. TMEM: S_0/P_0 [0, 128),
 // S_1/P_1 [128, 256), O_0 [256, 256 + D), O_1 [384, 384 + D).
+// What bounds it: with two halves of rows, the chain of a half - S (8 MMAs, 512 cycles), its softmax (about
+// 1400 cycles to the first 96 keys' P, 2200 with the other half's exponentials beside it), the rest
+// of P V - of which two run at a time: 3000 cycles a pair of chunks, where the MMAs alone take 2048; over
+// seconds, the power limit (SM clock 1.55 GHz). 148 tiles on 4096 keys: tensor pipe 62 % active, 64 % of
+// the exponential units. 64 tokens of 32 sequences on 10007 prefix keys (32 / 8 heads, D 128): 302 us =
+// 1.16 PFLOP/s, 70 % of the measured burst rate and 82 % of the sustained one. With two streams, the
+// keys: 50 GB/s an SM, 6.4 TB/s while the ring runs.
+// Not kept: a part of the exponentials as polynomials on the FMA pipe (every 8th pair: no change, every
+// 4th 3 % slower, every 2nd 15 %); a polling MMA thread in place of try_wait (no change).
 // Rows of V at or past a sequence's length are zeroed in shared memory before their product, so
 // whatever an unwritten slot holds (0 x NaN) stays out.
 //
