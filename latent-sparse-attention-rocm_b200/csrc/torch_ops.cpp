@@ -8,7 +8,8 @@
 //                     sink, top_k) -> (lists, lengths)          flat_select fused, pipeline.py:274-316
 //                     (index_queries [R, d], or raw queries [R, Hq, D]: regroup fused in)
 //   lsa::sparse_read(q, k, v, ids, lengths, scale) -> out     sparse_read_auto, read_kernel_tiled.py:147
-//   lsa::shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths, scale, return_lse) -> (out, lse)
+//   lsa::shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths, scale) -> out
+//   lsa::shared_prefix_attention_lse(the same) -> (out, lse)
 //   lsa::scored_attention(q, k, v, lengths, scores, scale, k_prefix, v_prefix) -> (out, scores)
 //   lsa::evict(k, v, scores, lengths, budget, window, sink, capacity)
 //                     -> (k, v, scores, lengths, ids)            no reference counterpart
@@ -18,6 +19,7 @@
 // per (device, stream), grown on demand - the same contract as the C ABI's callers keep.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 
@@ -201,6 +203,11 @@ at::Tensor rows16(const at::Tensor& t) {
 // stride of a dimension; 0 where the dimension has one entry and any stride would do
 int64_t stride_of(const at::Tensor& t, int64_t i) { return t.size(i) == 1 ? 0 : t.stride(i); }
 
+// an uninitialised tensor on a CUDA device, past the dispatcher (half a microsecond each)
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType dtype, const at::Device& dev) {
+    return at::Tensor(at::detail::empty_cuda(sizes, dtype, dev, std::nullopt));
+}
+
 at::Tensor as_lengths(const at::Tensor& t) {
     return t.scalar_type() == at::kInt && t.is_contiguous() ? t : t.to(at::kInt).contiguous();
 }
@@ -243,8 +250,8 @@ PrefixOut prefix_attention(const at::Tensor& q_in, const at::Tensor* kp_in, cons
     if (B > 1 && Tq > 1 && q.stride(0) != Tq * q.stride(1)) q = q.contiguous();  // tokens one stride apart
     auto lengths = as_lengths(lengths_in);
     PrefixOut r;
-    r.out = at::empty({B, Tq, Hq, D}, q.options());
-    if (want_lse) r.lse = at::empty({B, Tq, Hq}, q.options().dtype(at::kFloat));
+    r.out = fresh({B, Tq, Hq, D}, q.scalar_type(), q.device());
+    if (want_lse) r.lse = fresh({B, Tq, Hq}, at::kFloat, q.device());
     at::Tensor scores;
     if (scores_in) {
         TORCH_CHECK_VALUE(scores_in->device() == q_in.device() && scores_in->scalar_type() == at::kFloat &&
@@ -252,7 +259,7 @@ PrefixOut prefix_attention(const at::Tensor& q_in, const at::Tensor* kp_in, cons
                               scores_in->size(2) == T,
                           what, ": scores [B, Hkv, T] fp32");
         scores = scores_in->contiguous();
-        r.scores = B * Tq == 0 ? scores.clone() : at::empty_like(scores);
+        r.scores = B * Tq == 0 ? scores.clone() : fresh({B, Hkv, T}, at::kFloat, q.device());
     }
     if (B * Tq == 0) return r;
     const int code = dtype_code(q.scalar_type());
@@ -275,11 +282,17 @@ PrefixOut prefix_attention(const at::Tensor& q_in, const at::Tensor* kp_in, cons
     return r;
 }
 
-std::tuple<at::Tensor, at::Tensor> shared_prefix_cuda(const at::Tensor& q, const at::Tensor& kp, const at::Tensor& vp,
-                                                      const at::Tensor& k, const at::Tensor& v,
-                                                      const at::Tensor& lengths, double scale, bool return_lse) {
-    auto r = prefix_attention(q, &kp, &vp, k, v, lengths, nullptr, scale, return_lse, "shared_prefix_attention");
-    return {r.out, return_lse ? r.lse : at::empty({0}, q.options().dtype(at::kFloat))};
+at::Tensor shared_prefix_cuda(const at::Tensor& q, const at::Tensor& kp, const at::Tensor& vp, const at::Tensor& k,
+                              const at::Tensor& v, const at::Tensor& lengths, double scale) {
+    return prefix_attention(q, &kp, &vp, k, v, lengths, nullptr, scale, false, "shared_prefix_attention").out;
+}
+
+std::tuple<at::Tensor, at::Tensor> shared_prefix_lse_cuda(const at::Tensor& q, const at::Tensor& kp,
+                                                          const at::Tensor& vp, const at::Tensor& k,
+                                                          const at::Tensor& v, const at::Tensor& lengths,
+                                                          double scale) {
+    auto r = prefix_attention(q, &kp, &vp, k, v, lengths, nullptr, scale, true, "shared_prefix_attention");
+    return {r.out, r.lse};
 }
 
 std::tuple<at::Tensor, at::Tensor> scored_cuda(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
@@ -312,9 +325,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> evict_cud
     auto k = rows16(k_in), v = rows16(v_in);
     auto scores = scores_in.contiguous();
     auto lengths = as_lengths(lengths_in);
-    auto ko = at::empty({B, capacity, Hkv, D}, k.options()), vo = at::empty({B, capacity, Hkv, D}, k.options());
-    auto so = at::empty({B, Hkv, capacity}, scores.options());
-    auto lo = at::empty({B}, lengths.options()), ids = at::empty({B, Hkv, capacity}, lengths.options());
+    const auto dev = k.device();
+    auto ko = fresh({B, capacity, Hkv, D}, k.scalar_type(), dev), vo = fresh({B, capacity, Hkv, D}, k.scalar_type(), dev);
+    auto so = fresh({B, Hkv, capacity}, at::kFloat, dev);
+    auto lo = fresh({B}, at::kInt, dev), ids = fresh({B, Hkv, capacity}, at::kInt, dev);
     if (B == 0) return {ko, vo, so, lo, ids};
     const int64_t strides[6] = {stride_of(k, 0) * es, stride_of(k, 1) * es, stride_of(k, 2) * es,
                                 stride_of(v, 0) * es, stride_of(v, 1) * es, stride_of(v, 2) * es};
@@ -353,12 +367,16 @@ at::Tensor sparse_read_meta(const at::Tensor& q, const at::Tensor&, const at::Te
     return at::empty_like(q);
 }
 
-std::tuple<at::Tensor, at::Tensor> shared_prefix_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor&,
-                                                      const at::Tensor&, const at::Tensor&, const at::Tensor&,
-                                                      double, bool return_lse) {
-    auto f32 = q.options().dtype(at::kFloat);
+at::Tensor shared_prefix_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                              const at::Tensor&, const at::Tensor&, double) {
+    return at::empty(q.sizes(), q.options());
+}
+
+std::tuple<at::Tensor, at::Tensor> shared_prefix_lse_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor&,
+                                                          const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                                                          double) {
     return {at::empty(q.sizes(), q.options()),
-            return_lse ? at::empty({q.size(0), q.size(1), q.size(2)}, f32) : at::empty({0}, f32)};
+            at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat))};
 }
 
 std::tuple<at::Tensor, at::Tensor> scored_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor&,
@@ -385,7 +403,9 @@ TORCH_LIBRARY(lsa, m) {
           "int top_p, int window, int sink, int top_k) -> (Tensor, Tensor)");
     m.def("sparse_read(Tensor q, Tensor k, Tensor v, Tensor ids, Tensor lengths, float scale) -> Tensor");
     m.def("shared_prefix_attention(Tensor q, Tensor k_prefix, Tensor v_prefix, Tensor k, Tensor v, Tensor lengths, "
-          "float scale, bool return_lse=False) -> (Tensor, Tensor)");
+          "float scale) -> Tensor");
+    m.def("shared_prefix_attention_lse(Tensor q, Tensor k_prefix, Tensor v_prefix, Tensor k, Tensor v, "
+          "Tensor lengths, float scale) -> (Tensor, Tensor)");
     m.def("scored_attention(Tensor q, Tensor k, Tensor v, Tensor lengths, Tensor scores, float scale, "
           "Tensor? k_prefix=None, Tensor? v_prefix=None) -> (Tensor, Tensor)");
     m.def("evict(Tensor k, Tensor v, Tensor scores, Tensor lengths, int budget, int window, int sink, int capacity) "
@@ -398,6 +418,7 @@ TORCH_LIBRARY_IMPL(lsa, CUDA, m) {
     m.impl("select_fused", &select_fused_cuda);
     m.impl("sparse_read", &sparse_read_cuda);
     m.impl("shared_prefix_attention", &shared_prefix_cuda);
+    m.impl("shared_prefix_attention_lse", &shared_prefix_lse_cuda);
     m.impl("scored_attention", &scored_cuda);
     m.impl("evict", &evict_cuda);
 }
@@ -405,6 +426,7 @@ TORCH_LIBRARY_IMPL(lsa, CUDA, m) {
 // CPU tensors: the operators' own refusal (a ValueError) in place of the dispatcher's
 TORCH_LIBRARY_IMPL(lsa, CPU, m) {
     m.impl("shared_prefix_attention", &shared_prefix_cuda);
+    m.impl("shared_prefix_attention_lse", &shared_prefix_lse_cuda);
     m.impl("scored_attention", &scored_cuda);
     m.impl("evict", &evict_cuda);
 }
@@ -414,6 +436,7 @@ TORCH_LIBRARY_IMPL(lsa, Meta, m) {
     m.impl("select_fused", &select_fused_meta);
     m.impl("sparse_read", &sparse_read_meta);
     m.impl("shared_prefix_attention", &shared_prefix_meta);
+    m.impl("shared_prefix_attention_lse", &shared_prefix_lse_meta);
     m.impl("scored_attention", &scored_meta);
     m.impl("evict", &evict_meta);
 }

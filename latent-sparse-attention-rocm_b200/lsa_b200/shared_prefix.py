@@ -26,6 +26,8 @@ def shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths, scale=None, re
     ``D ** -0.5``. Output like q, contiguous; with ``return_lse`` also the natural
     log-sum-exp of every row's scaled logits, fp32 [B, Tq, Hq]."""
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
-    out, lse = _lib.torch_ops().shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths, scale, return_lse)
+    ops = _lib.torch_ops()
+    fn = ops.shared_prefix_attention_lse if return_lse else ops.shared_prefix_attention
+    out = fn(q, k_prefix, v_prefix, k, v, lengths, scale)
     _lib.after_call(q.device, "shared_prefix_attention")
-    return (out, lse) if return_lse else out
+    return out

@@ -19,7 +19,8 @@ def _prefix_args(device, B=2, Tq=1, Hq=8, Hkv=2, D=128, P=16, T=8, dt=torch.bflo
 def test_meta_shapes():
     ops = _lib.torch_ops()
     a = _prefix_args("meta", Tq=3)
-    out, lse = ops.shared_prefix_attention(*a, 0.1, True)
+    out, lse = ops.shared_prefix_attention_lse(*a, 0.1)
+    assert ops.shared_prefix_attention(*a, 0.1).shape == a[0].shape
     assert out.shape == a[0].shape and out.dtype == a[0].dtype
     assert lse.shape == (2, 3, 8) and lse.dtype == torch.float32
     s = torch.empty(2, 2, 8, device="meta")
