@@ -108,7 +108,7 @@ __device__ __forceinline__ void copy_rows(const EvictArgs& a, int b, int h, int 
 // bins' owner, one cluster barrier a pass) and their kept counts.
 // Selection is a chain of short steps, the copy is bandwidth: with several CTAs an SM one row's
 // copy covers another's chain. Measured (D 128, bf16): 64 ragged caches of up to 8191 keys, 8 heads, to 2048:
-// 185 us = 5.9 TB/s; 4 of 131072 to 8192: 76 us, of which the selection takes about 28 (the rows are
+// 185 us = 5.9 TB/s; 4 of 131072 to 8192: 70 us, of which the selection takes about 23 (the rows are
 // in lock-step: 256 CTAs, 32 keys a thread) and 268 MB of copying the rest; one of 2112 to 2048: 9.6 us,
 // 7 of them selection (load 1.9, a pass 1.1, counts and ids 1.7).
 template <bool kSliced>
@@ -163,11 +163,16 @@ __global__ void __launch_bounds__(kThreads, 2) evict_kernel(const EvictArgs a, i
         }
         // f(j, key) for the warp's keys, 32 consecutive ones a step (j at or past w1: no key)
         auto each = [&](auto f) {
-#pragma unroll 2
-            for (int j0 = w0; j0 < w1; j0 += 32) {
-                const int j = j0 + lane;
-                f(j, j < w1 ? key_at(j) : 0u);
+            int j = w0 + lane;
+            for (; j - lane + 128 <= (w1 < s0 + kCached ? w1 : s0 + kCached); j += 128) {
+                uint32_t u[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) u[q] = keys[j - s0 + 32 * q];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) f(j + 32 * q, u[q]);
             }
+#pragma unroll 1
+            for (; j - lane < w1; j += 32) f(j, j < w1 ? key_at(j) : 0u);
         };
         if (kSliced) {
             for (int i = tid; i < 3 * kBins / 2; i += kThreads) joined[i] = 0;
@@ -184,10 +189,20 @@ __global__ void __launch_bounds__(kThreads, 2) evict_kernel(const EvictArgs a, i
                 shift -= width;
                 *reinterpret_cast<int4*>(hist + 4 * tid) = make_int4(0, 0, 0, 0);
                 __syncthreads();
-                for (int j = (s0 > lo ? s0 : lo) + tid; j < s1 && j < hi; j += kThreads) {
-                    const uint32_t u = key_at(j);
+                const int end = s1 < hi ? s1 : hi;
+                auto count = [&](uint32_t u) {
                     if (pass == 0 || (u >> up) == cut) atomicAdd(&hist[(u >> shift) & ((1u << width) - 1)], 1);
+                };
+                int j = (s0 > lo ? s0 : lo) + tid;
+                // four loads before their adds (which the compiler may not move them across)
+                for (; j + 3 * kThreads < (end < s0 + kCached ? end : s0 + kCached); j += 4 * kThreads) {
+                    uint32_t u[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) u[q] = keys[j - s0 + q * kThreads];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) count(u[q]);
                 }
+                for (; j < end; j += kThreads) count(key_at(j));
                 __syncthreads();
                 // bins in descending order, four a thread
                 const int at = kBins - 4 - 4 * tid;
@@ -305,7 +320,7 @@ int lsa_evict(const void* k, const void* v, int64_t row_bytes, const int64_t* st
     if (B < 0 || T < 0 || Hkv <= 0 || row_bytes <= 0 || row_bytes % 16 || row_bytes > 65536) return LSA_ERR_ARG;
     if (window < 0 || sink < 0 || budget < 0 || window > budget || sink > budget - window || capacity < budget)
         return LSA_ERR_ARG;
-    if (T > INT32_MAX - 4096 || capacity > INT32_MAX - 4096 || strides == nullptr) return LSA_ERR_ARG;
+    if (T > INT32_MAX - (1 << 16) || capacity > INT32_MAX - (1 << 16) || strides == nullptr) return LSA_ERR_ARG;
     for (int i = 0; i < 6; ++i)
         if (strides[i] < 0 || strides[i] % 16) return LSA_ERR_ARG;
     if (B == 0) return LSA_OK;
