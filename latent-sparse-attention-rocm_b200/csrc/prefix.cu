@@ -388,7 +388,7 @@ int finish_d(const PrefixArgs& a, const TilePlan& tp, int D, const RowsPlan& rp,
     const int64_t rows = tp.whole ? ((int64_t)a.B * a.Hkv * tp.seq_tiles - tp.whole) * 256 : a.rows;
     const int parts = a.parts_p + a.parts_o;
     int spread = 1;  // warps of a row: no more than the groups of eight parts, while the rows leave SMs idle
-    while (spread < 8 && 8 * spread < parts && rows * spread < 8 * kSMs) spread *= 2;
+    while (spread < 8 && 8 * spread < parts && rows * spread < 16 * kSMs) spread *= 2;
     const int64_t blocks = (rows * spread + 7) / 8;
     const int64_t keys = 1024 / weight_groups(a.Tq * a.G);
     const int64_t weights = rp.logits ? (int64_t)a.B * a.Hkv * (((int64_t)a.T + keys - 1) / keys) : 0;
