@@ -266,7 +266,10 @@ PrefixOut prefix_attention(const at::Tensor& q_in, const at::Tensor* kp_in, cons
     const int64_t bytes = lsa_shared_prefix_scratch(code, B, Tq, Hq, Hkv, D, P, T, scores_in != nullptr);
     TORCH_CHECK_VALUE(bytes >= 0, what, ": sizes out of range");
     auto stream = at::cuda::getCurrentCUDAStream();
-    Workspace& w = workspace(q.device(), stream, bytes, 64);
+    // The parts' scratch is the call's own: it may be gigabytes, and one kept for the stream would have to
+    // move when a larger call comes, under the feet of a captured graph. The status word is kept.
+    auto scratch = fresh({bytes}, at::kByte, q.device());
+    Workspace& w = workspace(q.device(), stream, 0, 64);
     const int64_t strides[13] = {stride_of(q, 0), stride_of(q, 1), stride_of(q, 2), P ? stride_of(kp, 0) : 0,
                                  P ? stride_of(kp, 1) : 0, P ? stride_of(vp, 0) : 0, P ? stride_of(vp, 1) : 0,
                                  stride_of(k, 0), stride_of(k, 1),
@@ -276,8 +279,8 @@ PrefixOut prefix_attention(const at::Tensor& q_in, const at::Tensor* kp_in, cons
                                          strides, lengths.data_ptr<int32_t>(), B, Tq, Hq, Hkv, D, P, T, (float)scale,
                                          r.out.data_ptr(), want_lse ? r.lse.data_ptr<float>() : nullptr,
                                          scores_in ? scores.data_ptr<float>() : nullptr,
-                                         scores_in ? r.scores.data_ptr<float>() : nullptr, w.scratch.data_ptr(),
-                                         w.scratch.numel(), w.counters.data_ptr<int32_t>(), stream),
+                                         scores_in ? r.scores.data_ptr<float>() : nullptr, scratch.data_ptr(), bytes,
+                                         w.counters.data_ptr<int32_t>(), stream),
              what);
     return r;
 }

@@ -288,6 +288,31 @@ def test_other_stream_and_graph(lsa, case):
     lsa.check_status()
 
 
+def test_a_larger_call_leaves_a_captured_graph_alone(lsa):
+    """A captured call replays the same bits after larger eager calls on its stream and after what
+    they freed has been written over."""
+    args = make(4, 1, 32, 8, 128, 1000, 200, BF, seed=18)
+    call = lambda a: lsa.scored_attention(a[0], a[3], a[4], a[5], a[6], k_prefix=a[1], v_prefix=a[2])
+    expect = [x.clone() for x in call(args)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(args)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = call(args)
+    big = make(24, 33, 32, 8, 128, 2000, 900, BF, seed=19)
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            call(big)
+        junk = [torch.full((1 << 22,), 255, dtype=torch.uint8, device=DEV) for _ in range(64)]
+        graph.replay()
+        same = [bool((x == 255).all()) for x in junk]
+    side.synchronize()
+    assert torch.equal(got[0], expect[0]) and torch.equal(got[1], expect[1]) and all(same)
+
+
 @pytest.mark.parametrize("Hq,own", [(8, False), (128, False), (8, True), (128, True)])
 def test_offsets_past_32_bits(lsa, Hq, own):
     """A cache of more than 2^31 elements: the last keys hold the weight."""
