@@ -210,8 +210,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ok = ok && role_wait(&sfull[buf], (it >> 1) & 1, abort_flag);
                 if (!ok) continue;
                 tc_fence_after();
-                const int64_t before = first - (int64_t)t * tile_rows;
-                const int hide = before > 128 ? 128 : (int)before;  // columns below it are hidden
+                const int64_t before = first - (int64_t)t * tile_rows;  // keys x heads: past 32 bits either way
+                const int hide = before > 128 ? 128 : (before < 0 ? 0 : (int)before);  // columns below it are hidden
                 const bool masked = __any_sync(0xFFFFFFFFu, hide > 0);
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
