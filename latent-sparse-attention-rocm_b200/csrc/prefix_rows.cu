@@ -8,7 +8,9 @@
 // keys (cp.async, 16 bytes, three stages of 8 KB in flight per warp, two CTAs an SM) and runs its
 // own online softmax on them: S = Q K^T and O += P V by mma.sync.m16n8k16 (one M = 16 tile holds
 // all rows; a 128-row tcgen05 tile would be 1/8 full or less and pass through TMEM), maximum and
-// sum in fp32 registers, P rounded to the inputs' type for its product. The warps join through
+// sum in fp32 registers, P rounded to the inputs' type for its product (fp16: times 2^15 first, the most
+// that it holds, or a weight below 2^-25 of the maximum would leave O and stay in the sum; the factor is in
+// both and cancels). The warps join through
 // shared memory at the end. Measured (32 / 8 heads, D 128, bf16, the join of the parts included): 48
 // ragged caches of up to 8191 keys, 1.19 GB, 181 us = 6.6 TB/s, the measured copy rate; 16 of 6144 keys 80
 // us = 5.1 TB/s; one of 24576 keys 24 us, of which 15 are the memory's. Keys at or past the range's end are zero-filled by the copy, so what
@@ -23,6 +25,9 @@ constexpr int kWarps = 4;
 constexpr int kRows = 16;
 constexpr int kKeys = 16;  // keys of a warp's tile
 constexpr int kRing = 3;   // tiles in a warp's ring
+
+template <typename T> constexpr float kLift = 0.0f;  // log2 of the factor that the weights carry
+template <> constexpr float kLift<__half> = 15.0f;
 
 template <int D> struct RowsShape {
     static constexpr int kTile = kKeys * D * 2;          // K or V bytes of a tile
@@ -222,8 +227,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2) prefix_rows_kernel(const Prefi
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const float base = m[u] == -INFINITY ? 0.0f : m[u];
-            const float p0 = ex2_approx(s[0][2 * u] - base), p1 = ex2_approx(s[0][2 * u + 1] - base);
-            const float p2 = ex2_approx(s[1][2 * u] - base), p3 = ex2_approx(s[1][2 * u + 1] - base);
+            auto weight = [&](float x) {  // at most 2^kLift, exactly
+                return ex2_approx(kLift<T> == 0.0f ? x - base : (x - base) + kLift<T>);
+            };
+            const float p0 = weight(s[0][2 * u]), p1 = weight(s[0][2 * u + 1]);
+            const float p2 = weight(s[1][2 * u]), p3 = weight(s[1][2 * u + 1]);
             l[u] += (p0 + p1) + (p2 + p3);
             p[u] = pk16(p0, p1, (T*)nullptr);
             p[u + 2] = pk16(p2, p3, (T*)nullptr);
@@ -276,7 +284,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) prefix_rows_kernel(const Prefi
         const int tok = (r0 + r) / a.G;
         const int64_t rid = row_index(a, (int64_t)b * a.Tq + tok, h, r0 + r - tok * a.G);
         const int64_t at = (int64_t)part * a.rows + rid;
-        if (c == 0) a.part_lse[at] = total == 0.0f ? -INFINITY : top + log2f(total);
+        if (c == 0) a.part_lse[at] = total == 0.0f ? -INFINITY : top + (log2f(total) - kLift<T>);
         *reinterpret_cast<float4*>(a.part_o + at * D + c) = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
     }
     if (rp.follows && blockIdx.x == gridDim.x - 1) grid_wait();

@@ -8,7 +8,7 @@
 // One CTA per item, two halves of 128 rows (M = 128 each):
 //   S_h = Q_h K^T   tcgen05.mma kind::f16, Q and K in 128B-swizzled shared memory, S in TMEM
 //   softmax         one thread per row: S row from TMEM, running maximum and sum in fp32 (exp2
-//                   domain; O is rescaled only when the maximum has grown by more than 2^8), P
+//                   domain; O is rescaled only when the maximum has grown by more than 2^kGrow), P
 //                   back over S as 16-bit pairs
 //   O_h += P_h V    tcgen05.mma with A = P from TMEM, V an MN-major shared-memory operand
 // With more than 128 rows the halves are different rows of the same chunks; with at most 128 both
@@ -42,6 +42,15 @@ namespace lsa {
 namespace {
 
 constexpr int kThreads = 384;
+
+// log2 of the factor that the weights carry into P and the sum, and of the growth of a row's maximum that is
+// let stand: bf16 has fp32's exponents; fp16 holds nothing below 2^-25, so its weights are 2^7 times as large
+// (2^-32 of the maximum is kept) and reach 2^11, which leaves 2^4 for the rounding of huge logits.
+template <typename T> constexpr float kLift = 0.0f;
+template <> constexpr float kLift<__half> = 7.0f;
+template <typename T> constexpr float kGrow = 8.0f;
+template <> constexpr float kGrow<__half> = 4.0f;
+
 struct TileMaps {
     CUtensorMap kp, vp, k, v, q;
 };
@@ -127,7 +136,7 @@ __device__ __forceinline__ void softmax_half(const PrefixArgs& a, const TilePlan
     const int step = w.streams ? 2 : 1, first = w.c0 + (w.streams ? hf : 0);
     const int n = w.c1 > first ? (w.c1 - first + step - 1) / step : 0;
     float m = -INFINITY, l = 0.0f;
-    const float sl = a.scale_log2, thresh = fminf(8.0f / sl, 1e30f);
+    const float sl = a.scale_log2, thresh = fminf(kGrow<T> / sl, 1e30f);
     bool ok = true;
     auto publish = [&](uint64_t* bar) {  // this warp's P so far: one arrival a warp
         tmem_wait_st();
@@ -150,7 +159,7 @@ __device__ __forceinline__ void softmax_half(const PrefixArgs& a, const TilePlan
         }
         // The exponentials start from the maximum of the chunks before, while this chunk's is
         // found beside them (a longest path of 64 dependent steps otherwise): fp32 and 16-bit P
-        // carry a factor of up to 2^8 as well as 1. Only when the maximum has grown by more does
+        // carry a factor of up to 2^kGrow as well as 1. Only when the maximum has grown by more does
         // the warp take the new one, do the first 96 keys again and rescale O - always on a row's
         // first chunk.
         float alpha = 1.0f;
@@ -167,7 +176,7 @@ __device__ __forceinline__ void softmax_half(const PrefixArgs& a, const TilePlan
         uint64_t neg2;
 #pragma unroll 1
         for (bool again = false;; again = true) {
-            const float neg = m == -INFINITY ? 0.0f : -m * sl;
+            const float neg = (m == -INFINITY ? 0.0f : -m * sl) + kLift<T>;
             neg2 = pair(neg, neg);
 #pragma unroll
             for (int i = 0; i < 4; ++i) sum[i] = 0ull;
@@ -225,7 +234,7 @@ __device__ __forceinline__ void softmax_half(const PrefixArgs& a, const TilePlan
     const int64_t rid = row_index(a, (int64_t)w.b * a.Tq + tok, w.h, g);
     const bool none = l == 0.0f;  // the row has seen no key (a NaN logit makes l NaN, and the output)
     const float inv = none ? 0.0f : 1.0f / l;
-    const float lse = none ? -INFINITY : m * sl + log2f(l);
+    const float lse = none ? -INFINITY : m * sl + (log2f(l) - kLift<T>);
     const int64_t at = (int64_t)(w.part + (w.streams ? hf : 0)) * a.rows + rid;
     if (live) {
         if (w.direct) {

@@ -1,11 +1,13 @@
 """Edges of the shared-prefix attention, the scored attention and the budgeted cache on the GPU."""
 
+import math
+
 import pytest
 import torch
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
-BF = torch.bfloat16
+BF, HF = torch.bfloat16, torch.float16
 
 
 def test_scores_where_keys_times_heads_pass_32_bits(lsa):
@@ -18,3 +20,58 @@ def test_scores_where_keys_times_heads_pass_32_bits(lsa):
     out, got = lsa.scored_attention(q, k, k, torch.tensor([n], device=DEV), scores)
     assert (out == 0).all()
     assert float((got.double() * n / 64 - 1).abs().max()) <= 2e-4
+
+
+def light_tail(B, Tq, Hq, Hkv, D, P, T):
+    """Every 2048 keys four heavy ones of value zero (16 keys apart), the others 2^-25.3 of their
+    weight and all of the output. A key that nothing but the first component tells apart, so a row's
+    logits are exact products."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(P + T)
+
+    def cache(*shape):
+        n = shape[-3]
+        j = torch.arange(n, device=DEV)
+        heavy = ((j % 16 == 3) & (j // 64 % 32 == 0)).view(*([1] * (len(shape) - 3)), n, 1, 1)
+        k = torch.zeros(*shape, device=DEV)
+        k[..., 0] = torch.where(heavy[..., 0], 25.3 * math.log(2.0) / 8.0, 0.0)
+        v = torch.where(heavy, 0.0, 40.0 + 20.0 * torch.rand(*shape, generator=g, device=DEV))
+        return k.to(HF), v.to(HF)
+
+    q = torch.randn(B, Tq, Hq, D, generator=g, device=DEV)
+    q[..., 0] = 8.0
+    lengths = torch.randint(min(Tq, T), T + 1, (B,), generator=g, device=DEV, dtype=torch.int32)
+    return (q.to(HF), *cache(P, Hkv, D), *cache(B, T, Hkv, D), lengths)
+
+
+@pytest.mark.parametrize("case", [
+    (1, 1, 4, 1, 128, 400000, 64),   # few rows, the prefix
+    (8, 1, 8, 8, 64, 0, 70000),      # few rows, own caches
+    (1, 1, 32, 1, 128, 400000, 64),  # one half's rows, two streams of chunks
+    (2, 100, 8, 2, 64, 100000, 500), # row tiles of a sequence that read the prefix, split
+    (37, 64, 16, 4, 128, 20000, 64), # the same, whole
+    (1, 40, 8, 2, 128, 0, 60000),    # row tiles of a sequence, own keys alone
+], ids=lambda c: "-".join(map(str, c)))
+def test_light_tails_in_fp16(lsa, case):
+    """Weights far below the row's largest keep their mass. fp16 holds a weight to 2^-25 absolute below
+    2^-14; the kernels scale the weights by 2^7 or more before they round, so a key is off by at most
+    2^-32 of the largest beside the usual bound of the attention's tests (u = 2^-11)."""
+    q, kp, vp, k, v, lengths = light_tail(*case)
+    B, Tq, Hq, D = q.shape
+    P, Hkv, _ = kp.shape
+    G, u = Hq // Hkv, 2.0 ** -11
+    got = lsa.shared_prefix_attention(q, kp, vp, k, v, lengths, 1.0)
+    worst = -math.inf
+    for b in range(B):
+        n = int(lengths[b])
+        for h in range(Hkv):
+            key, val = torch.cat([kp[:, h], k[b, :n, h]]).double(), torch.cat([vp[:, h], v[b, :n, h]]).double()
+            s = q[b, :, h * G:(h + 1) * G].double().reshape(Tq * G, D) @ key.T
+            last = (P + n - Tq + torch.arange(Tq, device=DEV)).repeat_interleave(G)
+            s = s.masked_fill(torch.arange(P + n, device=DEV) > last[:, None], -math.inf)
+            e = torch.exp(s - s.amax(-1, keepdim=True))
+            out = (e @ val) / e.sum(-1, keepdim=True)  # val >= 0: also the sum of p |v|
+            lost = 2.0 ** -32 * val.sum(0) / e.sum(-1, keepdim=True)
+            x = got[b, :, h * G:(h + 1) * G].double().reshape(Tq * G, D)
+            worst = max(worst, float(((x - out).abs() - u * out - (u + 2e-4) * out - lost - 1e-6).max()))
+    assert worst <= 0
