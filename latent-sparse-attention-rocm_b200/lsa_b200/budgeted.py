@@ -12,6 +12,8 @@ the keys that matter least leave. No reference counterpart.
 
 from __future__ import annotations
 
+import math
+
 import torch
 
 from .eviction import evict, scored_attention
@@ -51,18 +53,34 @@ class BudgetedCache:
         self.k, self.v, self.scores, self.lengths = kept.k, kept.v, kept.scores, kept.lengths
         self._longest = min(self._longest, self.budget)
 
+    def _check_step(self, q, k_new, v_new, scale):
+        """ValueError for a step that the writes below would spread over other slots (an indexed write
+        repeats what has one entry) or that the operator would refuse once they are done."""
+        B, _, Hkv, D = self.k.shape
+        if q.dim() != 4 or q.shape[0] != B or q.shape[3] != D or q.shape[2] % Hkv or q.shape[2] < Hkv:
+            raise ValueError(f"a step's q is [{B}, Tq, Hq, {D}], Hq a multiple of {Hkv}, got {list(q.shape)}")
+        want = (B, q.shape[1], Hkv, D)
+        if k_new.shape != want or v_new.shape != want:
+            raise ValueError(f"a step's keys and values are {list(want)}, got {list(k_new.shape)}, {list(v_new.shape)}")
+        if any(t.dtype != self.k.dtype or t.device != self.k.device for t in (q, k_new, v_new)):
+            raise ValueError(f"a step's tensors are {self.k.dtype} on {self.k.device}, as the cache")
+        if scale is not None and not 0.0 < scale < math.inf:
+            raise ValueError(f"the scale must be positive, got {scale}")
+        if q.shape[1] > self.capacity - self.budget:
+            raise ValueError(f"a step of {q.shape[1]} tokens does not fit the room of {self.capacity - self.budget}")
+
     def step(self, q, k_new, v_new, scale=None):
         """Append the step's Tq tokens, attend to the prefix and the own cache, score the keys.
-        Evicts first when the longest sequence has no room for them. Output like q."""
+        Evicts first when the longest sequence has no room for them. q [B, Tq, Hq, D], k_new and
+        v_new [B, Tq, Hkv, D]; a refused step (ValueError) leaves the cache as it was. Output like q."""
+        self._check_step(q, k_new, v_new, scale)
         Tq = q.shape[1]
-        if Tq > self.capacity - self.budget:
-            raise ValueError(f"a step of {Tq} tokens does not fit the room of {self.capacity - self.budget}")
         if self._longest + Tq > self.capacity:
             self._evict()
         at = self.lengths.long()[:, None] + torch.arange(Tq, device=q.device)
-        self.k[self._rows, at], self.v[self._rows, at] = k_new, v_new
-        self.lengths = self.lengths + Tq
+        self.k[self._rows, at], self.v[self._rows, at] = k_new, v_new  # past the lengths: not yet the cache's
+        lengths = self.lengths + Tq
+        out, scores = scored_attention(q, self.k, self.v, lengths, self.scores, scale, self.k_prefix, self.v_prefix)
+        self.lengths, self.scores = lengths, scores
         self._longest += Tq
-        out, self.scores = scored_attention(q, self.k, self.v, self.lengths, self.scores, scale, self.k_prefix,
-                                            self.v_prefix)
         return out

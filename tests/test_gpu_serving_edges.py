@@ -75,3 +75,33 @@ def test_light_tails_in_fp16(lsa, case):
             x = got[b, :, h * G:(h + 1) * G].double().reshape(Tq * G, D)
             worst = max(worst, float(((x - out).abs() - u * out - (u + 2e-4) * out - lost - 1e-6).max()))
     assert worst <= 0
+
+
+def budgeted(lsa, B=3, Hkv=2, D=64, dt=BF):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(5)
+    r = lambda *s: torch.randn(*s, generator=g, device=DEV).to(dt)
+    c = lsa.BudgetedCache(r(B, 90, Hkv, D), r(B, 90, Hkv, D), [90, 64, 10], 64, 8, window_size=8, sink_size=2)
+    return c, r
+
+
+def test_a_refused_step_changes_nothing(lsa):
+    """New keys of another batch or length (which an indexed write would repeat), of another type, a query
+    that the operator refuses: a ValueError, and the cache goes on as if the step had not been tried."""
+    cache, r = budgeted(lsa)
+    twin, _ = budgeted(lsa)
+    B, Hq, Hkv, D = 3, 4, 2, 64
+    first = (r(B, 4, Hq, D), r(B, 4, Hkv, D), r(B, 4, Hkv, D))
+    assert torch.equal(cache.step(*first), twin.step(*first))
+    q, kn, vn = r(B, 5, Hq, D), r(B, 5, Hkv, D), r(B, 5, Hkv, D)  # an eviction is due before it
+    bad = [(q, kn[:, :1], vn[:, :1]), (q, kn[:1], vn[:1]), (q, kn[:, :, :1], vn[:, :, :1]), (q, kn, vn[..., :1]),
+           (q[:1], kn, vn), (q, kn.float(), vn.float()), (q.half(), kn, vn), (q[:, :, :3], kn, vn), (q[0], kn, vn),
+           (q[..., :32], kn, vn), (q, kn.cpu(), vn.cpu()), (q, kn, vn, -1.0), (q, kn, vn, math.nan)]
+    for args in bad:
+        with pytest.raises(ValueError):
+            cache.step(*args)
+        assert torch.equal(cache.lengths, twin.lengths) and torch.equal(cache.scores, twin.scores)
+    n = int(cache.lengths.max())
+    assert torch.equal(cache.k[:, :n], twin.k[:, :n]) and torch.equal(cache.v[:, :n], twin.v[:, :n])
+    assert torch.equal(cache.step(q, kn, vn), twin.step(q, kn, vn))
+    assert torch.equal(cache.scores, twin.scores) and torch.equal(cache.lengths, twin.lengths)
