@@ -504,6 +504,9 @@ bool sizes_ok(int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_t
 
 int64_t round256(int64_t x) { return (x + 255) / 256 * 256; }
 
+constexpr int64_t kWaitNs = 1000000000;
+std::atomic<int64_t> g_wait_ns{kWaitNs};
+
 }  // namespace
 
 int launch_prefix_finish(const PrefixArgs& a, const TilePlan& tp, int dtype, int D, const RowsPlan& rp,
@@ -528,6 +531,12 @@ int64_t lsa_shared_prefix_scratch(int dtype, int64_t B, int64_t Tq, int64_t Hq, 
     const int64_t parts = p.parts_p + p.parts_o;
     return round256(parts * rows * D * 4) + round256(parts * rows * 4) + round256(rows * 4) +
            (p.logits ? round256(rows * p.rows.pitch * 4) : 0);
+}
+
+int lsa_shared_prefix_wait_limit(int64_t limit_ns) {
+    if (limit_ns > 10 * kWaitNs) return LSA_ERR_ARG;
+    g_wait_ns.store(limit_ns < 0 ? kWaitNs : limit_ns, std::memory_order_relaxed);
+    return LSA_OK;
 }
 
 int lsa_shared_prefix_attention(const void* q, const void* k_prefix, const void* v_prefix, const void* k,
@@ -572,6 +581,7 @@ int lsa_shared_prefix_attention(const void* q, const void* k_prefix, const void*
     a.P = (int)P, a.T = (int)T;
     a.Sp = p.Sp, a.So = p.So, a.parts_p = p.parts_p, a.parts_o = p.parts_o;
     a.status = status;
+    a.wait_ns = (uint64_t)g_wait_ns.load(std::memory_order_relaxed);
     a.rows = B * Tq * Hq;
     a.scale_log2 = scale * 1.4426950408889634f;
     uint8_t* s = static_cast<uint8_t*>(scratch);

@@ -39,6 +39,7 @@ struct PrefixArgs {
     int64_t rows;                         // B * Tq * Hq
     float scale_log2;                     // scale * log2(e)
     int32_t* status;                      // LSA_ERR_TIMEOUT after an expired wait
+    uint64_t wait_ns;                     // limit of each wait of the tensor-core kernels
 };
 
 // The work of the tensor-core kernel (prefix_tile.cu). A row tile is two halves of `tokens` tokens,

@@ -33,9 +33,9 @@
 // Rows of V at or past a sequence's length are zeroed in shared memory before their product, so
 // whatever an unwritten slot holds (0 x NaN) stays out.
 //
-// Every wait is bounded (1 s); an expired wait raises a CTA-wide flag, every role leaves, copies
-// and MMAs in flight are waited for (bounded), the TMEM is released and LSA_ERR_TIMEOUT lands in
-// the status word.
+// Every wait is bounded (PrefixArgs::wait_ns, 1 s unless set); an expired wait raises a CTA-wide
+// flag, every role leaves, copies and MMAs in flight are waited for (bounded), the TMEM is released
+// and LSA_ERR_TIMEOUT lands in the status word.
 #include "prefix_umma.cuh"
 
 namespace lsa {
@@ -147,7 +147,7 @@ __device__ __forceinline__ void softmax_half(const PrefixArgs& a, const TilePlan
     for (int j = 0; j < n; ++j) {
         const int c = first + j * step;
         const int seen = c < w.np ? pre_limit - c * kChunk : own_limit - (c - w.np) * kChunk;
-        ok = role_wait(&bar_s[hf], j & 1, abort_flag);
+        ok = role_wait(&bar_s[hf], j & 1, abort_flag, a.wait_ns);
         if (!ok) break;
         tc_fence_after();
         uint32_t s[128];
@@ -229,7 +229,7 @@ __device__ __forceinline__ void softmax_half(const PrefixArgs& a, const TilePlan
         for (int i = 0; i < 4; ++i) unpair(sum[i], x[2 * i], x[2 * i + 1]);
         l = l * alpha + (((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7])));
     }
-    if (ok && n > 0) ok = role_wait(&bar_o[hf], 0, abort_flag);
+    if (ok && n > 0) ok = role_wait(&bar_o[hf], 0, abort_flag, a.wait_ns);
     if (!ok) return;
     const int64_t rid = row_index(a, (int64_t)w.b * a.Tq + tok, w.h, g);
     const bool none = l == 0.0f;  // the row has seen no key (a NaN logit makes l NaN, and the output)
@@ -381,13 +381,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (lane == 0) {
                 int p = early;
                 for (; p < 2 * n; ++p) {
-                    if (!thread_wait(&empty[p % NS], (p / NS - 1) & 1, abort_flag)) break;
+                    if (!thread_wait(&empty[p % NS], (p / NS - 1) & 1, abort_flag, a.wait_ns)) break;
                     load(p);
                 }
-                if (p < 2 * n) {  // every copy issued lands before the CTA leaves
-                    for (int i = p > NS ? p - NS : 0; i < p; ++i) mbar_wait_bounded(&full[i % NS], (i / NS) & 1);
-                    mbar_wait_bounded(bar_q, 0);
-                }
+                // Every copy issued lands before the CTA leaves, also when it was another role that gave up.
+                if (n > 0) mbar_wait_bounded(bar_q, 0);
+                for (int i = p > NS ? p - NS : 0; i < p; ++i) mbar_wait_bounded(&full[i % NS], (i / NS) & 1);
             }
             __syncwarp();
         } else if (warp == 1) {
@@ -418,7 +417,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const uint32_t o = tmem + 256 + hf * 128, p = tmem + hf * 128;
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        if (!thread_wait(&bar_p[2 * hf + half], parity, abort_flag)) return false;
+                        if (!thread_wait(&bar_p[2 * hf + half], parity, abort_flag, a.wait_ns)) return false;
                         tc_fence_after();
 #pragma unroll
                         for (int kk = 6 * half; kk < 6 + 2 * half; ++kk)
@@ -428,19 +427,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                 };
                 // the V tile at the front of the ring; its rows past the sequence's keys zeroed
                 auto value = [&](bool last) -> bool {
-                    if (!thread_wait(&full[stage], phase, abort_flag)) return false;
+                    if (!thread_wait(&full[stage], phase, abort_flag, a.wait_ns)) return false;
                     if (last && tail) {
                         mbar_arrive(bar_tail);
-                        if (!thread_wait(bar_tail + 1, 0, abort_flag)) return false;
+                        if (!thread_wait(bar_tail + 1, 0, abort_flag, a.wait_ns)) return false;
                     }
                     return true;
                 };
                 auto key = [&]() -> bool {
-                    const bool ok = thread_wait(&full[stage], phase, abort_flag);
+                    const bool ok = thread_wait(&full[stage], phase, abort_flag, a.wait_ns);
                     tc_fence_after();
                     return ok;
                 };
-                bool ok = n == 0 || thread_wait(bar_q, 0, abort_flag);
+                bool ok = n == 0 || thread_wait(bar_q, 0, abort_flag, a.wait_ns);
                 if (ok && n > 0 && !w.streams) {
                     ok = key();
                     if (ok) {
@@ -496,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
         } else if (warp == 2 && tail) {
             // ------------------------------------------------ the tail of a sequence's last V tile
-            if (role_wait(bar_tail, 0, abort_flag)) {
+            if (role_wait(bar_tail, 0, abort_flag, a.wait_ns)) {
                 uint8_t* va = sm + Sh::kOffStage + ((2 * n - 1) % NS) * Sh::kTileBytes;  // the last load
                 for (int i = (w.len - (w.c1 - 1 - w.np) * kChunk) * 8 + lane; i < kChunk * 8; i += 32)
 #pragma unroll

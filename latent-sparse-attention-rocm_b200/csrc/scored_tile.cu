@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         int kpos = 0, qpos = 0;
         auto load_k = [&](int t) -> bool {
             const int s = kpos % kKStages;
-            if (kpos >= kKStages && !role_wait(&kempty[s], (kpos / kKStages - 1) & 1, abort_flag)) return false;
+            if (kpos >= kKStages && !role_wait(&kempty[s], (kpos / kKStages - 1) & 1, abort_flag, a.wait_ns)) return false;
             if (lane == 0) {
                 mbar_arrive_expect_tx(&kfull[s], Sh::kTileBytes);
 #pragma unroll
@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         auto load_q = [&](int t) -> bool {
             const int s = qpos % kQStages;
-            if (qpos >= kQStages && !role_wait(&qempty[s], (qpos / kQStages - 1) & 1, abort_flag)) return false;
+            if (qpos >= kQStages && !role_wait(&qempty[s], (qpos / kQStages - 1) & 1, abort_flag, a.wait_ns)) return false;
             if (lane == 0) {
                 mbar_arrive_expect_tx(&qfull[s], tile_rows * D * 2);
 #pragma unroll
@@ -128,12 +128,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!resident)
                 for (int t = 0; ok && t < nr; ++t) ok = load_q(t);
         }
-        if (!ok) {  // every copy issued lands before the CTA leaves
-            for (int p = kpos > kKStages ? kpos - kKStages : 0; p < kpos; ++p)
-                mbar_wait_bounded(&kfull[p % kKStages], (p / kKStages) & 1);
-            for (int p = qpos > kQStages ? qpos - kQStages : 0; p < qpos; ++p)
-                mbar_wait_bounded(&qfull[p % kQStages], (p / kQStages) & 1);
-        }
+        // every copy issued lands before the CTA leaves, whichever role gave up
+        for (int p = kpos > kKStages ? kpos - kKStages : 0; p < kpos; ++p)
+            mbar_wait_bounded(&kfull[p % kKStages], (p / kKStages) & 1);
+        for (int p = qpos > kQStages ? qpos - kQStages : 0; p < qpos; ++p)
+            mbar_wait_bounded(&qfull[p % kQStages], (p / kQStages) & 1);
     } else if (warp == 1) {
         // ---------------------------------------------------- MMAs
         constexpr uint32_t idS = umma_idesc_f16<T>(128, 128, false);
@@ -144,11 +143,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int p = p0; ok && p < p1; ++p, kpos += 2) {
                 for (int t = 0; ok && t < nr; ++t, ++it) {
                     const int q = resident ? t : qpos;
-                    ok = thread_wait(&qfull[q % kQStages], resident ? 0 : (q / kQStages) & 1, abort_flag);
+                    ok = thread_wait(&qfull[q % kQStages], resident ? 0 : (q / kQStages) & 1, abort_flag, a.wait_ns);
                     for (int g = 0; ok && g < 2; ++g) {
                         const int ks = (kpos + g) % kKStages, buf = 2 * g + (it & 1);
-                        if (t == 0) ok = thread_wait(&kfull[ks], ((kpos + g) / kKStages) & 1, abort_flag);
-                        if (ok && it >= 2) ok = thread_wait(&sfree[buf], (it / 2 - 1) & 1, abort_flag);
+                        if (t == 0) ok = thread_wait(&kfull[ks], ((kpos + g) / kKStages) & 1, abort_flag, a.wait_ns);
+                        if (ok && it >= 2) ok = thread_wait(&sfree[buf], (it / 2 - 1) & 1, abort_flag, a.wait_ns);
                         if (!ok) break;
                         tc_fence_after();
                         const uint64_t kd = desc_at(kd0, ks * Sh::kTileBytes);
@@ -207,7 +206,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     nlse[(it & 1) * 128 + tid] = lse_of(t);
                     group_sync();  // also: the buffer of two iterations ago has been read
                 }
-                ok = ok && role_wait(&sfull[buf], (it >> 1) & 1, abort_flag);
+                ok = ok && role_wait(&sfull[buf], (it >> 1) & 1, abort_flag, a.wait_ns);
                 if (!ok) continue;
                 tc_fence_after();
                 const int64_t before = first - (int64_t)t * tile_rows;  // keys x heads: past 32 bits either way

@@ -83,6 +83,7 @@ SIGNATURES = {
                                        _P, _I, _I, _P]),
     "lsa_merge_partials": (_INT, [_P, _P, _I, _I, _I, _INT, _P, _P]),
     "lsa_shared_prefix_scratch": (_I, [_INT, _I, _I, _I, _I, _I, _I, _I, _INT]),
+    "lsa_shared_prefix_wait_limit": (_INT, [_I]),
     "lsa_shared_prefix_attention": (_INT, [_P, _P, _P, _P, _P, _INT, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _P, _P,
                                            _P, _P, _P, _I, _P, _P]),
     "lsa_evict": (_INT, [_P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P]),

@@ -105,3 +105,51 @@ def test_a_refused_step_changes_nothing(lsa):
     assert torch.equal(cache.k[:, :n], twin.k[:, :n]) and torch.equal(cache.v[:, :n], twin.v[:, :n])
     assert torch.equal(cache.step(q, kn, vn), twin.step(q, kn, vn))
     assert torch.equal(cache.scores, twin.scores) and torch.equal(cache.lengths, twin.lengths)
+
+
+@pytest.fixture()
+def wait_limit():
+    """Sets the limit of the tensor-core kernels' waits (ns); the default again afterwards."""
+    from lsa_b200 import _lib
+
+    _lib.torch_ops()
+    yield lambda ns: _lib.check(_lib.lib().lsa_shared_prefix_wait_limit(ns), "wait limit")
+    assert _lib.lib().lsa_shared_prefix_wait_limit(-1) == _lib.OK
+
+
+@pytest.mark.parametrize("case", [
+    (40, 1, 32, 4, 64, 700, 500),   # prefix: two streams of chunks, more tiles than the ring holds
+    (40, 5, 32, 4, 128, 200, 200),  # few tiles: all of them in flight at once
+    (3, 64, 16, 4, 128, 2000, 300), # both halves, prefix and own keys, split
+    (40, 64, 16, 4, 128, 300, 130), # whole tiles
+    (2, 32, 32, 8, 128, 0, 3000),   # weights of 128 rows: Q resident
+    (1, 257, 6, 2, 64, 0, 400),     # weights of seven row tiles: Q streamed
+], ids=lambda c: "-".join(map(str, c)))
+def test_expired_waits_leave_with_their_copies_landed(lsa, wait_limit, case):
+    """Every role gives up at its first wait, with the first copies in flight. The call reports it, and calls
+    after it, on the same SMs, answer as before. (A CTA that left copies behind could have them land in the
+    next one's shared memory.)"""
+    B, Tq, Hq, Hkv, D, P, T = case
+    g = torch.Generator(device=DEV)
+    g.manual_seed(T)
+    r = lambda *s: torch.randn(*s, generator=g, device=DEV).to(BF)
+    q, kp, vp, k, v = r(B, Tq, Hq, D), r(P, Hkv, D), r(P, Hkv, D), r(B, T, Hkv, D), r(B, T, Hkv, D)
+    lengths = torch.randint(min(Tq, T), T + 1, (B,), generator=g, device=DEV, dtype=torch.int32)
+    scores = torch.rand(B, Hkv, T, generator=g, device=DEV)
+    call = lambda: lsa.scored_attention(q, k, v, lengths, scores, k_prefix=kp, v_prefix=vp)
+    want = call()
+    for _ in range(3):
+        wait_limit(0)
+        with pytest.raises(RuntimeError, match="bounded device wait expired"):
+            call()
+            lsa.check_status()  # without the checked mode
+        wait_limit(-1)
+        got = call()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    lsa.check_status()
+
+
+def test_wait_limits_out_of_range_are_refused(lsa):
+    from lsa_b200 import _lib
+
+    assert _lib.lib().lsa_shared_prefix_wait_limit(10 ** 10 + 1) == _lib.ERR_ARG
