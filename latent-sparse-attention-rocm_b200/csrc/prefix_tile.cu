@@ -495,7 +495,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
         } else if (warp == 2 && tail) {
             // ------------------------------------------------ the tail of a sequence's last V tile
-            if (role_wait(bar_tail, 0, abort_flag, a.wait_ns)) {
+            // (a wait as long as the item: the MMA thread has up to four a chunk of its own before it)
+            if (role_wait(bar_tail, 0, abort_flag, a.wait_ns * (4 * (uint64_t)n + 8))) {
                 uint8_t* va = sm + Sh::kOffStage + ((2 * n - 1) % NS) * Sh::kTileBytes;  // the last load
                 for (int i = (w.len - (w.c1 - 1 - w.np) * kChunk) * 8 + lane; i < kChunk * 8; i += 32)
 #pragma unroll

@@ -153,3 +153,21 @@ def test_wait_limits_out_of_range_are_refused(lsa):
     from lsa_b200 import _lib
 
     assert _lib.lib().lsa_shared_prefix_wait_limit(10 ** 10 + 1) == _lib.ERR_ARG
+
+
+def test_an_item_may_run_longer_than_a_wait(lsa, wait_limit):
+    """The limit is one wait's. Whole row tiles of 1025 chunks run 1.7 ms or more with waits of a few us, and
+    the warp that zeroes the last V tile's tail waits for all of them."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=g, device=DEV).to(BF)
+    q, kp, vp, k, v = r(37, 64, 16, 128), r(131072, 4, 128), r(131072, 4, 128), r(37, 70, 4, 128), r(37, 70, 4, 128)
+    lengths = torch.full((37,), 70, dtype=torch.int32, device=DEV)
+    want = lsa.shared_prefix_attention(q, kp, vp, k, v, lengths)
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    wait_limit(500_000)
+    start.record()
+    got = lsa.shared_prefix_attention(q, kp, vp, k, v, lengths)
+    end.record()
+    lsa.check_status()
+    assert torch.equal(got, want) and start.elapsed_time(end) > 1.0
