@@ -13,7 +13,7 @@
 //   lsa::scored_attention(q, k, v, lengths, scores, scale, k_prefix, v_prefix) -> (out, scores)
 //   lsa::evict(k, v, scores, lengths, budget, window, sink, capacity)
 //                     -> (k, v, scores, lengths, ids)            no reference counterpart
-//   lsa::workspace_counters() -> Tensor[]                      the cached counter buffers (checks)
+//   lsa::workspace_counters() -> Tensor[]                      the cached counter buffers and status words (checks)
 // Meta implementations give FX / torch.compile the output shapes. Workspaces: scratch (any
 // content) and int32 counters (zero at rest: the kernels that use them leave them zero) cached
 // per (device, stream), grown on demand - the same contract as the C ABI's callers keep.
@@ -51,6 +51,33 @@ Workspace& workspace(const at::Device& dev, cudaStream_t stream, int64_t scratch
         w.counters = at::zeros({std::max<int64_t>(n_counters, 64)}, at::TensorOptions().dtype(at::kInt).device(dev));
     }
     return w;
+}
+
+std::map<int, at::Tensor> g_status;  // under g_ws_mutex
+
+// The word that the shared-prefix operators' bounded waits report to, one a device (kernels only ever set it,
+// and it is read with the device idle). It is no ticket of another operator, and it neither moves nor is
+// zeroed again, since captured calls keep its address: memory of its own, made and zeroed beside a
+// capture that may be under way on the current stream (relaxed mode is for this).
+int32_t* status_word(const at::Device& dev) {
+    std::lock_guard<std::mutex> lock(g_ws_mutex);
+    at::Tensor& word = g_status[dev.index()];
+    if (!word.defined()) {
+        void* p = nullptr;
+        cudaStream_t aside = nullptr;
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        C10_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+        cudaError_t rc = cudaMalloc(&p, sizeof(int32_t));
+        if (rc == cudaSuccess) rc = cudaStreamCreateWithFlags(&aside, cudaStreamNonBlocking);
+        if (rc == cudaSuccess) rc = cudaMemsetAsync(p, 0, sizeof(int32_t), aside);
+        if (rc == cudaSuccess) rc = cudaStreamSynchronize(aside);
+        if (aside != nullptr) cudaStreamDestroy(aside);
+        if (rc != cudaSuccess && p != nullptr) cudaFree(p);
+        C10_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+        C10_CUDA_CHECK(rc);
+        word = at::from_blob(p, {1}, at::TensorOptions().dtype(at::kInt).device(dev));
+    }
+    return word.data_ptr<int32_t>();
 }
 
 int dtype_code(at::ScalarType t) {
@@ -267,9 +294,8 @@ PrefixOut prefix_attention(const at::Tensor& q_in, const at::Tensor* kp_in, cons
     TORCH_CHECK_VALUE(bytes >= 0, what, ": sizes out of range");
     auto stream = at::cuda::getCurrentCUDAStream();
     // The parts' scratch is the call's own: it may be gigabytes, and one kept for the stream would have to
-    // move when a larger call comes, under the feet of a captured graph. The status word is kept.
+    // move when a larger call comes, under the feet of a captured graph.
     auto scratch = fresh({bytes}, at::kByte, q.device());
-    Workspace& w = workspace(q.device(), stream, 0, 64);
     const int64_t strides[13] = {stride_of(q, 0), stride_of(q, 1), stride_of(q, 2), P ? stride_of(kp, 0) : 0,
                                  P ? stride_of(kp, 1) : 0, P ? stride_of(vp, 0) : 0, P ? stride_of(vp, 1) : 0,
                                  stride_of(k, 0), stride_of(k, 1),
@@ -280,7 +306,7 @@ PrefixOut prefix_attention(const at::Tensor& q_in, const at::Tensor* kp_in, cons
                                          r.out.data_ptr(), want_lse ? r.lse.data_ptr<float>() : nullptr,
                                          scores_in ? scores.data_ptr<float>() : nullptr,
                                          scores_in ? r.scores.data_ptr<float>() : nullptr, scratch.data_ptr(), bytes,
-                                         w.counters.data_ptr<int32_t>(), stream),
+                                         status_word(q.device()), stream),
              what);
     return r;
 }
@@ -348,6 +374,8 @@ std::vector<at::Tensor> workspace_counters() {
     std::vector<at::Tensor> out;
     for (auto& kv : g_ws)
         if (kv.second.counters.defined()) out.push_back(kv.second.counters);
+    for (auto& kv : g_status)
+        if (kv.second.defined()) out.push_back(kv.second);
     return out;
 }
 

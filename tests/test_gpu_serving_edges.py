@@ -171,3 +171,111 @@ def test_an_item_may_run_longer_than_a_wait(lsa, wait_limit):
     end.record()
     lsa.check_status()
     assert torch.equal(got, want) and start.elapsed_time(end) > 1.0
+
+
+def reported():
+    from lsa_b200 import _lib
+
+    return {t.data_ptr(): t for t in _lib.torch_ops().workspace_counters()}
+
+
+def small(lsa, seed=0):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g, device=DEV).to(BF)
+    return (r(30, 1, 8, 64), r(300, 2, 64), r(300, 2, 64), r(30, 40, 2, 64), r(30, 40, 2, 64),
+            torch.full((30,), 40, dtype=torch.int32, device=DEV))
+
+
+def read_rows(R):
+    """A sparse read of R rows (and R * Hkv counters) with split lists."""
+    from lsa_b200 import _lib
+
+    g = torch.Generator(device=DEV)
+    g.manual_seed(R)
+    r = lambda *s: torch.randn(*s, generator=g, device=DEV).to(BF)
+    q, k, v = r(1, R, 8, 64), r(1, 4096, 2, 64), r(1, 4096, 2, 64)
+    ids = torch.randint(0, 4096, (R, 2116), generator=g, device=DEV, dtype=torch.int32)
+    lengths = torch.full((R,), 2110, dtype=torch.int32, device=DEV)
+    return lambda: _lib.torch_ops().sparse_read(q, k, v, ids, lengths, 0.125)
+
+
+def test_the_status_word_outlives_larger_calls(lsa):
+    """Whatever a captured call may write its status to is still reported after the stream's counters have grown."""
+    args = small(lsa)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        lsa.shared_prefix_attention(*args)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        lsa.shared_prefix_attention(*args)
+    words = [p for p, t in reported().items() if t.numel() == 1]
+    before = max(t.numel() for t in reported().values())
+    with torch.cuda.stream(side):
+        read_rows(before)()
+    side.synchronize()
+    assert len(words) >= 1 and set(words) <= set(reported())
+
+
+def test_a_timeout_word_disturbs_no_other_operator(lsa, monkeypatch):
+    """The word that an expired wait leaves (planted here) is no ticket of the sparse read."""
+    from lsa_b200 import _lib
+
+    lsa.shared_prefix_attention(*small(lsa))
+    words = [t for t in reported().values() if t.numel() == 1]
+    assert words
+    read = read_rows(3)
+    want = read()
+    for w in words:
+        w.fill_(_lib.ERR_TIMEOUT)
+    got = read()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    with pytest.raises(RuntimeError, match="bounded device wait expired"):
+        lsa.check_status()
+    lsa.check_status()
+
+
+def test_a_first_call_inside_a_capture(tmp_path):
+    """In a fresh process: the first call of all is captured. The word is zero before any replay, and a
+    replay leaves an unread timeout in place."""
+    import pathlib
+    import subprocess
+    import sys
+
+    pkg = pathlib.Path(__file__).resolve().parents[1] / "latent-sparse-attention-rocm_b200"
+    code = f"""
+import sys; sys.path.insert(0, {str(pkg)!r})
+import torch, lsa_b200
+from lsa_b200 import _lib
+_lib.torch_ops()
+d = "cuda"
+a = [torch.randn(4, 1, 8, 64, device=d).bfloat16(), *(torch.randn(300, 2, 64, device=d).bfloat16() for _ in range(2)),
+     *(torch.randn(4, 40, 2, 64, device=d).bfloat16() for _ in range(2)),
+     torch.full((4,), 40, dtype=torch.int32, device=d)]
+junk = torch.full((1 << 22,), 77, dtype=torch.uint8, device=d)
+del junk
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = lsa_b200.shared_prefix_attention(*a)
+lsa_b200.check_status()
+words = [t for t in _lib.torch_ops().workspace_counters()]
+assert words and all(int(t.abs().sum()) == 0 for t in words)
+for t in words: t[0] = _lib.ERR_TIMEOUT
+g.replay(); torch.cuda.synchronize()
+assert all(int(t[0]) == _lib.ERR_TIMEOUT for t in words)
+try:
+    lsa_b200.check_status()
+    raise SystemExit("an unread timeout was wiped")
+except RuntimeError as e:
+    assert "expired" in str(e)
+g.replay(); torch.cuda.synchronize()
+assert torch.equal(out, lsa_b200.shared_prefix_attention(*a))
+lsa_b200.check_status()
+print("captured first")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured first" in r.stdout, r.stdout + r.stderr
