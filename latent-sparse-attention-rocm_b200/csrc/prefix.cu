@@ -279,6 +279,7 @@ __global__ void __launch_bounds__(256, 4) prefix_finish_kernel(const PrefixArgs 
     }
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % spread;
     int64_t row = (int64_t)(blockIdx.x - weight_blocks) * (8 / spread) + warp / spread;
+    const int64_t prow = row;
     if (tp.whole) {  // the rows of the split seq tiles, 256 a tile
         int b, h, tile;
         seq_tile(a, tp, tp.whole + (int)(row >> 8), &b, &h, &tile);
@@ -293,7 +294,7 @@ __global__ void __launch_bounds__(256, 4) prefix_finish_kernel(const PrefixArgs 
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             x[i] = -INFINITY;
-            if (32 * i < parts && lane + 32 * i < parts) x[i] = a.part_lse[(int64_t)(lane + 32 * i) * a.rows + row];
+            if (32 * i < parts && lane + 32 * i < parts) x[i] = a.part_lse[(int64_t)(lane + 32 * i) * a.part_rows + prow];
         }
         bool bad = false;
 #pragma unroll
@@ -320,7 +321,7 @@ __global__ void __launch_bounds__(256, 4) prefix_finish_kernel(const PrefixArgs 
 #pragma unroll
                 for (int u = 0; u < 8; ++u) {
                     const int c = f[u] > 0.0f ? c0 + u : best;
-                    const float* src = a.part_o + ((int64_t)c * a.rows + row) * D + lane * E;
+                    const float* src = a.part_o + ((int64_t)c * a.part_rows + prow) * D + lane * E;
                     if constexpr (E == 4) {
                         const float4 y = __ldcs(reinterpret_cast<const float4*>(src));
                         v[u][0] = y.x, v[u][1] = y.y, v[u][2] = y.z, v[u][3] = y.w;
@@ -404,9 +405,18 @@ struct Plan {
     bool merge;         // some row has parts to join
     TilePlan tile;
     RowsPlan rows;
+    int64_t part_rows;  // PrefixArgs::part_rows
 };
 
 constexpr int kItemsAPlace = 2;
+
+// Splits of `items` row tiles at most. Parts cost scratch, 132 KB a tile at D 128: split tiles fill no more than
+// eight rounds of the SMs (157 MB). With more rounds than that a last, short one is a ninth of the time at most.
+constexpr int kMostRounds = 8;
+int most_splits(int64_t items) {
+    const int64_t s = items ? kMostRounds * kSMs / items : 0;
+    return (int)(s < 1 ? 1 : (s < kMaxSplits ? s : kMaxSplits));
+}
 
 // Splits of the few-row kernel for `items` of `chunks` steps of 64 keys. One length: 256 CTAs draw the
 // memory's whole bandwidth, and more parts cost more to join (one sequence of 24k keys, 8 KV heads: 24.2
@@ -425,6 +435,7 @@ int few_splits(int64_t items, int64_t chunks, bool ragged) {
 Plan make_plan(int dtype, int64_t B, int64_t Tq, int64_t Hkv, int64_t G, int64_t D, int64_t P, int64_t T, bool scored) {
     Plan p = {};
     p.merge = true;
+    p.part_rows = B * Tq * Hkv * G;
     p.simt = dtype == kF32;
     if (p.simt) {
         // splits enough that the work items of each segment fill the GPU about four times
@@ -452,8 +463,9 @@ Plan make_plan(int dtype, int64_t B, int64_t Tq, int64_t Hkv, int64_t G, int64_t
         // of the last, short round are, so that it too fills the GPU
         t.whole = (int)(seq / kSMs * kSMs);
         const int64_t rest = seq - t.whole;
-        p.So = rest ? balance(rest, pc + oc, 4, kSMs, kMaxSplits) : 1;
+        p.So = rest ? balance(rest, pc + oc, 4, kSMs, most_splits(rest)) : 1;
         if (p.So == 1) t.whole = (int)seq;
+        if (t.whole) p.part_rows = (seq - t.whole) * 256;
         p.merge = p.So > 1;
         p.parts_o = p.merge ? p.So : 0;
         t.seq_items = (int)(t.whole + (seq - t.whole) * p.So);
@@ -475,7 +487,7 @@ Plan make_plan(int dtype, int64_t B, int64_t Tq, int64_t Hkv, int64_t G, int64_t
         p.rows.pitch = (T + 15) / 16 * 16;
         p.logits = scored;
     } else {
-        p.So = balance(seq, t.seq_streams ? (oc + 1) / 2 : oc, 4, kSMs, kMaxSplits);
+        p.So = balance(seq, t.seq_streams ? (oc + 1) / 2 : oc, 4, kSMs, most_splits(seq));
         p.parts_o = p.So * (t.seq_streams ? 2 : 1);
         t.seq_items = (int)(seq * p.So);
     }
@@ -485,7 +497,8 @@ Plan make_plan(int dtype, int64_t B, int64_t Tq, int64_t Hkv, int64_t G, int64_t
     } else {
         t.batch_streams = B * Tq <= t.tokens;
         t.batch_tiles = (int)((B * Tq + 2 * t.tokens - 1) / (2 * t.tokens));
-        p.Sp = balance_beside(Hkv * t.batch_tiles, t.batch_streams ? (pc + 1) / 2 : pc, 4, kSMs, beside);
+        const int64_t batch = (int64_t)Hkv * t.batch_tiles;
+        p.Sp = balance_beside(batch, t.batch_streams ? (pc + 1) / 2 : pc, 4, kSMs, beside, most_splits(batch));
         p.parts_p = p.Sp * (t.batch_streams ? 2 : 1);
         t.batch_items = (int)(Hkv * t.batch_tiles * p.Sp);
         p.rows.follows = t.batch_items > 0;
@@ -529,7 +542,7 @@ int64_t lsa_shared_prefix_scratch(int dtype, int64_t B, int64_t Tq, int64_t Hq, 
     const Plan p = make_plan(dtype, B, Tq, Hkv, Hq / Hkv, D, P, T, scored);
     const int64_t rows = B * Tq * Hq;
     const int64_t parts = p.parts_p + p.parts_o;
-    return round256(parts * rows * D * 4) + round256(parts * rows * 4) + round256(rows * 4) +
+    return round256(parts * p.part_rows * D * 4) + round256(parts * p.part_rows * 4) + round256(rows * 4) +
            (p.logits ? round256(rows * p.rows.pitch * 4) : 0);
 }
 
@@ -583,12 +596,13 @@ int lsa_shared_prefix_attention(const void* q, const void* k_prefix, const void*
     a.status = status;
     a.wait_ns = (uint64_t)g_wait_ns.load(std::memory_order_relaxed);
     a.rows = B * Tq * Hq;
+    a.part_rows = p.part_rows;
     a.scale_log2 = scale * 1.4426950408889634f;
     uint8_t* s = static_cast<uint8_t*>(scratch);
     a.part_o = reinterpret_cast<float*>(s);
-    s += round256((p.parts_p + p.parts_o) * a.rows * D * 4);
+    s += round256((p.parts_p + p.parts_o) * a.part_rows * D * 4);
     a.part_lse = reinterpret_cast<float*>(s);
-    s += round256((p.parts_p + p.parts_o) * a.rows * 4);
+    s += round256((p.parts_p + p.parts_o) * a.part_rows * 4);
     a.lse2 = reinterpret_cast<float*>(s);
     RowsPlan few = p.rows;
     if (p.logits && T > 0) few.logits = reinterpret_cast<float*>(s + round256(a.rows * 4));

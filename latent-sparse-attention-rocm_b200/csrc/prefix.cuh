@@ -28,8 +28,8 @@ struct PrefixArgs {
     int64_t k_b, k_t, k_h, v_b, v_t, v_h; // own [B, T, Hkv, D]
     const int32_t* lengths;               // [B]
     void* out;                            // [B, Tq, Hq, D] contiguous
-    float* part_o;                        // [parts][rows][D], each part normalised by its own sum
-    float* part_lse;                      // [parts][rows], log2 domain, -inf: no key
+    float* part_o;                        // [parts][part_rows][D], each part normalised by its own sum
+    float* part_lse;                      // [parts][part_rows], log2 domain, -inf: no key
     float* lse2;                          // [rows], log2 domain: the joined lse
     float* lse;                           // [rows], natural, or null
     int B, Tq, Hq, Hkv, G;
@@ -37,6 +37,7 @@ struct PrefixArgs {
     int Sp, So;                           // splits of the prefix and of the own caches
     int parts_p, parts_o;                 // parts of a row from the prefix and from its own cache
     int64_t rows;                         // B * Tq * Hq
+    int64_t part_rows;                    // rows, or 256 a split tile where whole tiles have no parts (TilePlan::whole)
     float scale_log2;                     // scale * log2(e)
     int32_t* status;                      // LSA_ERR_TIMEOUT after an expired wait
     uint64_t wait_ns;                     // limit of each wait of the tensor-core kernels
@@ -84,11 +85,11 @@ inline int balance(int64_t items, int64_t chunks, double fixed, int64_t slots, i
 
 // The same for work that shares the GPU with `beside` chunks' worth of other work per place, which
 // starts on the places left free: the least of the longer of its own rounds and all the work together.
-inline int balance_beside(int64_t items, int64_t chunks, double fixed, int64_t slots, double beside) {
+inline int balance_beside(int64_t items, int64_t chunks, double fixed, int64_t slots, double beside, int most) {
     if (chunks == 0) return 0;
     int best = 1;
     double least = 1e300;
-    for (int s = 1; s <= kMaxSplits && s <= chunks; ++s) {
+    for (int s = 1; s <= most && s <= chunks; ++s) {
         const double one = (double)chunks / s + fixed;
         const double alone = (double)((items * s + slots - 1) / slots) * one;
         const double all = (double)(items * s) * one / slots + beside;

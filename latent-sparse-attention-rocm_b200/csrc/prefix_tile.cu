@@ -71,6 +71,7 @@ struct Item {
     bool own, streams;  // seq tile; both halves hold the same rows
     bool direct;        // all of its rows' keys: it writes the output itself
     int b, h, part, len;
+    int rest;        // which of the split seq tiles
     int t0, tokens;  // first token of the tile, tokens of the segment (all sequences' or one's)
     int np;      // prefix chunks of the item's chunk list
     int c0, c1;  // its chunks of the list [0, np + own chunks)
@@ -78,6 +79,7 @@ struct Item {
 
 __device__ __forceinline__ Item item_of(const PrefixArgs& a, const TilePlan& t) {
     Item w;
+    w.rest = 0;
     int i = blockIdx.x;
     w.own = i >= t.batch_items;
     int chunks, S, split, tile;
@@ -99,7 +101,8 @@ __device__ __forceinline__ Item item_of(const PrefixArgs& a, const TilePlan& t) 
         w.direct = i < t.whole;
         S = w.direct ? 1 : a.So;
         split = w.direct ? 0 : (i - t.whole) % S;
-        seq_tile(a, t, w.direct ? i : t.whole + (i - t.whole) / S, &w.b, &w.h, &tile);
+        w.rest = w.direct ? 0 : (i - t.whole) / S;
+        seq_tile(a, t, w.direct ? i : t.whole + w.rest, &w.b, &w.h, &tile);
         w.len = own_length(a, w.b);
         w.streams = t.seq_streams;
         w.tokens = a.Tq;
@@ -235,7 +238,8 @@ __device__ __forceinline__ void softmax_half(const PrefixArgs& a, const TilePlan
     const bool none = l == 0.0f;  // the row has seen no key (a NaN logit makes l NaN, and the output)
     const float inv = none ? 0.0f : 1.0f / l;
     const float lse = none ? -INFINITY : m * sl + (log2f(l) - kLift<T>);
-    const int64_t at = (int64_t)(w.part + (w.streams ? hf : 0)) * a.rows + rid;
+    const int64_t prow = tp.whole ? (int64_t)w.rest * 256 + hf * 128 + qd * 32 + lane : rid;
+    const int64_t at = (int64_t)(w.part + (w.streams ? hf : 0)) * a.part_rows + prow;
     if (live) {
         if (w.direct) {
             a.lse2[rid] = lse;

@@ -279,3 +279,12 @@ print("captured first")
 """
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "captured first" in r.stdout, r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("case", [(19, 64, 32, 8, 128, 10007, 100), (19, 70, 56, 8, 64, 5000, 90)],
+                         ids=lambda c: "-".join(map(str, c)))
+def test_few_split_tiles_beside_whole_ones(lsa, case):
+    """148 whole tiles and four in many parts, numbered by tile; with seven heads a group a tile has rows of no one."""
+    from test_gpu_shared_prefix import check_all, make
+
+    check_all(lsa, make(*case, BF, seed=21), BF)
