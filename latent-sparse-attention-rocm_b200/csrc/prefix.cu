@@ -560,7 +560,13 @@ int lsa_shared_prefix_attention(const void* q, const void* k_prefix, const void*
     if (!sizes_ok(B, Tq, Hq, Hkv, D, P, T) || dtype < kF32 || dtype > kBF16) return LSA_ERR_ARG;
     if ((scores == nullptr) != (scores_out == nullptr) || strides == nullptr) return LSA_ERR_ARG;
     if (!(scale > 0.0f) || !(scale < INFINITY)) return LSA_ERR_ARG;  // the kernels take the maximum before the scale
-    if (B == 0 || Tq == 0) return LSA_OK;
+    if (B == 0 || Tq == 0) {  // no row: the scores are what they were
+        if (B == 0 || T == 0 || scores_out == scores) return LSA_OK;
+        return cudaMemcpyAsync(scores_out, scores, (size_t)(B * Hkv * T) * 4, cudaMemcpyDeviceToDevice, stream) ==
+                       cudaSuccess
+                   ? LSA_OK
+                   : LSA_ERR_CUDA;
+    }
     if (q == nullptr || out == nullptr || lengths == nullptr || scratch == nullptr || status == nullptr) return LSA_ERR_ARG;
     if ((P > 0 && (k_prefix == nullptr || v_prefix == nullptr)) || (T > 0 && (k == nullptr || v == nullptr)))
         return LSA_ERR_ARG;

@@ -1,5 +1,6 @@
 """Edges of the shared-prefix attention, the scored attention and the budgeted cache on the GPU."""
 
+import ctypes
 import math
 
 import pytest
@@ -288,3 +289,31 @@ def test_few_split_tiles_beside_whole_ones(lsa, case):
     from test_gpu_shared_prefix import check_all, make
 
     check_all(lsa, make(*case, BF, seed=21), BF)
+
+
+def call_entry(lsa, q, k, v, lengths, scores, out, scores_out):
+    """lsa_shared_prefix_attention itself, without a prefix."""
+    from lsa_b200 import _lib
+
+    L = _lib.lib()
+    B, Tq, Hq, D = q.shape
+    T, Hkv = k.shape[1:3]
+    st = (ctypes.c_int64 * 13)(*q.stride()[:3], D, D, D, D, *k.stride()[:3], *v.stride()[:3])
+    nbytes = L.lsa_shared_prefix_scratch(_lib.BF16, B, Tq, Hq, Hkv, D, 0, T, 1)
+    scratch = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=DEV)
+    return L.lsa_shared_prefix_attention(_lib.ptr(q), None, None, _lib.ptr(k), _lib.ptr(v), _lib.BF16, st,
+                                         _lib.ptr(lengths), B, Tq, Hq, Hkv, D, 0, T, D ** -0.5, _lib.ptr(out), None,
+                                         _lib.ptr(scores), _lib.ptr(scores_out), _lib.ptr(scratch), nbytes,
+                                         _lib.ptr(_lib.status_word(q.device)), _lib.stream_of(q))
+
+
+def test_the_entry_without_rows_passes_the_scores_on(lsa):
+    k = torch.randn(2, 40, 2, 64, device=DEV).to(BF)
+    q = torch.empty(2, 0, 4, 64, dtype=BF, device=DEV)
+    scores = torch.rand(2, 2, 40, device=DEV)
+    got = torch.full_like(scores, -7.0)
+    lengths = torch.tensor([40, 3], dtype=torch.int32, device=DEV)
+    assert call_entry(lsa, q, k, k, lengths, scores, torch.empty_like(q), got) == 0
+    assert torch.equal(got, scores)
+    assert call_entry(lsa, q, k, k, lengths, got, torch.empty_like(q), got) == 0  # in place
+    assert torch.equal(got, scores)
