@@ -46,7 +46,8 @@ extern "C" {
  * caches hold at or past lengths[b] is never used. strides[13], in elements: q (b, t, h),
  * k_prefix (t, h), v_prefix (t, h), k (b, t, h), v (b, t, h); the head dimension is contiguous,
  * every base and stride a multiple of 16 bytes, every stride of a dimension longer than one positive,
- * and for 16-bit types q's batch stride Tq times its token stride. D 64 or 128, Hq / Hkv at most 64; scale > 0.
+ * and for 16-bit types q's batch stride Tq times its token stride. D 64 or 128, Hq / Hkv at most 64; scale > 0,
+ * scale * log2(e) finite in fp32.
  * out [B, Tq, Hq, D] contiguous, lse [B, Tq, Hq] (natural logarithm) or NULL.
  * scores / scores_out [B, Hkv, T] fp32, or both NULL: scores_out = scores + the attention
  * weight that own key j received from every (row, query head of the group) of the call; the

@@ -559,7 +559,8 @@ int lsa_shared_prefix_attention(const void* q, const void* k_prefix, const void*
                                 int64_t scratch_bytes, int32_t* status, cudaStream_t stream) {
     if (!sizes_ok(B, Tq, Hq, Hkv, D, P, T) || dtype < kF32 || dtype > kBF16) return LSA_ERR_ARG;
     if ((scores == nullptr) != (scores_out == nullptr) || strides == nullptr) return LSA_ERR_ARG;
-    if (!(scale > 0.0f) || !(scale < INFINITY)) return LSA_ERR_ARG;  // the kernels take the maximum before the scale
+    const float scale_log2 = scale * 1.4426950408889634f;
+    if (!(scale_log2 > 0.0f) || !(scale_log2 < INFINITY)) return LSA_ERR_ARG;  // the kernels take the maximum before it
     if (B == 0 || Tq == 0) {  // no row: the scores are what they were
         if (B == 0 || T == 0 || scores_out == scores) return LSA_OK;
         return cudaMemcpyAsync(scores_out, scores, (size_t)(B * Hkv * T) * 4, cudaMemcpyDeviceToDevice, stream) ==
@@ -603,7 +604,7 @@ int lsa_shared_prefix_attention(const void* q, const void* k_prefix, const void*
     a.wait_ns = (uint64_t)g_wait_ns.load(std::memory_order_relaxed);
     a.rows = B * Tq * Hq;
     a.part_rows = p.part_rows;
-    a.scale_log2 = scale * 1.4426950408889634f;
+    a.scale_log2 = scale_log2;
     uint8_t* s = static_cast<uint8_t*>(scratch);
     a.part_o = reinterpret_cast<float*>(s);
     s += round256((p.parts_p + p.parts_o) * a.part_rows * D * 4);

@@ -269,7 +269,8 @@ PrefixOut prefix_attention(const at::Tensor& q_in, const at::Tensor* kp_in, cons
                           q_in.scalar_type() == at::kBFloat16,
                       what, ": fp32, fp16 or bf16, got ", q_in.scalar_type());
     TORCH_CHECK_VALUE(lengths_in.numel() == B && !lengths_in.is_floating_point(), what, ": one whole length a sequence");
-    TORCH_CHECK_VALUE(std::isfinite(scale) && scale > 0, what, ": the scale must be positive, got ", scale);
+    const float scale_log2 = (float)scale * 1.4426950408889634f;  // as the entry point takes it
+    TORCH_CHECK_VALUE(std::isfinite(scale_log2) && scale_log2 > 0, what, ": the scale must be positive, and with log2(e) within fp32, got ", scale);
     c10::cuda::CUDAGuard guard(q_in.device());
     auto q = rows16(q_in), k = rows16(k_in), v = rows16(v_in);
     at::Tensor kp, vp;

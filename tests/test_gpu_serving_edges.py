@@ -317,3 +317,13 @@ def test_the_entry_without_rows_passes_the_scores_on(lsa):
     assert torch.equal(got, scores)
     assert call_entry(lsa, q, k, k, lengths, got, torch.empty_like(q), got) == 0  # in place
     assert torch.equal(got, scores)
+
+
+def test_scales_past_fp32_are_refused(lsa):
+    """A scale whose product with log2(e) is no finite positive fp32 number has no answer."""
+    q, k = torch.ones(1, 1, 2, 64, dtype=BF, device=DEV), torch.zeros(1, 8, 2, 64, dtype=BF, device=DEV)
+    lengths = torch.tensor([8], device=DEV)
+    for scale in (1e-50, 3e38, 1e300):
+        with pytest.raises(ValueError, match="scale"):
+            lsa.shared_prefix_attention(q, k[0], k[0], k, k, lengths, scale)
+    assert (lsa.shared_prefix_attention(q, k[0], k[0], k, k, lengths, 2e38) == 0).all()
