@@ -16,7 +16,7 @@ import math
 
 import torch
 
-from .eviction import evict, scored_attention
+from .eviction import EvictedCache, evict, scored_attention
 
 
 class BudgetedCache:
@@ -45,13 +45,15 @@ class BudgetedCache:
         self.lengths = torch.tensor(lengths, dtype=torch.int32, device=k.device)
         self._longest = max(lengths, default=0)  # of the batch, known without asking the device
         self._rows = torch.arange(B, device=k.device)[:, None]
-        self._evict()
+        self._take(self._evicted(), min(self._longest, self.budget))
 
-    def _evict(self):
-        kept = evict(self.k, self.v, self.scores, self.lengths, self.budget, self.window_size, self.sink_size,
+    def _evicted(self):
+        return evict(self.k, self.v, self.scores, self.lengths, self.budget, self.window_size, self.sink_size,
                      self.capacity)
-        self.k, self.v, self.scores, self.lengths = kept.k, kept.v, kept.scores, kept.lengths
-        self._longest = min(self._longest, self.budget)
+
+    def _take(self, cache, longest):
+        self.k, self.v, self.scores, self.lengths = cache.k, cache.v, cache.scores, cache.lengths
+        self._longest = longest
 
     def _check_step(self, q, k_new, v_new, scale):
         """ValueError for a step that the writes below would spread over other slots (an indexed write
@@ -74,13 +76,13 @@ class BudgetedCache:
         Evicts first when the longest sequence has no room for them. q [B, Tq, Hq, D], k_new and
         v_new [B, Tq, Hkv, D]; a refused step (ValueError) leaves the cache as it was. Output like q."""
         self._check_step(q, k_new, v_new, scale)
-        Tq = q.shape[1]
-        if self._longest + Tq > self.capacity:
-            self._evict()
-        at = self.lengths.long()[:, None] + torch.arange(Tq, device=q.device)
-        self.k[self._rows, at], self.v[self._rows, at] = k_new, v_new  # past the lengths: not yet the cache's
-        lengths = self.lengths + Tq
-        out, scores = scored_attention(q, self.k, self.v, lengths, self.scores, scale, self.k_prefix, self.v_prefix)
-        self.lengths, self.scores = lengths, scores
-        self._longest += Tq
+        Tq, cache, longest = q.shape[1], self, self._longest
+        if longest + Tq > self.capacity:
+            cache, longest = self._evicted(), min(longest, self.budget)
+        at = cache.lengths.long()[:, None] + torch.arange(Tq, device=q.device)
+        cache.k[self._rows, at], cache.v[self._rows, at] = k_new, v_new  # past the lengths: not yet the cache's
+        lengths = cache.lengths + Tq
+        out, scores = scored_attention(q, cache.k, cache.v, lengths, cache.scores, scale, self.k_prefix,
+                                       self.v_prefix)
+        self._take(EvictedCache(cache.k, cache.v, scores, lengths, None), longest + Tq)
         return out

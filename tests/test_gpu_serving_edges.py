@@ -327,3 +327,18 @@ def test_scales_past_fp32_are_refused(lsa):
         with pytest.raises(ValueError, match="scale"):
             lsa.shared_prefix_attention(q, k[0], k[0], k, k, lengths, scale)
     assert (lsa.shared_prefix_attention(q, k[0], k[0], k, k, lengths, 2e38) == 0).all()
+
+
+def test_a_step_refused_by_the_operator_undoes_its_eviction(lsa):
+    """What the step itself does not look at - here a prefix that does not fit - is refused by the operator,
+    after the eviction that the step was due; the cache is as before."""
+    cache, r = budgeted(lsa)
+    cache.step(r(3, 4, 4, 64), r(3, 4, 2, 64), r(3, 4, 2, 64))
+    k, v, scores, lengths = cache.k, cache.v, cache.scores, cache.lengths.clone()
+    cache.k_prefix = cache.v_prefix = r(10, 1, 64)
+    with pytest.raises(ValueError):
+        cache.step(r(3, 5, 4, 64), r(3, 5, 2, 64), r(3, 5, 2, 64))
+    assert cache.k is k and cache.v is v and cache.scores is scores and torch.equal(cache.lengths, lengths)
+    cache.k_prefix = cache.v_prefix = None
+    cache.step(r(3, 4, 4, 64), r(3, 4, 2, 64), r(3, 4, 2, 64))  # fits without an eviction
+    assert cache.k is k and torch.equal(cache.lengths, lengths + 4)
