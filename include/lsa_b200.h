@@ -55,8 +55,9 @@ extern "C" {
  * status: a device int32 that receives LSA_ERR_TIMEOUT if a bounded wait expires.
  * lsa_shared_prefix_scratch: the scratch bytes of a call, with scores or not (LSA_ERR_ARG for refused sizes).
  * lsa_shared_prefix_wait_limit: the limit of each bounded wait, in nanoseconds (at most 1e10), of the calls
- * that the process launches from then on; negative: 1e9, as at the start; 0: every wait expires at once, which
- * takes the failure path without a failure. A captured call keeps the limit it was captured with. */
+ * that the process launches from then on; negative: 1e9, as at the start; 0: the kernels give up before their
+ * first wait, which takes the failure path without a failure. A captured call keeps the limit it was captured
+ * with. */
 int64_t lsa_shared_prefix_scratch(int dtype, int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_t P,
                                   int64_t T, int scored);
 int lsa_shared_prefix_wait_limit(int64_t limit_ns);

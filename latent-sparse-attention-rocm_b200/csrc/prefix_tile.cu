@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(bar_drain, 1);
         mbar_init(bar_tail, 1);
         mbar_init(bar_tail + 1, 32);
-        *abort_flag = 0;
+        *abort_flag = a.wait_ns == 0;  // then the MMA thread gives up before its first wait, copies in flight
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     grid_wait();  // the inputs, the lengths among them, and the parts' last readers
@@ -443,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tc_fence_after();
                     return ok;
                 };
-                bool ok = n == 0 || thread_wait(bar_q, 0, abort_flag, a.wait_ns);
+                bool ok = *abort_flag == 0 && (n == 0 || thread_wait(bar_q, 0, abort_flag, a.wait_ns));
                 if (ok && n > 0 && !w.streams) {
                     ok = key();
                     if (ok) {

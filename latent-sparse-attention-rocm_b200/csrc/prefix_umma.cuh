@@ -11,13 +11,8 @@ namespace lsa {
 
 constexpr int kChunk = 128;  // keys of a tile
 
-// Warp-uniform bounded wait on an mbarrier phase; false: it expired or another role gave up. A limit of
-// 0 expires without a look at the barrier.
+// Warp-uniform bounded wait on an mbarrier phase; false: it expired or another role gave up.
 __device__ __forceinline__ bool role_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint64_t limit_ns) {
-    if (limit_ns == 0) {
-        if ((threadIdx.x & 31) == 0) *abort_flag = 1;
-        return false;
-    }
     bool done = mbar_try_wait(bar, parity);
     if (__all_sync(0xFFFFFFFFu, done)) return true;
     const uint64_t t0 = global_ns();
@@ -35,10 +30,6 @@ __device__ __forceinline__ bool role_wait(uint64_t* bar, uint32_t parity, volati
 
 // The same for a role that is one thread; the flag and the clock are looked at now and then.
 __device__ __forceinline__ bool thread_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint64_t limit_ns) {
-    if (limit_ns == 0) {
-        *abort_flag = 1;
-        return false;
-    }
     uint64_t t0 = 0;
     for (int i = 0;; ++i) {
         if (mbar_try_wait(bar, parity)) return true;

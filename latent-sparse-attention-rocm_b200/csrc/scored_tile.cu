@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int s = 0; s < kQStages; ++s) mbar_init(&qfull[s], 1), mbar_init(&qempty[s], 1);
         for (int s = 0; s < 4; ++s) mbar_init(&sfull[s], 1), mbar_init(&sfree[s], 128);
         mbar_init(drain, 1);
-        *abort_flag = 0;
+        *abort_flag = a.wait_ns == 0;  // then the MMA thread gives up before its first wait, copies in flight
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) tmem_alloc(tmem_slot, 512);
@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (elect_one()) {
             const uint64_t kd0 = sw128_desc(sbase, 16, 1024), qd0 = sw128_desc(sbase + Sh::kOffQ, 16, 1024);
             int kpos = 0, qpos = 0, it = 0;
-            bool ok = true;
+            bool ok = *abort_flag == 0;
             for (int p = p0; ok && p < p1; ++p, kpos += 2) {
                 for (int t = 0; ok && t < nr; ++t, ++it) {
                     const int q = resident ? t : qpos;
