@@ -107,10 +107,10 @@ __device__ __forceinline__ void copy_rows(const EvictArgs& a, int b, int h, int 
 // CTAs are a cluster, hold a slice of the keys each, and join their histograms (DSMEM adds into the
 // bins' owner, one cluster barrier a pass) and their kept counts.
 // Selection is a chain of short steps, the copy is bandwidth: with several CTAs an SM one row's
-// copy covers another's chain. Measured (D 128, bf16): 64 ragged caches of up to 8191 keys, 8 heads, to 2048:
-// 185 us = 5.9 TB/s; 4 of 131072 to 8192: 70 us, of which the selection takes about 23 (the rows are
-// in lock-step: 256 CTAs, 32 keys a thread) and 268 MB of copying the rest; one of 2112 to 2048: 9.6 us,
-// 7 of them selection (load 1.9, a pass 1.1, counts and ids 1.7).
+// copy covers another's chain. Measured (D 128, bf16, called in a loop): 64 ragged caches of up to 8191 keys, 8
+// heads, to 2048: 187 us = 5.9 TB/s; 4 of 131072 to 8192: 72 us, of which the selection takes about 23 (the
+// rows are in lock-step: 256 CTAs, 32 keys a thread) and 268 MB of copying the rest; one of 2112 to 2048: 12 us
+// (the host's), the kernel alone 9.6, 7 of them selection (load 1.9, a pass 1.1, counts and ids 1.7).
 template <bool kSliced>
 __global__ void __launch_bounds__(kThreads, 2) evict_kernel(const EvictArgs a, int ranks_arg) {
     __shared__ __align__(16) int hist[kBins];

@@ -33,7 +33,10 @@ __device__ __forceinline__ void stage_rows(float* dst, int ld, const float* src,
 // fp32 inputs. One work item: up to 16 rows of a KV head x a range of keys, on the FMA pipes. A
 // warp holds two rows; a lane scores one key of a 32-key tile for both, the warp's running
 // maximum and sum follow the tile, and a lane then owns D / 32 output columns. Rows past a
-// sequence's length are staged as zeros, so what an unwritten slot holds is never used.
+// sequence's length are staged as zeros, so what an unwritten slot holds is never used. What bounds it: a
+// tile's loads are waited for at a barrier with nothing in flight beside them, and 16 rows are computed
+// whatever is live. Measured (32 / 8 heads, D 128): 16 sequences on 8192 prefix and up to 2048 own keys 286 us, where
+// the keys' bytes take 41; 8 x 64 tokens on 4096 keys 2.4 ms.
 template <int D>
 __global__ void __launch_bounds__(kSimtWarps * 32) prefix_simt_kernel(const PrefixArgs a, int prefix_items, int ptiles,
                                                                       int otiles) {

@@ -11,10 +11,10 @@
 // sum in fp32 registers, P rounded to the inputs' type for its product (fp16: times 2^15 first, the most
 // that it holds, or a weight below 2^-25 of the maximum would leave O and stay in the sum; the factor is in
 // both and cancels). The warps join through
-// shared memory at the end. Measured (32 / 8 heads, D 128, bf16, the join of the parts included): 48
-// ragged caches of up to 8191 keys, 1.19 GB, 181 us = 6.6 TB/s, the measured copy rate; 16 of 6144 keys 80
-// us = 5.1 TB/s; one of 24576 keys 24 us, of which 15 are the memory's. Keys at or past the range's end are zero-filled by the copy, so what
-// an unwritten slot holds is never used.
+// shared memory at the end. Measured (32 / 8 heads, D 128, bf16, called in a loop, the join of the parts
+// included): 48 ragged caches of up to 8191 keys, 1.2 GB, 188 us = 6.4 TB/s, 97 % of the measured copy rate; 16 of
+// 6144 keys 79 us = 5.1 TB/s; one of 24576 keys 23 us, of which 15 are the memory's. Keys at or past the range's
+// end are zero-filled by the copy, so what an unwritten slot holds is never used.
 #include "prefix.cuh"
 #include "umma.cuh"
 

@@ -25,9 +25,10 @@
 // 1400 cycles to the first 96 keys' P, 2200 with the other half's exponentials beside it), the rest
 // of P V - of which two run at a time: 3000 cycles a pair of chunks, where the MMAs alone take 2048; over
 // seconds, the power limit (SM clock 1.55 GHz). 148 tiles on 4096 keys: tensor pipe 62 % active, 64 % of
-// the exponential units. 64 tokens of 32 sequences on 10007 prefix keys (32 / 8 heads, D 128): 302 us =
-// 1.16 PFLOP/s, 70 % of the measured burst rate and 82 % of the sustained one. With two streams, the
-// keys: 50 GB/s an SM, 6.4 TB/s while the ring runs.
+// the exponential units. 64 tokens of 32 sequences on 10007 prefix keys (32 / 8 heads, D 128): 308 us =
+// 1.13 PFLOP/s in bursts of 40 graph replays (68 % of the measured burst rate), 352 us = 0.99 PFLOP/s called
+// in a loop (70 % of the sustained one). With two streams, the keys: 50 GB/s an SM, 6.4 TB/s while the
+// ring runs. A tile's dead rows cost what live ones do: the softmax masks them, it does not skip them.
 // Not kept: a part of the exponentials as polynomials on the FMA pipe (every 8th pair: no change, every
 // 4th 3 % slower, every 2nd 15 %); a polling MMA thread in place of try_wait (no change).
 // Rows of V at or past a sequence's length are zeroed in shared memory before their product, so

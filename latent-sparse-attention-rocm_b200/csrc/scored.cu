@@ -3,7 +3,9 @@
 // With every row's lse known (prefix.cuh), key j of sequence b and KV head h gains
 //   w_j = sum over the rows r = (token, head of the group) that see j of 2^(s_rj - lse_r)
 // (log2 domain), the total attention it received. One thread owns a key, so the sum has one
-// order and one writer: no atomics, the same bits every time.
+// order and one writer: no atomics, the same bits every time. K is read a second time and nothing is in flight
+// while a block computes: 8 caches of up to 8191 keys (32 / 8 heads, D 128) take 415 us with the attention, where
+// the bytes take 62.
 #include "prefix.cuh"
 
 namespace lsa {

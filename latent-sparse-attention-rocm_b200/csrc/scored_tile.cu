@@ -9,7 +9,9 @@
 // apiece. Row tiles are whole tokens ((token, query head of the group) rows, 128 / G tokens); up
 // to two of them stay in shared memory, more are streamed once per pair.
 // What bounds it: the memory and the exponential units about alike (128 rows: 2048 cycles of exponentials
-// a pair of tiles, 2900 in all). 32 rows x 4 heads of 4 sequences of 24576 keys: 41 us = 4.9 TB/s of K.
+// a pair of tiles, 2900 in all). 32 rows x 4 heads of 4 sequences of 24576 keys: 41 us = 4.9 TB/s of K
+// (the kernel alone). Fewer rows take the same: a tile's 128 columns are walked whatever is live (8 rows x 4 heads of 4
+// ragged sequences of up to 32768 keys, both passes: 134 us called in a loop, 32 rows: 141).
 // Warps: 0 TMA loads, 1 MMAs, 4-7 / 8-11 epilogue of the pair's first / second tile. What keys at
 // or past a sequence's length hold stays in their own lanes, which store nothing but the old score.
 #include "prefix_umma.cuh"

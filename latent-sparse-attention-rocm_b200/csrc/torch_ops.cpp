@@ -294,8 +294,8 @@ PrefixOut prefix_attention(const at::Tensor& q_in, const at::Tensor* kp_in, cons
     const int64_t bytes = lsa_shared_prefix_scratch(code, B, Tq, Hq, Hkv, D, P, T, scores_in != nullptr);
     TORCH_CHECK_VALUE(bytes >= 0, what, ": sizes out of range");
     auto stream = at::cuda::getCurrentCUDAStream();
-    // The parts' scratch is the call's own: it may be gigabytes, and one kept for the stream would have to
-    // move when a larger call comes, under the feet of a captured graph.
+    // The parts' scratch is the call's own: one kept for the stream would have to move when a larger call
+    // comes, under the feet of a captured graph.
     auto scratch = fresh({bytes}, at::kByte, q.device());
     const int64_t strides[13] = {stride_of(q, 0), stride_of(q, 1), stride_of(q, 2), P ? stride_of(kp, 0) : 0,
                                  P ? stride_of(kp, 1) : 0, P ? stride_of(vp, 0) : 0, P ? stride_of(vp, 1) : 0,

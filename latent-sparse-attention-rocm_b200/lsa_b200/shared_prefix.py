@@ -22,8 +22,9 @@ def shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths, scale=None, re
     that sees no key reads as zeros (log-sum-exp -inf). What the caches hold at or past
     ``lengths[b]`` is never used; a key that some row of the call sees must be finite.
     Tensors may be strided views (the head dimension contiguous, rows on 16-byte
-    boundaries); others are copied. fp32, fp16 or bf16; D 64 or 128. ``scale`` defaults to
-    ``D ** -0.5``. Output like q, contiguous; with ``return_lse`` also the natural
+    boundaries); others are copied. fp32, fp16 or bf16; D 64 or 128. For 16-bit inputs the
+    weights are rounded to the inputs' type for their product with the values (sums, joins and
+    log-sum-exp are fp32). ``scale``, positive, defaults to ``D ** -0.5``. Output like q, contiguous; with ``return_lse`` also the natural
     log-sum-exp of every row's scaled logits, fp32 [B, Tq, Hq]."""
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     ops = _lib.torch_ops()
