@@ -132,13 +132,13 @@ def draw(rng):
 
 
 def _power_scale(top, code):
-    """The smallest power of two s >= 2^-100 with top <= (the code's largest value) * s."""
+    """The smallest power of two s >= 2^-60 with top <= (the code's largest value) * s."""
     fraction, e = torch.frexp(top)  # top = fraction * 2^e, fraction in [0.5, 1)
     if code == "e4m3":  # 448 = 0.875 * 2^9
         e = torch.where(fraction <= 0.875, e - 9, e - 8)
     else:  # 127 = 0.9921875 * 2^7
         e = torch.where(fraction <= 0.9921875, e - 7, e - 6)
-    e = torch.where(top > 0, e, torch.full_like(e, -100)).clamp(min=-100)
+    e = torch.where(top > 0, e, torch.full_like(e, -60)).clamp(min=-60)
     return ((e.int() + 127) << 23).view(torch.float32)
 
 
@@ -480,7 +480,7 @@ def _exact_append(s):
     qmax = 448.0 if code == "e4m3" else 127.0
     B, Tq, Hkv, D = s["k"].shape
     page = s["k8"].shape[2]
-    powers = torch.tensor([2.0 ** e for e in range(-100, 121)], dtype=torch.float64, device="cuda")
+    powers = torch.tensor([2.0 ** e for e in range(-60, 121)], dtype=torch.float64, device="cuda")
     got = []
     for x, codes, scale in ((s["k"], s["k8"], s["ks"]), (s["v"], s["v8"], s["vs"])):
         codes, scale = codes.double(), scale.double()
