@@ -78,6 +78,62 @@ int lsa_evict(const void* k, const void* v, int64_t row_bytes, const int64_t* st
               int64_t capacity, void* k_out, void* v_out, float* scores_out, int32_t* lengths_out, int32_t* ids,
               cudaStream_t stream);
 
+/* ---------------------------------------------------------------- rotation, 8-bit paged cache */
+
+/* Norms of q and k for each head with the position rotation (no reference counterpart). q [B, T, Hq, D],
+ * k [B, T, Hkv, D] at strides[6], in elements: q (b, t, h), k (b, t, h), multiples of 16 bytes, the head dimension
+ * contiguous; D 64, 128 or 256. y = x * rsqrt(mean(x^2) + eps) * weight where a weight [D] (dtype or fp32, its code
+ * given) is not NULL; the first R values of a head (a multiple of 16, 0 to D) turn by positions[b pos_b + t pos_t] *
+ * frequencies[i] (fp64, R / 2 of them, radians), pairs (i, i + R / 2) or, interleaved, (2 i, 2 i + 1), times
+ * amplitude. positions int32, or int64 where wide_positions. Outputs contiguous. */
+int lsa_norm_rotate(const void* q, const void* k, int dtype, const int64_t* strides, int64_t B, int64_t T, int64_t Hq,
+                    int64_t Hkv, int64_t D, const void* positions, int wide_positions, int64_t pos_b, int64_t pos_t,
+                    const double* frequencies, int64_t R, int interleaved, float amplitude, const void* q_weight,
+                    int q_weight_dtype, const void* k_weight, int k_weight_dtype, float eps, void* q_out, void* k_out,
+                    cudaStream_t stream);
+
+/* A paged cache in 8 bits (no reference counterpart): k8 / v8 [pages, Hkv, page, D] codes (code 0: e4m3, 1: int8),
+ * k_scale / v_scale [pages, Hkv] fp32, all contiguous, codes 16-byte aligned; page 16, 32, 64 or 128, D 64 or 128,
+ * pages * Hkv * page below 2^31. table [rows, M] int32, rows table_ld apart: token t of sequence b is row t % page of
+ * page table[b][t / page]; entries outside [0, pages) hold nothing. M * page at most 2^30. */
+
+/* Append: k / v [B, Tq, Hkv, D] (dtype) at strides[6] as above; row i is token lengths[b] - Tq + i of sequence b; rows
+ * before token 0 or, where counts is not NULL, before the last counts[b], and tokens on unmapped pages, are dropped. A page's scale becomes the smallest power of two, at least
+ * 2^-60, that holds its new tokens' largest magnitude in a code (448, 127), or stays where older tokens of the page
+ * have a larger one; older codes follow a scale that grows. Ties round to even. */
+int lsa_append_quantized(const void* k, const void* v, int dtype, const int64_t* strides, void* k8, void* v8,
+                         float* k_scale, float* v_scale, int code, int64_t pages, int64_t page, const int32_t* table,
+                         int64_t table_ld, int64_t M, const int32_t* lengths, const int32_t* counts, int64_t B,
+                         int64_t Tq, int64_t Hkv, int64_t D, cudaStream_t stream);
+
+/* Page dst[i] becomes a copy of page src[i], i < n; pairs outside the pool are skipped. No page may be written twice,
+ * or read and written. */
+int lsa_move_pages(void* k8, void* v8, float* k_scale, float* v_scale, int64_t pages, int64_t page, int64_t Hkv,
+                   int64_t D, const int32_t* src, const int32_t* dst, int64_t n, cudaStream_t stream);
+
+/* Attention: q [B, Tq, Hq, D] fp16 or bf16 at q_strides[3] (b, t, h; elements, multiples of 8). Row (b, i) sees the
+ * tokens j < lengths[b] - Tq + i + 1 on mapped pages; none: zeros, lse -inf. out contiguous, lse [B, Tq, Hq] (natural
+ * logarithm) or NULL. scale > 0, scale * log2(e) finite in fp32. status: a device int32 that receives
+ * LSA_ERR_TIMEOUT if a bounded wait expires (their limit is lsa_shared_prefix_wait_limit's).
+ * lsa_quantized_scratch: the scratch bytes of a call with that many keys a sequence at most (M * page; W for the
+ * read, with Tq 1), LSA_ERR_ARG for refused sizes. */
+int64_t lsa_quantized_scratch(int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_t keys);
+int lsa_quantized_attention(const void* q, int dtype, const int64_t* q_strides, const void* k8, const void* v8,
+                            const float* k_scale, const float* v_scale, int code, int64_t pages, int64_t page,
+                            const int32_t* table, int64_t table_ld, int64_t M, const int32_t* lengths, int64_t B,
+                            int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, float scale, void* out, float* lse,
+                            void* scratch, int64_t scratch_bytes, int32_t* status, cudaStream_t stream);
+
+/* The sparse read: q [R, Hq, D] at q_strides[2] (row, h); row r attends to the positions lists[r][j], j < counts[r]
+ * (lists [R, W] contiguous), of table row rows[r] (r itself where rows is NULL). Positions outside
+ * [0, lengths[table row]) or on unmapped pages, and table rows outside [0, table_rows), are skipped. */
+int lsa_quantized_read(const void* q, int dtype, const int64_t* q_strides, const void* k8, const void* v8,
+                       const float* k_scale, const float* v_scale, int code, int64_t pages, int64_t page,
+                       const int32_t* table, int64_t table_ld, int64_t table_rows, int64_t M, const int32_t* lengths,
+                       const int32_t* lists, const int32_t* counts, const int32_t* rows, int64_t R, int64_t W,
+                       int64_t Hq, int64_t Hkv, int64_t D, float scale, void* out, void* scratch,
+                       int64_t scratch_bytes, cudaStream_t stream);
+
 /* ---------------------------------------------------------------- peer-memory exchange */
 
 /* The sharded decode steps' all-gathers over peer memory (no reference counterpart: the

@@ -1,0 +1,127 @@
+// quant.cu - attention over the 8-bit paged cache: the entry points and their plans (sm_100a).
+// quant.cuh has the formulas.
+#include <math.h>
+
+#include "prefix.cuh"
+#include "quant.cuh"
+
+namespace lsa {
+namespace {
+
+constexpr int kPlaces = 2 * 148;  // CTAs of the few-row kernel that run at a time
+constexpr int kFewRows = 16;      // rows of its tiles
+constexpr int kUnit = 128;        // keys that a CTA's four warps take at a time
+
+struct Plan {
+    int parts;
+    int64_t bytes;  // of scratch
+};
+
+// keys: the most that a row sees
+bool make_plan(int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_t keys, Plan* p) {
+    const int64_t rows = B * Tq * Hq, tiles = (Tq * (Hq / Hkv) + kFewRows - 1) / kFewRows;
+    p->parts = balance(B * Hkv * tiles, (keys + kUnit - 1) / kUnit, 1.5, kPlaces, kMaxQuantParts);
+    if (p->parts < 1) p->parts = 1;
+    p->bytes = p->parts > 1 ? p->parts * rows * (D + 1) * 4 : 0;
+    return true;
+}
+
+bool sizes_ok(int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_t keys) {
+    if (B < 0 || Tq < 0 || keys < 0 || Hkv < 1 || Hq < 1 || Hq % Hkv != 0 || (D != 64 && D != 128)) return false;
+    if (B > INT32_MAX || Tq > (1 << 24) || Hq > 65536 || keys > (1 << 30)) return false;
+    return B * Tq <= (int64_t)INT32_MAX / Hq;
+}
+
+int pool(QuantArgs* a, const void* k8, const void* v8, const float* ks, const float* vs, int code, int64_t pages,
+         int64_t page, int64_t Hkv, const int32_t* table, int64_t table_ld, int64_t table_rows, int64_t M,
+         const int32_t* lengths) {
+    if (code != kE4M3 && code != kInt8) return LSA_ERR_ARG;
+    if (page != 16 && page != 32 && page != 64 && page != 128) return LSA_ERR_ARG;
+    if (pages < 0 || M < 0 || table_ld < 0 || table_rows < 0) return LSA_ERR_ARG;
+    if (M > (1 << 30) / page || pages > INT32_MAX / (page * Hkv) || table_rows > INT32_MAX) return LSA_ERR_SIZE;
+    if (lengths == nullptr || (M > 0 && table == nullptr)) return LSA_ERR_ARG;
+    if (pages > 0 && (!k8 || !v8 || !ks || !vs)) return LSA_ERR_ARG;
+    if (reinterpret_cast<uintptr_t>(k8) % 16 != 0 || reinterpret_cast<uintptr_t>(v8) % 16 != 0) return LSA_ERR_ARG;
+    a->k8 = static_cast<const uint8_t*>(k8), a->v8 = static_cast<const uint8_t*>(v8);
+    a->ks = ks, a->vs = vs;
+    a->table = table, a->table_ld = table_ld, a->table_rows = (int)table_rows, a->M = (int)M, a->pages = (int)pages;
+    a->shift = page == 16 ? 4 : (page == 32 ? 5 : (page == 64 ? 6 : 7));
+    a->lengths = lengths;
+    return LSA_OK;
+}
+
+int run(QuantArgs& a, int dtype, int code, int64_t D, int64_t keys, float scale, void* scratch, int64_t scratch_bytes,
+        cudaStream_t stream) {
+    a.scale_log2 = scale * 1.4426950408889634f;
+    if (!(a.scale_log2 > 0) || !isfinite(a.scale_log2)) return LSA_ERR_ARG;
+    if (reinterpret_cast<uintptr_t>(a.q) % 16 != 0 || reinterpret_cast<uintptr_t>(a.out) % 16 != 0) return LSA_ERR_ARG;
+    if (a.q_b % 8 != 0 || a.q_t % 8 != 0 || a.q_h % 8 != 0) return LSA_ERR_ARG;
+    Plan p;
+    make_plan(a.B, a.Tq, a.Hq, a.Hkv, D, keys, &p);
+    if (p.bytes > 0 && (scratch == nullptr || scratch_bytes < p.bytes || reinterpret_cast<uintptr_t>(scratch) % 16 != 0))
+        return LSA_ERR_ARG;
+    a.rows = (int64_t)a.B * a.Tq * a.Hq;
+    a.parts = p.parts;
+    a.part_o = static_cast<float*>(scratch);
+    a.part_lse = a.part_o + p.parts * a.rows * D;
+    const int rc = launch_quant_rows(a, dtype, code, (int)D, stream);
+    return rc != LSA_OK || a.parts == 1 ? rc : launch_quant_join(a, dtype, (int)D, stream);
+}
+
+}  // namespace
+}  // namespace lsa
+
+extern "C" {
+
+int64_t lsa_quantized_scratch(int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_t keys) {
+    using namespace lsa;
+    if (!sizes_ok(B, Tq, Hq, Hkv, D, keys)) return LSA_ERR_ARG;
+    if (B == 0 || Tq == 0) return 0;
+    Plan p;
+    make_plan(B, Tq, Hq, Hkv, D, keys, &p);
+    return p.bytes;
+}
+
+int lsa_quantized_attention(const void* q, int dtype, const int64_t* q_strides, const void* k8, const void* v8,
+                            const float* k_scale, const float* v_scale, int code, int64_t pages, int64_t page,
+                            const int32_t* table, int64_t table_ld, int64_t M, const int32_t* lengths, int64_t B,
+                            int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, float scale, void* out, float* lse,
+                            void* scratch, int64_t scratch_bytes, int32_t* status, cudaStream_t stream) {
+    using namespace lsa;
+    if (page < 16 || page > 128 || M < 0 || M > (1 << 30)) return LSA_ERR_ARG;
+    if ((dtype != kF16 && dtype != kBF16) || !sizes_ok(B, Tq, Hq, Hkv, D, M * page)) return LSA_ERR_ARG;
+    if (B == 0 || Tq == 0) return LSA_OK;
+    if (q == nullptr || out == nullptr || q_strides == nullptr || status == nullptr) return LSA_ERR_ARG;
+    QuantArgs a = {};
+    const int rc = pool(&a, k8, v8, k_scale, v_scale, code, pages, page, Hkv, table, table_ld, B, M, lengths);
+    if (rc != LSA_OK) return rc;
+    a.q = q, a.q_b = q_strides[0], a.q_t = q_strides[1], a.q_h = q_strides[2];
+    a.out = out, a.lse = lse;
+    a.B = (int)B, a.Tq = (int)Tq, a.Hq = (int)Hq, a.Hkv = (int)Hkv, a.G = (int)(Hq / Hkv);
+    return run(a, dtype, code, D, M * page, scale, scratch, scratch_bytes, stream);
+}
+
+int lsa_quantized_read(const void* q, int dtype, const int64_t* q_strides, const void* k8, const void* v8,
+                       const float* k_scale, const float* v_scale, int code, int64_t pages, int64_t page,
+                       const int32_t* table, int64_t table_ld, int64_t table_rows, int64_t M, const int32_t* lengths,
+                       const int32_t* lists, const int32_t* counts, const int32_t* rows, int64_t R, int64_t W,
+                       int64_t Hq, int64_t Hkv, int64_t D, float scale, void* out, void* scratch,
+                       int64_t scratch_bytes, cudaStream_t stream) {
+    using namespace lsa;
+    if ((dtype != kF16 && dtype != kBF16) || !sizes_ok(R, 1, Hq, Hkv, D, W)) return LSA_ERR_ARG;
+    if (R == 0) return LSA_OK;
+    if (q == nullptr || out == nullptr || q_strides == nullptr || counts == nullptr || (W > 0 && lists == nullptr))
+        return LSA_ERR_ARG;
+    if (rows == nullptr && table_rows < R) return LSA_ERR_ARG;
+    QuantArgs a = {};
+    const int rc = pool(&a, k8, v8, k_scale, v_scale, code, pages, page, Hkv, table, table_ld, table_rows, M, lengths);
+    if (rc != LSA_OK) return rc;
+    a.q = q, a.q_b = q_strides[0], a.q_t = 0, a.q_h = q_strides[1];
+    a.lists = W > 0 ? lists : counts;  // without entries nothing is read of it
+    a.counts = counts, a.list_rows = rows, a.W = (int)W;
+    a.out = out, a.lse = nullptr;
+    a.B = (int)R, a.Tq = 1, a.Hq = (int)Hq, a.Hkv = (int)Hkv, a.G = (int)(Hq / Hkv);
+    return run(a, dtype, code, D, W, scale, scratch, scratch_bytes, stream);
+}
+
+}  // extern "C"

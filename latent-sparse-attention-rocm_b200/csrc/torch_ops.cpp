@@ -13,6 +13,12 @@
 //   lsa::scored_attention(q, k, v, lengths, scores, scale, k_prefix, v_prefix) -> (out, scores)
 //   lsa::evict(k, v, scores, lengths, budget, window, sink, capacity)
 //                     -> (k, v, scores, lengths, ids)            no reference counterpart
+//   lsa::norm_rotate(q, k, positions, frequencies, q_weight, k_weight, eps, interleaved, amplitude) -> (q, k)
+//   lsa::append_quantized(k, v, k8, v8, k_scale, v_scale, page_table, lengths, counts)  in place
+//   lsa::move_pages(k8, v8, k_scale, v_scale, src, dst)                              in place
+//   lsa::quantized_attention(q, k8, v8, k_scale, v_scale, page_table, lengths, scale) -> out
+//   lsa::quantized_attention_lse(the same) -> (out, lse)
+//   lsa::quantized_read(q, k8, v8, k_scale, v_scale, page_table, lengths, lists, counts, rows, scale) -> out
 //   lsa::workspace_counters() -> Tensor[]                      the cached counter buffers and status words (checks)
 // Meta implementations give FX / torch.compile the output shapes. Workspaces: scratch (any
 // content) and int32 counters (zero at rest: the kernels that use them leave them zero) cached
@@ -370,6 +376,251 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> evict_cud
     return {ko, vo, so, lo, ids};
 }
 
+std::tuple<at::Tensor, at::Tensor> norm_rotate_cuda(const at::Tensor& q_in, const at::Tensor& k_in,
+                                                    const at::Tensor& positions, const at::Tensor& frequencies_in,
+                                                    const std::optional<at::Tensor>& qw_in,
+                                                    const std::optional<at::Tensor>& kw_in, double eps,
+                                                    bool interleaved, double amplitude) {
+    const char* what = "norm_rotate";
+    for (const at::Tensor* t : {&q_in, &k_in, &positions, &frequencies_in, qw_in ? &*qw_in : nullptr, kw_in ? &*kw_in : nullptr})
+        TORCH_CHECK_VALUE(t == nullptr || (t->is_cuda() && t->device() == q_in.device()), what,
+                          " is a CUDA kernel (B200, sm_100a): every tensor on one CUDA device");
+    TORCH_CHECK_VALUE(q_in.dim() == 4 && k_in.dim() == 4 && k_in.size(0) == q_in.size(0) && k_in.size(1) == q_in.size(1) &&
+                          k_in.size(3) == q_in.size(3),
+                      what, ": q [B, T, Hq, D], k [B, T, Hkv, D]");
+    const int64_t B = q_in.size(0), T = q_in.size(1), Hq = q_in.size(2), D = q_in.size(3), Hkv = k_in.size(2);
+    TORCH_CHECK_VALUE(Hq > 0 && Hkv > 0 && Hq + Hkv <= 65536, what, ": at least a head of q and of k each");
+    TORCH_CHECK_VALUE(D == 64 || D == 128 || D == 256, what, ": head dim 64, 128 or 256, got ", D);
+    const auto dt = q_in.scalar_type();
+    TORCH_CHECK_VALUE((dt == at::kFloat || dt == at::kHalf || dt == at::kBFloat16) && k_in.scalar_type() == dt, what,
+                      ": q and k fp32, fp16 or bf16, of one type, got ", dt, ", ", k_in.scalar_type());
+    for (const auto* w : {&qw_in, &kw_in})
+        TORCH_CHECK_VALUE(!*w || ((*w)->dim() == 1 && (*w)->size(0) == D &&
+                                  ((*w)->scalar_type() == dt || (*w)->scalar_type() == at::kFloat)),
+                          what, ": a weight is [D], of q's type or fp32");
+    TORCH_CHECK_VALUE(positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong, what,
+                      ": positions int32 or int64, got ", positions.scalar_type());
+    const bool shared = positions.dim() == 1;
+    TORCH_CHECK_VALUE(shared ? positions.size(0) == T
+                             : positions.dim() == 2 && positions.size(0) == B && positions.size(1) == T,
+                      what, ": positions [B, T] or [T]");
+    TORCH_CHECK_VALUE(frequencies_in.dim() == 1 && frequencies_in.is_floating_point(), what, ": frequencies [R / 2] fp64");
+    const int64_t R = 2 * frequencies_in.size(0);
+    TORCH_CHECK_VALUE(R <= D && R % 16 == 0, what, ": a multiple of 16 values turn, at most the head's ", D, ", got ", R);
+    TORCH_CHECK_VALUE(std::isfinite((float)amplitude) && std::isfinite((float)eps) && eps >= 0, what,
+                      ": amplitude and eps finite, eps not negative, got ", amplitude, ", ", eps);
+    c10::cuda::CUDAGuard guard(q_in.device());
+    auto q = rows16(q_in), k = rows16(k_in);
+    auto f = frequencies_in.scalar_type() == at::kDouble && frequencies_in.is_contiguous()
+                 ? frequencies_in
+                 : frequencies_in.to(at::kDouble).contiguous();
+    at::Tensor qw, kw;
+    if (qw_in) qw = rows16(*qw_in);
+    if (kw_in) kw = rows16(*kw_in);
+    auto qo = fresh({B, T, Hq, D}, dt, q.device()), ko = fresh({B, T, Hkv, D}, dt, q.device());
+    if (B * T == 0) return {qo, ko};
+    const int64_t strides[6] = {stride_of(q, 0), stride_of(q, 1), stride_of(q, 2),
+                                stride_of(k, 0), stride_of(k, 1), stride_of(k, 2)};
+    check_rc(lsa_norm_rotate(q.data_ptr(), k.data_ptr(), dtype_code(dt), strides, B, T, Hq, Hkv, D, positions.data_ptr(),
+                             positions.scalar_type() == at::kLong, shared ? 0 : positions.stride(0), positions.stride(-1),
+                             R ? f.data_ptr<double>() : nullptr, R, interleaved, (float)amplitude,
+                             qw_in ? qw.data_ptr() : nullptr, qw_in ? dtype_code(qw.scalar_type()) : 0,
+                             kw_in ? kw.data_ptr() : nullptr, kw_in ? dtype_code(kw.scalar_type()) : 0, (float)eps,
+                             qo.data_ptr(), ko.data_ptr(), at::cuda::getCurrentCUDAStream()),
+             what);
+    return {qo, ko};
+}
+
+// The pool of an 8-bit paged cache, as it is (it is written in place, and too large to copy).
+struct Pool {
+    int code;
+    int64_t pages, Hkv, page, D;
+};
+
+Pool check_pool(const at::Tensor& k8, const at::Tensor& v8, const at::Tensor& ks, const at::Tensor& vs, const char* what) {
+    for (const at::Tensor* t : {&k8, &v8, &ks, &vs}) {
+        TORCH_CHECK_VALUE(t->is_cuda() && t->device() == k8.device(), what,
+                          " is a CUDA kernel (B200, sm_100a): every tensor on one CUDA device");
+        TORCH_CHECK_VALUE(t->is_contiguous(), what, ": a pool's codes and scales are contiguous");
+    }
+    TORCH_CHECK_VALUE(k8.dim() == 4 && v8.sizes() == k8.sizes(), what, ": codes [pages, Hkv, page, D]");
+    TORCH_CHECK_VALUE((k8.scalar_type() == at::kFloat8_e4m3fn || k8.scalar_type() == at::kChar) &&
+                          v8.scalar_type() == k8.scalar_type(),
+                      what, ": codes are float8_e4m3fn or int8, of one type, got ", k8.scalar_type(), ", ", v8.scalar_type());
+    Pool p{k8.scalar_type() == at::kChar ? 1 : 0, k8.size(0), k8.size(1), k8.size(2), k8.size(3)};
+    TORCH_CHECK_VALUE(p.page == 16 || p.page == 32 || p.page == 64 || p.page == 128, what,
+                      ": pages of 16, 32, 64 or 128 tokens, got ", p.page);
+    TORCH_CHECK_VALUE(p.Hkv > 0 && p.Hkv <= 65535 && (p.D == 64 || p.D == 128), what, ": KV heads, and head dim 64 or 128, got ", p.D);
+    TORCH_CHECK_VALUE(p.pages <= INT32_MAX / (p.Hkv * p.page), what, ": a pool of fewer than 2^31 (page, head, token) rows");
+    for (const at::Tensor* t : {&ks, &vs})
+        TORCH_CHECK_VALUE(t->scalar_type() == at::kFloat && t->dim() == 2 && t->size(0) == p.pages && t->size(1) == p.Hkv,
+                          what, ": scales [pages, Hkv] fp32");
+    for (const at::Tensor* t : {&k8, &v8})
+        TORCH_CHECK_VALUE(reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0, what, ": codes on a 16-byte boundary");
+    return p;
+}
+
+// Page table [rows, M] as int32 with contiguous rows, and its lengths.
+at::Tensor check_table(const at::Tensor& table, const at::Tensor& lengths, const Pool& p, const at::Device& dev,
+                       const char* what) {
+    TORCH_CHECK_VALUE(table.is_cuda() && lengths.is_cuda() && table.device() == dev && lengths.device() == dev, what,
+                      " is a CUDA kernel (B200, sm_100a): every tensor on one CUDA device");
+    TORCH_CHECK_VALUE(table.dim() == 2 && !table.is_floating_point(), what, ": a page table [B, M] of whole numbers");
+    TORCH_CHECK_VALUE(lengths.numel() == table.size(0) && !lengths.is_floating_point(), what, ": one whole length a sequence");
+    TORCH_CHECK_VALUE(table.size(1) <= (1 << 30) / p.page, what, ": a table of at most 2^30 tokens a sequence");
+    if (table.scalar_type() == at::kInt && (table.size(1) <= 1 || table.stride(1) == 1) && (table.size(0) <= 1 || table.stride(0) >= 0))
+        return table;
+    return table.to(at::kInt).contiguous();
+}
+
+void append_quantized_cuda(const at::Tensor& k_in, const at::Tensor& v_in, const at::Tensor& k8, const at::Tensor& v8,
+                           const at::Tensor& ks, const at::Tensor& vs, const at::Tensor& table_in,
+                           const at::Tensor& lengths_in, const std::optional<at::Tensor>& counts_in) {
+    const char* what = "append_quantized";
+    const Pool p = check_pool(k8, v8, ks, vs, what);
+    TORCH_CHECK_VALUE(k_in.is_cuda() && k_in.device() == k8.device() && v_in.is_cuda() && v_in.device() == k8.device(), what,
+                      " is a CUDA kernel (B200, sm_100a): every tensor on one CUDA device");
+    TORCH_CHECK_VALUE(k_in.dim() == 4 && v_in.sizes() == k_in.sizes() && k_in.size(2) == p.Hkv && k_in.size(3) == p.D &&
+                          k_in.size(0) == table_in.size(0),
+                      what, ": k and v [B, Tq, ", p.Hkv, ", ", p.D, "], a table row a sequence");
+    const auto dt = k_in.scalar_type();
+    TORCH_CHECK_VALUE((dt == at::kFloat || dt == at::kHalf || dt == at::kBFloat16) && v_in.scalar_type() == dt, what,
+                      ": k and v fp32, fp16 or bf16, of one type, got ", dt, ", ", v_in.scalar_type());
+    c10::cuda::CUDAGuard guard(k8.device());
+    auto table = check_table(table_in, lengths_in, p, k8.device(), what);
+    auto lengths = as_lengths(lengths_in);
+    at::Tensor counts;
+    if (counts_in) {
+        TORCH_CHECK_VALUE(counts_in->is_cuda() && counts_in->device() == k8.device() && !counts_in->is_floating_point() &&
+                              counts_in->numel() == k_in.size(0),
+                          what, ": one whole count a sequence, on the pool's device");
+        counts = as_lengths(*counts_in);
+    }
+    auto k = rows16(k_in), v = rows16(v_in);
+    const int64_t strides[6] = {stride_of(k, 0), stride_of(k, 1), stride_of(k, 2),
+                                stride_of(v, 0), stride_of(v, 1), stride_of(v, 2)};
+    check_rc(lsa_append_quantized(k.data_ptr(), v.data_ptr(), dtype_code(dt), strides, k8.data_ptr(), v8.data_ptr(),
+                                  ks.data_ptr<float>(), vs.data_ptr<float>(), p.code, p.pages, p.page,
+                                  table.data_ptr<int32_t>(), stride_of(table, 0), table.size(1),
+                                  lengths.data_ptr<int32_t>(), counts_in ? counts.data_ptr<int32_t>() : nullptr, k.size(0),
+                                  k.size(1), p.Hkv, p.D,
+                                  at::cuda::getCurrentCUDAStream()),
+             what);
+}
+
+void move_pages_cuda(const at::Tensor& k8, const at::Tensor& v8, const at::Tensor& ks, const at::Tensor& vs,
+                     const at::Tensor& src_in, const at::Tensor& dst_in) {
+    const char* what = "move_pages";
+    const Pool p = check_pool(k8, v8, ks, vs, what);
+    for (const at::Tensor* t : {&src_in, &dst_in})
+        TORCH_CHECK_VALUE(t->is_cuda() && t->device() == k8.device(), what,
+                          " is a CUDA kernel (B200, sm_100a): every tensor on one CUDA device");
+    TORCH_CHECK_VALUE(src_in.dim() == 1 && dst_in.sizes() == src_in.sizes() && !src_in.is_floating_point() &&
+                          !dst_in.is_floating_point(),
+                      what, ": src and dst [n] of whole numbers");
+    c10::cuda::CUDAGuard guard(k8.device());
+    auto src = as_lengths(src_in), dst = as_lengths(dst_in);
+    check_rc(lsa_move_pages(k8.data_ptr(), v8.data_ptr(), ks.data_ptr<float>(), vs.data_ptr<float>(), p.pages, p.page,
+                            p.Hkv, p.D, src.data_ptr<int32_t>(), dst.data_ptr<int32_t>(), src.size(0),
+                            at::cuda::getCurrentCUDAStream()),
+             what);
+}
+
+void check_rows(const at::Tensor& q, const Pool& p, const at::Device& dev, double scale, const char* what) {
+    TORCH_CHECK_VALUE(q.is_cuda() && q.device() == dev, what,
+                      " is a CUDA kernel (B200, sm_100a): every tensor on one CUDA device");
+    TORCH_CHECK_VALUE(q.dim() == 4 && q.size(3) == p.D && q.size(2) > 0 && q.size(2) % p.Hkv == 0, what,
+                      ": q [B, Tq, Hq, ", p.D, "], Hq a multiple of ", p.Hkv);
+    TORCH_CHECK_VALUE(q.scalar_type() == at::kHalf || q.scalar_type() == at::kBFloat16, what, ": q fp16 or bf16, got ",
+                      q.scalar_type());
+    const float scale_log2 = (float)scale * 1.4426950408889634f;  // as the entry point takes it
+    TORCH_CHECK_VALUE(std::isfinite(scale_log2) && scale_log2 > 0, what,
+                      ": the scale must be positive, and with log2(e) within fp32, got ", scale);
+}
+
+std::pair<at::Tensor, at::Tensor> quantized(const at::Tensor& q_in, const at::Tensor& k8, const at::Tensor& v8,
+                                            const at::Tensor& ks, const at::Tensor& vs, const at::Tensor& table_in,
+                                            const at::Tensor& lengths_in, double scale, bool want_lse) {
+    const char* what = "quantized_attention";
+    const Pool p = check_pool(k8, v8, ks, vs, what);
+    check_rows(q_in, p, k8.device(), scale, what);
+    const int64_t B = q_in.size(0), Tq = q_in.size(1), Hq = q_in.size(2);
+    TORCH_CHECK_VALUE(table_in.dim() == 2 && table_in.size(0) == B, what, ": a table row a sequence");
+    c10::cuda::CUDAGuard guard(k8.device());
+    auto table = check_table(table_in, lengths_in, p, k8.device(), what);
+    auto lengths = as_lengths(lengths_in);
+    auto q = rows16(q_in);
+    auto out = fresh({B, Tq, Hq, p.D}, q.scalar_type(), q.device());
+    at::Tensor lse;
+    if (want_lse) lse = fresh({B, Tq, Hq}, at::kFloat, q.device());
+    if (B * Tq == 0) return {out, lse};
+    const int64_t M = table.size(1), bytes = lsa_quantized_scratch(B, Tq, Hq, p.Hkv, p.D, M * p.page);
+    TORCH_CHECK_VALUE(bytes >= 0, what, ": sizes out of range");
+    at::Tensor scratch;  // the call's own, as the shared-prefix operators'
+    if (bytes > 0) scratch = fresh({bytes}, at::kByte, q.device());
+    const int64_t strides[3] = {stride_of(q, 0), stride_of(q, 1), stride_of(q, 2)};
+    check_rc(lsa_quantized_attention(q.data_ptr(), dtype_code(q.scalar_type()), strides, k8.data_ptr(), v8.data_ptr(),
+                                     ks.data_ptr<float>(), vs.data_ptr<float>(), p.code, p.pages, p.page,
+                                     table.data_ptr<int32_t>(), stride_of(table, 0), M, lengths.data_ptr<int32_t>(), B, Tq,
+                                     Hq, p.Hkv, p.D, (float)scale, out.data_ptr(),
+                                     want_lse ? lse.data_ptr<float>() : nullptr, bytes > 0 ? scratch.data_ptr() : nullptr,
+                                     bytes, status_word(q.device()), at::cuda::getCurrentCUDAStream()),
+             what);
+    return {out, lse};
+}
+
+at::Tensor quantized_cuda(const at::Tensor& q, const at::Tensor& k8, const at::Tensor& v8, const at::Tensor& ks,
+                          const at::Tensor& vs, const at::Tensor& table, const at::Tensor& lengths, double scale) {
+    return quantized(q, k8, v8, ks, vs, table, lengths, scale, false).first;
+}
+
+std::tuple<at::Tensor, at::Tensor> quantized_lse_cuda(const at::Tensor& q, const at::Tensor& k8, const at::Tensor& v8,
+                                                      const at::Tensor& ks, const at::Tensor& vs,
+                                                      const at::Tensor& table, const at::Tensor& lengths, double scale) {
+    auto r = quantized(q, k8, v8, ks, vs, table, lengths, scale, true);
+    return {r.first, r.second};
+}
+
+at::Tensor quantized_read_cuda(const at::Tensor& q_in, const at::Tensor& k8, const at::Tensor& v8, const at::Tensor& ks,
+                               const at::Tensor& vs, const at::Tensor& table_in, const at::Tensor& lengths_in,
+                               const at::Tensor& lists_in, const at::Tensor& counts_in,
+                               const std::optional<at::Tensor>& rows_in, double scale) {
+    const char* what = "quantized_read";
+    const Pool p = check_pool(k8, v8, ks, vs, what);
+    check_rows(q_in, p, k8.device(), scale, what);
+    for (const at::Tensor* t : {&lists_in, &counts_in, rows_in ? &*rows_in : nullptr})
+        TORCH_CHECK_VALUE(t == nullptr || (t->is_cuda() && t->device() == k8.device() && !t->is_floating_point()), what,
+                          " is a CUDA kernel (B200, sm_100a): lists, counts and rows of whole numbers on one CUDA device");
+    const int64_t R = q_in.size(0), Hq = q_in.size(2);
+    TORCH_CHECK_VALUE(q_in.size(1) == 1 && lists_in.dim() == 2 && lists_in.size(0) == R && counts_in.numel() == R &&
+                          (!rows_in || rows_in->numel() == R),
+                      what, ": q [R, 1, Hq, D], lists [R, W], one count and one table row a row");
+    TORCH_CHECK_VALUE(rows_in || (table_in.dim() == 2 && table_in.size(0) == R), what,
+                      ": without rows, a table row a query row");
+    c10::cuda::CUDAGuard guard(k8.device());
+    auto table = check_table(table_in, lengths_in, p, k8.device(), what);
+    auto lengths = as_lengths(lengths_in), counts = as_lengths(counts_in), lists = as_lengths(lists_in);
+    at::Tensor rows;
+    if (rows_in) rows = as_lengths(*rows_in);
+    auto q = rows16(q_in);
+    auto out = fresh({R, 1, Hq, p.D}, q.scalar_type(), q.device());
+    if (R == 0) return out;
+    const int64_t W = lists.size(1), bytes = lsa_quantized_scratch(R, 1, Hq, p.Hkv, p.D, W);
+    TORCH_CHECK_VALUE(bytes >= 0, what, ": sizes out of range");
+    at::Tensor scratch;
+    if (bytes > 0) scratch = fresh({bytes}, at::kByte, q.device());
+    const int64_t strides[2] = {stride_of(q, 0), stride_of(q, 2)};
+    check_rc(lsa_quantized_read(q.data_ptr(), dtype_code(q.scalar_type()), strides, k8.data_ptr(), v8.data_ptr(),
+                                ks.data_ptr<float>(), vs.data_ptr<float>(), p.code, p.pages, p.page,
+                                table.data_ptr<int32_t>(), stride_of(table, 0), table.size(0), table.size(1),
+                                lengths.data_ptr<int32_t>(), lists.data_ptr<int32_t>(), counts.data_ptr<int32_t>(),
+                                rows_in ? rows.data_ptr<int32_t>() : nullptr, R, W, Hq, p.Hkv, p.D, (float)scale,
+                                out.data_ptr(), bytes > 0 ? scratch.data_ptr() : nullptr, bytes,
+                                at::cuda::getCurrentCUDAStream()),
+             what);
+    return out;
+}
+
 std::vector<at::Tensor> workspace_counters() {
     std::lock_guard<std::mutex> lock(g_ws_mutex);
     std::vector<at::Tensor> out;
@@ -427,6 +678,36 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> evict_met
             at::empty({B, Hkv, capacity}, i32)};
 }
 
+std::tuple<at::Tensor, at::Tensor> norm_rotate_meta(const at::Tensor& q, const at::Tensor& k, const at::Tensor&,
+                                                    const at::Tensor&, const std::optional<at::Tensor>&,
+                                                    const std::optional<at::Tensor>&, double, bool, double) {
+    return {at::empty(q.sizes(), q.options()), at::empty(k.sizes(), k.options())};
+}
+
+void append_quantized_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                           const at::Tensor&, const at::Tensor&, const at::Tensor&, const std::optional<at::Tensor>&) {}
+
+void move_pages_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                     const at::Tensor&) {}
+
+at::Tensor quantized_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                          const at::Tensor&, const at::Tensor&, double) {
+    return at::empty(q.sizes(), q.options());
+}
+
+std::tuple<at::Tensor, at::Tensor> quantized_lse_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor&,
+                                                      const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                                                      const at::Tensor&, double) {
+    return {at::empty(q.sizes(), q.options()),
+            at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat))};
+}
+
+at::Tensor quantized_read_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                               const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                               const at::Tensor&, const std::optional<at::Tensor>&, double) {
+    return at::empty(q.sizes(), q.options());
+}
+
 }  // namespace
 
 TORCH_LIBRARY(lsa, m) {
@@ -442,6 +723,17 @@ TORCH_LIBRARY(lsa, m) {
           "Tensor? k_prefix=None, Tensor? v_prefix=None) -> (Tensor, Tensor)");
     m.def("evict(Tensor k, Tensor v, Tensor scores, Tensor lengths, int budget, int window, int sink, int capacity) "
           "-> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+    m.def("norm_rotate(Tensor q, Tensor k, Tensor positions, Tensor frequencies, Tensor? q_weight, Tensor? k_weight, "
+          "float eps, bool interleaved, float amplitude) -> (Tensor, Tensor)");
+    m.def("append_quantized(Tensor k, Tensor v, Tensor(a!) k8, Tensor(b!) v8, Tensor(c!) k_scale, Tensor(d!) v_scale, "
+          "Tensor page_table, Tensor lengths, Tensor? counts=None) -> ()");
+    m.def("move_pages(Tensor(a!) k8, Tensor(b!) v8, Tensor(c!) k_scale, Tensor(d!) v_scale, Tensor src, Tensor dst) -> ()");
+    m.def("quantized_attention(Tensor q, Tensor k8, Tensor v8, Tensor k_scale, Tensor v_scale, Tensor page_table, "
+          "Tensor lengths, float scale) -> Tensor");
+    m.def("quantized_attention_lse(Tensor q, Tensor k8, Tensor v8, Tensor k_scale, Tensor v_scale, Tensor page_table, "
+          "Tensor lengths, float scale) -> (Tensor, Tensor)");
+    m.def("quantized_read(Tensor q, Tensor k8, Tensor v8, Tensor k_scale, Tensor v_scale, Tensor page_table, "
+          "Tensor lengths, Tensor lists, Tensor counts, Tensor? rows, float scale) -> Tensor");
     m.def("workspace_counters() -> Tensor[]", &workspace_counters);
 }
 
@@ -453,6 +745,12 @@ TORCH_LIBRARY_IMPL(lsa, CUDA, m) {
     m.impl("shared_prefix_attention_lse", &shared_prefix_lse_cuda);
     m.impl("scored_attention", &scored_cuda);
     m.impl("evict", &evict_cuda);
+    m.impl("norm_rotate", &norm_rotate_cuda);
+    m.impl("append_quantized", &append_quantized_cuda);
+    m.impl("move_pages", &move_pages_cuda);
+    m.impl("quantized_attention", &quantized_cuda);
+    m.impl("quantized_attention_lse", &quantized_lse_cuda);
+    m.impl("quantized_read", &quantized_read_cuda);
 }
 
 // CPU tensors: the operators' own refusal (a ValueError) in place of the dispatcher's
@@ -461,6 +759,12 @@ TORCH_LIBRARY_IMPL(lsa, CPU, m) {
     m.impl("shared_prefix_attention_lse", &shared_prefix_lse_cuda);
     m.impl("scored_attention", &scored_cuda);
     m.impl("evict", &evict_cuda);
+    m.impl("norm_rotate", &norm_rotate_cuda);
+    m.impl("append_quantized", &append_quantized_cuda);
+    m.impl("move_pages", &move_pages_cuda);
+    m.impl("quantized_attention", &quantized_cuda);
+    m.impl("quantized_attention_lse", &quantized_lse_cuda);
+    m.impl("quantized_read", &quantized_read_cuda);
 }
 
 TORCH_LIBRARY_IMPL(lsa, Meta, m) {
@@ -471,4 +775,10 @@ TORCH_LIBRARY_IMPL(lsa, Meta, m) {
     m.impl("shared_prefix_attention_lse", &shared_prefix_lse_meta);
     m.impl("scored_attention", &scored_meta);
     m.impl("evict", &evict_meta);
+    m.impl("norm_rotate", &norm_rotate_meta);
+    m.impl("append_quantized", &append_quantized_meta);
+    m.impl("move_pages", &move_pages_meta);
+    m.impl("quantized_attention", &quantized_meta);
+    m.impl("quantized_attention_lse", &quantized_lse_meta);
+    m.impl("quantized_read", &quantized_read_meta);
 }

@@ -29,6 +29,15 @@ from .pipeline import (  # noqa: F401
     tree_select,
     visible_counts,
 )
+from .quantized import (  # noqa: F401
+    QuantizedCache,
+    QuantizedPages,
+    append_quantized,
+    move_pages,
+    quantized_attention,
+    quantized_read,
+)
+from .rotate import norm_rotate, rotary_frequencies  # noqa: F401
 from .shared_prefix import shared_prefix_attention  # noqa: F401
 
 __all__ = [
@@ -36,5 +45,6 @@ __all__ = [
     "build_hierarchy_gpu", "dense_read", "flat_select", "flat_select_reference", "lsa_read",
     "make_index_space", "position_buckets", "select_from_queries", "tree_select", "visible_counts",
     "check_status", "shared_prefix_attention", "scored_attention", "evict", "EvictedCache",
-    "BudgetedCache",
+    "BudgetedCache", "norm_rotate", "rotary_frequencies", "QuantizedPages", "append_quantized",
+    "quantized_attention", "quantized_read", "move_pages", "QuantizedCache",
 ]

@@ -87,6 +87,16 @@ SIGNATURES = {
     "lsa_shared_prefix_attention": (_INT, [_P, _P, _P, _P, _P, _INT, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _P, _P,
                                            _P, _P, _P, _I, _P, _P]),
     "lsa_evict": (_INT, [_P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P]),
+    "lsa_norm_rotate": (_INT, [_P, _P, _INT, _P, _I, _I, _I, _I, _I, _P, _INT, _I, _I, _P, _I, _INT, _F, _P, _INT, _P,
+                               _INT, _F, _P, _P, _P]),
+    "lsa_append_quantized": (_INT, [_P, _P, _INT, _P, _P, _P, _P, _P, _INT, _I, _I, _P, _I, _I, _P, _P, _I, _I, _I,
+                                    _I, _P]),
+    "lsa_move_pages": (_INT, [_P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _I, _P]),
+    "lsa_quantized_scratch": (_I, [_I, _I, _I, _I, _I, _I]),
+    "lsa_quantized_attention": (_INT, [_P, _INT, _P, _P, _P, _P, _P, _INT, _I, _I, _P, _I, _I, _P, _I, _I, _I, _I, _I,
+                                       _F, _P, _P, _P, _I, _P, _P]),
+    "lsa_quantized_read": (_INT, [_P, _INT, _P, _P, _P, _P, _P, _INT, _I, _I, _P, _I, _I, _I, _P, _P, _P, _P, _I, _I,
+                                  _I, _I, _I, _F, _P, _P, _I, _P]),
     "lsa_tree_plan": (_INT, [_I, _I, _P, _I, _I, _I, _I, _I, _P, _P]),
     "lsa_tree_select": (_INT, [_P, _I, _I, _P, _I, _I, _I, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _I, _P,
                                _I, _P]),
