@@ -8,8 +8,8 @@
 namespace lsa {
 namespace {
 
-constexpr int kPlaces = 2 * 148;  // CTAs of the few-row kernel that run at a time
-constexpr int kFewRows = 16;      // rows of its tiles
+constexpr int kSMs = 148;
+constexpr int kFewRows = 16;  // rows of the few-row kernel's tiles
 constexpr int kUnit = 128;        // keys that a CTA's four warps take at a time
 
 struct Plan {
@@ -20,7 +20,8 @@ struct Plan {
 // keys: the most that a row sees
 bool make_plan(int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_t keys, Plan* p) {
     const int64_t rows = B * Tq * Hq, tiles = (Tq * (Hq / Hkv) + kFewRows - 1) / kFewRows;
-    p->parts = balance(B * Hkv * tiles, (keys + kUnit - 1) / kUnit, 1.5, kPlaces, kMaxQuantParts);
+    const int places = kSMs * (Tq * (Hq / Hkv) <= 8 ? 3 : 2);  // CTAs of the few-row kernel that run at a time
+    p->parts = balance(B * Hkv * tiles, (keys + kUnit - 1) / kUnit, 1.5, places, kMaxQuantParts);
     if (p->parts < 1) p->parts = 1;
     p->bytes = p->parts > 1 ? p->parts * rows * (D + 1) * 4 : 0;
     return true;

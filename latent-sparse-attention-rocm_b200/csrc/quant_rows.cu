@@ -4,34 +4,35 @@
 // A work item is at most 16 query rows of one KV head (a sequence's last tokens; of the read one token's G query
 // heads) x a range of keys. The keys' bytes bound it: 2 D a key and head. So nothing waits for a neighbour in the
 // main loop: each of a CTA's four warps copies its own tiles of 32 keys (cp.async, 16 bytes, kRing tiles in
-// flight) and runs its own online softmax on them. S = Q K^T and O += P V by mma.sync.m16n8k16 in fp16 (one
-// M = 16 tile holds all rows), the codes made halves in registers on their way into the fragments, which
-// is exact:
+// flight) and runs its own online softmax on them. S^T = K Q^T and O^T += V^T P^T by mma.sync.m16n8k16 in fp16:
+// keys, then columns of V, are the M = 16 side and the rows the N = 8 (twice for more than eight), so few rows cost
+// few accumulators. The codes become halves in registers on their way into the fragments, which is exact:
 //   K: a lane takes 16 bytes of key g = lane / 4 at a time, four consecutive bytes a k-step; Q's fragments are
 //      loaded in the same order of D, which a product does not see.
 //   V: a lane takes D / 8 bytes of four keys and makes pairs of two keys' codes (the fragment's order) by byte
-//      permutes; a k-step's eight columns are then D / 8 apart, and the output's columns are put back at the end.
+//      permutes; M's rows g and g + 8 are then columns (D / 8) g + 2 j and + 1, put back at the end.
+//   P: 8 x 8 blocks transposed by movmatrix.
 // Q is made fp16 as well: bf16 rows by an exact power of two that brings their largest value to [2^8, 2^9)
 // (what is 2^-22 of it or less loses bits, 2^-33 of it at most), back in the row's factor.
-// P (at most 1) is rounded to fp16 for its product, times 2^15, the most that it holds: 2^-40 of a row's largest
-// is kept. Sums, maxima and joins are fp32.
+// P is rounded to fp16 for its product. It carries 2^kLift, and the maximum is let stand until it has grown by
+// more than 2^kGrow, so P is at most 2^15 and 2^-35 of a row's largest is kept. Sums, maxima and joins are fp32.
 #include <type_traits>
 
+#include "prefix_umma.cuh"
 #include "quant.cuh"
-#include "umma.cuh"
 
 namespace lsa {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kRows = 16;
 constexpr int kKeys = 32;  // keys of a warp's tile: one a lane where they are looked up
-constexpr float kLift = 15.0f;
+constexpr float kLift = 10.0f, kGrow = 5.0f;
 
-template <int D> struct QuantShape {
-    static constexpr int kRing = D == 128 ? 3 : 5;     // tiles in a warp's ring
+template <int D, int NT> struct QuantShape {
+    static constexpr int kRows = 8 * NT;
+    static constexpr int kRing = D == 128 ? (NT == 1 ? 2 : 3) : (NT == 1 ? 4 : 5);  // tiles in a warp's ring
     static constexpr int kTile = kKeys * D;            // K or V bytes of a tile
-    static constexpr int kStage = 2 * kTile + kKeys * 8 + 16;  // + the keys' scales, + which keys are there
+    static constexpr int kStage = 2 * kTile + kKeys * 12;  // + ks, vs (then its logarithm) and 1 / vs of every key
     static constexpr int kWarpBytes = (kRing * kStage + 127) / 128 * 128;
     static constexpr int kSmem = kWarps * kWarpBytes + kWarps * kRows * 2 * 4;
     static_assert(kWarpBytes >= kRows * D * 4, "the join reuses a warp's ring");
@@ -56,9 +57,36 @@ __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r) : "r"(addr) : "memory");
     return r;
 }
-__device__ __forceinline__ float2 lds_f2(uint32_t addr) {
-    float2 r;
-    asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(r.x), "=f"(r.y) : "r"(addr) : "memory");
+__device__ __forceinline__ uint64_t lds64(uint32_t addr) {
+    uint64_t r;
+    asm volatile("ld.shared.b64 %0, [%1];" : "=l"(r) : "r"(addr) : "memory");
+    return r;
+}
+// Block of 8 x 8 halves, lane (g, c) holding [g][2c], [g][2c + 1], transposed.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+}
+__device__ __forceinline__ void cp_async16_all(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void sts_f32(uint32_t addr, float x) {
+    asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(x) : "memory");
+}
+__device__ __forceinline__ float lg2_approx(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
 template <int N> __device__ __forceinline__ void lds_words(uint32_t (&r)[N], uint32_t addr) {
@@ -81,11 +109,14 @@ template <int D> __device__ __forceinline__ uint32_t v_at(int r, int c) {
     return D == 128 ? r * 128 + ((c ^ (r & 6)) << 4) : (r >> 1) * 128 + (((((r & 1) << 2) | c) ^ (r & 6)) << 4);
 }
 
-template <typename T, int CODE, int D, bool LISTS>
-__global__ void __launch_bounds__(kWarps * 32, 2) quant_rows_kernel(const QuantArgs a, const int row_tiles) {
-    using Sh = QuantShape<D>;
+// NT: tiles of eight rows.
+template <typename T, int CODE, int D, bool LISTS, int NT>
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) quant_rows_kernel(const QuantArgs a, const int row_tiles) {
+    using Sh = QuantShape<D, NT>;
+    constexpr int kRows = 8 * NT;
     constexpr int C = D / 16;       // 16-byte chunks of a key
     constexpr int KS = D / 16;      // k-steps of S
+    constexpr int MT = D / 16;      // M tiles of O
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, c = lane & 3;
@@ -125,58 +156,90 @@ __global__ void __launch_bounds__(kWarps * 32, 2) quant_rows_kernel(const QuantA
     const uint32_t ring = smem_u32(smem) + warp * Sh::kWarpBytes;
     const int tiles = k1 - k0 > warp * kKeys ? (k1 - k0 - warp * kKeys + kWarps * kKeys - 1) / (kWarps * kKeys) : 0;
 
-    // tile i of this warp: keys k0 + (warp + 4 i) 32 ..; a lane looks its key up, then the warp copies the rows
+    // Tile i of this warp: keys k0 + (warp + 4 i) 32 ..; a lane looks its key up, two tiles ahead the position, one
+    // the page; then the warp copies the rows.
+    auto position = [&](int i) {
+        const int key = k0 + (warp + kWarps * i) * kKeys + lane;
+        const bool in = i < tiles && key < k1;
+        return !in ? -1 : (LISTS ? list[key] : key);
+    };
+    auto page_of = [&](int pos) {
+        return pos >= 0 && pos < length && (pos >> a.shift) < a.M ? table[pos >> a.shift] : -1;
+    };
+    int pos1 = position(0), pos2 = position(1), page1 = page_of(pos1);
+    uint32_t there = 0;  // bit j: this lane's key of the j-th tile before the last copied is there
+    const uint8_t* const kl = a.k8 + (lane / C) * D + (lane % C) * 16;
+    const uint8_t* const vl = a.v8 + (lane / C) * D + (lane % C) * 16;
+    uint32_t slot = 0;  // of the next copy
     auto copy = [&](int i) {
+        const int pos = pos1, page = page1;
+        pos1 = pos2, page1 = page_of(pos2), pos2 = position(i + 2);
+        there <<= 1;
         if (i < tiles) {
-            const int key = k0 + (warp + kWarps * i) * kKeys + lane;
-            int pos = key;
-            bool in = key < k1;
-            if (LISTS) {
-                pos = in ? list[key] : 0;
-                in = in && pos >= 0 && pos < length && (pos >> a.shift) < a.M;
-            }
-            const int page = in ? table[pos >> a.shift] : -1;
-            in = in && page >= 0 && page < a.pages;
+            const bool in = page >= 0 && page < a.pages;
+            there |= in ? 1u : 0u;
             const int64_t head = in ? (int64_t)page * a.Hkv + h : 0;
             // row of the pool (below 2^31: the entry point checks); a key that is not there is not read
             const int row = in ? (int)((head << a.shift) + (pos & ((1 << a.shift) - 1))) : -1;
-            const uint32_t stage = ring + (i % Sh::kRing) * Sh::kStage;
-            const uint32_t scales = stage + 2 * Sh::kTile;
-            cp_async4(scales + lane * 8, a.ks + head, in ? 4u : 0u);
-            cp_async4(scales + lane * 8 + 4, a.vs + head, in ? 4u : 0u);
-            const uint32_t there = __ballot_sync(0xFFFFFFFFu, in);
-            if (lane == 0) asm volatile("st.shared.b32 [%0], %1;" ::"r"(scales + kKeys * 8), "r"(there) : "memory");
+            const uint32_t stage = ring + slot * Sh::kStage;
+            const uint32_t scales = stage + 2 * Sh::kTile + lane * 4;
+            cp_async4(scales, a.ks + head, in ? 4u : 0u);
+            cp_async4(scales + kKeys * 4, a.vs + head, in ? 4u : 0u);
+            if (LISTS) {
 #pragma unroll
-            for (int rr = 0; rr < kKeys; rr += 32 / C) {
-                const int r = rr + lane / C, ch = lane % C;
-                const int from = __shfl_sync(0xFFFFFFFFu, row, r);
-                const int64_t at = (int64_t)(from < 0 ? 0 : from) * D + ch * 16;
-                cp_async16(stage + k_at<D>(r, ch), a.k8 + at, from < 0 ? 0u : 16u);
-                cp_async16(stage + Sh::kTile + v_at<D>(r, ch), a.v8 + at, from < 0 ? 0u : 16u);
+                for (int rr = 0; rr < kKeys; rr += 32 / C) {
+                    const int r = rr + lane / C, ch = lane % C;
+                    const int from = __shfl_sync(0xFFFFFFFFu, row, r);
+                    const int64_t at = (int64_t)((from < 0 ? 0 : from) - lane / C) * D;
+                    cp_async16(stage + k_at<D>(r, ch), kl + at, from < 0 ? 0u : 16u);
+                    cp_async16(stage + Sh::kTile + v_at<D>(r, ch), vl + at, from < 0 ? 0u : 16u);
+                }
+            } else {
+                // 16 keys lie on one page: their rows follow one another, and the last ones may be past k1
+                const uint32_t live = __ballot_sync(0xFFFFFFFFu, in);
+                const int from = __shfl_sync(0xFFFFFFFFu, row, 0), from2 = __shfl_sync(0xFFFFFFFFu, row, 16);
+                const int64_t at = (int64_t)(from < 0 ? 0 : from) * D, at2 = (int64_t)(from2 < 0 ? 0 : from2) * D;
+                const uint8_t *kp = kl + at, *vp = vl + at, *kp2 = kl + at2 - 16 * D, *vp2 = vl + at2 - 16 * D;
+                const uint32_t kd = stage + k_at<D>(lane / C, lane % C);
+                if (live == 0xFFFFFFFFu) {
+#pragma unroll
+                    for (int rr = 0; rr < kKeys; rr += 32 / C) {
+                        cp_async16_all(kd + rr * D, (rr < 16 ? kp : kp2) + rr * D);
+                        cp_async16_all(stage + Sh::kTile + v_at<D>(rr + lane / C, lane % C), (rr < 16 ? vp : vp2) + rr * D);
+                    }
+                } else {
+#pragma unroll
+                    for (int rr = 0; rr < kKeys; rr += 32 / C) {
+                        const bool one = live >> (rr + lane / C) & 1u;
+                        cp_async16(kd + rr * D, one ? (rr < 16 ? kp : kp2) + rr * D : a.k8, one ? 16u : 0u);
+                        cp_async16(stage + Sh::kTile + v_at<D>(rr + lane / C, lane % C),
+                                   one ? (rr < 16 ? vp : vp2) + rr * D : a.v8, one ? 16u : 0u);
+                    }
+                }
             }
         }
+        if (++slot == Sh::kRing) slot = 0;
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
 #pragma unroll
     for (int i = 0; i < Sh::kRing - 1; ++i) copy(i);
 
-    // Q fragments: rows r0 + g and r0 + g + 8; k-step kk's four values of a lane are D's
+    // Q fragments: row r0 + g (and + 8); k-step kk's four values of a lane are D's
     // 16 (c + 4 (kk / 4)) + 4 (kk % 4) + 0..3
-    uint32_t qf[KS][4];
-    int limit[2];
-    float factor[2];
+    uint32_t qf[NT][KS][2];
+    uint64_t factor[NT];  // of rows r0 + 2c and 2c + 1 (and + 8), as the maxima and sums below
+    int limit[NT][2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < NT; ++u) {
         const int r = r0 + g + 8 * u;
         const int tok = r / a.G;
-        limit[u] = r >= nrows ? 0 : (LISTS ? k1 : length - a.Tq + tok + 1);
         const T* src = static_cast<const T*>(a.q) + b * a.q_b + tok * a.q_t + (h * (int64_t)a.G + r - tok * a.G) * a.q_h;
         uint2 raw[KS];
 #pragma unroll
         for (int kk = 0; kk < KS; ++kk)
             raw[kk] = r < nrows ? *reinterpret_cast<const uint2*>(src + 16 * (c + 4 * (kk >> 2)) + 4 * (kk & 3))
                                 : make_uint2(0, 0);
-        factor[u] = a.scale_log2;
+        float f = a.scale_log2;
         if constexpr (std::is_same<T, __nv_bfloat16>::value) {
             uint32_t top = 0;  // largest magnitude's bits, as a bf16
 #pragma unroll
@@ -189,90 +252,143 @@ __global__ void __launch_bounds__(kWarps * 32, 2) quant_rows_kernel(const QuantA
             top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
             const int e = (int)(top >> 7);  // biased exponent; zero, and infinities and NaN, stay as they are
             const int up = e == 0 || e == 255 ? 0 : min(8 - (e - 127), 100);
-            const float f = __uint_as_float((uint32_t)(up + 127) << 23);
-            factor[u] *= __uint_as_float((uint32_t)(127 - up) << 23);
+            const float by = __uint_as_float((uint32_t)(up + 127) << 23);
+            f *= __uint_as_float((uint32_t)(127 - up) << 23);
 #pragma unroll
             for (int kk = 0; kk < KS; ++kk) {
-                qf[kk][u] = pack_half(__uint_as_float(raw[kk].x << 16) * f, __uint_as_float(raw[kk].x & 0xFFFF0000u) * f);
-                qf[kk][u + 2] = pack_half(__uint_as_float(raw[kk].y << 16) * f, __uint_as_float(raw[kk].y & 0xFFFF0000u) * f);
+                qf[u][kk][0] = pack_half(__uint_as_float(raw[kk].x << 16) * by, __uint_as_float(raw[kk].x & 0xFFFF0000u) * by);
+                qf[u][kk][1] = pack_half(__uint_as_float(raw[kk].y << 16) * by, __uint_as_float(raw[kk].y & 0xFFFF0000u) * by);
             }
         } else {
 #pragma unroll
-            for (int kk = 0; kk < KS; ++kk) qf[kk][u] = raw[kk].x, qf[kk][u + 2] = raw[kk].y;
+            for (int kk = 0; kk < KS; ++kk) qf[u][kk][0] = raw[kk].x, qf[u][kk][1] = raw[kk].y;
+        }
+        factor[u] = pair(__shfl_sync(0xFFFFFFFFu, f, 8 * c), __shfl_sync(0xFFFFFFFFu, f, 8 * c + 4));
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int row = r0 + 8 * u + 2 * c + e;
+            limit[u][e] = row >= nrows ? 0 : length - a.Tq + row / a.G + 1;
         }
     }
-    float o[D / 8][4];
+    const int first_limit = length - a.Tq + r0 / a.G + 1;  // keys that the tile's first row sees
+    float o[NT][MT][4];  // O^T: columns (D / 8) g + 2 j (0, 1) and + 1 (2, 3) of rows 2c (0, 2) and 2c + 1 (1, 3)
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i)
+    for (int u = 0; u < NT; ++u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+        for (int j = 0; j < MT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[u][j][e] = 0.0f;
+    float m[NT][2];
+    uint64_t l[NT];
+#pragma unroll
+    for (int u = 0; u < NT; ++u) m[u][0] = m[u][1] = -INFINITY, l[u] = 0ull;
 
+    uint32_t read = 0;  // slot of tile i
     for (int i = 0; i < tiles; ++i) {
         copy(i + Sh::kRing - 1);
         asm volatile("cp.async.wait_group %0;" ::"n"(Sh::kRing - 1) : "memory");
-        __syncwarp();
-        const uint32_t ks = ring + (i % Sh::kRing) * Sh::kStage, vs = ks + Sh::kTile, scales = vs + Sh::kTile;
+        const uint32_t ks = ring + read * Sh::kStage, vs = ks + Sh::kTile, scales = vs + Sh::kTile;
+        if (++read == Sh::kRing) read = 0;
         const int key0 = k0 + (warp + kWarps * i) * kKeys;
-        const uint32_t there = lds32(scales + kKeys * 8);
-        float s[4][4];
+        // this lane's key: vs becomes its logarithm, -inf where there is no key, and its inverse
+        {
+            const bool in = there >> (Sh::kRing - 1) & 1u;
+            const float v = fmaxf(__uint_as_float(lds32(scales + kKeys * 4 + lane * 4)), 8.6736174e-19f);  // 2^-60
+            sts_f32(scales + kKeys * 4 + lane * 4, in ? lg2_approx(v) : -INFINITY);
+            sts_f32(scales + kKeys * 8 + lane * 4, in ? rcp_approx(v) : 0.0f);
+        }
+        __syncwarp();
+        // logits x[u][k]: key 8 k + g, rows 2c and 2c + 1, with the value scale in the exponent; -inf where there is no
+        // key, or none for the row
+        uint64_t x[NT][4];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
+        for (int t = 0; t < 2; ++t) {
+            float s[NT][4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[t][e] = 0.0f;
+            for (int u = 0; u < NT; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[u][e] = 0.0f;
 #pragma unroll
             for (int hh = 0; hh < KS / 4; ++hh) {
-                uint32_t w[4];
-                lds_words<4>(w, ks + k_at<D>(t * 8 + g, c + 4 * hh));
+                uint32_t w0[4], w1[4];
+                lds_words<4>(w0, ks + k_at<D>(t * 16 + g, c + 4 * hh));
+                lds_words<4>(w1, ks + k_at<D>(t * 16 + 8 + g, c + 4 * hh));
 #pragma unroll
-                for (int kk = 0; kk < 4; ++kk)
-                    mma_f16(s[t], qf[4 * hh + kk], halves_of<CODE>(w[kk], 0), halves_of<CODE>(w[kk], 1));
-            }
-        }
-        // logits with the value scale in the exponent; -inf where there is no key, or none for the row
-        float inv[4][2], mx[2] = {-INFINITY, -INFINITY};
+                for (int kk = 0; kk < 4; ++kk) {
+                    const uint32_t kf[4] = {halves_of<CODE>(w0[kk], 0), halves_of<CODE>(w1[kk], 0),
+                                            halves_of<CODE>(w0[kk], 1), halves_of<CODE>(w1[kk], 1)};
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int n = t * 8 + 2 * c + e;
-                const float2 sc = lds_f2(scales + n * 8);
-                const float v = fmaxf(sc.y, 8.6736174e-19f);  // 2^-60
-                const float lv = __log2f(v);
-                inv[t][e] = __frcp_rn(v);
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    float& x = s[t][2 * u + e];
-                    const bool seen = (there >> n & 1u) && (LISTS || key0 + n < limit[u]);
-                    x = seen ? fmaf(x * sc.x, factor[u], lv) : -INFINITY;
-                    mx[u] = fmaxf(mx[u], x);
+                    for (int u = 0; u < NT; ++u) mma_f16(s[u], kf, qf[u][4 * hh + kk][0], qf[u][4 * hh + kk][1]);
                 }
             }
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            mx[u] = fmaxf(mx[u], __shfl_xor_sync(0xFFFFFFFFu, mx[u], 1));
-            mx[u] = fmaxf(mx[u], __shfl_xor_sync(0xFFFFFFFFu, mx[u], 2));
-        }
-        if (__any_sync(0xFFFFFFFFu, mx[0] > m[0] || mx[1] > m[1])) {
+            for (int e = 0; e < 2; ++e) {
+                const uint32_t at = scales + (t * 16 + e * 8 + g) * 4;
+                const float key_scale = __uint_as_float(lds32(at)), lv = __uint_as_float(lds32(at + kKeys * 4));
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const float mn = fmaxf(m[u], mx[u]);
-                const float alpha = mn == -INFINITY ? 0.0f : ex2_approx(m[u] - mn);
-                m[u] = mn;
-                l[u] *= alpha;
-#pragma unroll
-                for (int d = 0; d < D / 8; ++d) o[d][2 * u] *= alpha, o[d][2 * u + 1] *= alpha;
+                for (int u = 0; u < NT; ++u)
+                    x[u][2 * t + e] = fma2(mul2(pair(s[u][2 * e], s[u][2 * e + 1]), pair(key_scale, key_scale)), factor[u],
+                                           pair(lv, lv));
             }
         }
-        uint32_t p[2][4];
+        if (!LISTS && key0 + kKeys > first_limit) {  // rows before the tile's last see less
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const float base = m[u] == -INFINITY ? 0.0f : m[u];
+            for (int u = 0; u < NT; ++u)
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const float p0 = ex2_approx((s[t][2 * u] - base) + kLift), p1 = ex2_approx((s[t][2 * u + 1] - base) + kLift);
-                l[u] = fmaf(p0, inv[t][0], fmaf(p1, inv[t][1], l[u]));
-                p[t >> 1][u + 2 * (t & 1)] = pack_half(p0, p1);
+                for (int k = 0; k < 4; ++k) {
+                    float x0, x1;
+                    unpair(x[u][k], x0, x1);
+                    const int key = key0 + 8 * k + g;
+                    x[u][k] = pair(key < limit[u][0] ? x0 : -INFINITY, key < limit[u][1] ? x1 : -INFINITY);
+                }
+        }
+        float mx[NT][2];
+        bool grow = false;
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+            float y[4][2];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) unpair(x[u][k], y[k][0], y[k][1]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float v = fmaxf(max3(y[0][e], y[1][e], y[2][e]), y[3][e]);
+#pragma unroll
+                for (int off = 4; off <= 16; off <<= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, off));
+                mx[u][e] = v;
+                grow = grow || v > m[u][e] + kGrow;  // m = -inf: any key
+            }
+        }
+        if (__any_sync(0xFFFFFFFFu, grow)) {
+#pragma unroll
+            for (int u = 0; u < NT; ++u) {
+                float alpha[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float mn = fmaxf(m[u][e], mx[u][e]);
+                    alpha[e] = mn == -INFINITY ? 0.0f : ex2_approx(m[u][e] - mn);
+                    m[u][e] = mn;
+                }
+                const uint64_t al = pair(alpha[0], alpha[1]);
+                l[u] = mul2(l[u], al);
+#pragma unroll
+                for (int j = 0; j < MT; ++j) {
+                    unpair(mul2(pair(o[u][j][0], o[u][j][1]), al), o[u][j][0], o[u][j][1]);
+                    unpair(mul2(pair(o[u][j][2], o[u][j][3]), al), o[u][j][2], o[u][j][3]);
+                }
+            }
+        }
+        uint32_t p[NT][4];  // P^T's fragments: row g, keys 8 k + 2c and + 1
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+            const uint64_t neg = pair(m[u][0] == -INFINITY ? 0.0f : -m[u][0], m[u][1] == -INFINITY ? 0.0f : -m[u][1]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float x0, x1;
+                unpair(add2(add2(x[u][k], neg), pair(kLift, kLift)), x0, x1);
+                const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+                const float inv = __uint_as_float(lds32(scales + kKeys * 8 + (8 * k + g) * 4));
+                l[u] = fma2(pair(p0, p1), pair(inv, inv), l[u]);
+                p[u][k] = transposed(pack_half(p0, p1));
             }
         }
 #pragma unroll
@@ -281,47 +397,51 @@ __global__ void __launch_bounds__(kWarps * 32, 2) quant_rows_kernel(const QuantA
             constexpr int NW = D / 32;  // words of a key a lane takes: D's (D / 8) g ..
             uint32_t w[4][NW];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const int r = 16 * kk + 2 * c + (x & 1) + 8 * (x >> 1);
+            for (int i = 0; i < 4; ++i) {
+                const int r = 16 * kk + 2 * c + (i & 1) + 8 * (i >> 1);
                 if constexpr (D == 128)
-                    lds_words<NW>(w[x], vs + v_at<D>(r, g));
+                    lds_words<NW>(w[i], vs + v_at<D>(r, g));
                 else
-                    lds_words<NW>(w[x], vs + v_at<D>(r, g >> 1) + (g & 1) * 8);
+                    lds_words<NW>(w[i], vs + v_at<D>(r, g >> 1) + (g & 1) * 8);
             }
 #pragma unroll
-            for (int j = 0; j < NW; ++j) {
-                const uint32_t lo0 = __byte_perm(w[0][j], w[1][j], 0x5140), lo1 = __byte_perm(w[0][j], w[1][j], 0x7362);
-                const uint32_t hi0 = __byte_perm(w[2][j], w[3][j], 0x5140), hi1 = __byte_perm(w[2][j], w[3][j], 0x7362);
-                mma_f16(o[4 * j], p[kk], halves_of<CODE>(lo0, 0), halves_of<CODE>(hi0, 0));
-                mma_f16(o[4 * j + 1], p[kk], halves_of<CODE>(lo0, 1), halves_of<CODE>(hi0, 1));
-                mma_f16(o[4 * j + 2], p[kk], halves_of<CODE>(lo1, 0), halves_of<CODE>(hi1, 0));
-                mma_f16(o[4 * j + 3], p[kk], halves_of<CODE>(lo1, 1), halves_of<CODE>(hi1, 1));
+            for (int j = 0; j < 2 * NW; ++j) {
+                const uint32_t sel = j & 1 ? 0x7362 : 0x5140;
+                const uint32_t lo = __byte_perm(w[0][j >> 1], w[1][j >> 1], sel), hi = __byte_perm(w[2][j >> 1], w[3][j >> 1], sel);
+                const uint32_t vf[4] = {halves_of<CODE>(lo, 0), halves_of<CODE>(lo, 1), halves_of<CODE>(hi, 0),
+                                        halves_of<CODE>(hi, 1)};
+#pragma unroll
+                for (int u = 0; u < NT; ++u) mma_f16(o[u][j], vf, p[u][2 * kk], p[u][2 * kk + 1]);
             }
         }
         __syncwarp();  // the tile's slot is refilled next
     }
     cp_async_wait_all();
+    float sum[NT][2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        l[u] += __shfl_xor_sync(0xFFFFFFFFu, l[u], 1);
-        l[u] += __shfl_xor_sync(0xFFFFFFFFu, l[u], 2);
+    for (int u = 0; u < NT; ++u) {
+        unpair(l[u], sum[u][0], sum[u][1]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int off = 4; off <= 16; off <<= 1) sum[u][e] += __shfl_xor_sync(0xFFFFFFFFu, sum[u][e], off);
     }
     // join the warps: each leaves its sums in its own ring, (m, l) after the rings
     __syncwarp();
     float* so = reinterpret_cast<float*>(smem + warp * Sh::kWarpBytes);
     float2* sml = reinterpret_cast<float2*>(smem + kWarps * Sh::kWarpBytes);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        // o[i]'s columns 2c and 2c + 1 are D's (D / 8) 2c + i and (D / 8)(2c + 1) + i
-        float* line = so + (g + 8 * u) * D + (D / 8) * 2 * c;
+    for (int u = 0; u < NT; ++u)
 #pragma unroll
-        for (int i = 0; i < D / 8; i += 4) {
-            *reinterpret_cast<float4*>(line + i) = make_float4(o[i][2 * u], o[i + 1][2 * u], o[i + 2][2 * u], o[i + 3][2 * u]);
-            *reinterpret_cast<float4*>(line + D / 8 + i) =
-                make_float4(o[i][2 * u + 1], o[i + 1][2 * u + 1], o[i + 2][2 * u + 1], o[i + 3][2 * u + 1]);
+        for (int e = 0; e < 2; ++e) {
+            const int r = 8 * u + 2 * c + e;
+            float* line = so + r * D + (D / 8) * g;
+#pragma unroll
+            for (int j = 0; j < MT; j += 2)
+                *reinterpret_cast<float4*>(line + 2 * j) =
+                    make_float4(o[u][j][e], o[u][j][2 + e], o[u][j + 1][e], o[u][j + 1][2 + e]);
+            if (g == 0) sml[warp * kRows + r] = make_float2(m[u][e], sum[u][e]);
         }
-        if (c == 0) sml[warp * kRows + g + 8 * u] = make_float2(m[u], l[u]);
-    }
     __syncthreads();
     for (int i = threadIdx.x; i < live * (D / 4); i += kWarps * 32) {
         const int r = i / (D / 4), col = i % (D / 4) * 4;
@@ -412,16 +532,19 @@ __global__ void __launch_bounds__(128) quant_join_kernel(const QuantArgs a) {
         a.lse[rid] = total == 0.0f ? -INFINITY : (top + log2f(total)) * 0.69314718055994531f;
 }
 
-template <typename T, int CODE, int D, bool LISTS>
+template <typename T, int CODE, int D, bool LISTS, int NT>
 int launch(const QuantArgs& a, int row_tiles, unsigned grid, cudaStream_t stream) {
-    if (!allow_kernel<quant_rows_kernel<T, CODE, D, LISTS>>(QuantShape<D>::kSmem)) return LSA_ERR_CUDA;
-    return launch_after(quant_rows_kernel<T, CODE, D, LISTS>, dim3(grid), kWarps * 32, QuantShape<D>::kSmem, stream, a,
-                        row_tiles);
+    constexpr int smem = QuantShape<D, NT>::kSmem;
+    if (!allow_kernel<quant_rows_kernel<T, CODE, D, LISTS, NT>>(smem)) return LSA_ERR_CUDA;
+    return launch_after(quant_rows_kernel<T, CODE, D, LISTS, NT>, dim3(grid), kWarps * 32, smem, stream, a, row_tiles);
 }
 template <typename T, int CODE, int D>
 int launch(const QuantArgs& a, int row_tiles, unsigned grid, cudaStream_t stream) {
-    return a.lists ? launch<T, CODE, D, true>(a, row_tiles, grid, stream)
-                   : launch<T, CODE, D, false>(a, row_tiles, grid, stream);
+    if (a.Tq * a.G <= 8)
+        return a.lists ? launch<T, CODE, D, true, 1>(a, row_tiles, grid, stream)
+                       : launch<T, CODE, D, false, 1>(a, row_tiles, grid, stream);
+    return a.lists ? launch<T, CODE, D, true, 2>(a, row_tiles, grid, stream)
+                   : launch<T, CODE, D, false, 2>(a, row_tiles, grid, stream);
 }
 template <typename T> int launch(const QuantArgs& a, int code, int D, int row_tiles, unsigned grid, cudaStream_t stream) {
     if (code == kE4M3)
@@ -432,7 +555,7 @@ template <typename T> int launch(const QuantArgs& a, int code, int D, int row_ti
 }  // namespace
 
 int launch_quant_rows(const QuantArgs& a, int dtype, int code, int D, cudaStream_t stream) {
-    const int row_tiles = (a.Tq * a.G + kRows - 1) / kRows;
+    const int row_tiles = (a.Tq * a.G + 15) / 16;
     const int64_t items = (int64_t)a.B * a.Hkv * row_tiles * a.parts;
     if (items > INT32_MAX) return LSA_ERR_SIZE;
     return dtype == kBF16 ? launch<__nv_bfloat16>(a, code, D, row_tiles, (unsigned)items, stream)
