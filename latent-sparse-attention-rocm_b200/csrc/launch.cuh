@@ -9,19 +9,28 @@ namespace lsa {
 
 // Launch that may start while the kernel before it drains (programmatic dependent launch): the
 // kernel waits (griddepcontrol.wait) before it touches what an earlier kernel writes.
+// launch_clusters: the same in clusters of `cluster` CTAs along x (1: none).
 template <typename K, typename... A>
-int launch_after(K kern, dim3 grid, unsigned threads, size_t smem, cudaStream_t stream, const A&... args) {
-    cudaLaunchAttribute attr[1];
+int launch_clusters(K kern, dim3 grid, unsigned threads, size_t smem, cudaStream_t stream, unsigned cluster,
+                    const A&... args) {
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess ? LSA_OK : LSA_ERR_CUDA;
+}
+template <typename K, typename... A>
+int launch_after(K kern, dim3 grid, unsigned threads, size_t smem, cudaStream_t stream, const A&... args) {
+    return launch_clusters(kern, grid, threads, smem, stream, 1, args...);
 }
 
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

@@ -41,6 +41,7 @@ struct QuantArgs {
     float* lse;                   // [rows] natural, or null
     int B, Tq, Hq, Hkv, G;
     int parts;
+    bool cluster;                 // the parts are a cluster's CTAs, which join them (few-row kernel)
     int64_t rows;                 // B * Tq * Hq
     float scale_log2;             // scale * log2(e)
 };

@@ -34,7 +34,7 @@ template <int D, int NT> struct QuantShape {
     static constexpr int kTile = kKeys * D;            // K or V bytes of a tile
     static constexpr int kStage = 2 * kTile + kKeys * 12;  // + ks, vs (then its logarithm) and 1 / vs of every key
     static constexpr int kWarpBytes = (kRing * kStage + 127) / 128 * 128;
-    static constexpr int kSmem = kWarps * kWarpBytes + kWarps * kRows * 2 * 4;
+    static constexpr int kSmem = kWarps * kWarpBytes + (kWarps + 1) * kRows * 2 * 4;
     static_assert(kWarpBytes >= kRows * D * 4, "the join reuses a warp's ring");
     static_assert(kStage % 16 == 0, "16-byte copies");
 };
@@ -61,6 +61,32 @@ __device__ __forceinline__ uint64_t lds64(uint32_t addr) {
     uint64_t r;
     asm volatile("ld.shared.b64 %0, [%1];" : "=l"(r) : "r"(addr) : "memory");
     return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// From CTA `rank` of the cluster's shared memory, at the address that this CTA has for the same thing.
+__device__ __forceinline__ uint32_t peer(uint32_t addr, int rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float2 peer_f2(uint32_t addr, int rank) {
+    float2 r;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(r.x), "=f"(r.y) : "r"(peer(addr, rank)) : "memory");
+    return r;
+}
+__device__ __forceinline__ float4 peer_f4(uint32_t addr, int rank) {
+    float4 r;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(r.x), "=f"(r.y), "=f"(r.z), "=f"(r.w)
+                 : "r"(peer(addr, rank))
+                 : "memory");
+    return r;
+}
+template <typename T> __device__ __forceinline__ void store4(T* dst, const float4& x) {
+    const T y[4] = {from_f32<T>(x.x), from_f32<T>(x.y), from_f32<T>(x.z), from_f32<T>(x.w)};
+    *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(y);
 }
 // Block of 8 x 8 halves, lane (g, c) holding [g][2c], [g][2c + 1], transposed.
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
@@ -147,9 +173,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) quant_rows_kerne
     }
     int k0, k1;
     {
-        const int64_t units = (keys + kWarps * kKeys - 1) / (kWarps * kKeys);
+        // a list is split by its width: its entries are asked for beside its count
+        const int64_t units = ((LISTS ? a.W : keys) + kWarps * kKeys - 1) / (kWarps * kKeys);
         const int64_t u0 = units * split / a.parts * (kWarps * kKeys), u1 = units * (split + 1) / a.parts * (kWarps * kKeys);
-        k0 = (int)(u0 < keys ? u0 : keys), k1 = (int)(u1 < keys ? u1 : keys);
+        const int all = LISTS ? a.W : keys;
+        k0 = (int)(u0 < all ? u0 : all), k1 = (int)(u1 < all ? u1 : all);
     }
     const int32_t* table = a.table + trow * a.table_ld;
     const int32_t* list = LISTS ? a.lists + (int64_t)b * a.W : nullptr;
@@ -161,7 +189,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) quant_rows_kerne
     auto position = [&](int i) {
         const int key = k0 + (warp + kWarps * i) * kKeys + lane;
         const bool in = i < tiles && key < k1;
-        return !in ? -1 : (LISTS ? list[key] : key);
+        const int pos = !in ? -1 : (LISTS ? list[key] : key);
+        return LISTS && key >= keys ? -1 : pos;
     };
     auto page_of = [&](int pos) {
         return pos >= 0 && pos < length && (pos >> a.shift) < a.M ? table[pos >> a.shift] : -1;
@@ -443,6 +472,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) quant_rows_kerne
             if (g == 0) sml[warp * kRows + r] = make_float2(m[u][e], sum[u][e]);
         }
     __syncthreads();
+    auto row_id = [&](int r) {
+        const int tok = (r0 + r) / a.G;
+        return ((int64_t)b * a.Tq + tok) * a.Hq + (int64_t)h * a.G + (r0 + r - tok * a.G);
+    };
+    float2* joined = sml + kWarps * kRows;  // the CTA's (maximum, sum) of a row
     for (int i = threadIdx.x; i < live * (D / 4); i += kWarps * 32) {
         const int r = i / (D / 4), col = i % (D / 4) * 4;
         float top = -INFINITY;
@@ -458,15 +492,17 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) quant_rows_kerne
             total = fmaf(f, ml.y, total);
             x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w);
         }
+        if (a.cluster) {  // left where warp 0's were: no other thread reads these
+            *reinterpret_cast<float4*>(smem + (r * D + col) * 4) = x;
+            if (col == 0) joined[r] = make_float2(top, total);
+            continue;
+        }
         const float norm = total == 0.0f ? 0.0f : 1.0f / total;
         x.x *= norm, x.y *= norm, x.z *= norm, x.w *= norm;
         const float lse = total == 0.0f ? -INFINITY : top + (log2f(total) - kLift);
-        const int tok = (r0 + r) / a.G;
-        const int64_t rid = ((int64_t)b * a.Tq + tok) * a.Hq + (int64_t)h * a.G + (r0 + r - tok * a.G);
+        const int64_t rid = row_id(r);
         if (a.parts == 1) {
-            T* dst = static_cast<T*>(a.out) + rid * D + col;
-            const T y[4] = {from_f32<T>(x.x), from_f32<T>(x.y), from_f32<T>(x.z), from_f32<T>(x.w)};
-            *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(y);
+            store4<T>(static_cast<T*>(a.out) + rid * D + col, x);
             if (col == 0 && a.lse) a.lse[rid] = lse * 0.69314718055994531f;
         } else {
             const int64_t at = (int64_t)split * a.rows + rid;
@@ -474,13 +510,40 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) quant_rows_kerne
             if (col == 0) a.part_lse[at] = lse;
         }
     }
+    if (!a.cluster) return;
+    __syncwarp();
+    // A cluster holds all parts of its rows: they join through its CTAs' shared memory, a part of the columns each.
+    cluster_sync();
+    const uint32_t base = smem_u32(smem), stats = smem_u32(joined);
+    for (int i = split * kWarps * 32 + threadIdx.x; i < live * (D / 4); i += a.parts * kWarps * 32) {
+        const int r = i / (D / 4), col = i % (D / 4) * 4;
+        float top = -INFINITY, total = 0.0f;
+        float4 x = make_float4(0, 0, 0, 0);
+        for (int p = 0; p < a.parts; ++p) top = fmaxf(top, peer_f2(stats + r * 8, p).x);
+#pragma unroll 4
+        for (int p = 0; p < a.parts; ++p) {
+            const float2 ml = peer_f2(stats + r * 8, p);
+            const float4 y = peer_f4(base + (r * D + col) * 4, p);
+            const float f = ml.y == 0.0f ? 0.0f : exp2f(ml.x - top);
+            total = fmaf(f, ml.y, total);
+            x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w);
+        }
+        const float norm = total == 0.0f ? 0.0f : 1.0f / total;
+        const int64_t rid = row_id(r);
+        store4<T>(static_cast<T*>(a.out) + rid * D + col, make_float4(x.x * norm, x.y * norm, x.z * norm, x.w * norm));
+        if (col == 0 && a.lse)
+            a.lse[rid] = total == 0.0f ? -INFINITY : (top + (log2f(total) - kLift)) * 0.69314718055994531f;
+    }
+    __syncwarp();
+    cluster_sync();  // no CTA leaves while another reads its memory
 }
 
-// The parts of a row joined: a CTA a row, a warp every fourth part.
+// The parts of a row joined: a CTA a row, a warp every eighth part. Every part's values are asked for before the
+// weights are known, so a row is one round of memory.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) quant_join_kernel(const QuantArgs a) {
-    constexpr int V = D / 32;
-    __shared__ float so[4][D];
+__global__ void __launch_bounds__(256) quant_join_kernel(const QuantArgs a) {
+    constexpr int V = D / 32, NW = 8, N = kMaxQuantParts / NW;
+    __shared__ float so[NW][D];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     grid_wait();
     grid_trigger();
@@ -490,42 +553,52 @@ __global__ void __launch_bounds__(128) quant_join_kernel(const QuantArgs a) {
     for (int i = 0; i < 3; ++i) {
         const int part = i * 32 + lane;
         lse[i] = part < a.parts ? a.part_lse[part * a.rows + rid] : -INFINITY;
-        top = fmaxf(top, lse[i]);
+    }
+    float y[N][V];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int part = warp + NW * i;
+        const float* src = a.part_o + (part * a.rows + rid) * D + lane * V;
+#pragma unroll
+        for (int e = 0; e < V; ++e) y[i][e] = 0.0f;
+        if (part < a.parts) {
+            if constexpr (V == 4) {
+                const float4 z = *reinterpret_cast<const float4*>(src);
+                y[i][0] = z.x, y[i][1] = z.y, y[i][2] = z.z, y[i][3] = z.w;
+            } else {
+                const float2 z = *reinterpret_cast<const float2*>(src);
+                y[i][0] = z.x, y[i][1] = z.y;
+            }
+        }
     }
 #pragma unroll
+    for (int i = 0; i < 3; ++i) top = fmaxf(top, lse[i]);
+#pragma unroll
     for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
-    float total = 0.0f, o[V];
+    float total = 0.0f, f[3], o[V];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {  // NaN passes on
+        f[i] = lse[i] == -INFINITY ? 0.0f : exp2f(lse[i] - (top == -INFINITY ? 0.0f : top));
+        total += f[i];
+    }
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, off);
 #pragma unroll
     for (int e = 0; e < V; ++e) o[e] = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 3; ++i) {
-        // NaN passes on; a part without a key is not read
-        const float f = lse[i] == -INFINITY ? 0.0f : exp2f(lse[i] - (top == -INFINITY ? 0.0f : top));
-        float w = f;
+    for (int i = 0; i < N; ++i) {
+        const float fi = __shfl_sync(0xFFFFFFFFu, f[i / 4], (warp + NW * i) & 31);
 #pragma unroll
-        for (int off = 16; off >= 1; off >>= 1) w += __shfl_xor_sync(0xFFFFFFFFu, w, off);
-        total += w;
-        const int n = a.parts - i * 32 < 32 ? a.parts - i * 32 : 32;
-#pragma unroll 4
-        for (int j = warp; j < n; j += 4) {
-            const float fj = __shfl_sync(0xFFFFFFFFu, f, j);
-            if (fj == 0.0f) continue;
-            const float* src = a.part_o + ((int64_t)(i * 32 + j) * a.rows + rid) * D + lane * V;
-            if constexpr (V == 4) {
-                const float4 y = *reinterpret_cast<const float4*>(src);
-                o[0] = fmaf(fj, y.x, o[0]), o[1] = fmaf(fj, y.y, o[1]), o[2] = fmaf(fj, y.z, o[2]), o[3] = fmaf(fj, y.w, o[3]);
-            } else {
-                const float2 y = *reinterpret_cast<const float2*>(src);
-                o[0] = fmaf(fj, y.x, o[0]), o[1] = fmaf(fj, y.y, o[1]);
-            }
-        }
+        for (int e = 0; e < V; ++e) o[e] = fmaf(fi, y[i][e], o[e]);
     }
 #pragma unroll
     for (int e = 0; e < V; ++e) so[warp][lane * V + e] = o[e];
     __syncthreads();
     const int col = threadIdx.x;
     if (col < D) {
-        const float x = (so[0][col] + so[1][col]) + (so[2][col] + so[3][col]);
+        float x = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) x += so[w][col];
         static_cast<T*>(a.out)[rid * D + col] = from_f32<T>(total == 0.0f ? 0.0f : x / total);
     }
     if (threadIdx.x == 0 && a.lse)
@@ -535,8 +608,9 @@ __global__ void __launch_bounds__(128) quant_join_kernel(const QuantArgs a) {
 template <typename T, int CODE, int D, bool LISTS, int NT>
 int launch(const QuantArgs& a, int row_tiles, unsigned grid, cudaStream_t stream) {
     constexpr int smem = QuantShape<D, NT>::kSmem;
-    if (!allow_kernel<quant_rows_kernel<T, CODE, D, LISTS, NT>>(smem)) return LSA_ERR_CUDA;
-    return launch_after(quant_rows_kernel<T, CODE, D, LISTS, NT>, dim3(grid), kWarps * 32, smem, stream, a, row_tiles);
+    if (!allow_kernel<quant_rows_kernel<T, CODE, D, LISTS, NT>>(smem, true)) return LSA_ERR_CUDA;
+    return launch_clusters(quant_rows_kernel<T, CODE, D, LISTS, NT>, dim3(grid), kWarps * 32, smem, stream,
+                           a.cluster ? a.parts : 1, a, row_tiles);
 }
 template <typename T, int CODE, int D>
 int launch(const QuantArgs& a, int row_tiles, unsigned grid, cudaStream_t stream) {
@@ -566,10 +640,10 @@ int launch_quant_join(const QuantArgs& a, int dtype, int D, cudaStream_t stream)
     if (a.rows > INT32_MAX) return LSA_ERR_SIZE;
     const dim3 grid((unsigned)a.rows);
     if (dtype == kBF16)
-        return D == 128 ? launch_after(quant_join_kernel<__nv_bfloat16, 128>, grid, 128, 0, stream, a)
-                        : launch_after(quant_join_kernel<__nv_bfloat16, 64>, grid, 128, 0, stream, a);
-    return D == 128 ? launch_after(quant_join_kernel<__half, 128>, grid, 128, 0, stream, a)
-                    : launch_after(quant_join_kernel<__half, 64>, grid, 128, 0, stream, a);
+        return D == 128 ? launch_after(quant_join_kernel<__nv_bfloat16, 128>, grid, 256, 0, stream, a)
+                        : launch_after(quant_join_kernel<__nv_bfloat16, 64>, grid, 256, 0, stream, a);
+    return D == 128 ? launch_after(quant_join_kernel<__half, 128>, grid, 256, 0, stream, a)
+                    : launch_after(quant_join_kernel<__half, 64>, grid, 256, 0, stream, a);
 }
 
 }  // namespace lsa
