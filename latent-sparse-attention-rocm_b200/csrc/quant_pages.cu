@@ -25,10 +25,24 @@ struct AppendArgs {
 
 constexpr int kSmallRows = 4;  // new tokens of a sequence that one warp takes
 
-template <typename T, int CODE, int D, int NT>
+// Eight values as they lie in memory: half the registers of fp32, so more CTAs an SM have their rows in flight.
+template <typename T> struct Raw {
+    uint4 u[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = reinterpret_cast<const uint4*>(p)[i];
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void floats(float (&x)[8]) const { load8<T>(reinterpret_cast<const T*>(u), x); }
+};
+
+// NT: threads of a (sequence, page, head, K or V); PASSES: of its rows.
+template <typename T, int CODE, int D, int NT, int PASSES>
 __global__ void __launch_bounds__(NT == 32 ? 128 : NT) append_kernel(const AppendArgs a) {
-    constexpr int L = D / 8, RP = NT / L;                      // lanes of a row, rows of a pass
-    constexpr int PASSES = NT == 32 ? (kSmallRows + RP - 1) / RP : 128 / RP;
+    constexpr int L = D / 8, RP = NT / L;  // lanes of a row, rows of a pass
     __shared__ float warp_top[NT / 32];
     const int tid = NT == 32 ? threadIdx.x & 31 : threadIdx.x;
     grid_wait();
@@ -67,17 +81,20 @@ __global__ void __launch_bounds__(NT == 32 ? 128 : NT) append_kernel(const Appen
 
     float was = 0.0f;
     if (kept > 0) was = *scale;
-    float x[PASSES][8], top = 0.0f;
+    Raw<T> raw[PASSES];
+    float top = 0.0f;
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[i][e] = 0.0f;
-        if (i * RP + r < n) load8<T>(src + (int64_t)i * RP * ld, x[i]);
+        raw[i].zero();
+        if (i * RP + r < n) raw[i].load(src + (int64_t)i * RP * ld);
     }
 #pragma unroll
-    for (int i = 0; i < PASSES; ++i)
+    for (int i = 0; i < PASSES; ++i) {
+        float x[8];
+        raw[i].floats(x);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[i][e]));
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
+    }
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
     was = __shfl_sync(0xFFFFFFFFu, was, 0);  // every lane's read is behind it, before the write below
@@ -96,10 +113,17 @@ __global__ void __launch_bounds__(NT == 32 ? 128 : NT) append_kernel(const Appen
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
         if (i * RP + r >= n) continue;
+        float x[8];
+        raw[i].floats(x);
+        if (power) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[i][e] = power ? x[i][e] * inv : __fdiv_rn(x[i][e], now);
+            for (int e = 0; e < 8; ++e) x[e] *= inv;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = __fdiv_rn(x[e], now);
+        }
         *reinterpret_cast<uint2*>(dst + (kept + i * RP + r) * D + c) =
-            make_uint2(codes_of<CODE>(x[i][0], x[i][1], x[i][2], x[i][3]), codes_of<CODE>(x[i][4], x[i][5], x[i][6], x[i][7]));
+            make_uint2(codes_of<CODE>(x[0], x[1], x[2], x[3]), codes_of<CODE>(x[4], x[5], x[6], x[7]));
     }
     if (kept > 0 && now != was) {  // now is a power of two
         for (int row = r; row < kept; row += RP) {
@@ -122,10 +146,17 @@ template <typename T, int CODE, int D> int launch(const AppendArgs& a, cudaStrea
     if (a.Tq <= kSmallRows) {
         const int64_t blocks = (a.units + 3) / 4;
         if (blocks > INT32_MAX) return LSA_ERR_SIZE;
-        return launch_after(append_kernel<T, CODE, D, 32>, dim3((unsigned)blocks), 128, 0, stream, a);
+        return launch_after(append_kernel<T, CODE, D, 32, kSmallRows * (D / 8) / 32>, dim3((unsigned)blocks), 128, 0, stream, a);
     }
     if (a.units > INT32_MAX) return LSA_ERR_SIZE;
-    return launch_after(append_kernel<T, CODE, D, 256>, dim3((unsigned)a.units), 256, 0, stream, a);
+    constexpr int NT = 2 * D;  // 16 rows a pass
+    const dim3 grid((unsigned)a.units);
+    switch (a.shift) {
+        case 4: return launch_after(append_kernel<T, CODE, D, NT, 1>, grid, NT, 0, stream, a);
+        case 5: return launch_after(append_kernel<T, CODE, D, NT, 2>, grid, NT, 0, stream, a);
+        case 6: return launch_after(append_kernel<T, CODE, D, NT, 4>, grid, NT, 0, stream, a);
+        default: return launch_after(append_kernel<T, CODE, D, NT, 8>, grid, NT, 0, stream, a);
+    }
 }
 template <typename T> int launch(const AppendArgs& a, int code, int64_t D, cudaStream_t stream) {
     if (code == kE4M3) return D == 64 ? launch<T, kE4M3, 64>(a, stream) : launch<T, kE4M3, 128>(a, stream);

@@ -110,11 +110,6 @@ __device__ __forceinline__ float rcp_approx(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 template <int N> __device__ __forceinline__ void lds_words(uint32_t (&r)[N], uint32_t addr) {
     if constexpr (N == 4)
         asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"

@@ -7,9 +7,10 @@
 // fp32, rounded once. The angle in turns is p * (f / 2 pi) in fp64, reduced there to half a turn either way:
 // what is left of a position's 2^-53 is the angle's error, whatever the position.
 //
-// A warp holds a token's heads one after another, D / 8 lanes a head (8 values a lane), and its lanes' angles
-// once for all of them; half-layout partners are a lane apart and change values by shuffle.
-#include "launch.cuh"
+// A warp holds a token's heads one after another, D / 8 lanes a head, and its lanes' angles once for all of them. A
+// lane has four values of either half and so both of a pair, in the half layout as in the interleaved one (two
+// 8-byte loads where one of 16 would want its partner's values by shuffle).
+#include "pairs.cuh"
 
 namespace lsa {
 namespace {
@@ -31,38 +32,54 @@ struct RotateArgs {
     float amplitude, eps;
 };
 
+// Eight values of a lane, four at either of two places, as they lie in memory.
 template <typename T> struct Raw8 {
-    uint4 u;
-    __device__ __forceinline__ void load(const T* p) { u = *reinterpret_cast<const uint4*>(p); }
-    __device__ __forceinline__ void floats(float (&x)[8]) const { load8<T>(reinterpret_cast<const T*>(&u), x); }
+    uint2 u[2];
+    __device__ __forceinline__ void load(const T* p, int off) {
+        u[0] = *reinterpret_cast<const uint2*>(p);
+        u[1] = *reinterpret_cast<const uint2*>(p + off);
+    }
+    __device__ __forceinline__ void floats(float (&x)[8]) const { load8<T>(reinterpret_cast<const T*>(u), x); }
 };
 template <> struct Raw8<float> {
     uint4 u[2];
-    __device__ __forceinline__ void load(const float* p) {
-        u[0] = reinterpret_cast<const uint4*>(p)[0];
-        u[1] = reinterpret_cast<const uint4*>(p)[1];
+    __device__ __forceinline__ void load(const float* p, int off) {
+        u[0] = *reinterpret_cast<const uint4*>(p);
+        u[1] = *reinterpret_cast<const uint4*>(p + off);
     }
     __device__ __forceinline__ void floats(float (&x)[8]) const { load8<float>(reinterpret_cast<const float*>(u), x); }
 };
 
-template <typename T> __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
-    uint4 u;
-    T* h = reinterpret_cast<T*>(&u);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) h[e] = from_f32<T>(x[e]);
-    *reinterpret_cast<uint4*>(p) = u;
+__device__ __forceinline__ uint32_t two(float a, float b, __nv_bfloat16*) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
 }
-template <> __device__ __forceinline__ void store8<float>(float* p, const float (&x)[8]) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+__device__ __forceinline__ uint32_t two(float a, float b, __half*) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T> __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(two(a, b, (T*)nullptr), two(c, d, (T*)nullptr));
+}
+template <> __device__ __forceinline__ void store4<float>(float* p, float a, float b, float c, float d) {
+    *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
+}
+
+// Sine and cosine of a turn's fraction, |turn| <= 1/2. For values that are rounded to 16 bits the special-function
+// unit's (2^-21 off at most on +-pi, and 2^-22 for the argument, against 2^-12 and 2^-9 of the rounding).
+template <typename T> __device__ __forceinline__ void sin_cos(float turn, float* s, float* c) {
+    const float x = turn * 6.283185307179586f;
+    *s = __sinf(x), *c = __cosf(x);
+}
+template <> __device__ __forceinline__ void sin_cos<float>(float turn, float* s, float* c) {
+    sincospif(turn + turn, s, c);
 }
 
 template <typename T, int D, bool INTER>
 __global__ void __launch_bounds__(kWarps * 32) norm_rotate_kernel(const RotateArgs a) {
-    constexpr int L = D / 8;    // lanes of a head
-    constexpr int N = 32 / L;   // heads of a pass
-    constexpr int A = INTER ? 4 : 8;
-    const int lane = threadIdx.x & 31, j = lane % L;
+    constexpr int L = D / 8;  // lanes of a head
+    constexpr int N = 32 / L; // heads of a pass
+    const int lane = threadIdx.x & 31, j = lane % L, own = lane / L;
     const int64_t unit = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
     const int64_t token = unit / a.sections;
     const int section = (int)(unit - token * a.sections);
@@ -70,99 +87,99 @@ __global__ void __launch_bounds__(kWarps * 32) norm_rotate_kernel(const RotateAr
     grid_trigger();
     if (token >= a.tokens) return;
     const int64_t b = token / a.T, t = token - b * a.T;
-    const int heads = a.Hq + a.Hkv;
-    const int h0 = (int)((int64_t)heads * section / a.sections), h1 = (int)((int64_t)heads * (section + 1) / a.sections);
+    // passes over q's heads, then k's; this warp's
+    const int q_passes = (a.Hq + N - 1) / N, passes = q_passes + (a.Hkv + N - 1) / N;
+    const int p0 = passes * section / a.sections, p1 = passes * (section + 1) / a.sections;
 
-    const T* qrow = static_cast<const T*>(a.q) + b * a.q_b + t * a.q_t + j * 8;
-    const T* krow = static_cast<const T*>(a.k) + b * a.k_b + t * a.k_t + j * 8;
-    auto src = [&](int h) { return h < a.Hq ? qrow + h * a.q_h : krow + (h - a.Hq) * a.k_h; };
+    // the lane's values: four from `at0` on, four `step` further
+    const bool turns = 8 * j < a.R;
+    const int at0 = INTER || !turns ? 8 * j : 4 * j, step = INTER || !turns ? 4 : a.R / 2;
+    const T* qrow = static_cast<const T*>(a.q) + b * a.q_b + t * a.q_t + own * a.q_h + at0;
+    const T* krow = static_cast<const T*>(a.k) + b * a.k_b + t * a.k_t + own * a.k_h + at0;
+    T* qdst = static_cast<T*>(a.q_out) + (token * a.Hq + own) * D + at0;
+    T* kdst = static_cast<T*>(a.k_out) + (token * a.Hkv + own) * D + at0;
+    auto is_q = [&](int p) { return p < q_passes; };
+    auto live = [&](int p) { return is_q(p) ? p * N + own < a.Hq : (p - q_passes) * N + own < a.Hkv; };
+    auto load = [&](Raw8<T>& raw, int p) {
+        if (p < p1 && live(p)) raw.load(is_q(p) ? qrow + p * N * a.q_h : krow + (p - q_passes) * N * a.k_h, step);
+    };
     Raw8<T> raw[kAhead];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-        const int h = h0 + i * N + lane / L;
-        if (h < h1) raw[i].load(src(h));
-    }
+    for (int i = 0; i < kAhead; ++i) load(raw[i], p0 + i);
 
     const int64_t at = b * a.pos_b + t * a.pos_t;
-    const double p = a.wide_positions ? (double)static_cast<const int64_t*>(a.positions)[at]
-                                      : (double)static_cast<const int32_t*>(a.positions)[at];
-    // half layout: a lane's 8 values lie in one half (R is a multiple of 16)
-    const int half = a.R / 2;
-    const bool turns = 8 * j < a.R, second = !INTER && 8 * j >= half;
-    const int partner = INTER || !turns ? lane : (second ? lane - half / 8 : lane + half / 8);
-    float cs[A], sn[A];
+    const double position = a.wide_positions ? (double)static_cast<const int64_t*>(a.positions)[at]
+                                             : (double)static_cast<const int32_t*>(a.positions)[at];
+    float cs[4], sn[4];
 #pragma unroll
-    for (int i = 0; i < A; ++i) {
+    for (int i = 0; i < 4; ++i) {
         cs[i] = 1.0f, sn[i] = 0.0f;
         if (turns) {
-            const int f = INTER ? 4 * j + i : 8 * j - (second ? half : 0) + i;
-            double turn = p * (a.frequencies[f] * 0.15915494309189535);
+            double turn = position * (a.frequencies[4 * j + i] * 0.15915494309189535);
             turn -= rint(turn);
-            sincospif((float)(turn + turn), &sn[i], &cs[i]);
+            sin_cos<T>((float)turn, &sn[i], &cs[i]);
             cs[i] *= a.amplitude;
-            sn[i] *= second ? a.amplitude : -a.amplitude;  // of the partner's value
+            sn[i] *= a.amplitude;
         }
     }
-    float w[8];
-    bool norm = false;
-    auto weight = [&](const void* src, int f32) {
-        norm = src != nullptr;
-        if (!norm) return;
-        if (f32)
-            load8<float>(static_cast<const float*>(src) + j * 8, w);
-        else
-            load8<T>(static_cast<const T*>(src) + j * 8, w);
+    // Pair e's new values are r (x_u uu - x_v vu) and r (x_v vv + x_u uv): the weights are in the rotation.
+    float uu[4], vu[4], vv[4], uv[4];
+    const void* weights = nullptr;
+    auto take = [&](const void* src, int f32) {
+        weights = src;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float wu = 1.0f, wv = 1.0f;
+            if (src) {
+                const int u = INTER ? 2 * e : e, v = INTER ? 2 * e + 1 : e + 4;
+                const int iu = at0 + (u < 4 ? u : step + u - 4), iv = at0 + (v < 4 ? v : step + v - 4);
+                wu = f32 ? static_cast<const float*>(src)[iu] : to_f32(static_cast<const T*>(src)[iu]);
+                wv = f32 ? static_cast<const float*>(src)[iv] : to_f32(static_cast<const T*>(src)[iv]);
+            }
+            uu[e] = wu * cs[e], vu[e] = wv * sn[e], vv[e] = wv * cs[e], uv[e] = wu * sn[e];
+        }
     };
-    int held = -1;  // whose weight w is: 0 q's, 1 k's
+    if (is_q(p0)) take(a.q_weight, a.q_weight_f32);
+    bool on_k = false;
 
-    for (int base = h0; base < h1; base += kAhead * N) {
+    for (int base = p0; base < p1; base += kAhead) {
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            const int h = base + i * N + lane / L;
-            if (base + i * N >= h1) break;
-            const bool live = h < h1;
+            const int p = base + i;
+            if (p >= p1) break;
+            if (!is_q(p) && !on_k) {
+                on_k = true;
+                take(a.k_weight, a.k_weight_f32);
+            }
             float x[8];
-            if (live) {
-                raw[i].floats(x);
-                const int next = h + kAhead * N;
-                if (next < h1) raw[i].load(src(next));
-            } else {
+            raw[i].floats(x);
+            load(raw[i], p + kAhead);
+            float r = 1.0f;
+            if (weights) {
+                uint64_t two = mul2(pair(x[0], x[1]), pair(x[0], x[1]));
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = 0.0f;
+                for (int e = 2; e < 8; e += 2) two = fma2(pair(x[e], x[e + 1]), pair(x[e], x[e + 1]), two);
+                float s0, s1;
+                unpair(two, s0, s1);
+                float sum = s0 + s1;
+#pragma unroll
+                for (int off = L / 2; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, off);
+                r = rsqrtf(sum * (1.0f / D) + a.eps);
             }
-            const int whose = h < a.Hq ? 0 : 1;
-            if (held != whose) {
-                held = whose;
-                weight(whose ? a.k_weight : a.q_weight, whose ? a.k_weight_f32 : a.q_weight_f32);
-            }
-            float sum = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
-#pragma unroll
-            for (int off = L / 2; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, off);
-            if (norm) {
-                const float r = rsqrtf(sum * (1.0f / D) + a.eps);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = x[e] * r * w[e];
-            }
+            const uint64_t rr = pair(r, r);
             float y[8];
-            if (INTER) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {  // sn: minus the sine
-                    y[2 * e] = fmaf(x[2 * e], cs[e], x[2 * e + 1] * sn[e]);
-                    y[2 * e + 1] = fmaf(x[2 * e + 1], cs[e], -(x[2 * e] * sn[e]));
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float o = __shfl_sync(0xFFFFFFFFu, x[e], partner);
-                    y[e] = fmaf(x[e], cs[e], o * sn[e]);
-                }
+            for (int e = 0; e < 4; e += 2) {
+                const int u0 = INTER ? 2 * e : e, u1 = INTER ? 2 * e + 2 : e + 1, dv = INTER ? 1 : 4;
+                const uint64_t xu = mul2(pair(x[u0], x[u1]), rr), xv = mul2(pair(x[u0 + dv], x[u1 + dv]), rr);
+                unpair(fma2(xu, pair(uu[e], uu[e + 1]), mul2(xv, pair(-vu[e], -vu[e + 1]))), y[u0], y[u1]);
+                unpair(fma2(xv, pair(vv[e], vv[e + 1]), mul2(xu, pair(uv[e], uv[e + 1]))), y[u0 + dv], y[u1 + dv]);
             }
-            if (live)
-                store8<T>(h < a.Hq ? static_cast<T*>(a.q_out) + (token * a.Hq + h) * D + j * 8
-                                   : static_cast<T*>(a.k_out) + (token * a.Hkv + h - a.Hq) * D + j * 8,
-                          y);
+            if (live(p)) {
+                T* dst = is_q(p) ? qdst + (int64_t)p * N * D : kdst + (int64_t)(p - q_passes) * N * D;
+                store4<T>(dst, y[0], y[1], y[2], y[3]);
+                store4<T>(dst + step, y[4], y[5], y[6], y[7]);
+            }
         }
     }
 }
@@ -210,7 +227,7 @@ extern "C" int lsa_norm_rotate(const void* q, const void* k, int dtype, const in
     a.tokens = B * T, a.T = (int)T, a.Hq = (int)Hq, a.Hkv = (int)Hkv, a.R = (int)R;
     a.amplitude = amplitude, a.eps = eps;
     // a token's heads over several warps where the tokens alone would not fill the SMs
-    const int64_t passes = (Hq + Hkv + 256 / D - 1) / (256 / D);
+    const int64_t each = 256 / D, passes = (Hq + each - 1) / each + (Hkv + each - 1) / each;
     int64_t sections = (148 * 16 + a.tokens - 1) / a.tokens;
     a.sections = (int)(sections < 1 ? 1 : (sections > passes ? passes : sections));
     const int64_t blocks = (a.tokens * a.sections + kWarps - 1) / kWarps;
