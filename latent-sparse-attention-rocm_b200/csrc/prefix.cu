@@ -525,6 +525,8 @@ std::atomic<int64_t> g_wait_ns{kWaitNs};
 
 }  // namespace
 
+uint64_t wait_limit_ns() { return (uint64_t)g_wait_ns.load(std::memory_order_relaxed); }
+
 int launch_prefix_finish(const PrefixArgs& a, const TilePlan& tp, int dtype, int D, const RowsPlan& rp,
                          const float* scores, float* scores_out, cudaStream_t stream) {
     if (dtype == kF32) return finish_d<float>(a, tp, D, rp, scores, scores_out, stream);
@@ -604,7 +606,7 @@ int lsa_shared_prefix_attention(const void* q, const void* k_prefix, const void*
     a.P = (int)P, a.T = (int)T;
     a.Sp = p.Sp, a.So = p.So, a.parts_p = p.parts_p, a.parts_o = p.parts_o;
     a.status = status;
-    a.wait_ns = (uint64_t)g_wait_ns.load(std::memory_order_relaxed);
+    a.wait_ns = wait_limit_ns();
     a.rows = B * Tq * Hq;
     a.part_rows = p.part_rows;
     a.scale_log2 = scale_log2;

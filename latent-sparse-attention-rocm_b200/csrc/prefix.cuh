@@ -128,6 +128,9 @@ struct RowsPlan {
     float* logits;  // [B, Hkv, Tq * G, pitch] log2-domain logits of the own keys, or null
 };
 
+// The limit of each bounded wait of the calls launched from now on (lsa_shared_prefix_wait_limit).
+uint64_t wait_limit_ns();
+
 int launch_prefix_simt(const PrefixArgs& a, int D, cudaStream_t stream);  // fp32 inputs
 int launch_prefix_tiles(const PrefixArgs& a, const TilePlan& tp, int dtype, int D, cudaStream_t stream);
 int launch_prefix_rows(const PrefixArgs& a, const RowsPlan& rp, int dtype, int D, cudaStream_t stream);

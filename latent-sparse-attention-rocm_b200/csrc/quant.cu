@@ -12,31 +12,54 @@ constexpr int kSMs = 148;
 constexpr int kFewRows = 16;  // rows of the few-row kernel's tiles
 constexpr int kUnit = 128;      // keys that a CTA's four warps take at a time
 constexpr int kMostCluster = 16;
+constexpr int kMaxTileParts = 32, kMostRounds = 8;  // splits of a tile; rounds of the SMs that split tiles fill
 constexpr double kItemCost = 1.5, kJoinCost = 3.0;  // a CTA's start and end, the join's launch, in units' times
 
 struct Plan {
     int parts;
-    bool cluster;   // joined within clusters of `parts` CTAs
-    int64_t bytes;  // of scratch
+    bool cluster;       // joined within clusters of `parts` CTAs
+    int tokens, tiles, whole;  // QuantArgs'
+    bool streams;
+    int64_t part_rows;
+    int64_t bytes;      // of scratch
 };
 
 // keys: the most that a row sees
-void make_plan(int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_t keys, Plan* p) {
-    const int64_t rows = B * Tq * Hq, tiles = (Tq * (Hq / Hkv) + kFewRows - 1) / kFewRows, items = B * Hkv * tiles;
-    const int64_t places = kSMs * (Tq * (Hq / Hkv) <= 8 ? 3 : 2);  // CTAs of the few-row kernel that run at a time
-    const int64_t chunks = (keys + kUnit - 1) / kUnit;
+Plan make_plan(int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_t keys) {
+    Plan p = {};
+    const int64_t G = Hq / Hkv, chunks = (keys + kUnit - 1) / kUnit;
+    p.part_rows = B * Tq * Hq;
+    p.parts = 1;
+    if (Tq * G > kFewRows && G <= 128) {
+        // Whole rounds of one tile an SM are not split (no parts to write, read and join); the tiles of the last, short
+        // round are, so that it too fills the GPU.
+        p.tokens = (int)(128 / G);
+        p.streams = Tq <= p.tokens;
+        p.tiles = (int)((Tq + 2 * p.tokens - 1) / (2 * p.tokens));
+        const int64_t all = B * Hkv * p.tiles, split = p.streams ? all : all % kSMs;
+        const int64_t most = split ? kMostRounds * kSMs / split : 0;
+        p.parts = balance(split, chunks, 4, kSMs, (int)(most < 1 ? 1 : (most < kMaxTileParts ? most : kMaxTileParts)));
+        if (p.parts < 1) p.parts = 1;
+        // two streams are parts of their own: they never write the output
+        p.whole = (int)(p.streams ? 0 : (p.parts == 1 ? all : all - split));
+        p.part_rows = (all - p.whole) * quant_tile_rows(p.streams);
+        p.bytes = p.part_rows * (p.streams ? 2 : 1) * p.parts * (D + 1) * 4;
+        return p;
+    }
+    const int64_t tiles = (Tq * G + kFewRows - 1) / kFewRows, items = B * Hkv * tiles;
+    const int64_t places = kSMs * (Tq * G <= 8 ? 3 : 2);  // CTAs of the few-row kernel that run at a time
     auto cost = [&](int64_t parts) {
         return (double)((items * parts + places - 1) / places) * ((double)chunks / parts + kItemCost);
     };
     // Parts that are a cluster's CTAs join within the launch, which pays where all clusters run at once (4 x 2k keys:
     // 10.3 us against 12.0 with a second launch); where CTAs wait for a place, a cluster waits for all of its own
     // (64 x 8k: 145 against 138 us; 32 lists of 2116: 51 against 43).
-    p->parts = 1, p->cluster = false;
     for (int c = 2; c <= kMostCluster && c / 2 < chunks && items * c <= places; c *= 2)
-        if (cost(c) < 0.99 * cost(p->parts)) p->parts = c, p->cluster = true;
+        if (cost(c) < 0.99 * cost(p.parts)) p.parts = c, p.cluster = true;
     const int s = balance(items, chunks, kItemCost, places, kMaxQuantParts);
-    if (s > 1 && cost(s) + kJoinCost < cost(p->parts)) p->parts = s, p->cluster = false;
-    p->bytes = p->parts > 1 && !p->cluster ? p->parts * rows * (D + 1) * 4 : 0;
+    if (s > 1 && cost(s) + kJoinCost < cost(p.parts)) p.parts = s, p.cluster = false;
+    p.bytes = p.parts > 1 && !p.cluster ? p.parts * p.part_rows * (D + 1) * 4 : 0;
+    return p;
 }
 
 bool sizes_ok(int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_t keys) {
@@ -69,16 +92,19 @@ int run(QuantArgs& a, int dtype, int code, int64_t D, int64_t keys, float scale,
     if (!(a.scale_log2 > 0) || !isfinite(a.scale_log2)) return LSA_ERR_ARG;
     if (reinterpret_cast<uintptr_t>(a.q) % 16 != 0 || reinterpret_cast<uintptr_t>(a.out) % 16 != 0) return LSA_ERR_ARG;
     if (a.q_b % 8 != 0 || a.q_t % 8 != 0 || a.q_h % 8 != 0) return LSA_ERR_ARG;
-    Plan p;
-    make_plan(a.B, a.Tq, a.Hq, a.Hkv, D, keys, &p);
+    const Plan p = make_plan(a.B, a.Tq, a.Hq, a.Hkv, D, keys);
     if (p.bytes > 0 && (scratch == nullptr || scratch_bytes < p.bytes || reinterpret_cast<uintptr_t>(scratch) % 16 != 0))
         return LSA_ERR_ARG;
     a.rows = (int64_t)a.B * a.Tq * a.Hq;
     a.parts = p.parts, a.cluster = p.cluster;
+    a.tokens = p.tokens, a.tiles = p.tiles, a.whole = p.whole, a.streams = p.streams;
+    a.part_rows = p.part_rows;
+    a.wait_ns = wait_limit_ns();
     a.part_o = static_cast<float*>(scratch);
-    a.part_lse = a.part_o + p.parts * a.rows * D;
-    const int rc = launch_quant_rows(a, dtype, code, (int)D, stream);
-    return rc != LSA_OK || a.parts == 1 || a.cluster ? rc : launch_quant_join(a, dtype, (int)D, stream);
+    a.part_lse = a.part_o + (p.streams ? 2 : 1) * p.parts * p.part_rows * D;
+    const int rc = a.tokens > 0 ? launch_quant_tiles(a, dtype, code, (int)D, stream)
+                                : launch_quant_rows(a, dtype, code, (int)D, stream);
+    return rc != LSA_OK || p.bytes == 0 ? rc : launch_quant_join(a, dtype, (int)D, stream);
 }
 
 }  // namespace
@@ -90,9 +116,7 @@ int64_t lsa_quantized_scratch(int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, in
     using namespace lsa;
     if (!sizes_ok(B, Tq, Hq, Hkv, D, keys)) return LSA_ERR_ARG;
     if (B == 0 || Tq == 0) return 0;
-    Plan p;
-    make_plan(B, Tq, Hq, Hkv, D, keys, &p);
-    return p.bytes;
+    return make_plan(B, Tq, Hq, Hkv, D, keys).bytes;
 }
 
 int lsa_quantized_attention(const void* q, int dtype, const int64_t* q_strides, const void* k8, const void* v8,
@@ -109,7 +133,7 @@ int lsa_quantized_attention(const void* q, int dtype, const int64_t* q_strides, 
     const int rc = pool(&a, k8, v8, k_scale, v_scale, code, pages, page, Hkv, table, table_ld, B, M, lengths);
     if (rc != LSA_OK) return rc;
     a.q = q, a.q_b = q_strides[0], a.q_t = q_strides[1], a.q_h = q_strides[2];
-    a.out = out, a.lse = lse;
+    a.out = out, a.lse = lse, a.status = status;
     a.B = (int)B, a.Tq = (int)Tq, a.Hq = (int)Hq, a.Hkv = (int)Hkv, a.G = (int)(Hq / Hkv);
     return run(a, dtype, code, D, M * page, scale, scratch, scratch_bytes, stream);
 }

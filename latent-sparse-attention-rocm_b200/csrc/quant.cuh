@@ -43,6 +43,14 @@ struct QuantArgs {
     int parts;
     bool cluster;                 // the parts are a cluster's CTAs, which join them (few-row kernel)
     int64_t rows;                 // B * Tq * Hq
+    // The tensor-core kernel's (quant_tile.cu): tokens of a half tile (0: the few-row kernel), tiles of a sequence and
+    // KV head, whether a tile is one half's rows, and the first tiles, which are not split and write the output
+    // themselves. A part then has the split tiles' rows, quant_tile_rows(a) a tile.
+    int tokens, tiles, whole;
+    bool streams;
+    int64_t part_rows;            // rows of a part
+    int32_t* status;              // LSA_ERR_TIMEOUT after an expired wait
+    uint64_t wait_ns;             // limit of each wait
     float scale_log2;             // scale * log2(e)
 };
 
@@ -91,6 +99,29 @@ template <int CODE> __device__ __forceinline__ float scale_for(float top) {
     return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
+// The power of two that brings a bf16 row to fp16, its largest magnitude (bits given) to [2^8, 2^9); *factor takes its
+// inverse. Zero, infinities and NaN stay as they are.
+__device__ __forceinline__ float half_factor(uint32_t top, float* factor) {
+    const int e = (int)(top >> 7);  // biased exponent
+    const int up = e == 0 || e == 255 ? 0 : min(8 - (e - 127), 100);
+    *factor *= __uint_as_float((uint32_t)(127 - up) << 23);
+    return __uint_as_float((uint32_t)(up + 127) << 23);
+}
+
+// Tile i of the tensor-core kernel: (sequence, KV head, row tile), the longest causal ranges first.
+__device__ __forceinline__ void quant_tile_at(const QuantArgs& a, int i, int* b, int* h, int* tile) {
+    *h = i % a.Hkv, i /= a.Hkv;
+    *b = i % a.B;
+    *tile = a.tiles - 1 - i / a.B;
+}
+__host__ __device__ __forceinline__ int quant_tile_rows(bool streams) { return streams ? 128 : 256; }
+// Row rl of half hf of split tile `rest`, in part `split` (two parts a split where the halves are streams).
+__device__ __forceinline__ int64_t quant_part_row(const QuantArgs& a, int split, int rest, int hf, int rl) {
+    return a.streams ? (2 * split + hf) * a.part_rows + (int64_t)rest * 128 + rl
+                     : split * a.part_rows + (int64_t)rest * 256 + hf * 128 + rl;
+}
+
+int launch_quant_tiles(const QuantArgs& a, int dtype, int code, int D, cudaStream_t stream);
 int launch_quant_rows(const QuantArgs& a, int dtype, int code, int D, cudaStream_t stream);
 int launch_quant_join(const QuantArgs& a, int dtype, int D, cudaStream_t stream);
 

@@ -26,6 +26,7 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kKeys = 32;  // keys of a warp's tile: one a lane where they are looked up
+constexpr int kFewParts = 8;  // that one warp joins
 constexpr float kLift = 10.0f, kGrow = 5.0f;
 
 template <int D, int NT> struct QuantShape {
@@ -274,10 +275,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) quant_rows_kerne
             }
             top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
             top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-            const int e = (int)(top >> 7);  // biased exponent; zero, and infinities and NaN, stay as they are
-            const int up = e == 0 || e == 255 ? 0 : min(8 - (e - 127), 100);
-            const float by = __uint_as_float((uint32_t)(up + 127) << 23);
-            f *= __uint_as_float((uint32_t)(127 - up) << 23);
+            const float by = half_factor(top, &f);
 #pragma unroll
             for (int kk = 0; kk < KS; ++kk) {
                 qf[u][kk][0] = pack_half(__uint_as_float(raw[kk].x << 16) * by, __uint_as_float(raw[kk].x & 0xFFFF0000u) * by);
@@ -500,7 +498,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) quant_rows_kerne
             store4<T>(static_cast<T*>(a.out) + rid * D + col, x);
             if (col == 0 && a.lse) a.lse[rid] = lse * 0.69314718055994531f;
         } else {
-            const int64_t at = (int64_t)split * a.rows + rid;
+            const int64_t at = (int64_t)split * a.part_rows + rid;
             *reinterpret_cast<float4*>(a.part_o + at * D + col) = x;
             if (col == 0) a.part_lse[at] = lse;
         }
@@ -533,30 +531,41 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) quant_rows_kerne
     cluster_sync();  // no CTA leaves while another reads its memory
 }
 
-// The parts of a row joined: a CTA a row, a warp every eighth part. Every part's values are asked for before the
-// weights are known, so a row is one round of memory.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) quant_join_kernel(const QuantArgs a) {
-    constexpr int V = D / 32, NW = 8, N = kMaxQuantParts / NW;
-    __shared__ float so[NW][D];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+// The parts of a row joined, SPREAD warps a row (one where the parts are few, so that a CTA takes eight rows). Every
+// part's values are asked for before the weights are known, so a row is one round of memory.
+template <typename T, int D, int SPREAD>
+__global__ void __launch_bounds__(256) quant_join_kernel(const QuantArgs a, const int parts) {
+    constexpr int V = D / 32, N = SPREAD == 1 ? kFewParts : kMaxQuantParts / SPREAD;
+    constexpr int L = SPREAD == 1 ? 1 : kMaxQuantParts / 32;  // loads of the parts' sums, 32 each
+    __shared__ float so[8][D];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % SPREAD;
     grid_wait();
     grid_trigger();
-    const int64_t rid = blockIdx.x;
-    float lse[3], top = -INFINITY;  // at most 96 parts, 32 a load
+    const int64_t prow = (int64_t)blockIdx.x * (8 / SPREAD) + warp / SPREAD;
+    int64_t rid = prow;
+    bool live = prow < a.part_rows;
+    if (a.tokens > 0 && live) {  // the rows of the split tiles
+        const int per = quant_tile_rows(a.streams), rl = (int)(prow % per), hf = rl >> 7;
+        int b, h, tile;
+        quant_tile_at(a, a.whole + (int)(prow / per), &b, &h, &tile);
+        const int tl = (rl & 127) / a.G, tok = tile * (per / 128) * a.tokens + hf * a.tokens + tl;
+        live = tl < a.tokens && tok < a.Tq;
+        rid = ((int64_t)b * a.Tq + tok) * a.Hq + (int64_t)h * a.G + (rl & 127) - tl * a.G;
+    }
+    float lse[L], top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 3; ++i) {
+    for (int i = 0; i < L; ++i) {
         const int part = i * 32 + lane;
-        lse[i] = part < a.parts ? a.part_lse[part * a.rows + rid] : -INFINITY;
+        lse[i] = live && part < parts ? a.part_lse[part * a.part_rows + prow] : -INFINITY;
     }
     float y[N][V];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const int part = warp + NW * i;
-        const float* src = a.part_o + (part * a.rows + rid) * D + lane * V;
+        const int part = sub + SPREAD * i;
+        const float* src = a.part_o + (part * a.part_rows + prow) * D + lane * V;
 #pragma unroll
         for (int e = 0; e < V; ++e) y[i][e] = 0.0f;
-        if (part < a.parts) {
+        if (live && part < parts) {
             if constexpr (V == 4) {
                 const float4 z = *reinterpret_cast<const float4*>(src);
                 y[i][0] = z.x, y[i][1] = z.y, y[i][2] = z.z, y[i][3] = z.w;
@@ -567,12 +576,12 @@ __global__ void __launch_bounds__(256) quant_join_kernel(const QuantArgs a) {
         }
     }
 #pragma unroll
-    for (int i = 0; i < 3; ++i) top = fmaxf(top, lse[i]);
+    for (int i = 0; i < L; ++i) top = fmaxf(top, lse[i]);
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
-    float total = 0.0f, f[3], o[V];
+    float total = 0.0f, f[L], o[V];
 #pragma unroll
-    for (int i = 0; i < 3; ++i) {  // NaN passes on
+    for (int i = 0; i < L; ++i) {  // NaN passes on
         f[i] = lse[i] == -INFINITY ? 0.0f : exp2f(lse[i] - (top == -INFINITY ? 0.0f : top));
         total += f[i];
     }
@@ -582,21 +591,33 @@ __global__ void __launch_bounds__(256) quant_join_kernel(const QuantArgs a) {
     for (int e = 0; e < V; ++e) o[e] = 0.0f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const float fi = __shfl_sync(0xFFFFFFFFu, f[i / 4], (warp + NW * i) & 31);
+        const float fi = __shfl_sync(0xFFFFFFFFu, f[SPREAD * i / 32], (sub + SPREAD * i) & 31);
+        // what a part without a key holds is never used
 #pragma unroll
-        for (int e = 0; e < V; ++e) o[e] = fmaf(fi, y[i][e], o[e]);
+        for (int e = 0; e < V; ++e) o[e] = fi == 0.0f ? o[e] : fmaf(fi, y[i][e], o[e]);
     }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    if constexpr (SPREAD == 1) {
+        if (live) {
+            T* dst = static_cast<T*>(a.out) + rid * D + lane * V;
+            if constexpr (V == 4)
+                store4<T>(dst, make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv));
+            else
+                *reinterpret_cast<uint32_t*>(dst) = pack16(o[0] * inv, o[1] * inv, (T*)nullptr);
+        }
+    } else {
 #pragma unroll
-    for (int e = 0; e < V; ++e) so[warp][lane * V + e] = o[e];
-    __syncthreads();
-    const int col = threadIdx.x;
-    if (col < D) {
-        float x = 0.0f;
+        for (int e = 0; e < V; ++e) so[warp][lane * V + e] = o[e];
+        __syncthreads();
+        const int col = threadIdx.x;
+        if (col < D && live) {
+            float x = 0.0f;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) x += so[w][col];
-        static_cast<T*>(a.out)[rid * D + col] = from_f32<T>(total == 0.0f ? 0.0f : x / total);
+            for (int w = 0; w < 8; ++w) x += so[w][col];
+            static_cast<T*>(a.out)[rid * D + col] = from_f32<T>(x * inv);
+        }
     }
-    if (threadIdx.x == 0 && a.lse)
+    if (lane == 0 && sub == 0 && live && a.lse)
         a.lse[rid] = total == 0.0f ? -INFINITY : (top + log2f(total)) * 0.69314718055994531f;
 }
 
@@ -631,14 +652,18 @@ int launch_quant_rows(const QuantArgs& a, int dtype, int code, int D, cudaStream
                           : launch<__half>(a, code, D, row_tiles, (unsigned)items, stream);
 }
 
+template <typename T, int D> static int join(const QuantArgs& a, cudaStream_t stream) {
+    const int parts = a.tokens > 0 && a.streams ? 2 * a.parts : a.parts;
+    const int64_t blocks = parts <= kFewParts ? (a.part_rows + 7) / 8 : a.part_rows;
+    if (blocks > INT32_MAX || parts > kMaxQuantParts) return LSA_ERR_SIZE;
+    const dim3 grid((unsigned)blocks);
+    return parts <= kFewParts ? launch_after(quant_join_kernel<T, D, 1>, grid, 256, 0, stream, a, parts)
+                              : launch_after(quant_join_kernel<T, D, 8>, grid, 256, 0, stream, a, parts);
+}
+
 int launch_quant_join(const QuantArgs& a, int dtype, int D, cudaStream_t stream) {
-    if (a.rows > INT32_MAX) return LSA_ERR_SIZE;
-    const dim3 grid((unsigned)a.rows);
-    if (dtype == kBF16)
-        return D == 128 ? launch_after(quant_join_kernel<__nv_bfloat16, 128>, grid, 256, 0, stream, a)
-                        : launch_after(quant_join_kernel<__nv_bfloat16, 64>, grid, 256, 0, stream, a);
-    return D == 128 ? launch_after(quant_join_kernel<__half, 128>, grid, 256, 0, stream, a)
-                    : launch_after(quant_join_kernel<__half, 64>, grid, 256, 0, stream, a);
+    if (dtype == kBF16) return D == 128 ? join<__nv_bfloat16, 128>(a, stream) : join<__nv_bfloat16, 64>(a, stream);
+    return D == 128 ? join<__half, 128>(a, stream) : join<__half, 64>(a, stream);
 }
 
 }  // namespace lsa

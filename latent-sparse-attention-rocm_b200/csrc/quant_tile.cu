@@ -1,0 +1,617 @@
+// quant_tile.cu - attention over the 8-bit paged cache for many rows, on the 5th-generation tensor cores (sm_100a).
+// quant.cuh has the formulas.
+//
+// A work item is a tile of query rows of one (sequence, KV head) - two halves of 128 rows (tokens x the G query heads
+// of the group) - x a range of 128-key chunks. One CTA an item:
+//   S_h = Q_h K^T   tcgen05.mma kind::f16, Q and K as fp16 in 128B-swizzled shared memory, S in TMEM
+//   softmax         one thread a row, maximum and sums in fp32, P back over S as pairs of halves
+//   O_h += P_h V    tcgen05.mma with A = P from TMEM, V an MN-major shared-memory operand
+// With at most 128 rows both halves hold the same rows and take alternate chunks, so that two softmax chains are in
+// flight where the keys' bandwidth is the bound.
+// The codes come as they are (bulk copies of a page's rows of a head, which are contiguous) into a ring of 8-bit tiles;
+// two warps make halves of them (exact) into a ring of operand tiles, zeros where there is no key, so what a page holds
+// behind a sequence's last token never meets a product. Scales stay out of the tiles: 16 keys share a page, so a
+// row's logits are s * (ks * factor) + log2 vs with constants for 16 keys, and the sum takes 1 / vs once for 16.
+// bf16 rows of Q become fp16 by a power of two of their own, as in the few-row kernel. P is rounded to fp16 and
+// carries 2^kLift; the maximum is let stand until it has grown by more than 2^kGrow.
+//
+// Warps: 0 asks for the codes and the scales, one thread of warp 1 issues every MMA, 2 and 3 convert, 4-7 / 8-11 are
+// the softmax of half 0 / 1. TMEM: S_0/P_0 [0, 128), S_1/P_1 [128, 256), O_0 [256, 256 + D), O_1 [384, 384 + D).
+//
+// Every wait is bounded (QuantArgs::wait_ns); an expired wait raises a CTA-wide flag, every role leaves, copies and
+// MMAs in flight are waited for (bounded), the TMEM is released and LSA_ERR_TIMEOUT lands in the status word.
+#include <type_traits>
+
+#include "prefix_umma.cuh"
+#include "quant.cuh"
+
+namespace lsa {
+namespace {
+
+constexpr int kThreads = 384;
+constexpr int kConvert = 64;  // threads that convert: 16 rows a step, four a row
+constexpr float kLift = 7.0f, kGrow = 4.0f;
+constexpr int kChunks = 8;  // chunks whose scales are kept: more than the rings and the softmax hold together
+constexpr int kGroups = kChunk / 16;
+
+template <int D> struct QuantTile {
+    static constexpr int kOperand = kChunk * D * 2;  // an fp16 K, V or half-Q tile
+    static constexpr int kCodes = kChunk * D;        // its codes
+    static constexpr int kOps = D == 128 ? 3 : 6, kStages = D == 128 ? 3 : 5;
+    static constexpr int kOffOps = 2 * kOperand;
+    static constexpr int kOffStage = kOffOps + kOps * kOperand;
+    static constexpr int kOffScales = kOffStage + kStages * kCodes;  // [kChunks][kGroups] (ks, log2 vs, 1 / vs, rows)
+    static constexpr int kOffFactor = kOffScales + kChunks * kGroups * 16;
+    static constexpr int kOffBar = kOffFactor + 256 * 4;
+    static constexpr int kNumBars = 2 * kStages + 2 * kOps + 2 + 4 + 2 + 1;
+    static constexpr int kOffMisc = kOffBar + kNumBars * 8;
+    static constexpr int kSmem = kOffMisc + 16 + 1024;  // slack: the base is aligned to 1024 B
+    static_assert(kSmem <= 232448, "shared memory of a CTA");
+    static_assert(kOffStage >= 256 * (D * 4 + 16), "the rows leave through Q and the operand ring");
+};
+
+// What a CTA works on.
+struct Item {
+    int b, h, split, rest, t0;
+    bool direct;       // all of its rows' keys: it writes the output itself
+    int length, keys;  // tokens of the sequence; those that the table has room for
+    int c0, c1;        // its chunks
+};
+
+__device__ __forceinline__ Item item_of(const QuantArgs& a) {
+    Item w;
+    int i = blockIdx.x;
+    w.direct = i < a.whole;
+    w.split = w.direct ? 0 : (i - a.whole) % a.parts;
+    w.rest = w.direct ? 0 : (i - a.whole) / a.parts;
+    int tile;
+    quant_tile_at(a, w.direct ? i : a.whole + w.rest, &w.b, &w.h, &tile);
+    const int tokens = (a.streams ? 1 : 2) * a.tokens;
+    w.t0 = tile * tokens;
+    const int end = w.t0 + tokens < a.Tq ? w.t0 + tokens : a.Tq;
+    w.length = max(a.lengths[w.b], 0);
+    const int64_t room = (int64_t)a.M << a.shift;
+    w.keys = w.length < room ? w.length : (int)room;
+    int seen = w.length - a.Tq + end;  // keys that the tile's last row sees
+    seen = seen < 0 ? 0 : (seen < w.keys ? seen : w.keys);
+    const int64_t chunks = (seen + kChunk - 1) / kChunk, S = w.direct ? 1 : a.parts;
+    w.c0 = (int)(chunks * w.split / S), w.c1 = (int)(chunks * (w.split + 1) / S);
+    return w;
+}
+
+// Tile p of an item of n chunks, in the order the MMAs use them: one chunk's K (two, with two streams) ahead of the
+// first V, then V and the K that follows in turn.
+__device__ __forceinline__ void tile_of(int p, int n, bool streams, int* c, bool* value) {
+    if (!streams) {
+        *value = p & 1, *c = p >> 1;
+    } else if (p < 2 && p < n) {
+        *value = false, *c = p;
+    } else if (n == 1) {
+        *value = true, *c = 0;
+    } else {
+        const int i = p - 2;
+        *value = i >= 2 * (n - 2) || (i & 1) == 0;
+        *c = i >= 2 * (n - 2) ? i - (n - 2) : (i >> 1) + (*value ? 0 : 2);
+    }
+}
+
+// Row rl of half hf: (token of the call, head of the group); false: no row there.
+__device__ __forceinline__ bool row_at(const QuantArgs& a, const Item& w, int hf, int rl, int* tok, int* g) {
+    const int tl = rl / a.G;
+    *tok = w.t0 + (a.streams ? 0 : hf) * a.tokens + tl;
+    *g = rl - tl * a.G;
+    return tl < a.tokens && *tok < a.Tq;
+}
+
+__device__ __forceinline__ float4 lds_f4(uint32_t addr) {
+    float4 r;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(r.x), "=f"(r.y), "=f"(r.z), "=f"(r.w)
+                 : "r"(addr)
+                 : "memory");
+    return r;
+}
+__device__ __forceinline__ uint4 lds_u4(uint32_t addr) {
+    uint4 r;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+                 : "r"(addr)
+                 : "memory");
+    return r;
+}
+__device__ __forceinline__ void sts_u4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// Q's rows as fp16 in their operand tiles, and each row's factor.
+template <typename T, int D>
+__device__ __forceinline__ void load_q(const QuantArgs& a, const Item& w, uint8_t* sm) {
+    using Sh = QuantTile<D>;
+    constexpr int L = D / 8, RP = kThreads / L;  // threads of a row, rows of a pass
+    constexpr int PASSES = (256 + RP - 1) / RP;
+    float* factor = reinterpret_cast<float*>(sm + Sh::kOffFactor);
+    const int lr = threadIdx.x / L, ch = threadIdx.x % L;
+    const int halves = a.streams ? 1 : 2;
+    uint4 raw[PASSES];
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+        const int row = i * RP + lr, hf = row >> 7;
+        raw[i] = make_uint4(0, 0, 0, 0);
+        int tok, g;
+        if (row < halves * 128 && row_at(a, w, hf, row & 127, &tok, &g))
+            raw[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + w.b * a.q_b + tok * a.q_t +
+                                                     (w.h * (int64_t)a.G + g) * a.q_h + ch * 8);
+    }
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+        const int row = i * RP + lr, hf = row >> 7, r = row & 127;
+        uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+        float f = a.scale_log2;
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            uint32_t top = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = max(top, max(u[e] & 0x7FFFu, (u[e] >> 16) & 0x7FFFu));
+#pragma unroll
+            for (int off = L / 2; off >= 1; off >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
+            const float by = half_factor(top, &f);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                u[e] = pack16(__uint_as_float(u[e] << 16) * by, __uint_as_float(u[e] & 0xFFFF0000u) * by, (__half*)nullptr);
+        }
+        if (row < halves * 128) {
+            sts_u4(smem_u32(sm) + hf * Sh::kOperand + (ch >> 3) * 16384 + r * 128 + (((ch & 7) ^ (r & 7)) << 4), u[0], u[1],
+                   u[2], u[3]);
+            if (ch == 0) factor[row] = f;
+        }
+    }
+}
+
+template <typename T, int D>
+__device__ __forceinline__ void softmax_half(const QuantArgs& a, const Item& w, uint8_t* sm, uint64_t* bar_s, uint64_t* bar_p,
+                                             uint64_t* bar_o, volatile int* abort_flag, uint32_t tmem) {
+    using Sh = QuantTile<D>;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int hf = (warp - 4) >> 2, qd = warp & 3;
+    int tok, g;
+    const bool live = row_at(a, w, hf, qd * 32 + lane, &tok, &g);
+    const int limit = live ? w.length - a.Tq + tok + 1 : 0;  // keys the row sees
+    const float factor = reinterpret_cast<const float*>(sm + Sh::kOffFactor)[(a.streams ? 0 : hf) * 128 + qd * 32 + lane];
+    const uint32_t lanes = (uint32_t)(qd * 32) << 16;
+    const uint32_t tS = tmem + lanes + hf * 128;
+    const uint32_t tO = tmem + lanes + 256 + hf * 128;
+    const int step = a.streams ? 2 : 1, first = w.c0 + (a.streams ? hf : 0);
+    const int n = w.c1 > first ? (w.c1 - first + step - 1) / step : 0;
+    const uint32_t scales = smem_u32(sm) + Sh::kOffScales;
+    float m = -INFINITY, l = 0.0f;
+    bool ok = true;
+    auto publish = [&](uint64_t* bar) {  // this warp's P so far: one arrival a warp
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
+    };
+    for (int j = 0; j < n; ++j) {
+        const int c = first + j * step;
+        const int seen = limit - c * kChunk;
+        ok = role_wait(&bar_s[hf], j & 1, abort_flag, a.wait_ns);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t sc = scales + (c % kChunks) * kGroups * 16;
+        uint32_t s[128];
+        tmem_ld128_wait(tS, s);
+        if (__any_sync(0xFFFFFFFFu, seen < kChunk)) {
+#pragma unroll
+            for (int i = 0; i < 128; ++i)
+                if (i >= seen) s[i] = 0xFF800000u;  // -inf
+        }
+        // The exponentials start from the maximum of the chunks before, while this chunk's is found beside them. Only
+        // when it has grown by more than 2^kGrow does the warp take the new one, do the first 96 keys again and rescale O
+        // - always on a row's first chunk.
+        float alpha = 1.0f;
+        uint64_t sum;
+        // logits of 16 keys from s: (multiplier, addend); the multiplier stays above 0, so that -inf does
+        auto group = [&](int i, float* mul, float* add) {
+            const float4 k = lds_f4(sc + i * 16);
+            *mul = fmaxf(k.x * factor, 1e-30f), *add = k.y;
+            return k.z;
+        };
+        auto exps = [&](auto& pk, int at, int i, float neg) {  // group i's 16 keys
+            float mul, add;
+            const float inv = group(i, &mul, &add);
+            const uint64_t mul2x = pair(mul, mul), add2x = pair(add + neg, add + neg);
+            uint64_t part[2] = {0ull, 0ull};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                float x0, x1;
+                unpair(fma2(pair(__uint_as_float(s[16 * i + 2 * e]), __uint_as_float(s[16 * i + 2 * e + 1])), mul2x, add2x), x0, x1);
+                const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+                part[e & 1] = add2(part[e & 1], pair(p0, p1));
+                pk[at + e] = pack16(p0, p1, (__half*)nullptr);
+            }
+            sum = fma2(add2(part[0], part[1]), pair(inv, inv), sum);
+        };
+        float neg;
+#pragma unroll 1
+        for (bool again = false;; again = true) {
+            neg = (m == -INFINITY ? 0.0f : -m) + kLift;
+            sum = 0ull;
+            uint32_t pk[32], pk2[16];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) exps(pk, 8 * i, i, neg);
+            tmem_st32(tS, pk);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) exps(pk2, 8 * i, 4 + i, neg);
+            tmem_st16(tS + 32, pk2);
+            if (again) break;
+            float mx = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < kGroups; ++i) {
+                float mul, add, mg = __uint_as_float(s[16 * i]), mh = __uint_as_float(s[16 * i + 1]);
+                group(i, &mul, &add);
+#pragma unroll
+                for (int e = 2; e < 16; e += 4) {
+                    mg = max3(mg, __uint_as_float(s[16 * i + e]), __uint_as_float(s[16 * i + e + 1]));
+                    if (e + 2 < 16) mh = max3(mh, __uint_as_float(s[16 * i + e + 2]), __uint_as_float(s[16 * i + e + 3]));
+                }
+                mx = fmaxf(mx, fmaf(fmaxf(mg, mh), mul, add));
+            }
+            const bool grow = mx > m + kGrow;
+            if (!__any_sync(0xFFFFFFFFu, grow)) break;
+            if (grow) {
+                alpha = ex2_approx(m - mx);
+                m = mx;
+            }
+            // O_h holds the earlier chunks' sum here (their products were issued before S_h(j) by the same thread); its
+            // rescale lands before any P of this chunk is published
+            if (j > 0) {
+#pragma unroll 1
+                for (int cc = 0; cc < D / 32; ++cc) {
+                    uint32_t o[32];
+                    tmem_ld32_wait(tO + cc * 32, o);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                    tmem_st32(tO + cc * 32, o);
+                }
+            }
+        }
+        publish(&bar_p[2 * hf]);
+        {
+            uint32_t pk2[16];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) exps(pk2, 8 * i, 6 + i, neg);
+            tmem_st16(tS + 48, pk2);
+        }
+        publish(&bar_p[2 * hf + 1]);
+        float s0, s1;
+        unpair(sum, s0, s1);
+        l = l * alpha + (s0 + s1);
+    }
+    if (ok && n > 0) ok = role_wait(&bar_o[hf], 0, abort_flag, a.wait_ns);
+    if (!ok) return;
+    const int64_t rid = ((int64_t)w.b * a.Tq + tok) * a.Hq + (int64_t)w.h * a.G + g;
+    const bool none = l == 0.0f;  // the row has seen no key (a NaN logit makes l NaN, and the output)
+    const float inv = none ? 0.0f : 1.0f / l;
+    const float lse = none ? -INFINITY : m + (log2f(l) - kLift);
+    const int64_t at = quant_part_row(a, w.split, w.rest, hf, qd * 32 + lane);
+    if (live) {
+        if (!w.direct)
+            a.part_lse[at] = lse;
+        else if (a.lse)
+            a.lse[rid] = lse * 0.69314718055994531f;
+    }
+    if (n == 0) {  // a part without a key is not read
+        if (w.direct && live)
+            for (int i = 0; i < D / 8; ++i)
+                reinterpret_cast<uint4*>(static_cast<T*>(a.out) + rid * D)[i] = make_uint4(0, 0, 0, 0);
+        return;
+    }
+    // The row through shared memory (every MMA is done) and out by one bulk copy: a thread holds a whole row, so its own
+    // stores would touch 32 rows an instruction. Rows 16 bytes apart from a multiple of 128: eight lanes' 16-byte stores
+    // fall into different banks.
+    tc_fence_after();
+    constexpr int kPitch = D * 4 + 16;
+    uint8_t* line = sm + ((warp - 4) * 32 + lane) * kPitch;
+#pragma unroll
+    for (int cc = 0; cc < D / 32; ++cc) {
+        uint32_t o[32];
+        tmem_ld32_wait(tO + cc * 32, o);
+        if (w.direct) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t u[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    u[e] = pack16(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv,
+                                  (T*)nullptr);
+                *reinterpret_cast<uint4*>(line + cc * 64 + i * 16) = make_uint4(u[0], u[1], u[2], u[3]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                *reinterpret_cast<float4*>(line + cc * 128 + i * 16) =
+                    make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv,
+                                __uint_as_float(o[4 * i + 2]) * inv, __uint_as_float(o[4 * i + 3]) * inv);
+        }
+    }
+    fence_proxy_async_smem();
+    if (live) {
+        if (w.direct)
+            bulk_s2g(static_cast<T*>(a.out) + rid * D, smem_u32(line), D * 2);
+        else
+            bulk_s2g(a.part_o + at * D, smem_u32(line), D * 4);
+    }
+    bulk_commit_wait();
+}
+
+template <typename T, int CODE, int D>
+__global__ void __launch_bounds__(kThreads, 1) quant_tile_kernel(const QuantArgs a) {
+    using Sh = QuantTile<D>;
+    constexpr int NS = Sh::kStages, NO = Sh::kOps, KS = D / 16;
+    extern __shared__ uint8_t raw[];
+    uint8_t* sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+    const uint32_t sbase = smem_u32(sm);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Sh::kOffBar);
+    uint64_t *codes_full = bars, *codes_empty = bars + NS, *op_full = bars + 2 * NS, *op_empty = op_full + NO,
+             *bar_s = op_empty + NO, *bar_p = bar_s + 2, *bar_o = bar_p + 4, *bar_drain = bar_o + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + Sh::kOffMisc);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + Sh::kOffMisc + 4);
+    const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    if (warp == 1) tmem_alloc(tmem_slot, 512);
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < NS; ++s) {
+            mbar_init(&codes_full[s], 2);   // the bytes, and the scales beside them
+            mbar_init(&codes_empty[s], 2);  // the converting warps
+        }
+        for (int s = 0; s < NO; ++s) {
+            mbar_init(&op_full[s], 2);
+            mbar_init(&op_empty[s], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bar_s[i], 1);
+            mbar_init(&bar_p[2 * i], 4);
+            mbar_init(&bar_p[2 * i + 1], 4);
+            mbar_init(&bar_o[i], 1);
+        }
+        mbar_init(bar_drain, 1);
+        *abort_flag = a.wait_ns == 0;  // then the MMA thread gives up before its first wait, copies in flight
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    grid_wait();  // the inputs, the lengths among them, and the parts' last readers
+    grid_trigger();
+    const Item w = item_of(a);
+    const int n = w.c1 - w.c0;
+    if (n > 0) load_q<T, D>(a, w, sm);
+    fence_proxy_async_smem();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp >= 4) {
+        // 384 threads launch at 168 registers: 128 x 56 + 256 x 224 = 384 x 168
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;" ::: "memory");
+        softmax_half<T, D>(a, w, sm, bar_s, bar_p, bar_o, abort_flag, tmem);
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;" ::: "memory");
+        if (warp == 0) {
+            // ------------------------------------------------ codes and scales: a lane a page of the chunk
+            const int page = 1 << a.shift, pages = kChunk >> a.shift;
+            const int32_t* table = a.table + w.b * a.table_ld;
+            auto lookup = [&](int c) {  // page id of this lane's page of chunk c, -1: none
+                const int64_t slot = (int64_t)(w.c0 + c) * pages + lane;
+                int id = -1;
+                if (lane < pages && c < n && slot < a.M && (slot << a.shift) < w.keys) id = table[slot];
+                return id >= 0 && id < a.pages ? id : -1;
+            };
+            // rows of chunk c's K are asked for up to two chunks ahead of its V's
+            int next = lookup(0), held[3] = {-1, -1, -1};
+            int p = 0;
+            bool ok = true;
+            for (; p < 2 * n; ++p) {
+                const int s = p % NS;
+                if (p >= NS && !(ok = role_wait(&codes_empty[s], (p / NS - 1) & 1, abort_flag, a.wait_ns))) break;
+                int c;
+                bool value;
+                tile_of(p, n, a.streams, &c, &value);
+                int id;
+                if (!value) {
+                    id = next, next = lookup(c + 1);
+                    held[2] = c % 3 == 2 ? id : held[2], held[1] = c % 3 == 1 ? id : held[1], held[0] = c % 3 == 0 ? id : held[0];
+                } else {
+                    id = c % 3 == 0 ? held[0] : (c % 3 == 1 ? held[1] : held[2]);
+                }
+                const int left = w.keys - (w.c0 + c) * kChunk - lane * page;
+                const int rows = id < 0 || left <= 0 ? 0 : (left < page ? left : page);
+                int total = rows;
+#pragma unroll
+                for (int off = 1; off < 8; off <<= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, off);
+                if (lane == 0) mbar_arrive_expect_tx(&codes_full[s], total * D);
+                __syncwarp();
+                const int64_t head = (int64_t)(id < 0 ? 0 : id) * a.Hkv + w.h;
+                if (rows > 0)
+                    bulk_g2s(sm + Sh::kOffStage + s * Sh::kCodes + lane * page * D,
+                             (value ? a.v8 : a.k8) + (head << a.shift) * D, rows * D, &codes_full[s]);
+                if (!value) {
+                    // 16 keys a lane: their page's scales, and how many of them are there
+                    const int from = (lane & 7) * 16 >> a.shift;
+                    const int gid = __shfl_sync(0xFFFFFFFFu, id, from);
+                    int grows = __shfl_sync(0xFFFFFFFFu, rows, from) - ((lane & 7) * 16 & (page - 1));
+                    grows = gid < 0 || grows < 0 ? 0 : (grows < 16 ? grows : 16);
+                    float4 k = make_float4(1.0f, -INFINITY, 0.0f, 0.0f);
+                    if (lane < kGroups && grows > 0) {
+                        const int64_t gh = (int64_t)gid * a.Hkv + w.h;
+                        const float vs = fmaxf(a.vs[gh], 8.6736174e-19f);  // 2^-60
+                        k = make_float4(a.ks[gh], log2f(vs), 1.0f / vs, __int_as_float(grows));
+                    }
+                    if (lane < kGroups)
+                        *reinterpret_cast<float4*>(sm + Sh::kOffScales + (((w.c0 + c) % kChunks) * kGroups + lane) * 16) = k;
+                    __syncwarp();
+                }
+                if (lane == 0) mbar_arrive(&codes_full[s]);
+            }
+            // Every copy issued lands before the CTA leaves, also when it was another role that gave up.
+            for (int i = p > NS ? p - NS : 0; i < p; ++i) mbar_wait_bounded(&codes_full[i % NS], (i / NS) & 1);
+            __syncwarp();
+        } else if (warp == 1) {
+            // ------------------------------------------------ every MMA of the CTA, from one thread
+            constexpr uint32_t idS = umma_idesc_f16<__half>(128, 128, false);
+            constexpr uint32_t idO = umma_idesc_f16<__half>(128, D, true);
+            if (elect_one()) {
+                const uint64_t qd0 = sw128_desc(sbase, 16, 1024);
+                const uint64_t kd0 = sw128_desc(sbase + Sh::kOffOps, 16, 1024);
+                const uint64_t vd0 = sw128_desc(sbase + Sh::kOffOps, 16384, 1024);
+                const uint32_t q1 = a.streams ? 0 : Sh::kOperand;
+                int stage = 0, phase = 0;  // of the next tile of the ring
+                auto advance = [&]() {
+                    if (++stage == NO) stage = 0, phase ^= 1;
+                };
+                auto scores = [&](int hf, int st) {
+                    const uint64_t qd = desc_at(qd0, hf ? q1 : 0), kd = desc_at(kd0, st * Sh::kOperand);
+#pragma unroll
+                    for (int kk = 0; kk < KS; ++kk) {
+                        const uint32_t off = (kk >> 2) * 16384 + (kk & 3) * 32;
+                        umma_f16_ss(tmem + hf * 128, desc_at(qd, off), desc_at(kd, off), idS, kk > 0);
+                    }
+                    umma_commit(&bar_s[hf]);
+                };
+                // P_h's first 96 and last 32 keys as they come; O_h starts afresh on a half's first chunk
+                auto product = [&](int hf, int st, bool fresh, uint32_t parity) -> bool {
+                    const uint64_t vd = desc_at(vd0, st * Sh::kOperand);
+                    const uint32_t o = tmem + 256 + hf * 128, p = tmem + hf * 128;
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        if (!thread_wait(&bar_p[2 * hf + half], parity, abort_flag, a.wait_ns)) return false;
+                        tc_fence_after();
+#pragma unroll
+                        for (int kk = 6 * half; kk < 6 + 2 * half; ++kk)
+                            umma_f16_ts(o, p + kk * 8, desc_at(vd, kk * 2048), idO, kk > 0 || !fresh);
+                    }
+                    return true;
+                };
+                auto tile = [&]() -> bool {
+                    const bool ok = thread_wait(&op_full[stage], phase, abort_flag, a.wait_ns);
+                    tc_fence_after();
+                    return ok;
+                };
+                bool ok = *abort_flag == 0;
+                if (ok && n > 0 && !a.streams) {
+                    ok = tile();
+                    if (ok) {
+                        scores(0, stage), scores(1, stage);
+                        umma_commit(&op_empty[stage]);
+                        advance();
+                    }
+                    for (int j = 0; ok && j < n; ++j) {
+                        const bool more = j + 1 < n;
+                        const int sv = stage;
+                        if (!(ok = tile())) break;
+                        advance();
+                        if (!(ok = product(0, sv, j == 0, j & 1))) break;
+                        if (more) {
+                            if (!(ok = tile())) break;
+                            scores(0, stage);
+                        }
+                        if (!(ok = product(1, sv, j == 0, j & 1))) break;
+                        umma_commit(&op_empty[sv]);
+                        if (more) {
+                            scores(1, stage);
+                            umma_commit(&op_empty[stage]);
+                            advance();
+                        }
+                    }
+                } else if (ok && n > 0) {
+                    for (int c = 0; ok && c < n && c < 2; ++c) {
+                        ok = tile();
+                        if (ok) {
+                            scores(c, stage);
+                            umma_commit(&op_empty[stage]);
+                            advance();
+                        }
+                    }
+                    for (int c = 0; ok && c < n; ++c) {
+                        const int hf = c & 1;
+                        if (!(ok = tile())) break;
+                        if (!(ok = product(hf, stage, c < 2, (c >> 1) & 1))) break;
+                        umma_commit(&op_empty[stage]);
+                        advance();
+                        if (c + 2 < n) {
+                            if (!(ok = tile())) break;
+                            scores(hf, stage);
+                            umma_commit(&op_empty[stage]);
+                            advance();
+                        }
+                    }
+                }
+                if (ok) umma_commit(&bar_o[0]), umma_commit(&bar_o[1]);
+                umma_commit(bar_drain);  // every MMA completes before the TMEM is released
+                mbar_wait_bounded(bar_drain, 0);
+            }
+            __syncwarp();
+        } else {
+            // ------------------------------------------------ codes to operand tiles: 16 rows a step, four threads a row
+            const int t = threadIdx.x - 64, lr = t >> 2, q = t & 3;
+            constexpr int X = D / 64;  // 64-element blocks of a row
+            for (int p = 0; p < 2 * n; ++p) {
+                const int s = p % NS, o = p % NO;
+                int c;
+                bool value;
+                tile_of(p, n, a.streams, &c, &value);
+                if (!role_wait(&codes_full[s], (p / NS) & 1, abort_flag, a.wait_ns)) break;
+                if (p >= NO && !role_wait(&op_empty[o], (p / NO - 1) & 1, abort_flag, a.wait_ns)) break;
+                const uint32_t from = sbase + Sh::kOffStage + s * Sh::kCodes;
+                const uint32_t to = sbase + Sh::kOffOps + o * Sh::kOperand;
+                const uint32_t sc = sbase + Sh::kOffScales + ((w.c0 + c) % kChunks) * kGroups * 16;
+#pragma unroll 2
+                for (int i = 0; i < kGroups; ++i) {
+                    const int row = i * 16 + lr;
+                    const int rows = __float_as_int(lds_f4(sc + i * 16).w);
+#pragma unroll
+                    for (int x = 0; x < X; ++x) {
+                        // neighbouring rows at different blocks: both the loads and the stores miss each other's banks
+                        const int blk = X == 1 ? 0 : (x ^ (lr & 1));
+                        uint4 k = lds_u4(from + row * D + blk * 64 + q * 16);
+                        if (lr >= rows) k = make_uint4(0, 0, 0, 0);
+                        const uint32_t line = to + blk * 16384 + row * 128;
+                        sts_u4(line + (((2 * q) ^ (row & 7)) << 4), halves_of<CODE>(k.x, 0), halves_of<CODE>(k.x, 1),
+                               halves_of<CODE>(k.y, 0), halves_of<CODE>(k.y, 1));
+                        sts_u4(line + (((2 * q + 1) ^ (row & 7)) << 4), halves_of<CODE>(k.z, 0), halves_of<CODE>(k.z, 1),
+                               halves_of<CODE>(k.w, 0), halves_of<CODE>(k.w, 1));
+                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&op_full[o]);
+                    mbar_arrive(&codes_empty[s]);
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+    if (threadIdx.x == 0 && *abort_flag) atomicExch(a.status, LSA_ERR_TIMEOUT);
+}
+
+template <typename T, int CODE, int D> int launch(const QuantArgs& a, unsigned grid, cudaStream_t stream) {
+    if (!allow_kernel<quant_tile_kernel<T, CODE, D>>(QuantTile<D>::kSmem)) return LSA_ERR_CUDA;
+    return launch_after(quant_tile_kernel<T, CODE, D>, dim3(grid), kThreads, QuantTile<D>::kSmem, stream, a);
+}
+template <typename T> int launch(const QuantArgs& a, int code, int D, unsigned grid, cudaStream_t stream) {
+    if (code == kE4M3) return D == 128 ? launch<T, kE4M3, 128>(a, grid, stream) : launch<T, kE4M3, 64>(a, grid, stream);
+    return D == 128 ? launch<T, kInt8, 128>(a, grid, stream) : launch<T, kInt8, 64>(a, grid, stream);
+}
+
+}  // namespace
+
+int launch_quant_tiles(const QuantArgs& a, int dtype, int code, int D, cudaStream_t stream) {
+    const int64_t all = (int64_t)a.B * a.Hkv * a.tiles, items = a.whole + (all - a.whole) * a.parts;
+    if (items > INT32_MAX) return LSA_ERR_SIZE;
+    return dtype == kBF16 ? launch<__nv_bfloat16>(a, code, D, (unsigned)items, stream)
+                          : launch<__half>(a, code, D, (unsigned)items, stream);
+}
+
+}  // namespace lsa
