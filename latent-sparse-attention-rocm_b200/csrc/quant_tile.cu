@@ -394,17 +394,24 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tile_kernel(const QuantArgs
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;" ::: "memory");
         if (warp == 0) {
-            // ------------------------------------------------ codes and scales: a lane a page of the chunk
-            const int page = 1 << a.shift, pages = kChunk >> a.shift;
+            // ------------------------------------------------ codes and scales: a lane 16 keys of the chunk
+            // (whose page's rows the first lane of a page asks for). Page ids two chunks ahead, scales one.
+            const int page = 1 << a.shift, in_page = (lane * 16) & (page - 1);
             const int32_t* table = a.table + w.b * a.table_ld;
-            auto lookup = [&](int c) {  // page id of this lane's page of chunk c, -1: none
-                const int64_t slot = (int64_t)(w.c0 + c) * pages + lane;
+            auto lookup = [&](int c) {  // page id of this lane's keys of chunk c, -1: none
+                const int64_t key = (int64_t)(w.c0 + c) * kChunk + lane * 16;
                 int id = -1;
-                if (lane < pages && c < n && slot < a.M && (slot << a.shift) < w.keys) id = table[slot];
+                if (lane < kGroups && c < n && key < w.keys) id = table[key >> a.shift];
                 return id >= 0 && id < a.pages ? id : -1;
             };
-            // rows of chunk c's K are asked for up to two chunks ahead of its V's
-            int next = lookup(0), held[3] = {-1, -1, -1};
+            int id0 = lookup(0), id1 = lookup(1), held[3] = {-1, -1, -1};
+            float ks = 1.0f, vs = 1.0f;
+            auto scales = [&](int id) {
+                const int64_t head = (int64_t)(id < 0 ? 0 : id) * a.Hkv + w.h;
+                ks = id < 0 ? 1.0f : a.ks[head];
+                vs = id < 0 ? 1.0f : a.vs[head];
+            };
+            scales(id0);
             int p = 0;
             bool ok = true;
             for (; p < 2 * n; ++p) {
@@ -413,39 +420,30 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tile_kernel(const QuantArgs
                 int c;
                 bool value;
                 tile_of(p, n, a.streams, &c, &value);
-                int id;
-                if (!value) {
-                    id = next, next = lookup(c + 1);
-                    held[2] = c % 3 == 2 ? id : held[2], held[1] = c % 3 == 1 ? id : held[1], held[0] = c % 3 == 0 ? id : held[0];
-                } else {
-                    id = c % 3 == 0 ? held[0] : (c % 3 == 1 ? held[1] : held[2]);
-                }
-                const int left = w.keys - (w.c0 + c) * kChunk - lane * page;
-                const int rows = id < 0 || left <= 0 ? 0 : (left < page ? left : page);
+                const int id = !value ? id0 : (c % 3 == 0 ? held[0] : (c % 3 == 1 ? held[1] : held[2]));
+                const int left = id < 0 ? 0 : w.keys - (w.c0 + c) * kChunk - lane * 16;  // keys from the lane's first on
+                const int rows = left < 0 ? 0 : (left < 16 ? left : 16);
                 int total = rows;
 #pragma unroll
                 for (int off = 1; off < 8; off <<= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, off);
                 if (lane == 0) mbar_arrive_expect_tx(&codes_full[s], total * D);
                 __syncwarp();
                 const int64_t head = (int64_t)(id < 0 ? 0 : id) * a.Hkv + w.h;
-                if (rows > 0)
-                    bulk_g2s(sm + Sh::kOffStage + s * Sh::kCodes + lane * page * D,
-                             (value ? a.v8 : a.k8) + (head << a.shift) * D, rows * D, &codes_full[s]);
+                if (rows > 0 && in_page == 0)
+                    bulk_g2s(sm + Sh::kOffStage + s * Sh::kCodes + lane * 16 * D, (value ? a.v8 : a.k8) + (head << a.shift) * D,
+                             (left < page ? left : page) * D, &codes_full[s]);
                 if (!value) {
-                    // 16 keys a lane: their page's scales, and how many of them are there
-                    const int from = (lane & 7) * 16 >> a.shift;
-                    const int gid = __shfl_sync(0xFFFFFFFFu, id, from);
-                    int grows = __shfl_sync(0xFFFFFFFFu, rows, from) - ((lane & 7) * 16 & (page - 1));
-                    grows = gid < 0 || grows < 0 ? 0 : (grows < 16 ? grows : 16);
-                    float4 k = make_float4(1.0f, -INFINITY, 0.0f, 0.0f);
-                    if (lane < kGroups && grows > 0) {
-                        const int64_t gh = (int64_t)gid * a.Hkv + w.h;
-                        const float vs = fmaxf(a.vs[gh], 8.6736174e-19f);  // 2^-60
-                        k = make_float4(a.ks[gh], log2f(vs), 1.0f / vs, __int_as_float(grows));
+                    held[2] = c % 3 == 2 ? id : held[2], held[1] = c % 3 == 1 ? id : held[1], held[0] = c % 3 == 0 ? id : held[0];
+                    if (lane < kGroups) {
+                        const float v = fmaxf(vs, 8.6736174e-19f);  // 2^-60
+                        *reinterpret_cast<float4*>(sm + Sh::kOffScales + (((w.c0 + c) % kChunks) * kGroups + lane) * 16) =
+                            rows > 0 ? make_float4(ks, log2f(v), 1.0f / v, __int_as_float(rows))
+                                     : make_float4(1.0f, -INFINITY, 0.0f, 0.0f);
                     }
-                    if (lane < kGroups)
-                        *reinterpret_cast<float4*>(sm + Sh::kOffScales + (((w.c0 + c) % kChunks) * kGroups + lane) * 16) = k;
                     __syncwarp();
+                    id0 = id1;
+                    scales(id0);
+                    id1 = lookup(c + 2);
                 }
                 if (lane == 0) mbar_arrive(&codes_full[s]);
             }
@@ -561,21 +559,33 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tile_kernel(const QuantArgs
                 const uint32_t from = sbase + Sh::kOffStage + s * Sh::kCodes;
                 const uint32_t to = sbase + Sh::kOffOps + o * Sh::kOperand;
                 const uint32_t sc = sbase + Sh::kOffScales + ((w.c0 + c) % kChunks) * kGroups * 16;
-#pragma unroll 2
-                for (int i = 0; i < kGroups; ++i) {
-                    const int row = i * 16 + lr;
-                    const int rows = __float_as_int(lds_f4(sc + i * 16).w);
+                const int rows = __float_as_int(lds_f4(sc + (lane & 7) * 16).w);  // of 16 keys a lane
+                const bool whole = __all_sync(0xFFFFFFFFu, rows == 16);
+                // neighbouring rows at different blocks: both the loads and the stores miss each other's banks
+                const int x0 = X == 1 ? 0 : (lr & 1);
+                const uint32_t src = from + lr * D + q * 16 + x0 * 64, dst = to + lr * 128 + x0 * 16384;
+                const uint32_t ca = ((2 * q) ^ (lr & 7)) << 4, cb = ((2 * q + 1) ^ (lr & 7)) << 4;
 #pragma unroll
-                    for (int x = 0; x < X; ++x) {
-                        // neighbouring rows at different blocks: both the loads and the stores miss each other's banks
-                        const int blk = X == 1 ? 0 : (x ^ (lr & 1));
-                        uint4 k = lds_u4(from + row * D + blk * 64 + q * 16);
-                        if (lr >= rows) k = make_uint4(0, 0, 0, 0);
-                        const uint32_t line = to + blk * 16384 + row * 128;
-                        sts_u4(line + (((2 * q) ^ (row & 7)) << 4), halves_of<CODE>(k.x, 0), halves_of<CODE>(k.x, 1),
-                               halves_of<CODE>(k.y, 0), halves_of<CODE>(k.y, 1));
-                        sts_u4(line + (((2 * q + 1) ^ (row & 7)) << 4), halves_of<CODE>(k.z, 0), halves_of<CODE>(k.z, 1),
-                               halves_of<CODE>(k.w, 0), halves_of<CODE>(k.w, 1));
+                for (int i = 0; i < kGroups; i += 4 / X) {
+                    uint4 k[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const int x = X == 1 ? 0 : u & 1, gi = i + u / X;
+                        k[u] = lds_u4(src + gi * 16 * D + (x ? 64 - 128 * x0 : 0));
+                    }
+                    if (!whole) {
+#pragma unroll
+                        for (int u = 0; u < 4; ++u)
+                            if (lr >= __shfl_sync(0xFFFFFFFFu, rows, i + u / X)) k[u] = make_uint4(0, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const int x = X == 1 ? 0 : u & 1, gi = i + u / X;
+                        const uint32_t line = dst + gi * 2048 + (x ? 16384 - 32768 * x0 : 0);
+                        sts_u4(line + ca, halves_of<CODE>(k[u].x, 0), halves_of<CODE>(k[u].x, 1), halves_of<CODE>(k[u].y, 0),
+                               halves_of<CODE>(k[u].y, 1));
+                        sts_u4(line + cb, halves_of<CODE>(k[u].z, 0), halves_of<CODE>(k[u].z, 1), halves_of<CODE>(k[u].w, 0),
+                               halves_of<CODE>(k[u].w, 1));
                     }
                 }
                 fence_proxy_async_smem();
