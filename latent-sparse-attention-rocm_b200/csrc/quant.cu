@@ -11,7 +11,7 @@ namespace {
 constexpr int kSMs = 148;
 constexpr int kFewRows = 16;  // rows of the few-row kernel's tiles
 constexpr int kUnit = 128;      // keys that a CTA's four warps take at a time
-constexpr int kMostCluster = 16;
+constexpr int64_t kFewKeys = 1 << 17;  // (key, head) pairs that the few-row kernel reads up to four times
 constexpr int kMaxTileParts = 32, kMostRounds = 8;  // splits of a tile; rounds of the SMs that split tiles fill
 constexpr double kItemCost = 1.5, kJoinCost = 3.0;  // a CTA's start and end, the join's launch, in units' times
 
@@ -30,7 +30,11 @@ Plan make_plan(int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_
     const int64_t G = Hq / Hkv, chunks = (keys + kUnit - 1) / kUnit;
     p.part_rows = B * Tq * Hq;
     p.parts = 1;
-    if (Tq * G > kFewRows && G <= 128) {
+    // The few-row kernel reads the keys once for each 16 rows, from L2 after the first time, and converts them in
+    // registers; the tensor-core kernel's converting goes through shared memory, which its products share, and its start
+    // takes 5 us (32 x 4096 keys: 20-32 rows 94 against 140 us, 48 rows 159 against 143, 64 rows 183 against 145; 4 x 2048:
+    // 48 rows 19.7 against 21.7; 16 x 2048: 58 against 46).
+    if (Tq * G > (B * Hkv * keys <= kFewKeys ? 64 : 32) && G <= 128) {
         // Whole rounds of one tile an SM are not split (no parts to write, read and join); the tiles of the last, short
         // round are, so that it too fills the GPU.
         p.tokens = (int)(128 / G);
@@ -54,7 +58,8 @@ Plan make_plan(int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_
     // Parts that are a cluster's CTAs join within the launch, which pays where all clusters run at once (4 x 2k keys:
     // 10.3 us against 12.0 with a second launch); where CTAs wait for a place, a cluster waits for all of its own
     // (64 x 8k: 145 against 138 us; 32 lists of 2116: 51 against 43).
-    for (int c = 2; c <= kMostCluster && c / 2 < chunks && items * c <= places; c *= 2)
+    // A cluster of 16 takes most of a GPC: one CTA an SM then (16 of them on two an SM: 33 us, in 18 parts 24).
+    for (int c = 2; c <= kMostCluster && c / 2 < chunks && items * c <= (c > 8 ? kSMs : places); c *= 2)
         if (cost(c) < 0.99 * cost(p.parts)) p.parts = c, p.cluster = true;
     const int s = balance(items, chunks, kItemCost, places, kMaxQuantParts);
     if (s > 1 && cost(s) + kJoinCost < cost(p.parts)) p.parts = s, p.cluster = false;

@@ -24,6 +24,7 @@ enum Code : int { kE4M3 = 0, kInt8 = 1 };
 
 constexpr int kMinExponent = -60;  // of a scale that the append writes
 constexpr int kMaxQuantParts = 96;
+constexpr int kMostCluster = 16;
 
 struct QuantArgs {
     const void* q;

@@ -511,15 +511,20 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) quant_rows_kerne
     for (int i = split * kWarps * 32 + threadIdx.x; i < live * (D / 4); i += a.parts * kWarps * 32) {
         const int r = i / (D / 4), col = i % (D / 4) * 4;
         float top = -INFINITY, total = 0.0f;
-        float4 x = make_float4(0, 0, 0, 0);
-        for (int p = 0; p < a.parts; ++p) top = fmaxf(top, peer_f2(stats + r * 8, p).x);
-#pragma unroll 4
-        for (int p = 0; p < a.parts; ++p) {
-            const float2 ml = peer_f2(stats + r * 8, p);
-            const float4 y = peer_f4(base + (r * D + col) * 4, p);
-            const float f = ml.y == 0.0f ? 0.0f : exp2f(ml.x - top);
-            total = fmaf(f, ml.y, total);
-            x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w);
+        float4 x = make_float4(0, 0, 0, 0), y[kMostCluster];
+        float2 ml[kMostCluster];
+#pragma unroll
+        for (int p = 0; p < kMostCluster; ++p) {
+            ml[p] = make_float2(-INFINITY, 0.0f), y[p] = x;
+            if (p < a.parts) ml[p] = peer_f2(stats + r * 8, p), y[p] = peer_f4(base + (r * D + col) * 4, p);
+        }
+#pragma unroll
+        for (int p = 0; p < kMostCluster; ++p) top = fmaxf(top, ml[p].x);
+#pragma unroll
+        for (int p = 0; p < kMostCluster; ++p) {
+            const float f = ml[p].y == 0.0f ? 0.0f : exp2f(ml[p].x - top);
+            total = fmaf(f, ml[p].y, total);
+            x.x = fmaf(f, y[p].x, x.x), x.y = fmaf(f, y[p].y, x.y), x.z = fmaf(f, y[p].z, x.z), x.w = fmaf(f, y[p].w, x.w);
         }
         const float norm = total == 0.0f ? 0.0f : 1.0f / total;
         const int64_t rid = row_id(r);

@@ -37,15 +37,19 @@ constexpr int kGroups = kChunk / 16;
 template <int D> struct QuantTile {
     static constexpr int kOperand = kChunk * D * 2;  // an fp16 K, V or half-Q tile
     static constexpr int kCodes = kChunk * D;        // its codes
-    static constexpr int kOps = D == 128 ? 3 : 6, kStages = D == 128 ? 3 : 5;
+    // Operand tiles and tiles of codes. A tile of one half's rows has the other half of Q for two more (D = 64: four).
+    static constexpr int kOps = D == 128 ? 3 : 6, kStages = D == 128 ? 4 : 5, kMore = kOperand / kCodes;
     static constexpr int kOffOps = 2 * kOperand;
     static constexpr int kOffStage = kOffOps + kOps * kOperand;
     static constexpr int kOffScales = kOffStage + kStages * kCodes;  // [kChunks][kGroups] (ks, log2 vs, 1 / vs, rows)
     static constexpr int kOffFactor = kOffScales + kChunks * kGroups * 16;
     static constexpr int kOffBar = kOffFactor + 256 * 4;
-    static constexpr int kNumBars = 2 * kStages + 2 * kOps + 2 + 4 + 2 + 1;
+    static constexpr int kNumBars = 2 * (kStages + kMore) + 2 * kOps + 2 + 4 + 2 + 1;
     static constexpr int kOffMisc = kOffBar + kNumBars * 8;
-    static constexpr int kSmem = kOffMisc + 16 + 1024;  // slack: the base is aligned to 1024 B
+    static constexpr int kSmem = kOffMisc + 16;
+    static __device__ __forceinline__ int codes_at(int s) {
+        return s < kStages ? kOffStage + s * kCodes : kOperand + (s - kStages) * kCodes;
+    }
     static_assert(kSmem <= 232448, "shared memory of a CTA");
     static_assert(kOffStage >= 256 * (D * 4 + 16), "the rows leave through Q and the operand ring");
 };
@@ -181,7 +185,7 @@ __device__ __forceinline__ void softmax_half(const QuantArgs& a, const Item& w, 
     const uint32_t tO = tmem + lanes + 256 + hf * 128;
     const int step = a.streams ? 2 : 1, first = w.c0 + (a.streams ? hf : 0);
     const int n = w.c1 > first ? (w.c1 - first + step - 1) / step : 0;
-    const uint32_t scales = smem_u32(sm) + Sh::kOffScales;
+    const float4* const scales = reinterpret_cast<const float4*>(sm + Sh::kOffScales);
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
     auto publish = [&](uint64_t* bar) {  // this warp's P so far: one arrival a warp
@@ -196,7 +200,7 @@ __device__ __forceinline__ void softmax_half(const QuantArgs& a, const Item& w, 
         ok = role_wait(&bar_s[hf], j & 1, abort_flag, a.wait_ns);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t sc = scales + (c % kChunks) * kGroups * 16;
+        const float4* const sc = scales + (c % kChunks) * kGroups;
         uint32_t s[128];
         tmem_ld128_wait(tS, s);
         if (__any_sync(0xFFFFFFFFu, seen < kChunk)) {
@@ -211,7 +215,7 @@ __device__ __forceinline__ void softmax_half(const QuantArgs& a, const Item& w, 
         uint64_t sum;
         // logits of 16 keys from s: (multiplier, addend); the multiplier stays above 0, so that -inf does
         auto group = [&](int i, float* mul, float* add) {
-            const float4 k = lds_f4(sc + i * 16);
+            const float4 k = sc[i];
             *mul = fmaxf(k.x * factor, 1e-30f), *add = k.y;
             return k.z;
         };
@@ -346,19 +350,19 @@ __device__ __forceinline__ void softmax_half(const QuantArgs& a, const Item& w, 
 template <typename T, int CODE, int D>
 __global__ void __launch_bounds__(kThreads, 1) quant_tile_kernel(const QuantArgs a) {
     using Sh = QuantTile<D>;
-    constexpr int NS = Sh::kStages, NO = Sh::kOps, KS = D / 16;
-    extern __shared__ uint8_t raw[];
-    uint8_t* sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+    constexpr int NO = Sh::kOps, KS = D / 16, kAll = Sh::kStages + Sh::kMore;
+    extern __shared__ __align__(1024) uint8_t sm[];
+    const int NS = a.streams ? kAll : Sh::kStages;
     const uint32_t sbase = smem_u32(sm);
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Sh::kOffBar);
-    uint64_t *codes_full = bars, *codes_empty = bars + NS, *op_full = bars + 2 * NS, *op_empty = op_full + NO,
+    uint64_t *codes_full = bars, *codes_empty = bars + kAll, *op_full = bars + 2 * kAll, *op_empty = op_full + NO,
              *bar_s = op_empty + NO, *bar_p = bar_s + 2, *bar_o = bar_p + 4, *bar_drain = bar_o + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + Sh::kOffMisc);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + Sh::kOffMisc + 4);
     const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if (warp == 1) tmem_alloc(tmem_slot, 512);
     if (threadIdx.x == 0) {
-        for (int s = 0; s < NS; ++s) {
+        for (int s = 0; s < kAll; ++s) {
             mbar_init(&codes_full[s], 2);   // the bytes, and the scales beside them
             mbar_init(&codes_empty[s], 2);  // the converting warps
         }
@@ -380,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tile_kernel(const QuantArgs
     grid_trigger();
     const Item w = item_of(a);
     const int n = w.c1 - w.c0;
-    if (n > 0) load_q<T, D>(a, w, sm);
+    load_q<T, D>(a, w, sm);  // whether or not it has keys: its loads go out beside the lengths'
     fence_proxy_async_smem();
     tc_fence_before();
     __syncthreads();
@@ -388,11 +392,11 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tile_kernel(const QuantArgs
     const uint32_t tmem = *tmem_slot;
 
     if (warp >= 4) {
-        // 384 threads launch at 168 registers: 128 x 56 + 256 x 224 = 384 x 168
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;" ::: "memory");
+        // 384 threads launch at 168 registers: 128 x 72 + 256 x 216 = 384 x 168
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;" ::: "memory");
         softmax_half<T, D>(a, w, sm, bar_s, bar_p, bar_o, abort_flag, tmem);
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;" ::: "memory");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;" ::: "memory");
         if (warp == 0) {
             // ------------------------------------------------ codes and scales: a lane 16 keys of the chunk
             // (whose page's rows the first lane of a page asks for). Page ids two chunks ahead, scales one.
@@ -414,9 +418,9 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tile_kernel(const QuantArgs
             scales(id0);
             int p = 0;
             bool ok = true;
-            for (; p < 2 * n; ++p) {
-                const int s = p % NS;
-                if (p >= NS && !(ok = role_wait(&codes_empty[s], (p / NS - 1) & 1, abort_flag, a.wait_ns))) break;
+            int s = 0, round = 0;
+            for (; p < 2 * n; ++p, s = s + 1 == NS ? 0 : s + 1, round += s == 0) {
+                if (round > 0 && !(ok = role_wait(&codes_empty[s], (round - 1) & 1, abort_flag, a.wait_ns))) break;
                 int c;
                 bool value;
                 tile_of(p, n, a.streams, &c, &value);
@@ -430,7 +434,7 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tile_kernel(const QuantArgs
                 __syncwarp();
                 const int64_t head = (int64_t)(id < 0 ? 0 : id) * a.Hkv + w.h;
                 if (rows > 0 && in_page == 0)
-                    bulk_g2s(sm + Sh::kOffStage + s * Sh::kCodes + lane * 16 * D, (value ? a.v8 : a.k8) + (head << a.shift) * D,
+                    bulk_g2s(sm + Sh::codes_at(s) + lane * 16 * D, (value ? a.v8 : a.k8) + (head << a.shift) * D,
                              (left < page ? left : page) * D, &codes_full[s]);
                 if (!value) {
                     held[2] = c % 3 == 2 ? id : held[2], held[1] = c % 3 == 1 ? id : held[1], held[0] = c % 3 == 0 ? id : held[0];
@@ -549,14 +553,15 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tile_kernel(const QuantArgs
             // ------------------------------------------------ codes to operand tiles: 16 rows a step, four threads a row
             const int t = threadIdx.x - 64, lr = t >> 2, q = t & 3;
             constexpr int X = D / 64;  // 64-element blocks of a row
-            for (int p = 0; p < 2 * n; ++p) {
-                const int s = p % NS, o = p % NO;
+            int s = 0, round = 0;
+            for (int p = 0; p < 2 * n; ++p, s = s + 1 == NS ? 0 : s + 1, round += s == 0) {
+                const int o = p % NO;
                 int c;
                 bool value;
                 tile_of(p, n, a.streams, &c, &value);
-                if (!role_wait(&codes_full[s], (p / NS) & 1, abort_flag, a.wait_ns)) break;
+                if (!role_wait(&codes_full[s], round & 1, abort_flag, a.wait_ns)) break;
                 if (p >= NO && !role_wait(&op_empty[o], (p / NO - 1) & 1, abort_flag, a.wait_ns)) break;
-                const uint32_t from = sbase + Sh::kOffStage + s * Sh::kCodes;
+                const uint32_t from = sbase + Sh::codes_at(s);
                 const uint32_t to = sbase + Sh::kOffOps + o * Sh::kOperand;
                 const uint32_t sc = sbase + Sh::kOffScales + ((w.c0 + c) % kChunks) * kGroups * 16;
                 const int rows = __float_as_int(lds_f4(sc + (lane & 7) * 16).w);  // of 16 keys a lane
@@ -565,27 +570,30 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tile_kernel(const QuantArgs
                 const int x0 = X == 1 ? 0 : (lr & 1);
                 const uint32_t src = from + lr * D + q * 16 + x0 * 64, dst = to + lr * 128 + x0 * 16384;
                 const uint32_t ca = ((2 * q) ^ (lr & 7)) << 4, cb = ((2 * q + 1) ^ (lr & 7)) << 4;
-#pragma unroll
-                for (int i = 0; i < kGroups; i += 4 / X) {
-                    uint4 k[4];
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const int x = X == 1 ? 0 : u & 1, gi = i + u / X;
-                        k[u] = lds_u4(src + gi * 16 * D + (x ? 64 - 128 * x0 : 0));
-                    }
-                    if (!whole) {
-#pragma unroll
-                        for (int u = 0; u < 4; ++u)
-                            if (lr >= __shfl_sync(0xFFFFFFFFu, rows, i + u / X)) k[u] = make_uint4(0, 0, 0, 0);
-                    }
+                // four loads are on their way while the four before them are converted and stored
+                constexpr int BATCHES = kGroups * X / 4;
+                uint4 k[2][4];
+                auto fetch = [&](int i) {
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
-                        const int x = X == 1 ? 0 : u & 1, gi = i + u / X;
+                        const int x = X == 1 ? 0 : u & 1, gi = i * (4 / X) + u / X;
+                        k[i & 1][u] = lds_u4(src + gi * 16 * D + (x ? 64 - 128 * x0 : 0));
+                    }
+                };
+                fetch(0);
+#pragma unroll
+                for (int i = 0; i < BATCHES; ++i) {
+                    if (i + 1 < BATCHES) fetch(i + 1);
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const int x = X == 1 ? 0 : u & 1, gi = i * (4 / X) + u / X;
+                        uint4& w4 = k[i & 1][u];
+                        if (!whole && lr >= __shfl_sync(0xFFFFFFFFu, rows, gi)) w4 = make_uint4(0, 0, 0, 0);
                         const uint32_t line = dst + gi * 2048 + (x ? 16384 - 32768 * x0 : 0);
-                        sts_u4(line + ca, halves_of<CODE>(k[u].x, 0), halves_of<CODE>(k[u].x, 1), halves_of<CODE>(k[u].y, 0),
-                               halves_of<CODE>(k[u].y, 1));
-                        sts_u4(line + cb, halves_of<CODE>(k[u].z, 0), halves_of<CODE>(k[u].z, 1), halves_of<CODE>(k[u].w, 0),
-                               halves_of<CODE>(k[u].w, 1));
+                        sts_u4(line + ca, halves_of<CODE>(w4.x, 0), halves_of<CODE>(w4.x, 1), halves_of<CODE>(w4.y, 0),
+                               halves_of<CODE>(w4.y, 1));
+                        sts_u4(line + cb, halves_of<CODE>(w4.z, 0), halves_of<CODE>(w4.z, 1), halves_of<CODE>(w4.w, 0),
+                               halves_of<CODE>(w4.w, 1));
                     }
                 }
                 fence_proxy_async_smem();
