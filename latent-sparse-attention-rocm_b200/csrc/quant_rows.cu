@@ -152,6 +152,18 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) quant_rows_kerne
     const int h = item % a.Hkv, b = item / a.Hkv;
     const int nrows = a.Tq * a.G;
     const int live = nrows - r0 < kRows ? nrows - r0 : kRows;
+    // Q's rows are asked for before what the lengths say is known: row r0 + g (and + 8); k-step kk's four values of a
+    // lane are D's 16 (c + 4 (kk / 4)) + 4 (kk % 4) + 0..3
+    uint2 raw[NT][KS];
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+        const int r = r0 + g + 8 * u, tok = r / a.G;
+        const T* src = static_cast<const T*>(a.q) + b * a.q_b + tok * a.q_t + (h * (int64_t)a.G + r - tok * a.G) * a.q_h;
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk)
+            raw[u][kk] = r < nrows ? *reinterpret_cast<const uint2*>(src + 16 * (c + 4 * (kk >> 2)) + 4 * (kk & 3))
+                                   : make_uint2(0, 0);
+    }
     // keys: positions of the sequence, or entries of the list
     int trow = b, length, keys;
     if (LISTS) {
@@ -249,27 +261,18 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) quant_rows_kerne
 #pragma unroll
     for (int i = 0; i < Sh::kRing - 1; ++i) copy(i);
 
-    // Q fragments: row r0 + g (and + 8); k-step kk's four values of a lane are D's
-    // 16 (c + 4 (kk / 4)) + 4 (kk % 4) + 0..3
+    // Q's fragments, as halves
     uint32_t qf[NT][KS][2];
     uint64_t factor[NT];  // of rows r0 + 2c and 2c + 1 (and + 8), as the maxima and sums below
     int limit[NT][2];
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
-        const int r = r0 + g + 8 * u;
-        const int tok = r / a.G;
-        const T* src = static_cast<const T*>(a.q) + b * a.q_b + tok * a.q_t + (h * (int64_t)a.G + r - tok * a.G) * a.q_h;
-        uint2 raw[KS];
-#pragma unroll
-        for (int kk = 0; kk < KS; ++kk)
-            raw[kk] = r < nrows ? *reinterpret_cast<const uint2*>(src + 16 * (c + 4 * (kk >> 2)) + 4 * (kk & 3))
-                                : make_uint2(0, 0);
         float f = a.scale_log2;
         if constexpr (std::is_same<T, __nv_bfloat16>::value) {
             uint32_t top = 0;  // largest magnitude's bits, as a bf16
 #pragma unroll
             for (int kk = 0; kk < KS; ++kk) {
-                const uint32_t w[2] = {raw[kk].x, raw[kk].y};
+                const uint32_t w[2] = {raw[u][kk].x, raw[u][kk].y};
 #pragma unroll
                 for (int e = 0; e < 2; ++e) top = max(top, max(w[e] & 0x7FFFu, (w[e] >> 16) & 0x7FFFu));
             }
@@ -278,12 +281,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) quant_rows_kerne
             const float by = half_factor(top, &f);
 #pragma unroll
             for (int kk = 0; kk < KS; ++kk) {
-                qf[u][kk][0] = pack_half(__uint_as_float(raw[kk].x << 16) * by, __uint_as_float(raw[kk].x & 0xFFFF0000u) * by);
-                qf[u][kk][1] = pack_half(__uint_as_float(raw[kk].y << 16) * by, __uint_as_float(raw[kk].y & 0xFFFF0000u) * by);
+                qf[u][kk][0] = pack_half(__uint_as_float(raw[u][kk].x << 16) * by, __uint_as_float(raw[u][kk].x & 0xFFFF0000u) * by);
+                qf[u][kk][1] = pack_half(__uint_as_float(raw[u][kk].y << 16) * by, __uint_as_float(raw[u][kk].y & 0xFFFF0000u) * by);
             }
         } else {
 #pragma unroll
-            for (int kk = 0; kk < KS; ++kk) qf[u][kk][0] = raw[kk].x, qf[u][kk][1] = raw[kk].y;
+            for (int kk = 0; kk < KS; ++kk) qf[u][kk][0] = raw[u][kk].x, qf[u][kk][1] = raw[u][kk].y;
         }
         factor[u] = pair(__shfl_sync(0xFFFFFFFFu, f, 8 * c), __shfl_sync(0xFFFFFFFFu, f, 8 * c + 4));
 #pragma unroll
@@ -508,7 +511,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) quant_rows_kerne
     // A cluster holds all parts of its rows: they join through its CTAs' shared memory, a part of the columns each.
     cluster_sync();
     const uint32_t base = smem_u32(smem), stats = smem_u32(joined);
-    for (int i = split * kWarps * 32 + threadIdx.x; i < live * (D / 4); i += a.parts * kWarps * 32) {
+    for (int i = threadIdx.x * a.parts + split; i < live * (D / 4); i += a.parts * kWarps * 32) {
         const int r = i / (D / 4), col = i % (D / 4) * 4;
         float top = -INFINITY, total = 0.0f;
         float4 x = make_float4(0, 0, 0, 0), y[kMostCluster];
