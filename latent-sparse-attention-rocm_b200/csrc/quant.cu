@@ -69,7 +69,8 @@ Plan make_plan(int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_
 
 bool sizes_ok(int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_t keys) {
     if (B < 0 || Tq < 0 || keys < 0 || Hkv < 1 || Hq < 1 || Hq % Hkv != 0 || (D != 64 && D != 128)) return false;
-    if (B > INT32_MAX || Tq > (1 << 24) || Hq > 65536 || keys > (1 << 30)) return false;
+    if (B > 65535 || Tq > (1 << 24) || Hq > 65536 || keys > (1 << 30)) return false;
+    if (Tq * (Hq / Hkv) > (1 << 30) || Tq * (Hq / Hkv) * (Hq / Hkv) > UINT32_MAX) return false;  // token_of
     return B * Tq <= (int64_t)INT32_MAX / Hq;
 }
 
@@ -97,6 +98,7 @@ int run(QuantArgs& a, int dtype, int code, int64_t D, int64_t keys, float scale,
     if (!(a.scale_log2 > 0) || !isfinite(a.scale_log2)) return LSA_ERR_ARG;
     if (reinterpret_cast<uintptr_t>(a.q) % 16 != 0 || reinterpret_cast<uintptr_t>(a.out) % 16 != 0) return LSA_ERR_ARG;
     if (a.q_b % 8 != 0 || a.q_t % 8 != 0 || a.q_h % 8 != 0) return LSA_ERR_ARG;
+    a.G_inverse = a.G > 1 ? (uint32_t)(((1ull << 32) + a.G - 1) / a.G) : 0;
     const Plan p = make_plan(a.B, a.Tq, a.Hq, a.Hkv, D, keys);
     if (p.bytes > 0 && (scratch == nullptr || scratch_bytes < p.bytes || reinterpret_cast<uintptr_t>(scratch) % 16 != 0))
         return LSA_ERR_ARG;

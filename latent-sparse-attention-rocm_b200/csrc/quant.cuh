@@ -41,6 +41,7 @@ struct QuantArgs {
     float *part_o, *part_lse;     // [parts][rows][D] (normalised), [parts][rows] (log2 domain; -inf: no key)
     float* lse;                   // [rows] natural, or null
     int B, Tq, Hq, Hkv, G;
+    uint32_t G_inverse;           // ceil(2^32 / G); 0 for G = 1
     int parts;
     bool cluster;                 // the parts are a cluster's CTAs, which join them (few-row kernel)
     int64_t rows;                 // B * Tq * Hq
@@ -107,6 +108,11 @@ __device__ __forceinline__ float half_factor(uint32_t top, float* factor) {
     const int up = e == 0 || e == 255 ? 0 : min(8 - (e - 127), 100);
     *factor *= __uint_as_float((uint32_t)(127 - up) << 23);
     return __uint_as_float((uint32_t)(up + 127) << 23);
+}
+
+// Token of row r of a (sequence, KV head), r < Tq G: r / G, exact for r G below 2^32 (the entry point checks).
+__device__ __forceinline__ int token_of(const QuantArgs& a, int r) {
+    return a.G_inverse ? (int)__umulhi((uint32_t)r, a.G_inverse) : r;
 }
 
 // Tile i of the tensor-core kernel: (sequence, KV head, row tile), the longest causal ranges first.

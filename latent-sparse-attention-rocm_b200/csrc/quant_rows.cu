@@ -144,12 +144,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) quant_rows_kerne
     const int g = lane >> 2, c = lane & 3;
     grid_wait();
     grid_trigger();
-    int item = blockIdx.x;
-    const int split = item % a.parts;
-    item /= a.parts;
-    const int r0 = item % row_tiles * kRows;
-    item /= row_tiles;
-    const int h = item % a.Hkv, b = item / a.Hkv;
+    // (parts, KV heads x row tiles, sequences)
+    const int split = blockIdx.x, b = blockIdx.z;
+    const int h = row_tiles == 1 ? (int)blockIdx.y : (int)blockIdx.y / row_tiles;
+    const int r0 = ((int)blockIdx.y - h * row_tiles) * kRows;
     const int nrows = a.Tq * a.G;
     const int live = nrows - r0 < kRows ? nrows - r0 : kRows;
     // Q's rows are asked for before what the lengths say is known: row r0 + g (and + 8); k-step kk's four values of a
@@ -157,7 +155,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) quant_rows_kerne
     uint2 raw[NT][KS];
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
-        const int r = r0 + g + 8 * u, tok = r / a.G;
+        const int r = r0 + g + 8 * u, tok = token_of(a, r);
         const T* src = static_cast<const T*>(a.q) + b * a.q_b + tok * a.q_t + (h * (int64_t)a.G + r - tok * a.G) * a.q_h;
 #pragma unroll
         for (int kk = 0; kk < KS; ++kk)
@@ -175,7 +173,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) quant_rows_kerne
         keys = !ok || keys < 0 ? 0 : (keys > a.W ? a.W : keys);
     } else {
         length = max(a.lengths[b], 0);
-        keys = length - a.Tq + (r0 + live - 1) / a.G + 1;  // that the tile's last row sees
+        keys = length - a.Tq + token_of(a, r0 + live - 1) + 1;  // that the tile's last row sees
         const int64_t room = (int64_t)a.M << a.shift;
         keys = keys < 0 ? 0 : (keys > room ? (int)room : keys);
     }
@@ -258,9 +256,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) quant_rows_kerne
         if (++slot == Sh::kRing) slot = 0;
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-#pragma unroll
-    for (int i = 0; i < Sh::kRing - 1; ++i) copy(i);
-
     // Q's fragments, as halves
     uint32_t qf[NT][KS][2];
     uint64_t factor[NT];  // of rows r0 + 2c and 2c + 1 (and + 8), as the maxima and sums below
@@ -292,10 +287,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) quant_rows_kerne
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const int row = r0 + 8 * u + 2 * c + e;
-            limit[u][e] = row >= nrows ? 0 : length - a.Tq + row / a.G + 1;
+            limit[u][e] = row >= nrows ? 0 : length - a.Tq + token_of(a, row) + 1;
         }
     }
-    const int first_limit = length - a.Tq + r0 / a.G + 1;  // keys that the tile's first row sees
+    const int first_limit = length - a.Tq + token_of(a, r0) + 1;  // keys that the tile's first row sees
     float o[NT][MT][4];  // O^T: columns (D / 8) g + 2 j (0, 1) and + 1 (2, 3) of rows 2c (0, 2) and 2c + 1 (1, 3)
 #pragma unroll
     for (int u = 0; u < NT; ++u)
@@ -309,8 +304,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) quant_rows_kerne
     for (int u = 0; u < NT; ++u) m[u][0] = m[u][1] = -INFINITY, l[u] = 0ull;
 
     uint32_t read = 0;  // slot of tile i
-    for (int i = 0; i < tiles; ++i) {
+    // one copy of the code that copies: a launch starts with it cold
+#pragma unroll 1
+    for (int i = 1 - Sh::kRing; i < tiles; ++i) {
         copy(i + Sh::kRing - 1);
+        if (i < 0) continue;
         asm volatile("cp.async.wait_group %0;" ::"n"(Sh::kRing - 1) : "memory");
         const uint32_t ks = ring + read * Sh::kStage, vs = ks + Sh::kTile, scales = vs + Sh::kTile;
         if (++read == Sh::kRing) read = 0;
@@ -469,7 +467,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) quant_rows_kerne
         }
     __syncthreads();
     auto row_id = [&](int r) {
-        const int tok = (r0 + r) / a.G;
+        const int tok = token_of(a, r0 + r);
         return ((int64_t)b * a.Tq + tok) * a.Hq + (int64_t)h * a.G + (r0 + r - tok * a.G);
     };
     float2* joined = sml + kWarps * kRows;  // the CTA's (maximum, sum) of a row
@@ -483,7 +481,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) quant_rows_kerne
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
             const float2 ml = sml[w * kRows + r];
-            const float f = ml.y == 0.0f ? 0.0f : exp2f(ml.x - top);  // NaN passes on
+            const float f = ml.y == 0.0f ? 0.0f : ex2_approx(ml.x - top);  // NaN passes on
             const float4 y = *reinterpret_cast<const float4*>(smem + w * Sh::kWarpBytes + (r * D + col) * 4);
             total = fmaf(f, ml.y, total);
             x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w);
@@ -525,7 +523,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) quant_rows_kerne
         for (int p = 0; p < kMostCluster; ++p) top = fmaxf(top, ml[p].x);
 #pragma unroll
         for (int p = 0; p < kMostCluster; ++p) {
-            const float f = ml[p].y == 0.0f ? 0.0f : exp2f(ml[p].x - top);
+            const float f = ml[p].y == 0.0f ? 0.0f : ex2_approx(ml[p].x - top);
             total = fmaf(f, ml[p].y, total);
             x.x = fmaf(f, y[p].x, x.x), x.y = fmaf(f, y[p].y, x.y), x.z = fmaf(f, y[p].z, x.z), x.w = fmaf(f, y[p].w, x.w);
         }
@@ -630,21 +628,21 @@ __global__ void __launch_bounds__(256) quant_join_kernel(const QuantArgs a, cons
 }
 
 template <typename T, int CODE, int D, bool LISTS, int NT>
-int launch(const QuantArgs& a, int row_tiles, unsigned grid, cudaStream_t stream) {
+int launch(const QuantArgs& a, int row_tiles, dim3 grid, cudaStream_t stream) {
     constexpr int smem = QuantShape<D, NT>::kSmem;
     if (!allow_kernel<quant_rows_kernel<T, CODE, D, LISTS, NT>>(smem, true)) return LSA_ERR_CUDA;
-    return launch_clusters(quant_rows_kernel<T, CODE, D, LISTS, NT>, dim3(grid), kWarps * 32, smem, stream,
+    return launch_clusters(quant_rows_kernel<T, CODE, D, LISTS, NT>, grid, kWarps * 32, smem, stream,
                            a.cluster ? a.parts : 1, a, row_tiles);
 }
 template <typename T, int CODE, int D>
-int launch(const QuantArgs& a, int row_tiles, unsigned grid, cudaStream_t stream) {
+int launch(const QuantArgs& a, int row_tiles, dim3 grid, cudaStream_t stream) {
     if (a.Tq * a.G <= 8)
         return a.lists ? launch<T, CODE, D, true, 1>(a, row_tiles, grid, stream)
                        : launch<T, CODE, D, false, 1>(a, row_tiles, grid, stream);
     return a.lists ? launch<T, CODE, D, true, 2>(a, row_tiles, grid, stream)
                    : launch<T, CODE, D, false, 2>(a, row_tiles, grid, stream);
 }
-template <typename T> int launch(const QuantArgs& a, int code, int D, int row_tiles, unsigned grid, cudaStream_t stream) {
+template <typename T> int launch(const QuantArgs& a, int code, int D, int row_tiles, dim3 grid, cudaStream_t stream) {
     if (code == kE4M3)
         return D == 128 ? launch<T, kE4M3, 128>(a, row_tiles, grid, stream) : launch<T, kE4M3, 64>(a, row_tiles, grid, stream);
     return D == 128 ? launch<T, kInt8, 128>(a, row_tiles, grid, stream) : launch<T, kInt8, 64>(a, row_tiles, grid, stream);
@@ -654,10 +652,10 @@ template <typename T> int launch(const QuantArgs& a, int code, int D, int row_ti
 
 int launch_quant_rows(const QuantArgs& a, int dtype, int code, int D, cudaStream_t stream) {
     const int row_tiles = (a.Tq * a.G + 15) / 16;
-    const int64_t items = (int64_t)a.B * a.Hkv * row_tiles * a.parts;
-    if (items > INT32_MAX) return LSA_ERR_SIZE;
-    return dtype == kBF16 ? launch<__nv_bfloat16>(a, code, D, row_tiles, (unsigned)items, stream)
-                          : launch<__half>(a, code, D, row_tiles, (unsigned)items, stream);
+    if (a.B > 65535 || (int64_t)a.Hkv * row_tiles > 65535) return LSA_ERR_SIZE;
+    const dim3 grid((unsigned)a.parts, (unsigned)(a.Hkv * row_tiles), (unsigned)a.B);
+    return dtype == kBF16 ? launch<__nv_bfloat16>(a, code, D, row_tiles, grid, stream)
+                          : launch<__half>(a, code, D, row_tiles, grid, stream);
 }
 
 template <typename T, int D> static int join(const QuantArgs& a, cudaStream_t stream) {

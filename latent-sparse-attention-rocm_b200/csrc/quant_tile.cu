@@ -101,7 +101,7 @@ __device__ __forceinline__ void tile_of(int p, int n, bool streams, int* c, bool
 
 // Row rl of half hf: (token of the call, head of the group); false: no row there.
 __device__ __forceinline__ bool row_at(const QuantArgs& a, const Item& w, int hf, int rl, int* tok, int* g) {
-    const int tl = rl / a.G;
+    const int tl = token_of(a, rl);
     *tok = w.t0 + (a.streams ? 0 : hf) * a.tokens + tl;
     *g = rl - tl * a.G;
     return tl < a.tokens && *tok < a.Tq;
