@@ -25,7 +25,7 @@ struct Plan {
 };
 
 // keys: the most that a row sees
-Plan make_plan(int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_t keys) {
+Plan make_plan(int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_t keys, bool lists) {
     Plan p = {};
     const int64_t G = Hq / Hkv, chunks = (keys + kUnit - 1) / kUnit;
     p.part_rows = B * Tq * Hq;
@@ -51,18 +51,34 @@ Plan make_plan(int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_
         return p;
     }
     const int64_t tiles = (Tq * G + kFewRows - 1) / kFewRows, items = B * Hkv * tiles;
-    const int64_t places = kSMs * (Tq * G <= 8 ? 3 : 2);  // CTAs of the few-row kernel that run at a time
-    auto cost = [&](int64_t parts) {
-        return (double)((items * parts + places - 1) / places) * ((double)chunks / parts + kItemCost);
-    };
-    // Parts that are a cluster's CTAs join within the launch, which pays where all clusters run at once (4 x 2k keys:
-    // 10.3 us against 12.0 with a second launch); where CTAs wait for a place, a cluster waits for all of its own
-    // (64 x 8k: 145 against 138 us; 32 lists of 2116: 51 against 43).
-    // A cluster of 16 takes most of a GPC: one CTA an SM then (16 of them on two an SM: 33 us, in 18 parts 24).
-    for (int c = 2; c <= kMostCluster && c / 2 < chunks && items * c <= (c > 8 ? kSMs : places); c *= 2)
-        if (cost(c) < 0.99 * cost(p.parts)) p.parts = c, p.cluster = true;
-    const int s = balance(items, chunks, kItemCost, places, kMaxQuantParts);
-    if (s > 1 && cost(s) + kJoinCost < cost(p.parts)) p.parts = s, p.cluster = false;
+    // Parts. One CTA in each of two places an SM draws the memory's whole rate; a third place only evens out ragged
+    // sequences, and a round that fills some SMs' third place and not others' is the worst (us in parts, CTAs in
+    // brackets; 32 / 8 heads, D 128): 1 x 32k 37 (296) 16.1, 42 (336) 17.8, 56 (448) 20.2; 4 x 16k 9 (288) 24.5, 14 (448)
+    // 29.5; 16 x 8k 2 (256) 41.9, 3 (384) 39.3, 5 (640) 44.1; 32 x 4k 1 (256) 49.0, 3 (768) 40.9; 64 x 8k 1 (512) 156,
+    // 4 (2048) 133, 12 (6144) 155. Lists are of one length: rounds of two places.
+    int64_t s;
+    if (lists) {
+        s = balance(items, chunks, kItemCost, 2 * kSMs, kMaxQuantParts);
+        auto cost = [&](int64_t n) {
+            return (double)((items * n + 2 * kSMs - 1) / (2 * kSMs)) * ((double)chunks / n + kItemCost);
+        };
+        if (s > 1 && cost(s) + kJoinCost >= cost(1)) s = 1;
+    } else if (items <= 100) {
+        s = 2 * kSMs / items;
+    } else if (items <= 200) {
+        s = (2 * kSMs + kSMs * 2 / 3) / items;
+    } else {
+        s = 2048 / items < chunks / 8 ? 2048 / items : chunks / 8;
+    }
+    if (s > chunks) s = chunks;
+    if (s > kMaxQuantParts) s = kMaxQuantParts;
+    p.parts = s < 1 ? 1 : (int)s;
+    // Parts that are a cluster's CTAs join within the launch, which pays where a CTA has little to do (4 x 2k keys, 8
+    // parts: 8.8 us against 10.5); clusters spread unevenly over the SMs (4 x 16k, 8 parts: 29.4 us, in a second launch
+    // 25.3).
+    int c = 1;
+    while (2 * c <= kMostCluster && 2 * c <= s && (c < 8 || items * 2 * c <= kSMs)) c *= 2;
+    if (c > 1 && (chunks <= 3 * c || (items * c <= kSMs && chunks <= 4 * c))) p.parts = c, p.cluster = true;
     p.bytes = p.parts > 1 && !p.cluster ? p.parts * p.part_rows * (D + 1) * 4 : 0;
     return p;
 }
@@ -99,7 +115,7 @@ int run(QuantArgs& a, int dtype, int code, int64_t D, int64_t keys, float scale,
     if (reinterpret_cast<uintptr_t>(a.q) % 16 != 0 || reinterpret_cast<uintptr_t>(a.out) % 16 != 0) return LSA_ERR_ARG;
     if (a.q_b % 8 != 0 || a.q_t % 8 != 0 || a.q_h % 8 != 0) return LSA_ERR_ARG;
     a.G_inverse = a.G > 1 ? (uint32_t)(((1ull << 32) + a.G - 1) / a.G) : 0;
-    const Plan p = make_plan(a.B, a.Tq, a.Hq, a.Hkv, D, keys);
+    const Plan p = make_plan(a.B, a.Tq, a.Hq, a.Hkv, D, keys, a.lists != nullptr);
     if (p.bytes > 0 && (scratch == nullptr || scratch_bytes < p.bytes || reinterpret_cast<uintptr_t>(scratch) % 16 != 0))
         return LSA_ERR_ARG;
     a.rows = (int64_t)a.B * a.Tq * a.Hq;
@@ -119,11 +135,11 @@ int run(QuantArgs& a, int dtype, int code, int64_t D, int64_t keys, float scale,
 
 extern "C" {
 
-int64_t lsa_quantized_scratch(int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_t keys) {
+int64_t lsa_quantized_scratch(int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_t keys, int lists) {
     using namespace lsa;
     if (!sizes_ok(B, Tq, Hq, Hkv, D, keys)) return LSA_ERR_ARG;
     if (B == 0 || Tq == 0) return 0;
-    return make_plan(B, Tq, Hq, Hkv, D, keys).bytes;
+    return make_plan(B, Tq, Hq, Hkv, D, keys, lists != 0).bytes;
 }
 
 int lsa_quantized_attention(const void* q, int dtype, const int64_t* q_strides, const void* k8, const void* v8,

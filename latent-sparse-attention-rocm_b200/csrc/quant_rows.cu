@@ -29,9 +29,10 @@ constexpr int kKeys = 32;  // keys of a warp's tile: one a lane where they are l
 constexpr int kFewParts = 8;  // that one warp joins
 constexpr float kLift = 10.0f, kGrow = 5.0f;
 
-template <int D, int NT> struct QuantShape {
+template <int D, int NT, bool LISTS> struct QuantShape {
     static constexpr int kRows = 8 * NT;
-    static constexpr int kRing = D == 128 ? (NT == 1 ? 2 : 3) : (NT == 1 ? 4 : 5);  // tiles in a warp's ring
+    static constexpr int kCTAs = NT == 1 && !LISTS ? 3 : 2;             // an SM
+    static constexpr int kRing = D == 128 ? (kCTAs == 3 ? 2 : 3) : (kCTAs == 3 ? 4 : 5);  // tiles in a warp's ring
     static constexpr int kTile = kKeys * D;            // K or V bytes of a tile
     static constexpr int kStage = 2 * kTile + kKeys * 12;  // + ks, vs (then its logarithm) and 1 / vs of every key
     static constexpr int kWarpBytes = (kRing * kStage + 127) / 128 * 128;
@@ -133,8 +134,8 @@ template <int D> __device__ __forceinline__ uint32_t v_at(int r, int c) {
 
 // NT: tiles of eight rows.
 template <typename T, int CODE, int D, bool LISTS, int NT>
-__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) quant_rows_kernel(const QuantArgs a, const int row_tiles) {
-    using Sh = QuantShape<D, NT>;
+__global__ void __launch_bounds__(kWarps * 32, QuantShape<D, NT, LISTS>::kCTAs) quant_rows_kernel(const QuantArgs a, const int row_tiles) {
+    using Sh = QuantShape<D, NT, LISTS>;
     constexpr int kRows = 8 * NT;
     constexpr int C = D / 16;       // 16-byte chunks of a key
     constexpr int KS = D / 16;      // k-steps of S
@@ -201,21 +202,25 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) quant_rows_kerne
     auto page_of = [&](int pos) {
         return pos >= 0 && pos < length && (pos >> a.shift) < a.M ? table[pos >> a.shift] : -1;
     };
+    // row of the pool (below 2^31: the entry point checks) of a position; a key that is not there is not read
+    auto row_of = [&](int pos, int page) {
+        return page >= 0 && page < a.pages
+                   ? (int)((((int64_t)page * a.Hkv + h) << a.shift) + (pos & ((1 << a.shift) - 1)))
+                   : -1;
+    };
     int pos1 = position(0), pos2 = position(1), page1 = page_of(pos1);
     uint32_t there = 0;  // bit j: this lane's key of the j-th tile before the last copied is there
     const uint8_t* const kl = a.k8 + (lane / C) * D + (lane % C) * 16;
     const uint8_t* const vl = a.v8 + (lane / C) * D + (lane % C) * 16;
     uint32_t slot = 0;  // of the next copy
     auto copy = [&](int i) {
-        const int pos = pos1, page = page1;
+        const int row = row_of(pos1, page1);
         pos1 = pos2, page1 = page_of(pos2), pos2 = position(i + 2);
         there <<= 1;
         if (i < tiles) {
-            const bool in = page >= 0 && page < a.pages;
+            const bool in = row >= 0;
             there |= in ? 1u : 0u;
-            const int64_t head = in ? (int64_t)page * a.Hkv + h : 0;
-            // row of the pool (below 2^31: the entry point checks); a key that is not there is not read
-            const int row = in ? (int)((head << a.shift) + (pos & ((1 << a.shift) - 1))) : -1;
+            const int64_t head = in ? row >> a.shift : 0;
             const uint32_t stage = ring + slot * Sh::kStage;
             const uint32_t scales = stage + 2 * Sh::kTile + lane * 4;
             cp_async4(scales, a.ks + head, in ? 4u : 0u);
@@ -226,8 +231,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) quant_rows_kerne
                     const int r = rr + lane / C, ch = lane % C;
                     const int from = __shfl_sync(0xFFFFFFFFu, row, r);
                     const int64_t at = (int64_t)((from < 0 ? 0 : from) - lane / C) * D;
-                    cp_async16(stage + k_at<D>(r, ch), kl + at, from < 0 ? 0u : 16u);
-                    cp_async16(stage + Sh::kTile + v_at<D>(r, ch), vl + at, from < 0 ? 0u : 16u);
+                    cp_async16(stage + k_at<D>(r, ch), from < 0 ? a.k8 : kl + at, from < 0 ? 0u : 16u);
+                    cp_async16(stage + Sh::kTile + v_at<D>(r, ch), from < 0 ? a.v8 : vl + at, from < 0 ? 0u : 16u);
                 }
             } else {
                 // 16 keys lie on one page: their rows follow one another, and the last ones may be past k1
@@ -629,7 +634,7 @@ __global__ void __launch_bounds__(256) quant_join_kernel(const QuantArgs a, cons
 
 template <typename T, int CODE, int D, bool LISTS, int NT>
 int launch(const QuantArgs& a, int row_tiles, dim3 grid, cudaStream_t stream) {
-    constexpr int smem = QuantShape<D, NT>::kSmem;
+    constexpr int smem = QuantShape<D, NT, LISTS>::kSmem;
     if (!allow_kernel<quant_rows_kernel<T, CODE, D, LISTS, NT>>(smem, true)) return LSA_ERR_CUDA;
     return launch_clusters(quant_rows_kernel<T, CODE, D, LISTS, NT>, grid, kWarps * 32, smem, stream,
                            a.cluster ? a.parts : 1, a, row_tiles);

@@ -554,7 +554,7 @@ std::pair<at::Tensor, at::Tensor> quantized(const at::Tensor& q_in, const at::Te
     at::Tensor lse;
     if (want_lse) lse = fresh({B, Tq, Hq}, at::kFloat, q.device());
     if (B * Tq == 0) return {out, lse};
-    const int64_t M = table.size(1), bytes = lsa_quantized_scratch(B, Tq, Hq, p.Hkv, p.D, M * p.page);
+    const int64_t M = table.size(1), bytes = lsa_quantized_scratch(B, Tq, Hq, p.Hkv, p.D, M * p.page, 0);
     TORCH_CHECK_VALUE(bytes >= 0, what, ": sizes out of range");
     at::Tensor scratch;  // the call's own, as the shared-prefix operators'
     if (bytes > 0) scratch = fresh({bytes}, at::kByte, q.device());
@@ -605,7 +605,7 @@ at::Tensor quantized_read_cuda(const at::Tensor& q_in, const at::Tensor& k8, con
     auto q = rows16(q_in);
     auto out = fresh({R, 1, Hq, p.D}, q.scalar_type(), q.device());
     if (R == 0) return out;
-    const int64_t W = lists.size(1), bytes = lsa_quantized_scratch(R, 1, Hq, p.Hkv, p.D, W);
+    const int64_t W = lists.size(1), bytes = lsa_quantized_scratch(R, 1, Hq, p.Hkv, p.D, W, 1);
     TORCH_CHECK_VALUE(bytes >= 0, what, ": sizes out of range");
     at::Tensor scratch;
     if (bytes > 0) scratch = fresh({bytes}, at::kByte, q.device());

@@ -92,7 +92,7 @@ SIGNATURES = {
     "lsa_append_quantized": (_INT, [_P, _P, _INT, _P, _P, _P, _P, _P, _INT, _I, _I, _P, _I, _I, _P, _P, _I, _I, _I,
                                     _I, _P]),
     "lsa_move_pages": (_INT, [_P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _I, _P]),
-    "lsa_quantized_scratch": (_I, [_I, _I, _I, _I, _I, _I]),
+    "lsa_quantized_scratch": (_I, [_I, _I, _I, _I, _I, _I, _INT]),
     "lsa_quantized_attention": (_INT, [_P, _INT, _P, _P, _P, _P, _P, _INT, _I, _I, _P, _I, _I, _P, _I, _I, _I, _I, _I,
                                        _F, _P, _P, _P, _I, _P, _P]),
     "lsa_quantized_read": (_INT, [_P, _INT, _P, _P, _P, _P, _P, _INT, _I, _I, _P, _I, _I, _I, _P, _P, _P, _P, _I, _I,

@@ -190,7 +190,7 @@ def test_entry_points_refuse_before_any_launch(lsa):
     assert read(R=2) == ERR_ARG and read(counts=None) == ERR_ARG and read(W=-1) == ERR_ARG and read(R=0) == OK
     assert L.lsa_move_pages(some, some, some, some, 4, 24, 1, 64, some, some, 1, None) == ERR_ARG
     assert L.lsa_move_pages(some, some, some, some, 4, 16, 1, 64, some, some, 0, None) == OK
-    assert L.lsa_quantized_scratch(1, 1, 3, 2, 64, 100) == ERR_ARG and L.lsa_quantized_scratch(0, 1, 2, 1, 64, 100) == 0
+    assert L.lsa_quantized_scratch(1, 1, 3, 2, 64, 100, 0) == ERR_ARG and L.lsa_quantized_scratch(0, 1, 2, 1, 64, 100, 0) == 0
 
 
 @pytest.mark.parametrize("code", ["e4m3", "int8"])
