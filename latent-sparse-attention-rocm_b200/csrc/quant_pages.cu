@@ -19,8 +19,8 @@ struct AppendArgs {
     int64_t table_ld;
     int M, pages, shift;
     const int32_t *lengths, *counts;  // counts: the rows of a sequence that are tokens, its last; null: all
-    int B, Tq, Hkv, slots;  // pages that a sequence's new tokens touch at most
-    int64_t units;
+    int B, Tq;
+    uint32_t Hkv, units;  // units of a sequence: pages that its new tokens touch at most x heads x 2
 };
 
 constexpr int kSmallRows = 4;  // new tokens of a sequence that one warp takes
@@ -47,13 +47,12 @@ __global__ void __launch_bounds__(NT == 32 ? 128 : NT) append_kernel(const Appen
     const int tid = NT == 32 ? threadIdx.x & 31 : threadIdx.x;
     grid_wait();
     grid_trigger();
-    int64_t unit = NT == 32 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
+    // (pages x heads x K and V, sequences); 32-bit divisions: those of 64 bits took half of the kernel's time
+    const uint32_t unit = NT == 32 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
     if (unit >= a.units) return;
     const bool value = unit & 1;
-    unit >>= 1;
-    const int h = (int)(unit % a.Hkv);
-    unit /= a.Hkv;
-    const int b = (int)(unit / a.slots);
+    const uint32_t nth = (unit >> 1) / a.Hkv;  // page of the call's
+    const int h = (int)((unit >> 1) - nth * a.Hkv), b = blockIdx.y;
     const int64_t length = a.lengths[b];
     const int64_t start = length - a.Tq;         // position of the call's first row; negative: rows that are padding
     int64_t first = start < 0 ? 0 : start;
@@ -62,7 +61,7 @@ __global__ void __launch_bounds__(NT == 32 ? 128 : NT) append_kernel(const Appen
         const int64_t from = length - (count < 0 ? 0 : (count > a.Tq ? a.Tq : count));
         first = first > from ? first : from;
     }
-    const int64_t slot = (first >> a.shift) + unit % a.slots;
+    const int64_t slot = (first >> a.shift) + nth;
     const int64_t p0 = slot << a.shift;
     const int page = 1 << a.shift;
     if (slot >= a.M || p0 >= length) return;
@@ -144,13 +143,11 @@ __global__ void __launch_bounds__(NT == 32 ? 128 : NT) append_kernel(const Appen
 
 template <typename T, int CODE, int D> int launch(const AppendArgs& a, cudaStream_t stream) {
     if (a.Tq <= kSmallRows) {
-        const int64_t blocks = (a.units + 3) / 4;
-        if (blocks > INT32_MAX) return LSA_ERR_SIZE;
-        return launch_after(append_kernel<T, CODE, D, 32, kSmallRows * (D / 8) / 32>, dim3((unsigned)blocks), 128, 0, stream, a);
+        const dim3 blocks((a.units + 3) / 4, (unsigned)a.B);
+        return launch_after(append_kernel<T, CODE, D, 32, kSmallRows * (D / 8) / 32>, blocks, 128, 0, stream, a);
     }
-    if (a.units > INT32_MAX) return LSA_ERR_SIZE;
     constexpr int NT = 2 * D;  // 16 rows a pass
-    const dim3 grid((unsigned)a.units);
+    const dim3 grid(a.units, (unsigned)a.B);
     switch (a.shift) {
         case 4: return launch_after(append_kernel<T, CODE, D, NT, 1>, grid, NT, 0, stream, a);
         case 5: return launch_after(append_kernel<T, CODE, D, NT, 2>, grid, NT, 0, stream, a);
@@ -230,11 +227,11 @@ int lsa_append_quantized(const void* k, const void* v, int dtype, const int64_t*
     a.table = table, a.table_ld = table_ld, a.M = (int)M, a.pages = (int)pages;
     a.shift = page == 16 ? 4 : (page == 32 ? 5 : (page == 64 ? 6 : 7));
     a.lengths = lengths, a.counts = counts;
-    a.B = (int)B, a.Tq = (int)Tq, a.Hkv = (int)Hkv;
+    a.B = (int)B, a.Tq = (int)Tq, a.Hkv = (uint32_t)Hkv;
     const int64_t slots = (Tq + page - 2) / page + 1;
-    a.slots = (int)(slots < M ? slots : M);
-    if (B * Hkv > INT64_MAX / 2 / a.slots) return LSA_ERR_SIZE;
-    a.units = B * a.slots * Hkv * 2;
+    const int64_t units = (slots < M ? slots : M) * Hkv * 2;
+    if (B > 65535 || units > INT32_MAX) return LSA_ERR_SIZE;
+    a.units = (uint32_t)units;
     switch (dtype) {
         case kF32: return launch<float>(a, code, D, stream);
         case kF16: return launch<__half>(a, code, D, stream);

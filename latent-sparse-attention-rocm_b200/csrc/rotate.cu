@@ -81,12 +81,13 @@ __global__ void __launch_bounds__(kWarps * 32) norm_rotate_kernel(const RotateAr
     constexpr int N = 32 / L; // heads of a pass
     const int lane = threadIdx.x & 31, j = lane % L, own = lane / L;
     const int64_t unit = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-    const int64_t token = unit / a.sections;
+    // (64-bit divisions only where the tokens want them)
+    const int64_t token = a.sections == 1 ? unit : (int64_t)((uint32_t)unit / (uint32_t)a.sections);
     const int section = (int)(unit - token * a.sections);
     grid_wait();
     grid_trigger();
     if (token >= a.tokens) return;
-    const int64_t b = token / a.T, t = token - b * a.T;
+    const int64_t b = a.tokens <= INT32_MAX ? (int64_t)((uint32_t)token / (uint32_t)a.T) : token / a.T, t = token - b * a.T;
     // passes over q's heads, then k's; this warp's
     const int q_passes = (a.Hq + N - 1) / N, passes = q_passes + (a.Hkv + N - 1) / N;
     const int p0 = passes * section / a.sections, p1 = passes * (section + 1) / a.sections;
@@ -98,10 +99,17 @@ __global__ void __launch_bounds__(kWarps * 32) norm_rotate_kernel(const RotateAr
     const T* krow = static_cast<const T*>(a.k) + b * a.k_b + t * a.k_t + own * a.k_h + at0;
     T* qdst = static_cast<T*>(a.q_out) + (token * a.Hq + own) * D + at0;
     T* kdst = static_cast<T*>(a.k_out) + (token * a.Hkv + own) * D + at0;
+    // passes that this lane has a head in: the last of q's and of k's may be short of heads
+    const int q_live = (a.Hq - own + N - 1) / N, k_live = q_passes + (a.Hkv - own + N - 1) / N;
     auto is_q = [&](int p) { return p < q_passes; };
-    auto live = [&](int p) { return is_q(p) ? p * N + own < a.Hq : (p - q_passes) * N + own < a.Hkv; };
-    auto load = [&](Raw8<T>& raw, int p) {
-        if (p < p1 && live(p)) raw.load(is_q(p) ? qrow + p * N * a.q_h : krow + (p - q_passes) * N * a.k_h, step);
+    auto live = [&](int p) { return p < (is_q(p) ? q_live : k_live); };
+    const bool from_q = is_q(p0);
+    const T* src = from_q ? qrow + (int64_t)p0 * N * a.q_h : krow + (int64_t)(p0 - q_passes) * N * a.k_h;
+    T* dst = from_q ? qdst + (int64_t)p0 * N * D : kdst + (int64_t)(p0 - q_passes) * N * D;
+    const int64_t q_next = N * a.q_h, k_next = N * a.k_h;
+    auto load = [&](Raw8<T>& raw, int p) {  // in the order of the passes
+        if (p < p1 && live(p)) raw.load(src, step);
+        src = p + 1 == q_passes ? krow : src + (is_q(p) ? q_next : k_next);
     };
     Raw8<T> raw[kAhead];
 #pragma unroll
@@ -176,10 +184,10 @@ __global__ void __launch_bounds__(kWarps * 32) norm_rotate_kernel(const RotateAr
                 unpair(fma2(xv, pair(vv[e], vv[e + 1]), mul2(xu, pair(uv[e], uv[e + 1]))), y[u0 + dv], y[u1 + dv]);
             }
             if (live(p)) {
-                T* dst = is_q(p) ? qdst + (int64_t)p * N * D : kdst + (int64_t)(p - q_passes) * N * D;
                 store4<T>(dst, y[0], y[1], y[2], y[3]);
                 store4<T>(dst + step, y[4], y[5], y[6], y[7]);
             }
+            dst = p + 1 == q_passes ? kdst : dst + N * D;
         }
     }
 }
