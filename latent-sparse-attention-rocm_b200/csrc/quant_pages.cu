@@ -5,10 +5,37 @@
 // two, so that growing moves e4m3's exponents and changes no other bit above its smallest step, and an integer's
 // successive roundings stay within one step of its scale. One CTA (or warp) a (sequence, page, KV head, K or V):
 // the new rows stay in registers between the maximum and the codes, so every byte moves once.
+#include <type_traits>
+
 #include "quant.cuh"
 
 namespace lsa {
 namespace {
+
+// Largest magnitude of a lane's values (NaN counts as nothing), two at a time where they are 16 bits wide.
+template <typename T, int N, typename Raw> __device__ __forceinline__ float largest(const Raw (&raw)[N]) {
+    if constexpr (sizeof(T) == 2) {
+        using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+        T2 top;
+#pragma unroll
+        for (int i = 0; i < 4 * N; ++i) {
+            const uint4& u = raw[i / 4].u[0];
+            const uint32_t w = (i % 4 == 0 ? u.x : (i % 4 == 1 ? u.y : (i % 4 == 2 ? u.z : u.w))) & 0x7FFF7FFFu;
+            top = i == 0 ? *reinterpret_cast<const T2*>(&w) : __hmax2(top, *reinterpret_cast<const T2*>(&w));
+        }
+        return fmaxf(to_f32(top.x), to_f32(top.y));
+    } else {
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float x[8];
+            raw[i].floats(x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
+        }
+        return top;
+    }
+}
 
 struct AppendArgs {
     const void *k, *v;
@@ -81,19 +108,12 @@ __global__ void __launch_bounds__(NT == 32 ? 128 : NT) append_kernel(const Appen
     float was = 0.0f;
     if (kept > 0) was = *scale;
     Raw<T> raw[PASSES];
-    float top = 0.0f;
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
         raw[i].zero();
         if (i * RP + r < n) raw[i].load(src + (int64_t)i * RP * ld);
     }
-#pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-        float x[8];
-        raw[i].floats(x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
-    }
+    float top = fmaxf(0.0f, largest<T>(raw));
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
     was = __shfl_sync(0xFFFFFFFFu, was, 0);  // every lane's read is behind it, before the write below
