@@ -170,7 +170,7 @@ __device__ __forceinline__ void load_q(const QuantArgs& a, const Item& w, uint8_
     }
 }
 
-template <typename T, int D>
+template <typename T, int D, int GK>
 __device__ __forceinline__ void softmax_half(const QuantArgs& a, const Item& w, uint8_t* sm, uint64_t* bar_s, uint64_t* bar_p,
                                              uint64_t* bar_o, volatile int* abort_flag, uint32_t tmem) {
     using Sh = QuantTile<D>;
@@ -213,13 +213,28 @@ __device__ __forceinline__ void softmax_half(const QuantArgs& a, const Item& w, 
         // - always on a row's first chunk.
         float alpha = 1.0f;
         uint64_t sum;
-        // logits of 16 keys from s: (multiplier, addend); the multiplier stays above 0, so that -inf does
-        auto group = [&](int i, float* mul, float* add) {
-            const float4 k = sc[i];
-            *mul = fmaxf(k.x * factor, 1e-30f), *add = k.y;
-            return k.z;
+        // logits from s, GK keys at a time: (multiplier, addend); the multiplier stays above 0, so that -inf does. Of 64
+        // keys, they are held; of 16, read when their turn comes.
+        constexpr int NG = kChunk / GK;
+        float muls[GK == 64 ? NG : 1], adds[GK == 64 ? NG : 1], invs[GK == 64 ? NG : 1];
+        if constexpr (GK == 64) {
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+                const float4 k = sc[i * (GK / 16)];
+                muls[i] = fmaxf(k.x * factor, 1e-30f), adds[i] = k.y, invs[i] = k.z;
+            }
+        }
+        auto group = [&](int i, float* mul, float* add) {  // of 16 keys
+            if constexpr (GK == 64) {
+                *mul = muls[i / 4], *add = adds[i / 4];
+                return invs[i / 4];
+            } else {
+                const float4 k = sc[i];
+                *mul = fmaxf(k.x * factor, 1e-30f), *add = k.y;
+                return k.z;
+            }
         };
-        auto exps = [&](auto& pk, int at, int i, float neg) {  // group i's 16 keys
+        auto exps = [&](auto& pk, int at, int i, float neg) {  // 16 keys
             float mul, add;
             const float inv = group(i, &mul, &add);
             const uint64_t mul2x = pair(mul, mul), add2x = pair(add + neg, add + neg);
@@ -249,15 +264,16 @@ __device__ __forceinline__ void softmax_half(const QuantArgs& a, const Item& w, 
             if (again) break;
             float mx = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < kGroups; ++i) {
-                float mul, add, mg = __uint_as_float(s[16 * i]), mh = __uint_as_float(s[16 * i + 1]);
-                group(i, &mul, &add);
+            for (int i = 0; i < NG; ++i) {
+                float mul, add, mg[4];
+                group(i * (GK / 16), &mul, &add);
 #pragma unroll
-                for (int e = 2; e < 16; e += 4) {
-                    mg = max3(mg, __uint_as_float(s[16 * i + e]), __uint_as_float(s[16 * i + e + 1]));
-                    if (e + 2 < 16) mh = max3(mh, __uint_as_float(s[16 * i + e + 2]), __uint_as_float(s[16 * i + e + 3]));
-                }
-                mx = fmaxf(mx, fmaf(fmaxf(mg, mh), mul, add));
+                for (int e = 0; e < 4; ++e)
+                    mg[e] = fmaxf(__uint_as_float(s[GK * i + 2 * e]), __uint_as_float(s[GK * i + 2 * e + 1]));
+#pragma unroll
+                for (int e = 8; e < GK; e += 2)
+                    mg[e / 2 & 3] = max3(mg[e / 2 & 3], __uint_as_float(s[GK * i + e]), __uint_as_float(s[GK * i + e + 1]));
+                mx = fmaxf(mx, fmaf(max3(mg[0], mg[1], fmaxf(mg[2], mg[3])), mul, add));
             }
             const bool grow = mx > m + kGrow;
             if (!__any_sync(0xFFFFFFFFu, grow)) break;
@@ -347,7 +363,8 @@ __device__ __forceinline__ void softmax_half(const QuantArgs& a, const Item& w, 
     bulk_commit_wait();
 }
 
-template <typename T, int CODE, int D>
+// GK: keys that share their scales (a page of 64 or 128 tokens: 64; else 16).
+template <typename T, int CODE, int D, int GK>
 __global__ void __launch_bounds__(kThreads, 1) quant_tile_kernel(const QuantArgs a) {
     using Sh = QuantTile<D>;
     constexpr int NO = Sh::kOps, KS = D / 16, kAll = Sh::kStages + Sh::kMore;
@@ -394,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tile_kernel(const QuantArgs
     if (warp >= 4) {
         // 384 threads launch at 168 registers: 128 x 72 + 256 x 216 = 384 x 168
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;" ::: "memory");
-        softmax_half<T, D>(a, w, sm, bar_s, bar_p, bar_o, abort_flag, tmem);
+        softmax_half<T, D, GK>(a, w, sm, bar_s, bar_p, bar_o, abort_flag, tmem);
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;" ::: "memory");
         if (warp == 0) {
@@ -614,9 +631,12 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tile_kernel(const QuantArgs
     if (threadIdx.x == 0 && *abort_flag) atomicExch(a.status, LSA_ERR_TIMEOUT);
 }
 
+template <typename T, int CODE, int D, int GK> int launch(const QuantArgs& a, unsigned grid, cudaStream_t stream) {
+    if (!allow_kernel<quant_tile_kernel<T, CODE, D, GK>>(QuantTile<D>::kSmem)) return LSA_ERR_CUDA;
+    return launch_after(quant_tile_kernel<T, CODE, D, GK>, dim3(grid), kThreads, QuantTile<D>::kSmem, stream, a);
+}
 template <typename T, int CODE, int D> int launch(const QuantArgs& a, unsigned grid, cudaStream_t stream) {
-    if (!allow_kernel<quant_tile_kernel<T, CODE, D>>(QuantTile<D>::kSmem)) return LSA_ERR_CUDA;
-    return launch_after(quant_tile_kernel<T, CODE, D>, dim3(grid), kThreads, QuantTile<D>::kSmem, stream, a);
+    return a.shift >= 6 ? launch<T, CODE, D, 64>(a, grid, stream) : launch<T, CODE, D, 16>(a, grid, stream);
 }
 template <typename T> int launch(const QuantArgs& a, int code, int D, unsigned grid, cudaStream_t stream) {
     if (code == kE4M3) return D == 128 ? launch<T, kE4M3, 128>(a, grid, stream) : launch<T, kE4M3, 64>(a, grid, stream);
