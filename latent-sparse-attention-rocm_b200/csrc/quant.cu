@@ -102,7 +102,8 @@ int pool(QuantArgs* a, const void* k8, const void* v8, const float* ks, const fl
     if (reinterpret_cast<uintptr_t>(k8) % 16 != 0 || reinterpret_cast<uintptr_t>(v8) % 16 != 0) return LSA_ERR_ARG;
     a->k8 = static_cast<const uint8_t*>(k8), a->v8 = static_cast<const uint8_t*>(v8);
     a->ks = ks, a->vs = vs;
-    a->table = table, a->table_ld = table_ld, a->table_rows = (int)table_rows, a->M = (int)M, a->pages = (int)pages;
+    a->table = table, a->table_ld = table_ld, a->table_rows = (int)table_rows, a->pages = (int)pages;
+    a->M = pages > 0 ? (int)M : 0;  // an empty pool holds nothing
     a->shift = page == 16 ? 4 : (page == 32 ? 5 : (page == 64 ? 6 : 7));
     a->lengths = lengths;
     return LSA_OK;
@@ -178,7 +179,7 @@ int lsa_quantized_read(const void* q, int dtype, const int64_t* q_strides, const
     if (rc != LSA_OK) return rc;
     a.q = q, a.q_b = q_strides[0], a.q_t = 0, a.q_h = q_strides[1];
     a.lists = W > 0 ? lists : counts;  // without entries nothing is read of it
-    a.counts = counts, a.list_rows = rows, a.W = (int)W;
+    a.counts = counts, a.list_rows = rows, a.W = a.M > 0 ? (int)W : 0;
     a.out = out, a.lse = nullptr;
     a.B = (int)R, a.Tq = 1, a.Hq = (int)Hq, a.Hkv = (int)Hkv, a.G = (int)(Hq / Hkv);
     return run(a, dtype, code, D, W, scale, scratch, scratch_bytes, stream);

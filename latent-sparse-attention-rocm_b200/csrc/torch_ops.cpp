@@ -481,8 +481,8 @@ void append_quantized_cuda(const at::Tensor& k_in, const at::Tensor& v_in, const
     TORCH_CHECK_VALUE(k_in.is_cuda() && k_in.device() == k8.device() && v_in.is_cuda() && v_in.device() == k8.device(), what,
                       " is a CUDA kernel (B200, sm_100a): every tensor on one CUDA device");
     TORCH_CHECK_VALUE(k_in.dim() == 4 && v_in.sizes() == k_in.sizes() && k_in.size(2) == p.Hkv && k_in.size(3) == p.D &&
-                          k_in.size(0) == table_in.size(0),
-                      what, ": k and v [B, Tq, ", p.Hkv, ", ", p.D, "], a table row a sequence");
+                          table_in.dim() == 2 && k_in.size(0) == table_in.size(0) && k_in.size(0) <= 65535,
+                      what, ": k and v [B, Tq, ", p.Hkv, ", ", p.D, "], a table row a sequence, at most 65535 sequences");
     const auto dt = k_in.scalar_type();
     TORCH_CHECK_VALUE((dt == at::kFloat || dt == at::kHalf || dt == at::kBFloat16) && v_in.scalar_type() == dt, what,
                       ": k and v fp32, fp16 or bf16, of one type, got ", dt, ", ", v_in.scalar_type());

@@ -162,6 +162,64 @@ def test_attention_empty(lsa, shape):
     assert out.shape == q.shape and bool((out == 0).all()) and bool((lse == -math.inf).all())
 
 
+@pytest.mark.parametrize("Tq,Hq,Hkv", [(1, 160, 1), (2, 33, 1), (3, 130, 1), (9, 21, 3)])
+def test_attention_head_groups(lsa, Tq, Hq, Hkv):
+    """Groups of odd sizes, and of more heads than a row tile of the tensor cores holds."""
+    attend_case(lsa, 18, [300, Tq, 40], Tq, Hq, Hkv, 64, 32, "e4m3", BF)
+
+
+@pytest.mark.parametrize("Tq", [1, 40])
+def test_attention_of_an_empty_pool(lsa, Tq):
+    pages = lsa.QuantizedPages.new(0, 2, 16, 64)
+    q = torch.randn(2, Tq, 4, 64, device="cuda").to(BF)
+    table, ln = torch.zeros(2, 3, dtype=torch.int32, device="cuda"), torch.tensor([40, 5], device="cuda")
+    out, lse = lsa.quantized_attention(q, pages, table, ln, return_lse=True)
+    assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+    lists = torch.zeros(2, 7, dtype=torch.int32, device="cuda")
+    assert bool((lsa.quantized_read(q[:, :1], pages, table, ln, lists, ln) == 0).all())
+    lsa.append_quantized(pages, q[:, :, :2], q[:, :, :2], table, ln)
+    lsa.move_pages(pages, lists[0], lists[1])
+    none = torch.zeros(2, 0, dtype=torch.int32, device="cuda")
+    some = lsa.QuantizedPages.new(3, 2, 16, 64)
+    assert bool((lsa.quantized_read(q[:, :1], some, table, ln, none, ln) == 0).all())
+
+
+@pytest.fixture()
+def wait_limit():
+    """Sets the limit of the tensor-core kernels' waits (ns); the default again afterwards."""
+    from lsa_b200 import _lib
+
+    _lib.torch_ops()
+    yield lambda ns: _lib.check(_lib.lib().lsa_shared_prefix_wait_limit(ns), "wait limit")
+    assert _lib.lib().lsa_shared_prefix_wait_limit(-1) == _lib.OK
+
+
+@pytest.mark.parametrize("code,D,page,B,Tq,Hq,Hkv,T", [
+    ("e4m3", 128, 64, 20, 16, 32, 4, 3000),  # two streams, split
+    ("int8", 64, 16, 2, 40, 8, 4, 700),
+    ("e4m3", 128, 128, 40, 64, 32, 4, 900),  # both halves, whole tiles and split ones
+    ("int8", 64, 32, 3, 257, 6, 2, 257),
+])
+def test_expired_waits_leave_with_their_copies_landed(lsa, wait_limit, code, D, page, B, Tq, Hq, Hkv, T):
+    """Every role gives up at its first wait, with the first copies in flight. The call reports it, and calls after it,
+    on the same SMs, answer as before."""
+    g = torch.Generator().manual_seed(19)
+    lengths = torch.randint(min(Tq, T), T + 1, (B,), generator=g).tolist()
+    table, n = F.paged(g, lengths, page)
+    pages = F.to(F.pool(g, n, Hkv, page, D, code), "cuda")
+    q = torch.randn(B, Tq, Hq, D, generator=g).to(BF).cuda()
+    table, ln = table.cuda(), torch.tensor(lengths, dtype=torch.int32).cuda()
+    want = lsa.quantized_attention(q, pages, table, ln)
+    for _ in range(3):
+        wait_limit(0)
+        with pytest.raises(RuntimeError, match="bounded device wait expired"):
+            lsa.quantized_attention(q, pages, table, ln)
+            lsa.check_status()  # without the checked mode
+        wait_limit(-1)
+        assert torch.equal(lsa.quantized_attention(q, pages, table, ln), want)
+    lsa.check_status()
+
+
 # ------------------------------------------------------------------ the read
 
 
