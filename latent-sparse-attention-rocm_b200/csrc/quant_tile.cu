@@ -9,7 +9,8 @@
 // With at most 128 rows both halves hold the same rows and take alternate chunks, so that two softmax chains are in
 // flight where the keys' bandwidth is the bound.
 // The codes come as they are (bulk copies of a page's rows of a head, which are contiguous) into a ring of 8-bit tiles;
-// two warps make halves of them (exact) into a ring of operand tiles, zeros where there is no key, so what a page holds
+// two warps, and softmax warps that no row wants, make halves of
+// them (exact) into a ring of operand tiles, zeros where there is no key, so what a page holds
 // behind a sequence's last token never meets a product. Scales stay out of the tiles: 16 keys share a page, so a
 // row's logits are s * (ks * factor) + log2 vs with constants for 16 keys, and the sum takes 1 / vs once for 16.
 // bf16 rows of Q become fp16 by a power of two of their own, as in the few-row kernel. P is rounded to fp16 and
@@ -29,7 +30,6 @@ namespace lsa {
 namespace {
 
 constexpr int kThreads = 384;
-constexpr int kConvert = 64;  // threads that convert: 16 rows a step, four a row
 constexpr float kLift = 7.0f, kGrow = 4.0f;
 constexpr int kChunks = 8;  // chunks whose scales are kept: more than the rings and the softmax hold together
 constexpr int kGroups = kChunk / 16;
@@ -131,10 +131,10 @@ __device__ __forceinline__ void sts_u4(uint32_t addr, uint32_t a, uint32_t b, ui
 template <typename T, int D>
 __device__ __forceinline__ void load_q(const QuantArgs& a, const Item& w, uint8_t* sm) {
     using Sh = QuantTile<D>;
-    constexpr int L = D / 8, RP = kThreads / L;  // threads of a row, rows of a pass
+    constexpr int L = D / 8, RP = (kThreads - 32) / L;  // threads of a row, rows of a pass
     constexpr int PASSES = (256 + RP - 1) / RP;
     float* factor = reinterpret_cast<float*>(sm + Sh::kOffFactor);
-    const int lr = threadIdx.x / L, ch = threadIdx.x % L;
+    const int t = threadIdx.x - 32, lr = t / L, ch = t % L;  // all warps but the first
     const int halves = a.streams ? 1 : 2;
     uint4 raw[PASSES];
 #pragma unroll
@@ -363,6 +363,135 @@ __device__ __forceinline__ void softmax_half(const QuantArgs& a, const Item& w, 
     bulk_commit_wait();
 }
 
+// The warp that asks for codes and scales: a lane 16 keys of the chunk (whose page's rows the first lane of a page asks
+// for), page ids two chunks ahead, scales one.
+template <int D> struct Loader {
+    using Sh = QuantTile<D>;
+    int id0, id1, held[3];  // page ids of the next K's chunk and of the one after it; of the chunks whose V is to come
+    float ks, vs;           // the next K's chunk's scales
+
+    // page id of this lane's keys of the item's chunk c, -1: none
+    static __device__ __forceinline__ int lookup(const QuantArgs& a, const Item& w, int c) {
+        const int lane = threadIdx.x & 31;
+        const int64_t key = (int64_t)(w.c0 + c) * kChunk + lane * 16;
+        int id = -1;
+        if (lane < kGroups && c < w.c1 - w.c0 && key < w.keys) id = a.table[w.b * a.table_ld + (key >> a.shift)];
+        return id >= 0 && id < a.pages ? id : -1;
+    }
+    __device__ __forceinline__ void scales(const QuantArgs& a, const Item& w) {
+        const int64_t head = (int64_t)(id0 < 0 ? 0 : id0) * a.Hkv + w.h;
+        ks = id0 < 0 ? 1.0f : a.ks[head];
+        vs = id0 < 0 ? 1.0f : a.vs[head];
+    }
+    __device__ __forceinline__ void start(const QuantArgs& a, const Item& w) {
+        id0 = lookup(a, w, 0), id1 = lookup(a, w, 1);
+        held[0] = held[1] = held[2] = -1;
+        scales(a, w);
+    }
+    // Tile p into stage s.
+    __device__ __forceinline__ void load(const QuantArgs& a, const Item& w, uint8_t* sm, uint64_t* codes_full, int p, int s) {
+        const int lane = threadIdx.x & 31, page = 1 << a.shift;
+        int c;
+        bool value;
+        tile_of(p, w.c1 - w.c0, a.streams, &c, &value);
+        const int id = !value ? id0 : (c % 3 == 0 ? held[0] : (c % 3 == 1 ? held[1] : held[2]));
+        const int left = id < 0 ? 0 : w.keys - (w.c0 + c) * kChunk - lane * 16;  // keys from the lane's first on
+        const int rows = left < 0 ? 0 : (left < 16 ? left : 16);
+        int total = rows;
+#pragma unroll
+        for (int off = 1; off < 8; off <<= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, off);
+        if (lane == 0) mbar_arrive_expect_tx(&codes_full[s], total * D);
+        __syncwarp();
+        const int64_t head = (int64_t)(id < 0 ? 0 : id) * a.Hkv + w.h;
+        if (rows > 0 && ((lane * 16) & (page - 1)) == 0)
+            bulk_g2s(sm + Sh::codes_at(s) + lane * 16 * D, (value ? a.v8 : a.k8) + (head << a.shift) * D,
+                     (left < page ? left : page) * D, &codes_full[s]);
+        if (!value) {
+            held[2] = c % 3 == 2 ? id : held[2], held[1] = c % 3 == 1 ? id : held[1], held[0] = c % 3 == 0 ? id : held[0];
+            if (lane < kGroups) {
+                const float v = fmaxf(vs, 8.6736174e-19f);  // 2^-60
+                *reinterpret_cast<float4*>(sm + Sh::kOffScales + (((w.c0 + c) % kChunks) * kGroups + lane) * 16) =
+                    rows > 0 ? make_float4(ks, log2f(v), 1.0f / v, __int_as_float(rows))
+                             : make_float4(1.0f, -INFINITY, 0.0f, 0.0f);
+            }
+            __syncwarp();
+            id0 = id1;
+            scales(a, w);
+            id1 = lookup(a, w, c + 2);
+        }
+        if (lane == 0) mbar_arrive(&codes_full[s]);
+    }
+};
+
+// Codes to operand tiles: warp `self` of WARPS (even). A warp's step is 8 rows, four lanes a row, half of a row's 64-byte
+// pieces each (D = 128: neighbouring rows at different blocks, so that both the loads and the stores miss each other's
+// banks). Zeros where there is no key.
+template <int CODE, int D, int WARPS>
+__device__ __forceinline__ void convert(const QuantArgs& a, const Item& w, uint8_t* sm, uint64_t* codes_full,
+                                        uint64_t* codes_empty, uint64_t* op_full, uint64_t* op_empty,
+                                        volatile int* abort_flag, int self) {
+    using Sh = QuantTile<D>;
+    // Of two blocks, a warp takes the same one of all of its rows: steps first, first + BY .. of 8 rows
+    constexpr int NO = Sh::kOps, X = D / 64, BY = WARPS / X, STEPS = (kChunk / 8 + BY - 1) / BY;
+    const int NS = a.streams ? Sh::kStages + Sh::kMore : Sh::kStages;
+    const int lane = threadIdx.x & 31, lr = lane >> 2, q = lane & 3, n = w.c1 - w.c0;
+    const uint32_t sbase = smem_u32(sm);
+    const int first = X == 1 ? self : self >> 1, x = X == 1 ? 0 : (self ^ lr) & 1;
+    const uint32_t src = (first * 8 + lr) * D + q * 16 + x * 64, dst = (first * 8 + lr) * 128 + x * 16384;
+    const uint32_t ca = dst + (((2 * q) ^ lr) << 4), cb = dst + (((2 * q + 1) ^ lr) << 4);
+    int s = 0, round = 0;
+    for (int p = 0; p < 2 * n; ++p, s = s + 1 == NS ? 0 : s + 1, round += s == 0) {
+        const int o = p % NO;
+        int c;
+        bool value;
+        tile_of(p, n, a.streams, &c, &value);
+        if (!role_wait(&codes_full[s], round & 1, abort_flag, a.wait_ns)) break;
+        if (p >= NO && !role_wait(&op_empty[o], (p / NO - 1) & 1, abort_flag, a.wait_ns)) break;
+        const uint32_t from = sbase + Sh::codes_at(s) + src;
+        const uint32_t to = sbase + Sh::kOffOps + o * Sh::kOperand;
+        const uint32_t sc = sbase + Sh::kOffScales + ((w.c0 + c) % kChunks) * kGroups * 16;
+        const int rows = __float_as_int(lds_f4(sc + (lane & 7) * 16).w);  // of 16 keys a lane
+        const bool whole = __all_sync(0xFFFFFFFFu, rows == 16);
+#pragma unroll
+        for (int base = 0; base < STEPS; base += 4) {
+            uint4 k[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (base + u < STEPS && (STEPS * BY == kChunk / 8 || first + (base + u) * BY < kChunk / 8))
+                    k[u] = lds_u4(from + (base + u) * BY * 8 * D);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int step = first + (base + u) * BY;
+                if (base + u >= STEPS || (STEPS * BY != kChunk / 8 && step >= kChunk / 8)) break;
+                if (!whole && (step * 8 + lr & 15) >= __shfl_sync(0xFFFFFFFFu, rows, step >> 1)) k[u] = make_uint4(0, 0, 0, 0);
+                const uint32_t line = to + (base + u) * BY * 1024;
+                sts_u4(line + ca, halves_of<CODE>(k[u].x, 0), halves_of<CODE>(k[u].x, 1), halves_of<CODE>(k[u].y, 0),
+                       halves_of<CODE>(k[u].y, 1));
+                sts_u4(line + cb, halves_of<CODE>(k[u].z, 0), halves_of<CODE>(k[u].z, 1), halves_of<CODE>(k[u].w, 0),
+                       halves_of<CODE>(k[u].w, 1));
+            }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+            mbar_arrive(&op_full[o]);
+            mbar_arrive(&codes_empty[s]);
+        }
+    }
+}
+
+template <int CODE, int D>
+__device__ __forceinline__ void convert(const QuantArgs& a, const Item& w, uint8_t* sm, uint64_t* codes_full,
+                                        uint64_t* codes_empty, uint64_t* op_full, uint64_t* op_empty,
+                                        volatile int* abort_flag, int self, int warps) {
+    switch (warps) {
+        case 2: return convert<CODE, D, 2>(a, w, sm, codes_full, codes_empty, op_full, op_empty, abort_flag, self);
+        case 4: return convert<CODE, D, 4>(a, w, sm, codes_full, codes_empty, op_full, op_empty, abort_flag, self);
+        case 6: return convert<CODE, D, 6>(a, w, sm, codes_full, codes_empty, op_full, op_empty, abort_flag, self);
+        default: return convert<CODE, D, 8>(a, w, sm, codes_full, codes_empty, op_full, op_empty, abort_flag, self);
+    }
+}
+
 // GK: keys that share their scales (a page of 64 or 128 tokens: 64; else 16).
 template <typename T, int CODE, int D, int GK>
 __global__ void __launch_bounds__(kThreads, 1) quant_tile_kernel(const QuantArgs a) {
@@ -377,20 +506,22 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tile_kernel(const QuantArgs
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + Sh::kOffMisc);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + Sh::kOffMisc + 4);
     const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    // Of one half's rows, the softmax warps without a row convert too.
+    const int row_warps = a.streams ? (a.Tq * a.G + 31) / 32 : 4, converters = 2 + 2 * (4 - row_warps);
     if (warp == 1) tmem_alloc(tmem_slot, 512);
     if (threadIdx.x == 0) {
         for (int s = 0; s < kAll; ++s) {
             mbar_init(&codes_full[s], 2);   // the bytes, and the scales beside them
-            mbar_init(&codes_empty[s], 2);  // the converting warps
+            mbar_init(&codes_empty[s], converters);
         }
         for (int s = 0; s < NO; ++s) {
-            mbar_init(&op_full[s], 2);
+            mbar_init(&op_full[s], converters);
             mbar_init(&op_empty[s], 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bar_s[i], 1);
-            mbar_init(&bar_p[2 * i], 4);
-            mbar_init(&bar_p[2 * i + 1], 4);
+            mbar_init(&bar_p[2 * i], row_warps);
+            mbar_init(&bar_p[2 * i + 1], row_warps);
             mbar_init(&bar_o[i], 1);
         }
         mbar_init(bar_drain, 1);
@@ -401,7 +532,14 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tile_kernel(const QuantArgs
     grid_trigger();
     const Item w = item_of(a);
     const int n = w.c1 - w.c0;
-    load_q<T, D>(a, w, sm);  // whether or not it has keys: its loads go out beside the lengths'
+    Loader<D> loader;
+    if (warp == 0) {  // the first tiles' copies are on their way while Q comes in
+        __syncwarp();
+        loader.start(a, w);
+        for (int i = 0; i < NS && i < 2 * n; ++i) loader.load(a, w, sm, codes_full, i, i);
+    } else {
+        load_q<T, D>(a, w, sm);
+    }
     fence_proxy_async_smem();
     tc_fence_before();
     __syncthreads();
@@ -411,62 +549,19 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tile_kernel(const QuantArgs
     if (warp >= 4) {
         // 384 threads launch at 168 registers: 128 x 72 + 256 x 216 = 384 x 168
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;" ::: "memory");
-        softmax_half<T, D, GK>(a, w, sm, bar_s, bar_p, bar_o, abort_flag, tmem);
+        if ((warp & 3) < row_warps)
+            softmax_half<T, D, GK>(a, w, sm, bar_s, bar_p, bar_o, abort_flag, tmem);
+        else
+            convert<CODE, D>(a, w, sm, codes_full, codes_empty, op_full, op_empty, abort_flag,
+                             2 + (warp - 4 >> 2) * (4 - row_warps) + (warp & 3) - row_warps, converters);
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;" ::: "memory");
         if (warp == 0) {
-            // ------------------------------------------------ codes and scales: a lane 16 keys of the chunk
-            // (whose page's rows the first lane of a page asks for). Page ids two chunks ahead, scales one.
-            const int page = 1 << a.shift, in_page = (lane * 16) & (page - 1);
-            const int32_t* table = a.table + w.b * a.table_ld;
-            auto lookup = [&](int c) {  // page id of this lane's keys of chunk c, -1: none
-                const int64_t key = (int64_t)(w.c0 + c) * kChunk + lane * 16;
-                int id = -1;
-                if (lane < kGroups && c < n && key < w.keys) id = table[key >> a.shift];
-                return id >= 0 && id < a.pages ? id : -1;
-            };
-            int id0 = lookup(0), id1 = lookup(1), held[3] = {-1, -1, -1};
-            float ks = 1.0f, vs = 1.0f;
-            auto scales = [&](int id) {
-                const int64_t head = (int64_t)(id < 0 ? 0 : id) * a.Hkv + w.h;
-                ks = id < 0 ? 1.0f : a.ks[head];
-                vs = id < 0 ? 1.0f : a.vs[head];
-            };
-            scales(id0);
-            int p = 0;
-            bool ok = true;
-            int s = 0, round = 0;
-            for (; p < 2 * n; ++p, s = s + 1 == NS ? 0 : s + 1, round += s == 0) {
-                if (round > 0 && !(ok = role_wait(&codes_empty[s], (round - 1) & 1, abort_flag, a.wait_ns))) break;
-                int c;
-                bool value;
-                tile_of(p, n, a.streams, &c, &value);
-                const int id = !value ? id0 : (c % 3 == 0 ? held[0] : (c % 3 == 1 ? held[1] : held[2]));
-                const int left = id < 0 ? 0 : w.keys - (w.c0 + c) * kChunk - lane * 16;  // keys from the lane's first on
-                const int rows = left < 0 ? 0 : (left < 16 ? left : 16);
-                int total = rows;
-#pragma unroll
-                for (int off = 1; off < 8; off <<= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, off);
-                if (lane == 0) mbar_arrive_expect_tx(&codes_full[s], total * D);
-                __syncwarp();
-                const int64_t head = (int64_t)(id < 0 ? 0 : id) * a.Hkv + w.h;
-                if (rows > 0 && in_page == 0)
-                    bulk_g2s(sm + Sh::codes_at(s) + lane * 16 * D, (value ? a.v8 : a.k8) + (head << a.shift) * D,
-                             (left < page ? left : page) * D, &codes_full[s]);
-                if (!value) {
-                    held[2] = c % 3 == 2 ? id : held[2], held[1] = c % 3 == 1 ? id : held[1], held[0] = c % 3 == 0 ? id : held[0];
-                    if (lane < kGroups) {
-                        const float v = fmaxf(vs, 8.6736174e-19f);  // 2^-60
-                        *reinterpret_cast<float4*>(sm + Sh::kOffScales + (((w.c0 + c) % kChunks) * kGroups + lane) * 16) =
-                            rows > 0 ? make_float4(ks, log2f(v), 1.0f / v, __int_as_float(rows))
-                                     : make_float4(1.0f, -INFINITY, 0.0f, 0.0f);
-                    }
-                    __syncwarp();
-                    id0 = id1;
-                    scales(id0);
-                    id1 = lookup(c + 2);
-                }
-                if (lane == 0) mbar_arrive(&codes_full[s]);
+            int p = 2 * n < NS ? 2 * n : NS, s = 0, round = 0;
+            for (; p < 2 * n; ++p) {
+                if (!role_wait(&codes_empty[s], round & 1, abort_flag, a.wait_ns)) break;
+                loader.load(a, w, sm, codes_full, p, s);
+                if (++s == NS) s = 0, ++round;
             }
             // Every copy issued lands before the CTA leaves, also when it was another role that gave up.
             for (int i = p > NS ? p - NS : 0; i < p; ++i) mbar_wait_bounded(&codes_full[i % NS], (i / NS) & 1);
@@ -567,59 +662,7 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tile_kernel(const QuantArgs
             }
             __syncwarp();
         } else {
-            // ------------------------------------------------ codes to operand tiles: 16 rows a step, four threads a row
-            const int t = threadIdx.x - 64, lr = t >> 2, q = t & 3;
-            constexpr int X = D / 64;  // 64-element blocks of a row
-            int s = 0, round = 0;
-            for (int p = 0; p < 2 * n; ++p, s = s + 1 == NS ? 0 : s + 1, round += s == 0) {
-                const int o = p % NO;
-                int c;
-                bool value;
-                tile_of(p, n, a.streams, &c, &value);
-                if (!role_wait(&codes_full[s], round & 1, abort_flag, a.wait_ns)) break;
-                if (p >= NO && !role_wait(&op_empty[o], (p / NO - 1) & 1, abort_flag, a.wait_ns)) break;
-                const uint32_t from = sbase + Sh::codes_at(s);
-                const uint32_t to = sbase + Sh::kOffOps + o * Sh::kOperand;
-                const uint32_t sc = sbase + Sh::kOffScales + ((w.c0 + c) % kChunks) * kGroups * 16;
-                const int rows = __float_as_int(lds_f4(sc + (lane & 7) * 16).w);  // of 16 keys a lane
-                const bool whole = __all_sync(0xFFFFFFFFu, rows == 16);
-                // neighbouring rows at different blocks: both the loads and the stores miss each other's banks
-                const int x0 = X == 1 ? 0 : (lr & 1);
-                const uint32_t src = from + lr * D + q * 16 + x0 * 64, dst = to + lr * 128 + x0 * 16384;
-                const uint32_t ca = ((2 * q) ^ (lr & 7)) << 4, cb = ((2 * q + 1) ^ (lr & 7)) << 4;
-                // four loads are on their way while the four before them are converted and stored
-                constexpr int BATCHES = kGroups * X / 4;
-                uint4 k[2][4];
-                auto fetch = [&](int i) {
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const int x = X == 1 ? 0 : u & 1, gi = i * (4 / X) + u / X;
-                        k[i & 1][u] = lds_u4(src + gi * 16 * D + (x ? 64 - 128 * x0 : 0));
-                    }
-                };
-                fetch(0);
-#pragma unroll
-                for (int i = 0; i < BATCHES; ++i) {
-                    if (i + 1 < BATCHES) fetch(i + 1);
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const int x = X == 1 ? 0 : u & 1, gi = i * (4 / X) + u / X;
-                        uint4& w4 = k[i & 1][u];
-                        if (!whole && lr >= __shfl_sync(0xFFFFFFFFu, rows, gi)) w4 = make_uint4(0, 0, 0, 0);
-                        const uint32_t line = dst + gi * 2048 + (x ? 16384 - 32768 * x0 : 0);
-                        sts_u4(line + ca, halves_of<CODE>(w4.x, 0), halves_of<CODE>(w4.x, 1), halves_of<CODE>(w4.y, 0),
-                               halves_of<CODE>(w4.y, 1));
-                        sts_u4(line + cb, halves_of<CODE>(w4.z, 0), halves_of<CODE>(w4.z, 1), halves_of<CODE>(w4.w, 0),
-                               halves_of<CODE>(w4.w, 1));
-                    }
-                }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&op_full[o]);
-                    mbar_arrive(&codes_empty[s]);
-                }
-            }
+            convert<CODE, D>(a, w, sm, codes_full, codes_empty, op_full, op_empty, abort_flag, warp - 2, converters);
         }
     }
     tc_fence_before();
