@@ -11,7 +11,6 @@ namespace {
 constexpr int kSMs = 148;
 constexpr int kFewRows = 16;  // rows of the few-row kernel's tiles
 constexpr int kUnit = 128;      // keys that a CTA's four warps take at a time
-constexpr int64_t kFewKeys = 1 << 17;  // (key, head) pairs that the few-row kernel reads up to four times
 constexpr int kMaxTileParts = 32, kMostRounds = 8;  // splits of a tile; rounds of the SMs that split tiles fill
 constexpr double kItemCost = 1.5, kJoinCost = 3.0;  // a CTA's start and end, the join's launch, in units' times
 
@@ -32,9 +31,11 @@ Plan make_plan(int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_
     p.parts = 1;
     // The few-row kernel reads the keys once for each 16 rows, from L2 after the first time, and converts them in
     // registers; the tensor-core kernel's converting goes through shared memory, which its products share, and its start
-    // takes 5 us (32 x 4096 keys: 20-32 rows 94 against 140 us, 48 rows 159 against 143, 64 rows 183 against 145; 4 x 2048:
-    // 48 rows 19.7 against 21.7; 16 x 2048: 58 against 46).
-    if (Tq * G > (B * Hkv * keys <= kFewKeys ? 64 : 32) && G <= 128) {
+    // takes 4 us (us, few-row / tensor cores: 32 x 4096 keys, 20-32 rows 89 / 120, 48 rows 159 / 122; 4 x 4096 48 rows 24.9
+    // / 26.9, 64 rows 37 / 26; 1 x 2048 128 rows 13.8 / 18.3, 256 rows 24.7 / 24.4; 1 x 512 512 rows 9.4 / 18.4).
+    const int64_t rows = Tq * G, heads = B * Hkv * keys;
+    const bool few = rows <= 32 || (rows <= 48 && heads <= 1 << 17) || (heads <= 1 << 21 && rows * heads <= 1 << 21);
+    if (!few && G <= 128) {
         // Whole rounds of one tile an SM are not split (no parts to write, read and join); the tiles of the last, short
         // round are, so that it too fills the GPU.
         p.tokens = (int)(128 / G);

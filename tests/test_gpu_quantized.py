@@ -71,6 +71,41 @@ def test_attention_chunks(lsa, Tq, code, dtype, D, page, Hq, Hkv):
     attend_case(lsa, 3, [Tq + 777, Tq, Tq // 2, 0, Tq + 1], Tq, Hq, Hkv, D, page, code, dtype)
 
 
+# What the tensor-core kernel takes: more rows x keys than the few-row kernel is faster on.
+@pytest.mark.parametrize("Tq,Hq,Hkv", [(9, 32, 8), (16, 32, 8), (13, 48, 8), (31, 32, 8), (64, 16, 4), (65, 24, 8)],
+                         ids=["36rows", "64rows", "78rows", "124rows", "two halves", "odd group"])
+@pytest.mark.parametrize("code,dtype,D,page", [("e4m3", BF, 128, 64), ("int8", HF, 64, 16), ("e4m3", HF, 64, 128),
+                                               ("int8", BF, 128, 32)])
+def test_attention_tiles(lsa, Tq, Hq, Hkv, code, dtype, D, page):
+    """Ragged batches: no key, fewer keys than rows, one chunk, its border, several; two streams with one to four
+    warps of rows, both halves."""
+    g = torch.Generator().manual_seed(Tq)
+    lengths = [0, 1, Tq - 1, Tq, 127, 128, 129, 255, 256, 257, 383, 1100, 1152] + torch.randint(1, 1152, (9,), generator=g).tolist()
+    attend_case(lsa, 20, lengths, Tq, Hq, Hkv, D, page, code, dtype)
+
+
+def test_attention_tiles_long(lsa):
+    """A long sequence's tiles split over many CTAs beside short ones; scales far apart; holes in the table."""
+    attend_case(lsa, 21, [9003, 70, 4096], 70, 16, 2, 128, 64, "e4m3", BF)
+    attend_case(lsa, 22, [3000] * 5, 40, 16, 8, 128, 16, "e4m3", HF, spread=60.0, scale=1e-6)
+    g = torch.Generator().manual_seed(23)
+    lengths = [1500] * 12
+    for Tq in (10, 70):
+        table, n = F.paged(g, lengths, 32)
+        table[:, 3::5], table[2], table[5, 1:] = -1, 1 << 30, -1
+        pages = F.pool(g, n, 8, 32, 64, "int8")
+        F.poison(pages, table, lengths)
+        q = torch.randn(12, Tq, 32, 64, generator=g).to(BF)
+        q[3, Tq - 1, 7, 5] = math.nan
+        ln = torch.tensor(lengths)
+        want, _, off, _ = F.attention(q, pages, table, ln)
+        got = lsa.quantized_attention(q.cuda(), F.to(pages, "cuda"), table.cuda(), ln.cuda()).cpu()
+        assert got[3, Tq - 1, 7].isnan().all()
+        keep = torch.ones(12, Tq, 32, dtype=torch.bool)
+        keep[3, Tq - 1, 7] = False
+        close(got[keep], want[keep], off[keep])
+
+
 @pytest.mark.parametrize("Tq", [1, 40])
 @pytest.mark.parametrize("dtype", [BF, HF])
 def test_attention_scales_far_apart(lsa, Tq, dtype):
@@ -196,9 +231,9 @@ def wait_limit():
 
 @pytest.mark.parametrize("code,D,page,B,Tq,Hq,Hkv,T", [
     ("e4m3", 128, 64, 20, 16, 32, 4, 3000),  # two streams, split
-    ("int8", 64, 16, 2, 40, 8, 4, 700),
+    ("int8", 64, 16, 24, 40, 8, 4, 700),
     ("e4m3", 128, 128, 40, 64, 32, 4, 900),  # both halves, whole tiles and split ones
-    ("int8", 64, 32, 3, 257, 6, 2, 257),
+    ("int8", 64, 32, 12, 257, 6, 2, 257),
 ])
 def test_expired_waits_leave_with_their_copies_landed(lsa, wait_limit, code, D, page, B, Tq, Hq, Hkv, T):
     """Every role gives up at its first wait, with the first copies in flight. The call reports it, and calls after it,
