@@ -36,7 +36,9 @@ template <int D, int NT, bool LISTS> struct QuantShape {
     static constexpr int kTile = kKeys * D;            // K or V bytes of a tile
     static constexpr int kStage = 2 * kTile + kKeys * 12;  // + ks, vs (then its logarithm) and 1 / vs of every key
     static constexpr int kWarpBytes = (kRing * kStage + 127) / 128 * 128;
-    static constexpr int kSmem = kWarps * kWarpBytes + (kWarps + 1) * kRows * 2 * 4;
+    static constexpr int kIn = kWarps * kWarpBytes + kWarps * kRows * 2 * 4;  // what a cluster's CTAs send: sums, lse
+    static constexpr int kItems = kRows * D / 4;                              // of 4 columns
+    static constexpr int kSmem = kIn + kItems * 20;
     static_assert(kWarpBytes >= kRows * D * 4, "the join reuses a warp's ring");
     static_assert(kStage % 16 == 0, "16-byte copies");
 };
@@ -64,27 +66,24 @@ __device__ __forceinline__ uint64_t lds64(uint32_t addr) {
     asm volatile("ld.shared.b64 %0, [%1];" : "=l"(r) : "r"(addr) : "memory");
     return r;
 }
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+// The cluster's barrier, by whole warps.
+__device__ __forceinline__ void cluster_arrive() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 }
-// From CTA `rank` of the cluster's shared memory, at the address that this CTA has for the same thing.
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// The address that CTA `rank` of the cluster has for what this CTA has at `addr`.
 __device__ __forceinline__ uint32_t peer(uint32_t addr, int rank) {
     uint32_t r;
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
-__device__ __forceinline__ float2 peer_f2(uint32_t addr, int rank) {
-    float2 r;
-    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(r.x), "=f"(r.y) : "r"(peer(addr, rank)) : "memory");
-    return r;
-}
-__device__ __forceinline__ float4 peer_f4(uint32_t addr, int rank) {
-    float4 r;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                 : "=f"(r.x), "=f"(r.y), "=f"(r.z), "=f"(r.w)
-                 : "r"(peer(addr, rank))
+__device__ __forceinline__ void send_f4(uint32_t addr, const float4& x) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(x.x), "f"(x.y), "f"(x.z), "f"(x.w)
                  : "memory");
-    return r;
+}
+__device__ __forceinline__ void send_f1(uint32_t addr, float x) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(x) : "memory");
 }
 template <typename T> __device__ __forceinline__ void store4(T* dst, const float4& x) {
     const T y[4] = {from_f32<T>(x.x), from_f32<T>(x.y), from_f32<T>(x.z), from_f32<T>(x.w)};
@@ -143,6 +142,7 @@ __global__ void __launch_bounds__(kWarps * 32, QuantShape<D, NT, LISTS>::kCTAs) 
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, c = lane & 3;
+    if (a.cluster) cluster_arrive();
     grid_wait();
     grid_trigger();
     // (parts, KV heads x row tiles, sequences)
@@ -191,8 +191,8 @@ __global__ void __launch_bounds__(kWarps * 32, QuantShape<D, NT, LISTS>::kCTAs) 
     const uint32_t ring = smem_u32(smem) + warp * Sh::kWarpBytes;
     const int tiles = k1 - k0 > warp * kKeys ? (k1 - k0 - warp * kKeys + kWarps * kKeys - 1) / (kWarps * kKeys) : 0;
 
-    // Tile i of this warp: keys k0 + (warp + 4 i) 32 ..; a lane looks its key up, two tiles ahead the position, one
-    // the page; then the warp copies the rows.
+    // Tile i of this warp: keys k0 + (warp + 4 i) 32 ..; a lane looks its key up, three tiles ahead the position,
+    // two the page; then the warp copies the rows.
     auto position = [&](int i) {
         const int key = k0 + (warp + kWarps * i) * kKeys + lane;
         const bool in = i < tiles && key < k1;
@@ -350,14 +350,17 @@ __global__ void __launch_bounds__(kWarps * 32, QuantShape<D, NT, LISTS>::kCTAs) 
                 }
             }
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const uint32_t at = scales + (t * 16 + e * 8 + g) * 4;
-                const float key_scale = __uint_as_float(lds32(at)), lv = __uint_as_float(lds32(at + kKeys * 4));
+            for (int e = 0; e < 2; ++e)
 #pragma unroll
-                for (int u = 0; u < NT; ++u)
-                    x[u][2 * t + e] = fma2(mul2(pair(s[u][2 * e], s[u][2 * e + 1]), pair(key_scale, key_scale)), factor[u],
-                                           pair(lv, lv));
-            }
+                for (int u = 0; u < NT; ++u) x[u][2 * t + e] = pair(s[u][2 * e], s[u][2 * e + 1]);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t at = scales + (k * 8 + g) * 4;
+            const float key_scale = __uint_as_float(lds32(at)), lv = __uint_as_float(lds32(at + kKeys * 4));
+#pragma unroll
+            for (int u = 0; u < NT; ++u)
+                x[u][k] = fma2(mul2(x[u][k], pair(key_scale, key_scale)), factor[u], pair(lv, lv));
         }
         if (!LISTS && key0 + kKeys > first_limit) {  // rows before the tile's last see less
 #pragma unroll
@@ -475,7 +478,7 @@ __global__ void __launch_bounds__(kWarps * 32, QuantShape<D, NT, LISTS>::kCTAs) 
         const int tok = token_of(a, r0 + r);
         return ((int64_t)b * a.Tq + tok) * a.Hq + (int64_t)h * a.G + (r0 + r - tok * a.G);
     };
-    float2* joined = sml + kWarps * kRows;  // the CTA's (maximum, sum) of a row
+    if (a.cluster) cluster_wait();  // every CTA of the cluster runs: its memory may be written
     for (int i = threadIdx.x; i < live * (D / 4); i += kWarps * 32) {
         const int r = i / (D / 4), col = i % (D / 4) * 4;
         float top = -INFINITY;
@@ -491,14 +494,15 @@ __global__ void __launch_bounds__(kWarps * 32, QuantShape<D, NT, LISTS>::kCTAs) 
             total = fmaf(f, ml.y, total);
             x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w);
         }
-        if (a.cluster) {  // left where warp 0's were: no other thread reads these
-            *reinterpret_cast<float4*>(smem + (r * D + col) * 4) = x;
-            if (col == 0) joined[r] = make_float2(top, total);
-            continue;
-        }
         const float norm = total == 0.0f ? 0.0f : 1.0f / total;
         x.x *= norm, x.y *= norm, x.z *= norm, x.w *= norm;
         const float lse = total == 0.0f ? -INFINITY : top + (log2f(total) - kLift);
+        if (a.cluster) {  // to the CTA that joins these columns: every parts-th item, in the sender's place
+            const int to = i & (a.parts - 1), at = split * (live * (D / 4) / a.parts) + i / a.parts;
+            send_f4(peer(smem_u32(smem + Sh::kIn) + at * 16, to), x);
+            send_f1(peer(smem_u32(smem + Sh::kIn) + Sh::kItems * 16 + at * 4, to), lse);
+            continue;
+        }
         const int64_t rid = row_id(r);
         if (a.parts == 1) {
             store4<T>(static_cast<T*>(a.out) + rid * D + col, x);
@@ -511,35 +515,32 @@ __global__ void __launch_bounds__(kWarps * 32, QuantShape<D, NT, LISTS>::kCTAs) 
     }
     if (!a.cluster) return;
     __syncwarp();
-    // A cluster holds all parts of its rows: they join through its CTAs' shared memory, a part of the columns each.
-    cluster_sync();
-    const uint32_t base = smem_u32(smem), stats = smem_u32(joined);
-    for (int i = threadIdx.x * a.parts + split; i < live * (D / 4); i += a.parts * kWarps * 32) {
-        const int r = i / (D / 4), col = i % (D / 4) * 4;
-        float top = -INFINITY, total = 0.0f;
-        float4 x = make_float4(0, 0, 0, 0), y[kMostCluster];
-        float2 ml[kMostCluster];
+    // A cluster holds all parts of its rows: every CTA has the others' sums of its own columns once all have arrived.
+    cluster_arrive();
+    cluster_wait();
+    const int per = live * (D / 4) / a.parts;
+    for (int j = threadIdx.x; j < per; j += kWarps * 32) {
+        const int i = j * a.parts + split, r = i / (D / 4), col = i % (D / 4) * 4;
+        float top = -INFINITY, total = 0.0f, lse[kMostCluster];
+        float4 x = make_float4(0, 0, 0, 0);
 #pragma unroll
         for (int p = 0; p < kMostCluster; ++p) {
-            ml[p] = make_float2(-INFINITY, 0.0f), y[p] = x;
-            if (p < a.parts) ml[p] = peer_f2(stats + r * 8, p), y[p] = peer_f4(base + (r * D + col) * 4, p);
+            lse[p] = p < a.parts ? *reinterpret_cast<const float*>(smem + Sh::kIn + Sh::kItems * 16 + (p * per + j) * 4) : -INFINITY;
+            top = fmaxf(top, lse[p]);
         }
 #pragma unroll
-        for (int p = 0; p < kMostCluster; ++p) top = fmaxf(top, ml[p].x);
-#pragma unroll
         for (int p = 0; p < kMostCluster; ++p) {
-            const float f = ml[p].y == 0.0f ? 0.0f : ex2_approx(ml[p].x - top);
-            total = fmaf(f, ml[p].y, total);
-            x.x = fmaf(f, y[p].x, x.x), x.y = fmaf(f, y[p].y, x.y), x.z = fmaf(f, y[p].z, x.z), x.w = fmaf(f, y[p].w, x.w);
+            if (p >= a.parts) break;
+            const float4 y = *reinterpret_cast<const float4*>(smem + Sh::kIn + (p * per + j) * 16);
+            const float f = lse[p] == -INFINITY ? 0.0f : ex2_approx(lse[p] - top);  // NaN passes on
+            total += f;
+            x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w);
         }
         const float norm = total == 0.0f ? 0.0f : 1.0f / total;
         const int64_t rid = row_id(r);
         store4<T>(static_cast<T*>(a.out) + rid * D + col, make_float4(x.x * norm, x.y * norm, x.z * norm, x.w * norm));
-        if (col == 0 && a.lse)
-            a.lse[rid] = total == 0.0f ? -INFINITY : (top + (log2f(total) - kLift)) * 0.69314718055994531f;
+        if (col == 0 && a.lse) a.lse[rid] = total == 0.0f ? -INFINITY : (top + log2f(total)) * 0.69314718055994531f;
     }
-    __syncwarp();
-    cluster_sync();  // no CTA leaves while another reads its memory
 }
 
 // The parts of a row joined, SPREAD warps a row (one where the parts are few, so that a CTA takes eight rows). Every

@@ -268,7 +268,7 @@ def check_status(device=None, what: str = "lsa") -> None:
 def after_call(device: torch.device, what: str) -> None:
     """The checked mode (LSA_CHECK_STATUS=1, read per call): synchronise and raise on a
     failure word right after the launch - skipped while a CUDA graph is being captured."""
-    if os.environ.get("LSA_CHECK_STATUS", "0") != "1":
+    if "LSA_CHECK_STATUS" not in os.environ or os.environ["LSA_CHECK_STATUS"] != "1":  # a get that finds nothing costs more
         return
     if torch.cuda.is_current_stream_capturing():
         return
