@@ -4,7 +4,11 @@
 // it has where older tokens stay on the page and need more; older codes follow a scale that grows. A power of
 // two, so that growing moves e4m3's exponents and changes no other bit above its smallest step, and an integer's
 // successive roundings stay within one step of its scale. One CTA (or warp) a (sequence, page, KV head, K or V):
-// the new rows stay in registers between the maximum and the codes, so every byte moves once.
+// the new rows stay in registers, as they lie in memory, between the maximum and the codes, so every byte moves once.
+// Measured (B200, 8 heads, D 128, bf16 to e4m3, pages of 64): 4 x 16383 tokens, 403 MB, 76 us = 5.3 TB/s, 82 % of the
+// measured copy rate; bounded by the loads' latency behind the length and the table (six CTAs an SM) and by the ALU pipe
+// (65 % active: unpacking, magnitudes, conversions). K and V in one CTA: 95 us (two CTAs an SM); eight CTAs an SM with
+// spilled registers: 89. 64 tokens: 2.0 us as graph replays, 6.6 in a loop (the host).
 #include <type_traits>
 
 #include "quant.cuh"

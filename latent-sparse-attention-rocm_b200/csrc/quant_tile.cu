@@ -9,15 +9,23 @@
 // With at most 128 rows both halves hold the same rows and take alternate chunks, so that two softmax chains are in
 // flight where the keys' bandwidth is the bound.
 // The codes come as they are (bulk copies of a page's rows of a head, which are contiguous) into a ring of 8-bit tiles;
-// two warps, and softmax warps that no row wants, make halves of
-// them (exact) into a ring of operand tiles, zeros where there is no key, so what a page holds
-// behind a sequence's last token never meets a product. Scales stay out of the tiles: 16 keys share a page, so a
-// row's logits are s * (ks * factor) + log2 vs with constants for 16 keys, and the sum takes 1 / vs once for 16.
+// two warps, and softmax warps that no row wants, make halves of them (exact) into a ring of operand tiles, zeros where
+// there is no key, so what a page holds behind a sequence's last token never meets a product. Scales stay out of the
+// tiles: 16 keys (64 on pages of 64 or 128) share theirs, so a row's logits are s * (ks * factor) + log2 vs with
+// constants for them, and the sum takes 1 / vs once.
 // bf16 rows of Q become fp16 by a power of two of their own, as in the few-row kernel. P is rounded to fp16 and
 // carries 2^kLift; the maximum is let stand until it has grown by more than 2^kGrow.
 //
 // Warps: 0 asks for the codes and the scales, one thread of warp 1 issues every MMA, 2 and 3 convert, 4-7 / 8-11 are
 // the softmax of half 0 / 1. TMEM: S_0/P_0 [0, 128), S_1/P_1 [128, 256), O_0 [256, 256 + D), O_1 [384, 384 + D).
+//
+// What bounds it (B200, 32 / 8 heads, D 128): with two halves of rows the chain of a half - softmax 2350 cycles, then its
+// product and the next S 1100 - of which two run at a time: 3500 cycles a pair of chunks, where the MMAs take 2048 and the
+// exponentials as many; 2 x 1024 tokens on 16384 keys 541 us = 0.98 PFLOP/s in a loop (70 % of the measured sustained
+// rate), 512 us = 1.04 PFLOP/s in bursts. With two streams, converting: about 1000 cycles a tile for two warps (500 alone;
+// shared memory and the ALU pipe are the softmax's and the MMAs' too), 32 tokens on 65536 keys 65 us = 2.1 TB/s. Not
+// kept: four more converting warps (a thread's 128 logits want 146 registers), loads of the next codes before the
+// stores of these (no change).
 //
 // Every wait is bounded (QuantArgs::wait_ns); an expired wait raises a CTA-wide flag, every role leaves, copies and
 // MMAs in flight are waited for (bounded), the TMEM is released and LSA_ERR_TIMEOUT lands in the status word.
@@ -37,7 +45,7 @@ constexpr int kGroups = kChunk / 16;
 template <int D> struct QuantTile {
     static constexpr int kOperand = kChunk * D * 2;  // an fp16 K, V or half-Q tile
     static constexpr int kCodes = kChunk * D;        // its codes
-    // Operand tiles and tiles of codes. A tile of one half's rows has the other half of Q for two more (D = 64: four).
+    // Operand tiles and tiles of codes. A tile of one half's rows has the other half of Q for two more.
     static constexpr int kOps = D == 128 ? 3 : 6, kStages = D == 128 ? 4 : 5, kMore = kOperand / kCodes;
     static constexpr int kOffOps = 2 * kOperand;
     static constexpr int kOffStage = kOffOps + kOps * kOperand;

@@ -9,7 +9,11 @@
 //
 // A warp holds a token's heads one after another, D / 8 lanes a head, and its lanes' angles once for all of them. A
 // lane has four values of either half and so both of a pair, in the half layout as in the interleaved one (two
-// 8-byte loads where one of 16 would want its partner's values by shuffle).
+// 8-byte loads where one of 16 would want its partner's values by shuffle: 213 us became 138 with the packed
+// arithmetic). A token's heads go to several warps where the tokens alone would not fill the SMs.
+// Measured (B200, 32 + 8 heads, D 128, bf16, norms): 2 x 16384 tokens, 671 MB, 125 us = 5.4 TB/s, 83 % of the measured copy
+// rate; bounded by issue (57 %) and the loads' latency together: 80 registers leave 24 warps an SM, and bounding them to
+// 64 spills (158 us). 64 tokens: 2.5 us as graph replays, 8.9 called in a loop (the host).
 #include "pairs.cuh"
 
 namespace lsa {
