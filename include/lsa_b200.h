@@ -94,7 +94,7 @@ int lsa_norm_rotate(const void* q, const void* k, int dtype, const int64_t* stri
 
 /* A paged cache in 8 bits (no reference counterpart): k8 / v8 [pages, Hkv, page, D] codes (code 0: e4m3, 1: int8),
  * k_scale / v_scale [pages, Hkv] fp32, all contiguous, codes 16-byte aligned; page 16, 32, 64 or 128, D 64 or 128,
- * pages * Hkv * page below 2^31. table [rows, M] int32, rows table_ld apart: token t of sequence b is row t % page of
+ * pages * Hkv * page below 2^31; at most 65535 sequences. table [rows, M] int32, rows table_ld apart: token t of sequence b is row t % page of
  * page table[b][t / page]; entries outside [0, pages) hold nothing. M * page at most 2^30. */
 
 /* Append: k / v [B, Tq, Hkv, D] (dtype) at strides[6] as above; row i is token lengths[b] - Tq + i of sequence b; rows

@@ -115,7 +115,8 @@ int run(QuantArgs& a, int dtype, int code, int64_t D, int64_t keys, float scale,
     a.scale_log2 = scale * 1.4426950408889634f;
     if (!(a.scale_log2 > 0) || !isfinite(a.scale_log2)) return LSA_ERR_ARG;
     if (reinterpret_cast<uintptr_t>(a.q) % 16 != 0 || reinterpret_cast<uintptr_t>(a.out) % 16 != 0) return LSA_ERR_ARG;
-    if (a.q_b % 8 != 0 || a.q_t % 8 != 0 || a.q_h % 8 != 0) return LSA_ERR_ARG;
+    for (int64_t st : {a.q_b, a.q_t, a.q_h})
+        if (st < 0 || st % 8 != 0) return LSA_ERR_ARG;
     a.G_inverse = a.G > 1 ? (uint32_t)(((1ull << 32) + a.G - 1) / a.G) : 0;
     const Plan p = make_plan(a.B, a.Tq, a.Hq, a.Hkv, D, keys, a.lists != nullptr);
     if (p.bytes > 0 && (scratch == nullptr || scratch_bytes < p.bytes || reinterpret_cast<uintptr_t>(scratch) % 16 != 0))

@@ -238,7 +238,7 @@ int lsa_append_quantized(const void* k, const void* v, int dtype, const int64_t*
     if (!k || !v || !k8 || !v8 || !k_scale || !v_scale || !table || !lengths) return LSA_ERR_ARG;
     const int64_t unit = 16 / (dtype == kF32 ? 4 : 2);
     for (int i = 0; i < 6; ++i)
-        if (strides[i] % unit != 0) return LSA_ERR_ARG;
+        if (strides[i] < 0 || strides[i] % unit != 0) return LSA_ERR_ARG;
     for (const void* p : {k, v, (const void*)k8, (const void*)v8})
         if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return LSA_ERR_ARG;
     if (pages > INT32_MAX || M > INT32_MAX || B > INT32_MAX || Tq > INT32_MAX || Hkv > 65535) return LSA_ERR_SIZE;

@@ -4,8 +4,8 @@
 //   y = x * rsqrt(mean(x^2) + eps) * w                      (where a weight is given)
 //   (a, b) -> amplitude * (a cos t - b sin t, a sin t + b cos t),  t = p f_i,  i < R / 2
 // over the pairs (y_i, y_{i + R/2}) or, interleaved, (y_2i, y_2i+1); the values past R are not rotated. All in
-// fp32, rounded once. The angle in turns is p * (f / 2 pi) in fp64, reduced there to half a turn either way:
-// what is left of a position's 2^-53 is the angle's error, whatever the position.
+// fp32, rounded once. The angle in turns is p * (f / 2 pi) in fp64, reduced there to half a turn either way
+// (off by 2^-27 of a turn at most below position 2^26) and then rounded to fp32.
 //
 // A warp holds a token's heads one after another, D / 8 lanes a head, and its lanes' angles once for all of them. A
 // lane has four values of either half and so both of a pair, in the half layout as in the interleaved one (two
@@ -223,7 +223,7 @@ extern "C" int lsa_norm_rotate(const void* q, const void* k, int dtype, const in
     if (!q || !k || !positions || (R > 0 && !frequencies) || !q_out || !k_out) return LSA_ERR_ARG;
     const int64_t unit = 16 / (dtype == kF32 ? 4 : 2);
     for (int i = 0; i < 6; ++i)
-        if (strides[i] % unit != 0) return LSA_ERR_ARG;
+        if (strides[i] < 0 || strides[i] % unit != 0) return LSA_ERR_ARG;
     for (const void* p : {q, k, (const void*)q_out, (const void*)k_out, q_weight, k_weight})
         if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return LSA_ERR_ARG;
     if (T > INT32_MAX || Hq + Hkv > 65536 || B > INT64_MAX / (T * 65536)) return LSA_ERR_SIZE;

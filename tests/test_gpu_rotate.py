@@ -12,8 +12,10 @@ def plain(x, positions, f, weight, eps, interleaved, amplitude):
     """(output, how far off a kernel may be), 64 bits on the CPU.
 
     fp32: the mean of D squares, its root, two products and the rotation's two products and sum are at most D + 16
-    roundings of 2^-24 of the pair's magnitudes; sine and cosine 2^-22 (the angle is reduced to 2^-29 of a turn at
-    positions below 2^26); the output is rounded once."""
+    roundings of 2^-24 of the pair's magnitudes (some fifteen of them in earnest: the mean's error is halved by the root
+    and its additions are pairwise; the others leave room for the special-function unit's sine and cosine of 16-bit
+    values, 2^-21); sine and cosine of fp32 values 2^-22 with the rounding of the reduced angle, 2^-26 of a turn; the
+    output is rounded once."""
     y = x.double()
     D, R = y.shape[-1], 2 * f.numel()
     if weight is not None:
