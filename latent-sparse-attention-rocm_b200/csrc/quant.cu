@@ -9,7 +9,6 @@ namespace lsa {
 namespace {
 
 constexpr int kSMs = 148;
-constexpr int kFewRows = 16;  // rows of the few-row kernel's tiles
 constexpr int kUnit = 128;      // keys that a CTA's four warps take at a time
 constexpr int kMaxTileParts = 32, kMostRounds = 8;  // splits of a tile; rounds of the SMs that split tiles fill
 constexpr double kItemCost = 1.5, kJoinCost = 3.0;  // a CTA's start and end, the join's launch, in units' times
@@ -51,7 +50,7 @@ Plan make_plan(int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_
         p.bytes = p.part_rows * (p.streams ? 2 : 1) * p.parts * (D + 1) * 4;
         return p;
     }
-    const int64_t tiles = (Tq * G + kFewRows - 1) / kFewRows, items = B * Hkv * tiles;
+    const int64_t tile = few_tile_rows(rows, lists), tiles = (rows + tile - 1) / tile, items = B * Hkv * tiles;
     // Parts. One CTA in each of two places an SM draws the memory's whole rate; a third place only evens out ragged
     // sequences, and a round that fills some SMs' third place and not others' is the worst (us in parts, CTAs in
     // brackets; 32 / 8 heads, D 128): 1 x 32k 37 (296) 16.1, 42 (336) 17.8, 56 (448) 20.2; 4 x 16k 9 (288) 24.5, 14 (448)

@@ -128,6 +128,9 @@ __device__ __forceinline__ int64_t quant_part_row(const QuantArgs& a, int split,
                      : split * a.part_rows + (int64_t)rest * 256 + hf * 128 + rl;
 }
 
+// Rows of the few-row kernel's tiles for so many rows of a sequence and KV head.
+inline int few_tile_rows(int64_t rows, bool lists) { return rows <= 16 || lists ? 16 : 32; }
+
 int launch_quant_tiles(const QuantArgs& a, int dtype, int code, int D, cudaStream_t stream);
 int launch_quant_rows(const QuantArgs& a, int dtype, int code, int D, cudaStream_t stream);
 int launch_quant_join(const QuantArgs& a, int dtype, int D, cudaStream_t stream);

@@ -1,12 +1,12 @@
 // quant_rows.cu - attention over the 8-bit paged cache for few rows, and its sparse read (sm_100a).
 // quant.cuh has the formulas.
 //
-// A work item is at most 16 query rows of one KV head (a sequence's last tokens; of the read one token's G query
+// A work item is at most 32 query rows of one KV head (a sequence's last tokens; of the read one token's G query
 // heads) x a range of keys. The keys' bytes bound it: 2 D a key and head. So nothing waits for a neighbour in the
 // main loop: each of a CTA's four warps copies its own tiles of 32 keys (cp.async, 16 bytes, kRing tiles in
 // flight) and runs its own online softmax on them. S^T = K Q^T and O^T += V^T P^T by mma.sync.m16n8k16 in fp16:
-// keys, then columns of V, are the M = 16 side and the rows the N = 8 (twice for more than eight), so few rows cost
-// few accumulators. The codes become halves in registers on their way into the fragments, which is exact:
+// keys, then columns of V, are the M = 16 side and the rows the N = 8 (twice for more than eight, four times for more
+// than 16), so few rows cost few accumulators. The codes become halves in registers on their way into the fragments, which is exact:
 //   K: a lane takes 16 bytes of key g = lane / 4 at a time, four consecutive bytes a k-step; Q's fragments are
 //      loaded in the same order of D, which a product does not see.
 //   V: a lane takes D / 8 bytes of four keys and makes pairs of two keys' codes (the fragment's order) by byte
@@ -41,13 +41,15 @@ constexpr float kLift = 10.0f, kGrow = 5.0f;
 template <int D, int NT, bool LISTS> struct QuantShape {
     static constexpr int kRows = 8 * NT;
     static constexpr int kCTAs = NT == 1 && !LISTS ? 3 : 2;             // an SM
-    static constexpr int kRing = D == 128 ? (kCTAs == 3 ? 2 : 3) : (kCTAs == 3 ? 4 : 5);  // tiles in a warp's ring
+    // tiles in a warp's ring
+    static constexpr int kRing = D == 128 ? (kCTAs == 3 || NT == 4 ? 2 : 3) : (kCTAs == 3 || NT == 4 ? 4 : 5);
     static constexpr int kTile = kKeys * D;            // K or V bytes of a tile
     static constexpr int kStage = 2 * kTile + kKeys * 12;  // + ks, vs (then its logarithm) and 1 / vs of every key
     static constexpr int kWarpBytes = (kRing * kStage + 127) / 128 * 128;
     static constexpr int kIn = kWarps * kWarpBytes + kWarps * kRows * 2 * 4;  // what a cluster's CTAs send: sums, lse
     static constexpr int kItems = kRows * D / 4;                              // of 4 columns
-    static constexpr int kSmem = kIn + kItems * 20;
+    static constexpr int kQ = kIn + kItems * 20;  // Q's fragments and the rows' factors, of 32 rows
+    static constexpr int kSmem = kQ + (NT == 4 ? kRows * D * 2 + kRows * 4 : 0);
     static_assert(kWarpBytes >= kRows * D * 4, "the join reuses a warp's ring");
     static_assert(kStage % 16 == 0, "16-byte copies");
 };
@@ -140,7 +142,7 @@ template <int D> __device__ __forceinline__ uint32_t v_at(int r, int c) {
     return D == 128 ? r * 128 + ((c ^ (r & 6)) << 4) : (r >> 1) * 128 + (((((r & 1) << 2) | c) ^ (r & 6)) << 4);
 }
 
-// NT: tiles of eight rows.
+// NT: tiles of eight rows. Of four, each warp makes the fragments of one, and they are read from shared memory.
 template <typename T, int CODE, int D, bool LISTS, int NT>
 __global__ void __launch_bounds__(kWarps * 32, QuantShape<D, NT, LISTS>::kCTAs) quant_rows_kernel(const QuantArgs a, const int row_tiles) {
     using Sh = QuantShape<D, NT, LISTS>;
@@ -162,15 +164,19 @@ __global__ void __launch_bounds__(kWarps * 32, QuantShape<D, NT, LISTS>::kCTAs) 
     const int live = nrows - r0 < kRows ? nrows - r0 : kRows;
     // Q's rows are asked for before what the lengths say is known: row r0 + g (and + 8); k-step kk's four values of a
     // lane are D's 16 (c + 4 (kk / 4)) + 4 (kk % 4) + 0..3
-    uint2 raw[NT][KS];
+    constexpr bool kShared = NT == 4;
+    constexpr int NQ = kShared ? 1 : NT;
+    uint32_t qf[NQ][KS][2];  // as they are, then as halves
 #pragma unroll
-    for (int u = 0; u < NT; ++u) {
-        const int r = r0 + g + 8 * u, tok = token_of(a, r);
+    for (int u = 0; u < NQ; ++u) {
+        const int r = r0 + g + 8 * (kShared ? warp : u), tok = token_of(a, r);
         const T* src = static_cast<const T*>(a.q) + b * a.q_b + tok * a.q_t + (h * (int64_t)a.G + r - tok * a.G) * a.q_h;
 #pragma unroll
-        for (int kk = 0; kk < KS; ++kk)
-            raw[u][kk] = r < nrows ? *reinterpret_cast<const uint2*>(src + 16 * (c + 4 * (kk >> 2)) + 4 * (kk & 3))
-                                   : make_uint2(0, 0);
+        for (int kk = 0; kk < KS; ++kk) {
+            const uint2 raw = r < nrows ? *reinterpret_cast<const uint2*>(src + 16 * (c + 4 * (kk >> 2)) + 4 * (kk & 3))
+                                        : make_uint2(0, 0);
+            qf[u][kk][0] = raw.x, qf[u][kk][1] = raw.y;
+        }
     }
     // keys: positions of the sequence, or entries of the list
     int trow = b, length, keys;
@@ -200,8 +206,8 @@ __global__ void __launch_bounds__(kWarps * 32, QuantShape<D, NT, LISTS>::kCTAs) 
     const uint32_t ring = smem_u32(smem) + warp * Sh::kWarpBytes;
     const int tiles = k1 - k0 > warp * kKeys ? (k1 - k0 - warp * kKeys + kWarps * kKeys - 1) / (kWarps * kKeys) : 0;
 
-    // Tile i of this warp: keys k0 + (warp + 4 i) 32 ..; a lane looks its key up, three tiles ahead the position,
-    // two the page; then the warp copies the rows.
+    // Tile i of this warp: keys k0 + (warp + 4 i) 32 ..; a lane looks its key up, two tiles ahead the position, one
+    // the page; then the warp copies the rows.
     auto position = [&](int i) {
         const int key = k0 + (warp + kWarps * i) * kKeys + lane;
         const bool in = i < tiles && key < k1;
@@ -271,39 +277,53 @@ __global__ void __launch_bounds__(kWarps * 32, QuantShape<D, NT, LISTS>::kCTAs) 
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     // Q's fragments, as halves
-    uint32_t qf[NT][KS][2];
     uint64_t factor[NT];  // of rows r0 + 2c and 2c + 1 (and + 8), as the maxima and sums below
     int limit[NT][2];
+    const uint32_t qs = smem_u32(smem + Sh::kQ), fs = qs + kRows * D * 2;
+    auto prepare = [&]() {
 #pragma unroll
-    for (int u = 0; u < NT; ++u) {
-        float f = a.scale_log2;
-        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-            uint32_t top = 0;  // largest magnitude's bits, as a bf16
+        for (int u = 0; u < NQ; ++u) {
+            float f = a.scale_log2;
+            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                uint32_t top = 0;  // largest magnitude's bits, as a bf16
 #pragma unroll
-            for (int kk = 0; kk < KS; ++kk) {
-                const uint32_t w[2] = {raw[u][kk].x, raw[u][kk].y};
+                for (int kk = 0; kk < KS; ++kk)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) top = max(top, max(w[e] & 0x7FFFu, (w[e] >> 16) & 0x7FFFu));
+                    for (int e = 0; e < 2; ++e)
+                        top = max(top, max(qf[u][kk][e] & 0x7FFFu, (qf[u][kk][e] >> 16) & 0x7FFFu));
+                top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+                top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+                const float by = half_factor(top, &f);
+#pragma unroll
+                for (int kk = 0; kk < KS; ++kk)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        qf[u][kk][e] = pack_half(__uint_as_float(qf[u][kk][e] << 16) * by,
+                                                 __uint_as_float(qf[u][kk][e] & 0xFFFF0000u) * by);
             }
-            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-            const float by = half_factor(top, &f);
+            if constexpr (kShared) {
 #pragma unroll
-            for (int kk = 0; kk < KS; ++kk) {
-                qf[u][kk][0] = pack_half(__uint_as_float(raw[u][kk].x << 16) * by, __uint_as_float(raw[u][kk].x & 0xFFFF0000u) * by);
-                qf[u][kk][1] = pack_half(__uint_as_float(raw[u][kk].y << 16) * by, __uint_as_float(raw[u][kk].y & 0xFFFF0000u) * by);
+                for (int kk = 0; kk < KS; ++kk)
+                    asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(qs + ((kk * NT + warp) * 32 + lane) * 8),
+                                 "r"(qf[u][kk][0]), "r"(qf[u][kk][1])
+                                 : "memory");
+                if (c == 0) sts_f32(fs + (warp * 8 + g) * 4, f);
+            } else {
+                factor[u] = pair(__shfl_sync(0xFFFFFFFFu, f, 8 * c), __shfl_sync(0xFFFFFFFFu, f, 8 * c + 4));
             }
-        } else {
-#pragma unroll
-            for (int kk = 0; kk < KS; ++kk) qf[u][kk][0] = raw[u][kk].x, qf[u][kk][1] = raw[u][kk].y;
         }
-        factor[u] = pair(__shfl_sync(0xFFFFFFFFu, f, 8 * c), __shfl_sync(0xFFFFFFFFu, f, 8 * c + 4));
+        if constexpr (kShared) __syncthreads();
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int row = r0 + 8 * u + 2 * c + e;
-            limit[u][e] = row >= nrows ? 0 : length - a.Tq + token_of(a, row) + 1;
+        for (int u = 0; u < NT; ++u) {
+            if constexpr (kShared) factor[u] = lds64(fs + (8 * u + 2 * c) * 4);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int row = r0 + 8 * u + 2 * c + e;
+                limit[u][e] = row >= nrows ? 0 : length - a.Tq + token_of(a, row) + 1;
+            }
         }
-    }
+    };
+    if (kShared) prepare();  // by all warps; else behind the first copies
     const int first_limit = length - a.Tq + token_of(a, r0) + 1;  // keys that the tile's first row sees
     float o[NT][MT][4];  // O^T: columns (D / 8) g + 2 j (0, 1) and + 1 (2, 3) of rows 2c (0, 2) and 2c + 1 (1, 3)
 #pragma unroll
@@ -323,6 +343,7 @@ __global__ void __launch_bounds__(kWarps * 32, QuantShape<D, NT, LISTS>::kCTAs) 
     for (int i = 1 - Sh::kRing; i < tiles; ++i) {
         copy(i + Sh::kRing - 1);
         if (i < 0) continue;
+        if (!kShared && i == 0) prepare();
         asm volatile("cp.async.wait_group %0;" ::"n"(Sh::kRing - 1) : "memory");
         const uint32_t ks = ring + read * Sh::kStage, vs = ks + Sh::kTile, scales = vs + Sh::kTile;
         if (++read == Sh::kRing) read = 0;
@@ -338,30 +359,63 @@ __global__ void __launch_bounds__(kWarps * 32, QuantShape<D, NT, LISTS>::kCTAs) 
         // logits x[u][k]: key 8 k + g, rows 2c and 2c + 1, with the value scale in the exponent; -inf where there is no
         // key, or none for the row
         uint64_t x[NT][4];
+        if constexpr (!kShared) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            float s[NT][4];
+            for (int t = 0; t < 2; ++t) {
+                float s[NT][4];
+#pragma unroll
+                for (int u = 0; u < NT; ++u)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[u][e] = 0.0f;
+#pragma unroll
+                for (int hh = 0; hh < KS / 4; ++hh) {
+                    uint32_t w0[4], w1[4];
+                    lds_words<4>(w0, ks + k_at<D>(t * 16 + g, c + 4 * hh));
+                    lds_words<4>(w1, ks + k_at<D>(t * 16 + 8 + g, c + 4 * hh));
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) {
+                        const uint32_t kf[4] = {halves_of<CODE>(w0[kk], 0), halves_of<CODE>(w1[kk], 0),
+                                                halves_of<CODE>(w0[kk], 1), halves_of<CODE>(w1[kk], 1)};
+#pragma unroll
+                        for (int u = 0; u < NT; ++u) mma_f16(s[u], kf, qf[u][4 * hh + kk][0], qf[u][4 * hh + kk][1]);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int u = 0; u < NT; ++u) x[u][2 * t + e] = pair(s[u][2 * e], s[u][2 * e + 1]);
+            }
+        } else {
+            float s[2][NT][4];
 #pragma unroll
             for (int u = 0; u < NT; ++u)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[u][e] = 0.0f;
+                for (int e = 0; e < 4; ++e) s[0][u][e] = s[1][u][e] = 0.0f;
 #pragma unroll
             for (int hh = 0; hh < KS / 4; ++hh) {
-                uint32_t w0[4], w1[4];
-                lds_words<4>(w0, ks + k_at<D>(t * 16 + g, c + 4 * hh));
-                lds_words<4>(w1, ks + k_at<D>(t * 16 + 8 + g, c + 4 * hh));
+                uint32_t w[4][4];
+#pragma unroll
+                for (int y = 0; y < 4; ++y) lds_words<4>(w[y], ks + k_at<D>(y * 8 + g, c + 4 * hh));
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk) {
-                    const uint32_t kf[4] = {halves_of<CODE>(w0[kk], 0), halves_of<CODE>(w1[kk], 0),
-                                            halves_of<CODE>(w0[kk], 1), halves_of<CODE>(w1[kk], 1)};
+                    uint32_t kf[2][4];
 #pragma unroll
-                    for (int u = 0; u < NT; ++u) mma_f16(s[u], kf, qf[u][4 * hh + kk][0], qf[u][4 * hh + kk][1]);
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) kf[t][e] = halves_of<CODE>(w[2 * t + (e & 1)][kk], e >> 1);
+#pragma unroll
+                    for (int u = 0; u < NT; ++u) {
+                        uint32_t q[2];
+                        lds_words<2>(q, qs + (((4 * hh + kk) * NT + u) * 32 + lane) * 8);
+                        mma_f16(s[0][u], kf[0], q[0], q[1]);
+                        mma_f16(s[1][u], kf[1], q[0], q[1]);
+                    }
                 }
             }
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
+            for (int u = 0; u < NT; ++u)
 #pragma unroll
-                for (int u = 0; u < NT; ++u) x[u][2 * t + e] = pair(s[u][2 * e], s[u][2 * e + 1]);
+                for (int k = 0; k < 4; ++k) x[u][k] = pair(s[k >> 1][u][2 * (k & 1)], s[k >> 1][u][2 * (k & 1) + 1]);
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -644,18 +698,23 @@ __global__ void __launch_bounds__(256) quant_join_kernel(const QuantArgs a, cons
 
 template <typename T, int CODE, int D, bool LISTS, int NT>
 int launch(const QuantArgs& a, int row_tiles, dim3 grid, cudaStream_t stream) {
-    constexpr int smem = QuantShape<D, NT, LISTS>::kSmem;
-    if (!allow_kernel<quant_rows_kernel<T, CODE, D, LISTS, NT>>(smem, true)) return LSA_ERR_CUDA;
+    // A grid of one round on two places an SM takes so much shared memory that no SM has a third: its CTAs start while
+    // those of the launch before leave, and would gather where places are free first (4 x 16k keys 28.8 us, so 24.4).
+    constexpr int least = QuantShape<D, NT, LISTS>::kSmem, two = 100 << 10;
+    const int smem = (int64_t)grid.x * grid.y * grid.z <= 2 * 148 && least < two ? two : least;
+    if (!allow_kernel<quant_rows_kernel<T, CODE, D, LISTS, NT>>(least < two ? two : least, true)) return LSA_ERR_CUDA;
     return launch_clusters(quant_rows_kernel<T, CODE, D, LISTS, NT>, grid, kWarps * 32, smem, stream,
                            a.cluster ? a.parts : 1, a, row_tiles);
 }
 template <typename T, int CODE, int D>
 int launch(const QuantArgs& a, int row_tiles, dim3 grid, cudaStream_t stream) {
-    if (a.Tq * a.G <= 8)
-        return a.lists ? launch<T, CODE, D, true, 1>(a, row_tiles, grid, stream)
-                       : launch<T, CODE, D, false, 1>(a, row_tiles, grid, stream);
-    return a.lists ? launch<T, CODE, D, true, 2>(a, row_tiles, grid, stream)
-                   : launch<T, CODE, D, false, 2>(a, row_tiles, grid, stream);
+    const int rows = a.Tq * a.G;
+    if (a.lists)
+        return rows <= 8 ? launch<T, CODE, D, true, 1>(a, row_tiles, grid, stream)
+                         : launch<T, CODE, D, true, 2>(a, row_tiles, grid, stream);
+    if (rows > 16) return launch<T, CODE, D, false, 4>(a, row_tiles, grid, stream);
+    return rows <= 8 ? launch<T, CODE, D, false, 1>(a, row_tiles, grid, stream)
+                     : launch<T, CODE, D, false, 2>(a, row_tiles, grid, stream);
 }
 template <typename T> int launch(const QuantArgs& a, int code, int D, int row_tiles, dim3 grid, cudaStream_t stream) {
     if (code == kE4M3)
@@ -666,7 +725,7 @@ template <typename T> int launch(const QuantArgs& a, int code, int D, int row_ti
 }  // namespace
 
 int launch_quant_rows(const QuantArgs& a, int dtype, int code, int D, cudaStream_t stream) {
-    const int row_tiles = (a.Tq * a.G + 15) / 16;
+    const int rows = few_tile_rows((int64_t)a.Tq * a.G, a.lists != nullptr), row_tiles = (a.Tq * a.G + rows - 1) / rows;
     if (a.B > 65535 || (int64_t)a.Hkv * row_tiles > 65535) return LSA_ERR_SIZE;
     const dim3 grid((unsigned)a.parts, (unsigned)(a.Hkv * row_tiles), (unsigned)a.B);
     return dtype == kBF16 ? launch<__nv_bfloat16>(a, code, D, row_tiles, grid, stream)
