@@ -28,12 +28,13 @@ Plan make_plan(int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_
     const int64_t G = Hq / Hkv, chunks = (keys + kUnit - 1) / kUnit;
     p.part_rows = B * Tq * Hq;
     p.parts = 1;
-    // The few-row kernel reads the keys once for each 16 rows, from L2 after the first time, and converts them in
+    // The few-row kernel reads the keys once for each 32 rows, from L2 after the first time, and converts them in
     // registers; the tensor-core kernel's converting goes through shared memory, which its products share, and its start
-    // takes 4 us (us, few-row / tensor cores: 32 x 4096 keys, 20-32 rows 89 / 120, 48 rows 159 / 122; 4 x 4096 48 rows 24.9
-    // / 26.9, 64 rows 37 / 26; 1 x 2048 128 rows 13.8 / 18.3, 256 rows 24.7 / 24.4; 1 x 512 512 rows 9.4 / 18.4).
+    // takes 4 us (us, few-row / tensor cores: 32 x 4096 keys, 32 rows 85 / 105, 48 rows 146 / 120; 1 x 65536 32 rows 37 / 45,
+    // 64 rows 62 / 51; 4 x 2048 64 rows 20.4 / 20.9; 1 x 2048 128 rows 15.8 / 18.2, 256 rows 24.7 / 24.4; 1 x 512 128 rows
+    // 10.6 / 13.4).
     const int64_t rows = Tq * G, heads = B * Hkv * keys;
-    const bool few = rows <= 32 || (rows <= 48 && heads <= 1 << 17) || (heads <= 1 << 21 && rows * heads <= 1 << 21);
+    const bool few = rows <= 32 || (rows <= 64 && heads <= 1 << 16) || (heads <= 1 << 21 && rows * heads <= 1 << 21);
     if (!few && G <= 128) {
         // Whole rounds of one tile an SM are not split (no parts to write, read and join); the tiles of the last, short
         // round are, so that it too fills the GPU.
@@ -74,7 +75,7 @@ Plan make_plan(int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_
     if (s > kMaxQuantParts) s = kMaxQuantParts;
     p.parts = s < 1 ? 1 : (int)s;
     // Parts that are a cluster's CTAs join within the launch, which pays where a CTA has little to do (4 x 2k keys, 8
-    // parts: 8.8 us against 10.5); clusters spread unevenly over the SMs (4 x 16k, 8 parts: 29.4 us, in a second launch
+    // parts: 7.2 us against 10.5); clusters spread unevenly over the SMs (4 x 16k, 8 parts: 29.4 us, in a second launch
     // 25.3).
     int c = 1;
     while (2 * c <= kMostCluster && 2 * c <= s && (c < 8 || items * 2 * c <= kSMs)) c *= 2;
