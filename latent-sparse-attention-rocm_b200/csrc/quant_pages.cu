@@ -5,10 +5,10 @@
 // two, so that growing moves e4m3's exponents and changes no other bit above its smallest step, and an integer's
 // successive roundings stay within one step of its scale. One CTA (or warp) a (sequence, page, KV head, K or V):
 // the new rows stay in registers, as they lie in memory, between the maximum and the codes, so every byte moves once.
-// Measured (B200, 8 heads, D 128, bf16 to e4m3, pages of 64): 4 x 16383 tokens, 403 MB, 76 us = 5.3 TB/s, 82 % of the
-// measured copy rate; bounded by the loads' latency behind the length and the table (six CTAs an SM) and by the ALU pipe
-// (65 % active: unpacking, magnitudes, conversions). K and V in one CTA: 95 us (two CTAs an SM); eight CTAs an SM with
-// spilled registers: 89. 64 tokens: 2.0 us as graph replays, 6.6 in a loop (the host).
+// Measured (B200, 8 heads, D 128, bf16 to e4m3, pages of 64): 4 x 16383 tokens, 403 MB, 63 us = 6.4 TB/s, the measured
+// copy rate. What counts is how many CTAs have rows in flight while others look their page up, reduce or store: 128
+// threads with eight rows of 16 bytes each; 256 threads with four 75 us, K and V in one CTA 95, registers bounded for
+// more CTAs (spills) 89. 64 tokens: 2.0 us as graph replays, 6.6 in a loop (the host).
 #include <type_traits>
 
 #include "quant.cuh"
@@ -170,13 +170,13 @@ template <typename T, int CODE, int D> int launch(const AppendArgs& a, cudaStrea
         const dim3 blocks((a.units + 3) / 4, (unsigned)a.B);
         return launch_after(append_kernel<T, CODE, D, 32, kSmallRows * (D / 8) / 32>, blocks, 128, 0, stream, a);
     }
-    constexpr int NT = 2 * D;  // 16 rows a pass
+    constexpr int NT = D;  // 8 rows a pass (4 x 16k tokens, D 128: 128 threads 63 us, 256 75, 512 107)
     const dim3 grid(a.units, (unsigned)a.B);
     switch (a.shift) {
-        case 4: return launch_after(append_kernel<T, CODE, D, NT, 1>, grid, NT, 0, stream, a);
-        case 5: return launch_after(append_kernel<T, CODE, D, NT, 2>, grid, NT, 0, stream, a);
-        case 6: return launch_after(append_kernel<T, CODE, D, NT, 4>, grid, NT, 0, stream, a);
-        default: return launch_after(append_kernel<T, CODE, D, NT, 8>, grid, NT, 0, stream, a);
+        case 4: return launch_after(append_kernel<T, CODE, D, NT, 2>, grid, NT, 0, stream, a);
+        case 5: return launch_after(append_kernel<T, CODE, D, NT, 4>, grid, NT, 0, stream, a);
+        case 6: return launch_after(append_kernel<T, CODE, D, NT, 8>, grid, NT, 0, stream, a);
+        default: return launch_after(append_kernel<T, CODE, D, NT, 16>, grid, NT, 0, stream, a);
     }
 }
 template <typename T> int launch(const AppendArgs& a, int code, int64_t D, cudaStream_t stream) {

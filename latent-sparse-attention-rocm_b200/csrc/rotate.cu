@@ -11,16 +11,16 @@
 // lane has four values of either half and so both of a pair, in the half layout as in the interleaved one (two
 // 8-byte loads where one of 16 would want its partner's values by shuffle: 213 us became 138 with the packed
 // arithmetic). A token's heads go to several warps where the tokens alone would not fill the SMs.
-// Measured (B200, 32 + 8 heads, D 128, bf16, norms): 2 x 16384 tokens, 671 MB, 125 us = 5.4 TB/s, 83 % of the measured copy
-// rate; bounded by issue (57 %) and the loads' latency together: 80 registers leave 24 warps an SM, and bounding them to
-// 64 spills (158 us). 64 tokens: 2.5 us as graph replays, 8.9 called in a loop (the host).
+// Measured (B200, 32 + 8 heads, D 128, bf16, norms): 2 x 16384 tokens, 671 MB, 111 us = 6.1 TB/s, 94 % of the measured copy
+// rate; bounded by issue and the loads' latency together: 80 registers leave 24 warps an SM, and bounding them to 64
+// spills (158 us). 64 tokens: 2.5 us as graph replays, 8.8 called in a loop (the host).
 #include "pairs.cuh"
 
 namespace lsa {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kAhead = 4;  // rows a lane group has in flight
+constexpr int kAhead = 3;  // rows a lane group has in flight (2 x 16k tokens: 2 120 us, 3 111, 4 122, 6 118, 8 127)
 
 struct RotateArgs {
     const void *q, *k;
