@@ -20,9 +20,9 @@
 // the softmax of half 0 / 1. TMEM: S_0/P_0 [0, 128), S_1/P_1 [128, 256), O_0 [256, 256 + D), O_1 [384, 384 + D).
 //
 // What bounds it (B200, 32 / 8 heads, D 128): with two halves of rows the chain of a half - softmax 2350 cycles, then its
-// product and the next S 1100 - of which two run at a time: 3500 cycles a pair of chunks, where the MMAs take 2048 and the
-// exponentials as many; 2 x 1024 tokens on 16384 keys 541 us = 0.98 PFLOP/s in a loop (70 % of the measured sustained
-// rate), 512 us = 1.04 PFLOP/s in bursts. With two streams, converting: about 1000 cycles a tile for two warps (500 alone;
+// product and the next S 1100 - of which two run at a time: 3400 cycles a pair of chunks, where the MMAs take 2048 and the
+// exponentials as many; 2 x 1024 tokens on 16384 keys 536 us = 0.99 PFLOP/s in a loop (70 % of the measured sustained
+// rate), 494 us = 1.08 PFLOP/s in bursts. With two streams, converting: about 1000 cycles a tile for two warps (500 alone;
 // shared memory and the ALU pipe are the softmax's and the MMAs' too), 32 tokens on 65536 keys 65 us = 2.1 TB/s. Not
 // kept: four more converting warps (a thread's 128 logits want 146 registers), loads of the next codes before the
 // stores of these (no change).
@@ -178,10 +178,15 @@ __device__ __forceinline__ void load_q(const QuantArgs& a, const Item& w, uint8_
     }
 }
 
+// How many 16-key steps of P are handed over ahead of the others: half, where a step's constants are at hand (2 x 1024
+// tokens on 16384 keys 494 us in bursts, with six 517; pages of 16 619 against 585, D 64 244 against 238).
+template <int D, int GK> constexpr int kFirst = GK == 64 && D == 128 ? 4 : 6;
+
 template <typename T, int D, int GK>
 __device__ __forceinline__ void softmax_half(const QuantArgs& a, const Item& w, uint8_t* sm, uint64_t* bar_s, uint64_t* bar_p,
                                              uint64_t* bar_o, volatile int* abort_flag, uint32_t tmem) {
     using Sh = QuantTile<D>;
+    constexpr int FIRST = kFirst<D, GK>;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int hf = (warp - 4) >> 2, qd = warp & 3;
     int tok, g;
@@ -217,7 +222,7 @@ __device__ __forceinline__ void softmax_half(const QuantArgs& a, const Item& w, 
                 if (i >= seen) s[i] = 0xFF800000u;  // -inf
         }
         // The exponentials start from the maximum of the chunks before, while this chunk's is found beside them. Only
-        // when it has grown by more than 2^kGrow does the warp take the new one, do the first 96 keys again and rescale O
+        // when it has grown by more than 2^kGrow does the warp take the new one, do the first keys again and rescale O
         // - always on a row's first chunk.
         float alpha = 1.0f;
         uint64_t sum;
@@ -262,13 +267,16 @@ __device__ __forceinline__ void softmax_half(const QuantArgs& a, const Item& w, 
         for (bool again = false;; again = true) {
             neg = (m == -INFINITY ? 0.0f : -m) + kLift;
             sum = 0ull;
-            uint32_t pk[32], pk2[16];
+            uint32_t pk[32];
 #pragma unroll
             for (int i = 0; i < 4; ++i) exps(pk, 8 * i, i, neg);
             tmem_st32(tS, pk);
+            if constexpr (FIRST == 6) {
+                uint32_t pk2[16];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) exps(pk2, 8 * i, 4 + i, neg);
-            tmem_st16(tS + 32, pk2);
+                for (int i = 0; i < 2; ++i) exps(pk2, 8 * i, 4 + i, neg);
+                tmem_st16(tS + 32, pk2);
+            }
             if (again) break;
             float mx = -INFINITY;
 #pragma unroll
@@ -304,10 +312,13 @@ __device__ __forceinline__ void softmax_half(const QuantArgs& a, const Item& w, 
         }
         publish(&bar_p[2 * hf]);
         {
-            uint32_t pk2[16];
+            uint32_t rest[8 * (kGroups - FIRST)];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) exps(pk2, 8 * i, 6 + i, neg);
-            tmem_st16(tS + 48, pk2);
+            for (int i = 0; i < kGroups - FIRST; ++i) exps(rest, 8 * i, FIRST + i, neg);
+            if constexpr (FIRST == 6)
+                tmem_st16(tS + 48, rest);
+            else
+                tmem_st32(tS + 32, rest);
         }
         publish(&bar_p[2 * hf + 1]);
         float s0, s1;
@@ -504,7 +515,7 @@ __device__ __forceinline__ void convert(const QuantArgs& a, const Item& w, uint8
 template <typename T, int CODE, int D, int GK>
 __global__ void __launch_bounds__(kThreads, 1) quant_tile_kernel(const QuantArgs a) {
     using Sh = QuantTile<D>;
-    constexpr int NO = Sh::kOps, KS = D / 16, kAll = Sh::kStages + Sh::kMore;
+    constexpr int NO = Sh::kOps, KS = D / 16, kAll = Sh::kStages + Sh::kMore, FIRST = kFirst<D, GK>;
     extern __shared__ __align__(1024) uint8_t sm[];
     const int NS = a.streams ? kAll : Sh::kStages;
     const uint32_t sbase = smem_u32(sm);
@@ -596,7 +607,7 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tile_kernel(const QuantArgs
                     }
                     umma_commit(&bar_s[hf]);
                 };
-                // P_h's first 96 and last 32 keys as they come; O_h starts afresh on a half's first chunk
+                // P_h's first keys and the others as they come; O_h starts afresh on a half's first chunk
                 auto product = [&](int hf, int st, bool fresh, uint32_t parity) -> bool {
                     const uint64_t vd = desc_at(vd0, st * Sh::kOperand);
                     const uint32_t o = tmem + 256 + hf * 128, p = tmem + hf * 128;
@@ -605,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tile_kernel(const QuantArgs
                         if (!thread_wait(&bar_p[2 * hf + half], parity, abort_flag, a.wait_ns)) return false;
                         tc_fence_after();
 #pragma unroll
-                        for (int kk = 6 * half; kk < 6 + 2 * half; ++kk)
+                        for (int kk = FIRST * half; kk < (half ? kGroups : FIRST); ++kk)
                             umma_f16_ts(o, p + kk * 8, desc_at(vd, kk * 2048), idO, kk > 0 || !fresh);
                     }
                     return true;
