@@ -113,3 +113,16 @@ def test_empty_stream_and_graph(lsa):
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(x, y) and torch.equal(x, z) for x, y, z in zip(want, again, out))
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_infinities_that_do_not_turn_stay_their_own(lsa, dtype, interleaved):
+    """Without a norm every value past the first R leaves as it came, whatever lies beside it."""
+    g = torch.Generator().manual_seed(4)
+    q, k = (torch.randn(1, 2, 3, 128, generator=g).to(dtype) for _ in range(2))
+    q[0, 0, 0, 32], q[0, 1, 2, 127], q[0, 1, 1, 77] = math.inf, -math.inf, math.nan
+    f, _ = lsa.rotary_frequencies(32)
+    a, b = lsa.norm_rotate(q.cuda(), k.cuda(), torch.arange(2).cuda(), f.cuda(), interleaved=interleaved)
+    assert torch.equal(a.cpu()[..., 32:].nan_to_num(7.0), q[..., 32:].nan_to_num(7.0)) and torch.equal(b.cpu()[..., 32:], k[..., 32:])
+    assert bool(a.cpu()[..., :32].isfinite().all()) and bool((a.cpu().isnan() == q.isnan()).all())
