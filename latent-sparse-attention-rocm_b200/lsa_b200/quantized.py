@@ -246,8 +246,11 @@ class QuantizedCache:
 
     def fork(self, place: int) -> int:
         """A free place that holds what ``place`` holds, on the same pages; whichever of the two writes to
-        a shared page first takes a copy of it then."""
+        a shared page first takes a copy of it then. ``place`` holds something: an empty one's fork would be
+        free still, for the next fork to take."""
         (place,) = self._places([place], "fork")
+        if not self._held[place]:
+            raise ValueError(f"fork: place {place} is empty")
         free = next((i for i, held in enumerate(self._held) if not held and i != place), None)
         if free is None:
             raise ValueError("fork: no free place")

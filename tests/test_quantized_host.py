@@ -69,6 +69,14 @@ def test_both_of_a_fork_write_in_one_call(plain):
     assert len({x[0] for x in cache._held}) == 3 and cache.free_pages == 3
 
 
+def test_an_empty_place_has_no_fork(plain):
+    cache = plain.QuantizedCache(3, 6, 1, 64, 16, device="cpu")
+    with pytest.raises(ValueError):
+        cache.fork(0)  # its fork would be place 1, and the next fork's too
+    cache.append([0], *given(1, 5))
+    assert cache.fork(0) == 1 and cache.fork(0) == 2
+
+
 def test_cache_refusals_leave_it_as_it_was(plain):
     cache = plain.QuantizedCache(2, 3, 2, 64, 16, device="cpu")
     k, v = given(1, 30, Hkv=2)
