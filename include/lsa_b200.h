@@ -116,7 +116,8 @@ int lsa_move_pages(void* k8, void* v8, float* k_scale, float* v_scale, int64_t p
  * logarithm) or NULL. scale > 0, scale * log2(e) finite in fp32. status: a device int32 that receives
  * LSA_ERR_TIMEOUT if a bounded wait expires (their limit is lsa_shared_prefix_wait_limit's).
  * lsa_quantized_scratch: the scratch bytes of a call with that many keys a sequence at most (M * page; W for the
- * read, with Tq 1 and lists not 0), LSA_ERR_ARG for refused sizes. */
+ * read, with Tq 1 and lists not 0), LSA_ERR_ARG or LSA_ERR_SIZE for refused sizes (of more than 128 query heads a KV
+ * head at most 2^21 rows, Tq * Hq, among them). */
 int64_t lsa_quantized_scratch(int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_t keys, int lists);
 int lsa_quantized_attention(const void* q, int dtype, const int64_t* q_strides, const void* k8, const void* v8,
                             const float* k_scale, const float* v_scale, int code, int64_t pages, int64_t page,

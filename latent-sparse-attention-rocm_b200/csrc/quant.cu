@@ -33,7 +33,7 @@ Plan make_plan(int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_
     // takes 4 us (us, few-row / tensor cores: 32 x 4096 keys, 32 rows 85 / 105, 48 rows 146 / 120; 1 x 65536 32 rows 37 / 45,
     // 64 rows 62 / 51; 4 x 2048 64 rows 20.4 / 20.9; 1 x 2048 128 rows 15.8 / 18.2, 256 rows 24.7 / 24.4; 1 x 512 128 rows
     // 10.6 / 13.4).
-    const int64_t rows = Tq * G, heads = B * Hkv * keys;
+    const int64_t rows = Tq * G, heads = B * Hkv * (keys < kUnit ? kUnit : keys);
     const bool few = rows <= 32 || (rows <= 64 && heads <= 1 << 16) || (heads <= 1 << 21 && rows * heads <= 1 << 21);
     if (!few && G <= 128) {
         // Whole rounds of one tile an SM are not split (no parts to write, read and join); the tiles of the last, short
@@ -51,7 +51,7 @@ Plan make_plan(int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_
         p.bytes = p.part_rows * (p.streams ? 2 : 1) * p.parts * (D + 1) * 4;
         return p;
     }
-    const int64_t tile = few_tile_rows(rows, lists), tiles = (rows + tile - 1) / tile, items = B * Hkv * tiles;
+    const int64_t items = B * Hkv * few_row_tiles(rows, lists);
     // Parts. One CTA in each of two places an SM draws the memory's whole rate; a third place only evens out ragged
     // sequences, and a round that fills some SMs' third place and not others' is the worst (us in parts, CTAs in
     // brackets; 32 / 8 heads, D 128): 1 x 32k 37 (296) 16.1, 42 (336) 17.8, 56 (448) 20.2; 4 x 16k 9 (288) 24.5, 14 (448)
@@ -142,7 +142,9 @@ int64_t lsa_quantized_scratch(int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, in
     using namespace lsa;
     if (!sizes_ok(B, Tq, Hq, Hkv, D, keys)) return LSA_ERR_ARG;
     if (B == 0 || Tq == 0) return 0;
-    return make_plan(B, Tq, Hq, Hkv, D, keys, lists != 0).bytes;
+    const Plan p = make_plan(B, Tq, Hq, Hkv, D, keys, lists != 0);
+    if (p.tokens == 0 && Hkv * few_row_tiles(Tq * (Hq / Hkv), lists != 0) > 65535) return LSA_ERR_SIZE;
+    return p.bytes;
 }
 
 int lsa_quantized_attention(const void* q, int dtype, const int64_t* q_strides, const void* k8, const void* v8,

@@ -130,6 +130,9 @@ __device__ __forceinline__ int64_t quant_part_row(const QuantArgs& a, int split,
 
 // Rows of the few-row kernel's tiles for so many rows of a sequence and KV head.
 inline int few_tile_rows(int64_t rows, bool lists) { return rows <= 16 || lists ? 16 : 32; }
+inline int64_t few_row_tiles(int64_t rows, bool lists) {
+    return (rows + few_tile_rows(rows, lists) - 1) / few_tile_rows(rows, lists);
+}
 
 int launch_quant_tiles(const QuantArgs& a, int dtype, int code, int D, cudaStream_t stream);
 int launch_quant_rows(const QuantArgs& a, int dtype, int code, int D, cudaStream_t stream);

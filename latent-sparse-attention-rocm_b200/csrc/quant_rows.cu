@@ -725,8 +725,9 @@ template <typename T> int launch(const QuantArgs& a, int code, int D, int row_ti
 }  // namespace
 
 int launch_quant_rows(const QuantArgs& a, int dtype, int code, int D, cudaStream_t stream) {
-    const int rows = few_tile_rows((int64_t)a.Tq * a.G, a.lists != nullptr), row_tiles = (a.Tq * a.G + rows - 1) / rows;
-    if (a.B > 65535 || (int64_t)a.Hkv * row_tiles > 65535) return LSA_ERR_SIZE;
+    const int64_t tiles = few_row_tiles((int64_t)a.Tq * a.G, a.lists != nullptr);
+    if (a.B > 65535 || a.Hkv * tiles > 65535) return LSA_ERR_SIZE;
+    const int row_tiles = (int)tiles;
     const dim3 grid((unsigned)a.parts, (unsigned)(a.Hkv * row_tiles), (unsigned)a.B);
     return dtype == kBF16 ? launch<__nv_bfloat16>(a, code, D, row_tiles, grid, stream)
                           : launch<__half>(a, code, D, row_tiles, grid, stream);

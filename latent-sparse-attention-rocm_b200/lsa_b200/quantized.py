@@ -114,8 +114,8 @@ class QuantizedCache:
 
     def __init__(self, places: int, pages: int, kv_heads: int, head_dim: int, page: int = 64,
                  dtype=torch.float8_e4m3fn, device="cuda"):
-        if places < 1 or pages < 1:
-            raise ValueError(f"a cache has places and pages, got {places} and {pages}")
+        if not 1 <= places <= 65535 or pages < 1:
+            raise ValueError(f"a cache has pages and 1 to 65535 places, got {pages} and {places}")
         if page not in (16, 32, 64, 128) or head_dim not in (64, 128) or kv_heads < 1:
             raise ValueError(f"pages of 16, 32, 64 or 128 tokens and heads of 64 or 128, got {page} and {head_dim}")
         if dtype not in (torch.float8_e4m3fn, torch.int8):
@@ -171,6 +171,8 @@ class QuantizedCache:
         counts = [Tq] * len(places) if counts is None else [int(c) for c in counts]
         if len(counts) != len(places) or any(c < 0 or c > Tq for c in counts):
             raise ValueError(f"append: one count in [0, {Tq}] a place, got {counts}")
+        if any(self.lengths[p] + c > 1 << 30 for p, c in zip(places, counts)):
+            raise ValueError("append: a sequence holds at most 2^30 tokens")
         need, refs = 0, {}
         copies = []
         for p, c in zip(places, counts):
@@ -231,7 +233,11 @@ class QuantizedCache:
             raise ValueError(f"step: q is fp16 or bf16 [n, Tq, a multiple of {Hkv}, {D}], got {q.dtype} {list(q.shape)}")
         if scale is not None and not (0.0 < float(scale) < float("inf")):
             raise ValueError(f"step: the scale must be positive, got {scale}")
-        self._grow(places, None, k.shape[1])
+        n, Tq = q.shape[:2]
+        M = max([-(-(self.lengths[p] + Tq) // self.page) for p in places], default=0)
+        if _lib.lib().lsa_quantized_scratch(n, Tq, q.shape[2], Hkv, D, M * self.page, 0) < 0:
+            raise ValueError(f"step: sizes out of range, q {list(q.shape)}")
+        self._grow(places, None, Tq)
         table, lengths, _ = self._upload(places)
         if places:
             append_quantized(self.pages, k, v, table, lengths)

@@ -197,6 +197,25 @@ def test_attention_empty(lsa, shape):
     assert out.shape == q.shape and bool((out == 0).all()) and bool((lse == -math.inf).all())
 
 
+@pytest.mark.parametrize("M", [0, 1])
+def test_attention_many_rows_on_no_key(lsa, M):
+    """Rows of a long call whose table maps nothing, or one page behind almost all of them."""
+    pages = lsa.QuantizedPages.new(4, 8, 16, 64)
+    q = torch.zeros(1, 1 << 15, 64, 64, device="cuda", dtype=BF)
+    table = torch.zeros(1, M, dtype=torch.int32, device="cuda")
+    if M:
+        ones = torch.ones(1, 5, 8, 64, device="cuda")
+        lsa.append_quantized(pages, ones, ones, table, torch.tensor([5]).cuda())
+    out, lse = lsa.quantized_attention(q, pages, table, torch.tensor([5]).cuda(), return_lse=True)
+    seen = 5 * M
+    assert bool((out[:, :(1 << 15) - seen] == 0).all()) and bool((lse[:, :(1 << 15) - seen] == -math.inf).all())
+    if M:  # equal logits of zero: the values' mean, and the number of keys
+        assert bool((out[:, -seen:] == 1).all())
+        want = torch.arange(1, 6, device="cuda").log()[None, :, None].expand(1, 5, 64)
+        # log2 of a sum of up to 2^20.4, an ulp off, and two more roundings below it
+        assert bool(((lse[:, -seen:] - want).abs() <= 2.0 ** -18).all())
+
+
 @pytest.mark.parametrize("Tq,Hq,Hkv", [(1, 160, 1), (2, 33, 1), (3, 130, 1), (9, 21, 3)])
 def test_attention_head_groups(lsa, Tq, Hq, Hkv):
     """Groups of odd sizes, and of more heads than a row tile of the tensor cores holds."""

@@ -105,6 +105,9 @@ def test_cache_refusals_leave_it_as_it_was(plain):
     refused(cache.step, [0], q[:, :2].float(), k[:, :2], v[:, :2])
     refused(cache.step, [0], q[:, :2, :3], k[:, :2], v[:, :2])
     refused(cache.step, [0], q[:, :2], k[:, :2], v[:, :2], scale=0.0)
+    # rows that the attention has no grid for, before anything is appended
+    refused(cache.step, [0], q[:1, :1, :1].expand(1, 1 << 24, 128, 64), k[:1, :1].expand(1, 1 << 24, 2, 64),
+            v[:1, :1].expand(1, 1 << 24, 2, 64))
     refused(cache.attend, [0, 1], q)
     refused(cache.fork, 5)
     cache.append([1], *given(1, 3, Hkv=2))
@@ -112,7 +115,7 @@ def test_cache_refusals_leave_it_as_it_was(plain):
         cache.fork(0)  # no free place
 
 
-@pytest.mark.parametrize("bad", [dict(places=0), dict(pages=0), dict(page=24), dict(head_dim=96), dict(kv_heads=0),
+@pytest.mark.parametrize("bad", [dict(places=0), dict(places=65536), dict(pages=0), dict(page=24), dict(head_dim=96), dict(kv_heads=0),
                                  dict(dtype=torch.uint8)])
 def test_cache_sizes_refused(lsa, bad):
     with pytest.raises(ValueError):
@@ -198,6 +201,10 @@ def test_entry_points_refuse_before_any_launch(lsa):
     assert read(R=2) == ERR_ARG and read(counts=None) == ERR_ARG and read(W=-1) == ERR_ARG and read(R=0) == OK
     assert L.lsa_move_pages(some, some, some, some, 4, 24, 1, 64, some, some, 1, None) == ERR_ARG
     assert L.lsa_move_pages(some, some, some, some, 4, 16, 1, 64, some, some, 0, None) == OK
+    # query heads beyond the tensor cores' tiles: rows without a grid
+    assert L.lsa_quantized_scratch(1, 1 << 13, 256, 1, 64, 4096, 0) == ERR_SIZE
+    assert L.lsa_quantized_scratch(1, 1 << 12, 256, 1, 64, 4096, 0) >= 0
+    assert all(L.lsa_quantized_scratch(1, 1 << 20, 16, 4, 64, n, 0) >= 0 for n in (0, 16, 64, 4096))
     assert L.lsa_quantized_scratch(1, 1, 3, 2, 64, 100, 0) == ERR_ARG and L.lsa_quantized_scratch(0, 1, 2, 1, 64, 100, 0) == 0
 
 
