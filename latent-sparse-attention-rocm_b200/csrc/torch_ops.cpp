@@ -431,6 +431,11 @@ std::tuple<at::Tensor, at::Tensor> norm_rotate_cuda(const at::Tensor& q_in, cons
     return {qo, ko};
 }
 
+// Lengths, pages and positions as contiguous int32; those of 64 bits saturate, so that what lies outside stays outside.
+at::Tensor as_ids(const at::Tensor& t) {
+    return as_lengths(t.scalar_type() == at::kLong ? t.clamp(INT32_MIN, INT32_MAX) : t);
+}
+
 // The pool of an 8-bit paged cache, as it is (it is written in place, and too large to copy).
 struct Pool {
     int code;
@@ -470,7 +475,7 @@ at::Tensor check_table(const at::Tensor& table, const at::Tensor& lengths, const
     TORCH_CHECK_VALUE(table.size(1) <= (1 << 30) / p.page, what, ": a table of at most 2^30 tokens a sequence");
     if (table.scalar_type() == at::kInt && (table.size(1) <= 1 || table.stride(1) == 1) && (table.size(0) <= 1 || table.stride(0) >= 0))
         return table;
-    return table.to(at::kInt).contiguous();
+    return as_ids(table);
 }
 
 void append_quantized_cuda(const at::Tensor& k_in, const at::Tensor& v_in, const at::Tensor& k8, const at::Tensor& v8,
@@ -488,13 +493,13 @@ void append_quantized_cuda(const at::Tensor& k_in, const at::Tensor& v_in, const
                       ": k and v fp32, fp16 or bf16, of one type, got ", dt, ", ", v_in.scalar_type());
     c10::cuda::CUDAGuard guard(k8.device());
     auto table = check_table(table_in, lengths_in, p, k8.device(), what);
-    auto lengths = as_lengths(lengths_in);
+    auto lengths = as_ids(lengths_in);
     at::Tensor counts;
     if (counts_in) {
         TORCH_CHECK_VALUE(counts_in->is_cuda() && counts_in->device() == k8.device() && !counts_in->is_floating_point() &&
                               counts_in->numel() == k_in.size(0),
                           what, ": one whole count a sequence, on the pool's device");
-        counts = as_lengths(*counts_in);
+        counts = as_ids(*counts_in);
     }
     auto k = rows16(k_in), v = rows16(v_in);
     const int64_t strides[6] = {stride_of(k, 0), stride_of(k, 1), stride_of(k, 2),
@@ -519,7 +524,7 @@ void move_pages_cuda(const at::Tensor& k8, const at::Tensor& v8, const at::Tenso
                           !dst_in.is_floating_point(),
                       what, ": src and dst [n] of whole numbers");
     c10::cuda::CUDAGuard guard(k8.device());
-    auto src = as_lengths(src_in), dst = as_lengths(dst_in);
+    auto src = as_ids(src_in), dst = as_ids(dst_in);
     check_rc(lsa_move_pages(k8.data_ptr(), v8.data_ptr(), ks.data_ptr<float>(), vs.data_ptr<float>(), p.pages, p.page,
                             p.Hkv, p.D, src.data_ptr<int32_t>(), dst.data_ptr<int32_t>(), src.size(0),
                             at::cuda::getCurrentCUDAStream()),
@@ -548,7 +553,7 @@ std::pair<at::Tensor, at::Tensor> quantized(const at::Tensor& q_in, const at::Te
     TORCH_CHECK_VALUE(table_in.dim() == 2 && table_in.size(0) == B, what, ": a table row a sequence");
     c10::cuda::CUDAGuard guard(k8.device());
     auto table = check_table(table_in, lengths_in, p, k8.device(), what);
-    auto lengths = as_lengths(lengths_in);
+    auto lengths = as_ids(lengths_in);
     auto q = rows16(q_in);
     auto out = fresh({B, Tq, Hq, p.D}, q.scalar_type(), q.device());
     at::Tensor lse;
@@ -599,9 +604,9 @@ at::Tensor quantized_read_cuda(const at::Tensor& q_in, const at::Tensor& k8, con
                       ": without rows, a table row a query row");
     c10::cuda::CUDAGuard guard(k8.device());
     auto table = check_table(table_in, lengths_in, p, k8.device(), what);
-    auto lengths = as_lengths(lengths_in), counts = as_lengths(counts_in), lists = as_lengths(lists_in);
+    auto lengths = as_ids(lengths_in), counts = as_ids(counts_in), lists = as_ids(lists_in);
     at::Tensor rows;
-    if (rows_in) rows = as_lengths(*rows_in);
+    if (rows_in) rows = as_ids(*rows_in);
     auto q = rows16(q_in);
     auto out = fresh({R, 1, Hq, p.D}, q.scalar_type(), q.device());
     if (R == 0) return out;

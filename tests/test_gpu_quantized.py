@@ -409,6 +409,30 @@ def test_append_padding_counts_and_holes(lsa):
     same(dev, pages)
 
 
+def test_indexes_of_64_bits_that_wrap(lsa):
+    """Pages, positions and lengths beyond 32 bits are outside, not what they are modulo 2^32."""
+    g = torch.Generator().manual_seed(12)
+    pages = lsa.QuantizedPages.new(4, 1, 16, 64)
+    k, v = (torch.randn(1, 48, 1, 64, generator=g).cuda() for _ in range(2))
+    wrap = 1 << 32
+    lsa.append_quantized(pages, k, v, torch.tensor([[1, 2 + wrap, 3]]).cuda(), torch.tensor([48]).cuda())
+    assert not bool(pages.k[2].float().any()) and bool(pages.k[3].float().any())
+    before = [t.clone() for t in pages]
+    lsa.move_pages(pages, torch.tensor([1 + wrap, 1]).cuda(), torch.tensor([0, 2 + wrap]).cuda())
+    same(pages, before)
+    q = torch.randn(1, 1, 2, 64, generator=g).to(BF).cuda()
+    hole = torch.tensor([[1, -1, 3]], dtype=torch.int32).cuda()
+    want = lsa.quantized_attention(q, pages, hole, torch.tensor([48]).cuda())
+    for table, length in (([1, 2 + wrap, 3], 48), ([1, -1, 3], wrap + 5)):
+        # of the second, more tokens than the table has room for: all of its keys
+        assert torch.equal(lsa.quantized_attention(q, pages, torch.tensor([table]).cuda(), torch.tensor([length]).cuda()), want)
+    lists = torch.tensor([[0, 3 + wrap, 40, -wrap]]).cuda()
+    one = lsa.quantized_read(q, pages, hole, torch.tensor([48]).cuda(), lists, torch.tensor([wrap + 3]).cuda())
+    two = lsa.quantized_read(q, pages, hole, torch.tensor([48]).cuda(), torch.tensor([[0, 40]]).cuda(),
+                             torch.tensor([2]).cuda(), torch.tensor([0]).cuda())
+    assert torch.equal(one, two)
+
+
 def test_append_and_move_of_nothing(lsa):
     pages = lsa.QuantizedPages.new(2, 1, 16, 64)
     before = [t.clone() for t in pages]
