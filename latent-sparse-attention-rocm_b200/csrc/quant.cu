@@ -32,16 +32,22 @@ Plan make_plan(int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_
     // registers; the tensor-core kernel's converting goes through shared memory, which its products share, and its start
     // takes 4 us (us, few-row / tensor cores: 32 x 4096 keys, 32 rows 85 / 105, 48 rows 146 / 120; 1 x 65536 32 rows 37 / 45,
     // 64 rows 62 / 51; 4 x 2048 64 rows 20.4 / 20.9; 1 x 2048 128 rows 15.8 / 18.2, 256 rows 24.7 / 24.4; 1 x 512 128 rows
-    // 10.6 / 13.4).
+    // 10.6 / 13.4). Many sequences hide that kernel's chains and leave its join's traffic: 48 rows, 64 x 2048 147 / 135,
+    // 128 x 2048 237 / 262, 1024 x 1024 1069 / 1364.
     const int64_t rows = Tq * G, heads = B * Hkv * (keys < kUnit ? kUnit : keys);
-    const bool few = rows <= 32 || (rows <= 64 && heads <= 1 << 16) || (heads <= 1 << 21 && rows * heads <= 1 << 21);
+    const bool few = rows <= 32 || (rows <= 64 && (heads <= 1 << 16 || B * Hkv > 6 * kSMs)) ||
+                     (heads <= 1 << 21 && rows * heads <= 1 << 21);
     if (!few && G <= 128) {
         // Whole rounds of one tile an SM are not split (no parts to write, read and join); the tiles of the last, short
         // round are, so that it too fills the GPU.
         p.tokens = (int)(128 / G);
-        p.streams = Tq <= p.tokens;
         p.tiles = (int)((Tq + 2 * p.tokens - 1) / (2 * p.tokens));
-        const int64_t all = B * Hkv * p.tiles, split = p.streams ? all : all % kSMs;
+        const int64_t all = B * Hkv * p.tiles;
+        // Two streams write two parts a row: of more items than kMostRounds they would want more scratch than the other
+        // calls and gain nothing by it (96 rows, streams / whole tiles: 128 x 2048 261 / 292, 256 x 2048 507 / 572, 512 x
+        // 1024 707 / 687, 1024 x 512 1142 / 956).
+        p.streams = Tq <= p.tokens && all <= kMostRounds * kSMs;
+        const int64_t split = p.streams ? all : all % kSMs;
         const int64_t most = split ? kMostRounds * kSMs / split : 0;
         p.parts = balance(split, chunks, 4, kSMs, (int)(most < 1 ? 1 : (most < kMaxTileParts ? most : kMaxTileParts)));
         if (p.parts < 1) p.parts = 1;

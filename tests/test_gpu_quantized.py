@@ -186,6 +186,17 @@ def test_attention_beyond_32_bits(lsa):
          [s.view(torch.int8)[[0, 2]].view(s.dtype) if s.element_size() == 1 else s[[0, 2]] for s in small])
 
 
+@pytest.mark.parametrize("Tq", [12, 24, 31])
+def test_attention_many_sequences(lsa, Tq):
+    """More (sequence, KV head) pairs than the split tiles' rounds: nothing is kept for them beside the output."""
+    g = torch.Generator().manual_seed(Tq)
+    lengths = torch.randint(0, 200, (1201,), generator=g).tolist()
+    attend_case(lsa, 40 + Tq, lengths, Tq, 4, 1, 64, 32, "e4m3", BF)
+    from lsa_b200 import _lib
+
+    assert _lib.lib().lsa_quantized_scratch(1 << 14, Tq, 4, 1, 64, 224, 0) <= 157 << 20
+
+
 @pytest.mark.parametrize("shape", [(0, 1, 3), (2, 0, 3), (2, 1, 0)])
 def test_attention_empty(lsa, shape):
     B, Tq, M = shape
