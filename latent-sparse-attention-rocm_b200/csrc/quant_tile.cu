@@ -25,7 +25,8 @@
 // rate), 494 us = 1.08 PFLOP/s in bursts. With two streams, converting: about 1000 cycles a tile for two warps (500 alone;
 // shared memory and the ALU pipe are the softmax's and the MMAs' too), 32 tokens on 65536 keys 65 us = 2.1 TB/s. Not
 // kept: four more converting warps (a thread's 128 logits want 146 registers), loads of the next codes before the
-// stores of these (no change).
+// stores of these (no change), S and P in steps of 64 keys with the next step's S issued ahead (573 us against 538: what
+// a step costs a warp beside its exponentials - waits, TMEM loads and stores, barriers - comes twice as often).
 //
 // Every wait is bounded (QuantArgs::wait_ns); an expired wait raises a CTA-wide flag, every role leaves, copies and
 // MMAs in flight are waited for (bounded), the TMEM is released and LSA_ERR_TIMEOUT lands in the status word.
