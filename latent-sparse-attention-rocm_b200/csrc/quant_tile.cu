@@ -709,6 +709,7 @@ template <typename T> int launch(const QuantArgs& a, int code, int D, unsigned g
 }  // namespace
 
 int launch_quant_tiles(const QuantArgs& a, int dtype, int code, int D, cudaStream_t stream) {
+    if (a.lists != nullptr || a.status == nullptr) return LSA_ERR_ARG;  // a read's: it has neither kernel nor status here
     const int64_t all = (int64_t)a.B * a.Hkv * a.tiles, items = a.whole + (all - a.whole) * a.parts;
     if (items > INT32_MAX) return LSA_ERR_SIZE;
     return dtype == kBF16 ? launch<__nv_bfloat16>(a, code, D, (unsigned)items, stream)

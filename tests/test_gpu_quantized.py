@@ -605,3 +605,28 @@ def test_step_of_the_whole_path(lsa):
     F.append(pages, k[:, 30:].cpu(), qkv[:, 30:, Hq + Hkv:].cpu(), table.cpu(), torch.tensor([T, T]))
     want, _, off, _ = F.attention(q[:, 30:].cpu(), pages, table.cpu(), ln.cpu())
     close(out, want, off)
+
+
+@pytest.mark.parametrize("code,dtype,D,page,group,Hkv,R,W", [
+    ("e4m3", BF, 128, 64, 128, 1, 8, 2116), ("int8", HF, 64, 16, 64, 1, 32, 2116), ("e4m3", HF, 64, 32, 33, 2, 40, 1100),
+    ("int8", BF, 128, 128, 71, 1, 64, 1030), ("e4m3", BF, 64, 64, 129, 1, 6, 3000)])
+def test_read_of_wide_groups(lsa, code, dtype, D, page, group, Hkv, R, W):
+    """Groups of more heads than a row tile, on so many keys that rows of a dense call would be the tensor cores': the
+    lists count, and the table rows they name - repeated, fewer than the query rows, some outside the table."""
+    g = torch.Generator().manual_seed(group)
+    lengths = [4000, 0, 33, 2900, 517]
+    table, n = F.paged(g, lengths, page)
+    table[3, 1] = -1
+    pages = F.pool(g, n, Hkv, page, D, code)
+    F.poison(pages, table, lengths)
+    rows = torch.tensor([0, 3, 0, 4, 1, 9, -1, 2, 3, 0], dtype=torch.int32).repeat(-(-R // 10))[:R]
+    lists = torch.stack([torch.randperm(4100, generator=g)[:W] for _ in range(R)]).to(torch.int32)
+    counts = torch.randint(0, W + 1, (R,), generator=g, dtype=torch.int32)
+    counts[0], counts[1], counts[2] = W, W, 0
+    q = torch.randn(R, 1, group * Hkv, D, generator=g).to(dtype)
+    ln = torch.tensor(lengths, dtype=torch.int32)
+    want, off = F.read(q, pages, table, ln, lists, counts, rows)
+    assert bool((want[1] != 0).all())
+    got = lsa.quantized_read(q.cuda(), F.to(pages, "cuda"), table.cuda(), ln.cuda(), lists.cuda(), counts.cuda(), rows.cuda())
+    close(got, want, off)
+    assert bool((got[[2, 4, 5]] == 0).all())

@@ -233,3 +233,16 @@ def test_frequencies(lsa):
                 (64, math.inf), (64, 1e4, "yarn", 2.0, 4096, 1.0, 2.0)):
         with pytest.raises(ValueError):
             lsa.rotary_frequencies(*bad)
+
+
+@pytest.mark.parametrize("Hkv", [1, 2])
+@pytest.mark.parametrize("group", [31, 33, 47, 71, 127, 129])
+@pytest.mark.parametrize("R,W", [(1, 16385), (8, 2116), (64, 2116), (700, 300)])
+def test_reads_are_planned_by_their_own_rows(lsa, R, W, group, Hkv):
+    """A read's scratch is whole parts of its R rows a head, whatever the group: the kernel that knows lists plans it. (The
+    tensor cores' tiles of 128 rows, which the odd groups do not divide, hold no lists.)"""
+    from lsa_b200 import _lib
+
+    one = R * group * Hkv * (128 + 1) * 4
+    got = _lib.lib().lsa_quantized_scratch(R, 1, group * Hkv, Hkv, 128, W, 1)
+    assert got >= 0 and got % one == 0 and got // one <= 96
