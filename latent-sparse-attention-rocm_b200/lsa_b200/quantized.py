@@ -231,8 +231,10 @@ class QuantizedCache:
         Hkv, D = self.pages.k.shape[1], self.pages.k.shape[3]
         if q.dtype not in (torch.float16, torch.bfloat16) or q.shape[3] != D or q.shape[2] % Hkv or q.shape[2] < Hkv:
             raise ValueError(f"step: q is fp16 or bf16 [n, Tq, a multiple of {Hkv}, {D}], got {q.dtype} {list(q.shape)}")
-        if scale is not None and not (0.0 < float(scale) < float("inf")):
-            raise ValueError(f"step: the scale must be positive, got {scale}")
+        with np.errstate(over="ignore", under="ignore"):  # as the operator takes it: it refuses after the append
+            scale_log2 = np.float32(D ** -0.5 if scale is None else float(scale)) * np.float32(1.4426950408889634)
+        if not 0 < scale_log2 < np.inf:
+            raise ValueError(f"step: the scale must be positive, and with log2(e) within fp32, got {scale}")
         n, Tq = q.shape[:2]
         M = max([-(-(self.lengths[p] + Tq) // self.page) for p in places], default=0)
         if _lib.lib().lsa_quantized_scratch(n, Tq, q.shape[2], Hkv, D, M * self.page, 0) < 0:

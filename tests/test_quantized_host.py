@@ -246,3 +246,19 @@ def test_reads_are_planned_by_their_own_rows(lsa, R, W, group, Hkv):
     one = R * group * Hkv * (128 + 1) * 4
     got = _lib.lib().lsa_quantized_scratch(R, 1, group * Hkv, Hkv, 128, W, 1)
     assert got >= 0 and got % one == 0 and got // one <= 96
+
+
+@pytest.mark.parametrize("scale", [3e38, 1e39, 1e-46, -1e-46, math.nan, math.inf])
+def test_a_step_whose_scale_the_operator_refuses_appends_nothing(plain, scale):
+    """The operator takes the scale times log2(e) in fp32: 3e38 is an infinity there, 1e-46 a zero."""
+    cache = plain.QuantizedCache(1, 4, 2, 64, 16, device="cpu")
+    cache.append([0], *given(1, 10, Hkv=2))
+    before = [t.clone() for t in cache.pages]
+    k, v = given(1, 7, 1, Hkv=2)
+    with pytest.raises(ValueError):
+        cache.step([0], torch.zeros(1, 7, 4, 64, dtype=torch.bfloat16), k, v, scale=scale)
+    assert cache.lengths == [10] and cache.free_pages == 3
+    assert all(torch.equal(a.float(), b.float()) for a, b in zip(before, cache.pages))
+    for near in (2e38, 1e-38):  # taken by both
+        cache.step([0], torch.zeros(1, 1, 4, 64, dtype=torch.bfloat16), k[:, :1], v[:, :1], scale=near)
+    assert cache.lengths == [12]
