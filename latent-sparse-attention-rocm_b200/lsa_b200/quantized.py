@@ -120,6 +120,9 @@ class QuantizedCache:
             raise ValueError(f"pages of 16, 32, 64 or 128 tokens and heads of 64 or 128, got {page} and {head_dim}")
         if dtype not in (torch.float8_e4m3fn, torch.int8):
             raise ValueError(f"codes are float8_e4m3fn or int8, got {dtype}")
+        if kv_heads > 65535 or pages * kv_heads * page > (1 << 31) - 1:  # the operators' limits
+            raise ValueError(f"at most 65535 heads and fewer than 2^31 (page, head, token) rows, got {kv_heads} heads, "
+                             f"{pages} pages of {page}")
         self.pages = QuantizedPages.new(pages, kv_heads, page, head_dim, dtype, device)
         self.page = page
         self.lengths = [0] * places  # tokens of every place

@@ -262,3 +262,10 @@ def test_a_step_whose_scale_the_operator_refuses_appends_nothing(plain, scale):
     for near in (2e38, 1e-38):  # taken by both
         cache.step([0], torch.zeros(1, 1, 4, 64, dtype=torch.bfloat16), k[:, :1], v[:, :1], scale=near)
     assert cache.lengths == [12]
+
+
+@pytest.mark.parametrize("bad", [dict(kv_heads=65536), dict(kv_heads=1 << 12, pages=1 << 15), dict(pages=(1 << 24) + 1, page=128)])
+def test_pools_that_the_operators_refuse_are_no_cache(lsa, bad):
+    """Heads beyond a launch's, rows (page, head, token) beyond 2^31 - 1: refused before anything is allocated."""
+    with pytest.raises(ValueError):
+        lsa.QuantizedCache(**{**dict(places=1, pages=1, kv_heads=1, head_dim=64, page=16, device="meta"), **bad})
