@@ -49,6 +49,8 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: str = "none", f
 
     low, high = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), dim - 1)
     ramp = ((i - low) / max(high - low, 1e-3)).clamp(0, 1)
+    if pair(slow) < 0:  # the first pair turns less often too: the ramp ends before it
+        ramp = torch.ones_like(i)
     return f / factor * ramp + f * (1 - ramp), 0.1 * math.log(factor) + 1.0
 
 

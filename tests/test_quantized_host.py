@@ -269,3 +269,12 @@ def test_pools_that_the_operators_refuse_are_no_cache(lsa, bad):
     """Heads beyond a launch's, rows (page, head, token) beyond 2^31 - 1: refused before anything is allocated."""
     with pytest.raises(ValueError):
         lsa.QuantizedCache(**{**dict(places=1, pages=1, kv_heads=1, head_dim=64, page=16, device="meta"), **bad})
+
+
+@pytest.mark.parametrize("trained,fast,slow", [(4, 32.0, 1.0), (100, 64.0, 32.0), (6, 2.0, 1.0), (4096, 32.0, 1.0)])
+def test_yarn_pairs_below_slow_turns_are_over_the_factor(lsa, trained, fast, slow):
+    """The first pair too, where the trained length is too short for it to turn ``slow`` times."""
+    f, _ = lsa.rotary_frequencies(64, 10000.0)
+    g, _ = lsa.rotary_frequencies(64, 10000.0, "yarn", 8.0, trained, fast, slow)
+    below = f * trained / (2 * math.pi) < slow * (1 - 1e-9)
+    assert bool(below.any()) and torch.equal(g[below], f[below] / 8)
