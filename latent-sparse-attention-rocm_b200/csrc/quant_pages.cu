@@ -101,6 +101,7 @@ __global__ void __launch_bounds__(NT == 32 ? 128 : NT) append_kernel(const Appen
     const int kept = first > p0 ? (int)(first - p0) : 0;  // older tokens of the page
     const int end = length - p0 < page ? (int)(length - p0) : page;
     const int n = end - kept;
+    if (n <= 0) return;  // a count of 0 in the middle of a page: no new token, nothing of the page changes
     const T* src = static_cast<const T*>(value ? a.v : a.k) + (value ? b * a.v_b + h * a.v_h : b * a.k_b + h * a.k_h);
     const int64_t ld = value ? a.v_t : a.k_t;
     const int64_t head = (int64_t)id * a.Hkv + h;

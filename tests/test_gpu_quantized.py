@@ -630,3 +630,21 @@ def test_read_of_wide_groups(lsa, code, dtype, D, page, group, Hkv, R, W):
     got = lsa.quantized_read(q.cuda(), F.to(pages, "cuda"), table.cuda(), ln.cuda(), lists.cuda(), counts.cuda(), rows.cuda())
     close(got, want, off)
     assert bool((got[[2, 4, 5]] == 0).all())
+
+
+def test_append_of_no_token_leaves_the_page(lsa):
+    """A count of 0 (or a negative one) on a partly full page writes nothing, whatever scale the caller gave the page;
+    its neighbour in the call is written."""
+    g = torch.Generator().manual_seed(24)
+    for Tq in (1, 3, 20):  # a warp a page, a CTA a page
+        for code in ("e4m3", "int8"):
+            pages = F.pool(g, 5, 2, 32, 64, code)
+            for s in (pages.k_scale, pages.v_scale):
+                s.copy_(torch.tensor([2.0 ** -70, 0.75 * 2.0 ** -63, 2.0 ** -70, 1.0, 2.0 ** -70])[:, None].expand(5, 2))
+            table = torch.tensor([[0, -1], [1, 4], [2, 3]], dtype=torch.int32)
+            ln, counts = torch.tensor([20, 40, 25]), torch.tensor([0, 1, -3])
+            dev = F.to(pages, "cuda")
+            k, v = (torch.randn(3, Tq, 2, 64, generator=g) for _ in range(2))
+            F.append(pages, k, v, table, ln, counts)
+            lsa.append_quantized(dev, k.cuda(), v.cuda(), table.cuda(), ln.cuda(), counts.cuda())
+            same(dev, pages)
