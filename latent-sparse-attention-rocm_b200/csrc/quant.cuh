@@ -16,6 +16,8 @@
 
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "launch.cuh"
 
 namespace lsa {
@@ -108,6 +110,18 @@ __device__ __forceinline__ float half_factor(uint32_t top, float* factor) {
     const int up = e == 0 || e == 255 ? 0 : min(8 - (e - 127), 100);
     *factor *= __uint_as_float((uint32_t)(127 - up) << 23);
     return __uint_as_float((uint32_t)(up + 127) << 23);
+}
+
+// A row of q that is not finite (its largest magnitude's bits say) enters the products as zeros, with a factor of -0, so that
+// it is NaN only where a key is seen: a key that is not there has zeros for its codes, and NaN times those would make
+// rows without keys NaN. At the end its sum becomes NaN unless it is 0. (A finite row's factor is never -0. A row with
+// an infinity has only infinities and NaN for logits, so NaN is its softmax over any keys.)
+template <typename T> __device__ __forceinline__ bool infinite_row(uint32_t top) {
+    return top >= (std::is_same<T, __nv_bfloat16>::value ? 0x7F80u : 0x7C00u);
+}
+constexpr float kInfiniteRow = -0.0f;
+__device__ __forceinline__ float sum_of_row(float sum, float factor) {
+    return __float_as_uint(factor) == 0x80000000u && sum != 0.0f ? __uint_as_float(0x7FFFFFFFu) : sum;
 }
 
 // Token of row r of a (sequence, KV head), r < Tq G: r / G, exact for r G below 2^32 (the entry point checks).

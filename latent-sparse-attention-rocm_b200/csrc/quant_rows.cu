@@ -284,15 +284,15 @@ __global__ void __launch_bounds__(kWarps * 32, QuantShape<D, NT, LISTS>::kCTAs) 
 #pragma unroll
         for (int u = 0; u < NQ; ++u) {
             float f = a.scale_log2;
+            uint32_t top = 0;  // largest magnitude's bits
+#pragma unroll
+            for (int kk = 0; kk < KS; ++kk)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    top = max(top, max(qf[u][kk][e] & 0x7FFFu, (qf[u][kk][e] >> 16) & 0x7FFFu));
+            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
             if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-                uint32_t top = 0;  // largest magnitude's bits, as a bf16
-#pragma unroll
-                for (int kk = 0; kk < KS; ++kk)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        top = max(top, max(qf[u][kk][e] & 0x7FFFu, (qf[u][kk][e] >> 16) & 0x7FFFu));
-                top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-                top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
                 const float by = half_factor(top, &f);
 #pragma unroll
                 for (int kk = 0; kk < KS; ++kk)
@@ -300,6 +300,11 @@ __global__ void __launch_bounds__(kWarps * 32, QuantShape<D, NT, LISTS>::kCTAs) 
                     for (int e = 0; e < 2; ++e)
                         qf[u][kk][e] = pack_half(__uint_as_float(qf[u][kk][e] << 16) * by,
                                                  __uint_as_float(qf[u][kk][e] & 0xFFFF0000u) * by);
+            }
+            if (infinite_row<T>(top)) {
+                f = kInfiniteRow;
+#pragma unroll
+                for (int kk = 0; kk < KS; ++kk) qf[u][kk][0] = qf[u][kk][1] = 0;
             }
             if constexpr (kShared) {
 #pragma unroll
@@ -519,6 +524,10 @@ __global__ void __launch_bounds__(kWarps * 32, QuantShape<D, NT, LISTS>::kCTAs) 
         for (int e = 0; e < 2; ++e)
 #pragma unroll
             for (int off = 4; off <= 16; off <<= 1) sum[u][e] += __shfl_xor_sync(0xFFFFFFFFu, sum[u][e], off);
+        float f[2];
+        unpair(factor[u], f[0], f[1]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) sum[u][e] = sum_of_row(sum[u][e], f[e]);
     }
     // join the warps: each leaves its sums in its own ring, (m, l) after the rings
     __syncwarp();

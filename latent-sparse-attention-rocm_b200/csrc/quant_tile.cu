@@ -160,17 +160,18 @@ __device__ __forceinline__ void load_q(const QuantArgs& a, const Item& w, uint8_
         const int row = i * RP + lr, hf = row >> 7, r = row & 127;
         uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
         float f = a.scale_log2;
+        uint32_t top = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = max(top, max(u[e] & 0x7FFFu, (u[e] >> 16) & 0x7FFFu));
+#pragma unroll
+        for (int off = L / 2; off >= 1; off >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
         if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-            uint32_t top = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) top = max(top, max(u[e] & 0x7FFFu, (u[e] >> 16) & 0x7FFFu));
-#pragma unroll
-            for (int off = L / 2; off >= 1; off >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
             const float by = half_factor(top, &f);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 u[e] = pack16(__uint_as_float(u[e] << 16) * by, __uint_as_float(u[e] & 0xFFFF0000u) * by, (__half*)nullptr);
         }
+        if (infinite_row<T>(top)) f = kInfiniteRow, u[0] = u[1] = u[2] = u[3] = 0;
         if (row < halves * 128) {
             sts_u4(smem_u32(sm) + hf * Sh::kOperand + (ch >> 3) * 16384 + r * 128 + (((ch & 7) ^ (r & 7)) << 4), u[0], u[1],
                    u[2], u[3]);
@@ -329,7 +330,8 @@ __device__ __forceinline__ void softmax_half(const QuantArgs& a, const Item& w, 
     if (ok && n > 0) ok = role_wait(&bar_o[hf], 0, abort_flag, a.wait_ns);
     if (!ok) return;
     const int64_t rid = ((int64_t)w.b * a.Tq + tok) * a.Hq + (int64_t)w.h * a.G + g;
-    const bool none = l == 0.0f;  // the row has seen no key (a NaN logit makes l NaN, and the output)
+    l = sum_of_row(l, factor);
+    const bool none = l == 0.0f;  // the row has seen no key (a NaN makes the output NaN)
     const float inv = none ? 0.0f : 1.0f / l;
     const float lse = none ? -INFINITY : m + (log2f(l) - kLift);
     const int64_t at = quant_part_row(a, w.split, w.rest, hf, qd * 32 + lane);

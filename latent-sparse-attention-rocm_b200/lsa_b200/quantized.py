@@ -67,8 +67,8 @@ def quantized_attention(q, pages: QuantizedPages, page_table, lengths, scale=Non
 
     q [B, Tq, Hq, D] fp16 or bf16; sequence b holds ``lengths[b]`` tokens, the call's Tq new ones among
     them (append first). Row i sees the tokens ``j < lengths[b] - Tq + i + 1`` on pages that the table
-    maps; a row that sees none reads as zeros (log-sum-exp -inf). What pages hold behind a
-    sequence's last token is never used; what a row of the call sees must be finite, its scales
+    maps; a row that sees none reads as zeros (log-sum-exp -inf), whatever q holds there; one of q that is
+    not finite and sees a key is NaN. What pages hold behind a sequence's last token is never used; what a row of the call sees must be finite, its scales
     positive, the value scales within 2^100 of each other (they count as 2^-60 at least). ``scale``,
     positive, defaults to ``D ** -0.5``. The weights are rounded to 16 bits for their product with the
     codes; sums, joins and log-sum-exp are fp32. Output like q, contiguous; with ``return_lse`` also

@@ -648,3 +648,49 @@ def test_append_of_no_token_leaves_the_page(lsa):
             F.append(pages, k, v, table, ln, counts)
             lsa.append_quantized(dev, k.cuda(), v.cuda(), table.cuda(), ln.cuda(), counts.cuda())
             same(dev, pages)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("dtype,D,page,code", [(BF, 128, 64, "e4m3"), (HF, 64, 16, "int8"), (HF, 128, 32, "e4m3")])
+@pytest.mark.parametrize("Tq,Hq,Hkv", [(1, 4, 1), (3, 4, 1), (5, 16, 4), (40, 32, 8), (70, 32, 8)],
+                         ids=["8rows", "16rows", "32rows", "two halves", "many rows"])
+def test_rows_without_keys_read_as_zeros_whatever_they_hold(lsa, Tq, Hq, Hkv, dtype, D, page, code, bad):
+    """Rows of q that are not finite and see no key - all pages that they see unmapped, or before token 0 - are zeros
+    with log-sum-exp -inf; the rows beside them, of the same tile, are as they were."""
+    g = torch.Generator().manual_seed(25)
+    lengths = [Tq // 2, 700, page + Tq - 1, 0, 1150, 130, 900, 1000, 300, 40]
+    table, n = F.paged(g, lengths, page)
+    table[1] = -1
+    table[2, :1] = 1 << 30  # its first row sees this page only
+    table[4, ::2] = -1
+    pages = F.pool(g, n, Hkv, page, D, code)
+    F.poison(pages, table, lengths)
+    q = torch.randn(len(lengths), Tq, Hq, D, generator=g).to(dtype)
+    ln = torch.tensor(lengths, dtype=torch.int32)
+    want, want_lse, off, lse_off = F.attention(q, pages, table, ln)
+    none = want_lse == -math.inf
+    assert bool(none[1].all()) and bool(none[2, 0].all()) and not bool(none[4].any())
+    q[none] = bad
+    got, lse = lsa.quantized_attention(q.cuda(), F.to(pages, "cuda"), table.cuda(), ln.cuda(), return_lse=True)
+    assert bool((got[none.cuda()] == 0).all()) and bool((lse[none.cuda()] == -math.inf).all())
+    close(got, want, off)
+    close(lse, want_lse, lse_off + 2.0 ** -22)
+
+
+@pytest.mark.parametrize("dtype,group", [(BF, 4), (HF, 16), (BF, 40)])
+def test_reads_without_keys_are_zeros_whatever_they_hold(lsa, dtype, group):
+    g = torch.Generator().manual_seed(26)
+    lengths = [300, 0, 300, 300]
+    table, n = F.paged(g, lengths, 32)
+    table[2] = -1
+    pages = F.pool(g, n, 2, 32, 64, "e4m3")
+    q = torch.randn(5, 1, 2 * group, 64, generator=g).to(dtype)
+    lists = torch.randint(0, 300, (5, 200), generator=g, dtype=torch.int32)
+    lists[3] = 300
+    counts, rows = torch.tensor([0, 200, 200, 200, 200]), torch.tensor([0, 1, 2, 3, 0])
+    ln = torch.tensor(lengths)
+    want, off = F.read(q, pages, table, ln, lists, counts, rows)
+    q[:4] = torch.tensor([math.nan, math.inf, -math.inf, math.nan]).view(4, 1, 1, 1).to(dtype)
+    got = lsa.quantized_read(q.cuda(), F.to(pages, "cuda"), table.cuda(), ln.cuda(), lists.cuda(), counts.cuda(), rows.cuda())
+    assert bool((got[:4] == 0).all())
+    close(got, want, off)
