@@ -68,11 +68,12 @@ def quantized_attention(q, pages: QuantizedPages, page_table, lengths, scale=Non
     q [B, Tq, Hq, D] fp16 or bf16; sequence b holds ``lengths[b]`` tokens, the call's Tq new ones among
     them (append first). Row i sees the tokens ``j < lengths[b] - Tq + i + 1`` on pages that the table
     maps; a row that sees none reads as zeros (log-sum-exp -inf), whatever q holds there; one of q that is
-    not finite and sees a key is NaN. What pages hold behind a sequence's last token is never used; what a row of the call sees must be finite, its scales
-    positive, the value scales within 2^100 of each other (they count as 2^-60 at least). ``scale``,
-    positive, defaults to ``D ** -0.5``. The weights are rounded to 16 bits for their product with the
-    codes; sums, joins and log-sum-exp are fp32. Output like q, contiguous; with ``return_lse`` also
-    the natural log-sum-exp of every row's scaled logits, fp32 [B, Tq, Hq]."""
+    not finite and sees a key is NaN. What pages hold behind a sequence's last token is never used; what
+    a row of the call sees must be finite, its scales positive, the value scales within 2^100 of each
+    other (they count as 2^-60 at least). ``scale``, positive, defaults to ``D ** -0.5``. The weights are
+    rounded to 16 bits for their product with the codes; sums, joins and log-sum-exp are fp32. Output
+    like q, contiguous; with ``return_lse`` also the natural log-sum-exp of every row's scaled logits,
+    fp32 [B, Tq, Hq]."""
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     ops = _lib.torch_ops()
     fn = ops.quantized_attention_lse if return_lse else ops.quantized_attention
@@ -155,16 +156,23 @@ class QuantizedCache:
         if k.dtype not in _lib.DTYPE_CODE or v.dtype != k.dtype:
             raise ValueError(f"{what}: fp32, fp16 or bf16 keys and values of one type, got {k.dtype}, {v.dtype}")
 
+    def _staged(self, n):
+        """n int32 on the host, pinned where the pages are on a GPU: a copy from pageable memory would wait for all
+        that the stream holds. Torch keeps pinned memory until the copies from it have run."""
+        return torch.empty(n, dtype=torch.int32, pin_memory=self.pages.k.is_cuda)
+
     def _upload(self, places, counts=()):
         """(page table, lengths, counts) of the places on the device, in one copy."""
         n, M = len(places), max([len(self._held[p]) for p in places], default=0)
-        host = np.full(n * (M + 2), -1, np.int32)
+        staged = self._staged(n * (M + 2))
+        host = staged.numpy()
+        host[:] = -1
         host[:n] = [self.lengths[p] for p in places]
         host[n:n + len(counts)] = counts
         table = host[2 * n:].reshape(n, M)
         for i, p in enumerate(places):
             table[i, :len(self._held[p])] = self._held[p]
-        dev = torch.from_numpy(host).to(self.pages.k.device)
+        dev = staged.to(self.pages.k.device, non_blocking=True)
         return dev[2 * n:].view(n, M), dev[:n], dev[n:2 * n]
 
     def _grow(self, places, counts, Tq):
@@ -207,8 +215,10 @@ class QuantizedCache:
 
     def _move(self, src, dst):
         if src:
-            ids = torch.tensor([src, dst], dtype=torch.int32).to(self.pages.k.device)
-            move_pages(self.pages, ids[0], ids[1])
+            staged = self._staged(2 * len(src))
+            staged.numpy()[:] = src + dst
+            ids = staged.to(self.pages.k.device, non_blocking=True)
+            move_pages(self.pages, ids[:len(src)], ids[len(src):])
 
     def append(self, places, k, v, counts=None) -> None:
         """Append k, v [n, Tq, Hkv, D] to the n places; of place i's rows the last ``counts[i]`` (all of them

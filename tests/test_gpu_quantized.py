@@ -694,3 +694,37 @@ def test_reads_without_keys_are_zeros_whatever_they_hold(lsa, dtype, group):
     got = lsa.quantized_read(q.cuda(), F.to(pages, "cuda"), table.cuda(), ln.cuda(), lists.cuda(), counts.cuda(), rows.cuda())
     assert bool((got[:4] == 0).all())
     close(got, want, off)
+
+
+def test_cache_calls_do_not_wait_for_the_device(lsa, monkeypatch):
+    """Appends, steps, attention, reads and a fork's copies return while the stream is still busy with what came before
+    them (the checked mode waits by itself), and what they uploaded is what their kernels find."""
+    monkeypatch.delenv("LSA_CHECK_STATUS", raising=False)
+    g = torch.Generator().manual_seed(27)
+    Hkv, Hq, D = 2, 8, 64
+    k, v = (torch.randn(2, 40, Hkv, D, generator=g).to(BF).cuda() for _ in range(2))
+    q = torch.randn(2, 2, Hq, D, generator=g).to(BF).cuda()
+    lists, counts = torch.randint(0, 40, (2, 9), generator=g).cuda(), torch.tensor([9, 5]).cuda()
+
+    def use(busy):
+        cache = lsa.QuantizedCache(4, 64, Hkv, D, 16)
+        torch.cuda.synchronize()
+        done = torch.cuda.Event()
+        if busy:
+            torch.cuda._sleep(1 << 29)  # a quarter of a second
+            done.record()
+        outs, early = [], []
+        for call in (lambda: cache.append([0, 1], k, v), lambda: cache.step([0, 1], q, k[:, :2], v[:, :2]),
+                     lambda: cache.step([cache.fork(0), 0], q, k[:, 2:4], v[:, 2:4]), lambda: cache.attend([1, 0], q),
+                     lambda: cache.free([1]), cache.compact, lambda: cache.read([2, 0], q[:, :1], lists, counts)):
+            out = call()
+            early.append(busy and not done.query())
+            outs.append(out)
+        torch.cuda.synchronize()
+        return [x for x in outs if torch.is_tensor(x)], early
+
+    want, _ = use(False)
+    use(True)  # buffers of this many calls in flight at once
+    got, early = use(True)
+    assert all(early), early
+    assert len(want) == 4 and all(torch.equal(a, b) for a, b in zip(want, got))
