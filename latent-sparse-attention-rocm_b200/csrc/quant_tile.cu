@@ -506,11 +506,10 @@ template <int CODE, int D>
 __device__ __forceinline__ void convert(const QuantArgs& a, const Item& w, uint8_t* sm, uint64_t* codes_full,
                                         uint64_t* codes_empty, uint64_t* op_full, uint64_t* op_empty,
                                         volatile int* abort_flag, int self, int warps) {
-    switch (warps) {
+    switch (warps) {  // a call has more than one warp of rows: fewer are the few-row kernel's
         case 2: return convert<CODE, D, 2>(a, w, sm, codes_full, codes_empty, op_full, op_empty, abort_flag, self);
         case 4: return convert<CODE, D, 4>(a, w, sm, codes_full, codes_empty, op_full, op_empty, abort_flag, self);
-        case 6: return convert<CODE, D, 6>(a, w, sm, codes_full, codes_empty, op_full, op_empty, abort_flag, self);
-        default: return convert<CODE, D, 8>(a, w, sm, codes_full, codes_empty, op_full, op_empty, abort_flag, self);
+        default: return convert<CODE, D, 6>(a, w, sm, codes_full, codes_empty, op_full, op_empty, abort_flag, self);
     }
 }
 
@@ -712,6 +711,7 @@ template <typename T> int launch(const QuantArgs& a, int code, int D, unsigned g
 
 int launch_quant_tiles(const QuantArgs& a, int dtype, int code, int D, cudaStream_t stream) {
     if (a.lists != nullptr || a.status == nullptr) return LSA_ERR_ARG;  // a read's: it has neither kernel nor status here
+    if (a.streams && a.Tq * a.G <= 32) return LSA_ERR_ARG;  // its idle softmax warps would be converters that convert() has no form for
     const int64_t all = (int64_t)a.B * a.Hkv * a.tiles, items = a.whole + (all - a.whole) * a.parts;
     if (items > INT32_MAX) return LSA_ERR_SIZE;
     return dtype == kBF16 ? launch<__nv_bfloat16>(a, code, D, (unsigned)items, stream)
