@@ -728,3 +728,48 @@ def test_cache_calls_do_not_wait_for_the_device(lsa, monkeypatch):
     got, early = use(True)
     assert all(early), early
     assert len(want) == 4 and all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def weights_case(g, lengths, Tq, Hkv, group, D, page, code):
+    """Values of alternating sign with nearly equal weights, which all but cancel: what their rounding costs is not hidden
+    by the output's own."""
+    table, n = F.paged(g, lengths, page)
+    pages = F.pool(g, n, Hkv, page, D, code)
+    sign = (1 - 2 * (torch.arange(page) & 1))[None, None, :, None] * (1 - 2 * torch.randint(0, 2, (n, Hkv, 1, D), generator=g))
+    pages.v.copy_(sign.float().to(pages.v.dtype))
+    pages.v_scale.fill_(1.0)
+    F.poison(pages, table, lengths)
+    return pages, table, torch.tensor(lengths, dtype=torch.int32), torch.randn(len(lengths), Tq, Hkv * group, D, generator=g)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("B,Tq,Hkv,group,D,page,code", [(40, 1, 2, 4, 128, 64, "e4m3"), (40, 3, 2, 4, 64, 16, "int8"),
+                                                        (40, 5, 1, 6, 128, 32, "e4m3"), (16, 40, 8, 4, 128, 64, "e4m3"),
+                                                        (16, 70, 8, 4, 64, 16, "int8")])
+def test_weights_are_rounded_to_11_bits(lsa, B, Tq, Hkv, group, D, page, code, dtype):
+    """Off by 2^-11 of each weight at most, besides the output's rounding - also where q and the output are bf16. Weights
+    of 8 bits, as a bf16's, would not pass."""
+    g = torch.Generator().manual_seed(28)
+    lengths = [Tq + 1 + i % 5 for i in range(B)]
+    pages, table, ln, q = weights_case(g, lengths, Tq, Hkv, group, D, page, code)
+    q, scale = q.to(dtype), 0.05 * D ** -0.5
+    want = torch.zeros(q.shape, dtype=torch.float64)
+    off, worse = torch.zeros_like(want), torch.zeros_like(want)
+    for b, n in enumerate(lengths):
+        ids, key, val = F.keys(pages, table[b], torch.arange(n))
+        seen = ids[None, :] < (n - Tq + torch.arange(Tq) + 1)[:, None]
+        for h in range(q.shape[2]):
+            x, k, v = q[b, :, h].double(), key[:, h // group], val[:, h // group]
+            out, _, o, _ = F.rows(x, k, v, scale, seen, 2.0 ** -11)
+            logits = (x @ k.T * scale).masked_fill(~seen, -math.inf)
+            p = torch.exp(logits - logits.amax(-1, keepdim=True))
+            want[b, :, h], off[b, :, h] = out, o
+            worse[b, :, h] = p.to(BF).double() @ v / p.sum(-1, keepdim=True)
+    off += torch.finfo(dtype).eps / 2 * want.abs()
+    assert ((worse - want).abs() > off).double().mean() > 0.01
+    got = lsa.quantized_attention(q.cuda(), F.to(pages, "cuda"), table.cuda(), ln.cuda(), scale)
+    close(got, want, off)
+    if Tq == 1:
+        lists = torch.arange(8, dtype=torch.int32).expand(B, 8).contiguous()
+        close(lsa.quantized_read(q.cuda(), F.to(pages, "cuda"), table.cuda(), ln.cuda(), lists.cuda(), ln.cuda(), scale=scale),
+              want, off)
