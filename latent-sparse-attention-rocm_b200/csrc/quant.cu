@@ -30,10 +30,10 @@ Plan make_plan(int64_t B, int64_t Tq, int64_t Hq, int64_t Hkv, int64_t D, int64_
     p.parts = 1;
     // The few-row kernel reads the keys once for each 32 rows, from L2 after the first time, and converts them in
     // registers; the tensor-core kernel's converting goes through shared memory, which its products share, and its start
-    // takes 4 us (us, few-row / tensor cores: 32 x 4096 keys, 32 rows 85 / 105, 48 rows 146 / 120; 1 x 65536 32 rows 37 / 45,
-    // 64 rows 62 / 51; 4 x 2048 64 rows 20.4 / 20.9; 1 x 2048 128 rows 15.8 / 18.2, 256 rows 24.7 / 24.4; 1 x 512 128 rows
-    // 10.6 / 13.4). Many sequences hide that kernel's chains and leave its join's traffic: 48 rows, 64 x 2048 147 / 135,
-    // 128 x 2048 237 / 262, 1024 x 1024 1069 / 1364. Lists are the few-row kernel's at any size: the tensor-core kernel reads
+    // takes 4 us (us, few-row / tensor cores: 32 x 4096 keys, 32 rows 85 / 105, 48 rows 145 / 107; 1 x 65536 32 rows 37 / 45,
+    // 64 rows 61 / 44; 4 x 2048 64 rows 20.8 / 20.2; 1 x 2048 128 rows 16.4 / 18.1, 256 rows 20.0 / 24.2; 1 x 512 128 rows
+    // 10.6 / 13.4). Many sequences hide that kernel's chains and leave its join's traffic: 48 rows, 64 x 2048 145 / 126,
+    // 128 x 2048 236 / 246, 1024 x 1024 1070 / 1373. Lists are the few-row kernel's at any size: the tensor-core kernel reads
     // whole chunks of a sequence and knows none.
     const int64_t rows = Tq * G, heads = B * Hkv * (keys < kUnit ? kUnit : keys);
     const bool few = lists || rows <= 32 || (rows <= 64 && (heads <= 1 << 16 || B * Hkv > 6 * kSMs)) ||

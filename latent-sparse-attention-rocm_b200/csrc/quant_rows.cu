@@ -18,10 +18,12 @@
 // more than 2^kGrow, so P is at most 2^15 and 2^-35 of a row's largest is kept. Sums, maxima and joins are fp32.
 //
 // Measured (B200, 32 / 8 heads, D 128, bf16, pages of 64, called in a loop, joins included): 64 ragged sequences of up
-// to 8191 keys, 807 MB, 134 us = 6.0 TB/s, 93 % of the measured copy rate; one of 131072 (int8), 269 MB, 48 us = 5.6 TB/s;
+// to 8191 keys, 807 MB, 133-142 us = 5.7-6.1 TB/s, 88-94 % of the measured copy rate; one of 131072 (int8), 269 MB, 47-52 us;
 // 4 of up to 2048 7.2 us as graph replays (a chain of latencies: lengths, pages, two tiles of 1600 cycles, the warps' and
-// the cluster's joins), 8.7 called (the host). 32 rows on 65536 keys 37 us. 32 lists of 2116 keys, 141 MB, 42 us: rows of 128 bytes all over the pool come at 4.4 TB/s at
-// most (measured with plain loads), and two scale sectors a key come with them. Rows on the M side and keys on the N side
+// the cluster's joins), 8.7 to 10 called (the host). 32 rows on 65536 keys 37 us. 32 lists of 2116 keys, 141 MB, 42-45 us:
+// rows of 128 bytes all over the pool come at 4.4 TB/s at most (measured with plain loads), and two scale sectors a key
+// come with them. A list's rows are fetched again, from L2, for every 16 heads of its group (graph replays: 64 lists, one KV
+// head, 64 heads 40 us, 71 heads 65; 8 lists, 128 heads 16). Rows on the M side and keys on the N side
 // (an M = 16 tile for four rows) took 183 us for the 64 sequences, its P and O twice as large.
 // Not kept: rows of a list asked of L2 ahead (55 us against 44), pages looked up two tiles ahead and the scales'
 // logarithms behind S (no change).

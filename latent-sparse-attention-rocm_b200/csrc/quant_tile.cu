@@ -21,7 +21,7 @@
 //
 // What bounds it (B200, 32 / 8 heads, D 128): with two halves of rows the chain of a half - softmax 2350 cycles, then its
 // product and the next S 1100 - of which two run at a time: 3400 cycles a pair of chunks, where the MMAs take 2048 and the
-// exponentials as many; 2 x 1024 tokens on 16384 keys 536 us = 0.99 PFLOP/s in a loop (70 % of the measured sustained
+// exponentials as many; 2 x 1024 tokens on 16384 keys 497-536 us = 0.99-1.07 PFLOP/s in a loop (70-76 % of the sustained
 // rate), 494 us = 1.08 PFLOP/s in bursts. With two streams, converting: about 1000 cycles a tile for two warps (500 alone;
 // shared memory and the ALU pipe are the softmax's and the MMAs' too), 32 tokens on 65536 keys 65 us = 2.1 TB/s. Not
 // kept: four more converting warps (a thread's 128 logits want 146 registers), loads of the next codes before the

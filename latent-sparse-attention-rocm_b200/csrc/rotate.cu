@@ -11,9 +11,10 @@
 // lane has four values of either half and so both of a pair, in the half layout as in the interleaved one (two
 // 8-byte loads where one of 16 would want its partner's values by shuffle: 213 us became 138 with the packed
 // arithmetic). A token's heads go to several warps where the tokens alone would not fill the SMs.
-// Measured (B200, 32 + 8 heads, D 128, bf16, norms): 2 x 16384 tokens, 671 MB, 111 us = 6.1 TB/s, 94 % of the measured copy
-// rate; bounded by issue and the loads' latency together: 80 registers leave 24 warps an SM, and bounding them to 64
-// spills (158 us). 64 tokens: 2.5 us as graph replays, 8.8 called in a loop (the host).
+// Measured (B200, 32 + 8 heads, D 128, bf16, norms): 2 x 16384 tokens, 671 MB, 112-121 us = 5.5-6.0 TB/s, 86-93 % of the measured
+// copy rate; bounded by issue and the loads' latency together: 80 registers leave 24 warps an SM, and bounding them to 64
+// spills (158 us). 64 tokens: 2.6 us as graph replays, 9 to 13 called in a loop (the host). fp32, 2 x 8192 tokens, the same
+// bytes: 130 us; D 64 62 us (335 MB), D 256 231 (1342 MB); interleaved, or half of a head turned, 120.
 #include "pairs.cuh"
 
 namespace lsa {

@@ -85,7 +85,8 @@ def quantized_attention(q, pages: QuantizedPages, page_table, lengths, scale=Non
 def quantized_read(q, pages: QuantizedPages, page_table, lengths, lists, counts, rows=None, scale=None):
     """The sparse read over the pages: query row r attends to the listed positions of a sequence.
 
-    q [R, 1, Hq, D] fp16 or bf16; ``lists`` [R, W] int32 positions in any order, ``counts`` [R] how many
+    q [R, 1, Hq, D] fp16 or bf16, a list a row (``flat_select``, ``tree_select``; a tile's shared
+    lists are ``sparse_prefill``'s); ``lists`` [R, W] int32 positions in any order, ``counts`` [R] how many
     of a row's entries count; row r reads sequence ``rows[r]`` of the table (r itself when None). Positions
     outside [0, lengths[rows[r]]), on unmapped pages, and rows outside the table are skipped;
     duplicates count per occurrence; a row without keys reads as zeros. Otherwise as ``quantized_attention``."""

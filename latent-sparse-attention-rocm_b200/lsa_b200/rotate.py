@@ -64,7 +64,8 @@ def norm_rotate(q, k, positions, frequencies, q_weight=None, k_weight=None, eps:
     have q's type or fp32; without one its tensor is not normalised. ``frequencies`` [R / 2] fp64,
     radians a position: the first R values of a head turn (R a multiple of 16, at most D; 0: none),
     value i with value i + R / 2, or 2 i with 2 i + 1 where ``interleaved``, times ``amplitude``; the others
-    pass. In fp32, the angles reduced in fp64, rounded once. Outputs contiguous, like q and k."""
+    pass. In fp32 (the squares' sum too: values below 2^60), the angles reduced in fp64, rounded once.
+    Outputs contiguous, like q and k."""
     out = _lib.torch_ops().norm_rotate(q, k, positions, frequencies, q_weight, k_weight, eps, interleaved, amplitude)
     _lib.after_call(q.device, "norm_rotate")
     return out
