@@ -160,7 +160,7 @@ class QuantizedCache:
     def _staged(self, n):
         """n int32 on the host, pinned where the pages are on a GPU: a copy from pageable memory would wait for all
         that the stream holds. Torch keeps pinned memory until the copies from it have run."""
-        return torch.empty(n, dtype=torch.int32, pin_memory=self.pages.k.is_cuda)
+        return torch.empty(n, dtype=torch.int32, device="cpu", pin_memory=self.pages.k.is_cuda)
 
     def _upload(self, places, counts=()):
         """(page table, lengths, counts) of the places on the device, in one copy."""

@@ -773,3 +773,66 @@ def test_weights_are_rounded_to_11_bits(lsa, B, Tq, Hkv, group, D, page, code, d
         lists = torch.arange(8, dtype=torch.int32).expand(B, 8).contiguous()
         close(lsa.quantized_read(q.cuda(), F.to(pages, "cuda"), table.cuda(), ln.cuda(), lists.cuda(), ln.cuda(), scale=scale),
               want, off)
+
+
+def test_cache_calls_of_no_place_and_under_a_default_device(lsa):
+    g = torch.Generator().manual_seed(29)
+    cache = lsa.QuantizedCache(3, 8, 2, 64, 16)
+    none = torch.empty(0, 3, 2, 64, device="cuda", dtype=BF)
+    cache.append([], none, none)
+    assert cache.step([], none, none, none).shape == none.shape and cache.attend([], none).shape == none.shape
+    k, v, q = (torch.randn(2, 9, 2, 64, generator=g).to(BF).cuda() for _ in range(3))
+    lists, counts = torch.randint(0, 9, (2, 5), generator=g).cuda(), torch.tensor([5, 2]).cuda()
+
+    def use():
+        cache.append([0, 1], k, v)
+        out = cache.step([1, cache.fork(0)], q[:, :2], k[:, :2], v[:, :2])
+        out2 = cache.read([0, 1], q[:, :1], lists, counts)
+        cache.free([0])
+        cache.compact()
+        out3 = cache.attend([2, 1], q)
+        cache.free([0, 1, 2])
+        return out, out2, out3
+
+    want = use()
+    with torch.device("cuda"):
+        got = use()
+    assert all(torch.equal(a, b) for a, b in zip(want, got)) and cache.free_pages == 8
+
+
+@pytest.mark.parametrize("group,Hkv,R,W", [(4, 2, 12, 700), (64, 1, 32, 2116), (128, 1, 8, 2116)])
+def test_reads_captured_and_on_another_stream(lsa, group, Hkv, R, W):
+    """Two reads captured in graphs of their own, replayed in turn and beside an eager one on another stream."""
+    g = torch.Generator().manual_seed(30)
+    lengths = [4000, 2500, 900]
+    table, n = F.paged(g, lengths, 64)
+    pages = F.to(F.pool(g, n, Hkv, 64, 128, "e4m3"), "cuda")
+    table, ln = table.cuda(), torch.tensor(lengths, dtype=torch.int32).cuda()
+    args = []
+    for _ in range(2):
+        q = torch.randn(R, 1, group * Hkv, 128, generator=g).to(BF)
+        q[1] = math.nan
+        lists, counts = torch.randint(0, 4000, (R, W), generator=g, dtype=torch.int32), torch.randint(1, W + 1, (R,), generator=g)
+        counts[1] = 0
+        args.append((q.cuda(), lists.cuda(), counts.to(torch.int32).cuda(), torch.randint(0, 3, (R,), generator=g).to(torch.int32).cuda()))
+
+    def read(a):
+        return lsa.quantized_read(a[0], pages, table, ln, *a[1:])
+
+    want = [read(a) for a in args]
+    assert all(bool((w[1] == 0).all()) and bool(w.isfinite().all()) for w in want)
+    graphs, outs = [], []
+    for a in args:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(read(a))
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for o, graph in zip(outs, graphs):
+            o.zero_()
+            graph.replay()
+        with torch.cuda.stream(side):
+            beside = read(args[0])
+        torch.cuda.synchronize()
+        assert torch.equal(beside, want[0]) and all(torch.equal(a, b) for a, b in zip(outs, want))

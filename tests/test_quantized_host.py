@@ -278,3 +278,11 @@ def test_yarn_pairs_below_slow_turns_are_over_the_factor(lsa, trained, fast, slo
     g, _ = lsa.rotary_frequencies(64, 10000.0, "yarn", 8.0, trained, fast, slow)
     below = f * trained / (2 * math.pi) < slow * (1 - 1e-9)
     assert bool(below.any()) and torch.equal(g[below], f[below] / 8)
+
+
+def test_uploads_are_staged_on_the_host_whatever_the_default_device(plain):
+    cache = plain.QuantizedCache(2, 4, 1, 64, 16, device="cpu")
+    cache.append([0], *given(1, 20))
+    with torch.device("meta"):
+        table, lengths, counts = cache._upload([1, 0], [3, 4])
+    assert table.tolist() == [[-1, -1], [0, 1]] and lengths.tolist() == [0, 20] and counts.tolist() == [3, 4]
