@@ -8,8 +8,8 @@
 // Measured (B200, 8 heads, D 128, bf16 to e4m3, pages of 64): 4 x 16383 tokens, 403 MB, 63-68 us = 5.9-6.4 TB/s, 92-99 %
 // of the measured copy rate. What counts is how many CTAs have rows in flight while others look their page up, reduce
 // or store: 128 threads with eight rows of 16 bytes each; 256 threads with four 75 us, K and V in one CTA 95, registers
-// bounded for more CTAs (spills) 89. 64 tokens: 2.0-2.4 us as graph replays, 7 to 10 in a loop (the host). Pages of 16 tokens 96 us, 32
-// 74, 128 70; int8 74; fp32, 2 x 16383 tokens, 336 MB, 55.
+// bounded for more CTAs (spills) 89. 64 tokens: 2.0-2.4 us as graph replays, 7 to 10 in a loop (the host). Pages of 16
+// tokens 96 us, 32 74, 128 70; int8 74; fp32, 2 x 16383 tokens, 336 MB, 55.
 #include <type_traits>
 
 #include "quant.cuh"

@@ -711,7 +711,7 @@ template <typename T> int launch(const QuantArgs& a, int code, int D, unsigned g
 
 int launch_quant_tiles(const QuantArgs& a, int dtype, int code, int D, cudaStream_t stream) {
     if (a.lists != nullptr || a.status == nullptr) return LSA_ERR_ARG;  // a read's: it has neither kernel nor status here
-    if (a.streams && a.Tq * a.G <= 32) return LSA_ERR_ARG;  // its idle softmax warps would be converters that convert() has no form for
+    if (a.streams && a.Tq * a.G <= 32) return LSA_ERR_ARG;  // convert() has no form for that many idle softmax warps
     const int64_t all = (int64_t)a.B * a.Hkv * a.tiles, items = a.whole + (all - a.whole) * a.parts;
     if (items > INT32_MAX) return LSA_ERR_SIZE;
     return dtype == kBF16 ? launch<__nv_bfloat16>(a, code, D, (unsigned)items, stream)
